@@ -385,6 +385,66 @@ int mc_voting_resample(const int64_t* labels, const int64_t* map, int32_t B, int
                        int32_t IW, int32_t OH, int32_t OW, int32_t num_candidates, void* ws,
                        size_t ws_bytes, int64_t* out, void* stream);
 
+/* ---- channel mixing at every pixel -----------------------------------------------------------
+ * No counterpart in the reference, whose only way to mix channels at a pixel is a convolution with one tap.
+ * With P = B * S pixels and a row vector of channels per pixel:
+ *   pointwise   z = x W^T + b,  y = act(z) + r
+ *   gated       [g|u] = x W_in^T + b_in,  y = (act(g) * u) W_out^T + b_out + r
+ * x (B, C_in, H, W), residual r and y (B, C_out, H, W) in `layout`, S = H * W.  Parameters are contiguous, in `dtype`:
+ * w (C_out, C_in), bias (C_out); w_in (2 hidden, C_in) - gate rows first -, b_in (2 hidden), w_out (C_out, hidden),
+ * b_out (C_out).  residual and the outer biases may be NULL.  Sums are float32 (double for MC_F64); for MC_BF16 the
+ * values between two products (h, the pre-activations kept for the backward pass and the gradients behind them) are
+ * rounded to bf16, which is what the next product's operand is.  Limits: B * S < 2^31, channels <= 2^20. */
+enum {
+  MC_ACT_NONE = 0,
+  MC_ACT_RELU = 1,
+  MC_ACT_GELU = 2,      /* z * Phi(z) */
+  MC_ACT_GELU_TANH = 3, /* z / 2 * (1 + tanh(sqrt(2 / pi) (z + 0.044715 z^3))) */
+  MC_ACT_SILU = 4,      /* z / (1 + exp(-z)) */
+  MC_ACT_SIGMOID = 5
+};
+typedef struct mc_mix_desc {
+  int64_t B, S;
+  int32_t C_in, C_out;
+  int32_t hidden; /* gated block: channels between its two products; 0 for the pointwise layer */
+  int32_t act;    /* MC_ACT_* */
+  int32_t dtype, layout;
+} mc_mix_desc;
+/* saved: mc_*_saved_bytes of memory that the forward call fills for the backward call (NULL: no backward call follows);
+ * its contents are opaque.  ws: mc_*_workspace_bytes(d, backward) of scratch.  Both 256-byte aligned; sizes can be 0.
+ * In the backward calls any of the gradients may be NULL; grad_residual is grad_output itself.  Gradients of parameters
+ * are sums over all pixels in a fixed order (they repeat bit for bit), rounded once to `dtype`. */
+size_t mc_pointwise_saved_bytes(const mc_mix_desc* d);
+size_t mc_pointwise_workspace_bytes(const mc_mix_desc* d, int32_t backward);
+int mc_pointwise_fwd(const mc_mix_desc* d, const void* x, const void* w, const void* bias, const void* residual, void* y,
+                     void* saved, void* ws, size_t ws_bytes, void* stream);
+int mc_pointwise_bwd(const mc_mix_desc* d, const void* gy, const void* x, const void* w, const void* saved, void* gx,
+                     void* gw, void* gb, void* ws, size_t ws_bytes, void* stream);
+size_t mc_gated_saved_bytes(const mc_mix_desc* d);
+size_t mc_gated_workspace_bytes(const mc_mix_desc* d, int32_t backward);
+int mc_gated_fwd(const mc_mix_desc* d, const void* x, const void* w_in, const void* b_in, const void* w_out,
+                 const void* b_out, const void* residual, void* y, void* saved, void* ws, size_t ws_bytes, void* stream);
+int mc_gated_bwd(const mc_mix_desc* d, const void* gy, const void* x, const void* w_in, const void* w_out,
+                 const void* saved, void* gx, void* gw_in, void* gb_in, void* gw_out, void* gb_out, void* ws,
+                 size_t ws_bytes, void* stream);
+
+/* ---- norm of many gradients, clipping ----------------------------------------------------------
+ * No counterpart in the reference.  n tensors, given as HOST arrays: device pointers, element counts (0 allowed) and
+ * element types (MC_F32 / MC_F64 / MC_BF16, may differ).  The arrays are read before the call returns.
+ * mc_grad_norm: (sum |v|^2)^(1/2), max |v| or sum |v| over all elements of all tensors for norm_type 2, infinity or 1,
+ * written to norm (double) and, rounded, to norm32 (either may be NULL); NaN if an element is NaN.  Sums are doubles of
+ * float32 sums of eight elements; squares of float32 and bf16 elements neither overflow nor underflow.  They are added in
+ * a fixed order and repeat bit for bit.
+ * mc_grad_clip: the same, and dst[i] = src[i] * min(1, max_norm / (norm + 1e-6)); dst[i] == src[i] is allowed, any other
+ * overlap of a dst with a tensor of the call is not.  A NaN norm makes every element NaN.  The coefficient is a double,
+ * rounded to float32 for sources that are not MC_F64; products are formed in that type and rounded to dst's. */
+size_t mc_grad_workspace_bytes(int32_t n);
+int mc_grad_norm(int32_t n, const void* const* src, const int64_t* numel, const int32_t* dtype, double norm_type,
+                 double* norm, float* norm32, void* ws, size_t ws_bytes, void* stream);
+int mc_grad_clip(int32_t n, const void* const* src, const int32_t* src_dtype, void* const* dst, const int32_t* dst_dtype,
+                 const int64_t* numel, double norm_type, double max_norm, double* norm, float* norm32, void* ws,
+                 size_t ws_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

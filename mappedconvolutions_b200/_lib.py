@@ -12,12 +12,18 @@ LIB_PATH = os.path.join(_PKG, "lib", "libmc_b200.so")
 MC_F32, MC_F64, MC_BF16 = 0, 1, 2
 MC_NCHW, MC_NHWC = 0, 1
 MC_FLAG_RELU = 1
+MC_ACT_NONE, MC_ACT_RELU, MC_ACT_GELU, MC_ACT_GELU_TANH, MC_ACT_SILU, MC_ACT_SIGMOID = range(6)
 
 
 class McDesc(ctypes.Structure):
     _fields_ = [(n, ctypes.c_int32) for n in
                 ("B", "C_in", "C_out", "IH", "IW", "OH", "OW", "K", "P", "interp", "dtype", "layout",
                  "flags")]
+
+
+class McMixDesc(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int64) for n in ("B", "S")] + \
+        [(n, ctypes.c_int32) for n in ("C_in", "C_out", "hidden", "act", "dtype", "layout")]
 
 
 class McError(RuntimeError):
@@ -28,6 +34,9 @@ _lib = None
 
 _vp, _sz, _i32 = ctypes.c_void_p, ctypes.c_size_t, ctypes.c_int32
 _dp = ctypes.POINTER(McDesc)
+_mp = ctypes.POINTER(McMixDesc)
+_pp, _lp, _ip = ctypes.POINTER(_vp), ctypes.POINTER(ctypes.c_int64), ctypes.POINTER(_i32)
+_f64 = ctypes.c_double
 
 # name -> (restype, argtypes); mirrors include/mc_b200.h declaration by declaration
 SIGNATURES = {
@@ -94,6 +103,17 @@ SIGNATURES = {
     "mc_voting_resample_workspace": (_sz, [_i32, _i32, _i32, _i32, _i32]),
     "mc_voting_resample": (ctypes.c_int, [_vp, _vp, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _vp, _sz,
                                           _vp, _vp]),
+    "mc_pointwise_saved_bytes": (_sz, [_mp]),
+    "mc_pointwise_workspace_bytes": (_sz, [_mp, _i32]),
+    "mc_pointwise_fwd": (ctypes.c_int, [_mp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "mc_pointwise_bwd": (ctypes.c_int, [_mp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "mc_gated_saved_bytes": (_sz, [_mp]),
+    "mc_gated_workspace_bytes": (_sz, [_mp, _i32]),
+    "mc_gated_fwd": (ctypes.c_int, [_mp] + [_vp] * 9 + [_sz, _vp]),
+    "mc_gated_bwd": (ctypes.c_int, [_mp] + [_vp] * 11 + [_sz, _vp]),
+    "mc_grad_workspace_bytes": (_sz, [_i32]),
+    "mc_grad_norm": (ctypes.c_int, [_i32, _pp, _lp, _ip, _f64, _vp, _vp, _vp, _sz, _vp]),
+    "mc_grad_clip": (ctypes.c_int, [_i32, _pp, _ip, _pp, _ip, _lp, _f64, _f64, _vp, _vp, _vp, _sz, _vp]),
 }
 
 

@@ -880,6 +880,264 @@ Tensor voting_resample_to_map(const Tensor& input_in, const Tensor& map_in, int6
   return out;
 }
 
+// ---- channel mixing: pointwise layer, gated feed-forward block (no counterpart in the reference) ---------------
+
+void check_like(const Tensor& t, const char* name, at::IntArrayRef shape, const Tensor& x) {
+  TORCH_CHECK(t.scalar_type() == x.scalar_type(), name, " dtype ", t.scalar_type(), " does not match input dtype ",
+              x.scalar_type());
+  TORCH_CHECK(t.sizes() == shape, name, " must have shape ", shape, ", got ", t.sizes());
+}
+
+void check_param(const Tensor& t, const char* name, at::IntArrayRef shape, const Tensor& x) {
+  check_like(t, name, shape, x);
+  TORCH_CHECK(t.is_contiguous(), name, " must be contiguous");
+}
+
+void check_weight_dims(const Tensor& w, const char* name) {
+  TORCH_CHECK(w.dim() == 3 && w.size(2) == 1, name, " must be 3-D (out channels, in channels, 1)");
+}
+
+mc_mix_desc make_mix_desc(const Tensor& x, int layout, int64_t c_out, int64_t hidden, int64_t act) {
+  mc_mix_desc d{};
+  d.B = x.size(0);
+  d.S = x.size(2) * x.size(3);
+  d.C_in = (int32_t)x.size(1);
+  d.C_out = (int32_t)c_out;
+  d.hidden = (int32_t)hidden;
+  d.act = (int32_t)act;
+  const auto dt = x.scalar_type();
+  TORCH_CHECK(dt == at::kFloat || dt == at::kDouble || dt == at::kBFloat16, "unsupported dtype ", dt,
+              " (float32, float64, bfloat16)");
+  d.dtype = dt == at::kFloat ? MC_F32 : dt == at::kDouble ? MC_F64 : MC_BF16;
+  d.layout = layout;
+  return d;
+}
+
+Tensor out_layout(const OptTensor& t, int layout) { return t.has_value() ? as_layout(*t, layout) : Tensor(); }
+void* maybe(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
+
+// (output, what the backward call needs)
+std::pair<Tensor, Tensor> pointwise_forward(const Tensor& x, const Tensor& w, const Tensor& b, const OptTensor& r,
+                                            int64_t act, bool keep) {
+  const auto dev = need_cuda({&x, &w, &b, opt(r)});
+  check_weight_dims(w, "weight");
+  TORCH_CHECK(x.dim() == 4, "input must be 4-D (B, C, H, W)");
+  const int64_t c_out = w.size(0);
+  check_param(w, "weight", {c_out, x.size(1), 1}, x);
+  check_param(b, "bias", {c_out}, x);
+  const std::vector<int64_t> shape{x.size(0), c_out, x.size(2), x.size(3)};
+  if (r.has_value()) check_like(*r, "residual", shape, x);
+  const int layout = layout_of(x);
+  c10::cuda::CUDAGuard guard(dev);
+  Tensor y = empty_in(shape, x, layout);
+  const mc_mix_desc d = make_mix_desc(x, layout, c_out, 0, act);
+  if (y.numel() == 0) return {y, Tensor()};
+  const Tensor res = out_layout(r, layout);
+  Scratch saved = scratch(keep ? mc_pointwise_saved_bytes(&d) : 0, dev);
+  Scratch ws = scratch(mc_pointwise_workspace_bytes(&d, 0), dev);
+  check(mc_pointwise_fwd(&d, x.data_ptr(), w.data_ptr(), b.data_ptr(), maybe(res), y.data_ptr(), saved.p, ws.p, ws.n,
+                         cur_stream()));
+  return {y, saved.t};
+}
+
+std::vector<Tensor> pointwise_backward(const Tensor& gy_in, const OptTensor& saved, const Tensor& x, const Tensor& w,
+                                       int64_t act, bool need_input_grad, bool need_weight_grad) {
+  const auto dev = need_cuda({&gy_in, &x, &w, opt(saved)});
+  check_weight_dims(w, "weight");
+  TORCH_CHECK(x.dim() == 4, "input must be 4-D (B, C, H, W)");
+  const int64_t c_out = w.size(0);
+  check_param(w, "weight", {c_out, x.size(1), 1}, x);
+  check_like(gy_in, "grad_output", {x.size(0), c_out, x.size(2), x.size(3)}, x);
+  const int layout = layout_of(x);
+  c10::cuda::CUDAGuard guard(dev);
+  Tensor gx = need_input_grad ? empty_in(x.sizes(), x, layout) : Tensor();
+  Tensor gw, gb;
+  if (need_weight_grad) {
+    gw = x.numel() == 0 ? at::zeros(w.sizes(), w.options()) : at::empty(w.sizes(), w.options());
+    gb = x.numel() == 0 ? at::zeros({c_out}, w.options()) : at::empty({c_out}, w.options());
+  }
+  if (x.numel() == 0) return {gx, gw, gb};
+  const Tensor gy = as_layout(gy_in, layout);
+  const mc_mix_desc d = make_mix_desc(x, layout, c_out, 0, act);
+  Scratch ws = scratch(mc_pointwise_workspace_bytes(&d, 1), dev);
+  check(mc_pointwise_bwd(&d, gy.data_ptr(), x.data_ptr(), w.data_ptr(), ptr(saved), maybe(gx), maybe(gw), maybe(gb),
+                         ws.p, ws.n, cur_stream()));
+  return {gx, gw, gb};
+}
+
+std::pair<Tensor, Tensor> gated_forward(const Tensor& x, const Tensor& w_in, const Tensor& b_in, const Tensor& w_out,
+                                        const Tensor& b_out, const OptTensor& r, int64_t act, bool keep) {
+  const auto dev = need_cuda({&x, &w_in, &b_in, &w_out, &b_out, opt(r)});
+  check_weight_dims(w_in, "weight_in");
+  check_weight_dims(w_out, "weight_out");
+  TORCH_CHECK(x.dim() == 4, "input must be 4-D (B, C, H, W)");
+  const int64_t c_out = w_out.size(0), hidden = w_out.size(1);
+  check_param(w_in, "weight_in", {2 * hidden, x.size(1), 1}, x);
+  check_param(w_out, "weight_out", {c_out, hidden, 1}, x);
+  check_param(b_in, "bias_in", {2 * hidden}, x);
+  check_param(b_out, "bias_out", {c_out}, x);
+  const std::vector<int64_t> shape{x.size(0), c_out, x.size(2), x.size(3)};
+  if (r.has_value()) check_like(*r, "residual", shape, x);
+  const int layout = layout_of(x);
+  c10::cuda::CUDAGuard guard(dev);
+  Tensor y = empty_in(shape, x, layout);
+  const mc_mix_desc d = make_mix_desc(x, layout, c_out, hidden, act);
+  if (y.numel() == 0) return {y, Tensor()};
+  const Tensor res = out_layout(r, layout);
+  Scratch saved = scratch(keep ? mc_gated_saved_bytes(&d) : 0, dev);
+  Scratch ws = scratch(keep ? 0 : mc_gated_workspace_bytes(&d, 0), dev);
+  check(mc_gated_fwd(&d, x.data_ptr(), w_in.data_ptr(), b_in.data_ptr(), w_out.data_ptr(), b_out.data_ptr(), maybe(res),
+                     y.data_ptr(), saved.p, ws.p, ws.n, cur_stream()));
+  return {y, saved.t};
+}
+
+std::vector<Tensor> gated_backward(const Tensor& gy_in, const OptTensor& saved, const Tensor& x, const Tensor& w_in,
+                                   const Tensor& w_out, int64_t act, bool need_input_grad, bool need_weight_grad) {
+  const auto dev = need_cuda({&gy_in, &x, &w_in, &w_out, opt(saved)});
+  check_weight_dims(w_in, "weight_in");
+  check_weight_dims(w_out, "weight_out");
+  TORCH_CHECK(x.dim() == 4, "input must be 4-D (B, C, H, W)");
+  const int64_t c_out = w_out.size(0), hidden = w_out.size(1);
+  check_param(w_in, "weight_in", {2 * hidden, x.size(1), 1}, x);
+  check_param(w_out, "weight_out", {c_out, hidden, 1}, x);
+  check_like(gy_in, "grad_output", {x.size(0), c_out, x.size(2), x.size(3)}, x);
+  const int layout = layout_of(x);
+  c10::cuda::CUDAGuard guard(dev);
+  std::vector<Tensor> g(5);
+  if (need_input_grad) g[0] = empty_in(x.sizes(), x, layout);
+  if (need_weight_grad) {
+    const std::vector<std::vector<int64_t>> shapes{{2 * hidden, x.size(1), 1}, {2 * hidden}, {c_out, hidden, 1}, {c_out}};
+    for (int i = 0; i < 4; ++i)
+      g[i + 1] = x.numel() == 0 ? at::zeros(shapes[i], x.options()) : at::empty(shapes[i], x.options());
+  }
+  if (x.numel() == 0) return g;
+  const Tensor gy = as_layout(gy_in, layout);
+  const mc_mix_desc d = make_mix_desc(x, layout, c_out, hidden, act);
+  Scratch ws = scratch(mc_gated_workspace_bytes(&d, 1), dev);
+  check(mc_gated_bwd(&d, gy.data_ptr(), x.data_ptr(), w_in.data_ptr(), w_out.data_ptr(), ptr(saved), maybe(g[0]),
+                     maybe(g[1]), maybe(g[2]), maybe(g[3]), maybe(g[4]), ws.p, ws.n, cur_stream()));
+  return g;
+}
+
+// ---- norm of many gradients, clipping (no counterpart in the reference) -----------------------------------------
+
+int grad_dtype(const Tensor& t) {
+  const auto dt = t.scalar_type();
+  TORCH_CHECK(dt == at::kFloat || dt == at::kDouble || dt == at::kBFloat16, "unsupported dtype ", dt,
+              " (float32, float64, bfloat16)");
+  return dt == at::kFloat ? MC_F32 : dt == at::kDouble ? MC_F64 : MC_BF16;
+}
+
+c10::Device check_gradients(const std::vector<Tensor>& ts, double norm_type, c10::optional<c10::Device> dev = c10::nullopt) {
+  TORCH_CHECK(!ts.empty(), "no tensor given");
+  for (const Tensor& t : ts) {
+    need_cuda({&t});
+    if (!dev) dev = t.device();
+    TORCH_CHECK(t.device() == *dev, "all tensors must be on the same device");
+    grad_dtype(t);
+  }
+  TORCH_CHECK(norm_type == 1 || norm_type == 2 || norm_type == std::numeric_limits<double>::infinity(),
+              "norm_type must be 1, 2 or infinity");
+  return *dev;
+}
+
+struct GradLists {
+  std::vector<const void*> src;
+  std::vector<void*> dst;
+  std::vector<int64_t> numel;
+  std::vector<int32_t> src_type, dst_type;
+  void add(const Tensor& s) {
+    src.push_back(s.data_ptr());
+    numel.push_back(s.numel());
+    src_type.push_back(grad_dtype(s));
+  }
+  void add(const Tensor& s, const Tensor& d) {
+    add(s);
+    dst.push_back(d.data_ptr());
+    dst_type.push_back(grad_dtype(d));
+  }
+};
+
+// 0-dim result: float32, float64 if one of the gradients is
+struct NormOut {
+  Tensor t;
+  double* p64 = nullptr;
+  float* p32 = nullptr;
+  NormOut(const std::vector<Tensor>& ts, const c10::Device& dev) {
+    bool wide = false;
+    for (const Tensor& x : ts) wide |= x.scalar_type() == at::kDouble;
+    t = at::empty({}, at::TensorOptions().dtype(wide ? at::kDouble : at::kFloat).device(dev));
+    if (wide) p64 = t.data_ptr<double>();
+    else p32 = t.data_ptr<float>();
+  }
+};
+
+Tensor gradient_norm(const std::vector<Tensor>& tensors, double norm_type) {
+  const auto dev = check_gradients(tensors, norm_type);
+  c10::cuda::CUDAGuard guard(dev);
+  at::NoGradGuard no_grad;
+  GradLists l;
+  std::vector<Tensor> copies;
+  for (const Tensor& t : tensors) {
+    copies.push_back(t.is_non_overlapping_and_dense() ? t : t.contiguous());
+    l.add(copies.back());
+  }
+  NormOut norm(tensors, dev);
+  Scratch ws = scratch(mc_grad_workspace_bytes((int32_t)tensors.size()), dev);
+  check(mc_grad_norm((int32_t)tensors.size(), l.src.data(), l.numel.data(), l.src_type.data(), norm_type, norm.p64,
+                     norm.p32, ws.p, ws.n, cur_stream()));
+  return norm.t;
+}
+
+Tensor clip_gradients(const std::vector<Tensor>& tensors, double max_norm, double norm_type,
+                      const c10::optional<std::vector<Tensor>>& out) {
+  const auto dev = check_gradients(tensors, norm_type);
+  TORCH_CHECK(max_norm >= 0, "max_norm must not be negative");
+  const std::vector<Tensor>& outs = out.has_value() ? *out : tensors;
+  TORCH_CHECK(outs.size() == tensors.size(), "out must have as many tensors as there are gradients");
+  check_gradients(outs, norm_type, dev);
+  c10::cuda::CUDAGuard guard(dev);
+  at::NoGradGuard no_grad;
+  GradLists l;
+  std::vector<Tensor> keep;                     // copies that the kernels read
+  std::vector<std::pair<Tensor, Tensor>> back;  // results that are copied to where they belong
+  std::vector<std::tuple<uintptr_t, uintptr_t, bool>> spans;
+  for (size_t i = 0; i < tensors.size(); ++i) {
+    const Tensor &g = tensors[i], &o = outs[i];
+    TORCH_CHECK(g.sizes() == o.sizes(), "out must have the gradients' shapes");
+    Tensor s = g, d = o;
+    if (!(g.is_non_overlapping_and_dense() && o.is_non_overlapping_and_dense() &&
+          (g.strides() == o.strides() || (g.is_contiguous() && o.is_contiguous())))) {
+      for (int64_t k = 0; k < o.dim(); ++k)
+        TORCH_CHECK(o.size(k) <= 1 || o.stride(k) != 0, "a gradient to scale must not share memory with itself");
+      s = g.contiguous();
+      d = at::empty(g.sizes(), o.options());
+      keep.push_back(s);
+      back.emplace_back(o, d);
+    }
+    l.add(s, d);
+    if (d.numel() == 0) continue;
+    const auto begin = (uintptr_t)d.data_ptr(), from = (uintptr_t)s.data_ptr();
+    spans.emplace_back(begin, begin + d.numel() * d.element_size(), true);
+    if (from != begin || s.scalar_type() != d.scalar_type())
+      spans.emplace_back(from, from + s.numel() * s.element_size(), false);
+  }
+  std::sort(spans.begin(), spans.end());
+  uintptr_t end_any = 0, end_dst = 0;  // no destination may share memory with another tensor of the call
+  for (const auto& [begin, end, is_dst] : spans) {
+    TORCH_CHECK(begin >= (is_dst ? end_any : end_dst), "gradients to scale must not share memory with each other");
+    end_any = std::max(end_any, end);
+    if (is_dst) end_dst = std::max(end_dst, end);
+  }
+  NormOut norm(tensors, dev);
+  Scratch ws = scratch(mc_grad_workspace_bytes((int32_t)tensors.size()), dev);
+  check(mc_grad_clip((int32_t)tensors.size(), l.src.data(), l.src_type.data(), l.dst.data(), l.dst_type.data(),
+                     l.numel.data(), norm_type, max_norm, norm.p64, norm.p32, ws.p, ws.n, cur_stream()));
+  for (auto& b : back) b.first.copy_(b.second);
+  for (const Tensor& o : outs) o.unsafeGetTensorImpl()->bump_version();
+  return norm.t;
+}
+
 // ---- differentiable layer calls --------------------------------------------------------------------------
 // The pairing of forward and backward ops is the reference's (package/layers/nn/*.py): convolution <-> (input,
 // weight, bias gradient); max pool <-> max unpool through the stored tap offsets; average pool <-> average
@@ -1016,6 +1274,52 @@ OptTensor linear_layer(int64_t op, const Tensor& x, const Tensor& map, const Opt
   if (!records({&x, &map, opt(iw)})) return run_linear(op, x, map, iw, oh, ow, K, interp);
   return LinearFn::apply(x, map, iw, op, oh, ow, K, interp);
 }
+
+struct PointwiseFn : torch::autograd::Function<PointwiseFn> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const Tensor& b, const OptTensor& r,
+                        int64_t act) {
+    auto f = pointwise_forward(x, w, b, r, act, true);
+    ctx->save_for_backward({x, w, f.second});
+    ctx->saved_data["a"] = act;
+    ctx->saved_data["r"] = r.has_value();  // (needs_input_grad counts the tensors that were given)
+    return f.first;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    const auto s = ctx->get_saved_variables();
+    const bool need_x = ctx->needs_input_grad(0), need_p = ctx->needs_input_grad(1) || ctx->needs_input_grad(2);
+    variable_list out(5);
+    if (need_x || need_p) {
+      auto r = pointwise_backward(g[0], as_opt(s[2]), s[0], s[1], ctx->saved_data["a"].toInt(), need_x, need_p);
+      for (int i = 0; i < 3; ++i) out[i] = r[i];
+    }
+    if (ctx->saved_data["r"].toBool() && ctx->needs_input_grad(3)) out[3] = g[0];
+    return out;
+  }
+};
+
+struct GatedFn : torch::autograd::Function<GatedFn> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& wi, const Tensor& bi, const Tensor& wo,
+                        const Tensor& bo, const OptTensor& r, int64_t act) {
+    auto f = gated_forward(x, wi, bi, wo, bo, r, act, true);
+    ctx->save_for_backward({x, wi, wo, f.second});
+    ctx->saved_data["a"] = act;
+    ctx->saved_data["r"] = r.has_value();  // (needs_input_grad counts the tensors that were given)
+    return f.first;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    const auto s = ctx->get_saved_variables();
+    bool need_p = false;
+    for (int i = 1; i < 5; ++i) need_p |= ctx->needs_input_grad(i);
+    const bool need_x = ctx->needs_input_grad(0);
+    variable_list out(7);
+    if (need_x || need_p) {
+      auto r = gated_backward(g[0], as_opt(s[3]), s[0], s[1], s[2], ctx->saved_data["a"].toInt(), need_x, need_p);
+      for (int i = 0; i < 5; ++i) out[i] = r[i];
+    }
+    if (ctx->saved_data["r"].toBool() && ctx->needs_input_grad(5)) out[5] = g[0];
+    return out;
+  }
+};
 
 }  // namespace
 
@@ -1156,6 +1460,55 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   def("unresample_layer", [](const Tensor& x, const Tensor& map, int64_t i, const OptTensor& iw) {
     return linear_layer(3, x, map, iw, 0, 0, 1, i);
   });
+  // channel mixing: [output, saved] and the gradients, as in ops.py; the differentiable calls of the layers
+  def("pointwise_forward",
+        [](const Tensor& x, const Tensor& w, const Tensor& b, const OptTensor& r, int64_t act,
+           bool keep) -> std::vector<OptTensor> {
+          auto f = pointwise_forward(x, w, b, r, act, keep);
+          return {f.first, as_opt(f.second)};
+        },
+        py::arg("input"), py::arg("weight"), py::arg("bias"), py::arg("residual") = py::none(), py::arg("activation") = 0,
+        py::arg("keep") = false);
+  def("pointwise_backward",
+        [](const Tensor& gy, const OptTensor& saved, const Tensor& x, const Tensor& w, int64_t act, bool nx, bool np) {
+          std::vector<OptTensor> r;
+          for (const Tensor& t : pointwise_backward(gy, saved, x, w, act, nx, np)) r.push_back(as_opt(t));
+          return r;
+        },
+        py::arg("grad_output"), py::arg("saved"), py::arg("input"), py::arg("weight"), py::arg("activation") = 0,
+        py::arg("need_input_grad") = true, py::arg("need_weight_grad") = true);
+  def("gated_forward",
+        [](const Tensor& x, const Tensor& wi, const Tensor& bi, const Tensor& wo, const Tensor& bo, const OptTensor& r,
+           int64_t act, bool keep) -> std::vector<OptTensor> {
+          auto f = gated_forward(x, wi, bi, wo, bo, r, act, keep);
+          return {f.first, as_opt(f.second)};
+        },
+        py::arg("input"), py::arg("weight_in"), py::arg("bias_in"), py::arg("weight_out"), py::arg("bias_out"),
+        py::arg("residual") = py::none(), py::arg("activation") = 4, py::arg("keep") = false);
+  def("gated_backward",
+        [](const Tensor& gy, const OptTensor& saved, const Tensor& x, const Tensor& wi, const Tensor& wo, int64_t act, bool nx,
+           bool np) {
+          std::vector<OptTensor> r;
+          for (const Tensor& t : gated_backward(gy, saved, x, wi, wo, act, nx, np)) r.push_back(as_opt(t));
+          return r;
+        },
+        py::arg("grad_output"), py::arg("saved"), py::arg("input"), py::arg("weight_in"), py::arg("weight_out"),
+        py::arg("activation") = 4, py::arg("need_input_grad") = true, py::arg("need_weight_grad") = true);
+  def("pointwise_layer", [](const Tensor& x, const Tensor& w, const Tensor& b, const OptTensor& r, int64_t act) -> OptTensor {
+    if (seen_by_torch({&x, &w, &b, opt(r)})) return c10::nullopt;
+    if (!records({&x, &w, &b, opt(r)})) return pointwise_forward(x, w, b, r, act, false).first;
+    return PointwiseFn::apply(x, w, b, r, act);
+  });
+  def("gated_layer", [](const Tensor& x, const Tensor& wi, const Tensor& bi, const Tensor& wo, const Tensor& bo,
+                          const OptTensor& r, int64_t act) -> OptTensor {
+    if (seen_by_torch({&x, &wi, &bi, &wo, &bo, opt(r)})) return c10::nullopt;
+    if (!records({&x, &wi, &bi, &wo, &bo, opt(r)})) return gated_forward(x, wi, bi, wo, bo, r, act, false).first;
+    return GatedFn::apply(x, wi, bi, wo, bo, r, act);
+  });
+  // norm of many gradients, clipping
+  def("gradient_norm", &gradient_norm, py::arg("tensors"), py::arg("norm_type") = 2.0);
+  def("clip_gradients", &clip_gradients, py::arg("tensors"), py::arg("max_norm"), py::arg("norm_type") = 2.0,
+        py::arg("out") = py::none());
   def("clear_plan_cache", &clear_plan_cache);
   def("plan_cache_kinds", &plan_cache_kinds);
   // Row plans (the fast path for maps that are translation invariant along image rows) on / off;

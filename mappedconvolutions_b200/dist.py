@@ -29,3 +29,30 @@ def allreduce_gradients(tensors, group=None):
         t.detach().copy_(bucket[off:off + n].view_as(t))
         off += n
     return bucket
+
+
+def gradient_norm(tensors, norm_type=2.0):
+    """Norm of all elements of the given gradient tensors together (None entries are left out): 2, 1 or infinity.
+    CUDA tensors of one device, float32 / float64 / bfloat16 in any mixture.  Returns a 0-dim float32 tensor (float64 if
+    one of the gradients is) without waiting for the device, or None if there is no gradient."""
+    from .host import impl
+    tensors = [t for t in tensors if t is not None]
+    return impl.gradient_norm(tensors, float(norm_type)) if tensors else None
+
+
+def clip_gradients(tensors, max_norm, norm_type=2.0, out=None):
+    """Scale the gradients by min(1, max_norm / (norm + 1e-6)), with the norm over all of them together, as
+    torch.nn.utils.clip_grad_norm_ does; behind allreduce_gradients every rank finds the same norm.
+
+    In place, or into `out`: tensors of the same shapes (entries of None gradients are ignored), whose type may differ -
+    float32 from bfloat16 gradients, say, rounded once.  Returns the norm before scaling, as gradient_norm does.  A NaN
+    norm makes every element NaN; an infinite one makes finite elements zero.  Tensors that share memory are refused."""
+    from .host import impl
+    tensors = list(tensors)
+    if out is not None:
+        out = list(out)
+        if len(out) != len(tensors):
+            raise RuntimeError("out must have as many tensors as there are gradients")
+        out = [o for o, t in zip(out, tensors) if t is not None]
+    tensors = [t for t in tensors if t is not None]
+    return impl.clip_gradients(tensors, float(max_norm), float(norm_type), out) if tensors else None

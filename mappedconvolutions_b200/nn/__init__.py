@@ -1,5 +1,6 @@
-from .layers import (Convolution, MappedAvgPool, MappedAvgUnpool, MappedConvolution, MappedMaxPool,
-                     MappedTransposedConvolution, Resample, TransposedConvolution, Unresample)
+from .layers import (Convolution, GatedFeedForward, MappedAvgPool, MappedAvgUnpool, MappedConvolution, MappedMaxPool,
+                     MappedTransposedConvolution, PointwiseConvolution, Resample, TransposedConvolution, Unresample)
 
 __all__ = ["Convolution", "TransposedConvolution", "MappedConvolution", "MappedTransposedConvolution",
-           "MappedMaxPool", "MappedAvgPool", "MappedAvgUnpool", "Resample", "Unresample"]
+           "MappedMaxPool", "MappedAvgPool", "MappedAvgUnpool", "Resample", "Unresample", "PointwiseConvolution",
+           "GatedFeedForward"]

@@ -67,3 +67,24 @@ def check_input_map_shape(x, sample_map):
         'Input dimensions 2 and 3 must match sample map dimensions 0 and 1 ' \
         '(({},{}) != ({},{}))'.format(x.shape[2], x.shape[3], sample_map.shape[0],
                                       sample_map.shape[1])
+
+
+ACTIVATIONS = {None: 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4, "sigmoid": 5}
+
+
+def activation_code(name):
+    assert name in ACTIVATIONS, 'Unsupported activation ({} is none of {})'.format(name, list(ACTIVATIONS))
+    return ACTIVATIONS[name]
+
+
+def check_mix_args(x, in_channels, out_channels, residual):
+    """Arguments of the channel-mixing layers."""
+    assert x.dim() == 4, 'Input must have 4 dimensions ({} != 4)'.format(x.dim())
+    assert x.shape[1] == in_channels, \
+        'Number of input channels must match weight parameter ({} != {})'.format(x.shape[1], in_channels)
+    if residual is not None:
+        want = (x.shape[0], out_channels, x.shape[2], x.shape[3])
+        assert tuple(residual.shape) == want, \
+            'Residual must have the shape of the output ({} != {})'.format(tuple(residual.shape), want)
+        assert residual.dtype == x.dtype, \
+            'Input and residual must be the same dtype ({} != {})'.format(x.dtype, residual.dtype)

@@ -193,6 +193,46 @@ class UnresampleFn(Function):
         return gx, None, None, None
 
 
+class PointwiseFn(Function):
+    """act(W x + bias) + residual at every pixel (no counterpart in the reference)"""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, residual, activation):
+        ctx.activation = int(activation)
+        y, saved = ops.pointwise_forward(x, weight, bias, residual, ctx.activation, True)
+        ctx.save_for_backward(x, weight, saved)
+        return y
+
+    @staticmethod
+    def backward(ctx, gy):
+        x, weight, saved = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        g = [None] * 3
+        if any(need[:3]):
+            g = ops.pointwise_backward(gy, saved, x, weight, ctx.activation, need[0], need[1] or need[2])
+        return (*g, gy if need[3] else None, None)
+
+
+class GatedFn(Function):
+    """W_out (act(g) * u) + bias_out + residual with [g; u] = W_in x + bias_in (no counterpart in the reference)"""
+
+    @staticmethod
+    def forward(ctx, x, weight_in, bias_in, weight_out, bias_out, residual, activation):
+        ctx.activation = int(activation)
+        y, saved = ops.gated_forward(x, weight_in, bias_in, weight_out, bias_out, residual, ctx.activation, True)
+        ctx.save_for_backward(x, weight_in, weight_out, saved)
+        return y
+
+    @staticmethod
+    def backward(ctx, gy):
+        x, weight_in, weight_out, saved = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        g = [None] * 5
+        if any(need[:5]):
+            g = ops.gated_backward(gy, saved, x, weight_in, weight_out, ctx.activation, need[0], any(need[1:5]))
+        return (*g, gy if need[5] else None, None)
+
+
 def _layer_call(function, node_name):
     """The extension's node of that name, which returns None where torch has to see the Function (see above)."""
     node = getattr(ops, node_name, None)  # (the ctypes twin has no nodes)
@@ -212,3 +252,5 @@ avg_pool = _layer_call(MappedAvgPoolFn, "avg_pool_layer")
 avg_unpool = _layer_call(MappedAvgUnpoolFn, "avg_unpool_layer")
 resample = _layer_call(ResampleFn, "resample_layer")
 unresample = _layer_call(UnresampleFn, "unresample_layer")
+pointwise = _layer_call(PointwiseFn, "pointwise_layer")
+gated = _layer_call(GatedFn, "gated_layer")

@@ -6,7 +6,7 @@ import torch
 import torch.nn as nn
 
 from . import functions as F
-from .checks import check_args, check_input_map_shape, interp_code
+from .checks import activation_code, check_args, check_input_map_shape, check_mix_args, interp_code
 
 
 class _ConvBase(nn.Module):
@@ -208,3 +208,60 @@ class TransposedConvolution(_GridConvBase):
     def forward(self, x):
         return torch.nn.functional.conv_transpose2d(x, self.weight, self.bias, self.stride, self.padding, 0, 1,
                                                     self.dilation)
+
+
+class PointwiseConvolution(_ConvBase):
+    """act(W x + bias) + residual at every pixel or mesh vertex, in one kernel: a convolution with one tap and no sample
+    map.  Parameters and their initialisation are those of MappedConvolution with kernel_size=1.  Not in the reference.
+
+    forward(x (B,C_in,H,W), residual=None | (B,C_out,H,W)) -> (B,C_out,H,W) in x's layout
+    activation: None, 'relu', 'gelu', 'gelu_tanh', 'silu' or 'sigmoid'; the residual is added behind it.
+    """
+
+    def __init__(self, in_channels, out_channels, bias=True, *, activation=None):
+        super().__init__(in_channels, out_channels, 1, 'nearest', bias, False)
+        self.activation = activation
+        self._act = activation_code(activation)
+
+    def forward(self, x, residual=None):
+        check_mix_args(x, self.in_channels, self.out_channels, residual)
+        return F.pointwise(x, self.weight, self.bias, residual, self._act)
+
+
+class GatedFeedForward(nn.Module):
+    """W_out (act(W_g x + b_g) * (W_u x + b_u)) + bias_out + residual at every pixel or mesh vertex: both inner
+    projections, the activation and the product are one kernel, the outer projection with bias and residual a second.
+    weight_in (2 * hidden, in, 1) and bias_in hold the gate's rows first, then the factor's.  Not in the reference.
+
+    forward(x (B,C_in,H,W), residual=None | (B,C_out,H,W)) -> (B,C_out,H,W) in x's layout; out_channels defaults to
+    in_channels.  Initialisation: U(-s, s) with s = 1/sqrt(number of inputs) for each projection; bias=False keeps zero,
+    still trainable, biases.
+    """
+
+    def __init__(self, in_channels, hidden_channels, out_channels=None, bias=True, *, activation='silu'):
+        super().__init__()
+        self.in_channels = in_channels
+        self.hidden_channels = hidden_channels
+        self.out_channels = in_channels if out_channels is None else out_channels
+        self.activation = activation
+        self._act = activation_code(activation)
+        self.weight_in = nn.Parameter(torch.empty(2 * hidden_channels, in_channels, 1))
+        self.bias_in = nn.Parameter(torch.empty(2 * hidden_channels))
+        self.weight_out = nn.Parameter(torch.empty(self.out_channels, hidden_channels, 1))
+        self.bias_out = nn.Parameter(torch.empty(self.out_channels))
+        self.reset_parameters()
+        if not bias:
+            self.bias_in = nn.Parameter(torch.zeros(2 * hidden_channels))
+            self.bias_out = nn.Parameter(torch.zeros(self.out_channels))
+
+    def reset_parameters(self):
+        with torch.no_grad():
+            for n, params in ((self.in_channels, (self.weight_in, self.bias_in)),
+                              (self.hidden_channels, (self.weight_out, self.bias_out))):
+                s = 1.0 / math.sqrt(n)
+                for p in params:
+                    p.uniform_(-s, s)
+
+    def forward(self, x, residual=None):
+        check_mix_args(x, self.in_channels, self.out_channels, residual)
+        return F.gated(x, self.weight_in, self.bias_in, self.weight_out, self.bias_out, residual, self._act)

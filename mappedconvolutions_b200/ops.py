@@ -766,3 +766,253 @@ def voting_resample_to_map(input, sample_map, output_height, output_width, num_c
             check(lib().mc_voting_resample(input[b0:].data_ptr(), sample_map.data_ptr(), nb, C, IH, IW, OH, OW, NC,
                                            ws.data_ptr(), per_image * nb, out[b0:].data_ptr(), _stream()))
     return out
+
+
+# ------------------------------------------------------------------------------------------
+# channel mixing: pointwise layer, gated feed-forward block (no counterpart in the reference)
+# ------------------------------------------------------------------------------------------
+
+def _check_like(t, name, shape, x):
+    if t.dtype != x.dtype:
+        raise RuntimeError("%s dtype %s does not match input dtype %s" % (name, t.dtype, x.dtype))
+    if tuple(t.shape) != tuple(shape):
+        raise RuntimeError("%s must have shape %s, got %s" % (name, tuple(shape), tuple(t.shape)))
+
+
+def _check_mix(x, params, residual, c_out, grad_output=None):
+    """params: (name, tensor, shape).  Same checks and messages as the compiled binding."""
+    if x.dim() != 4:
+        raise RuntimeError("input must be 4-D (B, C, H, W)")
+    for name, t, shape in params:
+        _check_like(t, name, shape, x)
+        if not t.is_contiguous():
+            raise RuntimeError("%s must be contiguous" % name)
+    out = (x.shape[0], c_out, x.shape[2], x.shape[3])
+    if residual is not None:
+        _check_like(residual, "residual", out, x)
+    if grad_output is not None:
+        _check_like(grad_output, "grad_output", out, x)
+    return out
+
+
+def _mix_desc(x, layout, c_out, hidden, activation):
+    if x.dtype not in _DT:
+        raise RuntimeError("unsupported dtype %s (float32, float64, bfloat16)" % x.dtype)
+    return _lib.McMixDesc(x.shape[0], x.shape[2] * x.shape[3], x.shape[1], c_out, hidden, int(activation),
+                          _DT[x.dtype], layout)
+
+
+def _bytes(n, dev):
+    return torch.empty(int(n), dtype=torch.uint8, device=dev) if n else None
+
+
+def _weight_dims(weight, name):
+    if weight.dim() != 3 or weight.shape[2] != 1:
+        raise RuntimeError("%s must be 3-D (out channels, in channels, 1)" % name)
+    return weight.shape[0], weight.shape[1]
+
+
+def pointwise_forward(input, weight, bias, residual=None, activation=0, keep=False):
+    """act(W x + bias) + residual at every pixel -> [output, what pointwise_backward needs (keep) or None]"""
+    dev = _need_cuda(input, weight, bias, residual)
+    c_out, _ = _weight_dims(weight, "weight")
+    shape = _check_mix(input, [("weight", weight, (c_out, input.shape[1] if input.dim() > 1 else 0, 1)), ("bias", bias, (c_out,))],
+                       residual, c_out)
+    layout = _layout(input)
+    y = _empty(shape, input, layout)
+    d = _mix_desc(input, layout, c_out, 0, activation)
+    if y.numel() == 0:
+        return [y, None]
+    if residual is not None:
+        residual = _as_layout(residual, layout)
+    with torch.cuda.device(dev):
+        L = lib()
+        saved = _bytes(L.mc_pointwise_saved_bytes(d), dev) if keep else None
+        wst, wsn, wsp = _ws(L.mc_pointwise_workspace_bytes(d, 0), dev)
+        check(L.mc_pointwise_fwd(d, input.data_ptr(), weight.data_ptr(), bias.data_ptr(), _ptr(residual), y.data_ptr(),
+                                 _ptr(saved), wsp, wsn, _stream()))
+    return [y, saved]
+
+
+def pointwise_backward(grad_output, saved, input, weight, activation=0, need_input_grad=True, need_weight_grad=True):
+    """-> [grad_input, grad_weight, grad_bias]; the residual's gradient is grad_output"""
+    dev = _need_cuda(grad_output, input, weight, saved)
+    c_out, c_in = _weight_dims(weight, "weight")
+    _check_mix(input, [("weight", weight, (c_out, input.shape[1] if input.dim() > 1 else 0, 1))], None, c_out, grad_output)
+    layout = _layout(input)
+    gx = _empty(input.shape, input, layout) if need_input_grad else None
+    make = torch.zeros if input.numel() == 0 else torch.empty
+    gw = make(weight.shape, dtype=weight.dtype, device=dev) if need_weight_grad else None
+    gb = make((c_out,), dtype=weight.dtype, device=dev) if need_weight_grad else None
+    if input.numel() == 0:
+        return [gx, gw, gb]
+    grad_output = _as_layout(grad_output, layout)
+    d = _mix_desc(input, layout, c_out, 0, activation)
+    with torch.cuda.device(dev):
+        L = lib()
+        wst, wsn, wsp = _ws(L.mc_pointwise_workspace_bytes(d, 1), dev)
+        check(L.mc_pointwise_bwd(d, grad_output.data_ptr(), input.data_ptr(), weight.data_ptr(), _ptr(saved), _ptr(gx),
+                                 _ptr(gw), _ptr(gb), wsp, wsn, _stream()))
+    return [gx, gw, gb]
+
+
+def _gated_dims(x, weight_in, weight_out):
+    c_out, hidden = _weight_dims(weight_out, "weight_out")
+    _weight_dims(weight_in, "weight_in")
+    return c_out, hidden, [("weight_in", weight_in, (2 * hidden, x.shape[1] if x.dim() > 1 else 0, 1)),
+                           ("weight_out", weight_out, (c_out, hidden, 1))]
+
+
+def gated_forward(input, weight_in, bias_in, weight_out, bias_out, residual=None, activation=4, keep=False):
+    """W_out (act(g) * u) + bias_out + residual with [g; u] = W_in x + bias_in at every pixel
+    -> [output, what gated_backward needs (keep) or None]"""
+    dev = _need_cuda(input, weight_in, bias_in, weight_out, bias_out, residual)
+    c_out, hidden, params = _gated_dims(input, weight_in, weight_out)
+    shape = _check_mix(input, params + [("bias_in", bias_in, (2 * hidden,)), ("bias_out", bias_out, (c_out,))], residual, c_out)
+    layout = _layout(input)
+    y = _empty(shape, input, layout)
+    d = _mix_desc(input, layout, c_out, hidden, activation)
+    if y.numel() == 0:
+        return [y, None]
+    if residual is not None:
+        residual = _as_layout(residual, layout)
+    with torch.cuda.device(dev):
+        L = lib()
+        saved = _bytes(L.mc_gated_saved_bytes(d), dev) if keep else None
+        wst, wsn, wsp = _ws(0 if keep else L.mc_gated_workspace_bytes(d, 0), dev)
+        check(L.mc_gated_fwd(d, input.data_ptr(), weight_in.data_ptr(), bias_in.data_ptr(), weight_out.data_ptr(),
+                             bias_out.data_ptr(), _ptr(residual), y.data_ptr(), _ptr(saved), wsp, wsn, _stream()))
+    return [y, saved]
+
+
+def gated_backward(grad_output, saved, input, weight_in, weight_out, activation=4, need_input_grad=True,
+                   need_weight_grad=True):
+    """-> [grad_input, grad_weight_in, grad_bias_in, grad_weight_out, grad_bias_out]"""
+    dev = _need_cuda(grad_output, input, weight_in, weight_out, saved)
+    c_out, hidden, params = _gated_dims(input, weight_in, weight_out)
+    _check_mix(input, params, None, c_out, grad_output)
+    layout = _layout(input)
+    gx = _empty(input.shape, input, layout) if need_input_grad else None
+    make = torch.zeros if input.numel() == 0 else torch.empty
+    grads = [make(s, dtype=input.dtype, device=dev) if need_weight_grad else None
+             for s in (weight_in.shape, (2 * hidden,), weight_out.shape, (c_out,))]
+    if input.numel() == 0:
+        return [gx] + grads
+    grad_output = _as_layout(grad_output, layout)
+    d = _mix_desc(input, layout, c_out, hidden, activation)
+    with torch.cuda.device(dev):
+        L = lib()
+        wst, wsn, wsp = _ws(L.mc_gated_workspace_bytes(d, 1), dev)
+        check(L.mc_gated_bwd(d, grad_output.data_ptr(), input.data_ptr(), weight_in.data_ptr(), weight_out.data_ptr(),
+                             _ptr(saved), _ptr(gx), *[_ptr(g) for g in grads], wsp, wsn, _stream()))
+    return [gx] + grads
+
+
+# ------------------------------------------------------------------------------------------
+# gradient norm and clipping (no counterpart in the reference)
+# ------------------------------------------------------------------------------------------
+
+def _dense(t):
+    """Every element of one block of memory exactly once, in any order of the dimensions."""
+    n = 1
+    for size, stride in sorted(((s, st) for s, st in zip(t.shape, t.stride()) if s != 1), key=lambda p: p[1]):
+        if stride != n:
+            return False
+        n *= size
+    return True
+
+
+def _array(ctype, values):
+    return (ctype * max(1, len(values)))(*values)
+
+
+def _check_gradients(tensors, norm_type):
+    if not tensors:
+        raise RuntimeError("no tensor given")
+    _need_cuda(*tensors)
+    for t in tensors:
+        if t.dtype not in _DT:
+            raise RuntimeError("unsupported dtype %s (float32, float64, bfloat16)" % t.dtype)
+    if norm_type not in (1, 2, float("inf")):
+        raise RuntimeError("norm_type must be 1, 2 or infinity")
+
+
+def _check_apart(pairs):
+    """No destination may share memory with another tensor of the call."""
+    spans = []
+    for src, dst in pairs:
+        if dst.numel():
+            spans.append((dst.data_ptr(), dst.data_ptr() + dst.numel() * dst.element_size(), True))
+            if src.data_ptr() != dst.data_ptr() or src.dtype != dst.dtype:
+                spans.append((src.data_ptr(), src.data_ptr() + src.numel() * src.element_size(), False))
+    end_any = end_dst = 0
+    for begin, end, is_dst in sorted(spans):
+        if begin < (end_any if is_dst else end_dst):
+            raise RuntimeError("gradients to scale must not share memory with each other")
+        end_any = max(end_any, end)
+        if is_dst:
+            end_dst = max(end_dst, end)
+
+
+def _norm_out(tensors, dev):
+    wide = any(t.dtype == torch.float64 for t in tensors)
+    norm = torch.empty((), dtype=torch.float64 if wide else torch.float32, device=dev)
+    return norm, (norm.data_ptr() if wide else None), (None if wide else norm.data_ptr())
+
+
+def gradient_norm(tensors, norm_type=2.0):
+    """Norm of all elements of all tensors, a 0-dim float32 tensor (float64 if one of them is)."""
+    tensors = [t.detach() for t in tensors]
+    _check_gradients(tensors, norm_type)
+    dev = tensors[0].device
+    norm, p64, p32 = _norm_out(tensors, dev)
+    src = [t if _dense(t) else t.contiguous() for t in tensors]
+    ct, n = _lib.ctypes, len(src)
+    with torch.cuda.device(dev):
+        wst, wsn, wsp = _ws(lib().mc_grad_workspace_bytes(n), dev)
+        check(lib().mc_grad_norm(n, _array(ct.c_void_p, [t.data_ptr() for t in src]),
+                                 _array(ct.c_int64, [t.numel() for t in src]), _array(ct.c_int32, [_DT[t.dtype] for t in src]),
+                                 float(norm_type), p64, p32, wsp, wsn, _stream()))
+    return norm
+
+
+def clip_gradients(tensors, max_norm, norm_type=2.0, out=None):
+    """out[i] = tensors[i] * min(1, max_norm / (norm + 1e-6)), in place without out -> the norm before scaling"""
+    grads = [t.detach() for t in tensors]
+    _check_gradients(grads, norm_type)
+    if not max_norm >= 0:
+        raise RuntimeError("max_norm must not be negative")
+    outs = grads if out is None else [t.detach() for t in out]
+    if len(outs) != len(grads):
+        raise RuntimeError("out must have as many tensors as there are gradients")
+    _check_gradients(outs, norm_type)
+    dev = _need_cuda(*grads, *outs)
+    src, dst, back = [], [], []
+    for g, o in zip(grads, outs):
+        if g.shape != o.shape:
+            raise RuntimeError("out must have the gradients' shapes")
+        if _dense(g) and _dense(o) and (g.stride() == o.stride() or (g.is_contiguous() and o.is_contiguous())):
+            src.append(g)
+            dst.append(o)
+            continue
+        if any(s > 1 and st == 0 for s, st in zip(o.shape, o.stride())):
+            raise RuntimeError("a gradient to scale must not share memory with itself")
+        src.append(g.contiguous())
+        dst.append(torch.empty(g.shape, dtype=o.dtype, device=dev))
+        back.append((o, dst[-1]))
+    _check_apart(list(zip(src, dst)))
+    norm, p64, p32 = _norm_out(grads, dev)
+    ct, n = _lib.ctypes, len(src)
+    with torch.cuda.device(dev):
+        wst, wsn, wsp = _ws(lib().mc_grad_workspace_bytes(n), dev)
+        check(lib().mc_grad_clip(n, _array(ct.c_void_p, [t.data_ptr() for t in src]),
+                                 _array(ct.c_int32, [_DT[t.dtype] for t in src]),
+                                 _array(ct.c_void_p, [t.data_ptr() for t in dst]),
+                                 _array(ct.c_int32, [_DT[t.dtype] for t in dst]),
+                                 _array(ct.c_int64, [t.numel() for t in src]), float(norm_type), float(max_norm), p64, p32,
+                                 wsp, wsn, _stream()))
+        for o, t in back:
+            o.copy_(t)
+    for t in (tensors if out is None else out):
+        torch.autograd.graph.increment_version(t)
+    return norm
