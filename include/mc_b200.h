@@ -392,9 +392,10 @@ int mc_voting_resample(const int64_t* labels, const int64_t* map, int32_t B, int
  *   gated       [g|u] = x W_in^T + b_in,  y = (act(g) * u) W_out^T + b_out + r
  * x (B, C_in, H, W), residual r and y (B, C_out, H, W) in `layout`, S = H * W.  Parameters are contiguous, in `dtype`:
  * w (C_out, C_in), bias (C_out); w_in (2 hidden, C_in) - gate rows first -, b_in (2 hidden), w_out (C_out, hidden),
- * b_out (C_out).  residual and the outer biases may be NULL.  Sums are float32 (double for MC_F64); for MC_BF16 the
- * values between two products (h, the pre-activations kept for the backward pass and the gradients behind them) are
- * rounded to bf16, which is what the next product's operand is.  Limits: B * S < 2^31, channels <= 2^20. */
+ * b_out (C_out).  residual and biases may be NULL.  Sums are float32 (double for MC_F64); for MC_BF16 what stands
+ * between two products (h, and the gradients of the pre-activations) is rounded to bf16, which the next product's
+ * operand is, and the pre-activations themselves are float32: the backward calls compute them again.  MC_BF16 tensors
+ * must be 16-byte aligned (biases need not be).  Limits: B * S < 2^31, channels <= 2^20. */
 enum {
   MC_ACT_NONE = 0,
   MC_ACT_RELU = 1,
@@ -410,22 +411,26 @@ typedef struct mc_mix_desc {
   int32_t act;    /* MC_ACT_* */
   int32_t dtype, layout;
 } mc_mix_desc;
+/* Workspace of a forward call that no backward call follows (saved == NULL), of a backward call, and of a forward call
+ * that fills saved. */
+enum { MC_PHASE_FORWARD = 0, MC_PHASE_BACKWARD = 1, MC_PHASE_KEEP = 2 };
 /* saved: mc_*_saved_bytes of memory that the forward call fills for the backward call (NULL: no backward call follows);
- * its contents are opaque.  ws: mc_*_workspace_bytes(d, backward) of scratch.  Both 256-byte aligned; sizes can be 0.
+ * its contents are opaque.  ws: mc_*_workspace_bytes(d, phase) of scratch.  Both 256-byte aligned; sizes can be 0
+ * (and then the pointers NULL).
  * In the backward calls any of the gradients may be NULL; grad_residual is grad_output itself.  Gradients of parameters
  * are sums over all pixels in a fixed order (they repeat bit for bit), rounded once to `dtype`. */
 size_t mc_pointwise_saved_bytes(const mc_mix_desc* d);
-size_t mc_pointwise_workspace_bytes(const mc_mix_desc* d, int32_t backward);
+size_t mc_pointwise_workspace_bytes(const mc_mix_desc* d, int32_t phase);
 int mc_pointwise_fwd(const mc_mix_desc* d, const void* x, const void* w, const void* bias, const void* residual, void* y,
                      void* saved, void* ws, size_t ws_bytes, void* stream);
-int mc_pointwise_bwd(const mc_mix_desc* d, const void* gy, const void* x, const void* w, const void* saved, void* gx,
-                     void* gw, void* gb, void* ws, size_t ws_bytes, void* stream);
+int mc_pointwise_bwd(const mc_mix_desc* d, const void* gy, const void* x, const void* w, const void* bias,
+                     const void* saved, void* gx, void* gw, void* gb, void* ws, size_t ws_bytes, void* stream);
 size_t mc_gated_saved_bytes(const mc_mix_desc* d);
-size_t mc_gated_workspace_bytes(const mc_mix_desc* d, int32_t backward);
+size_t mc_gated_workspace_bytes(const mc_mix_desc* d, int32_t phase);
 int mc_gated_fwd(const mc_mix_desc* d, const void* x, const void* w_in, const void* b_in, const void* w_out,
                  const void* b_out, const void* residual, void* y, void* saved, void* ws, size_t ws_bytes, void* stream);
-int mc_gated_bwd(const mc_mix_desc* d, const void* gy, const void* x, const void* w_in, const void* w_out,
-                 const void* saved, void* gx, void* gw_in, void* gb_in, void* gw_out, void* gb_out, void* ws,
+int mc_gated_bwd(const mc_mix_desc* d, const void* gy, const void* x, const void* w_in, const void* b_in,
+                 const void* w_out, const void* saved, void* gx, void* gw_in, void* gb_in, void* gw_out, void* gb_out, void* ws,
                  size_t ws_bytes, void* stream);
 
 /* ---- norm of many gradients, clipping ----------------------------------------------------------

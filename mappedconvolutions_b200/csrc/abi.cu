@@ -20,6 +20,9 @@ size_t conv_tc_fwd_ws(const mc_desc*);
 int conv_tc_fwd_launch(const mc_desc*, const void*, const void*, const void*, const void*, void*,
                        void*, size_t, cudaStream_t);
 int device_status_read(cudaStream_t, int);
+namespace mix {
+int tc_status_read(int);
+}
 bool conv_tc_dgrad_supported(const mc_desc*);
 size_t conv_tc_dgrad_ws(const mc_desc*);
 int conv_tc_dgrad_launch(const mc_desc*, const void*, const void*, const void*, const void*, void*,
@@ -84,7 +87,8 @@ const char* mc_strerror(int code) {
 // ---- conv ----------------------------------------------------------------------------------
 
 int mc_device_status(void* stream, int reset) {
-  return device_status_read((cudaStream_t)stream, reset);
+  const int conv = device_status_read((cudaStream_t)stream, reset), mixing = mix::tc_status_read(reset);
+  return conv ? conv : mixing;
 }
 
 // Layers with padded output channels ask for a workspace and for aligned tensors only to be faster: without

@@ -41,18 +41,20 @@ static Shares shares_of(long long P, int M, int N, int dtype) {
   return s;
 }
 
-// gw and gb: the shares' sums added in order and rounded once.  gw may be null, gb may be null.
+// gw (M, N) and gb (M): the shares' sums added in order and rounded once.  Rows of part have ldn elements.  Either may
+// be null.
 template <typename T, typename CT>
-__global__ void __launch_bounds__(256) add_shares_kernel(const CT* __restrict__ part, long long nw, T* __restrict__ gw,
-                                                         const CT* __restrict__ csum, int nb, T* __restrict__ gb,
-                                                         int splits) {
-  const long long total = nw + nb;
+__global__ void __launch_bounds__(256) add_shares_kernel(const CT* __restrict__ part, int M, int N, int ldn,
+                                                         T* __restrict__ gw, const CT* __restrict__ csum,
+                                                         T* __restrict__ gb, int splits) {
+  const long long nw = (long long)M * N, total = nw + M;
   for (long long i = blockIdx.x * 256ll + threadIdx.x; i < total; i += gridDim.x * 256ll) {
     const bool w = i < nw;
     if (!(w ? (void*)gw : (void*)gb)) continue;
-    const CT* src = w ? part + i : csum + (i - nw);
-    const long long step = w ? nw : nb;
+    const CT* src = w ? part + i / N * ldn + i % N : csum + (i - nw);
+    const long long step = w ? (long long)M * ldn : M;
     CT s = CT(0);
+#pragma unroll 8
     for (int j = 0; j < splits; ++j) s += src[j * step];
     stv(w ? gw + i : gb + (i - nw), s);
   }
@@ -68,11 +70,8 @@ __global__ void __launch_bounds__(256) act_bwd_kernel(const T* __restrict__ gy, 
 
 template <typename F>
 static int by_type(int dtype, F f) {
-  switch (dtype) {
-    case MC_F32: f(float()); break;
-    case MC_F64: f(double()); break;
-    default: f(bf16()); break;
-  }
+  if (dtype == MC_F64) f(double());
+  else f(float());
   MC_CHECK_LAUNCH();
   return MC_OK;
 }
@@ -86,9 +85,186 @@ static int param_grads(int dtype, long long P, long long S, View g, int M, View 
   return by_type(dtype, [&](auto t) {
     typedef decltype(t) T;
     typedef typename Traits<T>::CT CT;
-    add_shares_kernel<T, CT><<<grid_for(nw + M, 256), 256, 0, st>>>((const CT*)part, nw, (T*)gw, (const CT*)csum, M,
+    add_shares_kernel<T, CT><<<grid_for(nw + M, 256), 256, 0, st>>>((const CT*)part, M, N, N, (T*)gw, (const CT*)csum,
                                                                     (T*)gb, s.splits), MC_COUNT(1);
   });
+}
+
+// ---- bf16: the tensor-core kernels, on rows of channels --------------------------------------------------------------
+// Rows whose length is a multiple of 8 channels (16 bytes) are read and written where they lie; anything else - other
+// channel counts, NCHW - is copied to padded rows in the workspace and back.
+static int pad8(int c) { return (c + 7) / 8 * 8; }
+static bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
+
+// (R, C) without gaps -> rows of ld elements, zeros behind the last one
+__global__ void __launch_bounds__(256) pack_rows_kernel(const bf16* __restrict__ src, bf16* __restrict__ dst, long long R,
+                                                        int C, int ld) {
+  const long long groups = R * (ld / 8);
+  for (long long i = blockIdx.x * 256ll + threadIdx.x; i < groups; i += gridDim.x * 256ll) {
+    const long long r = i / (ld / 8);
+    const int c = (int)(i - r * (ld / 8)) * 8;
+    __align__(16) bf16 v[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = c + j < C ? src[r * C + c + j] : bf16(0.f);
+    *reinterpret_cast<uint4*>(dst + r * ld + c) = *reinterpret_cast<const uint4*>(v);
+  }
+}
+__global__ void __launch_bounds__(256) unpack_rows_kernel(const bf16* __restrict__ src, bf16* __restrict__ dst, long long R,
+                                                          int C, int ld) {
+  const long long n = R * C;
+  for (long long i = blockIdx.x * 256ll + threadIdx.x; i < n; i += gridDim.x * 256ll) {
+    const long long r = i / C;
+    dst[i] = src[r * ld + (i - r * C)];
+  }
+}
+// rows -> (B, C, S): 64 pixels x 64 channels at a time through shared memory
+__global__ void __launch_bounds__(256) rows_to_planes_kernel(const bf16* __restrict__ src, bf16* __restrict__ dst,
+                                                             long long S, int C, int ld, int tiles_s, int tiles_c) {
+  __shared__ bf16 tile[64 * 66];
+  const int tc = blockIdx.x % tiles_c, ts = blockIdx.x / tiles_c % tiles_s;
+  const long long b = blockIdx.x / tiles_c / tiles_s, s0 = ts * 64ll;
+  const int c0 = tc * 64;
+  for (int i = threadIdx.x; i < 64 * 8; i += 256) {
+    const int s = i / 8, c = i % 8 * 8;
+    uint4 v = make_uint4(0, 0, 0, 0);
+    if (s0 + s < S && c0 + c < ld) v = __ldcs(reinterpret_cast<const uint4*>(src + (b * S + s0 + s) * ld + c0 + c));
+    uint32_t* w = reinterpret_cast<uint32_t*>(tile + s * 66 + c);
+    w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < 64 * 64; i += 256) {
+    const int c = i / 64, s = i % 64;
+    if (c0 + c < C && s0 + s < S) dst[(b * C + c0 + c) * S + s0 + s] = tile[s * 66 + c];
+  }
+}
+
+// Lays a call's temporary tensors out in the workspace; without a workspace it only adds up their sizes.
+struct Work {
+  char* base;
+  cudaStream_t st;
+  size_t used = 0;
+  int rc = MC_OK;
+  bool run() const { return base && rc == MC_OK; }
+  char* take(size_t n) {
+    char* p = base ? base + used : nullptr;
+    used += up256(n);
+    return p;
+  }
+  void did(int r) { if (rc == MC_OK) rc = r; }
+  static bool in_place(const mc_mix_desc* d, int C) { return C % 8 == 0 && (d->layout == MC_NHWC || d->S == 1); }
+  TcRows fresh(long long rows, int C) { return TcRows{take((size_t)rows * pad8(C) * 2), rows, C, pad8(C)}; }
+  // an activation as rows
+  TcRows in(const mc_mix_desc* d, const void* p, int C) {
+    const long long P = pixels(d);
+    if (in_place(d, C)) return TcRows{p, P, C, C};
+    const TcRows r = fresh(P, C);
+    if (!run() || !p) return p || !base ? r : TcRows{nullptr, P, C, C};
+    if (d->layout == MC_NHWC || d->S == 1 || C == 1) {
+      pack_rows_kernel<<<grid_for(P * (r.ld / 8), 256), 256, 0, st>>>((const bf16*)p, (bf16*)r.p, P, C, r.ld), MC_COUNT(1);
+      did(cudaGetLastError() == cudaSuccess ? MC_OK : MC_ERR_LAUNCH);
+    } else {
+      did(mc_transpose(2, d->B, C, d->S, p, (void*)r.p, r.ld, st));
+    }
+    return r;
+  }
+  TcRows weight(const void* p, int R, int C) {
+    if (C % 8 == 0) return TcRows{p, R, C, C};
+    const TcRows r = fresh(R, C);
+    if (run()) {
+      pack_rows_kernel<<<grid_for(R * (r.ld / 8ll), 256), 256, 0, st>>>((const bf16*)p, (bf16*)r.p, R, C, r.ld), MC_COUNT(1);
+      did(cudaGetLastError() == cudaSuccess ? MC_OK : MC_ERR_LAUNCH);
+    }
+    return r;
+  }
+  // where an activation is computed as rows, and its way to where it belongs
+  TcRows out(const mc_mix_desc* d, void* p, int C) {
+    return in_place(d, C) ? TcRows{p, pixels(d), C, C} : fresh(pixels(d), C);
+  }
+  void put(const mc_mix_desc* d, const TcRows& r, void* p, int C) {
+    if (!run() || in_place(d, C)) return;
+    if (d->layout == MC_NHWC || d->S == 1 || C == 1) {
+      unpack_rows_kernel<<<grid_for(r.rows * C, 256), 256, 0, st>>>((const bf16*)r.p, (bf16*)p, r.rows, C, r.ld), MC_COUNT(1);
+    } else {
+      const long long ts = (d->S + 63) / 64, tc = (C + 63) / 64;
+      rows_to_planes_kernel<<<(unsigned)(d->B * ts * tc), 256, 0, st>>>((const bf16*)r.p, (bf16*)p, d->S, C, r.ld, (int)ts,
+                                                                        (int)tc), MC_COUNT(1);
+    }
+    did(cudaGetLastError() == cudaSuccess ? MC_OK : MC_ERR_LAUNCH);
+  }
+  void param_grads(const TcRows& g0, const TcRows& g1, int segs, const TcRows& x, void* gw, void* gb) {
+    int splits, ldn;
+    const size_t n = tc_outer_floats(x.rows, g0.cols, segs, x.cols, &splits, &ldn);
+    const int M = segs * g0.cols;
+    float* part = (float*)take(n * 4);
+    float* csum = (float*)take((size_t)splits * M * 4);
+    if (!run() || (!gw && !gb)) return;
+    did(tc_outer(g0, g1, x, part, csum, st));
+    if (rc) return;
+    const long long total = (long long)M * x.cols + M;
+    add_shares_kernel<bf16, float><<<grid_for(total, 256), 256, 0, st>>>(part, M, x.cols, ldn, (bf16*)gw, csum, (bf16*)gb,
+                                                                         splits), MC_COUNT(1);
+    did(cudaGetLastError() == cudaSuccess ? MC_OK : MC_ERR_LAUNCH);
+  }
+};
+
+static void tc_pointwise_fwd(Work& k, const mc_mix_desc* d, const void* x, const void* w, const void* bias,
+                             const void* residual, void* y) {
+  const TcRows xr = k.in(d, x, d->C_in), wr = k.weight(w, d->C_out, d->C_in), rr = k.in(d, residual, d->C_out);
+  const TcRows yr = k.out(d, y, d->C_out);
+  if (k.run()) k.did(tc_layer(xr, wr, (const bf16*)bias, d->act, rr, yr, false, k.st));
+  k.put(d, yr, y, d->C_out);
+}
+
+static void tc_pointwise_bwd(Work& k, const mc_mix_desc* d, const void* gy, const void* x, const void* w,
+                             const void* bias, void* gx, void* gw, void* gb) {
+  const TcRows xr = k.in(d, x, d->C_in), wr = k.weight(w, d->C_out, d->C_in), gyr = k.in(d, gy, d->C_out);
+  TcRows gz = gyr;
+  if (d->act != MC_ACT_NONE) {
+    gz = k.fresh(pixels(d), d->C_out);
+    if (k.run()) k.did(tc_layer(xr, wr, (const bf16*)bias, d->act, gyr, gz, true, k.st));
+  }
+  if (gx || !k.base) {
+    const TcRows gxr = k.out(d, gx, d->C_in);
+    if (k.run()) k.did(tc_input_grad(gz, wr, TcRows{}, TcRows{}, gxr, k.st));
+    k.put(d, gxr, gx, d->C_in);
+  }
+  k.param_grads(gz, TcRows{}, 1, xr, gw, gb);
+}
+
+static void tc_gated_fwd(Work& k, const mc_mix_desc* d, const void* x, const void* w_in, const void* b_in,
+                         const void* w_out, const void* b_out, const void* residual, void* y, void* saved) {
+  const int H = d->hidden;
+  const TcRows xr = k.in(d, x, d->C_in), wi = k.weight(w_in, 2 * H, d->C_in), wo = k.weight(w_out, d->C_out, H);
+  const TcRows h = saved ? TcRows{saved, pixels(d), H, pad8(H)} : k.fresh(pixels(d), H);
+  if (k.run()) k.did(tc_gate(xr, wi, (const bf16*)b_in, d->act, h, k.st));
+  const TcRows rr = k.in(d, residual, d->C_out), yr = k.out(d, y, d->C_out);
+  if (k.run()) k.did(tc_layer(h, wo, (const bf16*)b_out, MC_ACT_NONE, rr, yr, false, k.st));
+  k.put(d, yr, y, d->C_out);
+}
+
+static void tc_gated_bwd(Work& k, const mc_mix_desc* d, const void* gy, const void* x, const void* w_in, const void* b_in,
+                         const void* w_out, const void* saved, void* gx, void* gw_in, void* gb_in, void* gw_out,
+                         void* gb_out) {
+  const int H = d->hidden;
+  const TcRows xr = k.in(d, x, d->C_in), wi = k.weight(w_in, 2 * H, d->C_in), wo = k.weight(w_out, d->C_out, H);
+  const TcRows gyr = k.in(d, gy, d->C_out), gg = k.fresh(pixels(d), H), gu = k.fresh(pixels(d), H);
+  if (k.run() && (gx || gw_in || gb_in)) k.did(tc_gate_bwd(xr, wi, (const bf16*)b_in, d->act, gyr, wo, gg, gu, k.st));
+  if (gx || !k.base) {
+    const TcRows gxr = k.out(d, gx, d->C_in);
+    const TcRows wg{wi.p, H, wi.cols, wi.ld}, wu{(const char*)wi.p + (size_t)H * wi.ld * 2, H, wi.cols, wi.ld};
+    if (k.run()) k.did(tc_input_grad(gg, wg, gu, wu, gxr, k.st));
+    k.put(d, gxr, gx, d->C_in);
+  }
+  k.param_grads(gg, gu, 2, xr, gw_in, gb_in);
+  k.param_grads(gyr, TcRows{}, 1, TcRows{saved, pixels(d), H, pad8(H)}, gw_out, gb_out);
+}
+
+// workspace of the whole call, for any choice of optional arguments
+template <typename F>
+static size_t work_size(F f) {
+  Work k{nullptr, nullptr};
+  f(k);
+  return k.used + 256;  // (never zero: a null workspace means that sizes are wanted)
 }
 
 }  // namespace mix
@@ -101,12 +277,19 @@ extern "C" {
 // ---- pointwise layer ----------------------------------------------------------------------------------------
 
 size_t mc_pointwise_saved_bytes(const mc_mix_desc* d) {
-  if (check_desc(d, false) || d->act == MC_ACT_NONE) return 0;
+  if (check_desc(d, false) || d->act == MC_ACT_NONE || d->dtype == MC_BF16) return 0;
   return up256((size_t)pixels(d) * d->C_out * esize(d->dtype));
 }
 
-size_t mc_pointwise_workspace_bytes(const mc_mix_desc* d, int32_t backward) {
-  if (check_desc(d, false) || !backward) return 0;
+size_t mc_pointwise_workspace_bytes(const mc_mix_desc* d, int32_t phase) {
+  const bool backward = phase == MC_PHASE_BACKWARD;
+  if (check_desc(d, false)) return 0;
+  if (d->dtype == MC_BF16)
+    return work_size([&](Work& k) {
+      if (backward) tc_pointwise_bwd(k, d, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr);
+      else tc_pointwise_fwd(k, d, nullptr, nullptr, nullptr, nullptr, nullptr);
+    });
+  if (!backward) return 0;
   const Shares s = shares_of(pixels(d), d->C_out, d->C_in, d->dtype);
   return mc_pointwise_saved_bytes(d) + s.part + s.csum;
 }
@@ -116,8 +299,14 @@ int mc_pointwise_fwd(const mc_mix_desc* d, const void* x, const void* w, const v
   const int rc = check_desc(d, false);
   if (rc) return rc;
   if (!x || !w || !y) return MC_ERR_BAD_ARG;
-  if (ws_bytes < mc_pointwise_workspace_bytes(d, 0)) return MC_ERR_WORKSPACE;
-  (void)ws;
+  const size_t need = mc_pointwise_workspace_bytes(d, saved ? MC_PHASE_KEEP : MC_PHASE_FORWARD);
+  if (need && (!ws || ws_bytes < need)) return MC_ERR_WORKSPACE;
+  if (d->dtype == MC_BF16) {
+    if (!aligned16(x) || !aligned16(w) || !aligned16(residual) || !aligned16(y) || !aligned16(ws)) return MC_ERR_BAD_ARG;
+    Work k{(char*)ws, (cudaStream_t)stream};
+    tc_pointwise_fwd(k, d, x, w, bias, residual, y);
+    return k.rc;
+  }
   RowsArgs r{};
   r.a = image_view(x, d->layout, d->S, d->C_in);
   r.w = w, r.wn = d->C_in, r.wk = 1, r.bias = bias;
@@ -128,12 +317,18 @@ int mc_pointwise_fwd(const mc_mix_desc* d, const void* x, const void* w, const v
   return simt_rows_launch(d->dtype, EPI_LAYER, r, (cudaStream_t)stream);
 }
 
-int mc_pointwise_bwd(const mc_mix_desc* d, const void* gy, const void* x, const void* w, const void* saved, void* gx,
-                     void* gw, void* gb, void* ws, size_t ws_bytes, void* stream) {
+int mc_pointwise_bwd(const mc_mix_desc* d, const void* gy, const void* x, const void* w, const void* bias,
+                     const void* saved, void* gx, void* gw, void* gb, void* ws, size_t ws_bytes, void* stream) {
   int rc = check_desc(d, false);
   if (rc) return rc;
-  if (!gy || !x || !w || (d->act != MC_ACT_NONE && !saved)) return MC_ERR_BAD_ARG;
-  if (!ws || ws_bytes < mc_pointwise_workspace_bytes(d, 1)) return MC_ERR_WORKSPACE;
+  if (!gy || !x || !w || (mc_pointwise_saved_bytes(d) && !saved)) return MC_ERR_BAD_ARG;
+  if (!ws || ws_bytes < mc_pointwise_workspace_bytes(d, MC_PHASE_BACKWARD)) return MC_ERR_WORKSPACE;
+  if (d->dtype == MC_BF16) {
+    if (!aligned16(gy) || !aligned16(x) || !aligned16(w) || !aligned16(gx) || !aligned16(ws)) return MC_ERR_BAD_ARG;
+    Work k{(char*)ws, (cudaStream_t)stream};
+    tc_pointwise_bwd(k, d, gy, x, w, bias, gx, gw, gb);
+    return k.rc;
+  }
   cudaStream_t st = (cudaStream_t)stream;
   const long long P = pixels(d), n = P * d->C_out;
   const Shares s = shares_of(P, d->C_out, d->C_in, d->dtype);
@@ -165,17 +360,27 @@ int mc_pointwise_bwd(const mc_mix_desc* d, const void* gy, const void* x, const 
 
 // ---- gated feed-forward block -----------------------------------------------------------------------------------
 
-// kept for the backward pass: [g|u] (P, 2 H), then h (P, H)
+// kept for the backward pass: [g|u] (P, 2 H), then h (P, H); bf16: h in padded rows
 size_t mc_gated_saved_bytes(const mc_mix_desc* d) {
   if (check_desc(d, true)) return 0;
+  if (d->dtype == MC_BF16) return up256((size_t)pixels(d) * pad8(d->hidden) * 2);
   const size_t h = (size_t)pixels(d) * d->hidden * esize(d->dtype);
   return up256(2 * h) + up256(h);
 }
 
-size_t mc_gated_workspace_bytes(const mc_mix_desc* d, int32_t backward) {
+size_t mc_gated_workspace_bytes(const mc_mix_desc* d, int32_t phase) {
+  const bool backward = phase == MC_PHASE_BACKWARD;
   if (check_desc(d, true)) return 0;
+  if (d->dtype == MC_BF16)
+    return work_size([&](Work& k) {
+      if (backward)
+        tc_gated_bwd(k, d, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr);
+      else
+        tc_gated_fwd(k, d, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr,
+                     phase == MC_PHASE_KEEP ? (void*)256 : nullptr);  // (not touched: only sizes are added up)
+    });
   const size_t h = (size_t)pixels(d) * d->hidden * esize(d->dtype);
-  if (!backward) return up256(h);
+  if (!backward) return phase == MC_PHASE_KEEP ? 0 : up256(h);
   const Shares a = shares_of(pixels(d), 2 * d->hidden, d->C_in, d->dtype);
   const Shares b = shares_of(pixels(d), d->C_out, d->hidden, d->dtype);
   const size_t sa = a.part + a.csum, sb = b.part + b.csum;
@@ -187,8 +392,17 @@ int mc_gated_fwd(const mc_mix_desc* d, const void* x, const void* w_in, const vo
                  void* stream) {
   int rc = check_desc(d, true);
   if (rc) return rc;
-  if (!x || !w_in || !b_in || !w_out || !y) return MC_ERR_BAD_ARG;
-  if (!saved && (!ws || ws_bytes < mc_gated_workspace_bytes(d, 0))) return MC_ERR_WORKSPACE;
+  if (!x || !w_in || !w_out || !y) return MC_ERR_BAD_ARG;
+  const size_t need = mc_gated_workspace_bytes(d, saved ? MC_PHASE_KEEP : MC_PHASE_FORWARD);
+  if (need && (!ws || ws_bytes < need)) return MC_ERR_WORKSPACE;
+  if (d->dtype == MC_BF16) {
+    if (!aligned16(x) || !aligned16(w_in) || !aligned16(w_out) || !aligned16(residual) || !aligned16(y) ||
+        !aligned16(saved) || !aligned16(ws))
+      return MC_ERR_BAD_ARG;
+    Work k{(char*)ws, (cudaStream_t)stream};
+    tc_gated_fwd(k, d, x, w_in, b_in, w_out, b_out, residual, y, saved);
+    return k.rc;
+  }
   cudaStream_t st = (cudaStream_t)stream;
   const int H = d->hidden;
   const long long P = pixels(d);
@@ -210,13 +424,21 @@ int mc_gated_fwd(const mc_mix_desc* d, const void* x, const void* w_in, const vo
   return simt_rows_launch(d->dtype, EPI_LAYER, o, st);
 }
 
-int mc_gated_bwd(const mc_mix_desc* d, const void* gy, const void* x, const void* w_in, const void* w_out,
-                 const void* saved, void* gx, void* gw_in, void* gb_in, void* gw_out, void* gb_out, void* ws,
-                 size_t ws_bytes, void* stream) {
+int mc_gated_bwd(const mc_mix_desc* d, const void* gy, const void* x, const void* w_in, const void* b_in,
+                 const void* w_out, const void* saved, void* gx, void* gw_in, void* gb_in, void* gw_out, void* gb_out,
+                 void* ws, size_t ws_bytes, void* stream) {
   int rc = check_desc(d, true);
   if (rc) return rc;
   if (!gy || !x || !w_in || !w_out || !saved) return MC_ERR_BAD_ARG;
-  if (!ws || ws_bytes < mc_gated_workspace_bytes(d, 1)) return MC_ERR_WORKSPACE;
+  if (!ws || ws_bytes < mc_gated_workspace_bytes(d, MC_PHASE_BACKWARD)) return MC_ERR_WORKSPACE;
+  if (d->dtype == MC_BF16) {
+    if (!aligned16(gy) || !aligned16(x) || !aligned16(w_in) || !aligned16(w_out) || !aligned16(saved) || !aligned16(gx) ||
+        !aligned16(ws))
+      return MC_ERR_BAD_ARG;
+    Work k{(char*)ws, (cudaStream_t)stream};
+    tc_gated_bwd(k, d, gy, x, w_in, b_in, w_out, saved, gx, gw_in, gb_in, gw_out, gb_out);
+    return k.rc;
+  }
   cudaStream_t st = (cudaStream_t)stream;
   const int H = d->hidden;
   const long long P = pixels(d);

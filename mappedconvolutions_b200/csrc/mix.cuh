@@ -115,5 +115,26 @@ struct OuterArgs {
 };
 int simt_outer_launch(int dtype, const OuterArgs& a, cudaStream_t st);
 
+// ---- kernels on the tensor cores (mix_tc.cu): bf16 rows of ld elements (a multiple of 8), 16-byte aligned ------------
+struct TcRows {
+  const void* p;
+  long long rows;
+  int cols, ld;
+};
+// y = act(a w^T + bias) + r, or with backward y = r act'(a w^T + bias); w (N, K), r.p may be null (not with backward)
+int tc_layer(const TcRows& a, const TcRows& w, const bf16* bias, int act, const TcRows& r, const TcRows& y, bool backward,
+             cudaStream_t st);
+// gx = g0 w0 + g1 w1, w (K, N); g1.p may be null
+int tc_input_grad(const TcRows& g0, const TcRows& w0, const TcRows& g1, const TcRows& w1, const TcRows& gx,
+                  cudaStream_t st);
+// h = act(g) u, [g|u] = x w_in^T + b_in
+int tc_gate(const TcRows& x, const TcRows& w_in, const bf16* b_in, int act, const TcRows& h, cudaStream_t st);
+// gg = gh u act'(g), gu = gh act(g), gh = gy w_out
+int tc_gate_bwd(const TcRows& x, const TcRows& w_in, const bf16* b_in, int act, const TcRows& gy, const TcRows& w_out,
+                const TcRows& gg, const TcRows& gu, cudaStream_t st);
+// part[s] = the s-th share of [g0|g1]^T x (rows of *ldn floats), csum[s] = its column sums of [g0|g1]; g1.p may be null
+size_t tc_outer_floats(long long P, int M, int segs, int N, int* splits, int* ldn);
+int tc_outer(const TcRows& g0, const TcRows& g1, const TcRows& x, float* part, float* csum, cudaStream_t st);
+
 }  // namespace mix
 }  // namespace mc

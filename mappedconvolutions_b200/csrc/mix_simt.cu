@@ -1,5 +1,5 @@
-// Channel mixing on the CUDA cores: products of (pixels, channels) matrices in float32, float64 (and bf16 with
-// float32 sums), any layout, size and alignment.
+// Channel mixing on the CUDA cores: products of (pixels, channels) matrices in float32 and float64, any layout, size and
+// alignment.
 //
 // 128 x 128 outputs per block of 256 threads, 8 x 8 per thread (rows and columns in two groups of four, 64 apart), so
 // that a thread's two column groups are a gate and its factor where a block holds 64 columns of each.  The operands'
@@ -131,7 +131,8 @@ __global__ void __launch_bounds__(256) rows_kernel(const RowsArgs a, const PixDi
         if (res) o += (CT)ldv(res + ro + n * a.res.ch);
         stv(y + yo + n * a.y.ch, o);
       } else if (EPI == EPI_GATE) {
-        const CT g = acc[i][j] + (CT)ldv(bias + n), u = acc[i][j + 4] + (CT)ldv(bias + a.N + n);
+        const CT g = acc[i][j] + (bias ? (CT)ldv(bias + n) : CT(0));
+        const CT u = acc[i][j + 4] + (bias ? (CT)ldv(bias + a.N + n) : CT(0));
         if (z) {
           stv(z + zo + n * a.z.ch, g);
           stv(z + zo + (long long)(a.N + n) * a.z.ch, u);
@@ -234,11 +235,7 @@ static int rows_typed(Epilogue epi, const RowsArgs& a, cudaStream_t st) {
   return MC_OK;
 }
 int simt_rows_launch(int dtype, Epilogue epi, const RowsArgs& a, cudaStream_t st) {
-  switch (dtype) {
-    case MC_F32: return rows_typed<float>(epi, a, st);
-    case MC_F64: return rows_typed<double>(epi, a, st);
-    default: return rows_typed<bf16>(epi, a, st);
-  }
+  return dtype == MC_F64 ? rows_typed<double>(epi, a, st) : rows_typed<float>(epi, a, st);
 }
 
 template <typename T>
@@ -253,11 +250,7 @@ static int outer_typed(const OuterArgs& a, cudaStream_t st) {
   return MC_OK;
 }
 int simt_outer_launch(int dtype, const OuterArgs& a, cudaStream_t st) {
-  switch (dtype) {
-    case MC_F32: return outer_typed<float>(a, st);
-    case MC_F64: return outer_typed<double>(a, st);
-    default: return outer_typed<bf16>(a, st);
-  }
+  return dtype == MC_F64 ? outer_typed<double>(a, st) : outer_typed<float>(a, st);
 }
 
 }  // namespace mix

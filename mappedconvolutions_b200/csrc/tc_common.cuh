@@ -10,9 +10,9 @@ namespace mc {
 namespace tc {
 
 // Device status word: 0 = ok, otherwise the code of the first bounded wait that ran out
-// (kernel id * 16 + role).  Read back by mc_device_status().  File-scope on purpose: this header
-// is included by exactly one translation unit (conv_tc.cu), which keeps the build free of
-// relocatable device code.
+// (kernel id * 16 + role).  Read back by mc_device_status().  File-scope on purpose, which keeps the build free
+// of relocatable device code: each translation unit that includes this header (conv_tc.cu, mix_tc.cu) has a
+// word of its own and a function that reads it.
 static __device__ int g_status = 0;
 
 

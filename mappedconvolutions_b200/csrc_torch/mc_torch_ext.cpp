@@ -913,12 +913,13 @@ mc_mix_desc make_mix_desc(const Tensor& x, int layout, int64_t c_out, int64_t hi
   return d;
 }
 
-Tensor out_layout(const OptTensor& t, int layout) { return t.has_value() ? as_layout(*t, layout) : Tensor(); }
+Tensor out_layout(const OptTensor& t, int layout) { return t.has_value() ? aligned16(as_layout(*t, layout)) : Tensor(); }
 void* maybe(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 
 // (output, what the backward call needs)
-std::pair<Tensor, Tensor> pointwise_forward(const Tensor& x, const Tensor& w, const Tensor& b, const OptTensor& r,
+std::pair<Tensor, Tensor> pointwise_forward(const Tensor& x_in, const Tensor& w_in, const Tensor& b, const OptTensor& r,
                                             int64_t act, bool keep) {
+  const Tensor x = aligned16(x_in), w = aligned16(w_in);
   const auto dev = need_cuda({&x, &w, &b, opt(r)});
   check_weight_dims(w, "weight");
   TORCH_CHECK(x.dim() == 4, "input must be 4-D (B, C, H, W)");
@@ -934,19 +935,21 @@ std::pair<Tensor, Tensor> pointwise_forward(const Tensor& x, const Tensor& w, co
   if (y.numel() == 0) return {y, Tensor()};
   const Tensor res = out_layout(r, layout);
   Scratch saved = scratch(keep ? mc_pointwise_saved_bytes(&d) : 0, dev);
-  Scratch ws = scratch(mc_pointwise_workspace_bytes(&d, 0), dev);
+  Scratch ws = scratch(mc_pointwise_workspace_bytes(&d, keep ? MC_PHASE_KEEP : MC_PHASE_FORWARD), dev);
   check(mc_pointwise_fwd(&d, x.data_ptr(), w.data_ptr(), b.data_ptr(), maybe(res), y.data_ptr(), saved.p, ws.p, ws.n,
                          cur_stream()));
   return {y, saved.t};
 }
 
-std::vector<Tensor> pointwise_backward(const Tensor& gy_in, const OptTensor& saved, const Tensor& x, const Tensor& w,
-                                       int64_t act, bool need_input_grad, bool need_weight_grad) {
-  const auto dev = need_cuda({&gy_in, &x, &w, opt(saved)});
+std::vector<Tensor> pointwise_backward(const Tensor& gy_in, const OptTensor& saved, const Tensor& x_in, const Tensor& w_in,
+                                       const Tensor& b, int64_t act, bool need_input_grad, bool need_weight_grad) {
+  const Tensor x = aligned16(x_in), w = aligned16(w_in);
+  const auto dev = need_cuda({&gy_in, &x, &w, &b, opt(saved)});
   check_weight_dims(w, "weight");
   TORCH_CHECK(x.dim() == 4, "input must be 4-D (B, C, H, W)");
   const int64_t c_out = w.size(0);
   check_param(w, "weight", {c_out, x.size(1), 1}, x);
+  check_param(b, "bias", {c_out}, x);
   check_like(gy_in, "grad_output", {x.size(0), c_out, x.size(2), x.size(3)}, x);
   const int layout = layout_of(x);
   c10::cuda::CUDAGuard guard(dev);
@@ -957,16 +960,18 @@ std::vector<Tensor> pointwise_backward(const Tensor& gy_in, const OptTensor& sav
     gb = x.numel() == 0 ? at::zeros({c_out}, w.options()) : at::empty({c_out}, w.options());
   }
   if (x.numel() == 0) return {gx, gw, gb};
-  const Tensor gy = as_layout(gy_in, layout);
+  const Tensor gy = aligned16(as_layout(gy_in, layout));
   const mc_mix_desc d = make_mix_desc(x, layout, c_out, 0, act);
-  Scratch ws = scratch(mc_pointwise_workspace_bytes(&d, 1), dev);
-  check(mc_pointwise_bwd(&d, gy.data_ptr(), x.data_ptr(), w.data_ptr(), ptr(saved), maybe(gx), maybe(gw), maybe(gb),
-                         ws.p, ws.n, cur_stream()));
+  Scratch ws = scratch(mc_pointwise_workspace_bytes(&d, MC_PHASE_BACKWARD), dev);
+  check(mc_pointwise_bwd(&d, gy.data_ptr(), x.data_ptr(), w.data_ptr(), b.data_ptr(), ptr(saved), maybe(gx), maybe(gw),
+                         maybe(gb), ws.p, ws.n, cur_stream()));
   return {gx, gw, gb};
 }
 
-std::pair<Tensor, Tensor> gated_forward(const Tensor& x, const Tensor& w_in, const Tensor& b_in, const Tensor& w_out,
-                                        const Tensor& b_out, const OptTensor& r, int64_t act, bool keep) {
+std::pair<Tensor, Tensor> gated_forward(const Tensor& x_any, const Tensor& w_in_any, const Tensor& b_in,
+                                        const Tensor& w_out_any, const Tensor& b_out, const OptTensor& r, int64_t act,
+                                        bool keep) {
+  const Tensor x = aligned16(x_any), w_in = aligned16(w_in_any), w_out = aligned16(w_out_any);
   const auto dev = need_cuda({&x, &w_in, &b_in, &w_out, &b_out, opt(r)});
   check_weight_dims(w_in, "weight_in");
   check_weight_dims(w_out, "weight_out");
@@ -985,21 +990,24 @@ std::pair<Tensor, Tensor> gated_forward(const Tensor& x, const Tensor& w_in, con
   if (y.numel() == 0) return {y, Tensor()};
   const Tensor res = out_layout(r, layout);
   Scratch saved = scratch(keep ? mc_gated_saved_bytes(&d) : 0, dev);
-  Scratch ws = scratch(keep ? 0 : mc_gated_workspace_bytes(&d, 0), dev);
+  Scratch ws = scratch(mc_gated_workspace_bytes(&d, keep ? MC_PHASE_KEEP : MC_PHASE_FORWARD), dev);
   check(mc_gated_fwd(&d, x.data_ptr(), w_in.data_ptr(), b_in.data_ptr(), w_out.data_ptr(), b_out.data_ptr(), maybe(res),
                      y.data_ptr(), saved.p, ws.p, ws.n, cur_stream()));
   return {y, saved.t};
 }
 
-std::vector<Tensor> gated_backward(const Tensor& gy_in, const OptTensor& saved, const Tensor& x, const Tensor& w_in,
-                                   const Tensor& w_out, int64_t act, bool need_input_grad, bool need_weight_grad) {
-  const auto dev = need_cuda({&gy_in, &x, &w_in, &w_out, opt(saved)});
+std::vector<Tensor> gated_backward(const Tensor& gy_in, const OptTensor& saved, const Tensor& x_any, const Tensor& w_in_any,
+                                   const Tensor& b_in, const Tensor& w_out_any, int64_t act, bool need_input_grad,
+                                   bool need_weight_grad) {
+  const Tensor x = aligned16(x_any), w_in = aligned16(w_in_any), w_out = aligned16(w_out_any);
+  const auto dev = need_cuda({&gy_in, &x, &w_in, &b_in, &w_out, opt(saved)});
   check_weight_dims(w_in, "weight_in");
   check_weight_dims(w_out, "weight_out");
   TORCH_CHECK(x.dim() == 4, "input must be 4-D (B, C, H, W)");
   const int64_t c_out = w_out.size(0), hidden = w_out.size(1);
   check_param(w_in, "weight_in", {2 * hidden, x.size(1), 1}, x);
   check_param(w_out, "weight_out", {c_out, hidden, 1}, x);
+  check_param(b_in, "bias_in", {2 * hidden}, x);
   check_like(gy_in, "grad_output", {x.size(0), c_out, x.size(2), x.size(3)}, x);
   const int layout = layout_of(x);
   c10::cuda::CUDAGuard guard(dev);
@@ -1011,11 +1019,11 @@ std::vector<Tensor> gated_backward(const Tensor& gy_in, const OptTensor& saved, 
       g[i + 1] = x.numel() == 0 ? at::zeros(shapes[i], x.options()) : at::empty(shapes[i], x.options());
   }
   if (x.numel() == 0) return g;
-  const Tensor gy = as_layout(gy_in, layout);
+  const Tensor gy = aligned16(as_layout(gy_in, layout));
   const mc_mix_desc d = make_mix_desc(x, layout, c_out, hidden, act);
-  Scratch ws = scratch(mc_gated_workspace_bytes(&d, 1), dev);
-  check(mc_gated_bwd(&d, gy.data_ptr(), x.data_ptr(), w_in.data_ptr(), w_out.data_ptr(), ptr(saved), maybe(g[0]),
-                     maybe(g[1]), maybe(g[2]), maybe(g[3]), maybe(g[4]), ws.p, ws.n, cur_stream()));
+  Scratch ws = scratch(mc_gated_workspace_bytes(&d, MC_PHASE_BACKWARD), dev);
+  check(mc_gated_bwd(&d, gy.data_ptr(), x.data_ptr(), w_in.data_ptr(), b_in.data_ptr(), w_out.data_ptr(), ptr(saved),
+                     maybe(g[0]), maybe(g[1]), maybe(g[2]), maybe(g[3]), maybe(g[4]), ws.p, ws.n, cur_stream()));
   return g;
 }
 
@@ -1279,7 +1287,7 @@ struct PointwiseFn : torch::autograd::Function<PointwiseFn> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const Tensor& b, const OptTensor& r,
                         int64_t act) {
     auto f = pointwise_forward(x, w, b, r, act, true);
-    ctx->save_for_backward({x, w, f.second});
+    ctx->save_for_backward({x, w, b, f.second});
     ctx->saved_data["a"] = act;
     ctx->saved_data["r"] = r.has_value();  // (needs_input_grad counts the tensors that were given)
     return f.first;
@@ -1289,7 +1297,7 @@ struct PointwiseFn : torch::autograd::Function<PointwiseFn> {
     const bool need_x = ctx->needs_input_grad(0), need_p = ctx->needs_input_grad(1) || ctx->needs_input_grad(2);
     variable_list out(5);
     if (need_x || need_p) {
-      auto r = pointwise_backward(g[0], as_opt(s[2]), s[0], s[1], ctx->saved_data["a"].toInt(), need_x, need_p);
+      auto r = pointwise_backward(g[0], as_opt(s[3]), s[0], s[1], s[2], ctx->saved_data["a"].toInt(), need_x, need_p);
       for (int i = 0; i < 3; ++i) out[i] = r[i];
     }
     if (ctx->saved_data["r"].toBool() && ctx->needs_input_grad(3)) out[3] = g[0];
@@ -1301,7 +1309,7 @@ struct GatedFn : torch::autograd::Function<GatedFn> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& wi, const Tensor& bi, const Tensor& wo,
                         const Tensor& bo, const OptTensor& r, int64_t act) {
     auto f = gated_forward(x, wi, bi, wo, bo, r, act, true);
-    ctx->save_for_backward({x, wi, wo, f.second});
+    ctx->save_for_backward({x, wi, bi, wo, f.second});
     ctx->saved_data["a"] = act;
     ctx->saved_data["r"] = r.has_value();  // (needs_input_grad counts the tensors that were given)
     return f.first;
@@ -1313,7 +1321,7 @@ struct GatedFn : torch::autograd::Function<GatedFn> {
     const bool need_x = ctx->needs_input_grad(0);
     variable_list out(7);
     if (need_x || need_p) {
-      auto r = gated_backward(g[0], as_opt(s[3]), s[0], s[1], s[2], ctx->saved_data["a"].toInt(), need_x, need_p);
+      auto r = gated_backward(g[0], as_opt(s[4]), s[0], s[1], s[2], s[3], ctx->saved_data["a"].toInt(), need_x, need_p);
       for (int i = 0; i < 5; ++i) out[i] = r[i];
     }
     if (ctx->saved_data["r"].toBool() && ctx->needs_input_grad(5)) out[5] = g[0];
@@ -1470,12 +1478,14 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("input"), py::arg("weight"), py::arg("bias"), py::arg("residual") = py::none(), py::arg("activation") = 0,
         py::arg("keep") = false);
   def("pointwise_backward",
-        [](const Tensor& gy, const OptTensor& saved, const Tensor& x, const Tensor& w, int64_t act, bool nx, bool np) {
+        [](const Tensor& gy, const OptTensor& saved, const Tensor& x, const Tensor& w, const Tensor& b, int64_t act, bool nx,
+           bool np) {
           std::vector<OptTensor> r;
-          for (const Tensor& t : pointwise_backward(gy, saved, x, w, act, nx, np)) r.push_back(as_opt(t));
+          for (const Tensor& t : pointwise_backward(gy, saved, x, w, b, act, nx, np)) r.push_back(as_opt(t));
           return r;
         },
-        py::arg("grad_output"), py::arg("saved"), py::arg("input"), py::arg("weight"), py::arg("activation") = 0,
+        py::arg("grad_output"), py::arg("saved"), py::arg("input"), py::arg("weight"), py::arg("bias"),
+        py::arg("activation") = 0,
         py::arg("need_input_grad") = true, py::arg("need_weight_grad") = true);
   def("gated_forward",
         [](const Tensor& x, const Tensor& wi, const Tensor& bi, const Tensor& wo, const Tensor& bo, const OptTensor& r,
@@ -1486,14 +1496,14 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("input"), py::arg("weight_in"), py::arg("bias_in"), py::arg("weight_out"), py::arg("bias_out"),
         py::arg("residual") = py::none(), py::arg("activation") = 4, py::arg("keep") = false);
   def("gated_backward",
-        [](const Tensor& gy, const OptTensor& saved, const Tensor& x, const Tensor& wi, const Tensor& wo, int64_t act, bool nx,
-           bool np) {
+        [](const Tensor& gy, const OptTensor& saved, const Tensor& x, const Tensor& wi, const Tensor& bi, const Tensor& wo,
+           int64_t act, bool nx, bool np) {
           std::vector<OptTensor> r;
-          for (const Tensor& t : gated_backward(gy, saved, x, wi, wo, act, nx, np)) r.push_back(as_opt(t));
+          for (const Tensor& t : gated_backward(gy, saved, x, wi, bi, wo, act, nx, np)) r.push_back(as_opt(t));
           return r;
         },
-        py::arg("grad_output"), py::arg("saved"), py::arg("input"), py::arg("weight_in"), py::arg("weight_out"),
-        py::arg("activation") = 4, py::arg("need_input_grad") = true, py::arg("need_weight_grad") = true);
+        py::arg("grad_output"), py::arg("saved"), py::arg("input"), py::arg("weight_in"), py::arg("bias_in"),
+        py::arg("weight_out"), py::arg("activation") = 4, py::arg("need_input_grad") = true, py::arg("need_weight_grad") = true);
   def("pointwise_layer", [](const Tensor& x, const Tensor& w, const Tensor& b, const OptTensor& r, int64_t act) -> OptTensor {
     if (seen_by_torch({&x, &w, &b, opt(r)})) return c10::nullopt;
     if (!records({&x, &w, &b, opt(r)})) return pointwise_forward(x, w, b, r, act, false).first;

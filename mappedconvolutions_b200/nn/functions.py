@@ -200,16 +200,16 @@ class PointwiseFn(Function):
     def forward(ctx, x, weight, bias, residual, activation):
         ctx.activation = int(activation)
         y, saved = ops.pointwise_forward(x, weight, bias, residual, ctx.activation, True)
-        ctx.save_for_backward(x, weight, saved)
+        ctx.save_for_backward(x, weight, bias, saved)
         return y
 
     @staticmethod
     def backward(ctx, gy):
-        x, weight, saved = ctx.saved_tensors
+        x, weight, bias, saved = ctx.saved_tensors
         need = ctx.needs_input_grad
         g = [None] * 3
         if any(need[:3]):
-            g = ops.pointwise_backward(gy, saved, x, weight, ctx.activation, need[0], need[1] or need[2])
+            g = ops.pointwise_backward(gy, saved, x, weight, bias, ctx.activation, need[0], need[1] or need[2])
         return (*g, gy if need[3] else None, None)
 
 
@@ -220,16 +220,17 @@ class GatedFn(Function):
     def forward(ctx, x, weight_in, bias_in, weight_out, bias_out, residual, activation):
         ctx.activation = int(activation)
         y, saved = ops.gated_forward(x, weight_in, bias_in, weight_out, bias_out, residual, ctx.activation, True)
-        ctx.save_for_backward(x, weight_in, weight_out, saved)
+        ctx.save_for_backward(x, weight_in, bias_in, weight_out, saved)
         return y
 
     @staticmethod
     def backward(ctx, gy):
-        x, weight_in, weight_out, saved = ctx.saved_tensors
+        x, weight_in, bias_in, weight_out, saved = ctx.saved_tensors
         need = ctx.needs_input_grad
         g = [None] * 5
         if any(need[:5]):
-            g = ops.gated_backward(gy, saved, x, weight_in, weight_out, ctx.activation, need[0], any(need[1:5]))
+            g = ops.gated_backward(gy, saved, x, weight_in, bias_in, weight_out, ctx.activation, need[0],
+                                   any(need[1:5]))
         return (*g, gy if need[5] else None, None)
 
 

@@ -828,17 +828,19 @@ def pointwise_forward(input, weight, bias, residual=None, activation=0, keep=Fal
     with torch.cuda.device(dev):
         L = lib()
         saved = _bytes(L.mc_pointwise_saved_bytes(d), dev) if keep else None
-        wst, wsn, wsp = _ws(L.mc_pointwise_workspace_bytes(d, 0), dev)
+        wst, wsn, wsp = _ws(L.mc_pointwise_workspace_bytes(d, 2 if keep else 0), dev)
+        input, weight, residual = _a16(input), _a16(weight), _a16(residual)
         check(L.mc_pointwise_fwd(d, input.data_ptr(), weight.data_ptr(), bias.data_ptr(), _ptr(residual), y.data_ptr(),
                                  _ptr(saved), wsp, wsn, _stream()))
     return [y, saved]
 
 
-def pointwise_backward(grad_output, saved, input, weight, activation=0, need_input_grad=True, need_weight_grad=True):
+def pointwise_backward(grad_output, saved, input, weight, bias, activation=0, need_input_grad=True, need_weight_grad=True):
     """-> [grad_input, grad_weight, grad_bias]; the residual's gradient is grad_output"""
-    dev = _need_cuda(grad_output, input, weight, saved)
+    dev = _need_cuda(grad_output, input, weight, bias, saved)
     c_out, c_in = _weight_dims(weight, "weight")
-    _check_mix(input, [("weight", weight, (c_out, input.shape[1] if input.dim() > 1 else 0, 1))], None, c_out, grad_output)
+    _check_mix(input, [("weight", weight, (c_out, input.shape[1] if input.dim() > 1 else 0, 1)), ("bias", bias, (c_out,))],
+               None, c_out, grad_output)
     layout = _layout(input)
     gx = _empty(input.shape, input, layout) if need_input_grad else None
     make = torch.zeros if input.numel() == 0 else torch.empty
@@ -851,8 +853,9 @@ def pointwise_backward(grad_output, saved, input, weight, activation=0, need_inp
     with torch.cuda.device(dev):
         L = lib()
         wst, wsn, wsp = _ws(L.mc_pointwise_workspace_bytes(d, 1), dev)
-        check(L.mc_pointwise_bwd(d, grad_output.data_ptr(), input.data_ptr(), weight.data_ptr(), _ptr(saved), _ptr(gx),
-                                 _ptr(gw), _ptr(gb), wsp, wsn, _stream()))
+        input, weight, grad_output = _a16(input), _a16(weight), _a16(grad_output)
+        check(L.mc_pointwise_bwd(d, grad_output.data_ptr(), input.data_ptr(), weight.data_ptr(), bias.data_ptr(), _ptr(saved),
+                                 _ptr(gx), _ptr(gw), _ptr(gb), wsp, wsn, _stream()))
     return [gx, gw, gb]
 
 
@@ -879,18 +882,19 @@ def gated_forward(input, weight_in, bias_in, weight_out, bias_out, residual=None
     with torch.cuda.device(dev):
         L = lib()
         saved = _bytes(L.mc_gated_saved_bytes(d), dev) if keep else None
-        wst, wsn, wsp = _ws(0 if keep else L.mc_gated_workspace_bytes(d, 0), dev)
+        wst, wsn, wsp = _ws(L.mc_gated_workspace_bytes(d, 2 if keep else 0), dev)
+        input, weight_in, weight_out, residual = _a16(input), _a16(weight_in), _a16(weight_out), _a16(residual)
         check(L.mc_gated_fwd(d, input.data_ptr(), weight_in.data_ptr(), bias_in.data_ptr(), weight_out.data_ptr(),
                              bias_out.data_ptr(), _ptr(residual), y.data_ptr(), _ptr(saved), wsp, wsn, _stream()))
     return [y, saved]
 
 
-def gated_backward(grad_output, saved, input, weight_in, weight_out, activation=4, need_input_grad=True,
+def gated_backward(grad_output, saved, input, weight_in, bias_in, weight_out, activation=4, need_input_grad=True,
                    need_weight_grad=True):
     """-> [grad_input, grad_weight_in, grad_bias_in, grad_weight_out, grad_bias_out]"""
-    dev = _need_cuda(grad_output, input, weight_in, weight_out, saved)
+    dev = _need_cuda(grad_output, input, weight_in, bias_in, weight_out, saved)
     c_out, hidden, params = _gated_dims(input, weight_in, weight_out)
-    _check_mix(input, params, None, c_out, grad_output)
+    _check_mix(input, params + [("bias_in", bias_in, (2 * hidden,))], None, c_out, grad_output)
     layout = _layout(input)
     gx = _empty(input.shape, input, layout) if need_input_grad else None
     make = torch.zeros if input.numel() == 0 else torch.empty
@@ -903,8 +907,9 @@ def gated_backward(grad_output, saved, input, weight_in, weight_out, activation=
     with torch.cuda.device(dev):
         L = lib()
         wst, wsn, wsp = _ws(L.mc_gated_workspace_bytes(d, 1), dev)
-        check(L.mc_gated_bwd(d, grad_output.data_ptr(), input.data_ptr(), weight_in.data_ptr(), weight_out.data_ptr(),
-                             _ptr(saved), _ptr(gx), *[_ptr(g) for g in grads], wsp, wsn, _stream()))
+        input, weight_in, weight_out, grad_output = _a16(input), _a16(weight_in), _a16(weight_out), _a16(grad_output)
+        check(L.mc_gated_bwd(d, grad_output.data_ptr(), input.data_ptr(), weight_in.data_ptr(), bias_in.data_ptr(),
+                             weight_out.data_ptr(), _ptr(saved), _ptr(gx), *[_ptr(g) for g in grads], wsp, wsn, _stream()))
     return [gx] + grads
 
 

@@ -54,13 +54,13 @@ def test_pointwise(ops, i, dtype, layout):
         y, saved = ops.pointwise_forward(x, weight, bias, r, R.ACTS[name], True)
         y2, none = ops.pointwise_forward(x, weight, bias, r, R.ACTS[name], False)
         assert none is None and torch.equal(y, y2) and layout_kept(y, layout)
-        gx, gw, gb = ops.pointwise_backward(gy, saved, x, weight, R.ACTS[name])
+        gx, gw, gb = ops.pointwise_backward(gy, saved, x, weight, bias, R.ACTS[name])
         assert layout_kept(gx, layout)
         R.check(dict(y=y, gx=gx, gw=gw, gb=gb), want, str((SHAPES[i], name)))
-        again = ops.pointwise_backward(gy, saved, x, weight, R.ACTS[name])
+        again = ops.pointwise_backward(gy, saved, x, weight, bias, R.ACTS[name])
         assert all(torch.equal(p, q) for p, q in zip((gx, gw, gb), again))  # fixed order of every sum
-        only_x = ops.pointwise_backward(gy, saved, x, weight, R.ACTS[name], True, False)
-        only_w = ops.pointwise_backward(gy, saved, x, weight, R.ACTS[name], False, True)
+        only_x = ops.pointwise_backward(gy, saved, x, weight, bias, R.ACTS[name], True, False)
+        only_w = ops.pointwise_backward(gy, saved, x, weight, bias, R.ACTS[name], False, True)
         assert torch.equal(only_x[0], gx) and only_x[1] is None and only_w[0] is None and torch.equal(only_w[1], gw)
 
 
@@ -79,14 +79,14 @@ def test_gated(ops, i, dtype, layout):
         y, saved = ops.gated_forward(x, wi, bi, wo, bo, r, R.ACTS[name], True)
         y2, none = ops.gated_forward(x, wi, bi, wo, bo, r, R.ACTS[name], False)
         assert none is None and torch.equal(y, y2) and layout_kept(y, layout)
-        grads = ops.gated_backward(gy, saved, x, wi, wo, R.ACTS[name])
+        grads = ops.gated_backward(gy, saved, x, wi, bi, wo, R.ACTS[name])
         assert layout_kept(grads[0], layout)
         names = ("gx", "gw_in", "gb_in", "gw_out", "gb_out")
         R.check(dict(zip(names, grads), y=y), want, str((SHAPES[i], name)))
-        again = ops.gated_backward(gy, saved, x, wi, wo, R.ACTS[name])
+        again = ops.gated_backward(gy, saved, x, wi, bi, wo, R.ACTS[name])
         assert all(torch.equal(p, q) for p, q in zip(grads, again))
-        only_x = ops.gated_backward(gy, saved, x, wi, wo, R.ACTS[name], True, False)
-        only_w = ops.gated_backward(gy, saved, x, wi, wo, R.ACTS[name], False, True)
+        only_x = ops.gated_backward(gy, saved, x, wi, bi, wo, R.ACTS[name], True, False)
+        only_w = ops.gated_backward(gy, saved, x, wi, bi, wo, R.ACTS[name], False, True)
         assert torch.equal(only_x[0], grads[0]) and only_x[1:] == [None] * 4 and only_w[0] is None
         assert all(torch.equal(p, q) for p, q in zip(grads[1:], only_w[1:]))
 
@@ -100,7 +100,7 @@ def test_many_pixels(dtype):
     wi, bi = params(g, 2 * hidden, cin, dtype)
     wo, bo = params(g, cout, hidden, dtype)
     y, saved = host.impl.gated_forward(x, wi, bi, wo, bo, None, 4, True)
-    grads = host.impl.gated_backward(gy, saved, x, wi, wo, 4)
+    grads = host.impl.gated_backward(gy, saved, x, wi, bi, wo, 4)
     R.check(dict(zip(("gx", "gw_in", "gb_in", "gw_out", "gb_out"), grads), y=y), R.gated(x, wi, bi, wo, bo, None, "silu", gy))
 
 
@@ -162,13 +162,13 @@ def test_no_pixels(ops, shape, dtype):
     w, b = torch.ones(8, 16, 1, device="cuda", dtype=dtype), torch.ones(8, device="cuda", dtype=dtype)
     y, saved = ops.pointwise_forward(x, w, b, None, 1, True)
     assert y.shape == (shape[0], 8, *shape[2:])
-    gx, gw, gb = ops.pointwise_backward(y, saved, x, w, 1)
+    gx, gw, gb = ops.pointwise_backward(y, saved, x, w, b, 1)
     assert gx.shape == x.shape and not gw.any() and not gb.any()
     wi, bi = torch.ones(8, 16, 1, device="cuda", dtype=dtype), torch.ones(8, device="cuda", dtype=dtype)
     wo, bo = torch.ones(16, 4, 1, device="cuda", dtype=dtype), torch.ones(16, device="cuda", dtype=dtype)
     y, saved = ops.gated_forward(x, wi, bi, wo, bo, None, 4, True)
     assert y.shape == shape
-    assert not any(t.any() for t in ops.gated_backward(y, saved, x, wi, wo, 4)[1:])
+    assert not any(t.any() for t in ops.gated_backward(y, saved, x, wi, bi, wo, 4)[1:])
 
 
 @pytest.mark.parametrize("dtype", [BF, F32, F64], ids=["bf16", "f32", "f64"])
@@ -206,10 +206,10 @@ def test_views_that_start_anywhere(ops):
             wi, bi = flat[55:115].view(12, 5, 1), flat[115:127]
             wo, bo = flat[127:181].view(9, 6, 1), flat[181:190]
             y, saved = ops.pointwise_forward(x, w, b, r, 2, True)
-            g3 = ops.pointwise_backward(gy, saved, x, w, 2)
+            g3 = ops.pointwise_backward(gy, saved, x, w, b, 2)
             R.check(dict(zip(("gx", "gw", "gb"), g3), y=y), R.pointwise(x, w, b, r, "gelu", gy))
             y, saved = ops.gated_forward(x, wi, bi, wo, bo, r, 2, True)
-            g5 = ops.gated_backward(gy, saved, x, wi, wo, 2)
+            g5 = ops.gated_backward(gy, saved, x, wi, bi, wo, 2)
             R.check(dict(zip(("gx", "gw_in", "gb_in", "gw_out", "gb_out"), g5), y=y), R.gated(x, wi, bi, wo, bo, r, "gelu", gy))
 
 
@@ -246,9 +246,9 @@ def test_refusals(ops):
         with pytest.raises(RuntimeError, match="bad argument"):
             ops.pointwise_forward(x, w, b, r, act)
     with pytest.raises(RuntimeError):  # needs what the forward call kept
-        ops.pointwise_backward(r, None, x, w, 1)
+        ops.pointwise_backward(r, None, x, w, b, 1)
     with pytest.raises(RuntimeError):
-        ops.pointwise_backward(r[:, :8], None, x, w, 0)
+        ops.pointwise_backward(r[:, :8], None, x, w, b, 0)
     wi, bi = torch.randn(24, 8, 1, device="cuda"), torch.randn(24, device="cuda")
     wo, bo = torch.randn(16, 12, 1, device="cuda"), torch.randn(16, device="cuda")
     ops.gated_forward(x, wi, bi, wo, bo, r)
@@ -257,7 +257,7 @@ def test_refusals(ops):
         with pytest.raises(RuntimeError):
             ops.gated_forward(*args)
     with pytest.raises(RuntimeError):
-        ops.gated_backward(r, None, x, wi, wo)
+        ops.gated_backward(r, None, x, wi, bi, wo)
 
 
 @pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "f32"])
@@ -312,6 +312,27 @@ def test_other_streams():
     assert all(torch.equal(a, b) for a, b in zip(got, want))
 
 
+def test_first_cuda_call_of_a_thread():
+    """with all memory cached, the tensor maps of a call are the first thing that its thread asks the driver for"""
+    import threading
+    g = torch.Generator("cuda").manual_seed(20)
+    x, (w, b) = image(g, (2, 64, 8, 16), BF, "nhwc"), params(g, 64, 64, BF)
+    want = host.impl.pointwise_forward(x, w, b, None, 1)[0].clone()
+    got = []
+    torch.cuda.synchronize()
+
+    def call():
+        try:
+            got.append(host.impl.pointwise_forward(x, w, b, None, 1)[0])
+        except RuntimeError as e:
+            got.append(e)
+    for _ in range(2):
+        t = threading.Thread(target=call)
+        t.start()
+        t.join()
+    assert all(isinstance(y, torch.Tensor) and torch.equal(y, want) for y in got), got
+
+
 def test_offsets_beyond_32_bits():
     """an activation of more than 2^32 bytes and 2^31 elements: its last pixels"""
     n, cin, cout = 35_000_001, 64, 8
@@ -324,7 +345,7 @@ def test_offsets_beyond_32_bits():
     R.check(dict(y=y[..., -300:]), R.pointwise(tail, w, b, None, "relu"))
     gy = torch.zeros_like(y)
     gy[..., -300:] = torch.randn(1, cout, 1, 300, generator=g, device="cuda").to(BF)
-    gx, gw, gb = host.impl.pointwise_backward(gy, saved, x, w, 1)
+    gx, gw, gb = host.impl.pointwise_backward(gy, saved, x, w, b, 1)
     want = R.pointwise(tail, w, b, None, "relu", gy[..., -300:])
     R.check(dict(gx=gx[..., -300:], gw=gw, gb=gb), want)
     assert not gx[..., :-300].any()

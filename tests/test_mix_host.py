@@ -49,9 +49,9 @@ def test_argument_checks():
 def test_no_cpu_path(ops):
     x, w, b = torch.zeros(1, 3, 4, 5), torch.zeros(4, 3, 1), torch.zeros(4)
     wi, bi, wo = torch.zeros(16, 3, 1), torch.zeros(16), torch.zeros(4, 8, 1)
-    for call in (lambda: ops.pointwise_forward(x, w, b), lambda: ops.pointwise_backward(torch.zeros(1, 4, 4, 5), None, x, w),
+    for call in (lambda: ops.pointwise_forward(x, w, b), lambda: ops.pointwise_backward(torch.zeros(1, 4, 4, 5), None, x, w, b),
                  lambda: ops.gated_forward(x, wi, bi, wo, b),
-                 lambda: ops.gated_backward(torch.zeros(1, 4, 4, 5), b, x, wi, wo),
+                 lambda: ops.gated_backward(torch.zeros(1, 4, 4, 5), b, x, wi, bi, wo),
                  lambda: ops.gradient_norm([b]), lambda: ops.clip_gradients([b], 1.0),
                  lambda: mnn.PointwiseConvolution(3, 4)(x), lambda: mdist.clip_gradients([None, b], 1.0)):
         with pytest.raises(RuntimeError, match="CUDA only"):
@@ -73,13 +73,16 @@ def test_abi_checks_come_before_any_cuda_call():
     assert fwd(desc(), None) == -1
     for change in (dict(B=1 << 20, S=1 << 20), dict(S=1 << 31), dict(B=1 << 33, S=1 << 30), dict(B=1 << 62, S=1 << 2), dict(C_in=1 << 21)):
         assert fwd(desc(**change)) == -6
-    assert L.mc_pointwise_bwd(desc(), 1, 1, 1, None, 1, 1, 1, 1, 1 << 30, None) == -1  # saved is missing
-    assert L.mc_pointwise_bwd(desc(), 1, 1, 1, 1, 1, 1, 1, None, 0, None) == -3
+    assert L.mc_pointwise_bwd(desc(), 1, 1, 1, 1, None, 1, 1, 1, 1, 1 << 30, None) == -1  # saved is missing
+    assert L.mc_pointwise_bwd(desc(), 1, 1, 1, 1, 1, 1, 1, 1, None, 0, None) == -3
     gated = dict(hidden=8, act=4)
     assert L.mc_gated_fwd(desc(), *[1] * 9, 1 << 30, None) == -1                       # no hidden channels
     assert L.mc_gated_fwd(desc(**gated), 1, 1, 1, 1, 1, None, 1, None, None, 0, None) == -3
-    assert L.mc_gated_bwd(desc(**gated), 1, 1, 1, 1, 1, 1, 1, 1, 1, 1, None, 0, None) == -3
-    assert L.mc_gated_bwd(desc(**gated), 1, 1, 1, 1, None, 1, 1, 1, 1, 1, 1, 1 << 30, None) == -1
+    assert L.mc_gated_bwd(desc(**gated), *[1] * 11, None, 0, None) == -3
+    assert L.mc_gated_bwd(desc(**gated), 1, 1, 1, 1, 1, None, 1, 1, 1, 1, 1, 1, 1 << 30, None) == -1
+    b16 = dict(dtype=_lib.MC_BF16, layout=_lib.MC_NHWC)                               # unaligned bf16 tensors
+    assert L.mc_pointwise_fwd(desc(**b16), 24, 16, None, None, 16, None, 256, 1 << 30, None) == -1
+    assert L.mc_gated_fwd(desc(**b16, **gated), 16, 16, 2, 24, 2, None, 16, None, 256, 1 << 30, None) == -1
     one = (ctypes.c_void_p * 1)(256)
     n, t, bad = (ctypes.c_int64 * 1)(5), (ctypes.c_int32 * 1)(0), (ctypes.c_int32 * 1)(7)
     assert L.mc_grad_norm(-1, one, n, t, 2.0, 1, None, 1, 1 << 20, None) == -1
