@@ -395,7 +395,7 @@ int mc_voting_resample(const int64_t* labels, const int64_t* map, int32_t B, int
  * b_out (C_out).  residual and biases may be NULL.  Sums are float32 (double for MC_F64); for MC_BF16 what stands
  * between two products (h, and the gradients of the pre-activations) is rounded to bf16, which the next product's
  * operand is, and the pre-activations themselves are float32: the backward calls compute them again.  MC_BF16 tensors
- * must be 16-byte aligned (biases need not be).  Limits: B * S < 2^31, channels <= 2^20. */
+ * must be 16-byte aligned (biases need not be).  Limits: B * S <= 2^31 - 256, channels <= 2^20. */
 enum {
   MC_ACT_NONE = 0,
   MC_ACT_RELU = 1,

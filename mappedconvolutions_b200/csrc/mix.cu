@@ -16,7 +16,7 @@ static int check_desc(const mc_mix_desc* d, bool gated) {
   if (d->layout != MC_NCHW && d->layout != MC_NHWC) return MC_ERR_BAD_ARG;
   if (d->act < MC_ACT_NONE || d->act > MC_ACT_SIGMOID) return MC_ERR_BAD_ARG;
   // pixel indices are 32-bit (element offsets are not); channel tiles are a grid's second dimension
-  if (d->S >= (1ll << 31) || d->B >= (1ll << 31) || d->B * d->S >= (1ll << 31)) return MC_ERR_TOO_LARGE;
+  if (d->S >= (1ll << 31) || d->B >= (1ll << 31) || d->B * d->S > (1ll << 31) - 256) return MC_ERR_TOO_LARGE;
   if (d->C_in > (1 << 20) || d->C_out > (1 << 20) || d->hidden > (1 << 19)) return MC_ERR_TOO_LARGE;
   return MC_OK;
 }
@@ -176,6 +176,12 @@ struct Work {
     }
     return r;
   }
+  // n matrices (R, C) on top of each other -> their transposes (C, R); the first one is returned, the others follow
+  TcRows weight_t(const void* p, int R, int C, int n = 1) {
+    const TcRows r = fresh((long long)n * C, R);
+    if (run()) did(mc_transpose(2, n, R, C, p, (void*)r.p, r.ld, st));
+    return TcRows{r.p, C, R, r.ld};
+  }
   // where an activation is computed as rows, and its way to where it belongs
   TcRows out(const mc_mix_desc* d, void* p, int C) {
     return in_place(d, C) ? TcRows{p, pixels(d), C, C} : fresh(pixels(d), C);
@@ -217,15 +223,16 @@ static void tc_pointwise_fwd(Work& k, const mc_mix_desc* d, const void* x, const
 
 static void tc_pointwise_bwd(Work& k, const mc_mix_desc* d, const void* gy, const void* x, const void* w,
                              const void* bias, void* gx, void* gw, void* gb) {
-  const TcRows xr = k.in(d, x, d->C_in), wr = k.weight(w, d->C_out, d->C_in), gyr = k.in(d, gy, d->C_out);
+  const TcRows xr = k.in(d, x, d->C_in), gyr = k.in(d, gy, d->C_out);
   TcRows gz = gyr;
   if (d->act != MC_ACT_NONE) {
+    const TcRows wr = k.weight(w, d->C_out, d->C_in);
     gz = k.fresh(pixels(d), d->C_out);
     if (k.run()) k.did(tc_layer(xr, wr, (const bf16*)bias, d->act, gyr, gz, true, k.st));
   }
   if (gx || !k.base) {
-    const TcRows gxr = k.out(d, gx, d->C_in);
-    if (k.run()) k.did(tc_input_grad(gz, wr, TcRows{}, TcRows{}, gxr, k.st));
+    const TcRows wt = k.weight_t(w, d->C_out, d->C_in), gxr = k.out(d, gx, d->C_in);
+    if (k.run()) k.did(tc_input_grad(gz, wt, TcRows{}, TcRows{}, gxr, k.st));
     k.put(d, gxr, gx, d->C_in);
   }
   k.param_grads(gz, TcRows{}, 1, xr, gw, gb);
@@ -246,12 +253,13 @@ static void tc_gated_bwd(Work& k, const mc_mix_desc* d, const void* gy, const vo
                          const void* w_out, const void* saved, void* gx, void* gw_in, void* gb_in, void* gw_out,
                          void* gb_out) {
   const int H = d->hidden;
-  const TcRows xr = k.in(d, x, d->C_in), wi = k.weight(w_in, 2 * H, d->C_in), wo = k.weight(w_out, d->C_out, H);
+  const TcRows xr = k.in(d, x, d->C_in), wi = k.weight(w_in, 2 * H, d->C_in), wot = k.weight_t(w_out, d->C_out, H);
   const TcRows gyr = k.in(d, gy, d->C_out), gg = k.fresh(pixels(d), H), gu = k.fresh(pixels(d), H);
-  if (k.run() && (gx || gw_in || gb_in)) k.did(tc_gate_bwd(xr, wi, (const bf16*)b_in, d->act, gyr, wo, gg, gu, k.st));
+  if (k.run() && (gx || gw_in || gb_in)) k.did(tc_gate_bwd(xr, wi, (const bf16*)b_in, d->act, gyr, wot, gg, gu, k.st));
   if (gx || !k.base) {
-    const TcRows gxr = k.out(d, gx, d->C_in);
-    const TcRows wg{wi.p, H, wi.cols, wi.ld}, wu{(const char*)wi.p + (size_t)H * wi.ld * 2, H, wi.cols, wi.ld};
+    const TcRows gxr = k.out(d, gx, d->C_in), wg = k.weight_t(w_in, H, d->C_in, 2);
+    TcRows wu = wg;
+    wu.p = (const char*)wg.p + (size_t)d->C_in * wg.ld * 2;
     if (k.run()) k.did(tc_input_grad(gg, wg, gu, wu, gxr, k.st));
     k.put(d, gxr, gx, d->C_in);
   }

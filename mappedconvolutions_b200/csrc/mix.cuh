@@ -124,13 +124,13 @@ struct TcRows {
 // y = act(a w^T + bias) + r, or with backward y = r act'(a w^T + bias); w (N, K), r.p may be null (not with backward)
 int tc_layer(const TcRows& a, const TcRows& w, const bf16* bias, int act, const TcRows& r, const TcRows& y, bool backward,
              cudaStream_t st);
-// gx = g0 w0 + g1 w1, w (K, N); g1.p may be null
+// gx = g0 w0^T + g1 w1^T, w (N, K); g1.p may be null
 int tc_input_grad(const TcRows& g0, const TcRows& w0, const TcRows& g1, const TcRows& w1, const TcRows& gx,
                   cudaStream_t st);
 // h = act(g) u, [g|u] = x w_in^T + b_in
 int tc_gate(const TcRows& x, const TcRows& w_in, const bf16* b_in, int act, const TcRows& h, cudaStream_t st);
-// gg = gh u act'(g), gu = gh act(g), gh = gy w_out
-int tc_gate_bwd(const TcRows& x, const TcRows& w_in, const bf16* b_in, int act, const TcRows& gy, const TcRows& w_out,
+// gg = gh u act'(g), gu = gh act(g), gh = gy w_out, w_out_t = w_out^T (H, C_out)
+int tc_gate_bwd(const TcRows& x, const TcRows& w_in, const bf16* b_in, int act, const TcRows& gy, const TcRows& w_out_t,
                 const TcRows& gg, const TcRows& gu, cudaStream_t st);
 // part[s] = the s-th share of [g0|g1]^T x (rows of *ldn floats), csum[s] = its column sums of [g0|g1]; g1.p may be null
 size_t tc_outer_floats(long long P, int M, int segs, int N, int* splits, int* ldn);

@@ -1,6 +1,11 @@
 // Channel mixing on the tensor cores (bf16 operands, float32 sums in TMEM).
 //
-// rows kernel:  tiles of 128 pixels x BN channels.  One warp fetches operand tiles by TMA, one thread issues the MMAs into
+// Two blocks of a cluster work on one MMA (cta_group::2): each holds its own 128 pixels and half of the weights' rows,
+// the leader issues.  What bounds a block alone is its shared memory: TMA writes and operand reads share 128 bytes a
+// cycle, and a 128 x 256 tile asks for 96 + 96 of them at the tensor core's pace.  Halving the weights' part takes that
+// to 64 + 64.
+//
+// rows kernel:  tiles of 2 x 128 pixels x BN channels.  One warp fetches operand tiles by TMA, one thread issues the MMAs into
 // two accumulator sets in turn.  Each set has four read-out warps of its own (a tile's latencies - TMEM loads, elementary
 // functions, hand-over of the staged tiles - overlap with the other set's), which apply the epilogue and leave bf16 tiles
 // in shared memory, from where an I/O thread stores them by TMA; the same slots receive the tiles that an epilogue adds
@@ -24,7 +29,6 @@ constexpr int KB = 64;          // channels per pipeline stage: one 128-byte swi
 constexpr int A_BYTES = TILE * KB * 2;
 constexpr int THREADS = 384;    // loader, MMA, two I/O warps, eight read-out warps
 constexpr int MAX_STAGES = 12;
-constexpr int CH_BYTES = TILE * 64 * 2;  // a staged tile
 constexpr int SMEM_LIMIT = 226 * 1024;  // of 227 KB, the rest is static
 
 // ---- activations: fast forms, relative error below 2^-16 (half a bf16 step is 2^-9), two values at a time -----------------
@@ -58,69 +62,108 @@ __device__ __forceinline__ float exp2_(float v) {
 }
 __device__ __forceinline__ float2 rcp2(float2 v) { return make_float2(rcp_(v.x), rcp_(v.y)); }
 __device__ __forceinline__ float2 exp2_2(float2 v) { return make_float2(exp2_(v.x), exp2_(v.y)); }
-// 1 / (1 + 2^v): the logistic function of z for v = -z log2(e)
-__device__ __forceinline__ float2 logistic2(float2 v) { return rcp2(add2(exp2_2(v), two(1.f))); }
 constexpr float LOG2E = 1.44269504f;
+// The functions below take NV pairs at a time, one step for all of them after the other: elementary functions answer
+// after tens of cycles, and with two read-out warps per scheduler nobody else fills the time.
+constexpr int NV = 8;
+typedef float2 Pairs[NV];
+#define MC_EACH _Pragma("unroll") for (int j = 0; j < NV; ++j)
+// v <- 1 / (1 + 2^v): the logistic function of z for v = -z log2(e)
+__device__ __forceinline__ void logistic(Pairs& v) {
+  MC_EACH v[j] = exp2_2(v[j]);
+  MC_EACH v[j] = add2(v[j], two(1.f));
+  MC_EACH v[j] = rcp2(v[j]);
+}
+// value: z <- act(z).  both: z <- act(z), s = act'(z)
 struct ActNone {
-  __device__ static float2 value(float2 z) { return z; }
-  __device__ static void both(float2 z, float2& v, float2& s) { v = z, s = two(1.f); }
+  __device__ static void value(Pairs&) {}
+  __device__ static void both(Pairs&, Pairs& s) { MC_EACH s[j] = two(1.f); }
 };
 struct ActRelu {
   __device__ static float value1(float z) { return z < 0.f ? 0.f : z; }  // (NaN stays NaN)
   __device__ static float slope1(float z) { return z > 0.f ? 1.f : (z == z ? 0.f : z); }
-  __device__ static float2 value(float2 z) { return make_float2(value1(z.x), value1(z.y)); }
-  __device__ static void both(float2 z, float2& v, float2& s) {
-    v = value(z), s = make_float2(slope1(z.x), slope1(z.y));
+  __device__ static void value(Pairs& z) { MC_EACH z[j] = make_float2(value1(z[j].x), value1(z[j].y)); }
+  __device__ static void both(Pairs& z, Pairs& s) {
+    MC_EACH s[j] = make_float2(slope1(z[j].x), slope1(z[j].y));
+    value(z);
   }
 };
 struct ActGelu {
-  // Phi(z), and e = exp(-z^2 / 2).  With x = |z| / sqrt(2), t = 1 / (1 + 0.44 x): exp(x^2) erfc(x) / 2 = t q(t), q a
+  // p = Phi(z), e = exp(-z^2 / 2).  With x = |z| / sqrt(2), t = 1 / (1 + 0.44 x): exp(x^2) erfc(x) / 2 = t q(t), q a
   // least-squares fit of the relative error over x in [0, 10] (at most 5.2e-6; e alone decays beyond).
-  __device__ static float2 phi(float2 z, float2& e) {
-    const float2 t = rcp2(fma2(two(0.31112698f), make_float2(fabsf(z.x), fabsf(z.y)), two(1.f)));
-    e = exp2_2(mul2(mul2(z, two(-0.5f * LOG2E)), z));
-    float2 q = fma2(two(-0.07305045425891876f), t, two(0.1753196418285370f));
-    q = fma2(q, t, two(0.020372465252876282f));
-    q = fma2(q, t, two(0.1317897737026215f));
-    q = fma2(q, t, two(0.12128554284572601f));
-    q = fma2(q, t, two(0.12428044527769089f));
-    const float2 c = mul2(mul2(q, t), e), d = fma2(c, two(-1.f), two(1.f));
-    return make_float2(z.x < 0.f ? c.x : d.x, z.y < 0.f ? c.y : d.y);
+  __device__ static void phi(const Pairs& z, Pairs& p, Pairs& e) {
+    Pairs t;
+    MC_EACH t[j] = fma2(two(0.31112698f), make_float2(fabsf(z[j].x), fabsf(z[j].y)), two(1.f));
+    MC_EACH e[j] = mul2(mul2(z[j], two(-0.5f * LOG2E)), z[j]);
+    MC_EACH t[j] = rcp2(t[j]);
+    MC_EACH e[j] = exp2_2(e[j]);
+    MC_EACH p[j] = fma2(two(-0.07305045425891876f), t[j], two(0.1753196418285370f));
+    MC_EACH p[j] = fma2(p[j], t[j], two(0.020372465252876282f));
+    MC_EACH p[j] = fma2(p[j], t[j], two(0.1317897737026215f));
+    MC_EACH p[j] = fma2(p[j], t[j], two(0.12128554284572601f));
+    MC_EACH p[j] = fma2(p[j], t[j], two(0.12428044527769089f));
+    MC_EACH p[j] = mul2(mul2(p[j], t[j]), e[j]);
+    MC_EACH {
+      const float2 d = fma2(p[j], two(-1.f), two(1.f));
+      p[j] = make_float2(z[j].x < 0.f ? p[j].x : d.x, z[j].y < 0.f ? p[j].y : d.y);
+    }
   }
-  __device__ static float2 value(float2 z) {
-    float2 e;
-    return mul2(z, phi(z, e));
+  __device__ static void value(Pairs& z) {
+    Pairs p, e;
+    phi(z, p, e);
+    MC_EACH z[j] = mul2(z[j], p[j]);
   }
-  __device__ static void both(float2 z, float2& v, float2& s) {
-    float2 e;
-    const float2 p = phi(z, e);
-    v = mul2(z, p);
-    s = fma2(mul2(z, two(0.39894228f)), e, p);
+  __device__ static void both(Pairs& z, Pairs& s) {
+    Pairs p, e;
+    phi(z, p, e);
+    MC_EACH s[j] = fma2(mul2(z[j], two(0.39894228f)), e[j], p[j]);
+    MC_EACH z[j] = mul2(z[j], p[j]);
   }
 };
 struct ActGeluTanh {  // (1 + tanh(a)) / 2 is the logistic function of 2 a
-  __device__ static float2 part(float2 z) {
-    return logistic2(mul2(mul2(z, two(-1.59576912f * LOG2E)), fma2(mul2(z, two(0.044715f)), z, two(1.f))));
+  __device__ static void part(const Pairs& z, Pairs& p) {
+    MC_EACH p[j] = mul2(mul2(z[j], two(-1.59576912f * LOG2E)), fma2(mul2(z[j], two(0.044715f)), z[j], two(1.f)));
+    logistic(p);
   }
-  __device__ static float2 value(float2 z) { return mul2(z, part(z)); }
-  __device__ static void both(float2 z, float2& v, float2& s) {
-    const float2 p = part(z);
-    v = mul2(z, p);
-    s = fma2(mul2(v, fma2(p, two(-1.f), two(1.f))), fma2(mul2(z, two(1.59576912f * 0.134145f)), z, two(1.59576912f)), p);
+  __device__ static void value(Pairs& z) {
+    Pairs p;
+    part(z, p);
+    MC_EACH z[j] = mul2(z[j], p[j]);
+  }
+  __device__ static void both(Pairs& z, Pairs& s) {
+    Pairs p;
+    part(z, p);
+    MC_EACH {
+      const float2 v = mul2(z[j], p[j]);
+      s[j] = fma2(mul2(v, fma2(p[j], two(-1.f), two(1.f))),
+                  fma2(mul2(z[j], two(1.59576912f * 0.134145f)), z[j], two(1.59576912f)), p[j]);
+      z[j] = v;
+    }
   }
 };
 struct ActSilu {
-  __device__ static float2 value(float2 z) { return mul2(z, logistic2(mul2(z, two(-LOG2E)))); }
-  __device__ static void both(float2 z, float2& v, float2& s) {
-    const float2 p = logistic2(mul2(z, two(-LOG2E)));
-    v = mul2(z, p);
-    s = fma2(v, fma2(p, two(-1.f), two(1.f)), p);
+  __device__ static void value(Pairs& z) {
+    Pairs p;
+    MC_EACH p[j] = mul2(z[j], two(-LOG2E));
+    logistic(p);
+    MC_EACH z[j] = mul2(z[j], p[j]);
+  }
+  __device__ static void both(Pairs& z, Pairs& s) {
+    Pairs p;
+    MC_EACH p[j] = mul2(z[j], two(-LOG2E));
+    logistic(p);
+    MC_EACH z[j] = mul2(z[j], p[j]);
+    MC_EACH s[j] = fma2(z[j], fma2(p[j], two(-1.f), two(1.f)), p[j]);
   }
 };
 struct ActSigmoid {
-  __device__ static float2 value(float2 z) { return logistic2(mul2(z, two(-LOG2E))); }
-  __device__ static void both(float2 z, float2& v, float2& s) {
-    v = value(z), s = mul2(v, fma2(v, two(-1.f), two(1.f)));
+  __device__ static void value(Pairs& z) {
+    MC_EACH z[j] = mul2(z[j], two(-LOG2E));
+    logistic(z);
+  }
+  __device__ static void both(Pairs& z, Pairs& s) {
+    value(z);
+    MC_EACH s[j] = mul2(z[j], fma2(z[j], two(-1.f), two(1.f)));
   }
 };
 template <typename F>
@@ -135,17 +178,94 @@ __device__ __forceinline__ void with_act(int act, F f) {  // one branch per 32 c
   }
 }
 
+// 32 lanes x 16 columns of accumulators
+__device__ __forceinline__ void tmem_ld_32x16(uint32_t taddr, uint32_t (&v)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
+        "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+      : "r"(taddr)
+      : "memory");
+}
 template <int N>
 __device__ __forceinline__ float2 pair_of(const uint32_t (&v)[N], int j) {
   return make_float2(__uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1]));
 }
 __device__ __forceinline__ float2 bias2(const float* b, int j) { return reinterpret_cast<const float2*>(b)[j]; }
 
+// Has the phase completed?  Never suspends the thread, so that the answer for the next stage can be on its way while this
+// stage's MMAs are issued.
+__device__ __forceinline__ bool mbar_test(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+
+// ---- pairs of blocks -----------------------------------------------------------------------------------
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+}
+// the address that a barrier of the leader has from both blocks
+__device__ __forceinline__ uint32_t of_leader(uint32_t a) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(a));
+  return r;
+}
+__device__ __forceinline__ void arrive_leader(uint32_t bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void pair_alloc(uint32_t result_smem, uint32_t ncols) {
+  asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(result_smem), "r"(ncols) : "memory");
+  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void pair_dealloc(uint32_t taddr, uint32_t ncols) {
+  asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(ncols) : "memory");
+}
+// D (256 rows, 128 in each block's TMEM) (+)= A (128 rows in each block) B (half of the columns in each block)
+__device__ __forceinline__ void pair_mma(uint32_t d, uint32_t alo, uint32_t ahi, uint32_t blo, uint32_t bhi, uint32_t idesc,
+                                         uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\t"
+      "setp.ne.b32 p, %6, 0;\n\t"
+      "mov.b64 da, {%1, %2};\n\t"
+      "mov.b64 db, {%3, %4};\n\t"
+      "tcgen05.mma.cta_group::2.kind::f16 [%0], da, db, %5, p;\n\t}"
+      :
+      : "r"(d), "r"(alo), "r"(ahi), "r"(blo), "r"(bhi), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// one arrival at this barrier of both blocks when all MMAs issued so far have finished
+__device__ __forceinline__ void pair_commit(uint32_t bar) {
+  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
+               "h"((uint16_t)3)
+               : "memory");
+}
+
 // ---- TMA ---------------------------------------------------------------------------------------------
 __device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* tm, int x, int y, uint32_t bar) {
   asm volatile(
       "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
       "l"((uint64_t)tm), "r"(x), "r"(y), "r"(bar)
+      : "memory");
+}
+// into this block's shared memory, counted by a barrier of the leader
+__device__ __forceinline__ void tma_load_pair(uint32_t dst, const CUtensorMap* tm, int x, int y, uint32_t leader_bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::
+          "r"(dst),
+      "l"((uint64_t)tm), "r"(x), "r"(y), "r"(leader_bar)
       : "memory");
 }
 __device__ __forceinline__ void tma_store(const CUtensorMap* tm, int x, int y, uint32_t src) {
@@ -174,62 +294,186 @@ enum Mode {
   GATE_BWD = 2,  // [g|u] as above from the first operands, gh from the second: y0 = gh u act'(g), y1 = gh act(g)
   ACT_BWD = 3    // y = r act'(A B^T + bias)
 };
-// BN: channels of a tile; it is staged 64 channels (128 swizzled bytes a row) at a time.
+// BN: channels of a tile.  It is staged CW channels (128 or 64 swizzled bytes a row) at a time; the two results of
+// GATE_BWD side by side, in smaller tiles because its weights leave little room.
 template <int MODE, int BN> struct Cfg {
   static constexpr int N0 = MODE == GATE || MODE == GATE_BWD ? 2 * BN : BN;  // columns of the first product
   static constexpr int N1 = MODE == GATE_BWD ? BN : N0;                      // and of the second
   static constexpr int OFF1 = MODE == GATE_BWD ? N0 : 0;                     // its first accumulator column
-  static constexpr int NCH = MODE == GATE_BWD ? 2 : BN / 64;                 // staged tiles
-  static constexpr int BMAX = (N0 > N1 ? N0 : N1) * KB * 2;
+  static constexpr int CW = MODE == GATE_BWD ? 32 : 64;
+  static constexpr int NCH = (MODE == GATE_BWD ? 2 : 1) * BN / CW;           // staged tiles
+  static constexpr int CH_BYTES = TILE * CW * 2;
+  static constexpr int B0 = N0 / 2 * KB * 2, B1 = N1 / 2 * KB * 2;           // a block's weights per stage
+  static constexpr int BMAX = B0 > B1 ? B0 : B1;
 };
 
 struct alignas(64) GemmArgs {
   CUtensorMap a[2], b[2], r, y[2];
   const bf16* bias;  // null: none
-  int m_tiles, n_tiles, N, kb[2], act;
+  int m_pairs, rows; // pairs of tiles; pixels
+  int n_tiles, N, kb[2], act;
   int up;            // distance between a gate's row of b[0] and bias and its factor's
   int res;           // r is read
-  int resident, stages, slots;
+  int group;         // channel tiles of a pair of blocks whose weights stay in shared memory, 0: none do
+  int stages, slots;
 };
 
 constexpr int ROWS_BARS = 2 * MAX_STAGES + 1 + 4 + 8 + 1 + 2;
 
-struct TileWalk {  // this block's tiles
-  long long t, step, end;
-  int n_tiles, n;
-  bool fixed;
-  // from the `first`-th tile on, every `every`-th one
-  __device__ TileWalk(const GemmArgs& a, int first = 0, int every = 1) : n_tiles(a.n_tiles), fixed(a.resident) {
-    if (fixed) {
-      n = blockIdx.x % n_tiles;
-      t = blockIdx.x / n_tiles, step = gridDim.x / n_tiles, end = a.m_tiles;
+// The tiles of a pair of blocks, from the `first`-th on, every `every`-th one.  With resident weights a pair keeps its
+// group of channel tiles and takes every so many pixel tiles; otherwise the channel tiles of a pixel tile are next to
+// each other among the pairs.  Either way what is read of the pixels at one time is shared through L2.
+struct TileWalk {
+  uint32_t t, step, end, per, base;  // t = pixel tile * per + channel tile - base
+  __device__ TileWalk(const GemmArgs& a, int first = 0, int every = 1) {
+    const uint32_t pair = blockIdx.x / 2, pairs = gridDim.x / 2;
+    if (a.group) {
+      const uint32_t groups = a.n_tiles / a.group;
+      base = pair % groups * a.group;
+      per = a.group;
+      m0 = pair / groups, mstep = pairs / groups;
+      end = ((uint32_t)a.m_pairs - m0 + mstep - 1) / mstep * per;
+      t = 0, step = 1;
     } else {
-      t = blockIdx.x, step = gridDim.x, end = (long long)a.m_tiles * n_tiles;
+      base = 0, per = a.n_tiles, m0 = 0, mstep = 1;
+      t = pair, step = pairs, end = (uint32_t)a.m_pairs * per;
     }
     t += step * first;
     step *= every;
   }
+  uint32_t m0, mstep;
   __device__ bool more() const { return t < end; }
   __device__ void next() { t += step; }
-  __device__ int m() const { return (int)(fixed ? t : t / n_tiles); }
-  __device__ int nt() const { return fixed ? n : (int)(t % n_tiles); }
+  __device__ uint32_t local_n() const { return t % per; }
+  __device__ int nt() const { return (int)(base + t % per); }
+  __device__ int m() const { return (int)(m0 + t / per * mstep); }  // pair of pixel tiles
 };
 
-template <int MODE, int BN, bool BMN>
-__device__ __forceinline__ void load_b(const GemmArgs& g, int seg, uint32_t dst, int k, int n0, uint32_t bar) {
+// this block's half of the weights of one stage; boxes are half a product's columns (or one of gate and factor) high
+template <int MODE, int BN>
+__device__ __forceinline__ void load_b(const GemmArgs& g, int seg, uint32_t rank, uint32_t dst, int k, int n0, uint32_t bar) {
   typedef Cfg<MODE, BN> C;
-  if (MODE == GATE || (MODE == GATE_BWD && seg == 0)) {
-    tma_load(dst, &g.b[0], k, n0, bar);
-    tma_load(dst + BN * 128, &g.b[0], k, g.up + n0, bar);
-  } else if (BMN || MODE == GATE_BWD) {  // 64 channels x 64 rows along k per box
+  int row = n0;
+  if (MODE == GATE || (MODE == GATE_BWD && seg == 0)) row += rank ? g.up : 0;
+  else row += rank * (C::N1 / 2);
+  tma_load_pair(dst, &g.b[seg], k, row, bar);
+}
+
+// Offsets of the barriers behind bfull.
+constexpr uint32_t BAR_TFULL = 8, BAR_TEMPTY = 24, BAR_READY = 40, BAR_DONE = 72, BAR_DRAIN = 104, BAR_BIASED = 112;
+
+// Read-out warps of one accumulator set: thread = pixel.  Sixteen channels at a time in a loop that is not unrolled: the
+// code of a whole tile does not stay in the instruction cache, and then fetching it takes longer than running it.
+template <int MODE, int BN, typename Act>
+__device__ __forceinline__ void read_out(const GemmArgs& g, int set, uint32_t rank, float* bias_s, uint32_t out0,
+                                         uint32_t bfull, volatile int* abort_flag) {
+  typedef Cfg<MODE, BN> C;
+  constexpr int NP = BN / 16, PER = C::CW / 16;  // pieces of a tile, and of a staged tile
+  const int lane = threadIdx.x % 32, q = threadIdx.x / 32 & 3, row = q * 32 + lane;
+  const uint32_t buf = out0 + set * g.slots * C::CH_BYTES;
+  const uint32_t t0 = ((uint32_t)(q * 32) << 16) + set * 256;
+  const uint32_t tfull = bfull + BAR_TFULL + 8 * set, tempty = of_leader(bfull + BAR_TEMPTY + 8 * set);
+  // 16-byte piece j of this row of a staged tile
+  const uint32_t at0 = buf + row * C::CW * 2, swizzle = (C::CW == 64 ? row & 7 : (row >> 1) & 3) << 4;
+  const auto slot = [&](uint32_t i) { return at0 + (g.slots == 2 ? i & 1 : 0) * C::CH_BYTES; };
+  const auto bar_of = [&](uint32_t base, uint32_t i) { return bfull + base + 16 * set + 8 * (g.slots == 2 ? i & 1 : 0); };
+  const auto slot_ready = [&](uint32_t i) {
+    return warp_wait(bar_of(BAR_READY, i), (g.slots == 2 ? i >> 1 : i) & 1, abort_flag, 0x132);
+  };
+  const auto slot_done = [&](uint32_t i) {
+    fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(bar_of(BAR_DONE, i));
+  };
+  uint32_t it = 0, i = 0;
+  for (TileWalk w(g, set, 2); w.more(); w.next(), ++it) {
+    float* bs = bias_s + set * 512 + (g.group == 1 ? 0 : (it & 1) * 256);
+    if (it == 0 || g.group != 1) {
+      // (the other half is still being read by warps that are a tile behind; nobody is two behind)
+      const int n0 = w.nt() * BN;
+      for (int e = row; e < C::N0; e += 128) {
+        const int n = n0 + e % BN + (e >= BN ? g.up : 0);
+        bs[e] = g.bias && n0 + e % BN < g.N
+                    ? __bfloat162float(__ushort_as_bfloat16(__ldg((const unsigned short*)g.bias + n)))
+                    : 0.f;
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bfull + BAR_BIASED + 8 * set);
+      if (!warp_wait(bfull + BAR_BIASED + 8 * set, it & 1, abort_flag, 0x133)) return;  // (bounded, unlike bar.sync)
+    }
+    if (!warp_wait(tfull, it & 1, abort_flag, 0x131)) return;
+    tc_fence_after_sync();
+    constexpr int NL = MODE == GATE_BWD ? 3 : MODE == GATE ? 2 : 1;
+    uint32_t v[2][NL][16];
+    const auto fetch = [&](uint32_t (&d)[NL][16], int p) {
+      tmem_ld_32x16(t0 + 16 * p, d[0]);
+      if (NL > 1) tmem_ld_32x16(t0 + BN + 16 * p, d[NL > 1 ? 1 : 0]);
+      if (NL > 2) tmem_ld_32x16(t0 + C::OFF1 + 16 * p, d[NL > 2 ? 2 : 0]);
+    };
+    // one piece from `cur`, while the next one is on its way to `other`
+    const auto step = [&](uint32_t (&cur)[NL][16], uint32_t (&other)[NL][16], int p) -> bool {
+      tmem_ld_wait();
+      if (p + 1 < NP) {
+        fetch(other, p + 1);
+      } else {  // the accumulators are free
+        tc_fence_before_sync();
+        __syncwarp();
+        if (lane == 0) arrive_leader(tempty);
+      }
+      const float* b = bs + 16 * p;
+      Pairs z, o;
+      MC_EACH z[j] = add2(pair_of(cur[0], j), bias2(b, j));
+      if (MODE == ACT_BWD || MODE == GATE_BWD) Act::both(z, o);
+      else Act::value(z);
+      uint32_t r0[8], r1[8];
+      if (MODE == GATE) MC_EACH z[j] = mul2(z[j], add2(pair_of(cur[NL > 1 ? 1 : 0], j), bias2(b + BN, j)));
+      if (MODE == GATE_BWD) MC_EACH {
+        const float2 gh = pair_of(cur[NL > 2 ? 2 : 0], j), u = add2(pair_of(cur[NL > 1 ? 1 : 0], j), bias2(b + BN, j));
+        o[j] = mul2(mul2(gh, u), o[j]);
+        z[j] = mul2(gh, z[j]);
+        r1[j] = pack_bf16x2(z[j].x, z[j].y);
+      }
+      const uint32_t j0 = p % PER * 2;
+      if (p % PER == 0) {
+        if (!slot_ready(i)) return false;
+        if (MODE == GATE_BWD && !slot_ready(i + 1)) return false;
+      }
+      const uint32_t at[2] = {slot(i) + ((j0 << 4) ^ swizzle), slot(i) + (((j0 + 1) << 4) ^ swizzle)};
+      if (MODE == ACT_BWD || (MODE == LAYER && g.res)) {
 #pragma unroll
-    for (int i = 0; i < C::N1 / 64; ++i) tma_load(dst + i * 8192, &g.b[seg], n0 + 64 * i, k, bar);
-  } else {
-    tma_load(dst, &g.b[seg], k, n0, bar);
+        for (int h = 0; h < 2; ++h) {
+          const uint4 r = lds16(at[h]);
+          const uint32_t rw[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float2 f = make_float2(__uint_as_float(rw[e] << 16), __uint_as_float(rw[e] & 0xFFFF0000u));
+            if (MODE == ACT_BWD) o[4 * h + e] = mul2(o[4 * h + e], f);
+            else z[4 * h + e] = add2(z[4 * h + e], f);
+          }
+        }
+      }
+      if (MODE == ACT_BWD || MODE == GATE_BWD) MC_EACH r0[j] = pack_bf16x2(o[j].x, o[j].y);
+      else MC_EACH r0[j] = pack_bf16x2(z[j].x, z[j].y);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        sts16(at[h], make_uint4(r0[4 * h], r0[4 * h + 1], r0[4 * h + 2], r0[4 * h + 3]));
+        if (MODE == GATE_BWD)
+          sts16(at[h] - slot(i) + slot(i + 1), make_uint4(r1[4 * h], r1[4 * h + 1], r1[4 * h + 2], r1[4 * h + 3]));
+      }
+      if (p % PER == PER - 1) {
+        slot_done(i++);
+        if (MODE == GATE_BWD) slot_done(i++);
+      }
+      return true;
+    };
+    fetch(v[0], 0);
+#pragma unroll 1
+    for (int p = 0; p < NP; p += 2)
+      if (!step(v[0], v[1], p) || !step(v[1], v[0], p + 1)) return;
   }
 }
 
-template <int MODE, int BN, bool BMN>
+template <int MODE, int BN>
 __global__ void __launch_bounds__(THREADS, 1) rows_tc_kernel(const __grid_constant__ GemmArgs g) {
   typedef Cfg<MODE, BN> C;
   extern __shared__ unsigned char raw[];
@@ -238,21 +482,23 @@ __global__ void __launch_bounds__(THREADS, 1) rows_tc_kernel(const __grid_consta
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   volatile int* abort_flag = &abort_flag_s;
   const uint32_t out0 = smem_u32(sm);
-  const uint32_t a0 = out0 + 2 * g.slots * CH_BYTES;
+  const uint32_t a0 = out0 + 2 * g.slots * C::CH_BYTES;
   const uint32_t b0 = a0 + g.stages * A_BYTES;
-  const int bbytes = g.resident ? g.kb[0] * C::N0 * 128 + g.kb[1] * C::N1 * 128 : g.stages * C::BMAX;
+  const uint32_t btile = g.kb[0] * C::B0 + g.kb[1] * C::B1;  // a channel tile's weights
+  const int bbytes = g.group ? g.group * btile : g.stages * C::BMAX;
+  const uint32_t rank = cluster_rank();
   float* bias_s = (float*)(sm + (b0 - out0) + bbytes);  // two tiles' worth per set
   const uint32_t bar0 = smem_u32(bias_s + 4 * 256);
   uint32_t* tmem_s = (uint32_t*)((unsigned char*)(bias_s + 4 * 256) + ROWS_BARS * 8);
   const auto full = [&](uint32_t s) { return bar0 + 8 * s; };
   const auto empty = [&](uint32_t s) { return bar0 + 8 * (MAX_STAGES + s); };
   const uint32_t bfull = bar0 + 8 * (2 * MAX_STAGES);
-  const auto tfull = [&](uint32_t s) { return bfull + 8 + 8 * s; };
-  const auto tempty = [&](uint32_t s) { return bfull + 24 + 8 * s; };
-  const auto ready = [&](int set, uint32_t s) { return bfull + 40 + 8 * (2 * set + s); };
-  const auto done = [&](int set, uint32_t s) { return bfull + 72 + 8 * (2 * set + s); };
-  const uint32_t drain = bfull + 104;
-  const auto biased = [&](int set) { return bfull + 112 + 8 * set; };
+  const auto tfull = [&](uint32_t s) { return bfull + BAR_TFULL + 8 * s; };
+  const auto tempty = [&](uint32_t s) { return bfull + BAR_TEMPTY + 8 * s; };
+  const auto ready = [&](int set, uint32_t s) { return bfull + BAR_READY + 8 * (2 * set + s); };
+  const auto done = [&](int set, uint32_t s) { return bfull + BAR_DONE + 8 * (2 * set + s); };
+  const uint32_t drain = bfull + BAR_DRAIN;
+  const auto biased = [&](int set) { return bfull + BAR_BIASED + 8 * set; };
 
   if (threadIdx.x == 0) {
     abort_flag_s = 0;
@@ -261,100 +507,106 @@ __global__ void __launch_bounds__(THREADS, 1) rows_tc_kernel(const __grid_consta
     mbar_init(drain, 1);
     for (int i = 0; i < 2; ++i) {
       mbar_init(tfull(i), 1);
-      mbar_init(tempty(i), 4);
+      mbar_init(tempty(i), 8);  // (the leader's: four warps of each block)
       mbar_init(biased(i), 4);
       for (int s = 0; s < 2; ++s) mbar_init(ready(i, s), 1), mbar_init(done(i, s), 4);
     }
     fence_barrier_init();
     fence_proxy_async_smem();
   }
-  if (warp == 1) tmem_alloc(smem_u32(tmem_s), 512);
+  if (warp == 1) pair_alloc(smem_u32(tmem_s), 512);
   tc_fence_before_sync();
   __syncthreads();
+  cluster_sync();
   tc_fence_after_sync();
-  const uint32_t tmem = *tmem_s;
+  constexpr uint32_t tmem = 0;  // (all columns are allocated; a constant stays in uniform registers)
 
   if (warp == 0) {
     // ---- loader.  (Loader and MMA warp run converged, one elected lane issues: addresses and descriptors then live in
     // uniform registers.  In a branch of a single lane each of them is moved there for every instruction, and the
     // issuing thread, not the tensor core, sets the pace: 240 instead of 128 cycles per MMA of 256 columns.)
-    const bool leader = elect_one();
+    const bool elected = elect_one();
     TileWalk w(g);
-    if (g.resident && w.more() && leader) {
-      mbar_expect_tx(bfull, bbytes);
-      const int n0 = w.nt() * BN;
+    if (g.group && w.more() && elected) {
+      const uint32_t bar = of_leader(bfull);
+      if (rank == 0) mbar_expect_tx(bfull, 2 * bbytes);
       uint32_t dst = b0;
-      for (int seg = 0; seg < 2; ++seg)
-        for (int k = 0; k < g.kb[seg]; ++k) {
-          load_b<MODE, BN, BMN>(g, seg, dst, k * KB, n0, bfull);
-          dst += (seg ? C::N1 : C::N0) * 128;
-        }
+      for (int n = 0; n < g.group; ++n)
+        for (int seg = 0; seg < 2; ++seg)
+          for (int k = 0; k < g.kb[seg]; ++k) {
+            load_b<MODE, BN>(g, seg, rank, dst, k * KB, (w.base + n) * BN, bar);
+            dst += seg ? C::B1 : C::B0;
+          }
     }
     __syncwarp();
     uint32_t st = 0, ph = 0;
     bool ok = true;
     for (; w.more() && ok; w.next()) {
-      const int m0 = w.m() * TILE, n0 = w.nt() * BN;
+      const int m0 = (w.m() * 2 + rank) * TILE, n0 = w.nt() * BN;
       for (int seg = 0; seg < 2 && ok; ++seg)
         for (int k = 0; k < g.kb[seg]; ++k) {
-          ok = mbar_wait(empty(st), ph ^ 1, abort_flag, 0x101);
-          if (!__all_sync(~0u, ok)) {
-            ok = false;
-            break;
-          }
-          if (leader) {
-            mbar_expect_tx(full(st), A_BYTES + (g.resident ? 0 : (seg ? C::N1 : C::N0) * 128));
-            tma_load(a0 + st * A_BYTES, &g.a[seg], k * KB, m0, full(st));
-            if (!g.resident) load_b<MODE, BN, BMN>(g, seg, b0 + st * C::BMAX, k * KB, n0, full(st));
+          ok = __all_sync(~0u, mbar_wait(empty(st), ph ^ 1, abort_flag, 0x101));
+          if (!ok) break;
+          if (elected) {
+            const uint32_t bar = of_leader(full(st));
+            if (rank == 0) mbar_expect_tx(full(st), 2 * (A_BYTES + (g.group ? 0 : seg ? C::B1 : C::B0)));
+            tma_load_pair(a0 + st * A_BYTES, &g.a[seg], k * KB, m0, bar);
+            if (!g.group) load_b<MODE, BN>(g, seg, rank, b0 + st * C::BMAX, k * KB, n0, bar);
           }
           __syncwarp();
           if (++st == (uint32_t)g.stages) st = 0, ph ^= 1;
         }
     }
   } else if (warp == 1) {
-    // ---- MMA issuer
-    const bool leader = elect_one();
-    uint32_t st = 0, ph = 0, it = 0;
-    TileWalk w(g);
-    bool ok = true;
-    if (g.resident && w.more()) ok = __all_sync(~0u, mbar_wait(bfull, 0, abort_flag, 0x111));
-    for (; w.more() && ok; w.next(), ++it) {
-      const uint32_t acc = it & 1, aph = (it >> 1) & 1;
-      ok = __all_sync(~0u, mbar_wait(tempty(acc), aph ^ 1, abort_flag, 0x112));
-      if (!ok) break;
-      tc_fence_after_sync();
-      uint32_t bres = b0;
+    // ---- MMA issuer, in the leader only
+    if (rank == 0) {
+      const bool elected = elect_one();
+      uint32_t st = 0, ph = 0;
+      TileWalk w(g);
+      uint32_t n = w.local_n();
+      const uint32_t a_lo = desc_sw128_lo(a0, 16), b_lo = desc_sw128_lo(b0, 16);
+      bool ok = true, there = false;
+      if (g.group && w.more()) ok = __all_sync(~0u, mbar_wait(bfull, 0, abort_flag, 0x111));
+      for (uint32_t it = 0; w.more() && ok; w.next(), ++it) {
+        const uint32_t acc = it & 1, aph = (it >> 1) & 1;
+        ok = __all_sync(~0u, mbar_wait(tempty(acc), aph ^ 1, abort_flag, 0x112));
+        if (!ok) break;
+        tc_fence_after_sync();
+        uint32_t bres = b_lo + n * (btile >> 4);
+        if (++n == (uint32_t)g.group) n = 0;
 #pragma unroll
-      for (int seg = 0; seg < 2; ++seg) {
-        constexpr uint32_t HI = desc_sw128_hi(1024);
-        const bool mn = MODE == GATE_BWD ? seg == 1 : BMN;
-        const uint32_t idesc = make_idesc_bf16(TILE, seg ? C::N1 : C::N0, 0, mn ? 1 : 0);
-        const uint32_t d = tmem + acc * 256 + (seg ? C::OFF1 : 0);
-        const uint32_t bstep = mn ? 128 : 2;  // sixteen rows along k, or 32 bytes
-        for (int k = 0; k < g.kb[seg] && ok; ++k) {
-          ok = __all_sync(~0u, mbar_wait(full(st), ph, abort_flag, 0x113));
-          if (!ok) break;
-          const uint32_t ad = desc_sw128_lo(a0 + st * A_BYTES, 16);
-          const uint32_t bd = desc_sw128_lo(g.resident ? bres : b0 + st * C::BMAX, mn ? 8192 : 16);
-          if (leader) {
+        for (int seg = 0; seg < 2; ++seg) {
+          constexpr uint32_t HI = desc_sw128_hi(1024);
+          const uint32_t idesc = make_idesc_bf16(2 * TILE, seg ? C::N1 : C::N0, 0, 0);
+          const uint32_t d = acc * 256 + (seg ? C::OFF1 : 0);
+          for (int k = 0; k < g.kb[seg]; ++k) {
+            if (!there) {
+              ok = __all_sync(~0u, mbar_wait(full(st), ph, abort_flag, 0x113));
+              if (!ok) break;
+            }
+            const uint32_t cur = st, ad = a_lo + st * (A_BYTES >> 4), bd = g.group ? bres : b_lo + st * (C::BMAX >> 4);
+            if (++st == (uint32_t)g.stages) st = 0, ph ^= 1;
+            const bool next = mbar_test(full(st), ph);
+            if (elected) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-              mma_bf16_ss_lo(d, ad + 2 * j, HI, bd + bstep * j, HI, idesc, (k | j) != 0 || (seg && C::OFF1 == 0));
-            mma_commit(empty(st));
+              for (int j = 0; j < 4; ++j)  // sixteen channels, 32 bytes each
+                pair_mma(d, ad + 2 * j, HI, bd + 2 * j, HI, idesc, (k | j) != 0 || (seg && C::OFF1 == 0));
+              pair_commit(empty(cur));
+            }
+            bres += (seg ? C::B1 : C::B0) >> 4;
+            there = __all_sync(~0u, next);
           }
-          __syncwarp();
-          bres += (seg ? C::N1 : C::N0) * 128;
-          if (++st == (uint32_t)g.stages) st = 0, ph ^= 1;
+          if (!ok) break;
         }
+        if (ok && elected) pair_commit(tfull(acc));
+        __syncwarp();
       }
-      if (ok && leader) mma_commit(tfull(acc));
+      if (elected) {
+        pair_commit(drain);
+        mbar_wait(drain, 0, abort_flag, 0x114);
+      }
       __syncwarp();
     }
-    if (leader) {
-      mma_commit(drain);
-      mbar_wait(drain, 0, abort_flag, 0x114);
-    }
-    __syncwarp();
   } else if (warp < 4) {
     // ---- I/O of one set's staged tiles: fill the slots ahead (residual), store what the read-out warps leave in them
     if (lane == 0) {
@@ -362,15 +614,15 @@ __global__ void __launch_bounds__(THREADS, 1) rows_tc_kernel(const __grid_consta
       TileWalk lead(g, set, 2);
       int lead_c = 0;
       uint32_t lead_i = 0;
-      const uint32_t buf = out0 + set * g.slots * CH_BYTES;
-      const auto column = [&](const TileWalk& w, int c) { return w.nt() * BN + (MODE == GATE_BWD ? 0 : c * 64); };
+      const uint32_t buf = out0 + set * g.slots * C::CH_BYTES;
+      const auto column = [&](const TileWalk& w, int c) { return w.nt() * BN + (MODE == GATE_BWD ? c / 2 : c) * C::CW; };
       const auto advance = [&]() {
         if (!lead.more()) return;
         const uint32_t s = lead_i % g.slots;
         const int col = column(lead, lead_c);
-        if (g.res && col < g.N) {
-          mbar_expect_tx(ready(set, s), CH_BYTES);
-          tma_load(buf + s * CH_BYTES, &g.r, col, lead.m() * TILE, ready(set, s));
+        if (g.res && col < g.N && (lead.m() * 2 + rank) * TILE < g.rows) {
+          mbar_expect_tx(ready(set, s), C::CH_BYTES);
+          tma_load(buf + s * C::CH_BYTES, &g.r, col, (lead.m() * 2 + rank) * TILE, ready(set, s));
         } else {
           mbar_arrive(ready(set, s));
         }
@@ -385,9 +637,9 @@ __global__ void __launch_bounds__(THREADS, 1) rows_tc_kernel(const __grid_consta
           const uint32_t s = i % g.slots;
           ok = mbar_wait(done(set, s), (i / g.slots) & 1, abort_flag, 0x121);
           if (!ok) break;
-          const int col = column(w, c);
-          if (col < g.N) {
-            tma_store(&g.y[MODE == GATE_BWD ? c : 0], col, w.m() * TILE, buf + s * CH_BYTES);
+          const int col = column(w, c), m0 = (w.m() * 2 + rank) * TILE;
+          if (col < g.N && m0 < g.rows) {
+            tma_store(&g.y[MODE == GATE_BWD ? c % 2 : 0], col, m0, buf + s * C::CH_BYTES);
             bulk_commit();
             bulk_wait_read();
           }
@@ -397,141 +649,10 @@ __global__ void __launch_bounds__(THREADS, 1) rows_tc_kernel(const __grid_consta
     }
     __syncwarp();
   } else {
-    // ---- read-out: thread = pixel, 32 channels at a time
-    const int set = (warp - 4) / 4, q = warp & 3, row = q * 32 + lane;
-    const uint32_t buf = out0 + set * g.slots * CH_BYTES;
-    const uint32_t t0 = tmem + ((uint32_t)(q * 32) << 16) + set * 256;
-    // 16-byte piece j of this row of a staged tile
-    const auto piece = [&](uint32_t slot, int j) { return buf + slot * CH_BYTES + row * 128 + ((j ^ (row & 7)) << 4); };
-    const auto slot_ready = [&](uint32_t i) { return warp_wait(ready(set, i % g.slots), (i / g.slots) & 1, abort_flag, 0x132); };
-    const auto slot_done = [&](uint32_t i) {
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(done(set, i % g.slots));
-    };
-    const auto accumulators_free = [&]() {
-      tc_fence_before_sync();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(tempty(set));
-    };
-    uint32_t it = 0, i = 0;
-    bool ok = true;
-    for (TileWalk w(g, set, 2); w.more() && ok; w.next(), ++it) {
-      float* bs = bias_s + set * 512 + (g.resident ? 0 : (it & 1) * 256);
-      if (it == 0 || !g.resident) {
-        // (the other half is still being read by warps that are a tile behind; nobody is two behind)
-        const int n0 = w.nt() * BN;
-#pragma unroll
-        for (int e = row; e < C::N0; e += 128) {
-          const int n = n0 + e % BN + (e >= BN ? g.up : 0);
-          bs[e] = g.bias && n0 + e % BN < g.N
-                      ? __bfloat162float(__ushort_as_bfloat16(__ldg((const unsigned short*)g.bias + n)))
-                      : 0.f;
-        }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(biased(set));
-        ok = warp_wait(biased(set), it & 1, abort_flag, 0x133);  // (a bounded wait, unlike bar.sync)
-        if (!ok) break;
-      }
-      ok = warp_wait(tfull(set), it & 1, abort_flag, 0x131);
-      if (!ok) break;
-      tc_fence_after_sync();
-      if constexpr (MODE == GATE_BWD) {
-        uint32_t pu[2][16];  // the second result, packed, until its slot is free
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          uint32_t vg[32], vu[32], vh[32];
-          tmem_ld_32x32(t0 + 32 * k, vg);
-          tmem_ld_32x32(t0 + BN + 32 * k, vu);
-          tmem_ld_32x32(t0 + C::OFF1 + 32 * k, vh);
-          tmem_ld_wait();
-          if (k == 1) accumulators_free();
-          with_act(g.act, [&](auto a) {
-            typedef decltype(a) Act;
-#pragma unroll
-            for (int j = 0; j < 16; ++j) {
-              float2 v, s;
-              Act::both(add2(pair_of(vg, j), bias2(bs, 16 * k + j)), v, s);
-              const float2 gh = pair_of(vh, j), u = add2(pair_of(vu, j), bias2(bs + BN, 16 * k + j));
-              const float2 og = mul2(mul2(gh, u), s), ou = mul2(gh, v);
-              vg[j] = pack_bf16x2(og.x, og.y);
-              pu[k][j] = pack_bf16x2(ou.x, ou.y);
-            }
-          });
-          if (k == 0) ok = slot_ready(i);
-          if (!ok) break;
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            sts16(piece(i % g.slots, 4 * k + j), make_uint4(vg[4 * j], vg[4 * j + 1], vg[4 * j + 2], vg[4 * j + 3]));
-        }
-        if (!ok) break;
-        slot_done(i++);
-        ok = slot_ready(i);
-        if (!ok) break;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const uint32_t* v = &pu[j / 4][j % 4 * 4];
-          sts16(piece(i % g.slots, j), make_uint4(v[0], v[1], v[2], v[3]));
-        }
-        slot_done(i++);
-      } else {
-#pragma unroll 1
-        for (int c = 0; c < C::NCH && ok; ++c) {
-          const uint32_t s = i % g.slots;
-#pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            uint32_t v[32], u[32];
-            tmem_ld_32x32(t0 + 64 * c + 32 * k, v);
-            if (MODE == GATE) tmem_ld_32x32(t0 + BN + 64 * c + 32 * k, u);
-            tmem_ld_wait();
-            if (c == C::NCH - 1 && k == 1) accumulators_free();
-            const float* b = bs + 64 * c + 32 * k;
-            with_act(g.act, [&](auto a) {
-              typedef decltype(a) Act;
-#pragma unroll
-              for (int j = 0; j < 16; ++j) {
-                const float2 z = add2(pair_of(v, j), bias2(b, j));
-                float2 o;
-                if (MODE == ACT_BWD) {
-                  float2 val;
-                  Act::both(z, val, o);
-                } else {
-                  o = Act::value(z);
-                  if (MODE == GATE) o = mul2(o, add2(pair_of(u, j), bias2(b + BN, j)));
-                }
-                if (MODE == GATE) v[j] = pack_bf16x2(o.x, o.y);
-                else v[2 * j] = __float_as_uint(o.x), v[2 * j + 1] = __float_as_uint(o.y);
-              }
-            });
-            if (k == 0) ok = slot_ready(i);
-            if (!ok) break;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              const uint32_t at = piece(s, 4 * k + j);
-              if (MODE == GATE) {
-                sts16(at, make_uint4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]));
-                continue;
-              }
-              float2 f[4];
-#pragma unroll
-              for (int e = 0; e < 4; ++e) f[e] = pair_of(v, 4 * j + e);
-              if (MODE == ACT_BWD || (MODE == LAYER && g.res)) {
-                const uint4 r = lds16(at);
-                const uint32_t rw[4] = {r.x, r.y, r.z, r.w};
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                  const float2 w = make_float2(__uint_as_float(rw[e] << 16), __uint_as_float(rw[e] & 0xFFFF0000u));
-                  f[e] = MODE == ACT_BWD ? mul2(f[e], w) : add2(f[e], w);
-                }
-              }
-              sts16(at, make_uint4(pack_bf16x2(f[0].x, f[0].y), pack_bf16x2(f[1].x, f[1].y), pack_bf16x2(f[2].x, f[2].y),
-                                   pack_bf16x2(f[3].x, f[3].y)));
-            }
-          }
-          if (ok) slot_done(i++);
-        }
-      }
-    }
+    // ---- read-out
+    with_act(g.act, [&](auto act) {
+      read_out<MODE, BN, decltype(act)>(g, (warp - 4) / 4, rank, bias_s, out0, bfull, abort_flag);
+    });
   }
   __syncthreads();
   if (*abort_flag && threadIdx.x == 0) {  // given up: copies still in flight land within microseconds
@@ -540,7 +661,8 @@ __global__ void __launch_bounds__(THREADS, 1) rows_tc_kernel(const __grid_consta
   }
   tc_fence_before_sync();
   __syncthreads();
-  if (warp == 1) tmem_dealloc(tmem, 512);
+  cluster_sync();  // (no block leaves while the other's MMAs, copies or arrivals still reach it)
+  if (warp == 1) pair_dealloc(tmem, 512);
 }
 
 // ---- outer kernel ----------------------------------------------------------------------------------------
@@ -552,12 +674,12 @@ struct alignas(64) OuterTcArgs {
   int kblocks, per;    // 64-pixel blocks in all, and of a share
   int stages;
 };
-constexpr int OUTER_BARS = 2 * MAX_STAGES + 1;
+constexpr int OUTER_BARS = 3 * MAX_STAGES + 1;
 
-// MT: groups of 128 channels of the first operand, BN: channels of the second
+// MT: groups of 2 x 128 channels of the first operand, BN: channels of the second.  A block holds half of either.
 template <int MT, int BN>
 __global__ void __launch_bounds__(THREADS, 1) outer_tc_kernel(const __grid_constant__ OuterTcArgs g) {
-  constexpr int GB = MT * A_BYTES, STAGE = GB + BN * 128;
+  constexpr int GB = MT * A_BYTES, STAGE = GB + BN / 2 * 128;
   extern __shared__ unsigned char raw[];
   __shared__ volatile int abort_flag_s;
   __shared__ uint64_t bars[OUTER_BARS];
@@ -568,63 +690,75 @@ __global__ void __launch_bounds__(THREADS, 1) outer_tc_kernel(const __grid_const
   const uint32_t s0 = smem_u32(sm), bar0 = smem_u32(bars);
   const auto full = [&](uint32_t s) { return bar0 + 8 * s; };
   const auto empty = [&](uint32_t s) { return bar0 + 8 * (MAX_STAGES + s); };
-  const uint32_t done = bar0 + 16 * MAX_STAGES;
+  const auto landed = [&](uint32_t s) { return bar0 + 8 * (2 * MAX_STAGES + s); };  // (full is the leader's alone)
+  const uint32_t done = bar0 + 24 * MAX_STAGES;
   const int tiles = g.segs * g.m_tiles * g.n_tiles;
-  const int split = blockIdx.x / tiles, tile = blockIdx.x % tiles;
+  const uint32_t rank = cluster_rank();
+  const int split = blockIdx.x / 2 / tiles, tile = blockIdx.x / 2 % tiles;
   const int nt = tile % g.n_tiles, mt = tile / g.n_tiles % g.m_tiles, seg = tile / g.n_tiles / g.m_tiles;
-  const int m0 = mt * MT * 128, n0 = nt * BN;
+  // channel group m of this block starts at m0 + 256 m
+  const int m0 = mt * MT * 256 + rank * 128, n0 = nt * BN;
   const int k0 = split * g.per, k1 = min(g.kblocks, k0 + g.per);
   const bool sums = nt == 0;
 
   if (threadIdx.x == 0) {
     abort_flag_s = 0;
-    for (int i = 0; i < g.stages; ++i) mbar_init(full(i), 1), mbar_init(empty(i), sums ? 9 : 1);
+    for (int i = 0; i < g.stages; ++i) mbar_init(full(i), 1), mbar_init(landed(i), 1), mbar_init(empty(i), sums ? 9 : 1);
     mbar_init(done, 1);
     fence_barrier_init();
     fence_proxy_async_smem();
   }
-  if (warp == 1) tmem_alloc(smem_u32(&tmem_s), MT * BN < 32 ? 32 : MT * BN);
+  if (warp == 1) pair_alloc(smem_u32(&tmem_s), MT * BN);
   tc_fence_before_sync();
   __syncthreads();
+  cluster_sync();
   tc_fence_after_sync();
   const uint32_t tmem = tmem_s;
 
   if (warp == 0) {  // (converged, one elected lane issues: see the rows kernel)
-    const bool leader = elect_one();
+    const bool elected = elect_one();
     uint32_t st = 0, ph = 0;
     for (int k = k0; k < k1; ++k) {
       if (!__all_sync(~0u, mbar_wait(empty(st), ph ^ 1, abort_flag, 0x141))) break;
-      if (leader) {
-        mbar_expect_tx(full(st), STAGE);
-        const uint32_t dst = s0 + st * STAGE;
+      if (elected) {
+        const uint32_t bar = of_leader(full(st)), dst = s0 + st * STAGE;
+        if (rank == 0) mbar_expect_tx(full(st), 2 * STAGE);
 #pragma unroll
-        for (int i = 0; i < 2 * MT; ++i) tma_load(dst + i * 8192, &g.g[seg], m0 + 64 * i, k * KB, full(st));
+        for (int i = 0; i < 2 * MT; ++i)
+          tma_load_pair(dst + i * 8192, &g.g[seg], m0 + i / 2 * 256 + i % 2 * 64, k * KB, bar);
 #pragma unroll
-        for (int i = 0; i < BN / 64; ++i) tma_load(dst + GB + i * 8192, &g.x, n0 + 64 * i, k * KB, full(st));
+        for (int i = 0; i < BN / 128; ++i)
+          tma_load_pair(dst + GB + i * 8192, &g.x, n0 + rank * (BN / 2) + 64 * i, k * KB, bar);
       }
       __syncwarp();
       if (++st == (uint32_t)g.stages) st = 0, ph ^= 1;
     }
   } else if (warp == 1) {
-    const bool leader = elect_one();
-    constexpr uint32_t idesc = make_idesc_bf16(128, BN, 1, 1), HI = desc_sw128_hi(1024);
-    uint32_t st = 0, ph = 0;
-    for (int k = k0; k < k1; ++k) {
-      if (!__all_sync(~0u, mbar_wait(full(st), ph, abort_flag, 0x142))) break;
-      if (leader) {
-        const uint32_t bd = desc_sw128_lo(s0 + st * STAGE + GB, 8192), ad = desc_sw128_lo(s0 + st * STAGE, 8192);
+    if (rank == 0) {
+      const bool elected = elect_one();
+      constexpr uint32_t idesc = make_idesc_bf16(256, BN, 1, 1), HI = desc_sw128_hi(1024);
+      uint32_t st = 0, ph = 0;
+      bool there = false;
+      for (int k = k0; k < k1; ++k) {
+        if (!there && !__all_sync(~0u, mbar_wait(full(st), ph, abort_flag, 0x142))) break;
+        const uint32_t cur = st;
+        if (++st == (uint32_t)g.stages) st = 0, ph ^= 1;
+        const bool next = mbar_test(full(st), ph);
+        if (elected) {
+          const uint32_t bd = desc_sw128_lo(s0 + cur * STAGE + GB, 8192), ad = desc_sw128_lo(s0 + cur * STAGE, 8192);
 #pragma unroll
-        for (int m = 0; m < MT; ++m)
+          for (int m = 0; m < MT; ++m)
 #pragma unroll
-          for (int j = 0; j < 4; ++j)  // sixteen pixels each
-            mma_bf16_ss_lo(tmem + m * BN, ad + m * (A_BYTES >> 4) + 128 * j, HI, bd + 128 * j, HI, idesc, k != k0 || j != 0);
-        mma_commit(empty(st));
+            for (int j = 0; j < 4; ++j)  // sixteen pixels each
+              pair_mma(tmem + m * BN, ad + m * (A_BYTES >> 4) + 128 * j, HI, bd + 128 * j, HI, idesc, k != k0 || j != 0);
+          pair_commit(empty(cur));
+          if (sums) pair_commit(landed(cur));
+        }
+        there = __all_sync(~0u, next);
       }
+      if (elected) pair_commit(done);
       __syncwarp();
-      if (++st == (uint32_t)g.stages) st = 0, ph ^= 1;
     }
-    if (leader) mma_commit(done);
-    __syncwarp();
   } else if (warp >= 4) {
     const int ew = warp - 4, q = warp & 3;
     bool ok = true;
@@ -635,7 +769,7 @@ __global__ void __launch_bounds__(THREADS, 1) outer_tc_kernel(const __grid_const
       float acc[8] = {};
       uint32_t st = 0, ph = 0;
       for (int k = k0; k < k1; ++k) {
-        ok = warp_wait(full(st), ph, abort_flag, 0x143);
+        ok = warp_wait(landed(st), ph, abort_flag, 0x143);
         if (!ok) break;
         const uint32_t base = s0 + st * STAGE + box * 8192;
 #pragma unroll
@@ -656,7 +790,7 @@ __global__ void __launch_bounds__(THREADS, 1) outer_tc_kernel(const __grid_const
       for (int e = 0; e < 8; ++e) {
 #pragma unroll
         for (int o = 16; o >= PC; o >>= 1) acc[e] += __shfl_xor_sync(~0u, acc[e], o);
-        const int m = m0 + piece * 8 + e;
+        const int m = m0 + piece / 16 * 256 + piece % 16 * 8 + e;
         if (lane < PC && m < g.M) g.csum[((size_t)split * g.segs + seg) * g.M + m] = acc[e];
       }
     }
@@ -668,7 +802,7 @@ __global__ void __launch_bounds__(THREADS, 1) outer_tc_kernel(const __grid_const
         uint32_t v[32];
         tmem_ld_32x32(tmem + ((uint32_t)(q * 32) << 16) + t * 32, v);
         tmem_ld_wait();
-        const int m = m0 + t * 32 / BN * 128 + q * 32 + lane, n = n0 + t * 32 % BN;
+        const int m = m0 + t * 32 / BN * 256 + q * 32 + lane, n = n0 + t * 32 % BN;
         float* out = g.part + (((size_t)split * g.segs + seg) * g.M + m) * g.ldn + n;
 #pragma unroll
         for (int j = 0; j < 8; ++j)
@@ -687,12 +821,13 @@ __global__ void __launch_bounds__(THREADS, 1) outer_tc_kernel(const __grid_const
     while (clock64() - c < 4000000) __nanosleep(1000);
   }
   __syncthreads();
-  if (warp == 1) tmem_dealloc(tmem, MT * BN < 32 ? 32 : MT * BN);
+  cluster_sync();
+  if (warp == 1) pair_dealloc(tmem, MT * BN);
 }
 
 // ---- host ------------------------------------------------------------------------------------------------
-// boxes of 64 channels x box_r rows, 128-byte swizzle
-static bool encode(CUtensorMap* tm, const TcRows& t, int box_r) {
+// boxes of 64 channels x box_r rows, 128-byte swizzle (32 channels: 64-byte)
+static bool encode(CUtensorMap* tm, const TcRows& t, int box_r, int box_c = KB) {
   static std::atomic<void*> fn{nullptr};
   void* f = fn.load(std::memory_order_acquire);
   if (!f) {
@@ -706,10 +841,10 @@ static bool encode(CUtensorMap* tm, const TcRows& t, int box_r) {
                               const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
                               CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
   const cuuint64_t dims[2] = {(cuuint64_t)t.cols, (cuuint64_t)t.rows}, strides[1] = {(cuuint64_t)t.ld * 2};
-  const cuuint32_t box[2] = {KB, (cuuint32_t)box_r}, es[2] = {1, 1};
+  const cuuint32_t box[2] = {(cuuint32_t)box_c, (cuuint32_t)box_r}, es[2] = {1, 1};
   for (int attempt = 0; attempt < 2; ++attempt) {
     if (((Encode)f)(tm, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(t.p), dims, strides, box, es,
-                    CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                    CU_TENSOR_MAP_INTERLEAVE_NONE, box_c == 32 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
                     CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS)
       return true;
     // A thread whose first CUDA call this is (autograd's, with all memory cached) has no context yet; selecting its
@@ -735,38 +870,62 @@ static bool allow_smem(Kern kern) {
   return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_LIMIT) == cudaSuccess;
 }
 
-template <int MODE, int BN, bool BMN>
-static int launch_rows(GemmArgs& g, int n_cover, cudaStream_t st) {
-  typedef Cfg<MODE, BN> C;
-  g.n_tiles = (n_cover + BN - 1) / BN;
-  const int fixed_bytes = 1024 + 4 * 256 * 4 + ROWS_BARS * 8 + 16 + 64;
-  const int b_all = g.kb[0] * C::N0 * 128 + g.kb[1] * C::N1 * 128;
-  const int sms = sm_total();
-  g.slots = 2;
-  int left = SMEM_LIMIT - fixed_bytes - 2 * g.slots * CH_BYTES;
-  // Weights stay where at least three stages of pixels fit beside them and every channel tile gets a block.
-  g.resident = g.n_tiles <= sms && b_all + 3 * A_BYTES <= left;
-  if (!g.resident && g.n_tiles <= sms) {  // one slot per set makes room for 128 KB of them
-    const int one = left + 2 * CH_BYTES;
-    if (b_all + 3 * A_BYTES <= one) g.slots = 1, left = one, g.resident = 1;
-  }
-  g.stages = g.resident ? (left - b_all) / A_BYTES : left / (A_BYTES + C::BMAX);
-  if (g.stages > MAX_STAGES) g.stages = MAX_STAGES;
-  const size_t smem = fixed_bytes + 2 * g.slots * CH_BYTES + (size_t)g.stages * A_BYTES +
-                      (g.resident ? b_all : g.stages * C::BMAX);
-  long long grid;
-  if (g.resident) {
-    grid = sms / g.n_tiles;
-    if (grid > g.m_tiles) grid = g.m_tiles;
-    grid *= g.n_tiles;
-  } else {
-    grid = (long long)g.m_tiles * g.n_tiles;
-    if (grid > sms) grid = sms;
-  }
-  if (!allow_smem(rows_tc_kernel<MODE, BN, BMN>)) return MC_ERR_LAUNCH;
-  rows_tc_kernel<MODE, BN, BMN><<<(unsigned)grid, THREADS, smem, st>>>(g), MC_COUNT(1);
-  MC_CHECK_LAUNCH();
+// Blocks in clusters of two.
+template <typename Kern, typename Args>
+static int launch_pairs(Kern kern, unsigned pairs, size_t smem, const Args& args, cudaStream_t st) {
+  if (!allow_smem(kern)) return MC_ERR_LAUNCH;
+  cudaLaunchAttribute attr = {};
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = 2, attr.val.clusterDim.y = 1, attr.val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(2 * pairs);
+  cfg.blockDim = dim3(THREADS);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  if (cudaLaunchKernelEx(&cfg, kern, args) != cudaSuccess) return MC_ERR_LAUNCH;
+  MC_COUNT(1);
   return MC_OK;
+}
+
+template <int MODE, int BN>
+static int launch_rows(GemmArgs& g, cudaStream_t st) {
+  typedef Cfg<MODE, BN> C;
+  g.n_tiles = (g.N + BN - 1) / BN;
+  const int fixed_bytes = 1024 + 4 * 256 * 4 + ROWS_BARS * 8 + 16 + 64;
+  const int b_tile = g.kb[0] * C::B0 + g.kb[1] * C::B1, pairs = sm_total() / 2;
+  g.slots = 2;
+  int left = SMEM_LIMIT - fixed_bytes - 2 * g.slots * C::CH_BYTES;
+  // Weights stay in shared memory where at least three stages of pixels fit beside them.  How many channel tiles a pair
+  // keeps: the number that leaves the fewest pairs without work; more tiles cost stages, below four of which the pixels'
+  // latency shows.
+  double best = 0;
+  for (int group = 1; group <= g.n_tiles; ++group) {
+    const int groups = g.n_tiles / group;
+    if (g.n_tiles % group || groups > pairs) continue;
+    if ((long long)group * b_tile + 3 * A_BYTES > left) break;
+    const int stages = (left - group * b_tile) / A_BYTES;
+    const double used = (double)(pairs / groups * groups) / pairs * (stages >= 4 ? 1.0 : 0.93);
+    if (used > best + 1e-9) best = used, g.group = group;
+  }
+  if (!g.group && MODE != GATE_BWD && g.n_tiles <= pairs && b_tile + 3 * A_BYTES <= left + 2 * C::CH_BYTES)
+    g.group = g.slots = 1, left += 2 * C::CH_BYTES;  // one slot per set makes room for one tile's
+  g.stages = g.group ? (left - g.group * b_tile) / A_BYTES : left / (A_BYTES + C::BMAX);
+  if (g.stages > MAX_STAGES) g.stages = MAX_STAGES;
+  const size_t smem = fixed_bytes + 2 * g.slots * C::CH_BYTES + (size_t)g.stages * A_BYTES +
+                      (g.group ? g.group * b_tile : g.stages * C::BMAX);
+  long long n;
+  if (g.group) {
+    const int groups = g.n_tiles / g.group;
+    n = pairs / groups;
+    if (n > g.m_pairs) n = g.m_pairs;
+    n *= groups;
+  } else {
+    n = (long long)g.m_pairs * g.n_tiles;
+    if (n > pairs) n = pairs;
+  }
+  return launch_pairs(rows_tc_kernel<MODE, BN>, (unsigned)n, smem, g, st);
 }
 
 // Channels of a tile: the smallest of 64, 128, 256 that holds all of them, else the one that pads least.
@@ -776,16 +935,22 @@ static int tile_width(int n) {
   return (n + 255) / 256 * 256 <= (n + 127) / 128 * 128 + 64 ? 256 : 128;
 }
 static int kblocks(int c) { return (c + KB - 1) / KB; }
-static int tiles_of(long long P) { return (int)((P + TILE - 1) / TILE); }
 
 static GemmArgs base_args(const TcRows& a, const TcRows& y, const bf16* bias, int act) {
   GemmArgs g{};
   g.bias = bias;
-  g.m_tiles = tiles_of(a.rows);
+  g.rows = (int)a.rows;
+  g.m_pairs = (int)((a.rows + 2 * TILE - 1) / (2 * TILE));
   g.N = y.cols;
   g.kb[0] = kblocks(a.cols);
   g.act = act;
   return g;
+}
+template <int MODE>
+static int launch_wide(GemmArgs& g, int bn, cudaStream_t st) {
+  if (bn == 64) return launch_rows<MODE, 64>(g, st);
+  if (bn == 128) return launch_rows<MODE, 128>(g, st);
+  return launch_rows<MODE, 256>(g, st);
 }
 
 int tc_layer(const TcRows& a, const TcRows& w, const bf16* bias, int act, const TcRows& r, const TcRows& y,
@@ -793,48 +958,39 @@ int tc_layer(const TcRows& a, const TcRows& w, const bf16* bias, int act, const 
   GemmArgs g = base_args(a, y, bias, act);
   g.res = r.p != nullptr;
   const int bn = tile_width(y.cols);
-  if (!encode(&g.a[0], a, TILE) || !encode(&g.b[0], w, bn) || !encode(&g.y[0], y, TILE)) return MC_ERR_LAUNCH;
+  if (!encode(&g.a[0], a, TILE) || !encode(&g.b[0], w, bn / 2) || !encode(&g.y[0], y, TILE)) return MC_ERR_LAUNCH;
   if (g.res && !encode(&g.r, r, TILE)) return MC_ERR_LAUNCH;
-  if (backward) {
-    if (bn == 64) return launch_rows<ACT_BWD, 64, false>(g, y.cols, st);
-    if (bn == 128) return launch_rows<ACT_BWD, 128, false>(g, y.cols, st);
-    return launch_rows<ACT_BWD, 256, false>(g, y.cols, st);
-  }
-  if (bn == 64) return launch_rows<LAYER, 64, false>(g, y.cols, st);
-  if (bn == 128) return launch_rows<LAYER, 128, false>(g, y.cols, st);
-  return launch_rows<LAYER, 256, false>(g, y.cols, st);
+  return backward ? launch_wide<ACT_BWD>(g, bn, st) : launch_wide<LAYER>(g, bn, st);
 }
 
 int tc_input_grad(const TcRows& g0, const TcRows& w0, const TcRows& g1, const TcRows& w1, const TcRows& gx,
                   cudaStream_t st) {
   GemmArgs g = base_args(g0, gx, nullptr, MC_ACT_NONE);
   const int bn = tile_width(gx.cols);
-  if (!encode(&g.a[0], g0, TILE) || !encode(&g.b[0], w0, 64) || !encode(&g.y[0], gx, TILE)) return MC_ERR_LAUNCH;
+  if (!encode(&g.a[0], g0, TILE) || !encode(&g.b[0], w0, bn / 2) || !encode(&g.y[0], gx, TILE)) return MC_ERR_LAUNCH;
   if (g1.p) {
     g.kb[1] = kblocks(g1.cols);
-    if (!encode(&g.a[1], g1, TILE) || !encode(&g.b[1], w1, 64)) return MC_ERR_LAUNCH;
+    if (!encode(&g.a[1], g1, TILE) || !encode(&g.b[1], w1, bn / 2)) return MC_ERR_LAUNCH;
   }
-  if (bn == 64) return launch_rows<LAYER, 64, true>(g, gx.cols, st);
-  if (bn == 128) return launch_rows<LAYER, 128, true>(g, gx.cols, st);
-  return launch_rows<LAYER, 256, true>(g, gx.cols, st);
+  return launch_wide<LAYER>(g, bn, st);
 }
 
 int tc_gate(const TcRows& x, const TcRows& w_in, const bf16* b_in, int act, const TcRows& h, cudaStream_t st) {
   GemmArgs g = base_args(x, h, b_in, act);
   g.up = h.cols;
   if (!encode(&g.a[0], x, TILE) || !encode(&g.b[0], w_in, 128) || !encode(&g.y[0], h, TILE)) return MC_ERR_LAUNCH;
-  return launch_rows<GATE, 128, false>(g, h.cols, st);
+  return launch_rows<GATE, 128>(g, st);
 }
 
-int tc_gate_bwd(const TcRows& x, const TcRows& w_in, const bf16* b_in, int act, const TcRows& gy, const TcRows& w_out,
+int tc_gate_bwd(const TcRows& x, const TcRows& w_in, const bf16* b_in, int act, const TcRows& gy, const TcRows& w_out_t,
                 const TcRows& gg, const TcRows& gu, cudaStream_t st) {
   GemmArgs g = base_args(x, gg, b_in, act);
   g.up = gg.cols;
   g.kb[1] = kblocks(gy.cols);
   if (!encode(&g.a[0], x, TILE) || !encode(&g.b[0], w_in, 64) || !encode(&g.a[1], gy, TILE) ||
-      !encode(&g.b[1], w_out, 64) || !encode(&g.y[0], gg, TILE) || !encode(&g.y[1], gu, TILE))
+      !encode(&g.b[1], w_out_t, 32) || !encode(&g.y[0], gg, TILE, 32) || !encode(&g.y[1], gu, TILE, 32))
     return MC_ERR_LAUNCH;
-  return launch_rows<GATE_BWD, 64, false>(g, gg.cols, st);
+  return launch_rows<GATE_BWD, 64>(g, st);
 }
 
 // Blocks per gradient tile: as many as fill the SMs once or a whole number of times with equal shares.
@@ -843,17 +999,18 @@ struct OuterPlan {
 };
 static OuterPlan outer_plan(long long P, int M, int segs, int N) {
   OuterPlan p;
-  p.mt = M > 128 ? 2 : 1;
-  p.bn = N <= 64 ? 64 : N <= 128 ? 128 : 256;
-  p.m_tiles = (M + 128 * p.mt - 1) / (128 * p.mt);
+  p.mt = M > 256 ? 2 : 1;
+  p.bn = N <= 128 ? 128 : 256;
+  p.m_tiles = (M + 256 * p.mt - 1) / (256 * p.mt);
   p.n_tiles = (N + p.bn - 1) / p.bn;
   const long long tiles = (long long)segs * p.m_tiles * p.n_tiles, kb = (P + KB - 1) / KB;
   double best = 1e30;
   p.splits = 1, p.per = (int)kb;
-  for (long long s = 1; s <= 148 && s <= (kb + 3) / 4; ++s) {
+  const int pairs = sm_total() / 2;
+  for (long long s = 1; s <= pairs && s <= (kb + 3) / 4; ++s) {
     const long long per = (kb + s - 1) / s;
-    const double waves = (double)((tiles * s + 147) / 148);
-    // a block's stages, and what it costs to write its sums and to add them up again
+    const double waves = (double)((tiles * s + pairs - 1) / pairs);
+    // a pair's stages, and what it costs to write its sums and to add them up again
     const double t = waves * (per + 8.0) + 0.05 * tiles * s;
     if (t < best) best = t, p.splits = (int)((kb + per - 1) / per), p.per = (int)per;
   }
@@ -868,13 +1025,10 @@ size_t tc_outer_floats(long long P, int M, int segs, int N, int* splits, int* ld
 
 template <int MT, int BN>
 static int launch_outer(OuterTcArgs& g, const OuterPlan& p, cudaStream_t st) {
-  constexpr int STAGE = MT * A_BYTES + BN * 128;
+  constexpr int STAGE = MT * A_BYTES + BN / 2 * 128;
   g.stages = (SMEM_LIMIT - 2048) / STAGE;
   if (g.stages > MAX_STAGES) g.stages = MAX_STAGES;
-  if (!allow_smem(outer_tc_kernel<MT, BN>)) return MC_ERR_LAUNCH;
-  outer_tc_kernel<MT, BN><<<g.segs * p.m_tiles * p.n_tiles * p.splits, THREADS, 1024 + g.stages * STAGE, st>>>(g), MC_COUNT(1);
-  MC_CHECK_LAUNCH();
-  return MC_OK;
+  return launch_pairs(outer_tc_kernel<MT, BN>, g.segs * p.m_tiles * p.n_tiles * p.splits, 1024 + g.stages * STAGE, g, st);
 }
 int tc_outer(const TcRows& g0, const TcRows& g1, const TcRows& x, float* part, float* csum, cudaStream_t st) {
   OuterTcArgs g{};
@@ -885,14 +1039,8 @@ int tc_outer(const TcRows& g0, const TcRows& g1, const TcRows& x, float* part, f
   g.M = g0.cols, g.N = x.cols, g.ldn = (x.cols + 3) / 4 * 4;
   g.m_tiles = p.m_tiles, g.n_tiles = p.n_tiles;
   g.kblocks = (int)((x.rows + KB - 1) / KB), g.per = p.per;
-  if (p.mt == 1) {
-    if (p.bn == 64) return launch_outer<1, 64>(g, p, st);
-    if (p.bn == 128) return launch_outer<1, 128>(g, p, st);
-    return launch_outer<1, 256>(g, p, st);
-  }
-  if (p.bn == 64) return launch_outer<2, 64>(g, p, st);
-  if (p.bn == 128) return launch_outer<2, 128>(g, p, st);
-  return launch_outer<2, 256>(g, p, st);
+  if (p.mt == 1) return p.bn == 128 ? launch_outer<1, 128>(g, p, st) : launch_outer<1, 256>(g, p, st);
+  return p.bn == 128 ? launch_outer<2, 128>(g, p, st) : launch_outer<2, 256>(g, p, st);
 }
 
 int tc_status_read(int reset) {
