@@ -23,41 +23,55 @@ static int check_desc(const mc_mix_desc* d, bool gated) {
 
 static long long pixels(const mc_mix_desc* d) { return d->B * d->S; }
 
-// Shares of the pixels that a parameter gradient is summed in: about two waves of blocks, at least 256 pixels each.
+// Shares of the pixels that a parameter gradient is summed in: about four waves of blocks, at least 256 pixels each where
+// images are that large; parts of an image or groups of images (channels-last batches are one image).
 struct Shares {
-  long long share;
-  int splits;
+  long long S, share;
+  int B, group, per_image, splits;
   size_t part, csum;  // bytes
 };
-static Shares shares_of(long long P, int M, int N, int dtype) {
-  const long long tiles = (long long)((M + 127) / 128) * ((N + 127) / 128);
-  long long n = (2 * 148 + tiles - 1) / tiles, most = (P + 255) / 256;
-  if (n > most) n = most;
+static Shares shares_of(const mc_mix_desc* d, int M, int N) {
   Shares s;
-  s.share = ((P + n - 1) / n + 15) / 16 * 16;
-  s.splits = (int)((P + s.share - 1) / s.share);
-  s.part = up256((size_t)s.splits * M * N * acc_size(dtype));
-  s.csum = up256((size_t)s.splits * M * acc_size(dtype));
+  const bool whole = d->layout == MC_NHWC || d->S == 1 || d->B == 1;
+  s.B = whole ? 1 : (int)d->B;
+  s.S = whole ? d->B * d->S : d->S;
+  const long long tiles = (long long)((M + 127) / 128) * ((N + 127) / 128);
+  long long want = (4 * 148 + tiles - 1) / tiles, most = (s.B * s.S + 255) / 256;
+  if (want > most) want = most;
+  s.group = (int)((s.B + want - 1) / want);
+  const long long n = s.group > 1 ? 1 : (want + s.B - 1) / s.B;
+  s.share = ((s.S + n - 1) / n + 15) / 16 * 16;
+  s.per_image = (int)((s.S + s.share - 1) / s.share);
+  s.splits = (s.B + s.group - 1) / s.group * s.per_image;
+  s.part = up256((size_t)s.splits * M * N * acc_size(d->dtype));
+  s.csum = up256((size_t)s.splits * M * acc_size(d->dtype));
   return s;
 }
 
 // gw (M, N) and gb (M): the shares' sums added in order and rounded once.  Rows of part have ldn elements.  Either may
 // be null.
+// A block takes 32 sums; eight threads for each add every eighth share, and their results are added in order.
 template <typename T, typename CT>
 __global__ void __launch_bounds__(256) add_shares_kernel(const CT* __restrict__ part, int M, int N, int ldn,
                                                          T* __restrict__ gw, const CT* __restrict__ csum,
                                                          T* __restrict__ gb, int splits) {
-  const long long nw = (long long)M * N, total = nw + M;
-  for (long long i = blockIdx.x * 256ll + threadIdx.x; i < total; i += gridDim.x * 256ll) {
-    const bool w = i < nw;
-    if (!(w ? (void*)gw : (void*)gb)) continue;
+  __shared__ CT sums[8][32];
+  const long long nw = (long long)M * N, i = blockIdx.x * 32ll + threadIdx.x % 32;
+  const bool w = i < nw, in = i < nw + M && (w ? (void*)gw : (void*)gb);
+  const int j0 = threadIdx.x / 32;
+  CT s = CT(0);
+  if (in) {
     const CT* src = w ? part + i / N * ldn + i % N : csum + (i - nw);
     const long long step = w ? (long long)M * ldn : M;
-    CT s = CT(0);
 #pragma unroll 8
-    for (int j = 0; j < splits; ++j) s += src[j * step];
-    stv(w ? gw + i : gb + (i - nw), s);
+    for (int j = j0; j < splits; j += 8) s += src[j * step];
   }
+  sums[j0][threadIdx.x % 32] = s;
+  __syncthreads();
+  if (j0 || !in) return;
+#pragma unroll
+  for (int j = 1; j < 8; ++j) s += sums[j][threadIdx.x];
+  stv(w ? gw + i : gb + (i - nw), s);
 }
 
 template <typename T>
@@ -76,17 +90,16 @@ static int by_type(int dtype, F f) {
   return MC_OK;
 }
 
-static int param_grads(int dtype, long long P, long long S, View g, int M, View x, int N, const Shares& s, char* part,
-                       char* csum, void* gw, void* gb, cudaStream_t st) {
-  OuterArgs o{g, x, part, csum, P, s.share, (int)S, M, N, s.splits};
+static int param_grads(int dtype, View g, int M, View x, int N, const Shares& s, char* part, char* csum, void* gw,
+                       void* gb, cudaStream_t st) {
+  const OuterArgs o{g, x, part, csum, s.S, s.share, M, N, s.B, s.group, s.per_image, s.splits};
   const int rc = simt_outer_launch(dtype, o, st);
   if (rc) return rc;
-  const long long nw = (long long)M * N;
   return by_type(dtype, [&](auto t) {
     typedef decltype(t) T;
     typedef typename Traits<T>::CT CT;
-    add_shares_kernel<T, CT><<<grid_for(nw + M, 256), 256, 0, st>>>((const CT*)part, M, N, N, (T*)gw, (const CT*)csum,
-                                                                    (T*)gb, s.splits), MC_COUNT(1);
+    add_shares_kernel<T, CT><<<(unsigned)(((long long)M * N + M + 31) / 32), 256, 0, st>>>(
+        (const CT*)part, M, N, N, (T*)gw, (const CT*)csum, (T*)gb, s.splits), MC_COUNT(1);
   });
 }
 
@@ -207,8 +220,8 @@ struct Work {
     did(tc_outer(g0, g1, x, part, csum, st));
     if (rc) return;
     const long long total = (long long)M * x.cols + M;
-    add_shares_kernel<bf16, float><<<grid_for(total, 256), 256, 0, st>>>(part, M, x.cols, ldn, (bf16*)gw, csum, (bf16*)gb,
-                                                                         splits), MC_COUNT(1);
+    add_shares_kernel<bf16, float><<<(unsigned)((total + 31) / 32), 256, 0, st>>>(part, M, x.cols, ldn, (bf16*)gw, csum,
+                                                                                 (bf16*)gb, splits), MC_COUNT(1);
     did(cudaGetLastError() == cudaSuccess ? MC_OK : MC_ERR_LAUNCH);
   }
 };
@@ -298,7 +311,7 @@ size_t mc_pointwise_workspace_bytes(const mc_mix_desc* d, int32_t phase) {
       else tc_pointwise_fwd(k, d, nullptr, nullptr, nullptr, nullptr, nullptr);
     });
   if (!backward) return 0;
-  const Shares s = shares_of(pixels(d), d->C_out, d->C_in, d->dtype);
+  const Shares s = shares_of(d, d->C_out, d->C_in);
   return mc_pointwise_saved_bytes(d) + s.part + s.csum;
 }
 
@@ -339,7 +352,7 @@ int mc_pointwise_bwd(const mc_mix_desc* d, const void* gy, const void* x, const 
   }
   cudaStream_t st = (cudaStream_t)stream;
   const long long P = pixels(d), n = P * d->C_out;
-  const Shares s = shares_of(P, d->C_out, d->C_in, d->dtype);
+  const Shares s = shares_of(d, d->C_out, d->C_in);
   char* gz = (char*)ws;
   char* part = gz + mc_pointwise_saved_bytes(d);
   const void* g = gy;
@@ -361,7 +374,7 @@ int mc_pointwise_bwd(const mc_mix_desc* d, const void* gy, const void* x, const 
     if (rc) return rc;
   }
   if (gw || gb)
-    rc = param_grads(d->dtype, P, d->S, image_view(g, d->layout, d->S, d->C_out), d->C_out,
+    rc = param_grads(d->dtype, image_view(g, d->layout, d->S, d->C_out), d->C_out,
                      image_view(x, d->layout, d->S, d->C_in), d->C_in, s, part, part + s.part, gw, gb, st);
   return rc;
 }
@@ -389,8 +402,8 @@ size_t mc_gated_workspace_bytes(const mc_mix_desc* d, int32_t phase) {
     });
   const size_t h = (size_t)pixels(d) * d->hidden * esize(d->dtype);
   if (!backward) return phase == MC_PHASE_KEEP ? 0 : up256(h);
-  const Shares a = shares_of(pixels(d), 2 * d->hidden, d->C_in, d->dtype);
-  const Shares b = shares_of(pixels(d), d->C_out, d->hidden, d->dtype);
+  const Shares a = shares_of(d, 2 * d->hidden, d->C_in);
+  const Shares b = shares_of(d, d->C_out, d->hidden);
   const size_t sa = a.part + a.csum, sb = b.part + b.csum;
   return up256(2 * h) + (sa > sb ? sa : sb);
 }
@@ -475,14 +488,14 @@ int mc_gated_bwd(const mc_mix_desc* d, const void* gy, const void* x, const void
     if (rc) return rc;
   }
   if (gw_in || gb_in) {
-    const Shares s = shares_of(P, 2 * H, d->C_in, d->dtype);
-    rc = param_grads(d->dtype, P, d->S, vgz, 2 * H, image_view(x, d->layout, d->S, d->C_in), d->C_in, s, part,
+    const Shares s = shares_of(d, 2 * H, d->C_in);
+    rc = param_grads(d->dtype, vgz, 2 * H, image_view(x, d->layout, d->S, d->C_in), d->C_in, s, part,
                      part + s.part, gw_in, gb_in, st);
     if (rc) return rc;
   }
   if (gw_out || gb_out) {
-    const Shares s = shares_of(P, d->C_out, H, d->dtype);
-    rc = param_grads(d->dtype, P, d->S, vgy, d->C_out, row_view(h, d->S, H), H, s, part, part + s.part, gw_out, gb_out, st);
+    const Shares s = shares_of(d, d->C_out, H);
+    rc = param_grads(d->dtype, vgy, d->C_out, row_view(h, d->S, H), H, s, part, part + s.part, gw_out, gb_out, st);
   }
   return rc;
 }

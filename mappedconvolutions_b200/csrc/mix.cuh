@@ -20,7 +20,7 @@ inline View image_view(const void* p, int layout, long long S, int C) {
   View v;
   v.ptr = p;
   v.img = (long long)C * S;
-  if (layout == MC_NHWC) { v.pix = C; v.ch = 1; } else { v.pix = 1; v.ch = S; }
+  if (layout == MC_NHWC || S == 1) { v.pix = C; v.ch = 1; } else { v.pix = 1; v.ch = S; }
   return v;
 }
 // (P, C) rows of ld elements, whatever the number of images
@@ -105,13 +105,14 @@ struct RowsArgs {
 };
 int simt_rows_launch(int dtype, Epilogue epi, const RowsArgs& a, cudaStream_t st);
 
-// part[s][m][n] = sum over the s-th share of the pixels of g[p, m] x[p, n]; behind those splits * M * N sums,
-// csum[s][m] = sum of g[p, m] over the share.  Sums are float (double for MC_F64).
+// part[s][m][n] = sum over the s-th share of the pixels of g[p, m] x[p, n]; csum[s][m] = sum of g[p, m] over it.  Sums are
+// float (double for MC_F64).  A share is `share` pixels (or what is left of them) of one of B images of S pixels, or
+// `group` whole images; per_image shares to an image (1 where group > 1).
 struct OuterArgs {
   View g, x;
   void *part, *csum;
-  long long P, share;  // pixels per share
-  int S, M, N, splits;
+  long long S, share;
+  int M, N, B, group, per_image, splits;
 };
 int simt_outer_launch(int dtype, const OuterArgs& a, cudaStream_t st);
 

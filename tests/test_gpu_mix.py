@@ -104,6 +104,26 @@ def test_many_pixels(dtype):
     R.check(dict(zip(("gx", "gw_in", "gb_in", "gw_out", "gb_out"), grads), y=y), R.gated(x, wi, bi, wo, bo, None, "silu", gy))
 
 
+@pytest.mark.parametrize("dtype", [BF, F32, F64], ids=["bf16", "f32", "f64"])
+@pytest.mark.parametrize("layout", ["nhwc", "nchw"])
+@pytest.mark.parametrize("shape", [(3000, 2, 3), (70_000, 1, 2), (5, 1, 1), (2, 40, 64)])
+def test_many_small_images(shape, layout, dtype):
+    """more images than a grid's last dimension, images smaller than a tile, single pixels"""
+    b, h, w = shape
+    g = torch.Generator("cuda").manual_seed(8)
+    x, gy = image(g, (b, 6, h, w), dtype, layout), image(g, (b, 5, h, w), dtype, layout, 0.01)
+    r = image(g, (b, 5, h, w), dtype, layout)
+    weight, bias = params(g, 5, 6, dtype)
+    y, saved = host.impl.pointwise_forward(x, weight, bias, r, 4, True)
+    g3 = host.impl.pointwise_backward(gy, saved, x, weight, bias, 4)
+    R.check(dict(zip(("gx", "gw", "gb"), g3), y=y), R.pointwise(x, weight, bias, r, "silu", gy))
+    wi, bi = params(g, 16, 6, dtype)
+    wo, bo = params(g, 5, 8, dtype)
+    y, saved = host.impl.gated_forward(x, wi, bi, wo, bo, r, 4, True)
+    g5 = host.impl.gated_backward(gy, saved, x, wi, bi, wo, 4)
+    R.check(dict(zip(("gx", "gw_in", "gb_in", "gw_out", "gb_out"), g5), y=y), R.gated(x, wi, bi, wo, bo, r, "silu", gy))
+
+
 @pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "f32"])
 def test_layers_and_their_gradients(dtype):
     """two layers as a block would chain them, through autograd, against the chained formulas"""
