@@ -1,5 +1,7 @@
 // C-ABI entry points of the channel-mixing layers: argument checks, workspace layout, and the sequence of products
 // behind each call.
+#include <type_traits>
+
 #include "mix.cuh"
 
 namespace mc {
@@ -7,6 +9,7 @@ namespace mix {
 
 static int esize(int dtype) { return dtype == MC_F64 ? 8 : dtype == MC_F32 ? 4 : 2; }
 static int acc_size(int dtype) { return dtype == MC_F64 ? 8 : 4; }
+static bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 static size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
 
 static int check_desc(const mc_mix_desc* d, bool gated) {
@@ -23,7 +26,7 @@ static int check_desc(const mc_mix_desc* d, bool gated) {
 
 static long long pixels(const mc_mix_desc* d) { return d->B * d->S; }
 
-// Shares of the pixels that a parameter gradient is summed in: about four waves of blocks, at least 256 pixels each where
+// Shares of the pixels that a parameter gradient is summed in: about a wave of blocks (two to an SM), at least 256 pixels each where
 // images are that large; parts of an image or groups of images (channels-last batches are one image).
 struct Shares {
   long long S, share;
@@ -36,7 +39,7 @@ static Shares shares_of(const mc_mix_desc* d, int M, int N) {
   s.B = whole ? 1 : (int)d->B;
   s.S = whole ? d->B * d->S : d->S;
   const long long tiles = (long long)((M + 127) / 128) * ((N + 127) / 128);
-  long long want = (4 * 148 + tiles - 1) / tiles, most = (s.B * s.S + 255) / 256;
+  long long want = (2 * 148 + tiles - 1) / tiles, most = (s.B * s.S + 255) / 256;
   if (want > most) want = most;
   s.group = (int)((s.B + want - 1) / want);
   const long long n = s.group > 1 ? 1 : (want + s.B - 1) / s.B;
@@ -74,12 +77,23 @@ __global__ void __launch_bounds__(256) add_shares_kernel(const CT* __restrict__ 
   stv(w ? gw + i : gb + (i - nw), s);
 }
 
+// gz = gy act'(z), sixteen bytes at a time (vec: all three start on multiples of them)
 template <typename T>
 __global__ void __launch_bounds__(256) act_bwd_kernel(const T* __restrict__ gy, const T* __restrict__ z,
-                                                      T* __restrict__ gz, long long n, int act) {
-  typedef typename Traits<T>::CT CT;
-  for (long long i = blockIdx.x * 256ll + threadIdx.x; i < n; i += gridDim.x * 256ll)
-    stv(gz + i, (CT)ldv(gy + i) * act_slope<CT>(act, (CT)ldv(z + i)));
+                                                      T* __restrict__ gz, long long n, int act, bool vec) {
+  constexpr int V = 16 / sizeof(T);
+  for (long long i = (blockIdx.x * 256ll + threadIdx.x) * V; i < n; i += gridDim.x * 256ll * V) {
+    __align__(16) T g[V], v[V];
+    if (vec && i + V <= n) {
+      *reinterpret_cast<uint4*>(g) = __ldcs(reinterpret_cast<const uint4*>(gy + i));
+      *reinterpret_cast<uint4*>(v) = __ldcs(reinterpret_cast<const uint4*>(z + i));
+#pragma unroll
+      for (int e = 0; e < V; ++e) g[e] *= act_slope<T>(act, v[e]);
+      *reinterpret_cast<uint4*>(gz + i) = *reinterpret_cast<const uint4*>(g);
+    } else {
+      for (int e = 0; e < V && i + e < n; ++e) gz[i + e] = gy[i + e] * act_slope<T>(act, z[i + e]);
+    }
+  }
 }
 
 template <typename F>
@@ -107,7 +121,6 @@ static int param_grads(int dtype, View g, int M, View x, int N, const Shares& s,
 // Rows whose length is a multiple of 8 channels (16 bytes) are read and written where they lie; anything else - other
 // channel counts, NCHW - is copied to padded rows in the workspace and back.
 static int pad8(int c) { return (c + 7) / 8 * 8; }
-static bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
 // (R, C) without gaps -> rows of ld elements, zeros behind the last one
 __global__ void __launch_bounds__(256) pack_rows_kernel(const bf16* __restrict__ src, bf16* __restrict__ dst, long long R,
@@ -130,25 +143,56 @@ __global__ void __launch_bounds__(256) unpack_rows_kernel(const bf16* __restrict
     dst[i] = src[r * ld + (i - r * C)];
   }
 }
-// rows -> (B, C, S): 64 pixels x 64 channels at a time through shared memory
+// (B, C, S) <-> rows of ld channels (zeros behind the last one): CT channels x 4096 / CT pixels at a time through shared
+// memory.  The planes are read and written value by value, neighbouring threads at neighbouring pixels, because with an
+// odd number of pixels they start anywhere; sixteen values per thread are on their way at once.  64 channels of
+// 8 x 125 x 251 pixels to rows: 35 us with the general transpose.
+template <int CT>
+__global__ void __launch_bounds__(256) planes_to_rows_kernel(const bf16* __restrict__ src, bf16* __restrict__ dst,
+                                                             long long S, int C, int ld, int tiles_s, int tiles_c) {
+  constexpr int PX = 4096 / CT, PITCH = CT + 2;
+  __shared__ __align__(16) bf16 tile[PX * PITCH];
+  const int tc = blockIdx.x % tiles_c, ts = blockIdx.x / tiles_c % tiles_s, c0 = tc * CT;
+  const long long b = blockIdx.x / tiles_c / tiles_s, s0 = (long long)ts * PX;
+  const int s = threadIdx.x % PX, c = threadIdx.x / PX;
+  const bf16* from = src + (b * C + c0 + c) * S + s0 + s;
+  bf16 v[16];
+#pragma unroll
+  for (int i = 0; i < 16; ++i)
+    v[i] = s0 + s < S && c0 + c + i * (256 / PX) < C ? __ldcs(from + (long long)i * (256 / PX) * S) : bf16(0.f);
+#pragma unroll
+  for (int i = 0; i < 16; ++i) tile[s * PITCH + c + i * (256 / PX)] = v[i];
+  __syncthreads();
+#pragma unroll
+  for (int i = threadIdx.x; i < 512; i += 256) {
+    const int r = i / (CT / 8), j = i % (CT / 8) * 8;
+    if (s0 + r >= S || c0 + j >= ld) continue;
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(tile + r * PITCH + j);
+    *reinterpret_cast<uint4*>(dst + (b * S + s0 + r) * ld + c0 + j) = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+}
+template <int CT>
 __global__ void __launch_bounds__(256) rows_to_planes_kernel(const bf16* __restrict__ src, bf16* __restrict__ dst,
                                                              long long S, int C, int ld, int tiles_s, int tiles_c) {
-  __shared__ bf16 tile[64 * 66];
-  const int tc = blockIdx.x % tiles_c, ts = blockIdx.x / tiles_c % tiles_s;
-  const long long b = blockIdx.x / tiles_c / tiles_s, s0 = ts * 64ll;
-  const int c0 = tc * 64;
-  for (int i = threadIdx.x; i < 64 * 8; i += 256) {
-    const int s = i / 8, c = i % 8 * 8;
+  constexpr int PX = 4096 / CT, PITCH = CT + 2;
+  __shared__ __align__(16) bf16 tile[PX * PITCH];
+  const int tc = blockIdx.x % tiles_c, ts = blockIdx.x / tiles_c % tiles_s, c0 = tc * CT;
+  const long long b = blockIdx.x / tiles_c / tiles_s, s0 = (long long)ts * PX;
+#pragma unroll
+  for (int i = threadIdx.x; i < 512; i += 256) {
+    const int r = i / (CT / 8), j = i % (CT / 8) * 8;
     uint4 v = make_uint4(0, 0, 0, 0);
-    if (s0 + s < S && c0 + c < ld) v = __ldcs(reinterpret_cast<const uint4*>(src + (b * S + s0 + s) * ld + c0 + c));
-    uint32_t* w = reinterpret_cast<uint32_t*>(tile + s * 66 + c);
+    if (s0 + r < S && c0 + j < ld) v = __ldcs(reinterpret_cast<const uint4*>(src + (b * S + s0 + r) * ld + c0 + j));
+    uint32_t* w = reinterpret_cast<uint32_t*>(tile + r * PITCH + j);
     w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < 64 * 64; i += 256) {
-    const int c = i / 64, s = i % 64;
-    if (c0 + c < C && s0 + s < S) dst[(b * C + c0 + c) * S + s0 + s] = tile[s * 66 + c];
-  }
+  const int s = threadIdx.x % PX, c = threadIdx.x / PX;
+  bf16* to = dst + (b * C + c0 + c) * S + s0 + s;
+#pragma unroll
+  for (int i = 0; i < 16; ++i)
+    if (s0 + s < S && c0 + c + i * (256 / PX) < C)
+      to[(long long)i * (256 / PX) * S] = tile[s * PITCH + c + i * (256 / PX)];
 }
 
 // Lays a call's temporary tensors out in the workspace; without a workspace it only adds up their sizes.
@@ -176,9 +220,22 @@ struct Work {
       pack_rows_kernel<<<grid_for(P * (r.ld / 8), 256), 256, 0, st>>>((const bf16*)p, (bf16*)r.p, P, C, r.ld), MC_COUNT(1);
       did(cudaGetLastError() == cudaSuccess ? MC_OK : MC_ERR_LAUNCH);
     } else {
-      did(mc_transpose(2, d->B, C, d->S, p, (void*)r.p, r.ld, st));
+      planes(d, C, [&](auto ct, unsigned blocks, int ts, int tc) {
+        planes_to_rows_kernel<decltype(ct)::value><<<blocks, 256, 0, st>>>((const bf16*)p, (bf16*)r.p, d->S, C, r.ld, ts, tc);
+      });
     }
     return r;
+  }
+  // f(channels of a tile, blocks, tiles along S, tiles along C): 16 channels where there are no more
+  template <typename F>
+  void planes(const mc_mix_desc* d, int C, F f) {
+    const int ct = C <= 16 ? 16 : 64, px = 4096 / ct;
+    const long long ts = (d->S + px - 1) / px, tc = (C + ct - 1) / ct, blocks = d->B * ts * tc;
+    if (blocks >= (1ll << 31)) return did(MC_ERR_TOO_LARGE);
+    if (ct == 16) f(std::integral_constant<int, 16>(), (unsigned)blocks, (int)ts, (int)tc);
+    else f(std::integral_constant<int, 64>(), (unsigned)blocks, (int)ts, (int)tc);
+    MC_COUNT(1);
+    did(cudaGetLastError() == cudaSuccess ? MC_OK : MC_ERR_LAUNCH);
   }
   TcRows weight(const void* p, int R, int C) {
     if (C % 8 == 0) return TcRows{p, R, C, C};
@@ -204,9 +261,9 @@ struct Work {
     if (d->layout == MC_NHWC || d->S == 1 || C == 1) {
       unpack_rows_kernel<<<grid_for(r.rows * C, 256), 256, 0, st>>>((const bf16*)r.p, (bf16*)p, r.rows, C, r.ld), MC_COUNT(1);
     } else {
-      const long long ts = (d->S + 63) / 64, tc = (C + 63) / 64;
-      rows_to_planes_kernel<<<(unsigned)(d->B * ts * tc), 256, 0, st>>>((const bf16*)r.p, (bf16*)p, d->S, C, r.ld, (int)ts,
-                                                                        (int)tc), MC_COUNT(1);
+      planes(d, C, [&](auto ct, unsigned blocks, int ts, int tc) {
+        rows_to_planes_kernel<decltype(ct)::value><<<blocks, 256, 0, st>>>((const bf16*)r.p, (bf16*)p, d->S, C, r.ld, ts, tc);
+      });
     }
     did(cudaGetLastError() == cudaSuccess ? MC_OK : MC_ERR_LAUNCH);
   }
@@ -359,7 +416,8 @@ int mc_pointwise_bwd(const mc_mix_desc* d, const void* gy, const void* x, const 
   if (d->act != MC_ACT_NONE) {
     rc = by_type(d->dtype, [&](auto t) {
       typedef decltype(t) T;
-      act_bwd_kernel<T><<<grid_for(n, 256), 256, 0, st>>>((const T*)gy, (const T*)saved, (T*)gz, n, d->act), MC_COUNT(1);
+      act_bwd_kernel<T><<<grid_for(n / (16 / (long)sizeof(T)) + 1, 256), 256, 0, st>>>(
+          (const T*)gy, (const T*)saved, (T*)gz, n, d->act, aligned16(gy) && aligned16(saved)), MC_COUNT(1);
     });
     if (rc) return rc;
     g = gz;

@@ -194,7 +194,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 ? 2 : 1) rows_kernel(const
         const T bj = bias ? bias[n0 + n] : T(0);
         T v[4], o[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = acc[4 * h + e][j] + bj, o[e] = act_value<T>(a.act, v[e]);
+        for (int e = 0; e < 4; ++e) v[e] = acc[4 * h + e][j] + bj, o[e] = a.act ? act_value_call<T>(a.act, v[e]) : v[e];
         if (whole) {
           const long long c = n0 + n;
           if (z) store_run(z + b * a.z.img + s * a.z.pix + c * a.z.ch, a.z.pix, v, 4, f.vec_z);
@@ -239,7 +239,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 ? 2 : 1) rows_kernel(const
 #pragma unroll
         for (int e = 0; e < W; ++e) {
           v[e] = acc[i][W * h + e] + (bias && e < left ? bias[c + e] : T(0));
-          o[e] = act_value<T>(a.act, v[e]);
+          o[e] = a.act ? act_value_call<T>(a.act, v[e]) : v[e];
         }
         if (z) store_run(zr + c * a.z.ch, a.z.ch, v, left, f.vec_z);
         if (res) {
@@ -255,7 +255,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 ? 2 : 1) rows_kernel(const
         for (int e = 0; e < W; ++e) {
           v[e] = acc[i][e] + (bias && e < left ? bias[c + e] : T(0));
           u[e] = acc[i][W + e] + (bias && e < left ? bias[a.N + c + e] : T(0));
-          o[e] = act_value<T>(a.act, v[e]) * u[e];
+          o[e] = act_value_call<T>(a.act, v[e]) * u[e];
         }
         if (z) {
           store_run(zr + c * a.z.ch, a.z.ch, v, left, f.vec_z);
@@ -268,8 +268,9 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 ? 2 : 1) rows_kernel(const
         load_run(rr + (a.N + c) * a.res.ch, a.res.ch, u, left, f.vec_r);
 #pragma unroll
         for (int e = 0; e < W; ++e) {
-          v[e] = acc[i][W * h + e] * u[e] * act_slope<T>(a.act, g[e]);
-          o[e] = acc[i][W * h + e] * act_value<T>(a.act, g[e]);
+          const ActBoth<T> f = act_both_call<T>(a.act, g[e]);
+          v[e] = acc[i][W * h + e] * u[e] * f.slope;
+          o[e] = acc[i][W * h + e] * f.value;
         }
         store_run(yr + c * a.y.ch, a.y.ch, v, left, f.vec_y);
         store_run(yr + (a.N + c) * a.y.ch, a.y.ch, o, left, f.vec_y);

@@ -928,11 +928,20 @@ static int launch_rows(GemmArgs& g, cudaStream_t st) {
   return launch_pairs(rows_tc_kernel<MODE, BN>, (unsigned)n, smem, g, st);
 }
 
-// Channels of a tile: the smallest of 64, 128, 256 that holds all of them, else the one that pads least.
-static int tile_width(int n) {
-  if (n <= 64) return 64;
-  if (n <= 128) return 128;
-  return (n + 255) / 256 * 256 <= (n + 127) / 128 * 128 + 64 ? 256 : 128;
+// Channels of a tile, for `pairs` pixel tiles, n channels, kb stages: the least estimated time.  A tile costs its MMAs
+// (half a cycle per column and 16 channels, not less than its stages' hand-over), its read-out and a start; many pixels
+// want wide tiles, few pixels so many tiles that every pair of blocks has one (680 -> 256 channels at 2 562 pixels, 11
+// pixel tiles: 14.2 us with one tile of 256 columns each).
+static int tile_width(long long pairs, int n, int kb) {
+  const int all = sm_total() / 2;
+  int best = 64;
+  double least = 1e300;
+  for (int w = 64; w <= 256; w *= 2) {
+    const double tiles = (double)pairs * ((n + w - 1) / w), waves = tiles <= all ? 1 : tiles / all;
+    const double t = waves * (1500 + kb * (w > 150 ? 2.0 * w : 300.0) + 16.0 * w);
+    if (t < least) least = t, best = w;
+  }
+  return best;
 }
 static int kblocks(int c) { return (c + KB - 1) / KB; }
 
@@ -957,7 +966,7 @@ int tc_layer(const TcRows& a, const TcRows& w, const bf16* bias, int act, const 
              bool backward, cudaStream_t st) {
   GemmArgs g = base_args(a, y, bias, act);
   g.res = r.p != nullptr;
-  const int bn = tile_width(y.cols);
+  const int bn = tile_width(g.m_pairs, y.cols, g.kb[0]);
   if (!encode(&g.a[0], a, TILE) || !encode(&g.b[0], w, bn / 2) || !encode(&g.y[0], y, TILE)) return MC_ERR_LAUNCH;
   if (g.res && !encode(&g.r, r, TILE)) return MC_ERR_LAUNCH;
   return backward ? launch_wide<ACT_BWD>(g, bn, st) : launch_wide<LAYER>(g, bn, st);
@@ -966,12 +975,10 @@ int tc_layer(const TcRows& a, const TcRows& w, const bf16* bias, int act, const 
 int tc_input_grad(const TcRows& g0, const TcRows& w0, const TcRows& g1, const TcRows& w1, const TcRows& gx,
                   cudaStream_t st) {
   GemmArgs g = base_args(g0, gx, nullptr, MC_ACT_NONE);
-  const int bn = tile_width(gx.cols);
+  if (g1.p) g.kb[1] = kblocks(g1.cols);
+  const int bn = tile_width(g.m_pairs, gx.cols, g.kb[0] + g.kb[1]);
   if (!encode(&g.a[0], g0, TILE) || !encode(&g.b[0], w0, bn / 2) || !encode(&g.y[0], gx, TILE)) return MC_ERR_LAUNCH;
-  if (g1.p) {
-    g.kb[1] = kblocks(g1.cols);
-    if (!encode(&g.a[1], g1, TILE) || !encode(&g.b[1], w1, bn / 2)) return MC_ERR_LAUNCH;
-  }
+  if (g1.p && (!encode(&g.a[1], g1, TILE) || !encode(&g.b[1], w1, bn / 2))) return MC_ERR_LAUNCH;
   return launch_wide<LAYER>(g, bn, st);
 }
 
