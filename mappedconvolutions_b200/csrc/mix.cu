@@ -143,8 +143,8 @@ __global__ void __launch_bounds__(256) unpack_rows_kernel(const bf16* __restrict
     dst[i] = src[r * ld + (i - r * C)];
   }
 }
-// (B, C, S) <-> rows of ld channels (zeros behind the last one): CT channels x 4096 / CT pixels at a time through shared
-// memory.  The planes are read and written value by value, neighbouring threads at neighbouring pixels, because with an
+// (B, C, S) -> rows of ld channels (zeros behind the last one): CT channels x 4096 / CT pixels at a time through shared
+// memory.  The planes are read value by value, neighbouring threads at neighbouring pixels, because with an
 // odd number of pixels they start anywhere; sixteen values per thread are on their way at once.  64 channels of
 // 8 x 125 x 251 pixels to rows: 35 us with the general transpose.
 template <int CT>
@@ -171,30 +171,6 @@ __global__ void __launch_bounds__(256) planes_to_rows_kernel(const bf16* __restr
     *reinterpret_cast<uint4*>(dst + (b * S + s0 + r) * ld + c0 + j) = make_uint4(w[0], w[1], w[2], w[3]);
   }
 }
-template <int CT>
-__global__ void __launch_bounds__(256) rows_to_planes_kernel(const bf16* __restrict__ src, bf16* __restrict__ dst,
-                                                             long long S, int C, int ld, int tiles_s, int tiles_c) {
-  constexpr int PX = 4096 / CT, PITCH = CT + 2;
-  __shared__ __align__(16) bf16 tile[PX * PITCH];
-  const int tc = blockIdx.x % tiles_c, ts = blockIdx.x / tiles_c % tiles_s, c0 = tc * CT;
-  const long long b = blockIdx.x / tiles_c / tiles_s, s0 = (long long)ts * PX;
-#pragma unroll
-  for (int i = threadIdx.x; i < 512; i += 256) {
-    const int r = i / (CT / 8), j = i % (CT / 8) * 8;
-    uint4 v = make_uint4(0, 0, 0, 0);
-    if (s0 + r < S && c0 + j < ld) v = __ldcs(reinterpret_cast<const uint4*>(src + (b * S + s0 + r) * ld + c0 + j));
-    uint32_t* w = reinterpret_cast<uint32_t*>(tile + r * PITCH + j);
-    w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
-  }
-  __syncthreads();
-  const int s = threadIdx.x % PX, c = threadIdx.x / PX;
-  bf16* to = dst + (b * C + c0 + c) * S + s0 + s;
-#pragma unroll
-  for (int i = 0; i < 16; ++i)
-    if (s0 + s < S && c0 + c + i * (256 / PX) < C)
-      to[(long long)i * (256 / PX) * S] = tile[s * PITCH + c + i * (256 / PX)];
-}
-
 // Lays a call's temporary tensors out in the workspace; without a workspace it only adds up their sizes.
 struct Work {
   char* base;
@@ -215,16 +191,21 @@ struct Work {
     const long long P = pixels(d);
     if (in_place(d, C)) return TcRows{p, P, C, C};
     const TcRows r = fresh(P, C);
-    if (!run() || !p) return p || !base ? r : TcRows{nullptr, P, C, C};
+    if (!p && base) return TcRows{nullptr, P, C, C};
+    lay_out(d, p, r);
+    return r;
+  }
+  void lay_out(const mc_mix_desc* d, const void* p, const TcRows& r) {
+    if (!run()) return;
+    const int C = r.cols;
     if (d->layout == MC_NHWC || d->S == 1 || C == 1) {
-      pack_rows_kernel<<<grid_for(P * (r.ld / 8), 256), 256, 0, st>>>((const bf16*)p, (bf16*)r.p, P, C, r.ld), MC_COUNT(1);
+      pack_rows_kernel<<<grid_for(r.rows * (r.ld / 8), 256), 256, 0, st>>>((const bf16*)p, (bf16*)r.p, r.rows, C, r.ld), MC_COUNT(1);
       did(cudaGetLastError() == cudaSuccess ? MC_OK : MC_ERR_LAUNCH);
     } else {
       planes(d, C, [&](auto ct, unsigned blocks, int ts, int tc) {
         planes_to_rows_kernel<decltype(ct)::value><<<blocks, 256, 0, st>>>((const bf16*)p, (bf16*)r.p, d->S, C, r.ld, ts, tc);
       });
     }
-    return r;
   }
   // f(channels of a tile, blocks, tiles along S, tiles along C): 16 channels where there are no more
   template <typename F>
@@ -252,19 +233,19 @@ struct Work {
     if (run()) did(mc_transpose(2, n, R, C, p, (void*)r.p, r.ld, st));
     return TcRows{r.p, C, R, r.ld};
   }
-  // where an activation is computed as rows, and its way to where it belongs
+  // where a layer leaves an activation: where it belongs (rows in place, planes), or rows that put() brings there
+  static bool as_planes(const mc_mix_desc* d, int C) { return d->layout == MC_NCHW && d->S > 1 && C > 1; }
   TcRows out(const mc_mix_desc* d, void* p, int C) {
-    return in_place(d, C) ? TcRows{p, pixels(d), C, C} : fresh(pixels(d), C);
+    if (in_place(d, C)) return TcRows{p, pixels(d), C, C};
+    return as_planes(d, C) ? TcRows{p, pixels(d), C, 0, d->S} : fresh(pixels(d), C);
+  }
+  // a residual, laid out as the output that it is added to
+  TcRows added(const mc_mix_desc* d, const void* p, int C) {
+    return as_planes(d, C) ? TcRows{p, pixels(d), C, 0, d->S} : in(d, p, C);
   }
   void put(const mc_mix_desc* d, const TcRows& r, void* p, int C) {
-    if (!run() || in_place(d, C)) return;
-    if (d->layout == MC_NHWC || d->S == 1 || C == 1) {
-      unpack_rows_kernel<<<grid_for(r.rows * C, 256), 256, 0, st>>>((const bf16*)r.p, (bf16*)p, r.rows, C, r.ld), MC_COUNT(1);
-    } else {
-      planes(d, C, [&](auto ct, unsigned blocks, int ts, int tc) {
-        rows_to_planes_kernel<decltype(ct)::value><<<blocks, 256, 0, st>>>((const bf16*)r.p, (bf16*)p, d->S, C, r.ld, ts, tc);
-      });
-    }
+    if (!run() || r.p == p) return;
+    unpack_rows_kernel<<<grid_for(r.rows * C, 256), 256, 0, st>>>((const bf16*)r.p, (bf16*)p, r.rows, C, r.ld), MC_COUNT(1);
     did(cudaGetLastError() == cudaSuccess ? MC_OK : MC_ERR_LAUNCH);
   }
   void param_grads(const TcRows& g0, const TcRows& g1, int segs, const TcRows& x, void* gw, void* gb) {
@@ -283,17 +264,32 @@ struct Work {
   }
 };
 
+static size_t input_rows_bytes(const mc_mix_desc* d) {
+  return Work::in_place(d, d->C_in) ? 0 : up256((size_t)pixels(d) * pad8(d->C_in) * 2);
+}
+// The input as rows: laid out at `kept` by a forward call (which may be null), found there by a backward call.
+static TcRows input_rows(Work& k, const mc_mix_desc* d, const void* x, void* kept) {
+  if (Work::in_place(d, d->C_in) || !kept) return k.in(d, x, d->C_in);
+  const TcRows r{kept, pixels(d), d->C_in, pad8(d->C_in)};
+  k.lay_out(d, x, r);
+  return r;
+}
+static TcRows kept_rows(const mc_mix_desc* d, const void* x, const void* kept) {
+  if (Work::in_place(d, d->C_in)) return TcRows{x, pixels(d), d->C_in, d->C_in};
+  return TcRows{kept, pixels(d), d->C_in, pad8(d->C_in)};
+}
+
 static void tc_pointwise_fwd(Work& k, const mc_mix_desc* d, const void* x, const void* w, const void* bias,
-                             const void* residual, void* y) {
-  const TcRows xr = k.in(d, x, d->C_in), wr = k.weight(w, d->C_out, d->C_in), rr = k.in(d, residual, d->C_out);
+                             const void* residual, void* y, void* saved) {
+  const TcRows xr = input_rows(k, d, x, saved), wr = k.weight(w, d->C_out, d->C_in), rr = k.added(d, residual, d->C_out);
   const TcRows yr = k.out(d, y, d->C_out);
   if (k.run()) k.did(tc_layer(xr, wr, (const bf16*)bias, d->act, rr, yr, false, k.st));
   k.put(d, yr, y, d->C_out);
 }
 
 static void tc_pointwise_bwd(Work& k, const mc_mix_desc* d, const void* gy, const void* x, const void* w,
-                             const void* bias, void* gx, void* gw, void* gb) {
-  const TcRows xr = k.in(d, x, d->C_in), gyr = k.in(d, gy, d->C_out);
+                             const void* bias, const void* saved, void* gx, void* gw, void* gb) {
+  const TcRows xr = kept_rows(d, x, saved), gyr = k.in(d, gy, d->C_out);
   TcRows gz = gyr;
   if (d->act != MC_ACT_NONE) {
     const TcRows wr = k.weight(w, d->C_out, d->C_in);
@@ -311,10 +307,12 @@ static void tc_pointwise_bwd(Work& k, const mc_mix_desc* d, const void* gy, cons
 static void tc_gated_fwd(Work& k, const mc_mix_desc* d, const void* x, const void* w_in, const void* b_in,
                          const void* w_out, const void* b_out, const void* residual, void* y, void* saved) {
   const int H = d->hidden;
-  const TcRows xr = k.in(d, x, d->C_in), wi = k.weight(w_in, 2 * H, d->C_in), wo = k.weight(w_out, d->C_out, H);
+  const size_t hb = up256((size_t)pixels(d) * pad8(H) * 2);
+  const TcRows xr = input_rows(k, d, x, saved ? (char*)saved + hb : nullptr);
+  const TcRows wi = k.weight(w_in, 2 * H, d->C_in), wo = k.weight(w_out, d->C_out, H);
   const TcRows h = saved ? TcRows{saved, pixels(d), H, pad8(H)} : k.fresh(pixels(d), H);
   if (k.run()) k.did(tc_gate(xr, wi, (const bf16*)b_in, d->act, h, k.st));
-  const TcRows rr = k.in(d, residual, d->C_out), yr = k.out(d, y, d->C_out);
+  const TcRows rr = k.added(d, residual, d->C_out), yr = k.out(d, y, d->C_out);
   if (k.run()) k.did(tc_layer(h, wo, (const bf16*)b_out, MC_ACT_NONE, rr, yr, false, k.st));
   k.put(d, yr, y, d->C_out);
 }
@@ -323,7 +321,8 @@ static void tc_gated_bwd(Work& k, const mc_mix_desc* d, const void* gy, const vo
                          const void* w_out, const void* saved, void* gx, void* gw_in, void* gb_in, void* gw_out,
                          void* gb_out) {
   const int H = d->hidden;
-  const TcRows xr = k.in(d, x, d->C_in), wi = k.weight(w_in, 2 * H, d->C_in), wot = k.weight_t(w_out, d->C_out, H);
+  const TcRows xr = kept_rows(d, x, (const char*)saved + up256((size_t)pixels(d) * pad8(H) * 2));
+  const TcRows wi = k.weight(w_in, 2 * H, d->C_in), wot = k.weight_t(w_out, d->C_out, H);
   const TcRows gyr = k.in(d, gy, d->C_out), gg = k.fresh(pixels(d), H), gu = k.fresh(pixels(d), H);
   if (k.run() && (gx || gw_in || gb_in)) k.did(tc_gate_bwd(xr, wi, (const bf16*)b_in, d->act, gyr, wot, gg, gu, k.st));
   if (gx || !k.base) {
@@ -354,8 +353,11 @@ extern "C" {
 
 // ---- pointwise layer ----------------------------------------------------------------------------------------
 
+// kept for the backward pass: z in y's layout; bf16: the input as rows, where it is not rows already
 size_t mc_pointwise_saved_bytes(const mc_mix_desc* d) {
-  if (check_desc(d, false) || d->act == MC_ACT_NONE || d->dtype == MC_BF16) return 0;
+  if (check_desc(d, false)) return 0;
+  if (d->dtype == MC_BF16) return input_rows_bytes(d);
+  if (d->act == MC_ACT_NONE) return 0;
   return up256((size_t)pixels(d) * d->C_out * esize(d->dtype));
 }
 
@@ -364,8 +366,10 @@ size_t mc_pointwise_workspace_bytes(const mc_mix_desc* d, int32_t phase) {
   if (check_desc(d, false)) return 0;
   if (d->dtype == MC_BF16)
     return work_size([&](Work& k) {
-      if (backward) tc_pointwise_bwd(k, d, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr);
-      else tc_pointwise_fwd(k, d, nullptr, nullptr, nullptr, nullptr, nullptr);
+      if (backward) tc_pointwise_bwd(k, d, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr);
+      else
+        tc_pointwise_fwd(k, d, nullptr, nullptr, nullptr, nullptr, nullptr,
+                         phase == MC_PHASE_KEEP ? (void*)256 : nullptr);  // (not touched: only sizes are added up)
     });
   if (!backward) return 0;
   const Shares s = shares_of(d, d->C_out, d->C_in);
@@ -380,9 +384,10 @@ int mc_pointwise_fwd(const mc_mix_desc* d, const void* x, const void* w, const v
   const size_t need = mc_pointwise_workspace_bytes(d, saved ? MC_PHASE_KEEP : MC_PHASE_FORWARD);
   if (need && (!ws || ws_bytes < need)) return MC_ERR_WORKSPACE;
   if (d->dtype == MC_BF16) {
-    if (!aligned16(x) || !aligned16(w) || !aligned16(residual) || !aligned16(y) || !aligned16(ws)) return MC_ERR_BAD_ARG;
+    if (!aligned16(x) || !aligned16(w) || !aligned16(residual) || !aligned16(y) || !aligned16(saved) || !aligned16(ws))
+      return MC_ERR_BAD_ARG;
     Work k{(char*)ws, (cudaStream_t)stream};
-    tc_pointwise_fwd(k, d, x, w, bias, residual, y);
+    tc_pointwise_fwd(k, d, x, w, bias, residual, y, input_rows_bytes(d) ? saved : nullptr);
     return k.rc;
   }
   RowsArgs r{};
@@ -402,9 +407,10 @@ int mc_pointwise_bwd(const mc_mix_desc* d, const void* gy, const void* x, const 
   if (!gy || !x || !w || (mc_pointwise_saved_bytes(d) && !saved)) return MC_ERR_BAD_ARG;
   if (!ws || ws_bytes < mc_pointwise_workspace_bytes(d, MC_PHASE_BACKWARD)) return MC_ERR_WORKSPACE;
   if (d->dtype == MC_BF16) {
-    if (!aligned16(gy) || !aligned16(x) || !aligned16(w) || !aligned16(gx) || !aligned16(ws)) return MC_ERR_BAD_ARG;
+    if (!aligned16(gy) || !aligned16(x) || !aligned16(w) || !aligned16(saved) || !aligned16(gx) || !aligned16(ws))
+      return MC_ERR_BAD_ARG;
     Work k{(char*)ws, (cudaStream_t)stream};
-    tc_pointwise_bwd(k, d, gy, x, w, bias, gx, gw, gb);
+    tc_pointwise_bwd(k, d, gy, x, w, bias, saved, gx, gw, gb);
     return k.rc;
   }
   cudaStream_t st = (cudaStream_t)stream;
@@ -439,10 +445,11 @@ int mc_pointwise_bwd(const mc_mix_desc* d, const void* gy, const void* x, const 
 
 // ---- gated feed-forward block -----------------------------------------------------------------------------------
 
-// kept for the backward pass: [g|u] (P, 2 H), then h (P, H); bf16: h in padded rows
+// kept for the backward pass: [g|u] (P, 2 H), then h (P, H); bf16: h in padded rows, then the input as
+// rows where it is not rows already
 size_t mc_gated_saved_bytes(const mc_mix_desc* d) {
   if (check_desc(d, true)) return 0;
-  if (d->dtype == MC_BF16) return up256((size_t)pixels(d) * pad8(d->hidden) * 2);
+  if (d->dtype == MC_BF16) return up256((size_t)pixels(d) * pad8(d->hidden) * 2) + input_rows_bytes(d);
   const size_t h = (size_t)pixels(d) * d->hidden * esize(d->dtype);
   return up256(2 * h) + up256(h);
 }

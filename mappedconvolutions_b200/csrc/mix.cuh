@@ -31,6 +31,7 @@ inline View row_view(const void* p, long long S, long long ld) { return View{p, 
 struct PixDiv {
   uint32_t S, m;
   int l;
+  PixDiv() = default;
   __host__ explicit PixDiv(uint32_t s) : S(s), l(0) {
     while ((1ull << l) < s) ++l;
     m = (uint32_t)(((1ull << (31 + l)) + s - 1) / s);
@@ -135,7 +136,8 @@ int simt_outer_launch(int dtype, const OuterArgs& a, cudaStream_t st);
 struct TcRows {
   const void* p;
   long long rows;
-  int cols, ld;
+  int cols, ld;  // ld == 0: an NCHW tensor with S pixels an image, as output (and residual) of a layer only
+  long long S = 0;
 };
 // y = act(a w^T + bias) + r, or with backward y = r act'(a w^T + bias); w (N, K), r.p may be null (not with backward)
 int tc_layer(const TcRows& a, const TcRows& w, const bf16* bias, int act, const TcRows& r, const TcRows& y, bool backward,

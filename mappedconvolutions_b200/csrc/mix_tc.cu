@@ -208,6 +208,13 @@ __device__ __forceinline__ bool mbar_test(uint32_t bar, uint32_t parity) {
   return ok != 0;
 }
 
+// The kernels here may be launched while the one before them is still running: what they set up first touches no memory of
+// others, and here they wait until all of it is written.  (The next kernel may start likewise.)
+__device__ __forceinline__ void behind_previous_kernel() {
+  asm volatile("griddepcontrol.launch_dependents;");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+
 // ---- pairs of blocks -----------------------------------------------------------------------------------
 __device__ __forceinline__ uint32_t cluster_rank() {
   uint32_t r;
@@ -314,6 +321,10 @@ struct alignas(64) GemmArgs {
   int n_tiles, N, kb[2], act;
   int up;            // distance between a gate's row of b[0] and bias and its factor's
   int res;           // r is read
+  // LAYER: y (and r) in NCHW, written and read by the read-out warps themselves: their lanes are neighbouring pixels
+  bf16* planes;
+  const bf16* planes_r;
+  PixDiv pd;
   int group;         // channel tiles of a pair of blocks whose weights stay in shared memory, 0: none do
   int stages, slots;
 };
@@ -362,6 +373,11 @@ __device__ __forceinline__ void load_b(const GemmArgs& g, int seg, uint32_t rank
 // Offsets of the barriers behind bfull.
 constexpr uint32_t BAR_TFULL = 8, BAR_TEMPTY = 24, BAR_READY = 40, BAR_DONE = 72, BAR_DRAIN = 104, BAR_BIASED = 112;
 
+// 2-byte accesses of 32 lanes at neighbouring pixels
+__device__ __forceinline__ float plane_value(const bf16* p) {
+  return __bfloat162float(__ushort_as_bfloat16(__ldg(reinterpret_cast<const unsigned short*>(p))));
+}
+
 // Read-out warps of one accumulator set: thread = pixel.  Sixteen channels at a time in a loop that is not unrolled: the
 // code of a whole tile does not stay in the instruction cache, and then fetching it takes longer than running it.
 template <int MODE, int BN, typename Act>
@@ -403,6 +419,15 @@ __device__ __forceinline__ void read_out(const GemmArgs& g, int set, uint32_t ra
     }
     if (!warp_wait(tfull, it & 1, abort_flag, 0x131)) return;
     tc_fence_after_sync();
+    long long plane0 = -1;  // this pixel of channel n0 of the NCHW output
+    if (MODE == LAYER && g.planes) {
+      const uint32_t p = (w.m() * 2 + rank) * TILE + row;
+      if (p < (uint32_t)g.rows) {
+        uint32_t im, s;
+        g.pd.split(p, im, s);
+        plane0 = ((long long)im * g.N + w.nt() * BN) * g.pd.S + s;
+      }
+    }
     constexpr int NL = MODE == GATE_BWD ? 3 : MODE == GATE ? 2 : 1;
     uint32_t v[2][NL][16];
     const auto fetch = [&](uint32_t (&d)[NL][16], int p) {
@@ -432,6 +457,22 @@ __device__ __forceinline__ void read_out(const GemmArgs& g, int set, uint32_t ra
         o[j] = mul2(mul2(gh, u), o[j]);
         z[j] = mul2(gh, z[j]);
         r1[j] = pack_bf16x2(z[j].x, z[j].y);
+      }
+      if (MODE == LAYER && g.planes) {
+        if (plane0 >= 0) {
+          const int left = g.N - w.nt() * BN - 16 * p;
+          const long long at = plane0 + 16ll * p * g.pd.S;
+          if (g.planes_r) {
+            float r[16];
+#pragma unroll
+            for (int j = 0; j < 16; ++j) r[j] = j < left ? plane_value(g.planes_r + at + (long long)j * g.pd.S) : 0.f;
+            MC_EACH z[j] = add2(z[j], make_float2(r[2 * j], r[2 * j + 1]));
+          }
+#pragma unroll
+          for (int j = 0; j < 16; ++j)
+            if (j < left) g.planes[at + (long long)j * g.pd.S] = __float2bfloat16_rn(j & 1 ? z[j / 2].y : z[j / 2].x);
+        }
+        return true;
       }
       const uint32_t j0 = p % PER * 2;
       if (p % PER == 0) {
@@ -515,6 +556,7 @@ __global__ void __launch_bounds__(THREADS, 1) rows_tc_kernel(const __grid_consta
     fence_proxy_async_smem();
   }
   if (warp == 1) pair_alloc(smem_u32(tmem_s), 512);
+  behind_previous_kernel();
   tc_fence_before_sync();
   __syncthreads();
   cluster_sync();
@@ -609,7 +651,7 @@ __global__ void __launch_bounds__(THREADS, 1) rows_tc_kernel(const __grid_consta
     }
   } else if (warp < 4) {
     // ---- I/O of one set's staged tiles: fill the slots ahead (residual), store what the read-out warps leave in them
-    if (lane == 0) {
+    if (lane == 0 && !(MODE == LAYER && g.planes)) {
       const int set = warp - 2;
       TileWalk lead(g, set, 2);
       int lead_c = 0;
@@ -709,6 +751,7 @@ __global__ void __launch_bounds__(THREADS, 1) outer_tc_kernel(const __grid_const
     fence_proxy_async_smem();
   }
   if (warp == 1) pair_alloc(smem_u32(&tmem_s), MT * BN);
+  behind_previous_kernel();
   tc_fence_before_sync();
   __syncthreads();
   cluster_sync();
@@ -874,16 +917,18 @@ static bool allow_smem(Kern kern) {
 template <typename Kern, typename Args>
 static int launch_pairs(Kern kern, unsigned pairs, size_t smem, const Args& args, cudaStream_t st) {
   if (!allow_smem(kern)) return MC_ERR_LAUNCH;
-  cudaLaunchAttribute attr = {};
-  attr.id = cudaLaunchAttributeClusterDimension;
-  attr.val.clusterDim.x = 2, attr.val.clusterDim.y = 1, attr.val.clusterDim.z = 1;
+  cudaLaunchAttribute attr[2] = {};
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 2, attr[0].val.clusterDim.y = 1, attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(2 * pairs);
   cfg.blockDim = dim3(THREADS);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
   if (cudaLaunchKernelEx(&cfg, kern, args) != cudaSuccess) return MC_ERR_LAUNCH;
   MC_COUNT(1);
   return MC_OK;
@@ -965,6 +1010,12 @@ static int launch_wide(GemmArgs& g, int bn, cudaStream_t st) {
 int tc_layer(const TcRows& a, const TcRows& w, const bf16* bias, int act, const TcRows& r, const TcRows& y,
              bool backward, cudaStream_t st) {
   GemmArgs g = base_args(a, y, bias, act);
+  if (y.ld == 0) {  // NCHW
+    g.planes = (bf16*)y.p, g.planes_r = (const bf16*)r.p, g.pd = PixDiv((uint32_t)y.S);
+    const int bn = tile_width(g.m_pairs, y.cols, g.kb[0]);
+    if (!encode(&g.a[0], a, TILE) || !encode(&g.b[0], w, bn / 2)) return MC_ERR_LAUNCH;
+    return launch_wide<LAYER>(g, bn, st);
+  }
   g.res = r.p != nullptr;
   const int bn = tile_width(g.m_pairs, y.cols, g.kb[0]);
   if (!encode(&g.a[0], a, TILE) || !encode(&g.b[0], w, bn / 2) || !encode(&g.y[0], y, TILE)) return MC_ERR_LAUNCH;
@@ -977,7 +1028,9 @@ int tc_input_grad(const TcRows& g0, const TcRows& w0, const TcRows& g1, const Tc
   GemmArgs g = base_args(g0, gx, nullptr, MC_ACT_NONE);
   if (g1.p) g.kb[1] = kblocks(g1.cols);
   const int bn = tile_width(g.m_pairs, gx.cols, g.kb[0] + g.kb[1]);
-  if (!encode(&g.a[0], g0, TILE) || !encode(&g.b[0], w0, bn / 2) || !encode(&g.y[0], gx, TILE)) return MC_ERR_LAUNCH;
+  if (!encode(&g.a[0], g0, TILE) || !encode(&g.b[0], w0, bn / 2)) return MC_ERR_LAUNCH;
+  if (gx.ld == 0) g.planes = (bf16*)gx.p, g.pd = PixDiv((uint32_t)gx.S);
+  else if (!encode(&g.y[0], gx, TILE)) return MC_ERR_LAUNCH;
   if (g1.p && (!encode(&g.a[1], g1, TILE) || !encode(&g.b[1], w1, bn / 2))) return MC_ERR_LAUNCH;
   return launch_wide<LAYER>(g, bn, st);
 }
