@@ -239,10 +239,6 @@ struct Work {
     if (in_place(d, C)) return TcRows{p, pixels(d), C, C};
     return as_planes(d, C) ? TcRows{p, pixels(d), C, 0, d->S} : fresh(pixels(d), C);
   }
-  // a residual, laid out as the output that it is added to
-  TcRows added(const mc_mix_desc* d, const void* p, int C) {
-    return as_planes(d, C) ? TcRows{p, pixels(d), C, 0, d->S} : in(d, p, C);
-  }
   void put(const mc_mix_desc* d, const TcRows& r, void* p, int C) {
     if (!run() || r.p == p) return;
     unpack_rows_kernel<<<grid_for(r.rows * C, 256), 256, 0, st>>>((const bf16*)r.p, (bf16*)p, r.rows, C, r.ld), MC_COUNT(1);
@@ -281,7 +277,7 @@ static TcRows kept_rows(const mc_mix_desc* d, const void* x, const void* kept) {
 
 static void tc_pointwise_fwd(Work& k, const mc_mix_desc* d, const void* x, const void* w, const void* bias,
                              const void* residual, void* y, void* saved) {
-  const TcRows xr = input_rows(k, d, x, saved), wr = k.weight(w, d->C_out, d->C_in), rr = k.added(d, residual, d->C_out);
+  const TcRows xr = input_rows(k, d, x, saved), wr = k.weight(w, d->C_out, d->C_in), rr = k.in(d, residual, d->C_out);
   const TcRows yr = k.out(d, y, d->C_out);
   if (k.run()) k.did(tc_layer(xr, wr, (const bf16*)bias, d->act, rr, yr, false, k.st));
   k.put(d, yr, y, d->C_out);
@@ -312,7 +308,7 @@ static void tc_gated_fwd(Work& k, const mc_mix_desc* d, const void* x, const voi
   const TcRows wi = k.weight(w_in, 2 * H, d->C_in), wo = k.weight(w_out, d->C_out, H);
   const TcRows h = saved ? TcRows{saved, pixels(d), H, pad8(H)} : k.fresh(pixels(d), H);
   if (k.run()) k.did(tc_gate(xr, wi, (const bf16*)b_in, d->act, h, k.st));
-  const TcRows rr = k.added(d, residual, d->C_out), yr = k.out(d, y, d->C_out);
+  const TcRows rr = k.in(d, residual, d->C_out), yr = k.out(d, y, d->C_out);
   if (k.run()) k.did(tc_layer(h, wo, (const bf16*)b_out, MC_ACT_NONE, rr, yr, false, k.st));
   k.put(d, yr, y, d->C_out);
 }

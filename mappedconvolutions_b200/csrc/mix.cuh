@@ -136,7 +136,7 @@ int simt_outer_launch(int dtype, const OuterArgs& a, cudaStream_t st);
 struct TcRows {
   const void* p;
   long long rows;
-  int cols, ld;  // ld == 0: an NCHW tensor with S pixels an image, as output (and residual) of a layer only
+  int cols, ld;  // ld == 0: an NCHW tensor with S pixels an image, as output of a layer or input gradient only
   long long S = 0;
 };
 // y = act(a w^T + bias) + r, or with backward y = r act'(a w^T + bias); w (N, K), r.p may be null (not with backward)

@@ -321,9 +321,9 @@ struct alignas(64) GemmArgs {
   int n_tiles, N, kb[2], act;
   int up;            // distance between a gate's row of b[0] and bias and its factor's
   int res;           // r is read
-  // LAYER: y (and r) in NCHW, written and read by the read-out warps themselves: their lanes are neighbouring pixels
+  // LAYER: y in NCHW, written by the read-out warps themselves, whose lanes are neighbouring pixels.  (A residual comes as
+  // rows all the same: read here from planes, a piece ahead, its latency made the kernel twice as slow.)
   bf16* planes;
-  const bf16* planes_r;
   PixDiv pd;
   int group;         // channel tiles of a pair of blocks whose weights stay in shared memory, 0: none do
   int stages, slots;
@@ -373,11 +373,6 @@ __device__ __forceinline__ void load_b(const GemmArgs& g, int seg, uint32_t rank
 // Offsets of the barriers behind bfull.
 constexpr uint32_t BAR_TFULL = 8, BAR_TEMPTY = 24, BAR_READY = 40, BAR_DONE = 72, BAR_DRAIN = 104, BAR_BIASED = 112;
 
-// 2-byte accesses of 32 lanes at neighbouring pixels
-__device__ __forceinline__ float plane_value(const bf16* p) {
-  return __bfloat162float(__ushort_as_bfloat16(__ldg(reinterpret_cast<const unsigned short*>(p))));
-}
-
 // Read-out warps of one accumulator set: thread = pixel.  Sixteen channels at a time in a loop that is not unrolled: the
 // code of a whole tile does not stay in the instruction cache, and then fetching it takes longer than running it.
 template <int MODE, int BN, typename Act>
@@ -417,8 +412,6 @@ __device__ __forceinline__ void read_out(const GemmArgs& g, int set, uint32_t ra
       if (lane == 0) mbar_arrive(bfull + BAR_BIASED + 8 * set);
       if (!warp_wait(bfull + BAR_BIASED + 8 * set, it & 1, abort_flag, 0x133)) return;  // (bounded, unlike bar.sync)
     }
-    if (!warp_wait(tfull, it & 1, abort_flag, 0x131)) return;
-    tc_fence_after_sync();
     long long plane0 = -1;  // this pixel of channel n0 of the NCHW output
     if (MODE == LAYER && g.planes) {
       const uint32_t p = (w.m() * 2 + rank) * TILE + row;
@@ -430,16 +423,19 @@ __device__ __forceinline__ void read_out(const GemmArgs& g, int set, uint32_t ra
     }
     constexpr int NL = MODE == GATE_BWD ? 3 : MODE == GATE ? 2 : 1;
     uint32_t v[2][NL][16];
+    if (!warp_wait(tfull, it & 1, abort_flag, 0x131)) return;
+    tc_fence_after_sync();
     const auto fetch = [&](uint32_t (&d)[NL][16], int p) {
       tmem_ld_32x16(t0 + 16 * p, d[0]);
       if (NL > 1) tmem_ld_32x16(t0 + BN + 16 * p, d[NL > 1 ? 1 : 0]);
       if (NL > 2) tmem_ld_32x16(t0 + C::OFF1 + 16 * p, d[NL > 2 ? 2 : 0]);
     };
     // one piece from `cur`, while the next one is on its way to `other`
-    const auto step = [&](uint32_t (&cur)[NL][16], uint32_t (&other)[NL][16], int p) -> bool {
+    const auto step = [&](int now, int p) -> bool {
+      uint32_t(&cur)[NL][16] = v[now];
       tmem_ld_wait();
       if (p + 1 < NP) {
-        fetch(other, p + 1);
+        fetch(v[now ^ 1], p + 1);
       } else {  // the accumulators are free
         tc_fence_before_sync();
         __syncwarp();
@@ -458,24 +454,9 @@ __device__ __forceinline__ void read_out(const GemmArgs& g, int set, uint32_t ra
         z[j] = mul2(gh, z[j]);
         r1[j] = pack_bf16x2(z[j].x, z[j].y);
       }
-      if (MODE == LAYER && g.planes) {
-        if (plane0 >= 0) {
-          const int left = g.N - w.nt() * BN - 16 * p;
-          const long long at = plane0 + 16ll * p * g.pd.S;
-          if (g.planes_r) {
-            float r[16];
-#pragma unroll
-            for (int j = 0; j < 16; ++j) r[j] = j < left ? plane_value(g.planes_r + at + (long long)j * g.pd.S) : 0.f;
-            MC_EACH z[j] = add2(z[j], make_float2(r[2 * j], r[2 * j + 1]));
-          }
-#pragma unroll
-          for (int j = 0; j < 16; ++j)
-            if (j < left) g.planes[at + (long long)j * g.pd.S] = __float2bfloat16_rn(j & 1 ? z[j / 2].y : z[j / 2].x);
-        }
-        return true;
-      }
       const uint32_t j0 = p % PER * 2;
-      if (p % PER == 0) {
+      const bool staged = !(MODE == LAYER && g.planes);
+      if (p % PER == 0 && (staged || g.res)) {
         if (!slot_ready(i)) return false;
         if (MODE == GATE_BWD && !slot_ready(i + 1)) return false;
       }
@@ -492,6 +473,17 @@ __device__ __forceinline__ void read_out(const GemmArgs& g, int set, uint32_t ra
             else z[4 * h + e] = add2(z[4 * h + e], f);
           }
         }
+      }
+      if (!staged) {
+        if (plane0 >= 0) {
+          const int left = g.N - w.nt() * BN - 16 * p;
+          bf16* to = g.planes + plane0 + 16ll * p * g.pd.S;
+#pragma unroll
+          for (int j = 0; j < 16; ++j)
+            if (j < left) to[(long long)j * g.pd.S] = __float2bfloat16_rn(j & 1 ? z[j / 2].y : z[j / 2].x);
+        }
+        if (g.res && p % PER == PER - 1) slot_done(i++);
+        return true;
       }
       if (MODE == ACT_BWD || MODE == GATE_BWD) MC_EACH r0[j] = pack_bf16x2(o[j].x, o[j].y);
       else MC_EACH r0[j] = pack_bf16x2(z[j].x, z[j].y);
@@ -510,7 +502,7 @@ __device__ __forceinline__ void read_out(const GemmArgs& g, int set, uint32_t ra
     fetch(v[0], 0);
 #pragma unroll 1
     for (int p = 0; p < NP; p += 2)
-      if (!step(v[0], v[1], p) || !step(v[1], v[0], p + 1)) return;
+      if (!step(0, p) || !step(1, p + 1)) return;
   }
 }
 
@@ -651,7 +643,7 @@ __global__ void __launch_bounds__(THREADS, 1) rows_tc_kernel(const __grid_consta
     }
   } else if (warp < 4) {
     // ---- I/O of one set's staged tiles: fill the slots ahead (residual), store what the read-out warps leave in them
-    if (lane == 0 && !(MODE == LAYER && g.planes)) {
+    if (lane == 0 && !(MODE == LAYER && g.planes && !g.res)) {
       const int set = warp - 2;
       TileWalk lead(g, set, 2);
       int lead_c = 0;
@@ -680,7 +672,7 @@ __global__ void __launch_bounds__(THREADS, 1) rows_tc_kernel(const __grid_consta
           ok = mbar_wait(done(set, s), (i / g.slots) & 1, abort_flag, 0x121);
           if (!ok) break;
           const int col = column(w, c), m0 = (w.m() * 2 + rank) * TILE;
-          if (col < g.N && m0 < g.rows) {
+          if (col < g.N && m0 < g.rows && !(MODE == LAYER && g.planes)) {
             tma_store(&g.y[MODE == GATE_BWD ? c % 2 : 0], col, m0, buf + s * C::CH_BYTES);
             bulk_commit();
             bulk_wait_read();
@@ -1010,15 +1002,11 @@ static int launch_wide(GemmArgs& g, int bn, cudaStream_t st) {
 int tc_layer(const TcRows& a, const TcRows& w, const bf16* bias, int act, const TcRows& r, const TcRows& y,
              bool backward, cudaStream_t st) {
   GemmArgs g = base_args(a, y, bias, act);
-  if (y.ld == 0) {  // NCHW
-    g.planes = (bf16*)y.p, g.planes_r = (const bf16*)r.p, g.pd = PixDiv((uint32_t)y.S);
-    const int bn = tile_width(g.m_pairs, y.cols, g.kb[0]);
-    if (!encode(&g.a[0], a, TILE) || !encode(&g.b[0], w, bn / 2)) return MC_ERR_LAUNCH;
-    return launch_wide<LAYER>(g, bn, st);
-  }
   g.res = r.p != nullptr;
   const int bn = tile_width(g.m_pairs, y.cols, g.kb[0]);
-  if (!encode(&g.a[0], a, TILE) || !encode(&g.b[0], w, bn / 2) || !encode(&g.y[0], y, TILE)) return MC_ERR_LAUNCH;
+  if (!encode(&g.a[0], a, TILE) || !encode(&g.b[0], w, bn / 2)) return MC_ERR_LAUNCH;
+  if (y.ld == 0) g.planes = (bf16*)y.p, g.pd = PixDiv((uint32_t)y.S);
+  else if (!encode(&g.y[0], y, TILE)) return MC_ERR_LAUNCH;
   if (g.res && !encode(&g.r, r, TILE)) return MC_ERR_LAUNCH;
   return backward ? launch_wide<ACT_BWD>(g, bn, st) : launch_wide<LAYER>(g, bn, st);
 }
