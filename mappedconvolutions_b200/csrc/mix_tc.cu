@@ -6,7 +6,7 @@
 // to 64 + 64.
 //
 // rows kernel:  tiles of 2 x 128 pixels x BN channels.  One warp fetches operand tiles by TMA, one thread issues the MMAs into
-// two accumulator sets in turn.  Each set has four read-out warps of its own (a tile's latencies - TMEM loads, elementary
+// two or four accumulators in turn.  Every second tile has four read-out warps of its own (a tile's latencies - TMEM loads, elementary
 // functions, hand-over of the staged tiles - overlap with the other set's), which apply the epilogue and leave bf16 tiles
 // in shared memory, from where an I/O thread stores them by TMA; the same slots receive the tiles that an epilogue adds
 // or multiplies (residual, grad_output) beforehand.  Where all weights that a block needs fit beside the rings they stay
@@ -310,6 +310,8 @@ template <int MODE, int BN> struct Cfg {
   static constexpr int CW = MODE == GATE_BWD ? 32 : 64;
   static constexpr int NCH = (MODE == GATE_BWD ? 2 : 1) * BN / CW;           // staged tiles
   static constexpr int CH_BYTES = TILE * CW * 2;
+  // Accumulators in TMEM: as many as fit, since an epilogue's latencies are hidden by the tiles behind it.
+  static constexpr int NACC = MODE == GATE_BWD || N0 > 128 ? 2 : 4, ACC = 512 / NACC;
   static constexpr int B0 = N0 / 2 * KB * 2, B1 = N1 / 2 * KB * 2;           // a block's weights per stage
   static constexpr int BMAX = B0 > B1 ? B0 : B1;
 };
@@ -326,10 +328,10 @@ struct alignas(64) GemmArgs {
   bf16* planes;
   PixDiv pd;
   int group;         // channel tiles of a pair of blocks whose weights stay in shared memory, 0: none do
-  int stages, slots;
+  int stages, slot_bits;  // 2^slot_bits slots for staged tiles in each set
 };
 
-constexpr int ROWS_BARS = 2 * MAX_STAGES + 1 + 4 + 8 + 1 + 2;
+constexpr int ROWS_BARS = 2 * MAX_STAGES + 1 + 8 + 16 + 1 + 2;
 
 // The tiles of a pair of blocks, from the `first`-th on, every `every`-th one.  With resident weights a pair keeps its
 // group of channel tiles and takes every so many pixel tiles; otherwise the channel tiles of a pixel tile are next to
@@ -371,7 +373,7 @@ __device__ __forceinline__ void load_b(const GemmArgs& g, int seg, uint32_t rank
 }
 
 // Offsets of the barriers behind bfull.
-constexpr uint32_t BAR_TFULL = 8, BAR_TEMPTY = 24, BAR_READY = 40, BAR_DONE = 72, BAR_DRAIN = 104, BAR_BIASED = 112;
+constexpr uint32_t BAR_TFULL = 8, BAR_TEMPTY = 40, BAR_READY = 72, BAR_DONE = 136, BAR_DRAIN = 200, BAR_BIASED = 208;
 
 // Read-out warps of one accumulator set: thread = pixel.  Sixteen channels at a time in a loop that is not unrolled: the
 // code of a whole tile does not stay in the instruction cache, and then fetching it takes longer than running it.
@@ -381,15 +383,14 @@ __device__ __forceinline__ void read_out(const GemmArgs& g, int set, uint32_t ra
   typedef Cfg<MODE, BN> C;
   constexpr int NP = BN / 16, PER = C::CW / 16;  // pieces of a tile, and of a staged tile
   const int lane = threadIdx.x % 32, q = threadIdx.x / 32 & 3, row = q * 32 + lane;
-  const uint32_t buf = out0 + set * g.slots * C::CH_BYTES;
-  const uint32_t t0 = ((uint32_t)(q * 32) << 16) + set * 256;
-  const uint32_t tfull = bfull + BAR_TFULL + 8 * set, tempty = of_leader(bfull + BAR_TEMPTY + 8 * set);
+  const uint32_t buf = out0 + (set << g.slot_bits) * C::CH_BYTES, mask = (1u << g.slot_bits) - 1;
+  const uint32_t tempty0 = of_leader(bfull + BAR_TEMPTY);
   // 16-byte piece j of this row of a staged tile
   const uint32_t at0 = buf + row * C::CW * 2, swizzle = (C::CW == 64 ? row & 7 : (row >> 1) & 3) << 4;
-  const auto slot = [&](uint32_t i) { return at0 + (g.slots == 2 ? i & 1 : 0) * C::CH_BYTES; };
-  const auto bar_of = [&](uint32_t base, uint32_t i) { return bfull + base + 16 * set + 8 * (g.slots == 2 ? i & 1 : 0); };
+  const auto slot = [&](uint32_t i) { return at0 + (i & mask) * C::CH_BYTES; };
+  const auto bar_of = [&](uint32_t base, uint32_t i) { return bfull + base + 32 * set + 8 * (i & mask); };
   const auto slot_ready = [&](uint32_t i) {
-    return warp_wait(bar_of(BAR_READY, i), (g.slots == 2 ? i >> 1 : i) & 1, abort_flag, 0x132);
+    return warp_wait(bar_of(BAR_READY, i), i >> g.slot_bits & 1, abort_flag, 0x132);
   };
   const auto slot_done = [&](uint32_t i) {
     fence_proxy_async_smem();
@@ -423,7 +424,9 @@ __device__ __forceinline__ void read_out(const GemmArgs& g, int set, uint32_t ra
     }
     constexpr int NL = MODE == GATE_BWD ? 3 : MODE == GATE ? 2 : 1;
     uint32_t v[2][NL][16];
-    if (!warp_wait(tfull, it & 1, abort_flag, 0x131)) return;
+    const uint32_t tile = 2 * it + set, acc = tile % C::NACC;  // (the pair's tile, and where it is)
+    const uint32_t t0 = ((uint32_t)(q * 32) << 16) + acc * C::ACC;
+    if (!warp_wait(bfull + BAR_TFULL + 8 * acc, tile / C::NACC & 1, abort_flag, 0x131)) return;
     tc_fence_after_sync();
     const auto fetch = [&](uint32_t (&d)[NL][16], int p) {
       tmem_ld_32x16(t0 + 16 * p, d[0]);
@@ -439,7 +442,7 @@ __device__ __forceinline__ void read_out(const GemmArgs& g, int set, uint32_t ra
       } else {  // the accumulators are free
         tc_fence_before_sync();
         __syncwarp();
-        if (lane == 0) arrive_leader(tempty);
+        if (lane == 0) arrive_leader(tempty0 + 8 * acc);
       }
       const float* b = bs + 16 * p;
       Pairs z, o;
@@ -515,7 +518,7 @@ __global__ void __launch_bounds__(THREADS, 1) rows_tc_kernel(const __grid_consta
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   volatile int* abort_flag = &abort_flag_s;
   const uint32_t out0 = smem_u32(sm);
-  const uint32_t a0 = out0 + 2 * g.slots * C::CH_BYTES;
+  const uint32_t a0 = out0 + (2 << g.slot_bits) * C::CH_BYTES;
   const uint32_t b0 = a0 + g.stages * A_BYTES;
   const uint32_t btile = g.kb[0] * C::B0 + g.kb[1] * C::B1;  // a channel tile's weights
   const int bbytes = g.group ? g.group * btile : g.stages * C::BMAX;
@@ -528,8 +531,8 @@ __global__ void __launch_bounds__(THREADS, 1) rows_tc_kernel(const __grid_consta
   const uint32_t bfull = bar0 + 8 * (2 * MAX_STAGES);
   const auto tfull = [&](uint32_t s) { return bfull + BAR_TFULL + 8 * s; };
   const auto tempty = [&](uint32_t s) { return bfull + BAR_TEMPTY + 8 * s; };
-  const auto ready = [&](int set, uint32_t s) { return bfull + BAR_READY + 8 * (2 * set + s); };
-  const auto done = [&](int set, uint32_t s) { return bfull + BAR_DONE + 8 * (2 * set + s); };
+  const auto ready = [&](int set, uint32_t s) { return bfull + BAR_READY + 8 * (4 * set + s); };
+  const auto done = [&](int set, uint32_t s) { return bfull + BAR_DONE + 8 * (4 * set + s); };
   const uint32_t drain = bfull + BAR_DRAIN;
   const auto biased = [&](int set) { return bfull + BAR_BIASED + 8 * set; };
 
@@ -538,11 +541,13 @@ __global__ void __launch_bounds__(THREADS, 1) rows_tc_kernel(const __grid_consta
     for (int i = 0; i < g.stages; ++i) mbar_init(full(i), 1), mbar_init(empty(i), 1);
     mbar_init(bfull, 1);
     mbar_init(drain, 1);
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < C::NACC; ++i) {
       mbar_init(tfull(i), 1);
       mbar_init(tempty(i), 8);  // (the leader's: four warps of each block)
+    }
+    for (int i = 0; i < 2; ++i) {
       mbar_init(biased(i), 4);
-      for (int s = 0; s < 2; ++s) mbar_init(ready(i, s), 1), mbar_init(done(i, s), 4);
+      for (int s = 0; s < 4; ++s) mbar_init(ready(i, s), 1), mbar_init(done(i, s), 4);
     }
     fence_barrier_init();
     fence_proxy_async_smem();
@@ -602,7 +607,7 @@ __global__ void __launch_bounds__(THREADS, 1) rows_tc_kernel(const __grid_consta
       bool ok = true, there = false;
       if (g.group && w.more()) ok = __all_sync(~0u, mbar_wait(bfull, 0, abort_flag, 0x111));
       for (uint32_t it = 0; w.more() && ok; w.next(), ++it) {
-        const uint32_t acc = it & 1, aph = (it >> 1) & 1;
+        const uint32_t acc = it % C::NACC, aph = it / C::NACC & 1;
         ok = __all_sync(~0u, mbar_wait(tempty(acc), aph ^ 1, abort_flag, 0x112));
         if (!ok) break;
         tc_fence_after_sync();
@@ -612,7 +617,7 @@ __global__ void __launch_bounds__(THREADS, 1) rows_tc_kernel(const __grid_consta
         for (int seg = 0; seg < 2; ++seg) {
           constexpr uint32_t HI = desc_sw128_hi(1024);
           const uint32_t idesc = make_idesc_bf16(2 * TILE, seg ? C::N1 : C::N0, 0, 0);
-          const uint32_t d = acc * 256 + (seg ? C::OFF1 : 0);
+          const uint32_t d = acc * C::ACC + (seg ? C::OFF1 : 0);
           for (int k = 0; k < g.kb[seg]; ++k) {
             if (!there) {
               ok = __all_sync(~0u, mbar_wait(full(st), ph, abort_flag, 0x113));
@@ -648,11 +653,11 @@ __global__ void __launch_bounds__(THREADS, 1) rows_tc_kernel(const __grid_consta
       TileWalk lead(g, set, 2);
       int lead_c = 0;
       uint32_t lead_i = 0;
-      const uint32_t buf = out0 + set * g.slots * C::CH_BYTES;
+      const uint32_t buf = out0 + (set << g.slot_bits) * C::CH_BYTES, slots = 1u << g.slot_bits;
       const auto column = [&](const TileWalk& w, int c) { return w.nt() * BN + (MODE == GATE_BWD ? c / 2 : c) * C::CW; };
       const auto advance = [&]() {
         if (!lead.more()) return;
-        const uint32_t s = lead_i % g.slots;
+        const uint32_t s = lead_i & (slots - 1);
         const int col = column(lead, lead_c);
         if (g.res && col < g.N && (lead.m() * 2 + rank) * TILE < g.rows) {
           mbar_expect_tx(ready(set, s), C::CH_BYTES);
@@ -663,13 +668,13 @@ __global__ void __launch_bounds__(THREADS, 1) rows_tc_kernel(const __grid_consta
         ++lead_i;
         if (++lead_c == C::NCH) lead_c = 0, lead.next();
       };
-      for (int i = 0; i < g.slots; ++i) advance();
+      for (int i = 0; i < (int)slots; ++i) advance();
       bool ok = true;
       uint32_t i = 0;
       for (TileWalk w(g, set, 2); w.more() && ok; w.next())
         for (int c = 0; c < C::NCH; ++c, ++i) {
-          const uint32_t s = i % g.slots;
-          ok = mbar_wait(done(set, s), (i / g.slots) & 1, abort_flag, 0x121);
+          const uint32_t s = i & (slots - 1);
+          ok = mbar_wait(done(set, s), i >> g.slot_bits & 1, abort_flag, 0x121);
           if (!ok) break;
           const int col = column(w, c), m0 = (w.m() * 2 + rank) * TILE;
           if (col < g.N && m0 < g.rows && !(MODE == LAYER && g.planes)) {
@@ -932,8 +937,8 @@ static int launch_rows(GemmArgs& g, cudaStream_t st) {
   g.n_tiles = (g.N + BN - 1) / BN;
   const int fixed_bytes = 1024 + 4 * 256 * 4 + ROWS_BARS * 8 + 16 + 64;
   const int b_tile = g.kb[0] * C::B0 + g.kb[1] * C::B1, pairs = sm_total() / 2;
-  g.slots = 2;
-  int left = SMEM_LIMIT - fixed_bytes - 2 * g.slots * C::CH_BYTES;
+  g.slot_bits = MODE == GATE_BWD ? 2 : 1;
+  int left = SMEM_LIMIT - fixed_bytes - (2 << g.slot_bits) * C::CH_BYTES;
   // Weights stay in shared memory where at least three stages of pixels fit beside them.  How many channel tiles a pair
   // keeps: the number that leaves the fewest pairs without work; more tiles cost stages, below four of which the pixels'
   // latency shows.
@@ -947,10 +952,11 @@ static int launch_rows(GemmArgs& g, cudaStream_t st) {
     if (used > best + 1e-9) best = used, g.group = group;
   }
   if (!g.group && MODE != GATE_BWD && g.n_tiles <= pairs && b_tile + 3 * A_BYTES <= left + 2 * C::CH_BYTES)
-    g.group = g.slots = 1, left += 2 * C::CH_BYTES;  // one slot per set makes room for one tile's
+    g.group = 1, g.slot_bits = 0, left += 2 * C::CH_BYTES;  // one slot per set makes room for one tile's
+
   g.stages = g.group ? (left - g.group * b_tile) / A_BYTES : left / (A_BYTES + C::BMAX);
   if (g.stages > MAX_STAGES) g.stages = MAX_STAGES;
-  const size_t smem = fixed_bytes + 2 * g.slots * C::CH_BYTES + (size_t)g.stages * A_BYTES +
+  const size_t smem = fixed_bytes + (2 << g.slot_bits) * C::CH_BYTES + (size_t)g.stages * A_BYTES +
                       (g.group ? g.group * b_tile : g.stages * C::BMAX);
   long long n;
   if (g.group) {
