@@ -171,15 +171,16 @@ __global__ void __launch_bounds__(256) planes_to_rows_kernel(const bf16* __restr
     *reinterpret_cast<uint4*>(dst + (b * S + s0 + r) * ld + c0 + j) = make_uint4(w[0], w[1], w[2], w[3]);
   }
 }
-// Lays a call's temporary tensors out in the workspace; without a workspace it only adds up their sizes.
+// Lays a call's temporary tensors out in the workspace; with `sizes` set it only adds up what they need.
 struct Work {
   char* base;
   cudaStream_t st;
+  bool sizes = false;
   size_t used = 0;
   int rc = MC_OK;
-  bool run() const { return base && rc == MC_OK; }
+  bool run() const { return !sizes && rc == MC_OK; }
   char* take(size_t n) {
-    char* p = base ? base + used : nullptr;
+    char* p = sizes ? nullptr : base + used;
     used += up256(n);
     return p;
   }
@@ -191,7 +192,7 @@ struct Work {
     const long long P = pixels(d);
     if (in_place(d, C)) return TcRows{p, P, C, C};
     const TcRows r = fresh(P, C);
-    if (!p && base) return TcRows{nullptr, P, C, C};
+    if (!p && !sizes) return TcRows{nullptr, P, C, C};
     lay_out(d, p, r);
     return r;
   }
@@ -292,7 +293,7 @@ static void tc_pointwise_bwd(Work& k, const mc_mix_desc* d, const void* gy, cons
     gz = k.fresh(pixels(d), d->C_out);
     if (k.run()) k.did(tc_layer(xr, wr, (const bf16*)bias, d->act, gyr, gz, true, k.st));
   }
-  if (gx || !k.base) {
+  if (gx || k.sizes) {
     const TcRows wt = k.weight_t(w, d->C_out, d->C_in), gxr = k.out(d, gx, d->C_in);
     if (k.run()) k.did(tc_input_grad(gz, wt, TcRows{}, TcRows{}, gxr, k.st));
     k.put(d, gxr, gx, d->C_in);
@@ -321,7 +322,7 @@ static void tc_gated_bwd(Work& k, const mc_mix_desc* d, const void* gy, const vo
   const TcRows wi = k.weight(w_in, 2 * H, d->C_in), wot = k.weight_t(w_out, d->C_out, H);
   const TcRows gyr = k.in(d, gy, d->C_out), gg = k.fresh(pixels(d), H), gu = k.fresh(pixels(d), H);
   if (k.run() && (gx || gw_in || gb_in)) k.did(tc_gate_bwd(xr, wi, (const bf16*)b_in, d->act, gyr, wot, gg, gu, k.st));
-  if (gx || !k.base) {
+  if (gx || k.sizes) {
     const TcRows gxr = k.out(d, gx, d->C_in), wg = k.weight_t(w_in, H, d->C_in, 2);
     TcRows wu = wg;
     wu.p = (const char*)wg.p + (size_t)d->C_in * wg.ld * 2;
@@ -335,9 +336,9 @@ static void tc_gated_bwd(Work& k, const mc_mix_desc* d, const void* gy, const vo
 // workspace of the whole call, for any choice of optional arguments
 template <typename F>
 static size_t work_size(F f) {
-  Work k{nullptr, nullptr};
+  Work k{nullptr, nullptr, true};
   f(k);
-  return k.used + 256;  // (never zero: a null workspace means that sizes are wanted)
+  return k.used;
 }
 
 }  // namespace mix
@@ -401,7 +402,8 @@ int mc_pointwise_bwd(const mc_mix_desc* d, const void* gy, const void* x, const 
   int rc = check_desc(d, false);
   if (rc) return rc;
   if (!gy || !x || !w || (mc_pointwise_saved_bytes(d) && !saved)) return MC_ERR_BAD_ARG;
-  if (!ws || ws_bytes < mc_pointwise_workspace_bytes(d, MC_PHASE_BACKWARD)) return MC_ERR_WORKSPACE;
+  const size_t need = mc_pointwise_workspace_bytes(d, MC_PHASE_BACKWARD);
+  if (need && (!ws || ws_bytes < need)) return MC_ERR_WORKSPACE;
   if (d->dtype == MC_BF16) {
     if (!aligned16(gy) || !aligned16(x) || !aligned16(w) || !aligned16(saved) || !aligned16(gx) || !aligned16(ws))
       return MC_ERR_BAD_ARG;

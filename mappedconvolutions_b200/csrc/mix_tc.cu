@@ -905,15 +905,23 @@ static int sm_total() {
   }
   return v;
 }
-template <typename Kern>
-static bool allow_smem(Kern kern) {
-  return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_LIMIT) == cudaSuccess;
+// Once per kernel and device: the limit belongs to the kernel, not to a call.
+template <auto kern>
+static bool allow_smem() {
+  static std::atomic<uint64_t> done{0};  // a bit per device
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return false;
+  const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+  if (done.load(std::memory_order_relaxed) & bit) return true;
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_LIMIT) != cudaSuccess) return false;
+  done.fetch_or(bit, std::memory_order_relaxed);
+  return true;
 }
 
 // Blocks in clusters of two.
-template <typename Kern, typename Args>
-static int launch_pairs(Kern kern, unsigned pairs, size_t smem, const Args& args, cudaStream_t st) {
-  if (!allow_smem(kern)) return MC_ERR_LAUNCH;
+template <auto kern, typename Args>
+static int launch_pairs(unsigned pairs, size_t smem, const Args& args, cudaStream_t st) {
+  if (!allow_smem<kern>()) return MC_ERR_LAUNCH;
   cudaLaunchAttribute attr[2] = {};
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = 2, attr[0].val.clusterDim.y = 1, attr[0].val.clusterDim.z = 1;
@@ -968,7 +976,7 @@ static int launch_rows(GemmArgs& g, cudaStream_t st) {
     n = (long long)g.m_pairs * g.n_tiles;
     if (n > pairs) n = pairs;
   }
-  return launch_pairs(rows_tc_kernel<MODE, BN>, (unsigned)n, smem, g, st);
+  return launch_pairs<rows_tc_kernel<MODE, BN>>((unsigned)n, smem, g, st);
 }
 
 // Channels of a tile, for `pairs` pixel tiles, n channels, kb stages: the least estimated time.  A tile costs its MMAs
@@ -1082,7 +1090,7 @@ static int launch_outer(OuterTcArgs& g, const OuterPlan& p, cudaStream_t st) {
   constexpr int STAGE = MT * A_BYTES + BN / 2 * 128;
   g.stages = (SMEM_LIMIT - 2048) / STAGE;
   if (g.stages > MAX_STAGES) g.stages = MAX_STAGES;
-  return launch_pairs(outer_tc_kernel<MT, BN>, g.segs * p.m_tiles * p.n_tiles * p.splits, 1024 + g.stages * STAGE, g, st);
+  return launch_pairs<outer_tc_kernel<MT, BN>>(g.segs * p.m_tiles * p.n_tiles * p.splits, 1024 + g.stages * STAGE, g, st);
 }
 int tc_outer(const TcRows& g0, const TcRows& g1, const TcRows& x, float* part, float* csum, cudaStream_t st) {
   OuterTcArgs g{};
