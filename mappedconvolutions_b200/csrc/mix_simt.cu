@@ -67,6 +67,19 @@ struct alignas(sizeof(T) * W) Run {
   T v[W];
 };
 
+// two accumulators at once: one issue slot for a pair of float32 FMAs
+__device__ __forceinline__ void fma_pair(float* acc, float a, const float* b) {
+  const float2 av = make_float2(a, a), bv = make_float2(b[0], b[1]);
+  float2 c = make_float2(acc[0], acc[1]);
+  asm("fma.rn.f32x2 %0, %1, %2, %0;"
+      : "+l"(reinterpret_cast<unsigned long long&>(c))
+      : "l"(reinterpret_cast<const unsigned long long&>(av)), "l"(reinterpret_cast<const unsigned long long&>(bv)));
+  acc[0] = c.x, acc[1] = c.y;
+}
+__device__ __forceinline__ void fma_pair(double* acc, double a, const double* b) {
+  acc[0] += a * b[0], acc[1] += a * b[1];
+}
+
 // acc[i][j] += a[k][pixel i] b[k][channel j]; pixels tp * 4 + {0 .. 3} and 64 more, channels tc * W + {0 .. W - 1} and
 // TN / 2 more
 template <typename T, int TN>
@@ -92,7 +105,7 @@ __device__ __forceinline__ void multiply(const Slice<T, TN>& s, T (&acc)[8][TN /
 #pragma unroll
     for (int i = 0; i < 8; ++i)
 #pragma unroll
-      for (int j = 0; j < 2 * W; ++j) acc[i][j] += a[i] * b[j];
+      for (int j = 0; j < 2 * W; j += 2) fma_pair(acc[i] + j, a[i], b + j);
   }
 }
 
