@@ -192,10 +192,22 @@ __global__ void __launch_bounds__(THREADS) finish_kernel(int kind, const double*
 template <typename S, typename D>
 __device__ __forceinline__ void scale_chunk(const S* p, D* q, int n, double coefficient) {
   typedef typename Traits<S>::CT CT;
+  constexpr int ROUND = sizeof(CT) == 4 ? 4 : 2;
   const CT c = (CT)coefficient;
   int i = threadIdx.x * 8;
   if ((((uintptr_t)p | (uintptr_t)q) & 15) == 0) {
-#pragma unroll 4
+    // (all loads of a round before its stores: the compiler may not move them across, p and q can be the same)
+    for (; i + (ROUND - 1) * THREADS * 8 + 8 <= n; i += ROUND * THREADS * 8) {
+      CT v[ROUND][8];
+#pragma unroll
+      for (int r = 0; r < ROUND; ++r) load8(p + i + r * THREADS * 8, v[r]);
+#pragma unroll
+      for (int r = 0; r < ROUND; ++r) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[r][j] *= c;
+        store8(q + i + r * THREADS * 8, v[r]);
+      }
+    }
     for (; i + 8 <= n; i += THREADS * 8) {
       CT v[8];
       load8(p + i, v);
