@@ -104,6 +104,18 @@ def test_many_pixels(dtype):
     R.check(dict(zip(("gx", "gw_in", "gb_in", "gw_out", "gb_out"), grads), y=y), R.gated(x, wi, bi, wo, bo, None, "silu", gy))
 
 
+@pytest.mark.parametrize("layout", ["nhwc", "nchw"])
+def test_many_channels(layout):
+    """rows longer than a block's shared memory, odd in length, and more channel tiles than pairs of blocks"""
+    g = torch.Generator("cuda").manual_seed(9)
+    cin, cout = 1501, 9003
+    x, gy = image(g, (2, cin, 3, 5), BF, layout), image(g, (2, cout, 3, 5), BF, layout, 0.01)
+    weight, bias = params(g, cout, cin, BF)
+    y, saved = host.impl.pointwise_forward(x, weight, bias, None, 4, True)
+    g3 = host.impl.pointwise_backward(gy, saved, x, weight, bias, 4)
+    R.check(dict(zip(("gx", "gw", "gb"), g3), y=y), R.pointwise(x, weight, bias, None, "silu", gy))
+
+
 @pytest.mark.parametrize("dtype", [BF, F32, F64], ids=["bf16", "f32", "f64"])
 @pytest.mark.parametrize("layout", ["nhwc", "nchw"])
 @pytest.mark.parametrize("shape", [(3000, 2, 3), (70_000, 1, 2), (5, 1, 1), (2, 40, 64)])
