@@ -433,16 +433,31 @@ __device__ __forceinline__ void read_out(const GemmArgs& g, int set, uint32_t ra
       if (NL > 1) tmem_ld_32x16(t0 + BN + 16 * p, d[NL > 1 ? 1 : 0]);
       if (NL > 2) tmem_ld_32x16(t0 + C::OFF1 + 16 * p, d[NL > 2 ? 2 : 0]);
     };
-    // one piece from `cur`, while the next one is on its way to `other`
+    // pieces with channels that exist; whether staged tiles are handed over at all
+    // (the gate's kernels read out whole tiles: the tests cost them 4 - 10 %, and their tiles are seldom that empty)
+    int live = NP;
+    if (MODE == LAYER || MODE == ACT_BWD) {
+      const int left = (g.N - w.nt() * BN + 15) / 16;
+      if (left < NP) live = left;
+    }
+    const bool turns = !(MODE == LAYER && g.planes) || g.res;
+    // one piece, while the next one is on its way
     const auto step = [&](int now, int p) -> bool {
       uint32_t(&cur)[NL][16] = v[now];
-      tmem_ld_wait();
-      if (p + 1 < NP) {
-        fetch(v[now ^ 1], p + 1);
-      } else {  // the accumulators are free
+      if (p < live) tmem_ld_wait();
+      if (p + 1 < live) fetch(v[now ^ 1], p + 1);
+      if (p + 1 == NP) {  // the accumulators are free
         tc_fence_before_sync();
         __syncwarp();
         if (lane == 0) arrive_leader(tempty0 + 8 * acc);
+      }
+      if (p >= live) {  // (the staged tile takes its turn all the same)
+        if (p % PER == 0 && turns && (!slot_ready(i) || (MODE == GATE_BWD && !slot_ready(i + 1)))) return false;
+        if (p % PER == PER - 1 && turns) {
+          slot_done(i++);
+          if (MODE == GATE_BWD) slot_done(i++);
+        }
+        return true;
       }
       const float* b = bs + 16 * p;
       Pairs z, o;
