@@ -415,7 +415,7 @@ typedef struct mc_mix_desc {
  * that fills saved. */
 enum { MC_PHASE_FORWARD = 0, MC_PHASE_BACKWARD = 1, MC_PHASE_KEEP = 2 };
 /* saved: mc_*_saved_bytes of memory that the forward call fills for the backward call (NULL: no backward call follows);
- * its contents are opaque.  ws: mc_*_workspace_bytes(d, phase) of scratch.  Both 256-byte aligned; sizes can be 0
+ * its contents are opaque.  ws: mc_*_workspace_bytes(d, phase) of scratch.  Both 16-byte aligned; sizes can be 0
  * (and then the pointers NULL).
  * In the backward calls any of the gradients may be NULL; grad_residual is grad_output itself.  Gradients of parameters
  * are sums over all pixels in a fixed order (they repeat bit for bit), rounded once to `dtype`. */

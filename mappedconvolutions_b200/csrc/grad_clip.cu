@@ -352,6 +352,7 @@ static int run_sized(const Lists& l, bool scale, double norm_type, double max_no
   if (kind == 0) return MC_ERR_UNSUPPORTED;
   if (scale && !(max_norm >= 0)) return MC_ERR_BAD_ARG;
   if (!ws || ws_bytes < mc_grad_workspace_bytes(l.n)) return MC_ERR_WORKSPACE;
+  if ((uintptr_t)ws % sizeof(double)) return MC_ERR_BAD_ARG;
   return l.n <= SMALL ? run<SMALL>(l, scale, kind, max_norm, norm, norm32, (double*)ws, (cudaStream_t)stream)
                       : run<LARGE>(l, scale, kind, max_norm, norm, norm32, (double*)ws, (cudaStream_t)stream);
 }

@@ -1,5 +1,6 @@
 // C-ABI entry points of the channel-mixing layers: argument checks, workspace layout, and the sequence of products
 // behind each call.
+#include <initializer_list>
 #include <type_traits>
 
 #include "mix.cuh"
@@ -9,7 +10,11 @@ namespace mix {
 
 static int esize(int dtype) { return dtype == MC_F64 ? 8 : dtype == MC_F32 ? 4 : 2; }
 static int acc_size(int dtype) { return dtype == MC_F64 ? 8 : 4; }
-static bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
+static bool aligned(size_t n, std::initializer_list<const void*> ps) {
+  for (const void* p : ps)
+    if ((uintptr_t)p % n) return false;
+  return true;
+}
 static size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
 
 static int check_desc(const mc_mix_desc* d, bool gated) {
@@ -24,10 +29,16 @@ static int check_desc(const mc_mix_desc* d, bool gated) {
   return MC_OK;
 }
 
+// Activations and weights on 16 bytes for MC_BF16 (TMA), everything else on its elements, memory of calls on 16 bytes.
+static bool placed(const mc_mix_desc* d, std::initializer_list<const void*> tensors, std::initializer_list<const void*> vectors,
+                   std::initializer_list<const void*> memory) {
+  return aligned(d->dtype == MC_BF16 ? 16 : esize(d->dtype), tensors) && aligned(esize(d->dtype), vectors) && aligned(16, memory);
+}
+
 static long long pixels(const mc_mix_desc* d) { return d->B * d->S; }
 
-// Shares of the pixels that a parameter gradient is summed in: about a wave of blocks (two to an SM), at least 256 pixels each where
-// images are that large; parts of an image or groups of images (channels-last batches are one image).
+// Shares of the pixels that a parameter gradient is summed in: about a wave of blocks (two to an SM), at least 256 pixels
+// each where images are that large; parts of an image or groups of images (channels-last batches are one image).
 struct Shares {
   long long S, share;
   int B, group, per_image, splits;
@@ -51,8 +62,7 @@ static Shares shares_of(const mc_mix_desc* d, int M, int N) {
   return s;
 }
 
-// gw (M, N) and gb (M): the shares' sums added in order and rounded once.  Rows of part have ldn elements.  Either may
-// be null.
+// gw (M, N) and gb (M), either of which may be null: the shares' sums, rounded once.  Rows of part have ldn elements.
 // A block takes 32 sums; eight threads for each add every eighth share, and their results are added in order.
 template <typename T, typename CT>
 __global__ void __launch_bounds__(256) add_shares_kernel(const CT* __restrict__ part, int M, int N, int ldn,
@@ -77,7 +87,7 @@ __global__ void __launch_bounds__(256) add_shares_kernel(const CT* __restrict__ 
   stv(w ? gw + i : gb + (i - nw), s);
 }
 
-// gz = gy act'(z), sixteen bytes at a time (vec: all three start on multiples of them)
+// gz = gy act'(z), sixteen bytes at a time (vec: gy starts on a multiple of them, as the others do)
 template <typename T>
 __global__ void __launch_bounds__(256) act_bwd_kernel(const T* __restrict__ gy, const T* __restrict__ z,
                                                       T* __restrict__ gz, long long n, int act, bool vec) {
@@ -424,9 +434,8 @@ int mc_pointwise_fwd(const mc_mix_desc* d, const void* x, const void* w, const v
   if (!x || !w || !y) return MC_ERR_BAD_ARG;
   const size_t need = mc_pointwise_workspace_bytes(d, saved ? MC_PHASE_KEEP : MC_PHASE_FORWARD);
   if (need && (!ws || ws_bytes < need)) return MC_ERR_WORKSPACE;
+  if (!placed(d, {x, w, residual, y}, {bias}, {saved, ws})) return MC_ERR_BAD_ARG;
   if (d->dtype == MC_BF16) {
-    if (!aligned16(x) || !aligned16(w) || !aligned16(residual) || !aligned16(y) || !aligned16(saved) || !aligned16(ws))
-      return MC_ERR_BAD_ARG;
     Work k{(char*)ws, (cudaStream_t)stream};
     tc_pointwise_fwd(k, d, x, w, bias, residual, y, input_rows_bytes(d) ? saved : nullptr);
     return k.rc;
@@ -448,9 +457,8 @@ int mc_pointwise_bwd(const mc_mix_desc* d, const void* gy, const void* x, const 
   if (!gy || !x || !w || (mc_pointwise_saved_bytes(d) && !saved)) return MC_ERR_BAD_ARG;
   const size_t need = mc_pointwise_workspace_bytes(d, MC_PHASE_BACKWARD);
   if (need && (!ws || ws_bytes < need)) return MC_ERR_WORKSPACE;
+  if (!placed(d, {gy, x, w, gx}, {bias, gw, gb}, {saved, ws})) return MC_ERR_BAD_ARG;
   if (d->dtype == MC_BF16) {
-    if (!aligned16(gy) || !aligned16(x) || !aligned16(w) || !aligned16(saved) || !aligned16(gx) || !aligned16(ws))
-      return MC_ERR_BAD_ARG;
     Work k{(char*)ws, (cudaStream_t)stream};
     tc_pointwise_bwd(k, d, gy, x, w, bias, saved, gx, gw, gb);
     return k.rc;
@@ -465,7 +473,7 @@ int mc_pointwise_bwd(const mc_mix_desc* d, const void* gy, const void* x, const 
     rc = by_type(d->dtype, [&](auto t) {
       typedef decltype(t) T;
       act_bwd_kernel<T><<<grid_for(n / (16 / (long)sizeof(T)) + 1, 256), 256, 0, st>>>(
-          (const T*)gy, (const T*)saved, (T*)gz, n, d->act, aligned16(gy) && aligned16(saved)), MC_COUNT(1);
+          (const T*)gy, (const T*)saved, (T*)gz, n, d->act, aligned(16, {gy})), MC_COUNT(1);
     });
     if (rc) return rc;
     g = gz;
@@ -523,10 +531,8 @@ int mc_gated_fwd(const mc_mix_desc* d, const void* x, const void* w_in, const vo
   if (!x || !w_in || !w_out || !y) return MC_ERR_BAD_ARG;
   const size_t need = mc_gated_workspace_bytes(d, saved ? MC_PHASE_KEEP : MC_PHASE_FORWARD);
   if (need && (!ws || ws_bytes < need)) return MC_ERR_WORKSPACE;
+  if (!placed(d, {x, w_in, w_out, residual, y}, {b_in, b_out}, {saved, ws})) return MC_ERR_BAD_ARG;
   if (d->dtype == MC_BF16) {
-    if (!aligned16(x) || !aligned16(w_in) || !aligned16(w_out) || !aligned16(residual) || !aligned16(y) ||
-        !aligned16(saved) || !aligned16(ws))
-      return MC_ERR_BAD_ARG;
     Work k{(char*)ws, (cudaStream_t)stream};
     tc_gated_fwd(k, d, x, w_in, b_in, w_out, b_out, residual, y, saved);
     return k.rc;
@@ -559,10 +565,8 @@ int mc_gated_bwd(const mc_mix_desc* d, const void* gy, const void* x, const void
   if (rc) return rc;
   if (!gy || !x || !w_in || !w_out || !saved) return MC_ERR_BAD_ARG;
   if (!ws || ws_bytes < mc_gated_workspace_bytes(d, MC_PHASE_BACKWARD)) return MC_ERR_WORKSPACE;
+  if (!placed(d, {gy, x, w_in, w_out, gx}, {b_in, gw_in, gb_in, gw_out, gb_out}, {saved, ws})) return MC_ERR_BAD_ARG;
   if (d->dtype == MC_BF16) {
-    if (!aligned16(gy) || !aligned16(x) || !aligned16(w_in) || !aligned16(w_out) || !aligned16(saved) || !aligned16(gx) ||
-        !aligned16(ws))
-      return MC_ERR_BAD_ARG;
     Work k{(char*)ws, (cudaStream_t)stream};
     tc_gated_bwd(k, d, gy, x, w_in, b_in, w_out, saved, gx, gw_in, gb_in, gw_out, gb_out);
     return k.rc;

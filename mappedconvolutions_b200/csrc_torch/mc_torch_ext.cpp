@@ -913,6 +913,14 @@ mc_mix_desc make_mix_desc(const Tensor& x, int layout, int64_t c_out, int64_t hi
   return d;
 }
 
+// What a forward call kept is memory that the kernels read without further checks.
+void check_saved(const OptTensor& saved, size_t bytes) {
+  if (bytes == 0) return;
+  TORCH_CHECK(saved.has_value() && saved->scalar_type() == at::kByte && saved->is_contiguous() &&
+                  (size_t)saved->numel() >= bytes,
+              "saved must be what the forward call of the same input, parameters and activation kept");
+}
+
 Tensor out_layout(const OptTensor& t, int layout) { return t.has_value() ? aligned16(as_layout(*t, layout)) : Tensor(); }
 void* maybe(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 
@@ -962,6 +970,7 @@ std::vector<Tensor> pointwise_backward(const Tensor& gy_in, const OptTensor& sav
   if (x.numel() == 0) return {gx, gw, gb};
   const Tensor gy = aligned16(as_layout(gy_in, layout));
   const mc_mix_desc d = make_mix_desc(x, layout, c_out, 0, act);
+  check_saved(saved, mc_pointwise_saved_bytes(&d));
   Scratch ws = scratch(mc_pointwise_workspace_bytes(&d, MC_PHASE_BACKWARD), dev);
   check(mc_pointwise_bwd(&d, gy.data_ptr(), x.data_ptr(), w.data_ptr(), b.data_ptr(), ptr(saved), maybe(gx), maybe(gw),
                          maybe(gb), ws.p, ws.n, cur_stream()));
@@ -1021,6 +1030,7 @@ std::vector<Tensor> gated_backward(const Tensor& gy_in, const OptTensor& saved, 
   if (x.numel() == 0) return g;
   const Tensor gy = aligned16(as_layout(gy_in, layout));
   const mc_mix_desc d = make_mix_desc(x, layout, c_out, hidden, act);
+  check_saved(saved, mc_gated_saved_bytes(&d));
   Scratch ws = scratch(mc_gated_workspace_bytes(&d, MC_PHASE_BACKWARD), dev);
   check(mc_gated_bwd(&d, gy.data_ptr(), x.data_ptr(), w_in.data_ptr(), b_in.data_ptr(), w_out.data_ptr(), ptr(saved),
                      maybe(g[0]), maybe(g[1]), maybe(g[2]), maybe(g[3]), maybe(g[4]), ws.p, ws.n, cur_stream()));
@@ -1122,6 +1132,8 @@ Tensor clip_gradients(const std::vector<Tensor>& tensors, double max_norm, doubl
       d = at::empty(g.sizes(), o.options());
       keep.push_back(s);
       back.emplace_back(o, d);
+      // (of strided results only the first elements are compared: what lies between the others may belong to anyone)
+      if (o.numel()) spans.emplace_back((uintptr_t)o.data_ptr(), (uintptr_t)o.data_ptr() + o.element_size(), true);
     }
     l.add(s, d);
     if (d.numel() == 0) continue;

@@ -46,7 +46,7 @@ def clip_gradients(tensors, max_norm, norm_type=2.0, out=None):
 
     In place, or into `out`: tensors of the same shapes (entries of None gradients are ignored), whose type may differ -
     float32 from bfloat16 gradients, say, rounded once.  Returns the norm before scaling, as gradient_norm does.  A NaN
-    norm makes every element NaN; an infinite one makes finite elements zero.  Tensors that share memory are refused."""
+    norm makes every element NaN; an infinite one makes finite elements zero.  Dense tensors that share memory are refused."""
     from .host import impl
     tensors = list(tensors)
     if out is not None:

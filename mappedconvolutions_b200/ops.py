@@ -806,6 +806,12 @@ def _bytes(n, dev):
     return torch.empty(int(n), dtype=torch.uint8, device=dev) if n else None
 
 
+def _check_saved(saved, n):
+    """What a forward call kept is memory that the kernels read without further checks."""
+    if n and (saved is None or saved.dtype != torch.uint8 or not saved.is_contiguous() or saved.numel() < n):
+        raise RuntimeError("saved must be what the forward call of the same input, parameters and activation kept")
+
+
 def _weight_dims(weight, name):
     if weight.dim() != 3 or weight.shape[2] != 1:
         raise RuntimeError("%s must be 3-D (out channels, in channels, 1)" % name)
@@ -852,6 +858,7 @@ def pointwise_backward(grad_output, saved, input, weight, bias, activation=0, ne
     d = _mix_desc(input, layout, c_out, 0, activation)
     with torch.cuda.device(dev):
         L = lib()
+        _check_saved(saved, L.mc_pointwise_saved_bytes(d))
         wst, wsn, wsp = _ws(L.mc_pointwise_workspace_bytes(d, 1), dev)
         input, weight, grad_output = _a16(input), _a16(weight), _a16(grad_output)
         check(L.mc_pointwise_bwd(d, grad_output.data_ptr(), input.data_ptr(), weight.data_ptr(), bias.data_ptr(), _ptr(saved),
@@ -906,6 +913,7 @@ def gated_backward(grad_output, saved, input, weight_in, bias_in, weight_out, ac
     d = _mix_desc(input, layout, c_out, hidden, activation)
     with torch.cuda.device(dev):
         L = lib()
+        _check_saved(saved, L.mc_gated_saved_bytes(d))
         wst, wsn, wsp = _ws(L.mc_gated_workspace_bytes(d, 1), dev)
         input, weight_in, weight_out, grad_output = _a16(input), _a16(weight_in), _a16(weight_out), _a16(grad_output)
         check(L.mc_gated_bwd(d, grad_output.data_ptr(), input.data_ptr(), weight_in.data_ptr(), bias_in.data_ptr(),
@@ -942,9 +950,10 @@ def _check_gradients(tensors, norm_type):
         raise RuntimeError("norm_type must be 1, 2 or infinity")
 
 
-def _check_apart(pairs):
-    """No destination may share memory with another tensor of the call."""
-    spans = []
+def _check_apart(pairs, strided=()):
+    """No destination may share memory with another tensor of the call.  Of strided results only the first elements are
+    compared: what lies between the others may belong to anyone."""
+    spans = [(t.data_ptr(), t.data_ptr() + t.element_size(), True) for t in strided if t.numel()]
     for src, dst in pairs:
         if dst.numel():
             spans.append((dst.data_ptr(), dst.data_ptr() + dst.numel() * dst.element_size(), True))
@@ -1005,7 +1014,7 @@ def clip_gradients(tensors, max_norm, norm_type=2.0, out=None):
         src.append(g.contiguous())
         dst.append(torch.empty(g.shape, dtype=o.dtype, device=dev))
         back.append((o, dst[-1]))
-    _check_apart(list(zip(src, dst)))
+    _check_apart(list(zip(src, dst)), [o for o, _ in back])
     norm, p64, p32 = _norm_out(grads, dev)
     ct, n = _lib.ctypes, len(src)
     with torch.cuda.device(dev):

@@ -156,6 +156,19 @@ def test_refusals(ops):
     ops.clip_gradients([t[:50], t[50:]], 1.0)            # neighbours in one bucket are none either
 
 
+def test_strided_results_given_twice(ops):
+    t = torch.randn(6, 8, device="cuda")
+    for call in (lambda: ops.clip_gradients([t[:, ::2], t[:, ::2]], 1.0), lambda: ops.clip_gradients([t[:, :3], t], 1.0)):
+        keep = t.clone()
+        with pytest.raises(RuntimeError, match="share memory"):
+            call()
+        assert torch.equal(t, keep)
+    want = t * (0.5 / (t.double().square().sum().sqrt() + 1e-6)).float()
+    ops.clip_gradients([t[:, ::2], t[:, 1::2]], 0.5)     # what lies between them is another's
+    # (the norm is a double sum of float32 sums of eight squares: the coefficient is off by 8 roundings at most, and its own)
+    assert ((t - want).abs() <= 10 * 2.0 ** -24 * want.abs()).all()
+
+
 def test_dist_entry_points():
     g = torch.Generator("cuda").manual_seed(8)
     ts = [torch.randn(64, 3, 7, generator=g, device="cuda"), None, torch.randn(64, generator=g, device="cuda").to(BF)]

@@ -293,6 +293,24 @@ def test_refusals(ops):
 
 
 @pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "f32"])
+def test_backward_refuses_what_another_forward_call_kept(ops, dtype):
+    t = lambda *shape: torch.randn(*shape, device="cuda").to(dtype)
+    x, w, b, gy = t(2, 7, 4, 6), t(16, 7, 1), t(16), t(2, 16, 4, 6)
+    wi, bi, wo, bo = t(24, 7, 1), t(24), t(16, 12, 1), t(16)
+    one = ops.pointwise_forward(x, w, b, None, 1, True)[1]
+    two = ops.gated_forward(x, wi, bi, wo, bo, None, 4, True)[1]
+    few = ops.pointwise_forward(x[:1], w, b, None, 1, True)[1]
+    for bad in (None, few, one[:-1], one.float(), one.view(-1, 2)[:, 0]):
+        with pytest.raises(RuntimeError, match="saved must be"):
+            ops.pointwise_backward(gy, bad, x, w, b, 1)
+    for bad in (None, one, two[:-1], two.double()):
+        with pytest.raises(RuntimeError, match="saved must be"):
+            ops.gated_backward(gy, bad, x, wi, bi, wo, 4)
+    ops.pointwise_backward(gy, one, x, w, b, 1)
+    ops.gated_backward(gy, two, x, wi, bi, wo, 4)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "f32"])
 def test_captured_step(dtype):
     """forward and backward in a graph, replayed on other data.  (No eager graph of the same leaves is alive: torch's
     AccumulateGrad nodes would then belong to the default stream, which a capture must not touch, whatever the layer.)"""

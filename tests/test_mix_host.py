@@ -93,6 +93,30 @@ def test_abi_checks_come_before_any_cuda_call():
     assert L.mc_grad_clip(1, one, t, None, t, n, 2.0, 1.0, 1, None, 1, 1 << 20, None) == -1
 
 
+@pytest.mark.parametrize("dtype", [_lib.MC_F32, _lib.MC_F64, _lib.MC_BF16])
+def test_abi_refuses_memory_that_starts_anywhere(dtype):
+    """activations and weights on their elements (bf16: 16 bytes), vectors on their elements, memory of a call on 16 bytes"""
+    L, big = _lib.lib(), 1 << 30
+    element = {_lib.MC_F32: 4, _lib.MC_F64: 8, _lib.MC_BF16: 2}[dtype]
+    tensor = 16 if dtype == _lib.MC_BF16 else element
+    d = _lib.McMixDesc(B=1, S=20, C_in=3, C_out=4, hidden=0, act=1, dtype=dtype, layout=_lib.MC_NCHW)
+    g = _lib.McMixDesc(B=1, S=20, C_in=3, C_out=4, hidden=8, act=1, dtype=dtype, layout=_lib.MC_NCHW)
+    calls = [  # (call, which alignment each pointer needs)
+        (lambda *p: L.mc_pointwise_fwd(d, *p, big, None), [tensor, tensor, element, tensor, tensor, 16, 16]),
+        (lambda *p: L.mc_pointwise_bwd(d, *p, big, None), [tensor, tensor, tensor, element, 16, tensor, element, element, 16]),
+        (lambda *p: L.mc_gated_fwd(g, *p, big, None), [tensor, tensor, element, tensor, element, tensor, tensor, 16, 16]),
+        (lambda *p: L.mc_gated_bwd(g, *p, big, None),
+         [tensor, tensor, tensor, element, tensor, 16, tensor, element, element, element, element, 16]),
+    ]
+    for call, need in calls:
+        for i, n in enumerate(need):
+            pointers = [4096] * len(need)
+            pointers[i] += n // 2
+            assert call(*pointers) == -1, (i, n)
+    one, n, t = (ctypes.c_void_p * 1)(256), (ctypes.c_int64 * 1)(5), (ctypes.c_int32 * 1)(dtype)
+    assert L.mc_grad_norm(1, one, n, t, 2.0, 16, None, 4100, 1 << 20, None) == -1
+
+
 def test_traced_layers_run_again_on_replay(monkeypatch):
     """a tracer sees one Python operation, which computes the layer on every replay"""
     if not host.COMPILED:
