@@ -89,7 +89,8 @@ __device__ __forceinline__ CT act_slope(int act, CT z) {
 }
 
 // The same as calls, for kernels whose threads hold many values in registers: inlined for each of them the elementary
-// functions would be more code than the instruction cache holds (a 50 -> 99 channel layer took 196 us instead of 74).
+// functions would be more code than the instruction cache holds (a 50 -> 99 channel layer of 131 072 pixels took 196 us
+// instead of 117).
 template <typename CT>
 struct ActBoth {
   CT value, slope;
