@@ -90,18 +90,53 @@ __device__ __forceinline__ CT act_slope(int act, CT z) {
 
 // The same as calls, for kernels whose threads hold many values in registers: inlined for each of them the elementary
 // functions would be more code than the instruction cache holds (a 50 -> 99 channel layer of 131 072 pixels took 196 us
-// instead of 117).
-template <typename CT>
-struct ActBoth {
-  CT value, slope;
+// instead of 117).  W values per call, whose latencies overlap.
+template <typename CT, int W>
+struct Values {
+  CT v[W];
 };
-template <typename CT>
-__device__ __noinline__ CT act_value_call(int act, CT z) {
-  return act_value<CT>(act, z);
+template <typename CT, int W>
+struct ActBoth {
+  Values<CT, W> value, slope;
+};
+template <typename CT, int W>
+__device__ __noinline__ Values<CT, W> act_value_call(int act, Values<CT, W> z) {
+  Values<CT, W> o;
+#define MC_ACT_CASE(A)                                        \
+  case A:                                                     \
+    _Pragma("unroll") for (int e = 0; e < W; ++e) o.v[e] = act_value<CT>(A, z.v[e]); \
+    break;
+  switch (act) {
+    MC_ACT_CASE(MC_ACT_RELU)
+    MC_ACT_CASE(MC_ACT_GELU)
+    MC_ACT_CASE(MC_ACT_GELU_TANH)
+    MC_ACT_CASE(MC_ACT_SILU)
+    MC_ACT_CASE(MC_ACT_SIGMOID)
+    default: o = z;
+  }
+#undef MC_ACT_CASE
+  return o;
 }
-template <typename CT>
-__device__ __noinline__ ActBoth<CT> act_both_call(int act, CT z) {
-  return ActBoth<CT>{act_value<CT>(act, z), act_slope<CT>(act, z)};
+template <typename CT, int W>
+__device__ __noinline__ ActBoth<CT, W> act_both_call(int act, Values<CT, W> z) {
+  ActBoth<CT, W> o;
+#define MC_ACT_CASE(A)                                        \
+  case A:                                                     \
+    _Pragma("unroll") for (int e = 0; e < W; ++e) {           \
+      o.value.v[e] = act_value<CT>(A, z.v[e]);                \
+      o.slope.v[e] = act_slope<CT>(A, z.v[e]);                \
+    }                                                         \
+    break;
+  switch (act) {
+    MC_ACT_CASE(MC_ACT_RELU)
+    MC_ACT_CASE(MC_ACT_GELU)
+    MC_ACT_CASE(MC_ACT_GELU_TANH)
+    MC_ACT_CASE(MC_ACT_SILU)
+    MC_ACT_CASE(MC_ACT_SIGMOID)
+    MC_ACT_CASE(MC_ACT_NONE)
+  }
+#undef MC_ACT_CASE
+  return o;
 }
 
 // ---- kernels on the CUDA cores (mix_simt.cu) -----------------------------------------------------------------

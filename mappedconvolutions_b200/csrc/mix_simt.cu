@@ -134,6 +134,16 @@ __device__ __forceinline__ void load_run(const T* p, long long step, T (&v)[W], 
   for (int e = 0; e < W; ++e) v[e] = e < n ? p[e * step] : T(0);
 }
 
+template <typename T, int W>
+__device__ __forceinline__ void act_run(int act, const T (&v)[W], T (&o)[W]) {
+  Values<T, W> z;
+#pragma unroll
+  for (int e = 0; e < W; ++e) z.v[e] = v[e];
+  if (act) z = act_value_call<T, W>(act, z);
+#pragma unroll
+  for (int e = 0; e < W; ++e) o[e] = z.v[e];
+}
+
 struct RowsFlags {
   bool a_kfast, w_kfast;   // which direction of a and w is contiguous
   bool vec_y, vec_z, vec_r;  // runs of y, z, res are aligned (see aligned_runs)
@@ -207,7 +217,8 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 ? 2 : 1) rows_kernel(const
         const T bj = bias ? bias[n0 + n] : T(0);
         T v[4], o[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = acc[4 * h + e][j] + bj, o[e] = a.act ? act_value_call<T>(a.act, v[e]) : v[e];
+        for (int e = 0; e < 4; ++e) v[e] = acc[4 * h + e][j] + bj;
+        act_run(a.act, v, o);
         if (whole) {
           const long long c = n0 + n;
           if (z) store_run(z + b * a.z.img + s * a.z.pix + c * a.z.ch, a.z.pix, v, 4, f.vec_z);
@@ -252,8 +263,8 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 ? 2 : 1) rows_kernel(const
 #pragma unroll
         for (int e = 0; e < W; ++e) {
           v[e] = acc[i][W * h + e] + (bias && e < left ? bias[c + e] : T(0));
-          o[e] = a.act ? act_value_call<T>(a.act, v[e]) : v[e];
         }
+        act_run(a.act, v, o);
         if (z) store_run(zr + c * a.z.ch, a.z.ch, v, left, f.vec_z);
         if (res) {
           T q[W];
@@ -268,8 +279,10 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 ? 2 : 1) rows_kernel(const
         for (int e = 0; e < W; ++e) {
           v[e] = acc[i][e] + (bias && e < left ? bias[c + e] : T(0));
           u[e] = acc[i][W + e] + (bias && e < left ? bias[a.N + c + e] : T(0));
-          o[e] = act_value_call<T>(a.act, v[e]) * u[e];
         }
+        act_run(a.act, v, o);
+#pragma unroll
+        for (int e = 0; e < W; ++e) o[e] *= u[e];
         if (z) {
           store_run(zr + c * a.z.ch, a.z.ch, v, left, f.vec_z);
           store_run(zr + (a.N + c) * a.z.ch, a.z.ch, u, left, f.vec_z);
@@ -279,11 +292,14 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 ? 2 : 1) rows_kernel(const
         T g[W], u[W];
         load_run(rr + c * a.res.ch, a.res.ch, g, left, f.vec_r);
         load_run(rr + (a.N + c) * a.res.ch, a.res.ch, u, left, f.vec_r);
+        Values<T, W> z;
+#pragma unroll
+        for (int e = 0; e < W; ++e) z.v[e] = g[e];
+        const ActBoth<T, W> both = act_both_call<T, W>(a.act, z);
 #pragma unroll
         for (int e = 0; e < W; ++e) {
-          const ActBoth<T> f = act_both_call<T>(a.act, g[e]);
-          v[e] = acc[i][W * h + e] * u[e] * f.slope;
-          o[e] = acc[i][W * h + e] * f.value;
+          v[e] = acc[i][W * h + e] * u[e] * both.slope.v[e];
+          o[e] = acc[i][W * h + e] * both.value.v[e];
         }
         store_run(yr + c * a.y.ch, a.y.ch, v, left, f.vec_y);
         store_run(yr + (a.N + c) * a.y.ch, a.y.ch, o, left, f.vec_y);
