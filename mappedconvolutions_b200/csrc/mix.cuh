@@ -90,7 +90,7 @@ __device__ __forceinline__ CT act_slope(int act, CT z) {
 
 // The same as calls, for kernels whose threads hold many values in registers: inlined for each of them the elementary
 // functions would be more code than the instruction cache holds (a 50 -> 99 channel layer of 131 072 pixels took 196 us
-// instead of 117).  W values per call, whose latencies overlap.
+// instead of 117).  W values per call, whose latencies overlap: 90 us instead of 106.
 template <typename CT, int W>
 struct Values {
   CT v[W];

@@ -5,7 +5,9 @@
 // 256 threads, 8 x TN / 16 per thread from shared memory, which asynchronous copies of single elements fill three slices
 // ahead: element by element because nothing promises alignment (an icosphere has 10 * 4^l + 2 vertices, so that a channel
 // of an NCHW tensor starts on any multiple of 8 bytes), and because a copy can then land transposed.  A thread's rows lie
-// at one distance from each other, so that a copy costs an addition and a comparison.
+// at one distance from each other, so that a copy costs an addition and a comparison.  4 x 128 x 256 pixels in NCHW, 50 -> 99
+// channels, SiLU: layer 90 us, input gradient 52 us, weight and bias gradient 64 us (30 - 50 % of the FMA peak, padding
+// counted).
 #include "mix.cuh"
 
 namespace mc {
