@@ -314,6 +314,9 @@ template <int MODE, int BN> struct Cfg {
   static constexpr int CW = MODE == GATE_BWD ? 32 : 64;
   static constexpr int NCH = (MODE == GATE_BWD ? 2 : 1) * BN / CW;           // staged tiles
   static constexpr int CH_BYTES = TILE * CW * 2;
+  // 2^SLOT_BITS slots for staged tiles in each set.  (The gate's gradients with two: 11 % slower.  One, where that makes room
+  // for weights that stay: 512 -> 512 channels, 163 872 pixels 146 us instead of 115.)
+  static constexpr int SLOT_BITS = MODE == GATE_BWD ? 2 : 1;
   // Accumulators in TMEM: as many as fit, since an epilogue's latencies are hidden by the tiles behind it.
   static constexpr int NACC = MODE == GATE_BWD || N0 > 128 ? 2 : 4, ACC = 512 / NACC;
   static constexpr int B0 = N0 / 2 * KB * 2, B1 = N1 / 2 * KB * 2;           // a block's weights per stage
@@ -332,7 +335,7 @@ struct alignas(64) GemmArgs {
   bf16* planes;
   PixDiv pd;
   int group;         // channel tiles of a pair of blocks whose weights stay in shared memory, 0: none do
-  int stages, slot_bits;  // 2^slot_bits slots for staged tiles in each set
+  int stages;
 };
 
 constexpr int ROWS_BARS = 2 * MAX_STAGES + 1 + 8 + 16 + 1 + 2;
@@ -387,14 +390,14 @@ __device__ __forceinline__ void read_out(const GemmArgs& g, int set, uint32_t ra
   typedef Cfg<MODE, BN> C;
   constexpr int NP = BN / 16, PER = C::CW / 16;  // pieces of a tile, and of a staged tile
   const int lane = threadIdx.x % 32, q = threadIdx.x / 32 & 3, row = q * 32 + lane;
-  const uint32_t buf = out0 + (set << g.slot_bits) * C::CH_BYTES, mask = (1u << g.slot_bits) - 1;
+  const uint32_t buf = out0 + (set << C::SLOT_BITS) * C::CH_BYTES, mask = (1u << C::SLOT_BITS) - 1;
   const uint32_t tempty0 = of_leader(bfull + BAR_TEMPTY);
   // 16-byte piece j of this row of a staged tile
   const uint32_t at0 = buf + row * C::CW * 2, swizzle = (C::CW == 64 ? row & 7 : (row >> 1) & 3) << 4;
   const auto slot = [&](uint32_t i) { return at0 + (i & mask) * C::CH_BYTES; };
   const auto bar_of = [&](uint32_t base, uint32_t i) { return bfull + base + 32 * set + 8 * (i & mask); };
   const auto slot_ready = [&](uint32_t i) {
-    return warp_wait(bar_of(BAR_READY, i), i >> g.slot_bits & 1, abort_flag, 0x132);
+    return warp_wait(bar_of(BAR_READY, i), i >> C::SLOT_BITS & 1, abort_flag, 0x132);
   };
   const auto slot_done = [&](uint32_t i) {
     fence_proxy_async_smem();
@@ -537,7 +540,7 @@ __global__ void __launch_bounds__(THREADS, 1) rows_tc_kernel(const __grid_consta
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   volatile int* abort_flag = &abort_flag_s;
   const uint32_t out0 = smem_u32(sm);
-  const uint32_t a0 = out0 + (2 << g.slot_bits) * C::CH_BYTES;
+  const uint32_t a0 = out0 + (2 << C::SLOT_BITS) * C::CH_BYTES;
   const uint32_t b0 = a0 + g.stages * A_BYTES;
   const uint32_t btile = g.kb[0] * C::B0 + g.kb[1] * C::B1;  // a channel tile's weights
   const int bbytes = g.group ? g.group * btile : g.stages * C::BMAX;
@@ -672,7 +675,7 @@ __global__ void __launch_bounds__(THREADS, 1) rows_tc_kernel(const __grid_consta
       TileWalk lead(g, set, 2);
       int lead_c = 0;
       uint32_t lead_i = 0;
-      const uint32_t buf = out0 + (set << g.slot_bits) * C::CH_BYTES, slots = 1u << g.slot_bits;
+      const uint32_t buf = out0 + (set << C::SLOT_BITS) * C::CH_BYTES, slots = 1u << C::SLOT_BITS;
       const auto column = [&](const TileWalk& w, int c) { return w.nt() * BN + (MODE == GATE_BWD ? c / 2 : c) * C::CW; };
       const auto advance = [&]() {
         if (!lead.more()) return;
@@ -693,7 +696,7 @@ __global__ void __launch_bounds__(THREADS, 1) rows_tc_kernel(const __grid_consta
       for (TileWalk w(g, set, 2); w.more() && ok; w.next())
         for (int c = 0; c < C::NCH; ++c, ++i) {
           const uint32_t s = i & (slots - 1);
-          ok = mbar_wait(done(set, s), i >> g.slot_bits & 1, abort_flag, 0x121);
+          ok = mbar_wait(done(set, s), i >> C::SLOT_BITS & 1, abort_flag, 0x121);
           if (!ok) break;
           const int col = column(w, c), m0 = (w.m() * 2 + rank) * TILE;
           if (col < g.N && m0 < g.rows && !(MODE == LAYER && g.planes)) {
@@ -964,13 +967,14 @@ static int launch_rows(GemmArgs& g, cudaStream_t st) {
   g.n_tiles = (g.N + BN - 1) / BN;
   const int fixed_bytes = 1024 + 4 * 256 * 4 + ROWS_BARS * 8 + 16 + 64;
   const int b_tile = g.kb[0] * C::B0 + g.kb[1] * C::B1, pairs = sm_total() / 2;
-  g.slot_bits = MODE == GATE_BWD ? 2 : 1;
-  int left = SMEM_LIMIT - fixed_bytes - (2 << g.slot_bits) * C::CH_BYTES;
-  // Weights stay in shared memory where at least three stages of pixels fit beside them.  How many channel tiles a pair
-  // keeps: the number that leaves the fewest pairs without work; more tiles cost stages, below four of which the pixels'
-  // latency shows.
+  const int left = SMEM_LIMIT - fixed_bytes - (2 << C::SLOT_BITS) * C::CH_BYTES;
+  // Weights stay in shared memory where at least three stages of pixels fit beside them (128 -> 256 channels, 655 488 pixels:
+  // 167 us, 225 us with weights that travel).  How many channel tiles a pair keeps: the number that leaves the fewest pairs
+  // without work; more tiles cost stages, below four of which the pixels' latency shows.  The gate's gradients, two
+  // operands of pixels and small tiles, need the room for stages (256 -> 1024 channels, 163 872 pixels: 380 us, 451 us with
+  // weights that stay).
   double best = 0;
-  for (int group = 1; group <= g.n_tiles; ++group) {
+  for (int group = 1; MODE != GATE_BWD && group <= g.n_tiles; ++group) {
     const int groups = g.n_tiles / group;
     if (g.n_tiles % group || groups > pairs) continue;
     if ((long long)group * b_tile + 3 * A_BYTES > left) break;
@@ -978,12 +982,9 @@ static int launch_rows(GemmArgs& g, cudaStream_t st) {
     const double used = (double)(pairs / groups * groups) / pairs * (stages >= 4 ? 1.0 : 0.93);
     if (used > best + 1e-9) best = used, g.group = group;
   }
-  if (!g.group && MODE != GATE_BWD && g.n_tiles <= pairs && b_tile + 3 * A_BYTES <= left + 2 * C::CH_BYTES)
-    g.group = 1, g.slot_bits = 0, left += 2 * C::CH_BYTES;  // one slot per set makes room for one tile's
-
   g.stages = g.group ? (left - g.group * b_tile) / A_BYTES : left / (A_BYTES + C::BMAX);
   if (g.stages > MAX_STAGES) g.stages = MAX_STAGES;
-  const size_t smem = fixed_bytes + (2 << g.slot_bits) * C::CH_BYTES + (size_t)g.stages * A_BYTES +
+  const size_t smem = fixed_bytes + (2 << C::SLOT_BITS) * C::CH_BYTES + (size_t)g.stages * A_BYTES +
                       (g.group ? g.group * b_tile : g.stages * C::BMAX);
   long long n;
   if (g.group) {
