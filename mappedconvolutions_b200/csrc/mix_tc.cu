@@ -973,8 +973,12 @@ static int launch_rows(GemmArgs& g, cudaStream_t st) {
   // without work; more tiles cost stages, below four of which the pixels' latency shows.  The gate's gradients, two
   // operands of pixels and small tiles, need the room for stages (256 -> 1024 channels, 163 872 pixels: 380 us, 451 us with
   // weights that stay).
+  // Where a pair has a tile or two only, weights that stay are weights that are waited for (2 562 pixels, 680 -> 256
+  // channels, 44 tiles: 11.6 us, 9.0 us if they travel with the pixels; 128 -> 512, 88 tiles: 9.7 and 6.9; the gate with
+  // 64 -> 256 channels, 82 tiles: 18.8 and 20.5 for the block).
+  const bool stay = MODE != GATE_BWD && (long long)g.m_pairs * g.n_tiles > (MODE == GATE ? 1 : 2) * pairs;
   double best = 0;
-  for (int group = 1; MODE != GATE_BWD && group <= g.n_tiles; ++group) {
+  for (int group = 1; stay && group <= g.n_tiles; ++group) {
     const int groups = g.n_tiles / group;
     if (g.n_tiles % group || groups > pairs) continue;
     if ((long long)group * b_tile + 3 * A_BYTES > left) break;
