@@ -263,6 +263,10 @@ __device__ __forceinline__ void pair_commit(uint32_t bar) {
                "h"((uint16_t)3)
                : "memory");
 }
+// the same at this barrier of the issuing block alone
+__device__ __forceinline__ void leader_commit(uint32_t bar) {
+  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
 
 // ---- TMA ---------------------------------------------------------------------------------------------
 __device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* tm, int x, int y, uint32_t bar) {
@@ -618,6 +622,12 @@ __global__ void __launch_bounds__(THREADS, 1) rows_tc_kernel(const __grid_consta
           if (++st == (uint32_t)g.stages) st = 0, ph ^= 1;
         }
     }
+    // Every arrival that the leader's commits send here is waited for: a block that left before one came would have its
+    // shared memory written behind it.
+    for (int i = 0; i < g.stages && ok; ++i) {
+      ok = __all_sync(~0u, mbar_wait(empty(st), ph ^ 1, abort_flag, 0x102));
+      if (++st == (uint32_t)g.stages) st = 0, ph ^= 1;
+    }
   } else if (warp == 1) {
     // ---- MMA issuer, in the leader only
     if (rank == 0) {
@@ -663,7 +673,7 @@ __global__ void __launch_bounds__(THREADS, 1) rows_tc_kernel(const __grid_consta
         __syncwarp();
       }
       if (elected) {
-        pair_commit(drain);
+        leader_commit(drain);  // (nobody in the other block waits for it)
         mbar_wait(drain, 0, abort_flag, 0x114);
       }
       __syncwarp();
@@ -780,8 +790,10 @@ __global__ void __launch_bounds__(THREADS, 1) outer_tc_kernel(const __grid_const
   if (warp == 0) {  // (converged, one elected lane issues: see the rows kernel)
     const bool elected = elect_one();
     uint32_t st = 0, ph = 0;
-    for (int k = k0; k < k1; ++k) {
-      if (!__all_sync(~0u, mbar_wait(empty(st), ph ^ 1, abort_flag, 0x141))) break;
+    bool ok = true;
+    for (int k = k0; k < k1 && ok; ++k) {
+      ok = __all_sync(~0u, mbar_wait(empty(st), ph ^ 1, abort_flag, 0x141));
+      if (!ok) break;
       if (elected) {
         const uint32_t bar = of_leader(full(st)), dst = s0 + st * STAGE;
         if (rank == 0) mbar_expect_tx(full(st), 2 * STAGE);
@@ -793,6 +805,10 @@ __global__ void __launch_bounds__(THREADS, 1) outer_tc_kernel(const __grid_const
           tma_load_pair(dst + GB + i * 8192, &g.x, n0 + rank * (BN / 2) + 64 * i, k * KB, bar);
       }
       __syncwarp();
+      if (++st == (uint32_t)g.stages) st = 0, ph ^= 1;
+    }
+    for (int i = 0; i < g.stages && ok; ++i) {  // (no arrival of the leader's commits is left behind)
+      ok = __all_sync(~0u, mbar_wait(empty(st), ph ^ 1, abort_flag, 0x145));
       if (++st == (uint32_t)g.stages) st = 0, ph ^= 1;
     }
   } else if (warp == 1) {

@@ -1,0 +1,44 @@
+"""GPU: the paths that the channel-mixing kernels take for large layers, and what they leave behind."""
+import math
+
+import pytest
+import torch
+
+from mappedconvolutions_b200 import host
+
+pytestmark = pytest.mark.gpu
+BF, F32, F64 = torch.bfloat16, torch.float32, torch.float64
+
+
+@pytest.fixture(autouse=True)
+def no_wait_ran_out():
+    """a bounded wait that gives up after the results are stored shows in the device status only"""
+    yield
+    assert host.impl.device_status(True) == 0
+
+
+def image(g, shape, dtype, layout, scale=1.0):
+    t = (torch.randn(shape, generator=g, device="cuda", dtype=F32) * scale).to(dtype)
+    return t.contiguous(memory_format=torch.channels_last) if layout == "nhwc" else t
+
+
+def params(g, n_out, n_in, dtype):
+    s = 1 / math.sqrt(n_in)
+    u = lambda *shape: ((torch.rand(shape, generator=g, device="cuda") * 2 - 1) * s).to(dtype)
+    return u(n_out, n_in, 1), u(n_out)
+
+
+@pytest.mark.parametrize("channels", [(16, 8), (136, 320), (512, 64)])
+def test_short_kernels_one_behind_the_other(channels):
+    """blocks that end a few microseconds after they start, the next kernel's already waiting: a block may leave only when
+    every arrival and copy of its pair has come"""
+    cin, cout = channels
+    g = torch.Generator("cuda").manual_seed(cin)
+    x, gy = image(g, (1, cin, 1, 300), BF, "nhwc"), image(g, (1, cout, 1, 300), BF, "nhwc")
+    w, b = params(g, cout, cin, BF)
+    y0, saved = host.impl.pointwise_forward(x, w, b, None, 4, True)
+    g0 = host.impl.pointwise_backward(gy, saved, x, w, b, 4)
+    for _ in range(100):
+        y, saved = host.impl.pointwise_forward(x, w, b, None, 4, True)
+        got = host.impl.pointwise_backward(gy, saved, x, w, b, 4)
+    assert torch.equal(y, y0) and all(torch.equal(p, q) for p, q in zip(got, g0))
