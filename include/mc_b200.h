@@ -88,7 +88,9 @@ uint64_t mc_kernel_launch_count(void);
 
 /* Synchronises `stream` and returns the device status word: 0, or the code of the first bounded
  * device-side wait that ran out (the kernel then returned early and its output is invalid).
- * reset != 0 clears the word.  No counterpart in the reference (its kernels have no waits). */
+ * reset != 0 clears what is returned.  The mapped convolutions and the channel-mixing layers have a word each: if waits of
+ * both ran out, one call returns (and clears) the convolutions' code, the next the other.
+ * No counterpart in the reference (its kernels have no waits). */
 int mc_device_status(void* stream, int reset);
 
 /* Self-test of the bounded device-side waits: launches a one-warp kernel that waits about a
@@ -97,6 +99,8 @@ int mc_device_status(void* stream, int reset);
  * receives 2 (the block's abort flag was raised and the wait reported failure).  Nothing faults or
  * hangs.  No counterpart in the reference. */
 int mc_selftest_wait_expiry(int32_t* observed_dev, void* stream);
+/* The same with the status word of the channel-mixing layers, which then holds 0x7F2. */
+int mc_selftest_mix_wait_expiry(int32_t* observed_dev, void* stream);
 
 /* ---- mapped convolution ---------------------------------------------------------------
  * weight (C_out, C_in, K) and bias (C_out) in `dtype`, contiguous. */

@@ -45,6 +45,7 @@ SIGNATURES = {
     "mc_kernel_launch_count": (ctypes.c_uint64, []),
     "mc_device_status": (ctypes.c_int, [_vp, ctypes.c_int]),
     "mc_selftest_wait_expiry": (ctypes.c_int, [_vp, _vp]),
+    "mc_selftest_mix_wait_expiry": (ctypes.c_int, [_vp, _vp]),
     "mc_conv_fwd": (ctypes.c_int, [_dp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
     "mc_conv_fwd_workspace_bytes": (_sz, [_dp]),
     "mc_conv_fwd_static_scratch_limit": (_sz, []),

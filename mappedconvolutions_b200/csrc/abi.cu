@@ -87,8 +87,9 @@ const char* mc_strerror(int code) {
 // ---- conv ----------------------------------------------------------------------------------
 
 int mc_device_status(void* stream, int reset) {
-  const int conv = device_status_read((cudaStream_t)stream, reset), mixing = mix::tc_status_read(reset);
-  return conv ? conv : mixing;
+  // one code per call: a word whose code is not returned is not cleared either
+  const int conv = device_status_read((cudaStream_t)stream, reset);
+  return conv ? conv : mix::tc_status_read(reset);
 }
 
 // Layers with padded output channels ask for a workspace and for aligned tensors only to be faster: without

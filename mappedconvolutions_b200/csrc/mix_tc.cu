@@ -1157,5 +1157,16 @@ int tc_status_read(int reset) {
   return v;
 }
 
+// The waits' self-test on this file's status word.
+constexpr int SELFTEST_STATUS = 0x7F2;
+
 }  // namespace mix
 }  // namespace mc
+
+extern "C" int mc_selftest_mix_wait_expiry(int32_t* observed_dev, void* stream) {
+  using namespace mc;
+  tc::wait_expiry_selftest_kernel<<<1, 32, 0, (cudaStream_t)stream>>>(mix::SELFTEST_STATUS, 2000000LL, observed_dev),
+      MC_COUNT(1);
+  MC_CHECK_LAUNCH();
+  return MC_OK;
+}

@@ -240,5 +240,24 @@ __device__ __forceinline__ uint32_t pack_bf16x2(float lo, float hi) {
   return *reinterpret_cast<uint32_t*>(&v);
 }
 
+// ---- self-test of the bounded waits ---------------------------------------------------------------
+// One warp waits, with a limit of about a millisecond, on an mbarrier that nobody ever arrives at.
+// The wait must give up, raise the block's abort flag and the device status word, and the kernel
+// must return: the same path a tensor-core kernel takes if one of its roles stops answering.
+static __global__ void wait_expiry_selftest_kernel(int code, long long limit_cycles, int* observed) {
+  __shared__ uint64_t bar;
+  __shared__ int abort_flag, wait_ok;
+  if (threadIdx.x == 0) {
+    mbar_init(smem_u32(&bar), 1);
+    abort_flag = 0;
+    fence_barrier_init();
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) wait_ok = mbar_wait(smem_u32(&bar), 0, &abort_flag, code, 64, limit_cycles) ? 1 : 0;
+  __syncthreads();
+  // the other lanes see the abort flag, as the roles of a real kernel do
+  if (threadIdx.x == 1 && observed) *observed = (abort_flag ? 2 : 0) | (wait_ok ? 1 : 0);
+}
+
 }  // namespace tc
 }  // namespace mc

@@ -42,3 +42,17 @@ def test_short_kernels_one_behind_the_other(channels):
         y, saved = host.impl.pointwise_forward(x, w, b, None, 4, True)
         got = host.impl.pointwise_backward(gy, saved, x, w, b, 4)
     assert torch.equal(y, y0) and all(torch.equal(p, q) for p, q in zip(got, g0))
+
+
+def test_waits_of_both_kinds_of_kernels_are_reported():
+    """the convolutions' and the channel-mixing kernels' status words, one code a call, none cleared unread"""
+    from mappedconvolutions_b200 import _lib
+    L, st = _lib.lib(), torch.cuda.current_stream().cuda_stream
+    assert L.mc_device_status(st, 1) == 0
+    seen = torch.zeros(2, dtype=torch.int32, device="cuda")
+    _lib.check(L.mc_selftest_mix_wait_expiry(seen[:1].data_ptr(), st))
+    _lib.check(L.mc_selftest_wait_expiry(seen[1:].data_ptr(), st))
+    assert L.mc_device_status(st, 0) == 0x7F1 and seen.tolist() == [2, 2]
+    assert [L.mc_device_status(st, 1) for _ in range(3)] == [0x7F1, 0x7F2, 0]
+    _lib.check(L.mc_selftest_mix_wait_expiry(None, st))
+    assert [L.mc_device_status(st, r) for r in (0, 1, 0)] == [0x7F2, 0x7F2, 0]
