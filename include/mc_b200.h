@@ -436,6 +436,20 @@ int mc_gated_fwd(const mc_mix_desc* d, const void* x, const void* w_in, const vo
 int mc_gated_bwd(const mc_mix_desc* d, const void* gy, const void* x, const void* w_in, const void* b_in,
                  const void* w_out, const void* saved, void* gx, void* gw_in, void* gb_in, void* gw_out, void* gb_out, void* ws,
                  size_t ws_bytes, void* stream);
+/* Diagnostic: how the MC_BF16 kernels of a call divide a product on a GPU of `sms` SMs (0: the current device's).  Six
+ * numbers for products with weights: channels of a tile, channel tiles, pairs of pixel tiles (256 pixels), channel tiles
+ * whose weights a pair of blocks keeps (0: weights travel), pairs of blocks, pipeline stages.  For MC_MIX_WEIGHT_*GRAD:
+ * rows and columns of a tile, tiles along the rows (both halves of w_in) and columns, shares of the pixels, 64-pixel blocks
+ * of a share.  MC_ERR_BAD_ARG for a product that d's call has not. */
+enum {
+  MC_MIX_OUTPUT = 0,         /* y (of the pointwise layer, or from h) */
+  MC_MIX_GATE = 1,           /* h */
+  MC_MIX_ACT_GRAD = 2,       /* gradients of the pre-activations */
+  MC_MIX_INPUT_GRAD = 3,
+  MC_MIX_WEIGHT_GRAD = 4,    /* of w or w_in */
+  MC_MIX_WEIGHT_OUT_GRAD = 5
+};
+int mc_mix_plan(const mc_mix_desc* d, int32_t product, int32_t sms, int32_t* plan);
 
 /* ---- norm of many gradients, clipping ----------------------------------------------------------
  * No counterpart in the reference.  n tensors, given as HOST arrays: device pointers, element counts (0 allowed) and

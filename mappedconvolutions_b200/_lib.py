@@ -112,6 +112,7 @@ SIGNATURES = {
     "mc_gated_workspace_bytes": (_sz, [_mp, _i32]),
     "mc_gated_fwd": (ctypes.c_int, [_mp] + [_vp] * 9 + [_sz, _vp]),
     "mc_gated_bwd": (ctypes.c_int, [_mp] + [_vp] * 12 + [_sz, _vp]),
+    "mc_mix_plan": (ctypes.c_int, [_mp, _i32, _i32, _ip]),
     "mc_grad_workspace_bytes": (_sz, [_i32]),
     "mc_grad_norm": (ctypes.c_int, [_i32, _pp, _lp, _ip, _f64, _vp, _vp, _vp, _sz, _vp]),
     "mc_grad_clip": (ctypes.c_int, [_i32, _pp, _ip, _pp, _ip, _lp, _f64, _f64, _vp, _vp, _vp, _sz, _vp]),

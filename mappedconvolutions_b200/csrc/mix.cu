@@ -408,6 +408,14 @@ using namespace mc::mix;
 
 extern "C" {
 
+int mc_mix_plan(const mc_mix_desc* d, int32_t product, int32_t sms, int32_t* plan) {
+  const int rc = check_desc(d, d && d->hidden != 0);
+  if (rc) return rc;
+  if (!plan || sms < 0) return MC_ERR_BAD_ARG;
+  if (d->dtype != MC_BF16) return MC_ERR_UNSUPPORTED;
+  return tc_plan(d, product, sms, plan) ? MC_OK : MC_ERR_BAD_ARG;
+}
+
 // ---- pointwise layer ----------------------------------------------------------------------------------------
 
 // kept for the backward pass: z in y's layout; bf16: the input as rows, where it is not rows already

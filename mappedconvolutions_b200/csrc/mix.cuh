@@ -189,6 +189,8 @@ int tc_gate_bwd(const TcRows& x, const TcRows& w_in, const bf16* b_in, int act, 
 // part[s] = the s-th share of [g0|g1]^T x (rows of *ldn floats), csum[s] = its column sums of [g0|g1]; g1.p may be null
 size_t tc_outer_floats(long long P, int M, int segs, int N, int* splits, int* ldn);
 int tc_outer(const TcRows& g0, const TcRows& g1, const TcRows& x, float* part, float* csum, cudaStream_t st);
+// mc_mix_plan for a checked bf16 description; false: no such product
+bool tc_plan(const mc_mix_desc* d, int product, int sms, int32_t* out);
 
 }  // namespace mix
 }  // namespace mc

@@ -977,12 +977,19 @@ static int launch_pairs(unsigned pairs, size_t smem, const Args& args, cudaStrea
   return MC_OK;
 }
 
+struct RowsPlan {
+  int bn, n_tiles, group, stages;
+  unsigned pairs;  // of blocks that are launched
+  size_t smem;
+};
 template <int MODE, int BN>
-static int launch_rows(GemmArgs& g, cudaStream_t st) {
+static RowsPlan plan_rows(int m_pairs, int N, int kb0, int kb1, int sms) {
   typedef Cfg<MODE, BN> C;
-  g.n_tiles = (g.N + BN - 1) / BN;
+  RowsPlan p{};
+  p.bn = BN;
+  p.n_tiles = (N + BN - 1) / BN;
   const int fixed_bytes = 1024 + 4 * 256 * 4 + ROWS_BARS * 8 + 16 + 64;
-  const int b_tile = g.kb[0] * C::B0 + g.kb[1] * C::B1, pairs = sm_total() / 2;
+  const int b_tile = kb0 * C::B0 + kb1 * C::B1, pairs = sms / 2;
   const int left = SMEM_LIMIT - fixed_bytes - (2 << C::SLOT_BITS) * C::CH_BYTES;
   // Weights stay in shared memory where at least three stages of pixels fit beside them (128 -> 256 channels, 655 488 pixels:
   // 167 us, 225 us with weights that travel).  How many channel tiles a pair keeps: the number that leaves the fewest pairs
@@ -992,39 +999,47 @@ static int launch_rows(GemmArgs& g, cudaStream_t st) {
   // Where a pair has a tile or two only, weights that stay are weights that are waited for (2 562 pixels, 680 -> 256
   // channels, 44 tiles: 11.6 us, 9.0 us if they travel with the pixels; 128 -> 512, 88 tiles: 9.7 and 6.9; the gate with
   // 64 -> 256 channels, 82 tiles: 18.8 and 20.5 for the block).
-  const bool stay = MODE != GATE_BWD && (long long)g.m_pairs * g.n_tiles > (MODE == GATE ? 1 : 2) * pairs;
+  const bool stay = MODE != GATE_BWD && (long long)m_pairs * p.n_tiles > (MODE == GATE ? 1 : 2) * pairs;
   double best = 0;
-  for (int group = 1; stay && group <= g.n_tiles; ++group) {
-    const int groups = g.n_tiles / group;
-    if (g.n_tiles % group || groups > pairs) continue;
+  for (int group = 1; stay && group <= p.n_tiles; ++group) {
+    const int groups = p.n_tiles / group;
+    if (p.n_tiles % group || groups > pairs) continue;
     if ((long long)group * b_tile + 3 * A_BYTES > left) break;
     const int stages = (left - group * b_tile) / A_BYTES;
     const double used = (double)(pairs / groups * groups) / pairs * (stages >= 4 ? 1.0 : 0.93);
-    if (used > best + 1e-9) best = used, g.group = group;
+    if (used > best + 1e-9) best = used, p.group = group;
   }
-  g.stages = g.group ? (left - g.group * b_tile) / A_BYTES : left / (A_BYTES + C::BMAX);
-  if (g.stages > MAX_STAGES) g.stages = MAX_STAGES;
-  const size_t smem = fixed_bytes + (2 << C::SLOT_BITS) * C::CH_BYTES + (size_t)g.stages * A_BYTES +
-                      (g.group ? g.group * b_tile : g.stages * C::BMAX);
+  p.stages = p.group ? (left - p.group * b_tile) / A_BYTES : left / (A_BYTES + C::BMAX);
+  if (p.stages > MAX_STAGES) p.stages = MAX_STAGES;
+  p.smem = fixed_bytes + (2 << C::SLOT_BITS) * C::CH_BYTES + (size_t)p.stages * A_BYTES +
+                      (p.group ? p.group * b_tile : p.stages * C::BMAX);
   long long n;
-  if (g.group) {
-    const int groups = g.n_tiles / g.group;
+  if (p.group) {
+    const int groups = p.n_tiles / p.group;
     n = pairs / groups;
-    if (n > g.m_pairs) n = g.m_pairs;
+    if (n > m_pairs) n = m_pairs;
     n *= groups;
   } else {
-    n = (long long)g.m_pairs * g.n_tiles;
+    n = (long long)m_pairs * p.n_tiles;
     if (n > pairs) n = pairs;
   }
-  return launch_pairs<rows_tc_kernel<MODE, BN>>((unsigned)n, smem, g, st);
+  p.pairs = (unsigned)n;
+  return p;
+}
+
+template <int MODE, int BN>
+static int launch_rows(GemmArgs& g, cudaStream_t st) {
+  const RowsPlan p = plan_rows<MODE, BN>(g.m_pairs, g.N, g.kb[0], g.kb[1], sm_total());
+  g.n_tiles = p.n_tiles, g.group = p.group, g.stages = p.stages;
+  return launch_pairs<rows_tc_kernel<MODE, BN>>(p.pairs, p.smem, g, st);
 }
 
 // Channels of a tile, for `pairs` pixel tiles, n channels, kb stages: the least estimated time.  A tile costs its MMAs
 // (half a cycle per column and 16 channels, not less than its stages' hand-over), its read-out and a start; many pixels
 // want wide tiles, few pixels so many tiles that every pair of blocks has one (680 -> 256 channels at 2 562 pixels, 11
 // pixel tiles: 14.2 us with one tile of 256 columns each).
-static int tile_width(long long pairs, int n, int kb) {
-  const int all = sm_total() / 2;
+static int tile_width(long long pairs, int n, int kb, int sms) {
+  const int all = sms / 2;
   int best = 64;
   double least = 1e300;
   for (int w = 64; w <= 256; w *= 2) {
@@ -1057,7 +1072,7 @@ int tc_layer(const TcRows& a, const TcRows& w, const bf16* bias, int act, const 
              bool backward, cudaStream_t st) {
   GemmArgs g = base_args(a, y, bias, act);
   g.res = r.p != nullptr;
-  const int bn = tile_width(g.m_pairs, y.cols, g.kb[0]);
+  const int bn = tile_width(g.m_pairs, y.cols, g.kb[0], sm_total());
   if (!encode(&g.a[0], a, TILE) || !encode(&g.b[0], w, bn / 2)) return MC_ERR_LAUNCH;
   if (y.ld == 0) g.planes = (bf16*)y.p, g.pd = PixDiv((uint32_t)y.S);
   else if (!encode(&g.y[0], y, TILE)) return MC_ERR_LAUNCH;
@@ -1069,7 +1084,7 @@ int tc_input_grad(const TcRows& g0, const TcRows& w0, const TcRows& g1, const Tc
                   cudaStream_t st) {
   GemmArgs g = base_args(g0, gx, nullptr, MC_ACT_NONE);
   if (g1.p) g.kb[1] = kblocks(g1.cols);
-  const int bn = tile_width(g.m_pairs, gx.cols, g.kb[0] + g.kb[1]);
+  const int bn = tile_width(g.m_pairs, gx.cols, g.kb[0] + g.kb[1], sm_total());
   if (!encode(&g.a[0], g0, TILE) || !encode(&g.b[0], w0, bn / 2)) return MC_ERR_LAUNCH;
   if (gx.ld == 0) g.planes = (bf16*)gx.p, g.pd = PixDiv((uint32_t)gx.S);
   else if (!encode(&g.y[0], gx, TILE)) return MC_ERR_LAUNCH;
@@ -1077,11 +1092,13 @@ int tc_input_grad(const TcRows& g0, const TcRows& w0, const TcRows& g1, const Tc
   return launch_wide<LAYER>(g, bn, st);
 }
 
+// 128 hidden channels a tile of the gate, 64 where that pads less: 38 hidden channels take half the time (wide blocks 4 % more)
+static int gate_width(int hidden) { return hidden <= 256 && (hidden + 63) / 64 % 2 ? 64 : 128; }
+
 int tc_gate(const TcRows& x, const TcRows& w_in, const bf16* b_in, int act, const TcRows& h, cudaStream_t st) {
   GemmArgs g = base_args(x, h, b_in, act);
   g.up = h.cols;
-  // 128 hidden channels a tile, 64 where that pads less: 38 hidden channels take half the time (wide blocks 4 % more)
-  const int wide = h.cols <= 256 && (h.cols + 63) / 64 % 2 ? 64 : 128;
+  const int wide = gate_width(h.cols);
   if (!encode(&g.a[0], x, TILE) || !encode(&g.b[0], w_in, wide) || !encode(&g.y[0], h, TILE)) return MC_ERR_LAUNCH;
   return wide == 64 ? launch_rows<GATE, 64>(g, st) : launch_rows<GATE, 128>(g, st);
 }
@@ -1101,7 +1118,7 @@ int tc_gate_bwd(const TcRows& x, const TcRows& w_in, const bf16* b_in, int act, 
 struct OuterPlan {
   int mt, bn, m_tiles, n_tiles, splits, per;
 };
-static OuterPlan outer_plan(long long P, int M, int segs, int N) {
+static OuterPlan outer_plan(long long P, int M, int segs, int N, int sms) {
   OuterPlan p;
   p.mt = M > 256 ? 2 : 1;
   p.bn = N <= 128 ? 128 : 256;
@@ -1110,7 +1127,7 @@ static OuterPlan outer_plan(long long P, int M, int segs, int N) {
   const long long tiles = (long long)segs * p.m_tiles * p.n_tiles, kb = (P + KB - 1) / KB;
   double best = 1e30;
   p.splits = 1, p.per = (int)kb;
-  const int pairs = sm_total() / 2;
+  const int pairs = sms / 2;
   for (long long s = 1; s <= pairs && s <= (kb + 3) / 4; ++s) {
     const long long per = (kb + s - 1) / s;
     const double waves = (double)((tiles * s + pairs - 1) / pairs);
@@ -1121,7 +1138,7 @@ static OuterPlan outer_plan(long long P, int M, int segs, int N) {
   return p;
 }
 size_t tc_outer_floats(long long P, int M, int segs, int N, int* splits, int* ldn) {
-  const OuterPlan p = outer_plan(P, M, segs, N);
+  const OuterPlan p = outer_plan(P, M, segs, N, sm_total());
   *splits = p.splits;
   *ldn = (N + 3) / 4 * 4;
   return (size_t)p.splits * segs * M * *ldn;
@@ -1137,7 +1154,7 @@ static int launch_outer(OuterTcArgs& g, const OuterPlan& p, cudaStream_t st) {
 int tc_outer(const TcRows& g0, const TcRows& g1, const TcRows& x, float* part, float* csum, cudaStream_t st) {
   OuterTcArgs g{};
   g.segs = g1.p ? 2 : 1;
-  const OuterPlan p = outer_plan(x.rows, g0.cols, g.segs, x.cols);
+  const OuterPlan p = outer_plan(x.rows, g0.cols, g.segs, x.cols, sm_total());
   if (!encode(&g.g[0], g0, KB) || (g1.p && !encode(&g.g[1], g1, KB)) || !encode(&g.x, x, KB)) return MC_ERR_LAUNCH;
   g.part = part, g.csum = csum;
   g.M = g0.cols, g.N = x.cols, g.ldn = (x.cols + 3) / 4 * 4;
@@ -1145,6 +1162,48 @@ int tc_outer(const TcRows& g0, const TcRows& g1, const TcRows& x, float* part, f
   g.kblocks = (int)((x.rows + KB - 1) / KB), g.per = p.per;
   if (p.mt == 1) return p.bn == 128 ? launch_outer<1, 128>(g, p, st) : launch_outer<1, 256>(g, p, st);
   return p.bn == 128 ? launch_outer<2, 128>(g, p, st) : launch_outer<2, 256>(g, p, st);
+}
+
+// ---- what the rules above choose ------------------------------------------------------------------------------
+template <int MODE>
+static RowsPlan plan_wide(int m_pairs, int N, int kb0, int kb1, int sms) {
+  const int bn = tile_width(m_pairs, N, kb0 + kb1, sms);
+  return bn == 64 ? plan_rows<MODE, 64>(m_pairs, N, kb0, kb1, sms)
+         : bn == 128 ? plan_rows<MODE, 128>(m_pairs, N, kb0, kb1, sms) : plan_rows<MODE, 256>(m_pairs, N, kb0, kb1, sms);
+}
+bool tc_plan(const mc_mix_desc* d, int product, int sms, int32_t* out) {
+  if (sms == 0) sms = sm_total();
+  const long long P = d->B * d->S;
+  const int m = (int)((P + 2 * TILE - 1) / (2 * TILE)), H = d->hidden;
+  const int ki = kblocks(d->C_in), ko = kblocks(d->C_out), kh = kblocks(H ? H : 1);
+  if (sms < 2 || sms > 4096) return false;
+  RowsPlan p{};
+  OuterPlan o{};
+  switch (product) {
+    case MC_MIX_OUTPUT: p = plan_wide<LAYER>(m, d->C_out, H ? kh : ki, 0, sms); break;
+    case MC_MIX_GATE:
+      if (!H) return false;
+      p = gate_width(H) == 64 ? plan_rows<GATE, 64>(m, H, ki, 0, sms) : plan_rows<GATE, 128>(m, H, ki, 0, sms);
+      break;
+    case MC_MIX_ACT_GRAD:
+      p = H ? plan_rows<GATE_BWD, 64>(m, H, ki, ko, sms) : plan_wide<ACT_BWD>(m, d->C_out, ki, 0, sms);
+      break;
+    case MC_MIX_INPUT_GRAD: p = plan_wide<LAYER>(m, d->C_in, H ? kh : ko, H ? kh : 0, sms); break;
+    case MC_MIX_WEIGHT_GRAD: o = H ? outer_plan(P, H, 2, d->C_in, sms) : outer_plan(P, d->C_out, 1, d->C_in, sms); break;
+    case MC_MIX_WEIGHT_OUT_GRAD:
+      if (!H) return false;
+      o = outer_plan(P, d->C_out, 1, H, sms);
+      break;
+    default: return false;
+  }
+  if (o.mt) {
+    const int v[6] = {256 * o.mt, o.bn, o.m_tiles * (product == MC_MIX_WEIGHT_GRAD && H ? 2 : 1), o.n_tiles, o.splits, o.per};
+    for (int i = 0; i < 6; ++i) out[i] = v[i];
+  } else {
+    const int v[6] = {p.bn, p.n_tiles, m, p.group, (int)p.pairs, p.stages};
+    for (int i = 0; i < 6; ++i) out[i] = v[i];
+  }
+  return true;
 }
 
 int tc_status_read(int reset) {

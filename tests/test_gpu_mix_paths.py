@@ -4,6 +4,8 @@ import math
 import pytest
 import torch
 
+import mix_reference as R
+import mix_strict as M
 from mappedconvolutions_b200 import host
 
 pytestmark = pytest.mark.gpu
@@ -56,3 +58,31 @@ def test_waits_of_both_kinds_of_kernels_are_reported():
     assert [L.mc_device_status(st, 1) for _ in range(3)] == [0x7F1, 0x7F2, 0]
     _lib.check(L.mc_selftest_mix_wait_expiry(None, st))
     assert [L.mc_device_status(st, r) for r in (0, 1, 0)] == [0x7F2, 0x7F2, 0]
+
+
+@pytest.mark.parametrize("i", range(len(M.PATHS)))
+def test_paths(i):
+    """every way of dividing the products, as the table beside the reference says"""
+    from mappedconvolutions_b200 import _lib
+    case, ways = M.PATHS[i]
+    b, h, w, cin, hidden, cout, layout, name, residual = case
+    if torch.cuda.get_device_properties(0).multi_processor_count == 148:
+        assert {k: M.plan(_lib.lib(), M.path_desc(case), k, 0)[0] for k in ways} == ways
+    g = torch.Generator("cuda").manual_seed(50 + i)
+    x, gy = image(g, (b, cin, h, w), BF, layout), image(g, (b, cout, h, w), BF, layout, 0.01)
+    r = image(g, (b, cout, h, w), BF, layout) if residual else None
+    act = R.ACTS[name]
+    if hidden:
+        wi, bi = params(g, 2 * hidden, cin, BF)
+        wo, bo = params(g, cout, hidden, BF)
+        y, saved = host.impl.gated_forward(x, wi, bi, wo, bo, r, act, True)
+        call = lambda: host.impl.gated_backward(gy, saved, x, wi, bi, wo, act)
+        names, want = ("gx", "gw_in", "gb_in", "gw_out", "gb_out"), M.gated(x, wi, bi, wo, bo, r, name, gy)
+    else:
+        weight, bias = params(g, cout, cin, BF)
+        y, saved = host.impl.pointwise_forward(x, weight, bias, r, act, True)
+        call = lambda: host.impl.pointwise_backward(gy, saved, x, weight, bias, act)
+        names, want = ("gx", "gw", "gb"), M.pointwise(x, weight, bias, r, name, gy)
+    grads = call()
+    R.check(dict(zip(names, grads), y=y), want, str(case))
+    assert all(torch.equal(p, q) for p, q in zip(grads, call()))  # fixed order of every sum
