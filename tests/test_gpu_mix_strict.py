@@ -1,0 +1,41 @@
+"""GPU: channel mixing against bounds that hold pre-activations to float32 sums; few channels, so that one value's error shows."""
+import pytest
+import torch
+
+import mix_reference as R
+import mix_strict as M
+from mappedconvolutions_b200 import host
+
+pytestmark = pytest.mark.gpu
+BF, F32, F64 = torch.bfloat16, torch.float32, torch.float64
+
+
+@pytest.fixture(autouse=True)
+def no_wait_ran_out():
+    yield
+    assert host.impl.device_status(True) == 0
+
+
+def normal(g, shape, dtype, layout=None, scale=1.0):
+    t = (torch.randn(shape, generator=g, device="cuda") * scale).to(dtype)
+    return t.contiguous(memory_format=torch.channels_last) if layout == "nhwc" else t
+
+
+@pytest.mark.parametrize("dtype", [BF, F32, F64], ids=["bf16", "f32", "f64"])
+@pytest.mark.parametrize("layout", ["nhwc", "nchw"])
+@pytest.mark.parametrize("name", [None, "relu", "gelu", "gelu_tanh", "silu"])
+def test_pre_activations_are_float32(name, layout, dtype):
+    for i, (cin, hidden, cout) in enumerate([(2, 1, 1), (8, 2, 3), (5, 8, 16)]):
+        g = torch.Generator("cuda").manual_seed(30 + i)
+        x, gy = normal(g, (2, cin, 37, 61), dtype, layout), normal(g, (2, cout, 37, 61), dtype, layout)
+        r = normal(g, (2, cout, 37, 61), dtype, layout) if i else None
+        w, b = normal(g, (cout, cin, 1), dtype, scale=3 / cin ** 0.5), normal(g, (cout,), dtype)
+        y, saved = host.impl.pointwise_forward(x, w, b, r, R.ACTS[name], True)
+        got = host.impl.pointwise_backward(gy, saved, x, w, b, R.ACTS[name])
+        R.check(dict(zip(("gx", "gw", "gb"), got), y=y), M.pointwise(x, w, b, r, name, gy), str((cin, cout)))
+        wi, bi = normal(g, (2 * hidden, cin, 1), dtype, scale=3 / cin ** 0.5), normal(g, (2 * hidden,), dtype)
+        wo, bo = normal(g, (cout, hidden, 1), dtype), normal(g, (cout,), dtype)
+        y, saved = host.impl.gated_forward(x, wi, bi, wo, bo, r, R.ACTS[name], True)
+        got = host.impl.gated_backward(gy, saved, x, wi, bi, wo, R.ACTS[name])
+        R.check(dict(zip(("gx", "gw_in", "gb_in", "gw_out", "gb_out"), got), y=y), M.gated(x, wi, bi, wo, bo, r, name, gy),
+                str((cin, hidden, cout)))
