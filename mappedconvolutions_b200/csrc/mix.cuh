@@ -80,9 +80,9 @@ __device__ __forceinline__ CT act_slope(int act, CT z) {
       const CT s = CT(1) / (CT(1) + exp_(-z));
       return s * (CT(1) + z * (CT(1) - s));
     }
-    case MC_ACT_SIGMOID: {
-      const CT s = CT(1) / (CT(1) + exp_(-z));
-      return s * (CT(1) - s);
+    case MC_ACT_SIGMOID: {  // s(z) s(-z) with e = exp(-|z|): 1 - s(z) would cancel
+      const CT e = exp_(-fabs(z)), q = CT(1) / (CT(1) + e);
+      return e * q * q;
     }
     default: return CT(1);
   }

@@ -165,9 +165,16 @@ struct ActSigmoid {
     MC_EACH z[j] = mul2(z[j], two(-LOG2E));
     logistic(z);
   }
-  __device__ static void both(Pairs& z, Pairs& s) {
-    value(z);
-    MC_EACH s[j] = mul2(z[j], fma2(z[j], two(-1.f), two(1.f)));
+  __device__ static void both(Pairs& z, Pairs& s) {  // slope s(z) s(-z), e = 2^(-|z| log2 e): 1 - s(z) would cancel
+    Pairs e;
+    MC_EACH e[j] = mul2(make_float2(fabsf(z[j].x), fabsf(z[j].y)), two(-LOG2E));
+    MC_EACH e[j] = exp2_2(e[j]);
+    MC_EACH s[j] = rcp2(add2(e[j], two(1.f)));
+    MC_EACH {
+      const float2 q = s[j], m = mul2(e[j], q);
+      s[j] = mul2(m, q);
+      z[j] = make_float2(z[j].x < 0.f ? m.x : q.x, z[j].y < 0.f ? m.y : q.y);
+    }
   }
 };
 template <typename F>

@@ -39,3 +39,30 @@ def test_pre_activations_are_float32(name, layout, dtype):
         got = host.impl.gated_backward(gy, saved, x, wi, bi, wo, R.ACTS[name])
         R.check(dict(zip(("gx", "gw_in", "gb_in", "gw_out", "gb_out"), got), y=y), M.gated(x, wi, bi, wo, bo, r, name, gy),
                 str((cin, hidden, cout)))
+
+
+def one_channel(z, name, dtype):
+    """act(z) and act'(z) for every element of z, through a layer with one channel, weight one and bias zero"""
+    x = z.view(1, 1, 1, -1)
+    w, b = torch.ones(1, 1, 1, device="cuda", dtype=dtype), torch.zeros(1, device="cuda", dtype=dtype)
+    y, saved = host.impl.pointwise_forward(x, w, b, None, R.ACTS[name], True)
+    gx = host.impl.pointwise_backward(torch.ones_like(x), saved, x, w, b, R.ACTS[name], True, False)[0]
+    return y.view(-1).double(), gx.view(-1).double()
+
+
+def error_of_functions(dtype):
+    return {BF: 2.0 ** -15, F32: 2.0 ** -20, F64: 2.0 ** -48}[dtype]
+
+
+@pytest.mark.parametrize("dtype", [BF, F32, F64], ids=["bf16", "f32", "f64"])
+def test_sigmoid_and_its_slope_are_accurate_relative_to_their_values(dtype):
+    z = torch.cat([torch.linspace(-80, 80, 4001, device="cuda"), torch.linspace(-1, 1, 501, device="cuda")]).to(dtype)
+    y, s = one_channel(z, "sigmoid", dtype)
+    zd = z.double()
+    e = (-zd.abs()).exp()
+    q = 1 / (1 + e)
+    bound = torch.finfo(dtype).eps / 2 + error_of_functions(dtype)
+    assert ((y - torch.where(zd < 0, e * q, q)).abs() <= bound * y.abs()).all()
+    want = e * q * q
+    worst = ((s - want).abs() / want).max().item()
+    assert worst <= bound, worst
