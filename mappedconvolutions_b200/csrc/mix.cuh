@@ -74,7 +74,8 @@ __device__ __forceinline__ CT act_slope(int act, CT z) {
     case MC_ACT_GELU_TANH: {
       const CT c = CT(0.79788456080286535588), z2 = z * z;
       const CT t = tanh_(c * (z + CT(0.044715) * z2 * z));
-      return CT(0.5) * (CT(1) + t) + CT(0.5) * z * (CT(1) - t * t) * c * (CT(1) + CT(0.134145) * z2);
+      // (z^2 can overflow where 1 - t^2 is zero: kept finite, the product is zero as it should be)
+      return CT(0.5) * (CT(1) + t) + CT(0.5) * z * (CT(1) - t * t) * c * fmin(CT(1) + CT(0.134145) * z2, CT(3e38));
     }
     case MC_ACT_SILU: {
       const CT s = CT(1) / (CT(1) + exp_(-z));

@@ -137,10 +137,11 @@ struct ActGeluTanh {  // (1 + tanh(a)) / 2 is the logistic function of 2 a
   __device__ static void both(Pairs& z, Pairs& s) {
     Pairs p;
     part(z, p);
-    MC_EACH {
+    MC_EACH {  // (z^2 can overflow where p or 1 - p is zero: kept finite, the product is zero as it should be)
       const float2 v = mul2(z[j], p[j]);
-      s[j] = fma2(mul2(v, fma2(p[j], two(-1.f), two(1.f))),
-                  fma2(mul2(z[j], two(1.59576912f * 0.134145f)), z[j], two(1.59576912f)), p[j]);
+      float2 d = fma2(mul2(z[j], two(1.59576912f * 0.134145f)), z[j], two(1.59576912f));
+      d = make_float2(fminf(d.x, 3e38f), fminf(d.y, 3e38f));
+      s[j] = fma2(mul2(v, fma2(p[j], two(-1.f), two(1.f))), d, p[j]);
       z[j] = v;
     }
   }

@@ -66,3 +66,22 @@ def test_sigmoid_and_its_slope_are_accurate_relative_to_their_values(dtype):
     want = e * q * q
     worst = ((s - want).abs() / want).max().item()
     assert worst <= bound, worst
+
+
+@pytest.mark.parametrize("dtype", [BF, F32, F64], ids=["bf16", "f32", "f64"])
+@pytest.mark.parametrize("name", [None, "relu", "gelu", "gelu_tanh", "silu", "sigmoid"])
+def test_large_finite_values(name, dtype):
+    """where squares and exponentials of z overflow, act(z) is z or zero (sigmoid: one or zero), act'(z) one or zero"""
+    top = torch.finfo(dtype).max
+    z = torch.tensor([50.0, 1e6, 1e18, 3e19, 1e30, top / 4, top], device="cuda", dtype=F64).to(dtype)
+    y, s = one_channel(z, name, dtype)
+    ym, sm = one_channel(-z, name, dtype)
+    if name == "sigmoid":
+        assert ((y - 1).abs() <= 2.0 ** -8).all() and (ym.abs() <= 1e-21).all()
+        assert (s.abs() <= 1e-21).all() and (sm.abs() <= 1e-21).all()  # (e^-50 = 2e-22)
+        return
+    assert torch.equal(y, z.double()) and torch.equal(s, torch.ones_like(s))
+    if name is None:
+        assert torch.equal(ym, -y) and torch.equal(sm, s)
+    else:
+        assert (ym.abs() <= 1e-19).all() and (sm.abs() <= 1e-19).all()  # (50 e^-50 = 1e-20)
