@@ -1125,7 +1125,10 @@ int tc_gate_bwd(const TcRows& x, const TcRows& w_in, const bf16* b_in, int act, 
   return launch_rows<GATE_BWD, 64>(g, st);
 }
 
-// Blocks per gradient tile: as many as fill the SMs once or a whole number of times with equal shares.
+// Blocks per gradient tile: as many as fill the SMs once or a whole number of times with equal shares, of 2^17 pixels at most:
+// the accumulators truncate, up to 2^-23 of the sum for every sixteen pixels, which does not cancel where all terms have one
+// sign (2^30 pixels, 8 x 8 channels: 9 % off with 74 shares; 2^17 pixels: 2^-10, a quarter of half a bf16 step).
+constexpr int MOST_PER = (1 << 17) / KB;
 struct OuterPlan {
   int mt, bn, m_tiles, n_tiles, splits, per;
 };
@@ -1137,9 +1140,10 @@ static OuterPlan outer_plan(long long P, int M, int segs, int N, int sms) {
   p.n_tiles = (N + p.bn - 1) / p.bn;
   const long long tiles = (long long)segs * p.m_tiles * p.n_tiles, kb = (P + KB - 1) / KB;
   double best = 1e30;
-  p.splits = 1, p.per = (int)kb;
   const int pairs = sms / 2;
-  for (long long s = 1; s <= pairs && s <= (kb + 3) / 4; ++s) {
+  const long long least = (kb + MOST_PER - 1) / MOST_PER;
+  p.splits = 1, p.per = (int)kb;
+  for (long long s = least; s < least + pairs && s <= (kb + 3) / 4; ++s) {
     const long long per = (kb + s - 1) / s;
     const double waves = (double)((tiles * s + pairs - 1) / pairs);
     // a pair's stages, and what it costs to write its sums and to add them up again

@@ -86,3 +86,18 @@ def test_paths(i):
     grads = call()
     R.check(dict(zip(names, grads), y=y), want, str(case))
     assert all(torch.equal(p, q) for p, q in zip(grads, call()))  # fixed order of every sum
+
+
+def test_parameter_gradients_of_a_thousand_million_pixels():
+    """Sums whose terms have one sign, where what a sum loses does not cancel.  A share is 2^17 pixels at most: 2^13 additions
+    to an accumulator that truncates (at most 2^-23 of it, 2^-10 in all), 2^13 float32 additions of a column's sum (2^-11),
+    half a bf16 step of the result (2^-8), and float32 sums of 2^13 shares in 32 parts (2^-15)."""
+    g = torch.Generator("cuda").manual_seed(61)
+    block, times = (torch.rand(1 << 16, 8, generator=g, device="cuda") + 0.5).to(BF), 1 << 14
+    x = block.repeat(times, 1).view(1, 1, -1, 8).permute(0, 3, 1, 2)
+    w, b = torch.zeros(8, 8, 1, device="cuda", dtype=BF), torch.zeros(8, device="cuda", dtype=BF)
+    _, gw, gb = host.impl.pointwise_backward(x, None, x, w, b, 0, False, True)
+    d = block.double()
+    off = [((got.double() - want) / want).abs().max().item()
+           for got, want in ((gw[:, :, 0], d.T @ d * times), (gb, d.sum(0) * times))]
+    assert max(off) <= 2.0 ** -8 + 2.0 ** -10 + 2.0 ** -15, off
