@@ -1295,6 +1295,27 @@ OptTensor linear_layer(int64_t op, const Tensor& x, const Tensor& map, const Opt
   return LinearFn::apply(x, map, iw, op, oh, ow, K, interp);
 }
 
+// Behind the gradients of a backward call that is recorded (create_graph): the layers below have no second derivatives, and
+// a loss that asks for them must not train without them.  The node leads to what the gradients depend on, so that a
+// backward call for any of it comes through here.
+struct NoSecondDerivative : torch::autograd::Node {
+  variable_list apply(variable_list&&) override {
+    TORCH_CHECK(false, "second derivatives of the channel-mixing layers are not available");
+  }
+};
+void without_second(const variable_list& grads, const variable_list& inputs) {
+  if (!at::GradMode::is_enabled()) return;
+  const std::shared_ptr<NoSecondDerivative> node(new NoSecondDerivative(), torch::autograd::deleteNode);
+  torch::autograd::edge_list edges;
+  bool any = false;
+  for (const Tensor& t : inputs)
+    if (t.defined() && t.requires_grad()) edges.push_back(torch::autograd::impl::gradient_edge(t)), any = true;
+  if (!any) return;
+  node->set_next_edges(std::move(edges));
+  for (const Tensor& t : grads)
+    if (t.defined()) torch::autograd::impl::set_gradient_edge(t, {node, node->add_input_metadata(t)});
+}
+
 struct PointwiseFn : torch::autograd::Function<PointwiseFn> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const Tensor& b, const OptTensor& r,
                         int64_t act) {
@@ -1310,6 +1331,7 @@ struct PointwiseFn : torch::autograd::Function<PointwiseFn> {
     variable_list out(5);
     if (need_x || need_p) {
       auto r = pointwise_backward(g[0], as_opt(s[3]), s[0], s[1], s[2], ctx->saved_data["a"].toInt(), need_x, need_p);
+      without_second(r, {g[0], s[0], s[1], s[2]});
       for (int i = 0; i < 3; ++i) out[i] = r[i];
     }
     if (ctx->saved_data["r"].toBool() && ctx->needs_input_grad(3)) out[3] = g[0];
@@ -1334,6 +1356,7 @@ struct GatedFn : torch::autograd::Function<GatedFn> {
     variable_list out(7);
     if (need_x || need_p) {
       auto r = gated_backward(g[0], as_opt(s[4]), s[0], s[1], s[2], s[3], ctx->saved_data["a"].toInt(), need_x, need_p);
+      without_second(r, {g[0], s[0], s[1], s[2], s[3]});
       for (int i = 0; i < 5; ++i) out[i] = r[i];
     }
     if (ctx->saved_data["r"].toBool() && ctx->needs_input_grad(5)) out[5] = g[0];

@@ -193,6 +193,18 @@ class UnresampleFn(Function):
         return gx, None, None, None
 
 
+class FirstDerivative(Function):
+    """compute()'s gradients, which depend on `inputs`; a backward call through them is refused, not left out"""
+
+    @staticmethod
+    def forward(ctx, compute, *inputs):
+        return tuple(compute())
+
+    @staticmethod
+    def backward(ctx, *g):
+        raise RuntimeError("second derivatives of the channel-mixing layers are not available")
+
+
 class PointwiseFn(Function):
     """act(W x + bias) + residual at every pixel (no counterpart in the reference)"""
 
@@ -209,7 +221,8 @@ class PointwiseFn(Function):
         need = ctx.needs_input_grad
         g = [None] * 3
         if any(need[:3]):
-            g = ops.pointwise_backward(gy, saved, x, weight, bias, ctx.activation, need[0], need[1] or need[2])
+            g = FirstDerivative.apply(lambda: ops.pointwise_backward(gy, saved, x, weight, bias, ctx.activation, need[0],
+                                                                     need[1] or need[2]), gy, x, weight, bias)
         return (*g, gy if need[3] else None, None)
 
 
@@ -229,8 +242,8 @@ class GatedFn(Function):
         need = ctx.needs_input_grad
         g = [None] * 5
         if any(need[:5]):
-            g = ops.gated_backward(gy, saved, x, weight_in, bias_in, weight_out, ctx.activation, need[0],
-                                   any(need[1:5]))
+            g = FirstDerivative.apply(lambda: ops.gated_backward(gy, saved, x, weight_in, bias_in, weight_out, ctx.activation,
+                                                                 need[0], any(need[1:5])), gy, x, weight_in, bias_in, weight_out)
         return (*g, gy if need[5] else None, None)
 
 

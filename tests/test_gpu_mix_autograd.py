@@ -1,0 +1,36 @@
+"""GPU: what the channel-mixing layers keep and refuse under autograd."""
+import pytest
+import torch
+
+from mappedconvolutions_b200 import nn as mnn
+
+pytestmark = pytest.mark.gpu
+BF, F32 = torch.bfloat16, torch.float32
+
+
+def layers(dtype):
+    return [mnn.PointwiseConvolution(16, 24, activation="silu").cuda().to(dtype), mnn.GatedFeedForward(16, 32, 24).cuda().to(dtype)]
+
+
+@pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "f32"])
+def test_second_derivatives_are_refused(dtype):
+    for m in layers(dtype):
+        x = torch.randn(2, 16, 5, 7, device="cuda").to(dtype).requires_grad_(True)
+        w = next(m.parameters())
+        first = torch.autograd.grad(m(x).float().sum(), [x, w])
+        gx, gw = torch.autograd.grad(m(x).float().sum(), [x, w], create_graph=True)
+        assert torch.equal(gx, first[0]) and torch.equal(gw, first[1]) and not first[0].requires_grad
+        for g in (gx, gw):
+            for leaf in (x, w):
+                with pytest.raises(RuntimeError, match="second derivatives"):
+                    torch.autograd.grad(g.float().square().sum(), leaf, retain_graph=True, allow_unused=True)
+        with pytest.raises(RuntimeError, match="second derivatives"):
+            (m(x).float().sum() + gx.float().square().sum()).backward()
+
+
+def test_a_residuals_gradient_is_linear():
+    for m in layers(F32):
+        m.requires_grad_(False)
+        x, r = torch.randn(2, 16, 5, 7, device="cuda"), torch.randn(2, 24, 5, 7, device="cuda", requires_grad=True)
+        gr, = torch.autograd.grad(m(x, r).square().sum(), r, create_graph=True)
+        assert torch.equal(torch.autograd.grad(gr.sum(), r)[0], torch.full_like(r, 2.0))
