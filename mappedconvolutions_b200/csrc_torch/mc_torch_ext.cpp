@@ -1319,7 +1319,8 @@ void without_second(const variable_list& grads, const variable_list& inputs) {
 struct PointwiseFn : torch::autograd::Function<PointwiseFn> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const Tensor& b, const OptTensor& r,
                         int64_t act) {
-    auto f = pointwise_forward(x, w, b, r, act, true);
+    // (a residual's gradient alone needs nothing of the forward call)
+    auto f = pointwise_forward(x, w, b, r, act, x.requires_grad() || w.requires_grad() || b.requires_grad());
     ctx->save_for_backward({x, w, b, f.second});
     ctx->saved_data["a"] = act;
     ctx->saved_data["r"] = r.has_value();  // (needs_input_grad counts the tensors that were given)
@@ -1342,7 +1343,8 @@ struct PointwiseFn : torch::autograd::Function<PointwiseFn> {
 struct GatedFn : torch::autograd::Function<GatedFn> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& wi, const Tensor& bi, const Tensor& wo,
                         const Tensor& bo, const OptTensor& r, int64_t act) {
-    auto f = gated_forward(x, wi, bi, wo, bo, r, act, true);
+    const bool keep = x.requires_grad() || wi.requires_grad() || bi.requires_grad() || wo.requires_grad() || bo.requires_grad();
+    auto f = gated_forward(x, wi, bi, wo, bo, r, act, keep);
     ctx->save_for_backward({x, wi, bi, wo, f.second});
     ctx->saved_data["a"] = act;
     ctx->saved_data["r"] = r.has_value();  // (needs_input_grad counts the tensors that were given)

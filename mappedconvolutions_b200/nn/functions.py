@@ -211,7 +211,8 @@ class PointwiseFn(Function):
     @staticmethod
     def forward(ctx, x, weight, bias, residual, activation):
         ctx.activation = int(activation)
-        y, saved = ops.pointwise_forward(x, weight, bias, residual, ctx.activation, True)
+        # (a residual's gradient alone needs nothing of the forward call)
+        y, saved = ops.pointwise_forward(x, weight, bias, residual, ctx.activation, any(ctx.needs_input_grad[:3]))
         ctx.save_for_backward(x, weight, bias, saved)
         return y
 
@@ -232,7 +233,8 @@ class GatedFn(Function):
     @staticmethod
     def forward(ctx, x, weight_in, bias_in, weight_out, bias_out, residual, activation):
         ctx.activation = int(activation)
-        y, saved = ops.gated_forward(x, weight_in, bias_in, weight_out, bias_out, residual, ctx.activation, True)
+        y, saved = ops.gated_forward(x, weight_in, bias_in, weight_out, bias_out, residual, ctx.activation,
+                                     any(ctx.needs_input_grad[:5]))
         ctx.save_for_backward(x, weight_in, bias_in, weight_out, saved)
         return y
 

@@ -34,3 +34,25 @@ def test_a_residuals_gradient_is_linear():
         x, r = torch.randn(2, 16, 5, 7, device="cuda"), torch.randn(2, 24, 5, 7, device="cuda", requires_grad=True)
         gr, = torch.autograd.grad(m(x, r).square().sum(), r, create_graph=True)
         assert torch.equal(torch.autograd.grad(gr.sum(), r)[0], torch.full_like(r, 2.0))
+
+
+@pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "f32"])
+def test_nothing_is_kept_for_a_residual_alone(dtype):
+    def held(m, *args):
+        before = torch.cuda.memory_allocated()
+        y = m(*args)
+        return torch.cuda.memory_allocated() - before, y
+
+    x = torch.randn(2, 16, 50, 70, device="cuda").to(dtype)  # (NCHW: bf16 training calls keep its rows)
+    r = torch.randn(2, 24, 50, 70, device="cuda").to(dtype)
+    for m in layers(dtype):
+        m(x, r)  # (the first call's allocations)
+        with torch.no_grad():
+            least, _ = held(m, x, r)
+        assert held(m, x, r)[0] > least
+        m.requires_grad_(False)
+        got, y = held(m, x, r.requires_grad_(True))
+        assert got == least
+        y.float().sum().backward()
+        assert torch.equal(r.grad, torch.ones_like(r))
+        r = r.detach()

@@ -55,3 +55,16 @@ def test_a_residuals_gradient_is_linear(stand_ins):
         x, r = torch.rand(1, 1, 2, 3), torch.rand(1, 1, 2, 3, requires_grad=True)
         gr, = torch.autograd.grad(layer(x, r).square().sum(), r, create_graph=True)
         assert torch.equal(torch.autograd.grad(gr.sum(), r)[0], torch.full_like(r, 2.0))
+
+
+def test_nothing_is_kept_for_a_residual_alone(stand_ins):
+    for layer, w in layers():
+        x, r = torch.rand(1, 1, 2, 3), torch.rand(1, 1, 2, 3, requires_grad=True)
+        stand_ins.clear()
+        layer(x, r)
+        assert stand_ins == [("forward", True)]  # (the parameters)
+    frozen = [torch.rand(2, 1, 1), torch.rand(2), torch.rand(1, 1, 1), torch.rand(1)]
+    for call in (lambda: F.PointwiseFn.apply(x, frozen[2], frozen[3], r, 0), lambda: F.GatedFn.apply(x, *frozen, r, 4)):
+        stand_ins.clear()
+        call().sum().backward()
+        assert stand_ins == [("forward", False)] and r.grad is not None
