@@ -290,13 +290,17 @@ static int fill(Table<N>& t, const Lists& l, int at) {
 static int check_lists(const Lists& l, bool scale) {
   if (l.n < 0 || (l.n && (!l.src || !l.src_type || !l.numel || (scale && (!l.dst || !l.dst_type))))) return MC_ERR_BAD_ARG;
   const auto known = [](int t) { return t == MC_F32 || t == MC_F64 || t == MC_BF16; };
+  constexpr long long MOST = 1 << 30;  // chunks, which are counted in int
   long long chunks = 0;
+  bool many = false;  // (no sum is formed that could overflow; what is wrong with a later tensor is still reported first)
   for (int i = 0; i < l.n; ++i) {
     if (l.numel[i] < 0 || !known(l.src_type[i]) || (scale && !known(l.dst_type[i]))) return MC_ERR_BAD_ARG;
     if (l.numel[i] && (!l.src[i] || (scale && !l.dst[i]))) return MC_ERR_BAD_ARG;
-    chunks += (l.numel[i] + CHUNK - 1) / CHUNK;
+    const long long more = l.numel[i] / CHUNK + (l.numel[i] % CHUNK != 0);
+    many = many || more >= MOST || chunks + more >= MOST;
+    if (!many) chunks += more;
   }
-  return chunks < (1 << 30) ? MC_OK : MC_ERR_TOO_LARGE;
+  return many ? MC_ERR_TOO_LARGE : MC_OK;
 }
 
 template <typename... A>
