@@ -1142,6 +1142,15 @@ Tensor clip_gradients(const std::vector<Tensor>& tensors, double max_norm, doubl
     if (from != begin || s.scalar_type() != d.scalar_type())
       spans.emplace_back(from, from + s.numel() * s.element_size(), false);
   }
+  // results that are copied to where they belong: dense ones share memory with no other result
+  std::vector<std::pair<uintptr_t, uintptr_t>> finals;
+  for (const Tensor& o : outs)
+    if (o.numel())
+      finals.emplace_back((uintptr_t)o.data_ptr(),
+                          (uintptr_t)o.data_ptr() + (o.is_non_overlapping_and_dense() ? o.numel() : 1) * o.element_size());
+  std::sort(finals.begin(), finals.end());
+  for (size_t i = 1; i < finals.size(); ++i)
+    TORCH_CHECK(finals[i].first >= finals[i - 1].second, "gradients to scale must not share memory with each other");
   std::sort(spans.begin(), spans.end());
   uintptr_t end_any = 0, end_dst = 0;  // no destination may share memory with another tensor of the call
   for (const auto& [begin, end, is_dst] : spans) {

@@ -950,9 +950,12 @@ def _check_gradients(tensors, norm_type):
         raise RuntimeError("norm_type must be 1, 2 or infinity")
 
 
-def _check_apart(pairs, strided=()):
-    """No destination may share memory with another tensor of the call.  Of strided results only the first elements are
-    compared: what lies between the others may belong to anyone."""
+def _check_apart(pairs, outs, strided=()):
+    """No destination may share memory with another tensor of the call, no dense result with another result.  Of strided
+    results only the first elements are compared: what lies between the others may belong to anyone."""
+    finals = sorted((o.data_ptr(), o.data_ptr() + (o.numel() if _dense(o) else 1) * o.element_size()) for o in outs if o.numel())
+    if any(b[0] < a[1] for a, b in zip(finals, finals[1:])):
+        raise RuntimeError("gradients to scale must not share memory with each other")
     spans = [(t.data_ptr(), t.data_ptr() + t.element_size(), True) for t in strided if t.numel()]
     for src, dst in pairs:
         if dst.numel():
@@ -1014,7 +1017,7 @@ def clip_gradients(tensors, max_norm, norm_type=2.0, out=None):
         src.append(g.contiguous())
         dst.append(torch.empty(g.shape, dtype=o.dtype, device=dev))
         back.append((o, dst[-1]))
-    _check_apart(list(zip(src, dst)), [o for o, _ in back])
+    _check_apart(list(zip(src, dst)), outs, [o for o, _ in back])
     norm, p64, p32 = _norm_out(grads, dev)
     ct, n = _lib.ctypes, len(src)
     with torch.cuda.device(dev):
