@@ -1114,6 +1114,9 @@ Tensor clip_gradients(const std::vector<Tensor>& tensors, double max_norm, doubl
   const std::vector<Tensor>& outs = out.has_value() ? *out : tensors;
   TORCH_CHECK(outs.size() == tensors.size(), "out must have as many tensors as there are gradients");
   check_gradients(outs, norm_type, dev);
+  for (const Tensor& o : outs)  // (as torch's own in-place operations, but before anything is written)
+    TORCH_CHECK(!o.is_inference() || c10::InferenceMode::is_enabled(),
+                "a tensor made in inference mode can be scaled in place in inference mode only");
   c10::cuda::CUDAGuard guard(dev);
   at::NoGradGuard no_grad;
   GradLists l;

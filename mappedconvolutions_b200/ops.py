@@ -1003,6 +1003,8 @@ def clip_gradients(tensors, max_norm, norm_type=2.0, out=None):
     if len(outs) != len(grads):
         raise RuntimeError("out must have as many tensors as there are gradients")
     _check_gradients(outs, norm_type)
+    if any(o.is_inference() for o in (tensors if out is None else out)) and not torch.is_inference_mode_enabled():
+        raise RuntimeError("a tensor made in inference mode can be scaled in place in inference mode only")
     dev = _need_cuda(*grads, *outs)
     src, dst, back = [], [], []
     for g, o in zip(grads, outs):

@@ -27,3 +27,17 @@ def test_dense_results_in_another_order_share_no_memory(ops):
     for got, g in ((a.t(), g0), (b, g1)):
         # (the norm: eight roundings of a float32 sum, half of them behind the root; its own, the coefficient's, the product's)
         assert ((got.double() - g.double() * c).abs() <= 8 * 2.0 ** -24 * (g.double() * c).abs()).all()
+
+
+def test_tensors_of_inference_mode(ops):
+    """refused outside of it before anything is written, scaled inside"""
+    with torch.inference_mode():
+        t = torch.full((100,), 3.0, device="cuda")
+    g = torch.ones(100, device="cuda")
+    for call in (lambda: ops.clip_gradients([t], 1.0), lambda: ops.clip_gradients([g], 1.0, 2.0, [t])):
+        with pytest.raises(RuntimeError, match="inference mode"):
+            call()
+        assert (t == 3.0).all()
+    with torch.inference_mode():
+        assert ops.clip_gradients([t], 1.0).item() == 30.0
+        assert ((t - 0.1).abs() <= 2.0 ** -20).all()
