@@ -460,7 +460,8 @@ int mc_mix_plan(const mc_mix_desc* d, int32_t product, int32_t sms, int32_t* pla
  * a fixed order and repeat bit for bit.
  * mc_grad_clip: the same, and dst[i] = src[i] * min(1, max_norm / (norm + 1e-6)); dst[i] == src[i] is allowed, any other
  * overlap of a dst with a tensor of the call is not.  A NaN norm makes every element NaN.  The coefficient is a double,
- * rounded to float32 for sources that are not MC_F64; products are formed in that type and rounded to dst's. */
+ * rounded to 24 significant bits for sources that are not MC_F64, however small; products are formed in float32 (MC_F64:
+ * double) and rounded to dst's type. */
 size_t mc_grad_workspace_bytes(int32_t n);
 int mc_grad_norm(int32_t n, const void* const* src, const int64_t* numel, const int32_t* dtype, double norm_type,
                  double* norm, float* norm32, void* ws, size_t ws_bytes, void* stream);

@@ -189,11 +189,22 @@ __global__ void __launch_bounds__(THREADS) finish_kernel(int kind, const double*
   }
 }
 
+// A coefficient as c 2^e: where float32 would hold it with fewer bits, or as zero (a norm of 1e38, say, scaled to 1e-3), c has
+// the bits and 2^e the size, and v c 2^e is rounded once, as v c is otherwise (2^e = 1).
+struct Coefficient {
+  double c, power;
+  __device__ explicit Coefficient(double v) : c(v), power(1.0) {
+    if (v > 0 && v < 1e-30) {
+      const int e = max(ilogb(v) + 1, -126);  // c < 1: no product overflows
+      c = ldexp(v, -e), power = ldexp(1.0, e);
+    }
+  }
+};
 template <typename S, typename D>
-__device__ __forceinline__ void scale_chunk(const S* p, D* q, int n, double coefficient) {
+__device__ __forceinline__ void scale_chunk(const S* p, D* q, int n, double factor, double power) {
   typedef typename Traits<S>::CT CT;
   constexpr int ROUND = sizeof(CT) == 4 ? 4 : 2;
-  const CT c = (CT)coefficient;
+  const CT c = (CT)factor, c2 = (CT)power;
   int i = threadIdx.x * 8;
   if ((((uintptr_t)p | (uintptr_t)q) & 15) == 0) {
     // (all loads of a round before its stores: the compiler may not move them across, p and q can be the same)
@@ -204,7 +215,7 @@ __device__ __forceinline__ void scale_chunk(const S* p, D* q, int n, double coef
 #pragma unroll
       for (int r = 0; r < ROUND; ++r) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[r][j] *= c;
+        for (int j = 0; j < 8; ++j) v[r][j] = v[r][j] * c * c2;
         store8(q + i + r * THREADS * 8, v[r]);
       }
     }
@@ -212,26 +223,26 @@ __device__ __forceinline__ void scale_chunk(const S* p, D* q, int n, double coef
       CT v[8];
       load8(p + i, v);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] *= c;
+      for (int j = 0; j < 8; ++j) v[j] = v[j] * c * c2;
       store8(q + i, v);
     }
   }
   for (; i < n; i += THREADS * 8)
-    for (int j = 0; j < 8 && i + j < n; ++j) store1(q + i + j, (CT)ldv(p + i + j) * c);
+    for (int j = 0; j < 8 && i + j < n; ++j) store1(q + i + j, (CT)ldv(p + i + j) * c * c2);
 }
 template <typename S>
-__device__ __forceinline__ void scale_from(const S* p, void* q, int type, long long at, int n, double c) {
+__device__ __forceinline__ void scale_from(const S* p, void* q, int type, long long at, int n, double c, double c2) {
   switch (type) {
-    case MC_F32: scale_chunk(p + at, (float*)q + at, n, c); break;
-    case MC_F64: scale_chunk(p + at, (double*)q + at, n, c); break;
-    default: scale_chunk(p + at, (bf16*)q + at, n, c); break;
+    case MC_F32: scale_chunk(p + at, (float*)q + at, n, c, c2); break;
+    case MC_F64: scale_chunk(p + at, (double*)q + at, n, c, c2); break;
+    default: scale_chunk(p + at, (bf16*)q + at, n, c, c2); break;
   }
 }
 
 template <int N>
 __global__ void __launch_bounds__(THREADS) scale_kernel(const __grid_constant__ Table<N> t, int kind, const double* part,
                                                         int nparts, double max_norm, double* norm, float* norm32) {
-  __shared__ double shared_c;
+  __shared__ double shared_c, shared_c2;
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const double v = finish(kind, part, nparts);
   if (threadIdx.x == 0) {
@@ -240,19 +251,20 @@ __global__ void __launch_bounds__(THREADS) scale_kernel(const __grid_constant__ 
       if (norm32) *norm32 = (float)v;
     }
     const double c = max_norm / (v + 1e-6);
-    shared_c = c > 1.0 ? 1.0 : c;  // (NaN stays NaN)
+    const Coefficient k(c > 1.0 ? 1.0 : c);  // (NaN stays NaN)
+    shared_c = k.c, shared_c2 = k.power;
   }
   __syncthreads();
-  const double c = shared_c;
+  const double c = shared_c, c2 = shared_c2;
   for (int k = t.first[t.n] - 1 - (int)blockIdx.x; k >= 0; k -= gridDim.x) {
     const int i = tensor_of(t, k);
     const long long at = (long long)(k - t.first[i]) * CHUNK;
     const long long left = t.numel[i] - at;
     const int n = left < CHUNK ? (int)left : CHUNK;
     switch (t.src_type[i]) {
-      case MC_F32: scale_from((const float*)t.src[i], t.dst[i], t.dst_type[i], at, n, c); break;
-      case MC_F64: scale_from((const double*)t.src[i], t.dst[i], t.dst_type[i], at, n, c); break;
-      default: scale_from((const bf16*)t.src[i], t.dst[i], t.dst_type[i], at, n, c); break;
+      case MC_F32: scale_from((const float*)t.src[i], t.dst[i], t.dst_type[i], at, n, c, c2); break;
+      case MC_F64: scale_from((const double*)t.src[i], t.dst[i], t.dst_type[i], at, n, c, c2); break;
+      default: scale_from((const bf16*)t.src[i], t.dst[i], t.dst_type[i], at, n, c, c2); break;
     }
   }
 }

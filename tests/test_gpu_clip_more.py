@@ -41,3 +41,22 @@ def test_tensors_of_inference_mode(ops):
     with torch.inference_mode():
         assert ops.clip_gradients([t], 1.0).item() == 30.0
         assert ((t - 0.1).abs() <= 2.0 ** -20).all()
+
+
+@pytest.mark.parametrize("max_norm", [1e-3, 1e-6, 1e-20, 1e-35])
+@pytest.mark.parametrize("source,result", [(F32, F32), (BF, BF), (BF, F32), (F32, F64)])
+def test_coefficients_below_the_float32_range(ops, source, result, max_norm):
+    """gradients that exploded: max_norm / norm is far below 1e-38, its products with the gradients are not"""
+    g = torch.Generator("cuda").manual_seed(2)
+    ts = [(torch.randn(n, generator=g, device="cuda", dtype=F64) * 5e36).to(source) for n in (3, 50_000)]
+    out = [torch.empty(t.shape, device="cuda", dtype=result) for t in ts]
+    norm = torch.cat([t.double().view(-1) for t in ts]).norm().item()
+    ops.clip_gradients(ts, max_norm, 2.0, out)
+    # squares above 1e38 are summed in double; a rounding of the coefficient and of the product, and the result's
+    tol = 2.0 ** -22 + torch.finfo(result).eps / 2
+    # below the normal range steps have a fixed size, tiny * eps (bf16 2^-133, float32 2^-149): half of one of the result's type
+    # (float64: none is reached), and of float32 for each of the two products
+    denormal = torch.finfo(F32).tiny * (torch.finfo(F32).eps + torch.finfo(result).eps / 2)
+    for t, o in zip(ts, out):
+        want = t.double() * (max_norm / norm)
+        assert ((o.double() - want).abs() <= tol * want.abs() + denormal).all()
