@@ -898,6 +898,8 @@ void check_weight_dims(const Tensor& w, const char* name) {
 }
 
 mc_mix_desc make_mix_desc(const Tensor& x, int layout, int64_t c_out, int64_t hidden, int64_t act) {
+  constexpr int64_t most = std::numeric_limits<int32_t>::max();  // (of what the description can hold; the library's limit is lower)
+  TORCH_CHECK(x.size(1) <= most && c_out <= most && hidden <= most, "size beyond a fixed limit: more than 2^31 channels");
   mc_mix_desc d{};
   d.B = x.size(0);
   d.S = x.size(2) * x.size(3);

@@ -798,6 +798,8 @@ def _check_mix(x, params, residual, c_out, grad_output=None):
 def _mix_desc(x, layout, c_out, hidden, activation):
     if x.dtype not in _DT:
         raise RuntimeError("unsupported dtype %s (float32, float64, bfloat16)" % x.dtype)
+    if max(x.shape[1], c_out, hidden) >= 1 << 31:  # (of what the description can hold; the library's limit is lower)
+        raise RuntimeError("size beyond a fixed limit: more than 2^31 channels")
     return _lib.McMixDesc(x.shape[0], x.shape[2] * x.shape[3], x.shape[1], c_out, hidden, int(activation),
                           _DT[x.dtype], layout)
 

@@ -101,3 +101,20 @@ def test_parameter_gradients_of_a_thousand_million_pixels():
     off = [((got.double() - want) / want).abs().max().item()
            for got, want in ((gw[:, :, 0], d.T @ d * times), (gb, d.sum(0) * times))]
     assert max(off) <= 2.0 ** -8 + 2.0 ** -10 + 2.0 ** -15, off
+
+
+@pytest.mark.parametrize("binding", ["ctypes", "compiled"])
+def test_channel_counts_beyond_32_bits_are_refused(binding):
+    """2^32 + 8 channels are not eight"""
+    from mappedconvolutions_b200 import ops as twin
+    ops = twin if binding == "ctypes" else host.impl
+    n = (1 << 32) + 8
+    x = torch.empty(1, n, 1, 1, device="cuda", dtype=BF)
+    w, b = torch.empty(1, n, 1, device="cuda", dtype=BF), torch.empty(1, device="cuda", dtype=BF)
+    with pytest.raises(RuntimeError, match="size beyond"):
+        ops.pointwise_forward(x, w, b)
+    with pytest.raises(RuntimeError, match="size beyond"):
+        ops.pointwise_backward(b.view(1, 1, 1, 1), None, x, w, b)
+    with pytest.raises(RuntimeError, match="size beyond"):
+        ops.gated_forward(b.view(1, 1, 1, 1), torch.empty(2 * (n // 2), 1, 1, device="cuda", dtype=BF), torch.empty(n, device="cuda", dtype=BF),
+                          torch.empty(1, n // 2, 1, device="cuda", dtype=BF), b)
