@@ -963,13 +963,14 @@ std::vector<Tensor> pointwise_backward(const Tensor& gy_in, const OptTensor& sav
   check_like(gy_in, "grad_output", {x.size(0), c_out, x.size(2), x.size(3)}, x);
   const int layout = layout_of(x);
   c10::cuda::CUDAGuard guard(dev);
+  const bool nothing = x.numel() == 0 || gy_in.numel() == 0;  // no pixels, or no output channels: zeros
   Tensor gx = need_input_grad ? empty_in(x.sizes(), x, layout) : Tensor();
   Tensor gw, gb;
   if (need_weight_grad) {
-    gw = x.numel() == 0 ? at::zeros(w.sizes(), w.options()) : at::empty(w.sizes(), w.options());
-    gb = x.numel() == 0 ? at::zeros({c_out}, w.options()) : at::empty({c_out}, w.options());
+    gw = nothing ? at::zeros(w.sizes(), w.options()) : at::empty(w.sizes(), w.options());
+    gb = nothing ? at::zeros({c_out}, w.options()) : at::empty({c_out}, w.options());
   }
-  if (x.numel() == 0) return {gx, gw, gb};
+  if (nothing) return {need_input_grad ? gx.zero_() : gx, gw, gb};
   const Tensor gy = aligned16(as_layout(gy_in, layout));
   const mc_mix_desc d = make_mix_desc(x, layout, c_out, 0, act);
   check_saved(saved, mc_pointwise_saved_bytes(&d));
@@ -1022,14 +1023,18 @@ std::vector<Tensor> gated_backward(const Tensor& gy_in, const OptTensor& saved, 
   check_like(gy_in, "grad_output", {x.size(0), c_out, x.size(2), x.size(3)}, x);
   const int layout = layout_of(x);
   c10::cuda::CUDAGuard guard(dev);
+  const bool nothing = x.numel() == 0 || gy_in.numel() == 0;  // no pixels, or no output channels: zeros
   std::vector<Tensor> g(5);
   if (need_input_grad) g[0] = empty_in(x.sizes(), x, layout);
   if (need_weight_grad) {
     const std::vector<std::vector<int64_t>> shapes{{2 * hidden, x.size(1), 1}, {2 * hidden}, {c_out, hidden, 1}, {c_out}};
     for (int i = 0; i < 4; ++i)
-      g[i + 1] = x.numel() == 0 ? at::zeros(shapes[i], x.options()) : at::empty(shapes[i], x.options());
+      g[i + 1] = nothing ? at::zeros(shapes[i], x.options()) : at::empty(shapes[i], x.options());
   }
-  if (x.numel() == 0) return g;
+  if (nothing) {
+    if (need_input_grad) g[0].zero_();
+    return g;
+  }
   const Tensor gy = aligned16(as_layout(gy_in, layout));
   const mc_mix_desc d = make_mix_desc(x, layout, c_out, hidden, act);
   check_saved(saved, mc_gated_saved_bytes(&d));

@@ -851,11 +851,12 @@ def pointwise_backward(grad_output, saved, input, weight, bias, activation=0, ne
                None, c_out, grad_output)
     layout = _layout(input)
     gx = _empty(input.shape, input, layout) if need_input_grad else None
-    make = torch.zeros if input.numel() == 0 else torch.empty
+    nothing = input.numel() == 0 or grad_output.numel() == 0  # no pixels, or no output channels: zeros
+    make = torch.zeros if nothing else torch.empty
     gw = make(weight.shape, dtype=weight.dtype, device=dev) if need_weight_grad else None
     gb = make((c_out,), dtype=weight.dtype, device=dev) if need_weight_grad else None
-    if input.numel() == 0:
-        return [gx, gw, gb]
+    if nothing:
+        return [gx if gx is None else gx.zero_(), gw, gb]
     grad_output = _as_layout(grad_output, layout)
     d = _mix_desc(input, layout, c_out, 0, activation)
     with torch.cuda.device(dev):
@@ -906,11 +907,12 @@ def gated_backward(grad_output, saved, input, weight_in, bias_in, weight_out, ac
     _check_mix(input, params + [("bias_in", bias_in, (2 * hidden,))], None, c_out, grad_output)
     layout = _layout(input)
     gx = _empty(input.shape, input, layout) if need_input_grad else None
-    make = torch.zeros if input.numel() == 0 else torch.empty
+    nothing = input.numel() == 0 or grad_output.numel() == 0  # no pixels, or no output channels: zeros
+    make = torch.zeros if nothing else torch.empty
     grads = [make(s, dtype=input.dtype, device=dev) if need_weight_grad else None
              for s in (weight_in.shape, (2 * hidden,), weight_out.shape, (c_out,))]
-    if input.numel() == 0:
-        return [gx] + grads
+    if nothing:
+        return [gx if gx is None else gx.zero_()] + grads
     grad_output = _as_layout(grad_output, layout)
     d = _mix_desc(input, layout, c_out, hidden, activation)
     with torch.cuda.device(dev):

@@ -56,3 +56,21 @@ def test_nothing_is_kept_for_a_residual_alone(dtype):
         y.float().sum().backward()
         assert torch.equal(r.grad, torch.ones_like(r))
         r = r.detach()
+
+
+@pytest.mark.parametrize("binding", ["ctypes", "compiled"])
+@pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "f32"])
+def test_no_output_channels(binding, dtype):
+    """an output without elements has gradients: zeros"""
+    from mappedconvolutions_b200 import host, ops as twin
+    ops = twin if binding == "ctypes" else host.impl
+    t = lambda *s: torch.ones(*s, device="cuda", dtype=dtype)
+    x, w, b = t(2, 6, 3, 5), t(0, 6, 1), t(0)
+    y, saved = ops.pointwise_forward(x, w, b, None, 1, True)
+    assert y.shape == (2, 0, 3, 5)
+    gx, gw, gb = ops.pointwise_backward(y, saved, x, w, b, 1)
+    assert torch.equal(gx, torch.zeros_like(x)) and gw.shape == w.shape and gb.shape == b.shape
+    wi, bi, wo = t(8, 6, 1), t(8), t(0, 4, 1)
+    y, saved = ops.gated_forward(x, wi, bi, wo, b, None, 4, True)
+    g = ops.gated_backward(y, saved, x, wi, bi, wo, 4)
+    assert all(torch.equal(p, torch.zeros_like(q)) for p, q in zip(g, (x, wi, bi, wo, b)))
