@@ -48,3 +48,16 @@ def op_binding(request, monkeypatch):
         assert host.COMPILED, "extension not built: python -m mappedconvolutions_b200.build"
         monkeypatch.setattr(mappedconvolutions_b200, "ops", host.impl)
     return which
+
+
+# Modules after each of whose tests no bounded device-side wait may have run out: one that gives up after the results are
+# stored shows in the device status only.
+_WAITS_CHECKED = {"test_gpu_mix", "test_gpu_mix_paths", "test_gpu_mix_strict", "test_gpu_mix_autograd"}
+
+
+@pytest.fixture(autouse=True)
+def no_wait_ran_out(request):
+    yield
+    if request.module.__name__ in _WAITS_CHECKED and "gpu" in request.keywords:
+        from mappedconvolutions_b200 import host
+        assert host.impl.device_status(True) == 0

@@ -12,13 +12,6 @@ pytestmark = pytest.mark.gpu
 BF, F32, F64 = torch.bfloat16, torch.float32, torch.float64
 
 
-@pytest.fixture(autouse=True)
-def no_wait_ran_out():
-    """a bounded wait that gives up after the results are stored shows in the device status only"""
-    yield
-    assert host.impl.device_status(True) == 0
-
-
 def image(g, shape, dtype, layout, scale=1.0):
     t = (torch.randn(shape, generator=g, device="cuda", dtype=F32) * scale).to(dtype)
     return t.contiguous(memory_format=torch.channels_last) if layout == "nhwc" else t
