@@ -396,7 +396,8 @@ int mc_voting_resample(const int64_t* labels, const int64_t* map, int32_t B, int
  *   gated       [g|u] = x W_in^T + b_in,  y = (act(g) * u) W_out^T + b_out + r
  * x (B, C_in, H, W), residual r and y (B, C_out, H, W) in `layout`, S = H * W.  Parameters are contiguous, in `dtype`:
  * w (C_out, C_in), bias (C_out); w_in (2 hidden, C_in) - gate rows first -, b_in (2 hidden), w_out (C_out, hidden),
- * b_out (C_out).  residual and biases may be NULL.  Sums are float32 (double for MC_F64); for MC_BF16 what stands
+ * b_out (C_out).  residual and biases may be NULL.  Sums are float32 (double for MC_F64; for MC_BF16 the tensor cores',
+ * which lose up to 2^-23 of a sum per sixteen terms, parameter gradients over 2^17 pixels at a time); for MC_BF16 what stands
  * between two products (h, and the gradients of the pre-activations) is rounded to bf16, which the next product's
  * operand is, and the pre-activations themselves are float32: the backward calls compute them again.  MC_BF16 tensors
  * must be 16-byte aligned (biases need not be).  Limits: B * S <= 2^31 - 256, channels <= 2^20. */

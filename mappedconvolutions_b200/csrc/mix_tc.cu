@@ -13,7 +13,7 @@
 // rings they stay in shared memory and the block keeps its channel tile; otherwise they travel with the pixels.
 // 1024 -> 1024 channels at 655 488 pixels: 1281 TFLOP/s without an epilogue, 1094 with GELU, 1005 with GELU and residual
 // (first launches; over a second, with the clock held down by the power limit, 1118, 958 and 874; a library product of
-// these sizes 1338 and 1170).  128 -> 256 channels with residual, 655 488 pixels: 80 % of the copy bandwidth.
+// these sizes 1338 and 1170).  128 -> 256 channels with residual, 655 488 pixels: 78 % of the copy bandwidth.
 //
 // outer kernel: parameter gradients, both operands read along the pixels (MN-major); every block sums a share of the
 // pixels for one tile of the gradient and writes float32 partial sums, which are added in order afterwards.  The eight
@@ -1002,11 +1002,16 @@ static RowsPlan plan_rows(int m_pairs, int N, int kb0, int kb1, int sms) {
   const int fixed_bytes = 1024 + 4 * 256 * 4 + ROWS_BARS * 8 + 16 + 64;
   const int b_tile = kb0 * C::B0 + kb1 * C::B1, pairs = sms / 2;
   const int left = SMEM_LIMIT - fixed_bytes - (2 << C::SLOT_BITS) * C::CH_BYTES;
-  // Weights stay in shared memory where at least three stages of pixels fit beside them (128 -> 256 channels, 655 488 pixels:
-  // 167 us, 225 us with weights that travel).  How many channel tiles a pair keeps: the number that leaves the fewest pairs
-  // without work; more tiles cost stages, below four of which the pixels' latency shows.  The gate's gradients, two
-  // operands of pixels and small tiles, need the room for stages (256 -> 1024 channels, 163 872 pixels: 380 us, 451 us with
-  // weights that stay).
+  // Weights stay in shared memory where at least three stages of pixels fit beside them.  us at 655 488 pixels, weights that
+  // stay / that travel: without activation 96 -> 96 channels 63 / 70, 64 -> 64 49.6 / 50.4, 128 -> 256 114 / 113; ReLU and
+  // residual 128 -> 256 167 / 166, 256 -> 256 180 / 183; GELU 64 -> 64 63 / 66, 256 -> 256 198 / 197, 320 -> 320 312 / 277,
+  // 192 -> 768 559 / 539; the gate with 64 -> 64 -> 64 108 / 111, 256 -> 1024 -> 256 1092 / 1114, 128 -> 512 -> 128 482 / 484.
+  // Few channels gain, three channel tiles lose: groups of pairs leave two pairs idle, several tiles a pair round its share
+  // up (72 -> 328 at 40 962 pixels: 30.5 / 25.7).
+  // How many channel tiles a pair keeps: the number that leaves the fewest pairs without work; fewer than four stages count
+  // as 7 % of them (128 -> 768, one tile with seven stages / three tiles with three: 322 / 320, GELU 544 / 526; 256 -> 384
+  // 227 / 234, GELU 310 / 316).  The gate's gradients, two operands of pixels and small tiles, need the room for stages (256 ->
+  // 1024 channels, 163 872 pixels: 380 us, 451 us with weights that stay).
   // Where a pair has a tile or two only, weights that stay are weights that are waited for (2 562 pixels, 680 -> 256
   // channels, 44 tiles: 11.6 us, 9.0 us if they travel with the pixels; 128 -> 512, 88 tiles: 9.7 and 6.9; the gate with
   // 64 -> 256 channels, 82 tiles: 18.8 and 20.5 for the block).
@@ -1048,7 +1053,9 @@ static int launch_rows(GemmArgs& g, cudaStream_t st) {
 // Channels of a tile, for `pairs` pixel tiles, n channels, kb stages: the least estimated time.  A tile costs its MMAs
 // (half a cycle per column and 16 channels, not less than its stages' hand-over), its read-out and a start; many pixels
 // want wide tiles, few pixels so many tiles that every pair of blocks has one (680 -> 256 channels at 2 562 pixels, 11
-// pixel tiles: 14.2 us with one tile of 256 columns each).
+// pixel tiles: 9.8 us with tiles of 64, 15.6 with 256).  Against the best of the three widths, at 642 to 655 488 pixels and
+// eleven pairs of channel counts from 16 -> 8 to 1024 -> 1024: 1.7 % more time on average, at most 23 % (10 242 pixels, 64 ->
+// 160: 9.6 us with 128, 7.8 with 64), 9 - 19 % for seven shapes of 10 242 and 40 962 pixels that take 256 where 128 is faster.
 static int tile_width(long long pairs, int n, int kb, int sms) {
   const int all = sms / 2;
   int best = 64;
@@ -1146,7 +1153,8 @@ static OuterPlan outer_plan(long long P, int M, int segs, int N, int sms) {
   for (long long s = least; s < least + pairs && s <= (kb + 3) / 4; ++s) {
     const long long per = (kb + s - 1) / s;
     const double waves = (double)((tiles * s + pairs - 1) / pairs);
-    // a pair's stages, and what it costs to write its sums and to add them up again
+    // a pair's stages, and what it costs to write its sums and to add them up again (against eight other numbers of shares,
+    // at 642 to 655 488 pixels and ten pairs of channel counts: 1.6 % more time on average, at most 10 %)
     const double t = waves * (per + 8.0) + 0.05 * tiles * s;
     if (t < best) best = t, p.splits = (int)((kb + per - 1) / per), p.per = (int)per;
   }
