@@ -59,6 +59,11 @@ def path_desc(case):
     return _lib.McMixDesc(b, h * w, cin, cout, hidden, R.ACTS[act], _lib.MC_BF16, _lib.MC_NHWC if layout == "nhwc" else _lib.MC_NCHW)
 
 
+def slope(name, z):
+    """the sigmoid's as s(z) s(-z): 1 - s(z) cancels in 64 bits too (2^-53 of one where the slope is e^-|z|)"""
+    return z.sigmoid() * (-z).sigmoid() if name == "sigmoid" else R.slope(name, z)
+
+
 def value_error(t, name, z, ez, a, s):
     """z is off by ez; the functions are held to t.fn of the value, or (1 + erf, 1 + tanh in float32 / float64) of one"""
     if name is None:
@@ -105,7 +110,7 @@ def pointwise(x, w, b, r, name, gy=None, spoil=None):
     """{output name: (value, bound)}; spoil: what a worse implementation does to z before its backward pass"""
     t = R.Bounds(x.dtype)
     X, Wd, z, ez = pre_activations(x, w, b)
-    a, s = R.act(name, z), R.slope(name, z)
+    a, s = R.act(name, z), slope(name, z)
     y, ey = a, value_error(t, name, z, ez, a, s)
     if r is not None:
         rr = R.rows(r)
@@ -114,7 +119,7 @@ def pointwise(x, w, b, r, name, gy=None, spoil=None):
     if gy is not None:
         G = R.rows(gy)
         if spoil is not None:
-            s = R.slope(name, spoil(z))
+            s = slope(name, spoil(z))
         gz, egz = (G, torch.zeros_like(G)) if name is None else _product(t, [(G, 0), (s, slope_error(t, name, z, ez, s))])
         out.update(R._grads(t, gz, egz, X, Wd, ("gx", "gw", "gb")))
     return _shaped(out, x)
@@ -126,7 +131,7 @@ def gated(x, wi, bi, wo, bo, r, name, gy=None, spoil=None):
     Wo, bod = wo.detach().double()[:, :, 0], bo.detach().double()
     n = Wo.shape[1]
     g, u, eg, eu = z[:, :n], z[:, n:], ez[:, :n], ez[:, n:]
-    a, s = R.act(name, g), R.slope(name, g)
+    a, s = R.act(name, g), slope(name, g)
     ea = value_error(t, name, g, eg, a, s)
     h, eh = _product(t, [(a, ea), (u, eu)])
     y = h @ Wo.T + bod
@@ -140,7 +145,7 @@ def gated(x, wi, bi, wo, bo, r, name, gy=None, spoil=None):
         G = R.rows(gy)
         if spoil is not None:
             g, u = spoil(g), spoil(u)
-            a, s = R.act(name, g), R.slope(name, g)
+            a, s = R.act(name, g), slope(name, g)
         gh = G @ Wo
         egh = t.sum(G.shape[1]) * (G.abs() @ Wo.abs())
         gg, egg = _product(t, [(gh, egh), (u, eu), (s, slope_error(t, name, g, eg, s))])
