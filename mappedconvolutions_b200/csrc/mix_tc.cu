@@ -330,7 +330,7 @@ template <int MODE, int BN> struct Cfg {
   static constexpr int NCH = (MODE == GATE_BWD ? 2 : 1) * BN / CW;           // staged tiles
   static constexpr int CH_BYTES = TILE * CW * 2;
   // 2^SLOT_BITS slots for staged tiles in each set.  (The gate's gradients with two: 11 % slower.  One, where that makes room
-  // for weights that stay: 512 -> 512 channels, 163 872 pixels 146 us instead of 115.)
+  // for weights that stay: 512 -> 512 channels with residual, 163 872 pixels 146 us instead of 115.)
   static constexpr int SLOT_BITS = MODE == GATE_BWD ? 2 : 1;
   // Accumulators in TMEM: as many as fit, since an epilogue's latencies are hidden by the tiles behind it.
   static constexpr int NACC = MODE == GATE_BWD || N0 > 128 ? 2 : 4, ACC = 512 / NACC;
@@ -1209,6 +1209,7 @@ bool tc_plan(const mc_mix_desc* d, int product, int sms, int32_t* out) {
       p = gate_width(H) == 64 ? plan_rows<GATE, 64>(m, H, ki, 0, sms) : plan_rows<GATE, 128>(m, H, ki, 0, sms);
       break;
     case MC_MIX_ACT_GRAD:
+      if (!H && d->act == MC_ACT_NONE) return false;
       p = H ? plan_rows<GATE_BWD, 64>(m, H, ki, ko, sms) : plan_wide<ACT_BWD>(m, d->C_out, ki, 0, sms);
       break;
     case MC_MIX_INPUT_GRAD: p = plan_wide<LAYER>(m, d->C_in, H ? kh : ko, H ? kh : 0, sms); break;

@@ -56,4 +56,5 @@ def test_refusals():
     assert L.mc_mix_plan(d(dtype=_lib.MC_F32), 0, 148, v) == -2 and L.mc_mix_plan(d(S=1 << 31), 0, 148, v) == -6
     for product in (-1, 1, 5, 6):  # (a pointwise layer has no gate and no second weight)
         assert L.mc_mix_plan(d(), product, 148, v) == -1
+    assert L.mc_mix_plan(d(act=0), 2, 148, v) == -1 and L.mc_mix_plan(d(act=0, hidden=8), 2, 148, v) == 0  # nor, without one, an activation's gradient
     assert L.mc_mix_plan(d(), 0, -1, v) == -1 and L.mc_mix_plan(d(), 0, 1, v) == -1 and L.mc_mix_plan(d(), 0, 148, None) == -1
