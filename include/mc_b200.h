@@ -470,6 +470,82 @@ int mc_grad_clip(int32_t n, const void* const* src, const int32_t* src_dtype, vo
                  const int64_t* numel, double norm_type, double max_norm, double* norm, float* norm32, void* ws,
                  size_t ws_bytes, void* stream);
 
+/* ---- group normalisation with an activation -----------------------------------------------------
+ * No counterpart in the reference.  Over the C / groups * S elements of a group of neighbouring channels of one image:
+ *   xhat = (x - mean) / sqrt(var + eps),  y = act(xhat w_c + b_c),   var: the mean of (x - mean)^2
+ * x, y, gy, gx (B, C, H, W) in `layout`, S = H * W, 16-byte aligned; w and bias (C) in `dtype`, or NULL for ones and zeros.
+ * stats: mc_group_norm_stats_bytes of memory that the forward call fills (mean and 1 / sqrt(var + eps) of every group of
+ * every image, float32 or double) and the backward call reads.  ws: scratch, phases MC_PHASE_FORWARD and MC_PHASE_BACKWARD.  Both
+ * 16-byte aligned.  Any of the gradients may be NULL.  Arithmetic is float32 (double for MC_F64), sums over tiles are double
+ * and in a fixed order: results repeat bit for bit.  Limits: B * S <= 2^31 - 256, C <= 2^20. */
+typedef struct mc_norm_desc {
+  int64_t B, S;
+  int32_t C, groups;
+  int32_t act; /* MC_ACT_* */
+  int32_t dtype, layout;
+  double eps;
+} mc_norm_desc;
+size_t mc_group_norm_stats_bytes(const mc_norm_desc* d);
+size_t mc_group_norm_workspace_bytes(const mc_norm_desc* d, int32_t phase);
+int mc_group_norm_fwd(const mc_norm_desc* d, const void* x, const void* w, const void* bias, void* y, void* stats, void* ws,
+                      size_t ws_bytes, void* stream);
+int mc_group_norm_bwd(const mc_norm_desc* d, const void* gy, const void* x, const void* w, const void* bias, const void* stats,
+                      void* gx, void* gw, void* gb, void* ws, size_t ws_bytes, void* stream);
+
+/* ---- softmax cross entropy of a pointwise classifier ---------------------------------------------
+ * No counterpart in the reference.  With P = B * S pixels, a row vector x_p of C channels each, V classes and labels t_p:
+ *   z = x W^T + b,  loss = scale * sum_p (log sum_v exp(z_pv) - z_p,t_p)
+ * over the pixels whose label is not ignore_index; scale is 1 (MC_REDUCE_SUM) or 1 / their number (MC_REDUCE_MEAN: NaN where there is
+ * none, whose gradients are zero).  The class scores z are not kept: the backward call computes them again, piece by piece.
+ * x, gx (B, C, H, W) in `layout`, S = H * W, w and gw (V, C), bias (may be NULL) and gb (V) in `dtype`, x, w and gx 16-byte aligned;
+ * target (B, H, W) int64; loss and grad_loss (its gradient, in device memory) one float (MC_F64: double).  A pixel without a
+ * label has a zero gradient and adds nothing to the others, whatever its features are.  A label outside [0, V) that is not
+ * ignore_index makes the loss and the gradients that its pixel takes part in NaN.
+ * saved: mc_cross_entropy_saved_bytes of memory that the forward call fills and the backward call reads; ws: scratch, phases
+ * MC_PHASE_FORWARD and MC_PHASE_BACKWARD; both 16-byte aligned.  Any of the gradients may be NULL.  Scores, softmax sums and gradients of
+ * parameters are summed in float32 (MC_F64: double), the loss in double, all in a fixed order.
+ * Limits: B * S <= 2^31 - 256, C and V <= 2^20, C * V <= 2^31. */
+enum { MC_REDUCE_SUM = 0, MC_REDUCE_MEAN = 1 };
+typedef struct mc_ce_desc {
+  int64_t B, S, ignore_index;
+  int32_t C, V;
+  int32_t reduction; /* MC_REDUCE_* */
+  int32_t dtype, layout;
+} mc_ce_desc;
+size_t mc_cross_entropy_saved_bytes(const mc_ce_desc* d);
+size_t mc_cross_entropy_workspace_bytes(const mc_ce_desc* d, int32_t phase);
+int mc_cross_entropy_fwd(const mc_ce_desc* d, const void* x, const void* w, const void* bias, const int64_t* target, void* loss,
+                         void* saved, void* ws, size_t ws_bytes, void* stream);
+int mc_cross_entropy_bwd(const mc_ce_desc* d, const void* grad_loss, const void* x, const void* w, const void* bias,
+                         const int64_t* target, const void* saved, void* gx, void* gw, void* gb, void* ws, size_t ws_bytes,
+                         void* stream);
+
+/* ---- AdamW over many tensors -------------------------------------------------------------------
+ * No counterpart in the reference.  n tensors as a HOST array that is read before the call returns; element counts may be 0.
+ *   m = beta1 m + (1 - beta1) g,  v = beta2 v + (1 - beta2) g^2,
+ *   p = p (1 - lr weight_decay) - lr / (1 - beta1^step) m / (sqrt(v) / sqrt(1 - beta2^step) + eps),   step >= 1
+ * Arithmetic is float32 (double for MC_F64 parameters, whose gradients and moments are MC_F64).  MC_F32 and MC_BF16 parameters
+ * take MC_F32 or MC_BF16 gradients.  master (MC_BF16 parameters, may be NULL): float32 values that the step is taken on, p is their
+ * rounding.  bits 32: m and v are float32.  bits 8: m int8 and v uint8 codes, m_scale and v_scale one float per 256 consecutive
+ * elements; m stands for c |c| m_scale, v for (c^2 v_scale)^2, with m_scale = max|m| / 127^2 and v_scale = max sqrt(v) / 255^2 of the
+ * block (zero if below 2^-126) and the nearest codes, ties to even; a v that is not zero has a code that is not zero.  A block
+ * with an element that is not finite becomes NaN.  The update uses moments that are not rounded yet.  Nothing written may
+ * share memory with another tensor of the call. */
+typedef struct mc_adamw_tensor {
+  void* p;
+  const void* g;
+  void *master, *m, *v;
+  float *m_scale, *v_scale;
+  int64_t numel, step;
+  int32_t p_dtype, g_dtype, bits;
+} mc_adamw_tensor;
+typedef struct mc_adamw_hyper {
+  double lr, beta1, beta2, eps, weight_decay;
+} mc_adamw_hyper;
+int mc_adamw_step(int32_t n, const mc_adamw_tensor* tensors, const mc_adamw_hyper* h, void* stream);
+/* What 8-bit moments stand for, in float32: m to p, v to master (g, step and types are not read). */
+int mc_adamw_moments(int32_t n, const mc_adamw_tensor* tensors, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

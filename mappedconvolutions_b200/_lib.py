@@ -26,6 +26,25 @@ class McMixDesc(ctypes.Structure):
         [(n, ctypes.c_int32) for n in ("C_in", "C_out", "hidden", "act", "dtype", "layout")]
 
 
+class McNormDesc(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int64) for n in ("B", "S")] + \
+        [(n, ctypes.c_int32) for n in ("C", "groups", "act", "dtype", "layout")] + [("eps", ctypes.c_double)]
+
+
+class McCeDesc(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int64) for n in ("B", "S", "ignore_index")] + \
+        [(n, ctypes.c_int32) for n in ("C", "V", "reduction", "dtype", "layout")]
+
+
+class McAdamwTensor(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in ("p", "g", "master", "m", "v", "m_scale", "v_scale")] + \
+        [(n, ctypes.c_int64) for n in ("numel", "step")] + [(n, ctypes.c_int32) for n in ("p_dtype", "g_dtype", "bits")]
+
+
+class McAdamwHyper(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_double) for n in ("lr", "beta1", "beta2", "eps", "weight_decay")]
+
+
 class McError(RuntimeError):
     pass
 
@@ -35,6 +54,8 @@ _lib = None
 _vp, _sz, _i32 = ctypes.c_void_p, ctypes.c_size_t, ctypes.c_int32
 _dp = ctypes.POINTER(McDesc)
 _mp = ctypes.POINTER(McMixDesc)
+_np, _cp = ctypes.POINTER(McNormDesc), ctypes.POINTER(McCeDesc)
+_ap, _hp = ctypes.POINTER(McAdamwTensor), ctypes.POINTER(McAdamwHyper)
 _pp, _lp, _ip = ctypes.POINTER(_vp), ctypes.POINTER(ctypes.c_int64), ctypes.POINTER(_i32)
 _f64 = ctypes.c_double
 
@@ -116,6 +137,16 @@ SIGNATURES = {
     "mc_grad_workspace_bytes": (_sz, [_i32]),
     "mc_grad_norm": (ctypes.c_int, [_i32, _pp, _lp, _ip, _f64, _vp, _vp, _vp, _sz, _vp]),
     "mc_grad_clip": (ctypes.c_int, [_i32, _pp, _ip, _pp, _ip, _lp, _f64, _f64, _vp, _vp, _vp, _sz, _vp]),
+    "mc_group_norm_stats_bytes": (_sz, [_np]),
+    "mc_group_norm_workspace_bytes": (_sz, [_np, _i32]),
+    "mc_group_norm_fwd": (ctypes.c_int, [_np] + [_vp] * 6 + [_sz, _vp]),
+    "mc_group_norm_bwd": (ctypes.c_int, [_np] + [_vp] * 9 + [_sz, _vp]),
+    "mc_cross_entropy_saved_bytes": (_sz, [_cp]),
+    "mc_cross_entropy_workspace_bytes": (_sz, [_cp, _i32]),
+    "mc_cross_entropy_fwd": (ctypes.c_int, [_cp] + [_vp] * 7 + [_sz, _vp]),
+    "mc_cross_entropy_bwd": (ctypes.c_int, [_cp] + [_vp] * 10 + [_sz, _vp]),
+    "mc_adamw_step": (ctypes.c_int, [_i32, _ap, _hp, _vp]),
+    "mc_adamw_moments": (ctypes.c_int, [_i32, _ap, _vp]),
 }
 
 

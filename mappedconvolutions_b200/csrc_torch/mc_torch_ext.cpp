@@ -1177,6 +1177,262 @@ Tensor clip_gradients(const std::vector<Tensor>& tensors, double max_norm, doubl
   return norm.t;
 }
 
+// ---- group normalisation with an activation (no counterpart in the reference) ----------------------------------
+
+mc_norm_desc norm_desc(const Tensor& x, const OptTensor& w, const OptTensor& b, int64_t groups, double eps, int64_t act,
+                       int* layout) {
+  TORCH_CHECK(x.dim() == 4, "input must be 4-D (B, C, H, W)");
+  const int64_t c = x.size(1);
+  TORCH_CHECK(groups > 0 && c % groups == 0, "groups must divide the channels (", groups, ", ", c, ")");
+  if (w.has_value()) check_param(*w, "weight", {c}, x);
+  if (b.has_value()) check_param(*b, "bias", {c}, x);
+  TORCH_CHECK(c <= std::numeric_limits<int32_t>::max(), "size beyond a fixed limit: more than 2^31 channels");
+  const auto dt = x.scalar_type();
+  TORCH_CHECK(dt == at::kFloat || dt == at::kDouble || dt == at::kBFloat16, "unsupported dtype ", dt,
+              " (float32, float64, bfloat16)");
+  *layout = layout_of(x);
+  mc_norm_desc d{};
+  d.B = x.size(0), d.S = x.size(2) * x.size(3), d.C = (int32_t)c, d.groups = (int32_t)groups, d.act = (int32_t)act;
+  d.dtype = dt == at::kFloat ? MC_F32 : dt == at::kDouble ? MC_F64 : MC_BF16, d.layout = *layout, d.eps = eps;
+  return d;
+}
+
+// (output, statistics)
+std::pair<Tensor, Tensor> group_norm_forward(const Tensor& x_in, const OptTensor& w, const OptTensor& b, int64_t groups,
+                                             double eps, int64_t act) {
+  const auto dev = need_cuda({&x_in, opt(w), opt(b)});
+  const Tensor x = aligned16(x_in);
+  int layout;
+  const mc_norm_desc d = norm_desc(x, w, b, groups, eps, act, &layout);
+  c10::cuda::CUDAGuard guard(dev);
+  Tensor y = empty_in(x.sizes(), x, layout);
+  if (y.numel() == 0) return {y, Tensor()};
+  Scratch stats = scratch(mc_group_norm_stats_bytes(&d), dev);
+  Scratch ws = scratch(mc_group_norm_workspace_bytes(&d, MC_PHASE_FORWARD), dev);
+  check(mc_group_norm_fwd(&d, x.data_ptr(), ptr(w), ptr(b), y.data_ptr(), stats.p, ws.p, ws.n, cur_stream()));
+  return {y, stats.t};
+}
+
+std::vector<Tensor> group_norm_backward(const Tensor& gy_in, const OptTensor& stats, const Tensor& x_in, const OptTensor& w,
+                                        const OptTensor& b, int64_t groups, double eps, int64_t act, bool need_input_grad,
+                                        bool need_weight_grad) {
+  const auto dev = need_cuda({&gy_in, opt(stats), &x_in, opt(w), opt(b)});
+  const Tensor x = aligned16(x_in);
+  int layout;
+  const mc_norm_desc d = norm_desc(x, w, b, groups, eps, act, &layout);
+  check_like(gy_in, "grad_output", x.sizes(), x);
+  c10::cuda::CUDAGuard guard(dev);
+  const bool nothing = x.numel() == 0;
+  std::vector<Tensor> g(3);
+  if (need_input_grad) g[0] = empty_in(x.sizes(), x, layout);
+  const auto make = [&](const OptTensor& t) {
+    return !need_weight_grad || !t.has_value() ? Tensor() : nothing ? at::zeros(t->sizes(), t->options()) : at::empty(t->sizes(), t->options());
+  };
+  g[1] = make(w), g[2] = make(b);
+  if (nothing) return g;
+  check_saved(stats, mc_group_norm_stats_bytes(&d));
+  const Tensor gy = aligned16(as_layout(gy_in, layout));
+  Scratch ws = scratch(mc_group_norm_workspace_bytes(&d, MC_PHASE_BACKWARD), dev);
+  check(mc_group_norm_bwd(&d, gy.data_ptr(), x.data_ptr(), ptr(w), ptr(b), ptr(stats), maybe(g[0]), maybe(g[1]), maybe(g[2]),
+                          ws.p, ws.n, cur_stream()));
+  return g;
+}
+
+// ---- softmax cross entropy of a pointwise classifier (no counterpart in the reference) --------------------------
+
+mc_ce_desc ce_desc(const Tensor& x, const Tensor& w, const Tensor& b, const Tensor& target, int64_t ignore, bool mean, int* layout) {
+  check_weight_dims(w, "weight");
+  TORCH_CHECK(x.dim() == 4, "input must be 4-D (B, C, H, W)");
+  const int64_t classes = w.size(0);
+  check_param(w, "weight", {classes, x.size(1), 1}, x);
+  check_param(b, "bias", {classes}, x);
+  TORCH_CHECK(target.scalar_type() == at::kLong, "target must be int64");
+  const std::vector<int64_t> want{x.size(0), x.size(2), x.size(3)};
+  TORCH_CHECK(target.sizes() == at::IntArrayRef(want), "target must have shape ", want, ", got ", target.sizes());
+  const auto dt = x.scalar_type();
+  TORCH_CHECK(dt == at::kFloat || dt == at::kDouble || dt == at::kBFloat16, "unsupported dtype ", dt,
+              " (float32, float64, bfloat16)");
+  TORCH_CHECK(x.size(1) > 0 && classes > 0, "there must be a channel and a class");
+  TORCH_CHECK(std::max(x.size(1), classes) <= std::numeric_limits<int32_t>::max(),
+              "size beyond a fixed limit: more than 2^31 channels");
+  *layout = layout_of(x);
+  mc_ce_desc d{};
+  d.B = x.size(0), d.S = x.size(2) * x.size(3), d.ignore_index = ignore, d.C = (int32_t)x.size(1), d.V = (int32_t)classes;
+  d.reduction = mean ? MC_REDUCE_MEAN : MC_REDUCE_SUM;
+  d.dtype = dt == at::kFloat ? MC_F32 : dt == at::kDouble ? MC_F64 : MC_BF16, d.layout = *layout;
+  return d;
+}
+at::ScalarType loss_type(const Tensor& x) { return x.scalar_type() == at::kDouble ? at::kDouble : at::kFloat; }
+
+// (loss, what the backward call needs)
+std::pair<Tensor, Tensor> cross_entropy_forward(const Tensor& x_in, const Tensor& w_in, const Tensor& b, const Tensor& target_in,
+                                                int64_t ignore, bool mean) {
+  const auto dev = need_cuda({&x_in, &w_in, &b, &target_in});
+  const Tensor x = aligned16(x_in), w = aligned16(w_in);
+  int layout;
+  const mc_ce_desc d = ce_desc(x, w, b, target_in, ignore, mean, &layout);
+  c10::cuda::CUDAGuard guard(dev);
+  const auto options = x.options().dtype(loss_type(x)).memory_format(c10::nullopt);
+  if (target_in.numel() == 0)
+    return {at::full({}, mean ? std::numeric_limits<double>::quiet_NaN() : 0.0, options), Tensor()};
+  const Tensor target = target_in.contiguous();
+  Tensor loss = at::empty({}, options);
+  Scratch saved = scratch(mc_cross_entropy_saved_bytes(&d), dev);
+  Scratch ws = scratch(mc_cross_entropy_workspace_bytes(&d, MC_PHASE_FORWARD), dev);
+  check(mc_cross_entropy_fwd(&d, x.data_ptr(), w.data_ptr(), b.data_ptr(), target.data_ptr<int64_t>(), loss.data_ptr(), saved.p,
+                             ws.p, ws.n, cur_stream()));
+  return {loss, saved.t};
+}
+
+std::vector<Tensor> cross_entropy_backward(const Tensor& grad_in, const OptTensor& saved, const Tensor& x_in, const Tensor& w_in,
+                                           const Tensor& b, const Tensor& target_in, int64_t ignore, bool mean,
+                                           bool need_input_grad, bool need_weight_grad) {
+  const auto dev = need_cuda({&grad_in, opt(saved), &x_in, &w_in, &b, &target_in});
+  const Tensor x = aligned16(x_in), w = aligned16(w_in);
+  int layout;
+  const mc_ce_desc d = ce_desc(x, w, b, target_in, ignore, mean, &layout);
+  TORCH_CHECK(grad_in.scalar_type() == loss_type(x) && grad_in.numel() == 1, "grad_loss must be one value of the loss's type");
+  c10::cuda::CUDAGuard guard(dev);
+  const bool nothing = target_in.numel() == 0;
+  std::vector<Tensor> g(3);
+  if (need_input_grad) g[0] = empty_in(x.sizes(), x, layout);
+  if (need_weight_grad)
+    for (int i = 0; i < 2; ++i) {
+      const Tensor& t = i ? b : w;
+      g[1 + i] = nothing ? at::zeros(t.sizes(), t.options()) : at::empty(t.sizes(), t.options());
+    }
+  if (nothing) return g;
+  check_saved(saved, mc_cross_entropy_saved_bytes(&d));
+  const Tensor target = target_in.contiguous(), grad = grad_in.contiguous();
+  Scratch ws = scratch(mc_cross_entropy_workspace_bytes(&d, MC_PHASE_BACKWARD), dev);
+  check(mc_cross_entropy_bwd(&d, grad.data_ptr(), x.data_ptr(), w.data_ptr(), b.data_ptr(), target.data_ptr<int64_t>(), ptr(saved),
+                             maybe(g[0]), maybe(g[1]), maybe(g[2]), ws.p, ws.n, cur_stream()));
+  return g;
+}
+
+// ---- AdamW over many tensors (no counterpart in the reference) --------------------------------------------------
+
+// Element i of a's memory belongs to element i of b's.
+bool same_order(const Tensor& a, const Tensor& b) {
+  if (a.sizes() != b.sizes() || !a.is_non_overlapping_and_dense() || !b.is_non_overlapping_and_dense()) return false;
+  if (a.is_contiguous() && b.is_contiguous()) return true;
+  for (int64_t k = 0; k < a.dim(); ++k)
+    if (a.size(k) > 1 && a.stride(k) != b.stride(k)) return false;
+  return true;
+}
+bool known_type(const Tensor& t) {
+  const auto dt = t.scalar_type();
+  return dt == at::kFloat || dt == at::kDouble || dt == at::kBFloat16;
+}
+bool is_scale(const OptTensor& t, int64_t numel) {
+  return t.has_value() && t->scalar_type() == at::kFloat && t->dim() == 1 && t->size(0) == (numel + 255) / 256 && t->is_contiguous();
+}
+
+void adamw_step(const std::vector<Tensor>& params, const std::vector<Tensor>& grads, const std::vector<Tensor>& exp_avgs,
+                const std::vector<Tensor>& exp_avg_sqs, const std::vector<OptTensor>& scales,
+                const std::vector<OptTensor>& sq_scales, const std::vector<OptTensor>& masters, const std::vector<int64_t>& steps,
+                double lr, double beta1, double beta2, double eps, double weight_decay) {
+  const size_t n = params.size();
+  TORCH_CHECK(n > 0, "no tensor given");
+  TORCH_CHECK(grads.size() == n && exp_avgs.size() == n && exp_avg_sqs.size() == n && scales.size() == n && sq_scales.size() == n &&
+                  masters.size() == n && steps.size() == n, "all lists must have as many entries as there are parameters");
+  c10::optional<c10::Device> dev;
+  for (size_t i = 0; i < n; ++i) {
+    const auto d = need_cuda({&params[i], &grads[i], &exp_avgs[i], &exp_avg_sqs[i], opt(scales[i]), opt(sq_scales[i]), opt(masters[i])});
+    if (!dev) dev = d;
+    TORCH_CHECK(d == *dev, "all tensors must be on the same device");
+  }
+  c10::cuda::CUDAGuard guard(*dev);
+  at::NoGradGuard no_grad;
+  std::vector<mc_adamw_tensor> ts(n);
+  std::vector<Tensor> copies;
+  std::vector<const Tensor*> written;
+  std::vector<std::tuple<uintptr_t, uintptr_t, bool>> spans;
+  const auto span = [&](const Tensor& t, bool dst) {
+    if (t.numel()) spans.emplace_back((uintptr_t)t.data_ptr(), (uintptr_t)t.data_ptr() + t.numel() * t.element_size(), dst);
+    if (!dst) return;
+    TORCH_CHECK(!t.is_inference() || c10::InferenceMode::is_enabled(), "a tensor made in inference mode can be updated in inference mode only");
+    written.push_back(&t);
+  };
+  for (size_t i = 0; i < n; ++i) {
+    const Tensor &p = params[i], &m = exp_avgs[i], &v = exp_avg_sqs[i];
+    Tensor g = grads[i];
+    TORCH_CHECK(known_type(p), "unsupported dtype ", p.scalar_type(), " (float32, float64, bfloat16)");
+    const bool f64 = p.scalar_type() == at::kDouble;
+    TORCH_CHECK(g.layout() == at::kStrided && g.sizes() == p.sizes() && known_type(g) && (g.scalar_type() == at::kDouble) == f64,
+                "a gradient must be a dense tensor of its parameter's shape: float64 for float64 parameters, float32 or bfloat16 for the others");
+    TORCH_CHECK(p.is_non_overlapping_and_dense(), "a parameter must lie in memory without gaps and overlaps");
+    const bool eight = m.scalar_type() == at::kChar;
+    const auto wide = f64 ? at::kDouble : at::kFloat;
+    TORCH_CHECK(same_order(m, p) && same_order(v, p) &&
+                    (eight ? v.scalar_type() == at::kByte : m.scalar_type() == wide && v.scalar_type() == wide),
+                "moments must lie as their parameter does: float32 (float64 for float64 parameters), or int8 and uint8");
+    TORCH_CHECK(!(eight && f64), "moments of float64 parameters are float64");
+    TORCH_CHECK(!eight || (is_scale(scales[i], p.numel()) && is_scale(sq_scales[i], p.numel())),
+                "moments in 8 bits need a float32 scale for 256 elements each");
+    TORCH_CHECK(eight || (!scales[i].has_value() && !sq_scales[i].has_value()), "moments in 32 bits have no scales");
+    if (masters[i].has_value())
+      TORCH_CHECK(p.scalar_type() == at::kBFloat16 && masters[i]->scalar_type() == at::kFloat && same_order(*masters[i], p),
+                  "master weights are float32 copies of bfloat16 parameters that lie as these do");
+    TORCH_CHECK(steps[i] >= 1, "steps are counted from 1");
+    if (!same_order(g, p)) {
+      g = at::empty_strided(p.sizes(), p.strides(), g.options()).copy_(g);
+      copies.push_back(g);
+    }
+    span(p, true), span(m, true), span(v, true), span(g, false);
+    for (const OptTensor* t : {&scales[i], &sq_scales[i], &masters[i]})
+      if (t->has_value()) span(**t, true);
+    mc_adamw_tensor& t = ts[i];
+    t = mc_adamw_tensor{};
+    t.p = p.data_ptr(), t.g = g.data_ptr(), t.m = m.data_ptr(), t.v = v.data_ptr();
+    t.master = (void*)ptr(masters[i]), t.m_scale = (float*)ptr(scales[i]), t.v_scale = (float*)ptr(sq_scales[i]);
+    t.numel = p.numel(), t.step = steps[i], t.p_dtype = grad_dtype(p), t.g_dtype = grad_dtype(g), t.bits = eight ? 8 : 32;
+  }
+  std::sort(spans.begin(), spans.end());
+  uintptr_t end_any = 0, end_dst = 0;  // no destination may share memory with another tensor of the call
+  for (const auto& [begin, end, is_dst] : spans) {
+    TORCH_CHECK(begin >= (is_dst ? end_any : end_dst), "tensors of a step must not share memory with each other");
+    end_any = std::max(end_any, end);
+    if (is_dst) end_dst = std::max(end_dst, end);
+  }
+  const mc_adamw_hyper h{lr, beta1, beta2, eps, weight_decay};
+  check(mc_adamw_step((int32_t)n, ts.data(), &h, cur_stream()));
+  for (const Tensor* t : written) t->unsafeGetTensorImpl()->bump_version();
+}
+
+std::pair<std::vector<Tensor>, std::vector<Tensor>> adamw_moments(const std::vector<Tensor>& exp_avgs,
+                                                                  const std::vector<Tensor>& exp_avg_sqs,
+                                                                  const std::vector<Tensor>& scales,
+                                                                  const std::vector<Tensor>& sq_scales) {
+  const size_t n = exp_avgs.size();
+  TORCH_CHECK(n > 0, "no tensor given");
+  TORCH_CHECK(exp_avg_sqs.size() == n && scales.size() == n && sq_scales.size() == n, "all lists must have as many entries");
+  c10::optional<c10::Device> dev;
+  for (size_t i = 0; i < n; ++i) {
+    const auto d = need_cuda({&exp_avgs[i], &exp_avg_sqs[i], &scales[i], &sq_scales[i]});
+    if (!dev) dev = d;
+    TORCH_CHECK(d == *dev, "all tensors must be on the same device");
+  }
+  c10::cuda::CUDAGuard guard(*dev);
+  at::NoGradGuard no_grad;
+  std::vector<mc_adamw_tensor> ts(n);
+  std::vector<Tensor> ms, vs;
+  for (size_t i = 0; i < n; ++i) {
+    const Tensor &m = exp_avgs[i], &v = exp_avg_sqs[i];
+    TORCH_CHECK(m.scalar_type() == at::kChar && v.scalar_type() == at::kByte && same_order(m, v) && is_scale(scales[i], m.numel()) &&
+                    is_scale(sq_scales[i], m.numel()),
+                "moments in 8 bits are int8 and uint8 tensors that lie alike, with a float32 scale for 256 elements each");
+    ms.push_back(at::empty_strided(m.sizes(), m.strides(), m.options().dtype(at::kFloat)));
+    vs.push_back(at::empty_strided(m.sizes(), m.strides(), m.options().dtype(at::kFloat)));
+    mc_adamw_tensor& t = ts[i];
+    t = mc_adamw_tensor{};
+    t.p = ms.back().data_ptr(), t.master = vs.back().data_ptr(), t.m = m.data_ptr(), t.v = v.data_ptr();
+    t.m_scale = scales[i].data_ptr<float>(), t.v_scale = sq_scales[i].data_ptr<float>(), t.numel = m.numel(), t.bits = 8;
+  }
+  check(mc_adamw_moments((int32_t)n, ts.data(), cur_stream()));
+  return {ms, vs};
+}
+
 // ---- differentiable layer calls --------------------------------------------------------------------------
 // The pairing of forward and backward ops is the reference's (package/layers/nn/*.py): convolution <-> (input,
 // weight, bias gradient); max pool <-> max unpool through the stored tap offsets; average pool <-> average
@@ -1319,7 +1575,7 @@ OptTensor linear_layer(int64_t op, const Tensor& x, const Tensor& map, const Opt
 // backward call for any of it comes through here.
 struct NoSecondDerivative : torch::autograd::Node {
   variable_list apply(variable_list&&) override {
-    TORCH_CHECK(false, "second derivatives of the channel-mixing layers are not available");
+    TORCH_CHECK(false, "second derivatives of the channel-mixing, normalisation and loss layers are not available");
   }
 };
 void without_second(const variable_list& grads, const variable_list& inputs) {
@@ -1381,6 +1637,53 @@ struct GatedFn : torch::autograd::Function<GatedFn> {
       for (int i = 0; i < 5; ++i) out[i] = r[i];
     }
     if (ctx->saved_data["r"].toBool() && ctx->needs_input_grad(5)) out[5] = g[0];
+    return out;
+  }
+};
+
+struct GroupNormFn : torch::autograd::Function<GroupNormFn> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const OptTensor& w, const OptTensor& b, int64_t groups, double eps,
+                        int64_t act) {
+    auto f = group_norm_forward(x, w, b, groups, eps, act);
+    ctx->save_for_backward({x, or_undef(w), or_undef(b), f.second});
+    ctx->saved_data["g"] = groups;
+    ctx->saved_data["e"] = eps;
+    ctx->saved_data["a"] = act;
+    return f.first;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    const auto s = ctx->get_saved_variables();
+    const bool has_w = s[1].defined(), has_b = s[2].defined();  // (needs_input_grad counts the tensors that were given)
+    const bool need_x = ctx->needs_input_grad(0);
+    const bool need_p = (has_w && ctx->needs_input_grad(1)) || (has_b && ctx->needs_input_grad(has_w ? 2 : 1));
+    variable_list out(6);
+    if (!need_x && !need_p) return out;
+    auto r = group_norm_backward(g[0], as_opt(s[3]), s[0], as_opt(s[1]), as_opt(s[2]), ctx->saved_data["g"].toInt(),
+                                 ctx->saved_data["e"].toDouble(), ctx->saved_data["a"].toInt(), need_x, need_p);
+    without_second(r, {g[0], s[0], s[1], s[2]});
+    for (int i = 0; i < 3; ++i) out[i] = r[i];
+    return out;
+  }
+};
+
+struct CrossEntropyFn : torch::autograd::Function<CrossEntropyFn> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const Tensor& b, const Tensor& target,
+                        int64_t ignore, bool mean) {
+    auto f = cross_entropy_forward(x, w, b, target, ignore, mean);
+    ctx->save_for_backward({x, w, b, target, f.second});
+    ctx->saved_data["i"] = ignore;
+    ctx->saved_data["m"] = mean;
+    return f.first;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    const auto s = ctx->get_saved_variables();
+    const bool need_x = ctx->needs_input_grad(0), need_p = ctx->needs_input_grad(1) || ctx->needs_input_grad(2);
+    variable_list out(6);
+    if (!need_x && !need_p) return out;
+    auto r = cross_entropy_backward(g[0], as_opt(s[4]), s[0], s[1], s[2], s[3], ctx->saved_data["i"].toInt(),
+                                    ctx->saved_data["m"].toBool(), need_x, need_p);
+    without_second(r, {g[0], s[0], s[1], s[2]});
+    for (int i = 0; i < 3; ++i) out[i] = r[i];
     return out;
   }
 };
@@ -1575,6 +1878,56 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   def("gradient_norm", &gradient_norm, py::arg("tensors"), py::arg("norm_type") = 2.0);
   def("clip_gradients", &clip_gradients, py::arg("tensors"), py::arg("max_norm"), py::arg("norm_type") = 2.0,
         py::arg("out") = py::none());
+  // group normalisation, cross entropy of a pointwise classifier: as in ops.py; the differentiable calls of the layers
+  def("group_norm_forward",
+        [](const Tensor& x, const OptTensor& w, const OptTensor& b, int64_t groups, double eps, int64_t act) -> std::vector<OptTensor> {
+          auto f = group_norm_forward(x, w, b, groups, eps, act);
+          return {f.first, as_opt(f.second)};
+        },
+        py::arg("input"), py::arg("weight"), py::arg("bias"), py::arg("groups"), py::arg("eps") = 1e-5, py::arg("activation") = 0);
+  def("group_norm_backward",
+        [](const Tensor& gy, const OptTensor& stats, const Tensor& x, const OptTensor& w, const OptTensor& b, int64_t groups,
+           double eps, int64_t act, bool nx, bool np) {
+          std::vector<OptTensor> r;
+          for (const Tensor& t : group_norm_backward(gy, stats, x, w, b, groups, eps, act, nx, np)) r.push_back(as_opt(t));
+          return r;
+        },
+        py::arg("grad_output"), py::arg("stats"), py::arg("input"), py::arg("weight"), py::arg("bias"), py::arg("groups"),
+        py::arg("eps") = 1e-5, py::arg("activation") = 0, py::arg("need_input_grad") = true, py::arg("need_weight_grad") = true);
+  def("group_norm_layer", [](const Tensor& x, const OptTensor& w, const OptTensor& b, int64_t groups, double eps,
+                               int64_t act) -> OptTensor {
+    if (seen_by_torch({&x, opt(w), opt(b)})) return c10::nullopt;
+    if (!records({&x, opt(w), opt(b)})) return group_norm_forward(x, w, b, groups, eps, act).first;
+    return GroupNormFn::apply(x, w, b, groups, eps, act);
+  });
+  def("cross_entropy_forward",
+        [](const Tensor& x, const Tensor& w, const Tensor& b, const Tensor& target, int64_t ignore, bool mean) -> std::vector<OptTensor> {
+          auto f = cross_entropy_forward(x, w, b, target, ignore, mean);
+          return {f.first, as_opt(f.second)};
+        },
+        py::arg("input"), py::arg("weight"), py::arg("bias"), py::arg("target"), py::arg("ignore_index") = -100,
+        py::arg("mean") = true);
+  def("cross_entropy_backward",
+        [](const Tensor& g, const OptTensor& saved, const Tensor& x, const Tensor& w, const Tensor& b, const Tensor& target,
+           int64_t ignore, bool mean, bool nx, bool np) {
+          std::vector<OptTensor> r;
+          for (const Tensor& t : cross_entropy_backward(g, saved, x, w, b, target, ignore, mean, nx, np)) r.push_back(as_opt(t));
+          return r;
+        },
+        py::arg("grad_loss"), py::arg("saved"), py::arg("input"), py::arg("weight"), py::arg("bias"), py::arg("target"),
+        py::arg("ignore_index") = -100, py::arg("mean") = true, py::arg("need_input_grad") = true, py::arg("need_weight_grad") = true);
+  def("cross_entropy_layer", [](const Tensor& x, const Tensor& w, const Tensor& b, const Tensor& target, int64_t ignore,
+                                  bool mean) -> OptTensor {
+    if (seen_by_torch({&x, &w, &b, &target})) return c10::nullopt;
+    if (!records({&x, &w, &b})) return cross_entropy_forward(x, w, b, target, ignore, mean).first;
+    return CrossEntropyFn::apply(x, w, b, target, ignore, mean);
+  });
+  // AdamW over many tensors
+  def("adamw_step", &adamw_step, py::arg("params"), py::arg("grads"), py::arg("exp_avgs"), py::arg("exp_avg_sqs"),
+        py::arg("exp_avg_scales"), py::arg("exp_avg_sq_scales"), py::arg("masters"), py::arg("steps"), py::arg("lr"),
+        py::arg("beta1"), py::arg("beta2"), py::arg("eps"), py::arg("weight_decay"));
+  def("adamw_moments", &adamw_moments, py::arg("exp_avgs"), py::arg("exp_avg_sqs"), py::arg("exp_avg_scales"),
+        py::arg("exp_avg_sq_scales"));
   def("clear_plan_cache", &clear_plan_cache);
   def("plan_cache_kinds", &plan_cache_kinds);
   // Row plans (the fast path for maps that are translation invariant along image rows) on / off;

@@ -1,6 +1,7 @@
-from .layers import (Convolution, GatedFeedForward, MappedAvgPool, MappedAvgUnpool, MappedConvolution, MappedMaxPool,
-                     MappedTransposedConvolution, PointwiseConvolution, Resample, TransposedConvolution, Unresample)
+from .layers import (Convolution, GatedFeedForward, GroupNorm, MappedAvgPool, MappedAvgUnpool, MappedConvolution, MappedMaxPool,
+                     MappedTransposedConvolution, PointwiseConvolution, PointwiseCrossEntropy, Resample, TransposedConvolution,
+                     Unresample)
 
 __all__ = ["Convolution", "TransposedConvolution", "MappedConvolution", "MappedTransposedConvolution",
            "MappedMaxPool", "MappedAvgPool", "MappedAvgUnpool", "Resample", "Unresample", "PointwiseConvolution",
-           "GatedFeedForward"]
+           "GatedFeedForward", "GroupNorm", "PointwiseCrossEntropy"]

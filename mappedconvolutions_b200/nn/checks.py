@@ -88,3 +88,19 @@ def check_mix_args(x, in_channels, out_channels, residual):
             'Residual must have the shape of the output ({} != {})'.format(tuple(residual.shape), want)
         assert residual.dtype == x.dtype, \
             'Input and residual must be the same dtype ({} != {})'.format(x.dtype, residual.dtype)
+
+
+def check_norm_args(x, num_channels):
+    assert x.dim() == 4, 'Input must have 4 dimensions ({} != 4)'.format(x.dim())
+    assert x.shape[1] == num_channels, \
+        'Number of input channels must match the layer ({} != {})'.format(x.shape[1], num_channels)
+
+
+REDUCTIONS = {"sum": False, "mean": True}
+
+
+def check_target(x, target):
+    assert target.dtype == torch.int64, 'Target must be int64 ({})'.format(target.dtype)
+    want = (x.shape[0],) + tuple(x.shape[2:])
+    assert tuple(target.shape) == want, \
+        'Target must have the shape of the image ({} != {})'.format(tuple(target.shape), want)

@@ -202,7 +202,7 @@ class FirstDerivative(Function):
 
     @staticmethod
     def backward(ctx, *g):
-        raise RuntimeError("second derivatives of the channel-mixing layers are not available")
+        raise RuntimeError("second derivatives of the channel-mixing, normalisation and loss layers are not available")
 
 
 class PointwiseFn(Function):
@@ -249,6 +249,44 @@ class GatedFn(Function):
         return (*g, gy if need[5] else None, None)
 
 
+class GroupNormFn(Function):
+    """act(group norm); weight and bias may be None (no counterpart in the reference)"""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, groups, eps, activation):
+        ctx.args = int(groups), float(eps), int(activation)
+        y, stats = ops.group_norm_forward(x, weight, bias, *ctx.args)
+        ctx.save_for_backward(x, weight, bias, stats)
+        return y
+
+    @staticmethod
+    def backward(ctx, gy):
+        x, weight, bias, stats = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        g = FirstDerivative.apply(lambda: ops.group_norm_backward(gy, stats, x, weight, bias, *ctx.args, need[0],
+                                                                  need[1] or need[2]), gy, x, weight, bias)
+        return (*g, None, None, None)
+
+
+class CrossEntropyFn(Function):
+    """softmax cross entropy of W x + bias at every pixel (no counterpart in the reference)"""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, target, ignore_index, mean):
+        ctx.args = int(ignore_index), bool(mean)
+        loss, saved = ops.cross_entropy_forward(x, weight, bias, target, *ctx.args)
+        ctx.save_for_backward(x, weight, bias, target, saved)
+        return loss
+
+    @staticmethod
+    def backward(ctx, g):
+        x, weight, bias, target, saved = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        g = FirstDerivative.apply(lambda: ops.cross_entropy_backward(g.contiguous(), saved, x, weight, bias, target, *ctx.args,
+                                                                     need[0], need[1] or need[2]), g, x, weight, bias)
+        return (*g, None, None, None)
+
+
 def _layer_call(function, node_name):
     """The extension's node of that name, which returns None where torch has to see the Function (see above)."""
     node = getattr(ops, node_name, None)  # (the ctypes twin has no nodes)
@@ -270,3 +308,5 @@ resample = _layer_call(ResampleFn, "resample_layer")
 unresample = _layer_call(UnresampleFn, "unresample_layer")
 pointwise = _layer_call(PointwiseFn, "pointwise_layer")
 gated = _layer_call(GatedFn, "gated_layer")
+group_norm = _layer_call(GroupNormFn, "group_norm_layer")
+cross_entropy = _layer_call(CrossEntropyFn, "cross_entropy_layer")

@@ -6,7 +6,8 @@ import torch
 import torch.nn as nn
 
 from . import functions as F
-from .checks import activation_code, check_args, check_input_map_shape, check_mix_args, interp_code
+from .checks import (REDUCTIONS, activation_code, check_args, check_input_map_shape, check_mix_args, check_norm_args,
+                     check_target, interp_code)
 
 
 class _ConvBase(nn.Module):
@@ -265,3 +266,64 @@ class GatedFeedForward(nn.Module):
     def forward(self, x, residual=None):
         check_mix_args(x, self.in_channels, self.out_channels, residual)
         return F.gated(x, self.weight_in, self.bias_in, self.weight_out, self.bias_out, residual, self._act)
+
+
+class GroupNorm(nn.Module):
+    """act((x - mean) / sqrt(var + eps) * weight + bias), mean and variance over a group of neighbouring channels at all
+    pixels of an image: torch.nn.GroupNorm of an image or mesh, its parameters, their names and their initialisation, with the
+    activation in the same pass.  Not in the reference.
+
+    forward(x (B,C,H,W)) -> (B,C,H,W) in x's layout
+    activation: None, 'relu', 'gelu', 'gelu_tanh', 'silu' or 'sigmoid'.
+    """
+
+    def __init__(self, num_groups, num_channels, eps=1e-5, affine=True, *, activation=None):
+        super().__init__()
+        assert num_groups > 0 and num_channels > 0 and num_channels % num_groups == 0, \
+            'num_groups must divide num_channels ({}, {})'.format(num_groups, num_channels)
+        assert eps >= 0, 'eps must not be negative ({})'.format(eps)
+        self.num_groups = num_groups
+        self.num_channels = num_channels
+        self.eps = eps
+        self.affine = affine
+        self.activation = activation
+        self._act = activation_code(activation)
+        if affine:
+            self.weight = nn.Parameter(torch.empty(num_channels))
+            self.bias = nn.Parameter(torch.empty(num_channels))
+        else:
+            self.register_parameter("weight", None)
+            self.register_parameter("bias", None)
+        self.reset_parameters()
+
+    def reset_parameters(self):
+        if self.affine:
+            nn.init.ones_(self.weight)
+            nn.init.zeros_(self.bias)
+
+    def forward(self, x):
+        check_norm_args(x, self.num_channels)
+        return F.group_norm(x, self.weight, self.bias, self.num_groups, self.eps, self._act)
+
+
+class PointwiseCrossEntropy(_ConvBase):
+    """Softmax cross entropy of the class scores W x + bias at every pixel or mesh vertex against a label each, without the
+    scores in memory: for many classes, the vertices of a reference mesh say.  Parameters and their initialisation are those
+    of PointwiseConvolution, which gives the scores themselves.  Not in the reference.
+
+    forward(x (B,C_in,H,W), target (B,H,W) int64) -> 0-dim loss, float32 (float64 of a float64 input)
+    Pixels whose target is ignore_index are left out, whatever their features are; any other target outside
+    [0, num_classes) makes the loss NaN.  reduction: 'mean' over the other pixels (NaN if there are none) or 'sum'.
+    """
+
+    def __init__(self, in_channels, num_classes, bias=True, *, ignore_index=-100, reduction='mean'):
+        super().__init__(in_channels, num_classes, 1, 'nearest', bias, False)
+        assert reduction in REDUCTIONS, 'Unsupported reduction ({} is none of {})'.format(reduction, list(REDUCTIONS))
+        self.num_classes = num_classes
+        self.ignore_index = ignore_index
+        self.reduction = reduction
+
+    def forward(self, x, target):
+        check_mix_args(x, self.in_channels, self.out_channels, None)
+        check_target(x, target)
+        return F.cross_entropy(x, self.weight, self.bias, target, self.ignore_index, REDUCTIONS[self.reduction])

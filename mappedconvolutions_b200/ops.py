@@ -1039,3 +1039,237 @@ def clip_gradients(tensors, max_norm, norm_type=2.0, out=None):
     for t in (tensors if out is None else out):
         torch.autograd.graph.increment_version(t)
     return norm
+
+
+# ------------------------------------------------------------------------------------------
+# group normalisation with an activation (no counterpart in the reference)
+# ------------------------------------------------------------------------------------------
+
+def _norm_args(x, weight, bias, groups, eps, activation):
+    if x.dim() != 4:
+        raise RuntimeError("input must be 4-D (B, C, H, W)")
+    c = x.shape[1]
+    if not (groups > 0 and c % groups == 0):
+        raise RuntimeError("groups must divide the channels (%d, %d)" % (groups, c))
+    for name, t in (("weight", weight), ("bias", bias)):
+        if t is not None:
+            _check_like(t, name, (c,), x)
+            if not t.is_contiguous():
+                raise RuntimeError("%s must be contiguous" % name)
+    if x.dtype not in _DT:
+        raise RuntimeError("unsupported dtype %s (float32, float64, bfloat16)" % x.dtype)
+    if c >= 1 << 31:
+        raise RuntimeError("size beyond a fixed limit: more than 2^31 channels")
+    layout = _layout(x)
+    return layout, _lib.McNormDesc(x.shape[0], x.shape[2] * x.shape[3], c, int(groups), int(activation), _DT[x.dtype], layout,
+                                   float(eps))
+
+
+def group_norm_forward(input, weight, bias, groups, eps=1e-5, activation=0):
+    """act(group norm) -> [output, the statistics that group_norm_backward needs]; weight and bias may be None"""
+    dev = _need_cuda(input, weight, bias)
+    layout, d = _norm_args(input, weight, bias, groups, eps, activation)
+    y = _empty(input.shape, input, layout)
+    if y.numel() == 0:
+        return [y, None]
+    with torch.cuda.device(dev):
+        L = lib()
+        stats = _bytes(L.mc_group_norm_stats_bytes(d), dev)
+        wst, wsn, wsp = _ws(L.mc_group_norm_workspace_bytes(d, 0), dev)
+        input = _a16(input)
+        check(L.mc_group_norm_fwd(d, input.data_ptr(), _ptr(weight), _ptr(bias), y.data_ptr(), _ptr(stats), wsp, wsn, _stream()))
+    return [y, stats]
+
+
+def group_norm_backward(grad_output, stats, input, weight, bias, groups, eps=1e-5, activation=0, need_input_grad=True,
+                        need_weight_grad=True):
+    """-> [grad_input, grad_weight, grad_bias]; the latter two None where there is no weight or bias"""
+    dev = _need_cuda(grad_output, stats, input, weight, bias)
+    layout, d = _norm_args(input, weight, bias, groups, eps, activation)
+    _check_like(grad_output, "grad_output", input.shape, input)
+    nothing = input.numel() == 0
+    gx = _empty(input.shape, input, layout) if need_input_grad else None
+    make = torch.zeros_like if nothing else torch.empty_like
+    gw, gb = (make(t) if need_weight_grad and t is not None else None for t in (weight, bias))
+    if nothing:
+        return [gx, gw, gb]
+    with torch.cuda.device(dev):
+        L = lib()
+        _check_saved(stats, L.mc_group_norm_stats_bytes(d))
+        wst, wsn, wsp = _ws(L.mc_group_norm_workspace_bytes(d, 1), dev)
+        input, grad_output = _a16(input), _a16(_as_layout(grad_output, layout))
+        check(L.mc_group_norm_bwd(d, grad_output.data_ptr(), input.data_ptr(), _ptr(weight), _ptr(bias), _ptr(stats), _ptr(gx),
+                                  _ptr(gw), _ptr(gb), wsp, wsn, _stream()))
+    return [gx, gw, gb]
+
+
+# ------------------------------------------------------------------------------------------
+# softmax cross entropy of a pointwise classifier (no counterpart in the reference)
+# ------------------------------------------------------------------------------------------
+
+def _ce_args(x, weight, bias, target, ignore_index, mean):
+    if x.dim() != 4:
+        raise RuntimeError("input must be 4-D (B, C, H, W)")
+    classes, _ = _weight_dims(weight, "weight")
+    _check_mix(x, [("weight", weight, (classes, x.shape[1], 1)), ("bias", bias, (classes,))], None, classes)
+    if target.dtype != torch.int64:
+        raise RuntimeError("target must be int64")
+    want = (x.shape[0], x.shape[2], x.shape[3])
+    if tuple(target.shape) != want:
+        raise RuntimeError("target must have shape %s, got %s" % (want, tuple(target.shape)))
+    if x.dtype not in _DT:
+        raise RuntimeError("unsupported dtype %s (float32, float64, bfloat16)" % x.dtype)
+    if x.shape[1] == 0 or classes == 0:
+        raise RuntimeError("there must be a channel and a class")
+    if max(x.shape[1], classes) >= 1 << 31:
+        raise RuntimeError("size beyond a fixed limit: more than 2^31 channels")
+    layout = _layout(x)
+    loss = torch.float64 if x.dtype == torch.float64 else torch.float32
+    return layout, loss, _lib.McCeDesc(x.shape[0], x.shape[2] * x.shape[3], int(ignore_index), x.shape[1], classes,
+                                       1 if mean else 0, _DT[x.dtype], layout)
+
+
+def cross_entropy_forward(input, weight, bias, target, ignore_index=-100, mean=True):
+    """softmax cross entropy of the class scores W x + bias at every pixel -> [loss, what cross_entropy_backward needs]"""
+    dev = _need_cuda(input, weight, bias, target)
+    layout, dtype, d = _ce_args(input, weight, bias, target, ignore_index, mean)
+    if target.numel() == 0:
+        return [torch.full((), float("nan") if mean else 0.0, dtype=dtype, device=dev), None]
+    loss = torch.empty((), dtype=dtype, device=dev)
+    with torch.cuda.device(dev):
+        L = lib()
+        saved = _bytes(L.mc_cross_entropy_saved_bytes(d), dev)
+        wst, wsn, wsp = _ws(L.mc_cross_entropy_workspace_bytes(d, 0), dev)
+        input, weight, target = _a16(input), _a16(weight), target.contiguous()
+        check(L.mc_cross_entropy_fwd(d, input.data_ptr(), weight.data_ptr(), bias.data_ptr(), target.data_ptr(), loss.data_ptr(),
+                                     _ptr(saved), wsp, wsn, _stream()))
+    return [loss, saved]
+
+
+def cross_entropy_backward(grad_loss, saved, input, weight, bias, target, ignore_index=-100, mean=True, need_input_grad=True,
+                           need_weight_grad=True):
+    """-> [grad_input, grad_weight, grad_bias]"""
+    dev = _need_cuda(grad_loss, saved, input, weight, bias, target)
+    layout, dtype, d = _ce_args(input, weight, bias, target, ignore_index, mean)
+    if grad_loss.dtype != dtype or grad_loss.numel() != 1:
+        raise RuntimeError("grad_loss must be one value of the loss's type")
+    nothing = target.numel() == 0
+    gx = _empty(input.shape, input, layout) if need_input_grad else None
+    make = torch.zeros if nothing else torch.empty
+    gw, gb = (make(t.shape, dtype=t.dtype, device=dev) if need_weight_grad else None for t in (weight, bias))
+    if nothing:
+        return [gx, gw, gb]
+    with torch.cuda.device(dev):
+        L = lib()
+        _check_saved(saved, L.mc_cross_entropy_saved_bytes(d))
+        wst, wsn, wsp = _ws(L.mc_cross_entropy_workspace_bytes(d, 1), dev)
+        input, weight, target = _a16(input), _a16(weight), target.contiguous()
+        check(L.mc_cross_entropy_bwd(d, grad_loss.data_ptr(), input.data_ptr(), weight.data_ptr(), bias.data_ptr(),
+                                     target.data_ptr(), _ptr(saved), _ptr(gx), _ptr(gw), _ptr(gb), wsp, wsn, _stream()))
+    return [gx, gw, gb]
+
+
+# ------------------------------------------------------------------------------------------
+# AdamW over many tensors (no counterpart in the reference)
+# ------------------------------------------------------------------------------------------
+
+def _same_order(a, b):
+    """Element i of a's memory belongs to element i of b's."""
+    if a.shape != b.shape or not _dense(a) or not _dense(b):
+        return False
+    return all(s <= 1 or x == y for s, x, y in zip(a.shape, a.stride(), b.stride())) or (a.is_contiguous() and b.is_contiguous())
+
+
+def _adamw_check(params, grads, exp_avgs, exp_avg_sqs, scales, sq_scales, masters, steps):
+    if not params:
+        raise RuntimeError("no tensor given")
+    if len({len(v) for v in (params, grads, exp_avgs, exp_avg_sqs, scales, sq_scales, masters, steps)}) != 1:
+        raise RuntimeError("all lists must have as many entries as there are parameters")
+    dev = _need_cuda(*[t for v in (params, grads, exp_avgs, exp_avg_sqs, scales, sq_scales, masters) for t in v])
+    ready, written = [], []
+    for p, g, m, v, s, q, w, step in zip(params, grads, exp_avgs, exp_avg_sqs, scales, sq_scales, masters, steps):
+        if p.dtype not in _DT:
+            raise RuntimeError("unsupported dtype %s (float32, float64, bfloat16)" % p.dtype)
+        if g.layout != torch.strided or g.shape != p.shape or g.dtype not in _DT or \
+                (g.dtype == torch.float64) != (p.dtype == torch.float64):
+            raise RuntimeError("a gradient must be a dense tensor of its parameter's shape: float64 for float64 parameters, float32 or "
+                               "bfloat16 for the others")
+        if not _dense(p):
+            raise RuntimeError("a parameter must lie in memory without gaps and overlaps")
+        wide = torch.float64 if p.dtype == torch.float64 else torch.float32
+        eight = m.dtype == torch.int8
+        if not (_same_order(m, p) and _same_order(v, p) and
+                ((m.dtype, v.dtype) == (torch.int8, torch.uint8) if eight else m.dtype == v.dtype == wide)):
+            raise RuntimeError("moments must lie as their parameter does: float32 (float64 for float64 parameters), or int8 and uint8")
+        if eight and p.dtype == torch.float64:
+            raise RuntimeError("moments of float64 parameters are float64")
+        if eight:
+            want = ((p.numel() + 255) // 256,)
+            if any(t is None or t.dtype != torch.float32 or tuple(t.shape) != want or not t.is_contiguous() for t in (s, q)):
+                raise RuntimeError("moments in 8 bits need a float32 scale for 256 elements each")
+        elif s is not None or q is not None:
+            raise RuntimeError("moments in 32 bits have no scales")
+        if w is not None and (p.dtype != torch.bfloat16 or w.dtype != torch.float32 or not _same_order(w, p)):
+            raise RuntimeError("master weights are float32 copies of bfloat16 parameters that lie as these do")
+        if step < 1:
+            raise RuntimeError("steps are counted from 1")
+        mine = [t for t in (p, m, v, s, q, w) if t is not None]
+        if any(t.is_inference() for t in mine) and not torch.is_inference_mode_enabled():
+            raise RuntimeError("a tensor made in inference mode can be updated in inference mode only")
+        written += mine
+        if not _same_order(g, p):
+            g = torch.empty_strided(p.shape, p.stride(), dtype=g.dtype, device=dev).copy_(g)
+        ready.append(g)
+    spans = sorted([(t.data_ptr(), t.data_ptr() + t.numel() * t.element_size(), True) for t in written if t.numel()] +
+                   [(t.data_ptr(), t.data_ptr() + t.numel() * t.element_size(), False) for t in ready if t.numel()])
+    end_any = end_dst = 0
+    for begin, end, is_dst in spans:
+        if begin < (end_any if is_dst else end_dst):
+            raise RuntimeError("tensors of a step must not share memory with each other")
+        end_any = max(end_any, end)
+        if is_dst:
+            end_dst = max(end_dst, end)
+    return dev, ready, written
+
+
+def adamw_step(params, grads, exp_avgs, exp_avg_sqs, exp_avg_scales, exp_avg_sq_scales, masters, steps, lr, beta1, beta2, eps,
+               weight_decay):
+    """One AdamW step over all tensors, in place; `steps` counts this one.  Moments are float32 (float64), or int8 and uint8
+    codes with a float32 scale for 256 elements; scales and masters are None where there are none."""
+    lists = [[None if t is None else t.detach() for t in v]
+             for v in (params, grads, exp_avgs, exp_avg_sqs, exp_avg_scales, exp_avg_sq_scales, masters)]
+    dev, grads, written = _adamw_check(*lists, steps)
+    params, _, exp_avgs, exp_avg_sqs, exp_avg_scales, exp_avg_sq_scales, masters = lists
+    ts = (_lib.McAdamwTensor * len(params))()
+    for t, p, g, m, v, s, q, w, step in zip(ts, params, grads, exp_avgs, exp_avg_sqs, exp_avg_scales, exp_avg_sq_scales, masters,
+                                            steps):
+        t.p, t.g, t.master, t.m, t.v, t.m_scale, t.v_scale = (_ptr(x) for x in (p, g, w, m, v, s, q))
+        t.numel, t.step, t.p_dtype, t.g_dtype = p.numel(), int(step), _DT[p.dtype], _DT[g.dtype]
+        t.bits = 8 if m.dtype == torch.int8 else 32
+    with torch.cuda.device(dev):
+        check(lib().mc_adamw_step(len(params), ts, _lib.McAdamwHyper(lr, beta1, beta2, eps, weight_decay), _stream()))
+    for t in written:
+        torch.autograd.graph.increment_version(t)
+
+
+def adamw_moments(exp_avgs, exp_avg_sqs, exp_avg_scales, exp_avg_sq_scales):
+    """What moments in 8 bits stand for -> (list of float32 exp_avg, list of float32 exp_avg_sq)"""
+    lists = (exp_avgs, exp_avg_sqs, exp_avg_scales, exp_avg_sq_scales)
+    if not exp_avgs:
+        raise RuntimeError("no tensor given")
+    if len({len(v) for v in lists}) != 1:
+        raise RuntimeError("all lists must have as many entries")
+    dev = _need_cuda(*[t for v in lists for t in v])
+    ts, out = (_lib.McAdamwTensor * len(exp_avgs))(), ([], [])
+    for t, m, v, s, q in zip(ts, *lists):
+        want = ((m.numel() + 255) // 256,)
+        if m.dtype != torch.int8 or v.dtype != torch.uint8 or not _same_order(m, v) or \
+                any(x.dtype != torch.float32 or tuple(x.shape) != want or not x.is_contiguous() for x in (s, q)):
+            raise RuntimeError("moments in 8 bits are int8 and uint8 tensors that lie alike, with a float32 scale for 256 elements each")
+        for o in out:
+            o.append(torch.empty_strided(m.shape, m.stride(), dtype=torch.float32, device=dev))
+        t.p, t.master, t.m, t.v, t.m_scale, t.v_scale = (_ptr(x) for x in (out[0][-1], out[1][-1], m, v, s, q))
+        t.numel, t.bits = m.numel(), 8
+    with torch.cuda.device(dev):
+        check(lib().mc_adamw_moments(len(exp_avgs), ts, _stream()))
+    return out
