@@ -1,19 +1,30 @@
-// Softmax cross entropy of a pointwise classifier: entry points, and the way of float32, float64 and wide bf16 layers.
+// Softmax cross entropy of a pointwise classifier.
 //
-// Class scores are never kept: a call takes the pixels in pieces whose scores fit the workspace (PIECE bytes, which stay in L2),
-// multiplies with the kernels of the channel-mixing layers and reduces the piece's rows; the backward call computes the scores again.
-// Bound: the products (FMA issue).
-#include <initializer_list>
-
-#include "classify.cuh"
+// With P = B * S pixels, row vectors x_p, class scores z_p = x_p W^T + b (V of them) and labels t_p:
+//   lse_p = log sum_v exp(z_pv),   loss = scale sum_p (lse_p - z_p,t_p),   scale = 1 / labelled pixels, or 1
+//   gz_pv = g scale (exp(z_pv - lse_p) - [v = t_p]),   gx = gz W,   gW = gz^T x,   gb = sum_p gz
+// A pixel whose label is `ignore` counts nothing: its lse is kept as +infinity, its gz is zero and its features are read as
+// zeros, whatever they are.  A label outside [0, V) makes the loss NaN, and the gradients that the pixel takes part in: its lse is kept as NaN.
+//
+// bf16 (tensor cores): the scores of 256 pixels x up to 256 classes stand in TMEM; the forward call keeps their largest and the
+// sum of their exponentials, the backward call computes them again, rounds gz to bf16 - which the next two products' operand is -
+// and multiplies it, a piece of the pixels at a time.
+// float32 and float64 (CUDA cores): scores of a piece of the pixels in the workspace, with the kernels of the channel-mixing
+// layers.  Bound: the products.
+#include "mix_work.cuh"
 
 namespace mc {
 namespace classify {
 using mix::RowsArgs;
 using mix::View;
 
-constexpr size_t PIECE = 48u << 20;
+// What a forward call keeps: the number of labelled pixels (a double), from byte 256 on lse of every pixel, and behind it the input as
+// rows of channels where it lies in another way (bf16).
+constexpr size_t KEPT_HEAD = 256;
+constexpr size_t PIECE = 48u << 20;      // bytes of scores at a time, CUDA cores (they stay in L2)
+constexpr size_t PIECE_TC = 1024u << 20; // bytes of gz at a time, tensor cores
 constexpr int THREADS = 256;
+constexpr int SUM_BLOCKS = 296;          // blocks that add losses up
 
 __device__ __forceinline__ float exp_of(float v) { return expf(v); }
 __device__ __forceinline__ double exp_of(double v) { return exp(v); }
@@ -68,11 +79,11 @@ __global__ void __launch_bounds__(THREADS) score_grad_kernel(CT* __restrict__ z,
   }
 }
 
-// (pixels, C) wherever they lie -> rows of CT; those of pixels without a label are zero if lse is given
-template <typename T, typename CT>
+// (pixels, C) wherever they lie -> rows; those of pixels without a label are zero
+template <typename T>
 __global__ void __launch_bounds__(THREADS) rows_kernel(const T* __restrict__ src, long long pix, long long ch, long long n, int C,
-                                                       const CT* __restrict__ lse, CT* __restrict__ dst) {
-  __shared__ CT tile[32][33];
+                                                       const T* __restrict__ lse, T* __restrict__ dst) {
+  __shared__ T tile[32][33];
   // 32 pixels x 32 channels, read along whichever direction is contiguous
   const int tx = threadIdx.x % 32, ty = threadIdx.x / 32;
   const long long p0 = blockIdx.x * 32ll;
@@ -81,46 +92,21 @@ __global__ void __launch_bounds__(THREADS) rows_kernel(const T* __restrict__ src
     for (int k = ty; k < 32; k += THREADS / 32) {
       const long long p = p0 + (ch == 1 ? k : tx);
       const int c = c0 + (ch == 1 ? tx : k);
-      CT v = CT(0);
-      if (p < n && c < C && !(lse && lse[p] == CT(INFINITY))) v = (CT)ldv(src + p * pix + (long long)c * ch);
-      tile[ch == 1 ? k : tx][ch == 1 ? tx : k] = v;
+      tile[ch == 1 ? k : tx][ch == 1 ? tx : k] = p < n && c < C && lse[p] != T(INFINITY) ? src[p * pix + (long long)c * ch] : T(0);
     }
     __syncthreads();
     for (int k = ty; k < 32; k += THREADS / 32)
       if (p0 + k < n && c0 + tx < C) dst[(p0 + k) * C + c0 + tx] = tile[k][tx];
   }
 }
-// and back
-template <typename T, typename CT>
-__global__ void __launch_bounds__(THREADS) unrows_kernel(const CT* __restrict__ src, T* __restrict__ dst, long long pix,
-                                                         long long ch, long long n, int C) {
-  __shared__ CT tile[32][33];
-  const int tx = threadIdx.x % 32, ty = threadIdx.x / 32;
-  const long long p0 = blockIdx.x * 32ll;
-  for (int c0 = blockIdx.y * 32; c0 < C; c0 += gridDim.y * 32) {
-    __syncthreads();
-    for (int k = ty; k < 32; k += THREADS / 32)
-      if (p0 + k < n && c0 + tx < C) tile[k][tx] = src[(p0 + k) * C + c0 + tx];
-    __syncthreads();
-    for (int k = ty; k < 32; k += THREADS / 32) {
-      const int r = ch == 1 ? k : tx, q = ch == 1 ? tx : k;
-      if (p0 + r < n && c0 + q < C) stv(dst + (p0 + r) * pix + (long long)(c0 + q) * ch, tile[r][q]);
-    }
-  }
-}
-template <typename T, typename CT>
-__global__ void __launch_bounds__(THREADS) convert_kernel(const T* __restrict__ src, CT* __restrict__ dst, long long n) {
-  for (long long i = blockIdx.x * (long long)THREADS + threadIdx.x; i < n; i += gridDim.x * (long long)THREADS) stv(dst + i, (CT)ldv(src + i));
-}
-// acc (+)= the shares of one piece, in order; the last piece's call rounds to `out`
-template <typename T, typename CT>
-__global__ void __launch_bounds__(THREADS) gather_kernel(const CT* __restrict__ part, long long n, int splits, CT* __restrict__ acc,
+// acc (+)= the shares of one piece, in order; the last piece's sums go to `out`
+template <typename T>
+__global__ void __launch_bounds__(THREADS) gather_kernel(const T* __restrict__ part, long long n, int splits, T* __restrict__ acc,
                                                          bool first, T* __restrict__ out) {
   for (long long i = blockIdx.x * (long long)THREADS + threadIdx.x; i < n; i += gridDim.x * (long long)THREADS) {
-    CT s = first ? CT(0) : acc[i];
+    T s = first ? T(0) : acc[i];
     for (int j = 0; j < splits; ++j) s += part[j * n + i];
-    if (out) stv(out + i, s);
-    else acc[i] = s;
+    (out ? out : acc)[i] = s;
   }
 }
 
@@ -153,18 +139,73 @@ __global__ void __launch_bounds__(THREADS) loss_kernel(const double* part, int b
     *loss = (CT)(mean ? s / n : s);  // (no labelled pixel: 0 / 0)
   }
 }
-template <typename CT>
-int sum_loss(const CT* value, const int64_t* target, long long P, long long ignore, bool mean, double* part, double* count,
-             CT* loss, cudaStream_t st) {
-  const int blocks = grid_for(P, 4 * THREADS, SUM_BLOCKS);
-  loss_part_kernel<CT><<<blocks, THREADS, 0, st>>>(value, target, P, ignore, part), MC_COUNT(1);
-  loss_kernel<CT><<<1, THREADS, 0, st>>>(part, blocks, mean, count, loss), MC_COUNT(1);
-  MC_CHECK_LAUNCH();
-  return MC_OK;
+// ---- bf16 -----------------------------------------------------------------------------------------------
+// The tiles' sums of a pixel become its lse; the blocks' losses and labelled pixels go to `part`.
+__global__ void __launch_bounds__(THREADS) finish_kernel(const mix::Scores s, int tiles, long long P, int V, float* __restrict__ lse,
+                                                         double* part) {
+  __shared__ double sm[2][THREADS / 32];
+  double sum = 0, n = 0;
+  for (long long p = blockIdx.x * (long long)THREADS + threadIdx.x; p < P; p += gridDim.x * (long long)THREADS) {
+    const long long t = s.target[p];
+    if (t == s.ignore) {
+      lse[p] = INFINITY;
+      continue;
+    }
+    n += 1;
+    float out = NAN;
+    if (t >= 0 && t < V) {
+      float top = -INFINITY;
+#pragma unroll 8
+      for (int k = 0; k < tiles; ++k) top = fmaxf(top, __ldg(&s.part[k * P + p].x));  // (a NaN shows in the sum)
+      float all = 0.f;
+#pragma unroll 8
+      for (int k = 0; k < tiles; ++k) {
+        const float2 v = __ldg(s.part + k * P + p);
+        all += v.y * exp2f(v.x - top);
+      }
+      out = (top + log2f(all)) * 0.69314718056f;
+      sum += (double)(out - s.hit[p]);
+    } else {
+      sum = NAN;
+    }
+    lse[p] = out;
+  }
+  sum = warp_sum(sum), n = warp_sum(n);
+  if (threadIdx.x % 32 == 0) sm[0][threadIdx.x / 32] = sum, sm[1][threadIdx.x / 32] = n;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int i = 1; i < THREADS / 32; ++i) sum += sm[0][i], n += sm[1][i];
+    part[2 * blockIdx.x] = sum, part[2 * blockIdx.x + 1] = n;
+  }
+}
+// rows of `per` 16-byte vectors: those of pixels without a label become zeros, the others are copied (or stay, in place)
+__global__ void __launch_bounds__(THREADS) labelled_rows_kernel(const uint4* src, uint4* dst, const int64_t* __restrict__ target,
+                                                                long long ignore, long long n, int per) {
+  for (long long i = blockIdx.x * (long long)THREADS + threadIdx.x; i < n; i += gridDim.x * (long long)THREADS) {
+    const bool off = target[i / per] == ignore;
+    if (off) dst[i] = make_uint4(0, 0, 0, 0);
+    else if (src != dst) dst[i] = __ldg(src + i);
+  }
+}
+// acc (+)= the shares of one piece, in order: sums (V, C) in rows of ldn, and V column sums; the last piece rounds to gw and gb
+__global__ void __launch_bounds__(THREADS) add_piece_kernel(const float* __restrict__ part, const float* __restrict__ csum, int splits,
+                                                            int V, int C, int ldn, float* __restrict__ acc, bool first, bool last,
+                                                            bf16* gw, bf16* gb) {
+  const long long nw = (long long)V * C;
+  for (long long i = blockIdx.x * (long long)THREADS + threadIdx.x; i < nw + V; i += gridDim.x * (long long)THREADS) {
+    const bool w = i < nw;
+    float s = first ? 0.f : acc[i];
+    const float* src = w ? part + i / C * ldn + i % C : csum + (i - nw);
+    const long long step = w ? (long long)V * ldn : V;
+#pragma unroll 4
+    for (int j = 0; j < splits; ++j) s += src[j * step];
+    if (!last) acc[i] = s;
+    else if (w ? gw != nullptr : gb != nullptr) stv(w ? gw + i : gb + (i - nw), s);
+  }
 }
 
 // ---- host -----------------------------------------------------------------------------------------------
-static size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
+using mix::up256;
 static size_t csize(int dtype) { return dtype == MC_F64 ? 8 : 4; }
 static size_t esize(int dtype) { return dtype == MC_F64 ? 8 : dtype == MC_F32 ? 4 : 2; }
 static bool on(const void* p, size_t n) { return (uintptr_t)p % n == 0; }
@@ -219,33 +260,32 @@ struct Shares {
   }
 };
 
+// The way of float32 and float64 layers.
 template <typename T>
 struct General {
-  typedef typename Traits<T>::CT CT;
-  static constexpr bool CONVERT = sizeof(T) != sizeof(CT);
   const mc_ce_desc* d;
   Pieces pieces;
   Memory m;
   cudaStream_t st;
-  CT *z, *rows, *value, *w, *b, *gx, *part, *csum, *acc;
+  T *z, *rows, *value, *part, *csum, *acc;
   double* sums;
 
   General(const mc_ce_desc* desc, void* ws, bool backward, cudaStream_t s) : d(desc), pieces(desc), m(ws), st(s) {
-    const size_t n = pieces.most(), C = d->C, V = d->V, P = d->B * d->S;
-    z = (CT*)m.take(n * V * sizeof(CT));
-    rows = (CT*)(CONVERT || backward ? m.take(n * C * sizeof(CT)) : nullptr);
-    w = (CT*)(CONVERT ? m.take(V * C * sizeof(CT)) : nullptr);
-    b = (CT*)(CONVERT ? m.take(V * sizeof(CT)) : nullptr);
+    const size_t n = pieces.most(), C = d->C, V = d->V;
+    z = (T*)m.take(n * V * sizeof(T));
     if (!backward) {
-      value = (CT*)m.take(P * sizeof(CT));
+      value = (T*)m.take((size_t)d->B * d->S * sizeof(T));
       sums = (double*)m.take(SUM_BLOCKS * 16);
     } else {
-      gx = (CT*)(CONVERT ? m.take(n * C * sizeof(CT)) : nullptr);
+      rows = (T*)m.take(n * C * sizeof(T));
       int splits = 1;
-      each([&](long long, long long, long long k) { if (Shares(k, d->V, d->C).splits > splits) splits = Shares(k, d->V, d->C).splits; });
-      part = (CT*)m.take((size_t)splits * V * C * sizeof(CT));
-      csum = (CT*)m.take((size_t)splits * V * sizeof(CT));
-      acc = (CT*)m.take((V * C + V) * sizeof(CT));
+      each([&](long long, long long, long long k) {
+        const Shares sh(k, d->V, d->C);
+        if (sh.splits > splits) splits = sh.splits;
+      });
+      part = (T*)m.take((size_t)splits * V * C * sizeof(T));
+      csum = (T*)m.take((size_t)splits * V * sizeof(T));
+      acc = (T*)m.take((V * C + V) * sizeof(T));
     }
   }
   // f(image, first pixel of it, pixels in all)
@@ -266,76 +306,70 @@ struct General {
     v.ptr = p + i * v.img + s * v.pix;
     return v;
   }
-  View flat(const CT* p, long long n, int C) const { return View{p, n * C, C, 1}; }
-  dim3 tiles(long long n) const { return dim3((unsigned)((n + 31) / 32), (unsigned)((d->C + 31) / 32 < 64 ? (d->C + 31) / 32 : 64)); }
-  // pixels of a piece as rows of CT (several images one after the other)
-  void gather(const T* x, long long i, long long s, long long n, const CT* lse) {
+  View flat(const T* p, long long n, int C) const { return View{p, n * C, C, 1}; }
+  // labelled pixels of a piece as rows (several images one after the other)
+  void gather(const T* x, long long i, long long s, long long n, const T* lse) {
     const long long per = n < pieces.S ? n : pieces.S;
+    const dim3 tiles((unsigned)((per + 31) / 32), (unsigned)((d->C + 31) / 32 < 64 ? (d->C + 31) / 32 : 64));
     for (long long k = 0; k * per < n; ++k) {
       const View v = view(x, i + k, s);
-      rows_kernel<T, CT><<<tiles(per), THREADS, 0, st>>>((const T*)v.ptr, v.pix, v.ch, per, d->C, lse ? lse + k * per : nullptr,
-                                                         rows + k * per * d->C), MC_COUNT(1);
+      rows_kernel<T><<<tiles, THREADS, 0, st>>>((const T*)v.ptr, v.pix, v.ch, per, d->C, lse + k * per, rows + k * per * d->C);
+      MC_COUNT(1);
     }
   }
-  const CT* weights(const T* p, CT* to, long long n) {
-    if (!CONVERT || !p) return (const CT*)(const void*)p;
-    convert_kernel<T, CT><<<grid_for(n, THREADS, 1184), THREADS, 0, st>>>(p, to, n), MC_COUNT(1);
-    return to;
-  }
   // z = x W^T + b of a piece
-  int scores(const View& x, long long n, long long S, const CT* wc, const CT* bc) {
+  int scores(const View& x, long long n, long long S, const T* w, const T* b) {
     RowsArgs r{};
-    r.a = x, r.w = wc, r.wn = d->C, r.wk = 1, r.bias = bc, r.y = View{z, S * (long long)d->V, d->V, 1}, r.P = n, r.S = (int)S, r.N = d->V, r.K = d->C;
+    r.a = x, r.w = w, r.wn = d->C, r.wk = 1, r.bias = b, r.y = View{z, S * (long long)d->V, d->V, 1}, r.P = n, r.S = (int)S, r.N = d->V, r.K = d->C;
     return mix::simt_rows_launch(d->dtype, mix::EPI_LAYER, r, st);
   }
 
-  int forward(const T* x, const T* wt, const T* bt, const int64_t* target, CT* loss, void* kept) {
-    CT* lse = (CT*)((char*)kept + KEPT_HEAD);
-    const CT *wc = weights(wt, w, (long long)d->V * d->C), *bc = weights(bt, b, d->V);
+  int forward(const T* x, const T* w, const T* b, const int64_t* target, T* loss, void* kept) {
+    T* lse = (T*)((char*)kept + KEPT_HEAD);
     int rc = MC_OK;
     each([&](long long i, long long s, long long n) {
       if (rc) return;
-      const long long p = i * pieces.S + s, S = n < pieces.S ? n : pieces.S;
-      if (CONVERT) gather(x, i, s, n, nullptr), rc = scores(flat(rows, n, d->C), n, n, wc, bc);
-      else rc = scores(view(x, i, s), n, S, wc, bc);
-      if (rc) return;
-      lse_kernel<CT><<<(unsigned)((n + 7) / 8), THREADS, 0, st>>>(z, target + p, n, d->V, d->ignore_index, lse + p, value + p);
+      const long long p = i * pieces.S + s;
+      if ((rc = scores(view(x, i, s), n, n < pieces.S ? n : pieces.S, w, b))) return;
+      lse_kernel<T><<<(unsigned)((n + 7) / 8), THREADS, 0, st>>>(z, target + p, n, d->V, d->ignore_index, lse + p, value + p);
       MC_COUNT(1);
     });
     if (rc) return rc;
-    return sum_loss<CT>(value, target, d->B * d->S, d->ignore_index, d->reduction == MC_REDUCE_MEAN, sums, (double*)kept, loss, st);
+    const int blocks = grid_for(d->B * d->S, 4 * THREADS, SUM_BLOCKS);
+    loss_part_kernel<T><<<blocks, THREADS, 0, st>>>(value, target, d->B * d->S, d->ignore_index, sums), MC_COUNT(1);
+    loss_kernel<T><<<1, THREADS, 0, st>>>(sums, blocks, d->reduction == MC_REDUCE_MEAN, (double*)kept, loss), MC_COUNT(1);
+    MC_CHECK_LAUNCH();
+    return MC_OK;
   }
 
-  int backward(const CT* grad, const T* x, const T* wt, const T* bt, const int64_t* target, const void* kept, T* gxt, T* gw, T* gb) {
-    const CT* lse = (const CT*)((const char*)kept + KEPT_HEAD);
-    const CT *wc = weights(wt, w, (long long)d->V * d->C), *bc = weights(bt, b, d->V);
+  int backward(const T* grad, const T* x, const T* w, const T* b, const int64_t* target, const void* kept, T* gx, T* gw, T* gb) {
+    const T* lse = (const T*)((const char*)kept + KEPT_HEAD);
     const long long P = d->B * d->S, VC = (long long)d->V * d->C;
     int rc = MC_OK;
     each([&](long long i, long long s, long long n) {
       if (rc) return;
       const long long p = i * pieces.S + s, S = n < pieces.S ? n : pieces.S;
       gather(x, i, s, n, lse + p);
-      if ((rc = scores(flat(rows, n, d->C), n, n, wc, bc))) return;
-      score_grad_kernel<CT><<<grid_for(n, 8, 148 * 8), THREADS, 0, st>>>(z, target + p, lse + p, n, d->V, (const double*)kept, grad,
-                                                                        d->reduction == MC_REDUCE_MEAN), MC_COUNT(1);
-      if (gxt) {
+      if ((rc = scores(flat(rows, n, d->C), n, n, w, b))) return;
+      score_grad_kernel<T><<<grid_for(n, 8, 148 * 8), THREADS, 0, st>>>(z, target + p, lse + p, n, d->V, (const double*)kept, grad,
+                                                                       d->reduction == MC_REDUCE_MEAN), MC_COUNT(1);
+      if (gx) {
         RowsArgs r{};
-        r.a = flat(z, n, d->V), r.w = wc, r.wn = 1, r.wk = d->C, r.P = n, r.N = d->C, r.K = d->V, r.S = (int)S;
-        r.a.img = S * (long long)d->V;
-        r.y = CONVERT ? View{gx, S * (long long)d->C, d->C, 1} : view(gxt, i, s);
+        r.a = View{z, S * (long long)d->V, d->V, 1}, r.w = w, r.wn = 1, r.wk = d->C, r.P = n, r.N = d->C, r.K = d->V, r.S = (int)S;
+        r.y = view(gx, i, s);
         if ((rc = mix::simt_rows_launch(d->dtype, mix::EPI_LAYER, r, st))) return;
-        for (long long k = 0; CONVERT && k * S < n; ++k) {
-          const View v = view(gxt, i + k, s);
-          unrows_kernel<T, CT><<<tiles(S), THREADS, 0, st>>>(gx + k * S * d->C, (T*)v.ptr, v.pix, v.ch, S, d->C), MC_COUNT(1);
-        }
       }
       if (gw || gb) {
         const Shares sh(n, d->V, d->C);
         const mix::OuterArgs o{flat(z, n, d->V), flat(rows, n, d->C), part, csum, n, sh.share, d->V, d->C, 1, 1, sh.splits, sh.splits};
         if ((rc = mix::simt_outer_launch(d->dtype, o, st))) return;
         const bool first = p == 0, last = p + n == P;
-        if (gw) gather_kernel<T, CT><<<grid_for(VC, THREADS, 1184), THREADS, 0, st>>>(part, VC, sh.splits, acc, first, last ? gw : nullptr), MC_COUNT(1);
-        if (gb) gather_kernel<T, CT><<<grid_for(d->V, THREADS, 1184), THREADS, 0, st>>>(csum, d->V, sh.splits, acc + VC, first, last ? gb : nullptr), MC_COUNT(1);
+        if (first && last) {
+          mix::add_shares<T, T>(part, d->V, d->C, d->C, gw, csum, gb, sh.splits, st);
+        } else {
+          if (gw) gather_kernel<T><<<grid_for(VC, THREADS, 1184), THREADS, 0, st>>>(part, VC, sh.splits, acc, first, last ? gw : nullptr), MC_COUNT(1);
+          if (gb) gather_kernel<T><<<grid_for(d->V, THREADS, 1184), THREADS, 0, st>>>(csum, d->V, sh.splits, acc + VC, first, last ? gb : nullptr), MC_COUNT(1);
+        }
       }
     });
     if (rc) return rc;
@@ -344,11 +378,146 @@ struct General {
   }
 };
 
+// The way of bf16 layers.
+struct TensorCores {
+  const mc_ce_desc* d;
+  mc_mix_desc like;  // the same tensors as the channel-mixing kernels describe them
+  explicit TensorCores(const mc_ce_desc* desc) : d(desc) {
+    like = mc_mix_desc{d->B, d->S, d->C, d->V, 0, MC_ACT_NONE, MC_BF16, d->layout};
+  }
+  long long pixels() const { return d->B * d->S; }
+  size_t lse_bytes() const { return up256((size_t)pixels() * 4); }
+  bool in_place() const { return mix::Work::in_place(&like, d->C); }
+  size_t saved_bytes() const {
+    return KEPT_HEAD + lse_bytes() + (in_place() ? 0 : up256((size_t)pixels() * mix::pad8(d->C) * 2));
+  }
+  mix::TcRows rows_of(const void* p, long long n) const { return mix::TcRows{p, n, d->C, mix::pad8(d->C)}; }
+  void labelled(const void* src, const mix::TcRows& r, const int64_t* target, cudaStream_t st) const {
+    const int per = r.ld / 8;
+    const long long n = r.rows * per;
+    labelled_rows_kernel<<<grid_for(n, THREADS, 148 * 16), THREADS, 0, st>>>((const uint4*)src, (uint4*)r.p, target, d->ignore_index, n,
+                                                                             per), MC_COUNT(1);
+  }
+
+  int forward(mix::Work& k, const bf16* x, const bf16* w, const bf16* bias, const int64_t* target, float* loss, char* kept) const {
+    mix::TcRows xr = rows_of(x, pixels());
+    if (!in_place()) {
+      xr.p = kept ? kept + KEPT_HEAD + lse_bytes() : nullptr;
+      k.lay_out(&like, x, xr);
+      if (k.run()) labelled(xr.p, xr, target, k.st);
+    }
+    const mix::TcRows wr = k.weight(w, d->V, d->C);
+    const int tiles = mix::tc_scores_tiles(pixels(), d->C, d->V);
+    mix::Scores s{target, d->ignore_index};
+    s.part = (float2*)k.take((size_t)tiles * pixels() * 8);
+    s.hit = (float*)k.take((size_t)pixels() * 4);
+    double* part = (double*)k.take(SUM_BLOCKS * 16);
+    if (!k.run()) return k.rc;
+    k.did(mix::tc_scores_sum(xr, wr, bias, s, k.st));
+    if (k.rc) return k.rc;
+    const int blocks = grid_for(pixels(), THREADS, SUM_BLOCKS);
+    finish_kernel<<<blocks, THREADS, 0, k.st>>>(s, tiles, pixels(), d->V, (float*)(kept + KEPT_HEAD), part), MC_COUNT(1);
+    loss_kernel<float><<<1, THREADS, 0, k.st>>>(part, blocks, d->reduction == MC_REDUCE_MEAN, (double*)kept, loss), MC_COUNT(1);
+    MC_CHECK_LAUNCH();
+    return MC_OK;
+  }
+
+  // Pixels of a piece: whole images, or part of one.
+  struct Cut {
+    long long images, run;
+    Cut(const TensorCores& t) {
+      const mc_ce_desc* d = t.d;
+      const bool whole = !mix::Work::as_planes(&t.like, d->C);  // (the output need not be cut at images)
+      const long long S = whole ? d->B * d->S : d->S, B = whole ? 1 : d->B;
+      long long n = (long long)(PIECE_TC / ((size_t)mix::pad8(d->V) * 2)) / 256 * 256;
+      if (n < 256) n = 256;
+      images = n >= S ? n / S : 1;
+      if (images > B) images = B;
+      run = n >= S ? S : n;
+    }
+  };
+  int backward(mix::Work& k, const float* grad, const bf16* x, const bf16* w, const bf16* bias, const int64_t* target,
+               const char* kept, bf16* gx, bf16* gw, bf16* gb) const {
+    const long long P = pixels();
+    const Cut cut(*this);
+    const bool planes = mix::Work::as_planes(&like, d->C);
+    const long long S = planes ? d->S : P, B = planes ? d->B : 1, most = cut.images * cut.run;
+    mix::TcRows xr = rows_of(kept ? kept + KEPT_HEAD + lse_bytes() : nullptr, P);
+    if (in_place()) {
+      xr = k.fresh(P, d->C);
+      if (k.run()) labelled(x, xr, target, k.st);
+    }
+    const mix::TcRows wr = k.weight(w, d->V, d->C), wt = k.weight_t(w, d->V, d->C);
+    const mix::TcRows gz = k.fresh(most, d->V);
+    mix::TcRows out = rows_of(nullptr, most);
+    if (!planes && !in_place()) out = k.fresh(most, d->C);
+    // (shares of the largest piece; the last one can have other numbers of them)
+    int splits = 0, ldn = 0;
+    size_t floats = 0, sums = 0;
+    const auto each = [&](auto f) {
+      for (long long i = 0; i < B; i += cut.images)
+        for (long long s = 0; s < S; s += cut.run) {
+          const long long images = B - i < cut.images ? B - i : cut.images, run = S - s < cut.run ? S - s : cut.run;
+          f(i, s, images * run);
+        }
+    };
+    long long seen[2] = {0, 0};  // (there are at most a few sizes of pieces)
+    each([&](long long, long long, long long n) {
+      if (n == seen[0] || n == seen[1]) return;
+      seen[1] = seen[0], seen[0] = n;
+      const size_t f = mix::tc_outer_floats(n, d->V, 1, d->C, &splits, &ldn);
+      if (f > floats) floats = f;
+      if ((size_t)splits * d->V > sums) sums = (size_t)splits * d->V;
+    });
+    float* part = (float*)k.take(floats * 4);
+    float* csum = (float*)k.take(sums * 4);
+    float* acc = (float*)k.take(most < P ? ((size_t)d->V * d->C + d->V) * 4 : 0);
+    if (!k.run()) return k.rc;
+    const float* lse = (const float*)(kept + KEPT_HEAD);
+    each([&](long long i, long long s, long long n) {
+      if (k.rc) return;
+      const long long p = i * S + s;
+      mix::Scores sc{target + p, d->ignore_index, nullptr, nullptr, lse + p, grad,
+                     d->reduction == MC_REDUCE_MEAN ? (const double*)kept : nullptr};
+      const mix::TcRows xp = rows_of((const bf16*)xr.p + p * xr.ld, n), gp{gz.p, n, d->V, gz.ld};
+      k.did(mix::tc_scores_grad(xp, wr, bias, sc, gp, k.st));
+      if (gx && !k.rc) {
+        mix::TcRows to = rows_of(out.p, n);
+        if (planes) to = mix::TcRows{gx + i * S * d->C + s, n, d->C, 0, d->S};
+        else if (in_place()) to = mix::TcRows{gx + p * d->C, n, d->C, d->C};
+        k.did(mix::tc_input_grad(gp, wt, mix::TcRows{}, mix::TcRows{}, to, k.st));
+        if (!planes && !in_place() && !k.rc) k.did(mix::copy_rows(to.p, gx + p * d->C, n, to.ld, d->C, k.st));
+      }
+      if ((gw || gb) && !k.rc) {
+        mix::tc_outer_floats(n, d->V, 1, d->C, &splits, &ldn);
+        k.did(mix::tc_outer(gp, mix::TcRows{}, xp, part, csum, k.st));
+        if (k.rc) return;
+        const bool first = p == 0, last = p + n == P;
+        if (first && last) {
+          mix::add_shares<bf16, float>(part, d->V, d->C, ldn, gw, csum, gb, splits, k.st);
+        } else {
+          add_piece_kernel<<<grid_for((long long)d->V * d->C + d->V, THREADS, 148 * 8), THREADS, 0, k.st>>>(
+              part, csum, splits, d->V, d->C, ldn, acc, first, last, gw, gb), MC_COUNT(1);
+        }
+        k.did(cudaGetLastError() == cudaSuccess ? MC_OK : MC_ERR_LAUNCH);
+      }
+    });
+    return k.rc;
+  }
+};
+template <typename F>
+static size_t work_size(F f) {
+  mix::Work k{};
+  k.sizes = true;
+  f(k);
+  return k.used;
+}
+
+// f of the layer's arithmetic type: float32 or float64
 template <typename F>
 static auto by_type(int dtype, F f) {
   if (dtype == MC_F64) return f(double());
-  if (dtype == MC_F32) return f(float());
-  return f(bf16());
+  return f(float());
 }
 
 }  // namespace classify
@@ -359,10 +528,17 @@ extern "C" {
 
 size_t mc_cross_entropy_saved_bytes(const mc_ce_desc* d) {
   if (classify::check_desc(d)) return 0;
+  if (d->dtype == MC_BF16) return classify::TensorCores(d).saved_bytes();
   return classify::KEPT_HEAD + classify::up256((size_t)d->B * d->S * classify::csize(d->dtype));
 }
 size_t mc_cross_entropy_workspace_bytes(const mc_ce_desc* d, int32_t phase) {
   if (classify::check_desc(d)) return 0;
+  if (d->dtype == MC_BF16)
+    return classify::work_size([&](mix::Work& k) {
+      const classify::TensorCores t(d);
+      if (phase == MC_PHASE_BACKWARD) t.backward(k, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr);
+      else t.forward(k, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr);
+    });
   return classify::by_type(d->dtype, [&](auto t) {
     return classify::General<decltype(t)>(d, nullptr, phase == MC_PHASE_BACKWARD, nullptr).m.used;
   });
@@ -376,11 +552,14 @@ int mc_cross_entropy_fwd(const mc_ce_desc* d, const void* x, const void* w, cons
       !classify::on(loss, classify::csize(d->dtype)) || !classify::on(saved, 16) || !classify::on(ws, 16))
     return MC_ERR_BAD_ARG;
   if (!ws || ws_bytes < mc_cross_entropy_workspace_bytes(d, MC_PHASE_FORWARD)) return MC_ERR_WORKSPACE;
+  if (d->dtype == MC_BF16) {
+    mix::Work k{(char*)ws, (cudaStream_t)stream};
+    return classify::TensorCores(d).forward(k, (const bf16*)x, (const bf16*)w, (const bf16*)bias, target, (float*)loss, (char*)saved);
+  }
   return classify::by_type(d->dtype, [&](auto t) {
     typedef decltype(t) T;
-    typedef typename Traits<T>::CT CT;
     return classify::General<T>(d, ws, false, (cudaStream_t)stream)
-        .forward((const T*)x, (const T*)w, (const T*)bias, target, (CT*)loss, saved);
+        .forward((const T*)x, (const T*)w, (const T*)bias, target, (T*)loss, saved);
   });
 }
 int mc_cross_entropy_bwd(const mc_ce_desc* d, const void* grad_loss, const void* x, const void* w, const void* bias,
@@ -394,11 +573,15 @@ int mc_cross_entropy_bwd(const mc_ce_desc* d, const void* grad_loss, const void*
       !classify::on(gw, e) || !classify::on(gb, e) || !classify::on(ws, 16))
     return MC_ERR_BAD_ARG;
   if (!ws || ws_bytes < mc_cross_entropy_workspace_bytes(d, MC_PHASE_BACKWARD)) return MC_ERR_WORKSPACE;
+  if (d->dtype == MC_BF16) {
+    mix::Work k{(char*)ws, (cudaStream_t)stream};
+    return classify::TensorCores(d).backward(k, (const float*)grad_loss, (const bf16*)x, (const bf16*)w, (const bf16*)bias, target,
+                                             (const char*)saved, (bf16*)gx, (bf16*)gw, (bf16*)gb);
+  }
   return classify::by_type(d->dtype, [&](auto t) {
     typedef decltype(t) T;
-    typedef typename Traits<T>::CT CT;
     return classify::General<T>(d, ws, true, (cudaStream_t)stream)
-        .backward((const CT*)grad_loss, (const T*)x, (const T*)w, (const T*)bias, target, saved, (T*)gx, (T*)gw, (T*)gb);
+        .backward((const T*)grad_loss, (const T*)x, (const T*)w, (const T*)bias, target, saved, (T*)gx, (T*)gw, (T*)gb);
   });
 }
 

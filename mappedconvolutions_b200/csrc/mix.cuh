@@ -190,6 +190,22 @@ int tc_gate_bwd(const TcRows& x, const TcRows& w_in, const bf16* b_in, int act, 
 // part[s] = the s-th share of [g0|g1]^T x (rows of *ldn floats), csum[s] = its column sums of [g0|g1]; g1.p may be null
 size_t tc_outer_floats(long long P, int M, int segs, int N, int* splits, int* ldn);
 int tc_outer(const TcRows& g0, const TcRows& g1, const TcRows& x, float* part, float* csum, cudaStream_t st);
+// Class scores z = x w^T + bias (w: (V, C)), which are never stored, against labels:
+struct Scores {
+  const int64_t* target;
+  long long ignore;
+  // tc_scores_sum: the largest score of every tile of classes and the sum of exp(score - it), [tile][pixel]; the label's score
+  float2* part;
+  float* hit;
+  // tc_scores_grad: log-sum-exp (+infinity: no label, NaN: a bad one), gradient of the loss, pixels that it is divided by (or null)
+  const float* lse;
+  const float* grad;
+  const double* count;
+};
+int tc_scores_tiles(long long P, int C, int V);  // tiles of classes that tc_scores_sum leaves sums of
+int tc_scores_sum(const TcRows& x, const TcRows& w, const bf16* bias, const Scores& s, cudaStream_t st);
+// gz = grad / count (exp(z - lse) - [label])
+int tc_scores_grad(const TcRows& x, const TcRows& w, const bf16* bias, const Scores& s, const TcRows& gz, cudaStream_t st);
 // mc_mix_plan for a checked bf16 description; false: no such product
 bool tc_plan(const mc_mix_desc* d, int product, int sms, int32_t* out);
 

@@ -318,7 +318,9 @@ enum Mode {
   LAYER = 0,     // y = act(A B^T + bias) + r; two A B^T pairs can be summed
   GATE = 1,      // y = act(g) u, [g|u] = A B^T + bias: rows n and N + n of B
   GATE_BWD = 2,  // [g|u] as above from the first operands, gh from the second: y0 = gh u act'(g), y1 = gh act(g)
-  ACT_BWD = 3    // y = r act'(A B^T + bias)
+  ACT_BWD = 3,   // y = r act'(A B^T + bias)
+  SCORE_SUM = 4, // softmax sums of z = A B^T + bias over the tile's columns, the label's z
+  SCORE_GRAD = 5 // y = scale (exp(z - lse) - [label])
 };
 // BN: channels of a tile.  It is staged CW channels (128 or 64 swizzled bytes a row) at a time; the two results of
 // GATE_BWD side by side, in smaller tiles because its weights leave little room.
@@ -349,6 +351,7 @@ struct alignas(64) GemmArgs {
   // rows all the same: read here from planes, a piece ahead, its latency made the kernel twice as slow.)
   bf16* planes;
   PixDiv pd;
+  Scores sc;         // SCORE_*
   int group;         // channel tiles of a pair of blocks whose weights stay in shared memory, 0: none do
   int stages;
 };
@@ -546,6 +549,111 @@ __device__ __forceinline__ void read_out(const GemmArgs& g, int set, uint32_t ra
   }
 }
 
+// Read-out warps of a classifier: thread = pixel, sixteen classes at a time.
+// SCORE_SUM keeps the running maximum and sum of the tile's classes, in base 2; SCORE_GRAD leaves bf16 gradients of the scores in the
+// staged tiles.  Classes behind the last one have a bias of -infinity: exp makes zeros of them.
+template <int MODE, int BN>
+__device__ __forceinline__ void read_scores(const GemmArgs& g, int set, uint32_t rank, float* bias_s, uint32_t out0,
+                                            uint32_t bfull, volatile int* abort_flag) {
+  typedef Cfg<MODE, BN> C;
+  constexpr int NP = BN / 16, PER = C::CW / 16;
+  const int lane = threadIdx.x % 32, q = threadIdx.x / 32 & 3, row = q * 32 + lane;
+  const uint32_t mask = (1u << C::SLOT_BITS) - 1;
+  const uint32_t at0 = out0 + (set << C::SLOT_BITS) * C::CH_BYTES + row * C::CW * 2, swizzle = (row & 7) << 4;
+  const auto bar_of = [&](uint32_t base, uint32_t i) { return bfull + base + 32 * set + 8 * (i & mask); };
+  const uint32_t tempty0 = of_leader(bfull + BAR_TEMPTY);
+  float scale = 0.f;
+  if (MODE == SCORE_GRAD) scale = g.sc.count ? (float)((double)*g.sc.grad / *g.sc.count) : *g.sc.grad;
+  uint32_t it = 0, i = 0;
+  for (TileWalk w(g, set, 2); w.more(); w.next(), ++it) {
+    float* bs = bias_s + set * 512 + (g.group == 1 ? 0 : (it & 1) * 256);
+    const int n0 = w.nt() * BN;
+    if (it == 0 || g.group != 1) {
+      // (the other half is still being read by warps that are a tile behind; nobody is two behind)
+      for (int e = row; e < BN; e += 128) {
+        float b = n0 + e < g.N ? 0.f : -INFINITY;
+        if (g.bias && n0 + e < g.N) b = __bfloat162float(__ushort_as_bfloat16(__ldg((const unsigned short*)g.bias + n0 + e)));
+        bs[e] = b;
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bfull + BAR_BIASED + 8 * set);
+      if (!warp_wait(bfull + BAR_BIASED + 8 * set, it & 1, abort_flag, 0x153)) return;  // (bounded, unlike bar.sync)
+    }
+    const uint32_t p = (w.m() * 2 + rank) * TILE + row;
+    const bool in = p < (uint32_t)g.rows;
+    int label = -1;  // of this tile's columns
+    float lse2 = INFINITY;
+    if (in) {
+      const long long t = __ldg((const long long*)g.sc.target + p);
+      if (t >= n0 && t < n0 + BN && t < g.N && t != g.sc.ignore) label = (int)(t - n0);
+      if (MODE == SCORE_GRAD) lse2 = __ldg(g.sc.lse + p) * LOG2E;
+    }
+    const bool dead = lse2 == INFINITY;
+    const int left = (g.N - n0 + 15) / 16, live = left < NP ? left : NP;
+    uint32_t v[2][16];
+    const uint32_t tile = 2 * it + set, acc = tile % C::NACC;
+    const uint32_t t0 = ((uint32_t)(q * 32) << 16) + acc * C::ACC;
+    if (!warp_wait(bfull + BAR_TFULL + 8 * acc, tile / C::NACC & 1, abort_flag, 0x151)) return;
+    tc_fence_after_sync();
+    float top = -INFINITY, sum = 0.f, hit = 0.f;
+    const auto step = [&](int now, int pc) -> bool {
+      uint32_t(&cur)[16] = v[now];
+      if (pc < live) tmem_ld_wait();
+      if (pc + 1 < live) tmem_ld_32x16(t0 + 16 * (pc + 1), v[now ^ 1]);
+      if (pc + 1 == NP) {  // the accumulators are free
+        tc_fence_before_sync();
+        __syncwarp();
+        if (lane == 0) arrive_leader(tempty0 + 8 * acc);
+      }
+      const bool turn = MODE == SCORE_GRAD && pc % PER == 0, done = MODE == SCORE_GRAD && pc % PER == PER - 1;
+      if (turn && !warp_wait(bar_of(BAR_READY, i), i >> C::SLOT_BITS & 1, abort_flag, 0x152)) return false;
+      if (pc < live) {
+        Pairs z;
+        MC_EACH z[j] = add2(pair_of(cur, j), bias2(bs + 16 * pc, j));
+        // (a branch of the whole warp: few pieces hold a label of its pixels)
+        const int here = (label >> 4) == pc ? label & 15 : -1;
+        const bool any = __any_sync(~0u, here >= 0);
+        if (MODE == SCORE_SUM) {
+          if (any) MC_EACH hit = here == 2 * j ? z[j].x : here == 2 * j + 1 ? z[j].y : hit;
+          MC_EACH z[j] = mul2(z[j], two(LOG2E));
+          float m = top;
+          MC_EACH m = fmaxf(m, fmaxf(z[j].x, z[j].y));
+          const float base = m == -INFINITY ? 0.f : m;  // (nothing but ruled-out classes so far: sums of zeros)
+          sum *= exp2_(top - base);
+          MC_EACH z[j] = exp2_2(add2(z[j], two(-base)));
+          float2 s = add2(add2(add2(z[0], z[1]), add2(z[2], z[3])), add2(add2(z[4], z[5]), add2(z[6], z[7])));
+          sum += s.x + s.y;
+          top = m;
+        } else {
+          MC_EACH z[j] = exp2_2(fma2(z[j], two(LOG2E), two(-lse2)));
+          if (any) MC_EACH z[j] = add2(z[j], make_float2(here == 2 * j ? -1.f : 0.f, here == 2 * j + 1 ? -1.f : 0.f));
+          uint32_t r[8];
+          MC_EACH z[j] = mul2(z[j], two(scale));
+          MC_EACH r[j] = dead ? 0u : pack_bf16x2(z[j].x, z[j].y);
+          const uint32_t at = at0 + (i & mask) * C::CH_BYTES, j0 = pc % PER * 2;
+          sts16(at + ((j0 << 4) ^ swizzle), make_uint4(r[0], r[1], r[2], r[3]));
+          sts16(at + (((j0 + 1) << 4) ^ swizzle), make_uint4(r[4], r[5], r[6], r[7]));
+        }
+      }
+      if (done) {
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar_of(BAR_DONE, i));
+        ++i;
+      }
+      return true;
+    };
+    tmem_ld_32x16(t0, v[0]);
+#pragma unroll 1
+    for (int pc = 0; pc < NP; pc += 2)
+      if (!step(0, pc) || !step(1, pc + 1)) return;
+    if (MODE == SCORE_SUM && in) {
+      g.sc.part[(long long)w.nt() * g.rows + p] = make_float2(top, sum);
+      if (label >= 0) g.sc.hit[p] = hit;
+    }
+  }
+}
+
 template <int MODE, int BN>
 __global__ void __launch_bounds__(THREADS, 1) rows_tc_kernel(const __grid_constant__ GemmArgs g) {
   typedef Cfg<MODE, BN> C;
@@ -691,7 +799,7 @@ __global__ void __launch_bounds__(THREADS, 1) rows_tc_kernel(const __grid_consta
     }
   } else if (warp < 4) {
     // ---- I/O of one set's staged tiles: fill the slots ahead (residual), store what the read-out warps leave in them
-    if (lane == 0 && !(MODE == LAYER && g.planes && !g.res)) {
+    if (lane == 0 && MODE != SCORE_SUM && !(MODE == LAYER && g.planes && !g.res)) {
       const int set = warp - 2;
       TileWalk lead(g, set, 2);
       int lead_c = 0;
@@ -732,9 +840,13 @@ __global__ void __launch_bounds__(THREADS, 1) rows_tc_kernel(const __grid_consta
     __syncwarp();
   } else {
     // ---- read-out
-    with_act(g.act, [&](auto act) {
-      read_out<MODE, BN, decltype(act)>(g, (warp - 4) / 4, rank, bias_s, out0, bfull, abort_flag);
-    });
+    if constexpr (MODE == SCORE_SUM || MODE == SCORE_GRAD) {
+      read_scores<MODE, BN>(g, (warp - 4) / 4, rank, bias_s, out0, bfull, abort_flag);
+    } else {
+      with_act(g.act, [&](auto act) {
+        read_out<MODE, BN, decltype(act)>(g, (warp - 4) / 4, rank, bias_s, out0, bfull, abort_flag);
+      });
+    }
   }
   __syncthreads();
   if (*abort_flag && threadIdx.x == 0) {  // given up: copies still in flight land within microseconds
@@ -1108,6 +1220,25 @@ int tc_input_grad(const TcRows& g0, const TcRows& w0, const TcRows& g1, const Tc
   else if (!encode(&g.y[0], gx, TILE)) return MC_ERR_LAUNCH;
   if (g1.p && (!encode(&g.a[1], g1, TILE) || !encode(&g.b[1], w1, bn / 2))) return MC_ERR_LAUNCH;
   return launch_wide<LAYER>(g, bn, st);
+}
+
+int tc_scores_tiles(long long P, int C, int V) {
+  const int bn = tile_width((P + 2 * TILE - 1) / (2 * TILE), V, kblocks(C), sm_total());
+  return (V + bn - 1) / bn;
+}
+int tc_scores_sum(const TcRows& x, const TcRows& w, const bf16* bias, const Scores& s, cudaStream_t st) {
+  GemmArgs g = base_args(x, TcRows{nullptr, x.rows, (int)w.rows, 0}, bias, MC_ACT_NONE);
+  g.sc = s;
+  const int bn = tile_width(g.m_pairs, g.N, g.kb[0], sm_total());
+  if (!encode(&g.a[0], x, TILE) || !encode(&g.b[0], w, bn / 2)) return MC_ERR_LAUNCH;
+  return launch_wide<SCORE_SUM>(g, bn, st);
+}
+int tc_scores_grad(const TcRows& x, const TcRows& w, const bf16* bias, const Scores& s, const TcRows& gz, cudaStream_t st) {
+  GemmArgs g = base_args(x, gz, bias, MC_ACT_NONE);
+  g.sc = s;
+  const int bn = tile_width(g.m_pairs, g.N, g.kb[0], sm_total());
+  if (!encode(&g.a[0], x, TILE) || !encode(&g.b[0], w, bn / 2) || !encode(&g.y[0], gz, TILE)) return MC_ERR_LAUNCH;
+  return launch_wide<SCORE_GRAD>(g, bn, st);
 }
 
 // 128 hidden channels a tile of the gate, 64 where that pads less: 38 hidden channels take half the time (wide blocks 4 % more)
