@@ -187,20 +187,34 @@ __global__ void __launch_bounds__(THREADS) labelled_rows_kernel(const uint4* src
     else if (src != dst) dst[i] = __ldg(src + i);
   }
 }
-// acc (+)= the shares of one piece, in order: sums (V, C) in rows of ldn, and V column sums; the last piece rounds to gw and gb
+// acc (+)= the shares of one piece, in order: sums (V, C) in rows of ldn (a multiple of 4), and V column sums; the last piece's
+// go to gw and gb, rounded.  Four sums to a thread.
 __global__ void __launch_bounds__(THREADS) add_piece_kernel(const float* __restrict__ part, const float* __restrict__ csum, int splits,
                                                             int V, int C, int ldn, float* __restrict__ acc, bool first, bool last,
                                                             bf16* gw, bf16* gb) {
-  const long long nw = (long long)V * C;
-  for (long long i = blockIdx.x * (long long)THREADS + threadIdx.x; i < nw + V; i += gridDim.x * (long long)THREADS) {
-    const bool w = i < nw;
-    float s = first ? 0.f : acc[i];
-    const float* src = w ? part + i / C * ldn + i % C : csum + (i - nw);
-    const long long step = w ? (long long)V * ldn : V;
-#pragma unroll 4
-    for (int j = 0; j < splits; ++j) s += src[j * step];
-    if (!last) acc[i] = s;
-    else if (w ? gw != nullptr : gb != nullptr) stv(w ? gw + i : gb + (i - nw), s);
+  const long long nw = (long long)V * (ldn / 4), i = blockIdx.x * (long long)THREADS + threadIdx.x;
+  if (i < nw) {
+    float4 s = first ? make_float4(0.f, 0.f, 0.f, 0.f) : reinterpret_cast<const float4*>(acc)[i];
+#pragma unroll 8
+    for (int j = 0; j < splits; ++j) {
+      const float4 v = __ldcs(reinterpret_cast<const float4*>(part) + j * nw + i);
+      s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
+    }
+    if (!last) {
+      reinterpret_cast<float4*>(acc)[i] = s;
+    } else if (gw) {
+      const int row = (int)(i / (ldn / 4)), c = (int)(i % (ldn / 4)) * 4;
+      const float v[4] = {s.x, s.y, s.z, s.w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (c + e < C) stv(gw + (long long)row * C + c + e, v[e]);
+    }
+  } else if (i < nw + V) {
+    const long long v = i - nw;
+    float s = first ? 0.f : acc[4 * nw + v];
+    for (int j = 0; j < splits; ++j) s += csum[j * (long long)V + v];
+    if (!last) acc[4 * nw + v] = s;
+    else if (gb) stv(gb + v, s);
   }
 }
 
@@ -448,7 +462,9 @@ struct TensorCores {
       if (k.run()) labelled(x, xr, target, k.st);
     }
     const mix::TcRows wr = k.weight(w, d->V, d->C), wt = k.weight_t(w, d->V, d->C);
-    const mix::TcRows gz = k.fresh(most, d->V);
+    // (up to 64 classes are one block across: rows of their own length are shorter)
+    mix::TcRows gz{nullptr, most, d->V, d->V > 64 ? 64 : mix::pad8(d->V), 0, d->V > 64};
+    gz.p = k.take(gz.blocks ? gz.block_bytes() : (size_t)most * gz.ld * 2);
     mix::TcRows out = rows_of(nullptr, most);
     if (!planes && !in_place()) out = k.fresh(most, d->C);
     // (shares of the largest piece; the last one can have other numbers of them)
@@ -471,7 +487,8 @@ struct TensorCores {
     });
     float* part = (float*)k.take(floats * 4);
     float* csum = (float*)k.take(sums * 4);
-    float* acc = (float*)k.take(most < P ? ((size_t)d->V * d->C + d->V) * 4 : 0);
+    const long long sums_all = (long long)d->V * (ldn / 4) + d->V;  // threads of add_piece_kernel
+    float* acc = (float*)k.take(most < P ? ((size_t)d->V * ldn + d->V) * 4 : 0);
     if (!k.run()) return k.rc;
     const float* lse = (const float*)(kept + KEPT_HEAD);
     each([&](long long i, long long s, long long n) {
@@ -479,7 +496,7 @@ struct TensorCores {
       const long long p = i * S + s;
       mix::Scores sc{target + p, d->ignore_index, nullptr, nullptr, lse + p, grad,
                      d->reduction == MC_REDUCE_MEAN ? (const double*)kept : nullptr};
-      const mix::TcRows xp = rows_of((const bf16*)xr.p + p * xr.ld, n), gp{gz.p, n, d->V, gz.ld};
+      const mix::TcRows xp = rows_of((const bf16*)xr.p + p * xr.ld, n), gp{gz.p, n, d->V, gz.ld, 0, gz.blocks};
       k.did(mix::tc_scores_grad(xp, wr, bias, sc, gp, k.st));
       if (gx && !k.rc) {
         mix::TcRows to = rows_of(out.p, n);
@@ -492,13 +509,10 @@ struct TensorCores {
         mix::tc_outer_floats(n, d->V, 1, d->C, &splits, &ldn);
         k.did(mix::tc_outer(gp, mix::TcRows{}, xp, part, csum, k.st));
         if (k.rc) return;
-        const bool first = p == 0, last = p + n == P;
-        if (first && last) {
-          mix::add_shares<bf16, float>(part, d->V, d->C, ldn, gw, csum, gb, splits, k.st);
-        } else {
-          add_piece_kernel<<<grid_for((long long)d->V * d->C + d->V, THREADS, 148 * 8), THREADS, 0, k.st>>>(
-              part, csum, splits, d->V, d->C, ldn, acc, first, last, gw, gb), MC_COUNT(1);
-        }
+        // (many shares of few sums: several threads for each)
+        if (splits >= 64 && p == 0 && n == P) mix::add_shares<bf16, float>(part, d->V, d->C, ldn, gw, csum, gb, splits, k.st);
+        else add_piece_kernel<<<(unsigned)((sums_all + THREADS - 1) / THREADS), THREADS, 0, k.st>>>(
+            part, csum, splits, d->V, d->C, ldn, acc, p == 0, p + n == P, gw, gb), MC_COUNT(1);
         k.did(cudaGetLastError() == cudaSuccess ? MC_OK : MC_ERR_LAUNCH);
       }
     });

@@ -175,6 +175,11 @@ struct TcRows {
   long long rows;
   int cols, ld;  // ld == 0: an NCHW tensor with S pixels an image, as output of a layer or input gradient only
   long long S = 0;
+  // Blocks of 128 rows x 64 columns one after the other, those of the same rows next to each other; an even number of tiles of 128
+  // rows.  (Rows of 20 KB: a tile's 128 rows are 128 places in memory, 1 TB/s.)
+  bool blocks = false;
+  int across() const { return (cols + 63) / 64; }
+  size_t block_bytes() const { return (size_t)((rows + 255) / 256) * 2 * across() * (128 * 64 * 2); }
 };
 // y = act(a w^T + bias) + r, or with backward y = r act'(a w^T + bias); w (N, K), r.p may be null (not with backward)
 int tc_layer(const TcRows& a, const TcRows& w, const bf16* bias, int act, const TcRows& r, const TcRows& y, bool backward,
@@ -204,7 +209,7 @@ struct Scores {
 };
 int tc_scores_tiles(long long P, int C, int V);  // tiles of classes that tc_scores_sum leaves sums of
 int tc_scores_sum(const TcRows& x, const TcRows& w, const bf16* bias, const Scores& s, cudaStream_t st);
-// gz = grad / count (exp(z - lse) - [label])
+// gz = grad / count (exp(z - lse) - [label]), in blocks
 int tc_scores_grad(const TcRows& x, const TcRows& w, const bf16* bias, const Scores& s, const TcRows& gz, cudaStream_t st);
 // mc_mix_plan for a checked bf16 description; false: no such product
 bool tc_plan(const mc_mix_desc* d, int product, int sms, int32_t* out);

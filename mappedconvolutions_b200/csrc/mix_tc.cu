@@ -21,6 +21,7 @@
 // 2048 x 256 and 256 x 1024 gradients over 655 488 pixels: 954 us together, 1080 TFLOP/s.
 #include <cuda.h>
 
+#include "act_pairs.cuh"
 #include "mix.cuh"
 #include "tc_common.cuh"
 
@@ -35,152 +36,10 @@ constexpr int THREADS = 384;    // loader, MMA, two I/O warps, eight read-out wa
 constexpr int MAX_STAGES = 12;
 constexpr int SMEM_LIMIT = 226 * 1024;  // of 227 KB, the rest is static
 
-// ---- activations: fast forms, two values at a time ------------------------------------------------------------------
-// (packed float32 instructions: the read-out warps are short of issue slots, not of arithmetic)
-// Against 64 bits over [-100, 100] (half a bf16 step is 2^-8): values within 2^-16 of themselves for z >= -13 (GELU, 2^-17.3
-// for |z| < 5), -10 (tanh form, 2^-18.5) and -87 (SiLU, sigmoid, 2^-21.4), zero within 2e-36 below; slopes, where they are
-// sums that cross zero, within 2^-18 of one, the sigmoid's within 2^-17 of itself.
-__device__ __forceinline__ unsigned long long& bits(float2& v) { return reinterpret_cast<unsigned long long&>(v); }
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
-  float2 d;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(bits(d)) : "l"(bits(a)), "l"(bits(b)), "l"(bits(c)));
-  return d;
-}
-__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
-  float2 d;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(bits(d)) : "l"(bits(a)), "l"(bits(b)));
-  return d;
-}
-__device__ __forceinline__ float2 add2(float2 a, float2 b) {
-  float2 d;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(bits(d)) : "l"(bits(a)), "l"(bits(b)));
-  return d;
-}
-__device__ __forceinline__ float2 two(float v) { return make_float2(v, v); }
-__device__ __forceinline__ float rcp_(float v) {
-  float r;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
-  return r;
-}
-__device__ __forceinline__ float exp2_(float v) {
-  float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
-  return r;
-}
-__device__ __forceinline__ float2 rcp2(float2 v) { return make_float2(rcp_(v.x), rcp_(v.y)); }
-__device__ __forceinline__ float2 exp2_2(float2 v) { return make_float2(exp2_(v.x), exp2_(v.y)); }
-constexpr float LOG2E = 1.44269504f;
-// The functions below take NV pairs at a time, one step for all of them after the other: elementary functions answer
-// after tens of cycles, and with two read-out warps per scheduler nobody else fills the time.
+// ---- activations: the fast forms of act_pairs.cuh, sixteen values at a time
 constexpr int NV = 8;
 typedef float2 Pairs[NV];
 #define MC_EACH _Pragma("unroll") for (int j = 0; j < NV; ++j)
-// v <- 1 / (1 + 2^v): the logistic function of z for v = -z log2(e)
-__device__ __forceinline__ void logistic(Pairs& v) {
-  MC_EACH v[j] = exp2_2(v[j]);
-  MC_EACH v[j] = add2(v[j], two(1.f));
-  MC_EACH v[j] = rcp2(v[j]);
-}
-// value: z <- act(z).  both: z <- act(z), s = act'(z)
-struct ActNone {
-  __device__ static void value(Pairs&) {}
-  __device__ static void both(Pairs&, Pairs& s) { MC_EACH s[j] = two(1.f); }
-};
-struct ActRelu {
-  __device__ static float value1(float z) { return z < 0.f ? 0.f : z; }  // (NaN stays NaN)
-  __device__ static float slope1(float z) { return z > 0.f ? 1.f : (z == z ? 0.f : z); }
-  __device__ static void value(Pairs& z) { MC_EACH z[j] = make_float2(value1(z[j].x), value1(z[j].y)); }
-  __device__ static void both(Pairs& z, Pairs& s) {
-    MC_EACH s[j] = make_float2(slope1(z[j].x), slope1(z[j].y));
-    value(z);
-  }
-};
-struct ActGelu {
-  // p = Phi(z), e = exp(-z^2 / 2).  With x = |z| / sqrt(2), t = 1 / (1 + 0.44 x): exp(x^2) erfc(x) / 2 = t q(t), q a
-  // least-squares fit of the relative error over x in [0, 10] (at most 5.2e-6; e alone decays beyond).
-  __device__ static void phi(const Pairs& z, Pairs& p, Pairs& e) {
-    Pairs t;
-    MC_EACH t[j] = fma2(two(0.31112698f), make_float2(fabsf(z[j].x), fabsf(z[j].y)), two(1.f));
-    MC_EACH e[j] = mul2(mul2(z[j], two(-0.5f * LOG2E)), z[j]);
-    MC_EACH t[j] = rcp2(t[j]);
-    MC_EACH e[j] = exp2_2(e[j]);
-    MC_EACH p[j] = fma2(two(-0.07305045425891876f), t[j], two(0.1753196418285370f));
-    MC_EACH p[j] = fma2(p[j], t[j], two(0.020372465252876282f));
-    MC_EACH p[j] = fma2(p[j], t[j], two(0.1317897737026215f));
-    MC_EACH p[j] = fma2(p[j], t[j], two(0.12128554284572601f));
-    MC_EACH p[j] = fma2(p[j], t[j], two(0.12428044527769089f));
-    MC_EACH p[j] = mul2(mul2(p[j], t[j]), e[j]);
-    MC_EACH {
-      const float2 d = fma2(p[j], two(-1.f), two(1.f));
-      p[j] = make_float2(z[j].x < 0.f ? p[j].x : d.x, z[j].y < 0.f ? p[j].y : d.y);
-    }
-  }
-  __device__ static void value(Pairs& z) {
-    Pairs p, e;
-    phi(z, p, e);
-    MC_EACH z[j] = mul2(z[j], p[j]);
-  }
-  __device__ static void both(Pairs& z, Pairs& s) {
-    Pairs p, e;
-    phi(z, p, e);
-    MC_EACH s[j] = fma2(mul2(z[j], two(0.39894228f)), e[j], p[j]);
-    MC_EACH z[j] = mul2(z[j], p[j]);
-  }
-};
-struct ActGeluTanh {  // (1 + tanh(a)) / 2 is the logistic function of 2 a
-  __device__ static void part(const Pairs& z, Pairs& p) {
-    MC_EACH p[j] = mul2(mul2(z[j], two(-1.59576912f * LOG2E)), fma2(mul2(z[j], two(0.044715f)), z[j], two(1.f)));
-    logistic(p);
-  }
-  __device__ static void value(Pairs& z) {
-    Pairs p;
-    part(z, p);
-    MC_EACH z[j] = mul2(z[j], p[j]);
-  }
-  __device__ static void both(Pairs& z, Pairs& s) {
-    Pairs p;
-    part(z, p);
-    MC_EACH {  // (z^2 can overflow where p or 1 - p is zero: kept finite, the product is zero as it should be)
-      const float2 v = mul2(z[j], p[j]);
-      float2 d = fma2(mul2(z[j], two(1.59576912f * 0.134145f)), z[j], two(1.59576912f));
-      d = make_float2(fminf(d.x, 3e38f), fminf(d.y, 3e38f));
-      s[j] = fma2(mul2(v, fma2(p[j], two(-1.f), two(1.f))), d, p[j]);
-      z[j] = v;
-    }
-  }
-};
-struct ActSilu {
-  __device__ static void value(Pairs& z) {
-    Pairs p;
-    MC_EACH p[j] = mul2(z[j], two(-LOG2E));
-    logistic(p);
-    MC_EACH z[j] = mul2(z[j], p[j]);
-  }
-  __device__ static void both(Pairs& z, Pairs& s) {
-    Pairs p;
-    MC_EACH p[j] = mul2(z[j], two(-LOG2E));
-    logistic(p);
-    MC_EACH z[j] = mul2(z[j], p[j]);
-    MC_EACH s[j] = fma2(z[j], fma2(p[j], two(-1.f), two(1.f)), p[j]);
-  }
-};
-struct ActSigmoid {
-  __device__ static void value(Pairs& z) {
-    MC_EACH z[j] = mul2(z[j], two(-LOG2E));
-    logistic(z);
-  }
-  __device__ static void both(Pairs& z, Pairs& s) {  // slope s(z) s(-z), e = 2^(-|z| log2 e): 1 - s(z) would cancel
-    Pairs e;
-    MC_EACH e[j] = mul2(make_float2(fabsf(z[j].x), fabsf(z[j].y)), two(-LOG2E));
-    MC_EACH e[j] = exp2_2(e[j]);
-    MC_EACH s[j] = rcp2(add2(e[j], two(1.f)));
-    MC_EACH {
-      const float2 q = s[j], m = mul2(e[j], q);
-      s[j] = mul2(m, q);
-      z[j] = make_float2(z[j].x < 0.f ? m.x : q.x, z[j].y < 0.f ? m.y : q.y);
-    }
-  }
-};
 template <typename F>
 __device__ __forceinline__ void with_act(int act, F f) {  // one branch per read-out warp
   switch (act) {
@@ -344,6 +203,7 @@ struct alignas(64) GemmArgs {
   CUtensorMap a[2], b[2], r, y[2];
   const bf16* bias;  // null: none
   int m_pairs, rows; // pairs of tiles; pixels
+  int a_across[2], y_across;  // blocks next to each other where a tensor lies in blocks, else 0
   int n_tiles, N, kb[2], act;
   int up;            // distance between a gate's row of b[0] and bias and its factor's
   int res;           // r is read
@@ -589,7 +449,9 @@ __device__ __forceinline__ void read_scores(const GemmArgs& g, int set, uint32_t
       if (MODE == SCORE_GRAD) lse2 = __ldg(g.sc.lse + p) * LOG2E;
     }
     const bool dead = lse2 == INFINITY;
-    const int left = (g.N - n0 + 15) / 16, live = left < NP ? left : NP;
+    int live = (g.N - n0 + 15) / 16;  // pieces with classes; a staged tile is filled up with zeros
+    if (MODE == SCORE_GRAD) live = (live + PER - 1) / PER * PER;
+    if (live > NP) live = NP;
     uint32_t v[2][16];
     const uint32_t tile = 2 * it + set, acc = tile % C::NACC;
     const uint32_t t0 = ((uint32_t)(q * 32) << 16) + acc * C::ACC;
@@ -734,7 +596,8 @@ __global__ void __launch_bounds__(THREADS, 1) rows_tc_kernel(const __grid_consta
           if (elected) {
             const uint32_t bar = of_leader(full(st));
             if (rank == 0) mbar_expect_tx(full(st), 2 * (A_BYTES + (g.group ? 0 : seg ? C::B1 : C::B0)));
-            tma_load_pair(a0 + st * A_BYTES, &g.a[seg], k * KB, m0, bar);
+            const int across = g.a_across[seg];
+            tma_load_pair(a0 + st * A_BYTES, &g.a[seg], across ? 0 : k * KB, across ? m0 * across + k * TILE : m0, bar);
             if (!g.group) load_b<MODE, BN>(g, seg, rank, b0 + st * C::BMAX, k * KB, n0, bar);
           }
           __syncwarp();
@@ -829,7 +692,8 @@ __global__ void __launch_bounds__(THREADS, 1) rows_tc_kernel(const __grid_consta
           if (!ok) break;
           const int col = column(w, c), m0 = (w.m() * 2 + rank) * TILE;
           if (col < g.N && m0 < g.rows && !(MODE == LAYER && g.planes)) {
-            tma_store(&g.y[MODE == GATE_BWD ? c % 2 : 0], col, m0, buf + s * C::CH_BYTES);
+            if (MODE == SCORE_GRAD && g.y_across) tma_store(&g.y[0], 0, m0 * g.y_across + col / KB * TILE, buf + s * C::CH_BYTES);
+            else tma_store(&g.y[MODE == GATE_BWD ? c % 2 : 0], col, m0, buf + s * C::CH_BYTES);
             bulk_commit();
             bulk_wait_read();
           }
@@ -867,6 +731,7 @@ struct alignas(64) OuterTcArgs {
   int m_tiles, n_tiles;
   int kblocks, per;    // 64-pixel blocks in all, and of a share
   int stages;
+  int across;          // blocks next to each other where the first operand lies in blocks, else 0
 };
 constexpr int OUTER_BARS = 3 * MAX_STAGES + 1;
 
@@ -921,8 +786,12 @@ __global__ void __launch_bounds__(THREADS, 1) outer_tc_kernel(const __grid_const
         const uint32_t bar = of_leader(full(st)), dst = s0 + st * STAGE;
         if (rank == 0) mbar_expect_tx(full(st), 2 * STAGE);
 #pragma unroll
-        for (int i = 0; i < 2 * MT; ++i)
-          tma_load_pair(dst + i * 8192, &g.g[seg], m0 + i / 2 * 256 + i % 2 * 64, k * KB, bar);
+        for (int i = 0; i < 2 * MT; ++i) {
+          const int col = m0 + i / 2 * 256 + i % 2 * 64, row = k * KB;
+          // (columns past the last block are those of the next rows, or zeros: sums that nobody reads)
+          if (g.across) tma_load_pair(dst + i * 8192, &g.g[seg], 0, (row / TILE * g.across + col / KB) * TILE + row % TILE, bar);
+          else tma_load_pair(dst + i * 8192, &g.g[seg], col, row, bar);
+        }
 #pragma unroll
         for (int i = 0; i < BN / 128; ++i)
           tma_load_pair(dst + GB + i * 8192, &g.x, n0 + rank * (BN / 2) + 64 * i, k * KB, bar);
@@ -1041,7 +910,8 @@ static bool encode(CUtensorMap* tm, const TcRows& t, int box_r, int box_c = KB) 
   using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
                               const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
                               CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-  const cuuint64_t dims[2] = {(cuuint64_t)t.cols, (cuuint64_t)t.rows}, strides[1] = {(cuuint64_t)t.ld * 2};
+  cuuint64_t dims[2] = {(cuuint64_t)t.cols, (cuuint64_t)t.rows}, strides[1] = {(cuuint64_t)t.ld * 2};
+  if (t.blocks) dims[0] = KB, dims[1] = t.block_bytes() / (KB * 2), strides[0] = KB * 2;
   const cuuint32_t box[2] = {(cuuint32_t)box_c, (cuuint32_t)box_r}, es[2] = {1, 1};
   for (int attempt = 0; attempt < 2; ++attempt) {
     if (((Encode)f)(tm, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(t.p), dims, strides, box, es,
@@ -1128,7 +998,8 @@ static RowsPlan plan_rows(int m_pairs, int N, int kb0, int kb1, int sms) {
   // channels, 44 tiles: 11.6 us, 9.0 us if they travel with the pixels; 128 -> 512, 88 tiles: 9.7 and 6.9; the gate with
   // 64 -> 256 channels, 82 tiles: 18.8 and 20.5 for the block).
   const bool stay = MODE != GATE_BWD && (long long)m_pairs * p.n_tiles > (MODE == GATE ? 1 : 2) * pairs;
-  double best = 0;
+  // (a classifier's many channel tiles seldom divide the pairs: 41 tiles kept by 41 of 74 pairs took 1.7 times as long)
+  double best = MODE == SCORE_SUM || MODE == SCORE_GRAD ? 0.95 : 0;
   for (int group = 1; stay && group <= p.n_tiles; ++group) {
     const int groups = p.n_tiles / group;
     if (p.n_tiles % group || groups > pairs) continue;
@@ -1179,6 +1050,19 @@ static int tile_width(long long pairs, int n, int kb, int sms) {
   }
   return best;
 }
+// The same for a long sum over a classifier's classes: a tile is nothing but its MMAs then, and a last wave that is not full
+// counts in whole.  (Narrow tiles read more of the pixels for each MMA.)
+static int long_tile_width(long long pairs, int n, int sms) {
+  const int all = sms / 2;
+  int best = 64;
+  double least = 1e300;
+  for (int w = 64; w <= 256; w *= 2) {
+    const long long tiles = pairs * ((n + w - 1) / w);
+    const double t = (double)((tiles + all - 1) / all) * (w > 150 ? w : w > 100 ? 1.15 * w : 1.6 * w);
+    if (t < least) least = t, best = w;
+  }
+  return best;
+}
 static int kblocks(int c) { return (c + KB - 1) / KB; }
 
 static GemmArgs base_args(const TcRows& a, const TcRows& y, const bf16* bias, int act) {
@@ -1214,7 +1098,9 @@ int tc_input_grad(const TcRows& g0, const TcRows& w0, const TcRows& g1, const Tc
                   cudaStream_t st) {
   GemmArgs g = base_args(g0, gx, nullptr, MC_ACT_NONE);
   if (g1.p) g.kb[1] = kblocks(g1.cols);
-  const int bn = tile_width(g.m_pairs, gx.cols, g.kb[0] + g.kb[1], sm_total());
+  if (g0.blocks) g.a_across[0] = g0.across();
+  const int bn = g0.blocks ? long_tile_width(g.m_pairs, gx.cols, sm_total())
+                           : tile_width(g.m_pairs, gx.cols, g.kb[0] + g.kb[1], sm_total());
   if (!encode(&g.a[0], g0, TILE) || !encode(&g.b[0], w0, bn / 2)) return MC_ERR_LAUNCH;
   if (gx.ld == 0) g.planes = (bf16*)gx.p, g.pd = PixDiv((uint32_t)gx.S);
   else if (!encode(&g.y[0], gx, TILE)) return MC_ERR_LAUNCH;
@@ -1236,6 +1122,7 @@ int tc_scores_sum(const TcRows& x, const TcRows& w, const bf16* bias, const Scor
 int tc_scores_grad(const TcRows& x, const TcRows& w, const bf16* bias, const Scores& s, const TcRows& gz, cudaStream_t st) {
   GemmArgs g = base_args(x, gz, bias, MC_ACT_NONE);
   g.sc = s;
+  g.y_across = gz.blocks ? gz.across() : 0;
   const int bn = tile_width(g.m_pairs, g.N, g.kb[0], sm_total());
   if (!encode(&g.a[0], x, TILE) || !encode(&g.b[0], w, bn / 2) || !encode(&g.y[0], gz, TILE)) return MC_ERR_LAUNCH;
   return launch_wide<SCORE_GRAD>(g, bn, st);
@@ -1308,6 +1195,7 @@ static int launch_outer(OuterTcArgs& g, const OuterPlan& p, cudaStream_t st) {
 int tc_outer(const TcRows& g0, const TcRows& g1, const TcRows& x, float* part, float* csum, cudaStream_t st) {
   OuterTcArgs g{};
   g.segs = g1.p ? 2 : 1;
+  g.across = g0.blocks ? g0.across() : 0;
   const OuterPlan p = outer_plan(x.rows, g0.cols, g.segs, x.cols, sm_total());
   if (!encode(&g.g[0], g0, KB) || (g1.p && !encode(&g.g[1], g1, KB)) || !encode(&g.x, x, KB)) return MC_ERR_LAUNCH;
   g.part = part, g.csum = csum;
