@@ -23,9 +23,6 @@ int device_status_read(cudaStream_t, int);
 namespace mix {
 int tc_status_read(int);
 }
-namespace norm {
-int status_read(int);
-}
 bool conv_tc_dgrad_supported(const mc_desc*);
 size_t conv_tc_dgrad_ws(const mc_desc*);
 int conv_tc_dgrad_launch(const mc_desc*, const void*, const void*, const void*, const void*, void*,
@@ -92,9 +89,7 @@ const char* mc_strerror(int code) {
 int mc_device_status(void* stream, int reset) {
   // one code per call: a word whose code is not returned is not cleared either
   const int conv = device_status_read((cudaStream_t)stream, reset);
-  if (conv) return conv;
-  const int mixed = mix::tc_status_read(reset);
-  return mixed ? mixed : norm::status_read(reset);
+  return conv ? conv : mix::tc_status_read(reset);
 }
 
 // Layers with padded output channels ask for a workspace and for aligned tensors only to be faster: without
