@@ -528,8 +528,8 @@ int mc_cross_entropy_bwd(const mc_ce_desc* d, const void* grad_loss, const void*
  * take MC_F32 or MC_BF16 gradients.  master (MC_BF16 parameters, may be NULL): float32 values that the step is taken on, p is their
  * rounding.  bits 32: m and v are float32.  bits 8: m int8 and v uint8 codes, m_scale and v_scale one float per 256 consecutive
  * elements; m stands for c |c| m_scale, v for (c^2 v_scale)^2, with m_scale = max|m| / 127^2 and v_scale = max sqrt(v) / 255^2 of the
- * block (zero if below 2^-126) and the nearest codes, ties to even; a v that is not zero has a code that is not zero.  A block
- * with an element that is not finite becomes NaN.  The update uses moments that are not rounded yet.  Nothing written may
+ * block (zero if below 2^-126) and the nearest codes, ties to even; a v that is not zero has a code that is not zero.  In a block
+ * with a moment that is not finite no moment is.  The update uses moments that are not rounded yet.  Nothing written may
  * share memory with another tensor of the call. */
 typedef struct mc_adamw_tensor {
   void* p;

@@ -14,6 +14,7 @@
 // kernel parameters, so nothing is copied to the device.
 #include <math.h>
 
+#include "act_pairs.cuh"
 #include "common.cuh"
 
 namespace mc {
@@ -124,22 +125,34 @@ __device__ __forceinline__ void store_codes(uint8_t* p, int i, int n, bool vec, 
       if (i + j < n) p[i + j] = (uint8_t)(c[j / 4] >> (8 * (j % 4)));
   }
 }
-__device__ __forceinline__ float value_m(uint32_t c, int j, float s) {
-  const int k = (int)(int8_t)(c >> (8 * j));
-  return __fmul_rn((float)(k * abs(k)), s);
+// ---- 8 bits -------------------------------------------------------------------------------------------------
+// (instructions bound this path, not memory: packed float32 pairs, codes taken from and put into the last bits of floats)
+using mix::add2;
+using mix::fma2;
+using mix::mul2;
+using mix::two;
+// Byte j of c as a float, by way of a float whose last bits it is: 2^23 + c, or 2^23 + 128 + c for a signed one.
+__device__ __forceinline__ float byte_of(uint32_t c, int j) { return __uint_as_float(__byte_perm(c, 0x4B000000, 0x7540 + j)); }
+__device__ __forceinline__ float2 pair_of(uint32_t (&c)[2], int j) {
+  return make_float2(byte_of(c[j / 2], 2 * j % 4), byte_of(c[j / 2], 2 * j % 4 + 1));
 }
-__device__ __forceinline__ float value_v(uint32_t c, int j, float s) {
-  const int k = (int)(c >> (8 * j) & 255);
-  const float r = __fmul_rn((float)(k * k), s);
-  return __fmul_rn(r, r);
-}
-// The larger of two magnitudes; NaN if one is.
-__device__ __forceinline__ float larger(float a, float b) { return (b > a || b != b) ? b : a; }
-__device__ __forceinline__ float warp_largest(float a) {
+__device__ __forceinline__ void values_of(uint32_t (&cm)[2], uint32_t (&cv)[2], float s, float q, float2 (&m)[4], float2 (&v)[4]) {
+  uint32_t c[2] = {cm[0] ^ 0x80808080u, cm[1] ^ 0x80808080u};
 #pragma unroll
-  for (int o = 16; o; o >>= 1) a = larger(a, __shfl_xor_sync(~0u, a, o));
-  return a;
+  for (int j = 0; j < 4; ++j) {  // (squares of codes are whole numbers: exact)
+    const float2 k = add2(pair_of(c, j), two(-8388736.f)), l = add2(pair_of(cv, j), two(-8388608.f));
+    m[j] = mul2(make_float2(k.x * fabsf(k.x), k.y * fabsf(k.y)), two(s));
+    const float2 r = mul2(mul2(l, l), two(q));
+    v[j] = mul2(r, r);
+  }
 }
+__device__ __forceinline__ float sqrt_near(float v) {  // within 2^-22 of the root; zero below 2^-126
+  float r;
+  asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+// Largest of magnitudes, as bits: those of NaN are above all others.
+__device__ __forceinline__ uint32_t magnitude(float v) { return __float_as_uint(v) & 0x7FFFFFFFu; }
 // (below 2^-126 the reciprocal of a scale can overflow: such blocks are zero)
 __device__ __forceinline__ float scale_of(float a, float most, float* inverse) {
   float s = __fmul_rn(a, 1.f / most);
@@ -154,6 +167,55 @@ __device__ __forceinline__ float root_of(float a) { return __fsqrt_rn(a); }
 __device__ __forceinline__ double root_of(double a) { return sqrt(a); }
 __device__ __forceinline__ float quotient(float a, float b) { return __fdividef(a, b); }  // (2 ulp; b < 2^126, sqrt(v) ends at 2^64)
 __device__ __forceinline__ double quotient(double a, double b) { return a / b; }
+
+// The codes of a block from its moments, in registers of a warp.
+// Codes are whole numbers nearest to correctly rounded roots of correctly rounded products.  Approximate roots, 2^-21 off with what
+// goes into them, give the same codes but near the middle of two (256 2^-21 < 2e-4), where the exact ones are computed.
+// force: roots in reach of the type's smallest values, or a scale that is not finite.
+constexpr float SIGNED = 12582912.f, PLAIN = 8388608.f;  // 1.5 2^23 + a code, 2^23 + a code: the code is the last bits
+__device__ __forceinline__ void encode(const float2 (&m)[4], const float2 (&v)[4], const float2 (&r)[4], float s, float q, float im,
+                                       float iv, bool force, uint32_t (&cm)[2], uint32_t (&cv)[2]) {
+  const bool some = q > 0.f;
+  float a[8], b[8], least[8];
+  uint32_t ca[8], cb[8];
+  float off = 0.f;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const float2 z = mul2(r[j], two(iv));
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int e = 2 * j + h;
+      const float x = h ? m[j].y : m[j].x;
+      a[e] = copysignf(sqrt_near(fabsf(x) * im), x);
+      b[e] = sqrt_near(h ? z.y : z.x);
+      least[e] = some && (h ? v[j].y : v[j].x) > 0.f ? 1.f : 0.f;  // (a v that is not zero keeps a code that is not zero)
+    }
+    const float2 ta = add2(make_float2(a[2 * j], a[2 * j + 1]), two(SIGNED)), tb = add2(make_float2(b[2 * j], b[2 * j + 1]), two(PLAIN));
+    const float2 ra = add2(ta, two(-SIGNED)), rb = add2(tb, two(-PLAIN));
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int e = 2 * j + h;
+      off = fmaxf(off, fmaxf(fabsf(a[e] - (h ? ra.y : ra.x)), fabsf(b[e] - (h ? rb.y : rb.x))));
+    }
+  }
+  if (__any_sync(~0u, off > 0.4998f) || force) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float x = e & 1 ? m[e / 2].y : m[e / 2].x, y = e & 1 ? v[e / 2].y : v[e / 2].x;
+      if (force || fabsf(a[e] - rintf(a[e])) > 0.4998f) a[e] = copysignf(__fsqrt_rn(__fmul_rn(fabsf(x), im)), x);
+      if (force || fabsf(b[e] - rintf(b[e])) > 0.4998f) b[e] = __fsqrt_rn(__fmul_rn(__fsqrt_rn(y), iv));
+      if (force && !(fabsf(a[e]) < 127.5f)) a[e] = 0.f;  // (a scale that is not finite)
+      if (force && !(b[e] < 255.5f)) b[e] = 0.f;
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < 8; ++e) ca[e] = __float_as_uint(a[e] + SIGNED), cb[e] = __float_as_uint(fmaxf(b[e], least[e]) + PLAIN);
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    cm[h] = __byte_perm(__byte_perm(ca[4 * h], ca[4 * h + 1], 0x0040), __byte_perm(ca[4 * h + 2], ca[4 * h + 3], 0x0040), 0x5410);
+    cv[h] = __byte_perm(__byte_perm(cb[4 * h], cb[4 * h + 1], 0x0040), __byte_perm(cb[4 * h + 2], cb[4 * h + 3], 0x0040), 0x5410);
+  }
+}
 
 // P: the parameters' type, G: the gradients', M: with float32 copies of bf16 parameters, B8: moments in 8 bits
 template <int N, typename P, typename G, bool M, bool B8>
@@ -174,59 +236,64 @@ __global__ void __launch_bounds__(THREADS) step_kernel(const __grid_constant__ T
     const CT rate = (CT)t.rate[k], inv_root = (CT)t.inv_root[k];
     P* p = (P*)t.p[k] + at;
     float* master = (float*)t.master[k] + at;
-    CT g[8], w[8], m[8], v[8];
+    CT g[8], w[8];
     load8((const G*)t.g[k] + at, i, n, vec, g);
     if constexpr (M) load8(master, i, n, vec, w);
     else load8((const P*)p, i, n, vec, w);
-    uint32_t cm[2], cv[2];
-    float* ms = nullptr;
-    float* vs = nullptr;
     if constexpr (B8) {
-      const long long block = (at + i) / BLOCK8;
-      if (i < n) ms = t.ms[k] + block, vs = t.vs[k] + block;
+      uint32_t cm[2], cv[2];
       load_codes((const uint8_t*)t.m[k] + at, i, n, vec, cm);
       load_codes((const uint8_t*)t.v[k] + at, i, n, vec, cv);
-      const float s = ms ? *ms : 0.f, q = vs ? *vs : 0.f;
+      float *ms = nullptr, *vs = nullptr;
+      if (i < n) ms = t.ms[k] + (at + i) / BLOCK8, vs = t.vs[k] + (at + i) / BLOCK8;
+      float2 m[4], v[4], r[4];
+      values_of(cm, cv, ms ? *ms : 0.f, vs ? *vs : 0.f, m, v);
+      uint32_t am = 0, av = 0;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) m[j] = value_m(cm[j / 4], j % 4, s), v[j] = value_v(cv[j / 4], j % 4, q);
-    } else {
-      load8((const CT*)t.m[k] + at, i, n, vec, m);
-      load8((const CT*)t.v[k] + at, i, n, vec, v);
-    }
-    CT r[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      m[j] = add_rn(mul(m[j], b1), mul(g[j], c1));
-      v[j] = add_rn(mul(v[j], b2), mul(mul(g[j], g[j]), c2));
-      r[j] = root_of(v[j]);
-      const CT u = quotient(m[j], r[j] * inv_root + eps);
-      w[j] = w[j] * keep - rate * u;
-    }
-    if constexpr (M) store8(master, i, n, vec, w);
-    store8(p, i, n, vec, w);
-    if constexpr (B8) {
-      float am = 0.f, av = 0.f;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) am = larger(am, fabsf(m[j])), av = larger(av, r[j]);  // (elements behind the end are zeros)
-      float im, iv;
-      const float s = scale_of(warp_largest(am), MOST_M, &im), q = scale_of(warp_largest(av), MOST_V, &iv);
-      cm[0] = cm[1] = cv[0] = cv[1] = 0;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        int a = (int)rintf(__fsqrt_rn(__fmul_rn(fabsf(m[j]), im)));  // (NaN: zero; the scale is NaN)
-        if (a > 127) a = 127;
-        if (m[j] < 0.f) a = -a;
-        cm[j / 4] |= (uint32_t)(a & 255) << (8 * (j % 4));
-        int b = (int)rintf(__fsqrt_rn(__fmul_rn(r[j], iv)));
-        if (b > 255) b = 255;
-        if (b == 0 && r[j] > 0.f && q > 0.f) b = 1;
-        cv[j / 4] |= (uint32_t)b << (8 * (j % 4));
+      for (int j = 0; j < 4; ++j) {
+        // (not in pairs: packed products and sums came out as one operation, a last bit off)
+        m[j].x = add_rn(mul(m[j].x, b1), mul(g[2 * j], c1)), m[j].y = add_rn(mul(m[j].y, b1), mul(g[2 * j + 1], c1));
+        v[j].x = add_rn(mul(v[j].x, b2), mul(mul(g[2 * j], g[2 * j]), c2));
+        v[j].y = add_rn(mul(v[j].y, b2), mul(mul(g[2 * j + 1], g[2 * j + 1]), c2));
+        am = max(am, max(magnitude(m[j].x), magnitude(m[j].y)));  // (elements behind the end are zeros)
+        av = max(av, max(magnitude(v[j].x), magnitude(v[j].y)));
       }
+      av = __reduce_max_sync(~0u, av);
+      // A root of less than 2^-63 counts as zero below, and its code is none either, where the block's largest is 2^-45 or more.
+      const bool small = av < __float_as_uint(0x1p-90f) || eps == 0.f;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        r[j] = small ? make_float2(__fsqrt_rn(v[j].x), __fsqrt_rn(v[j].y)) : make_float2(sqrt_near(v[j].x), sqrt_near(v[j].y));
+        const float2 d = fma2(r[j], two(inv_root), two(eps));
+        float2 u;
+        if (small) u = make_float2(m[j].x / d.x, m[j].y / d.y);
+        else u = mul2(m[j], mix::rcp2(d));
+        const float2 x = fma2(u, two(-rate), mul2(make_float2(w[2 * j], w[2 * j + 1]), two(keep)));
+        w[2 * j] = x.x, w[2 * j + 1] = x.y;
+      }
+      if constexpr (M) store8(master, i, n, vec, w);
+      store8(p, i, n, vec, w);
+      float im, iv;
+      const float s = scale_of(__uint_as_float(__reduce_max_sync(~0u, am)), MOST_M, &im);
+      const float q = scale_of(__fsqrt_rn(__uint_as_float(av)), MOST_V, &iv);  // (roots keep their order)
+      encode(m, v, r, s, q, im, iv, small || !(s < INFINITY) || !(q < INFINITY), cm, cv);
       store_codes((uint8_t*)t.m[k] + at, i, n, vec, cm);
       store_codes((uint8_t*)t.v[k] + at, i, n, vec, cv);
       __syncwarp();  // (every lane has read the old scales)
       if (ms && threadIdx.x % 32 == 0) *ms = s, *vs = q;
     } else {
+      CT m[8], v[8];
+      load8((const CT*)t.m[k] + at, i, n, vec, m);
+      load8((const CT*)t.v[k] + at, i, n, vec, v);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        m[j] = add_rn(mul(m[j], b1), mul(g[j], c1));
+        v[j] = add_rn(mul(v[j], b2), mul(mul(g[j], g[j]), c2));
+        const CT u = quotient(m[j], root_of(v[j]) * inv_root + eps);
+        w[j] = w[j] * keep - rate * u;
+      }
+      if constexpr (M) store8(master, i, n, vec, w);
+      store8(p, i, n, vec, w);
       store8((CT*)t.m[k] + at, i, n, vec, m);
       store8((CT*)t.v[k] + at, i, n, vec, v);
     }
@@ -252,11 +319,15 @@ __global__ void __launch_bounds__(THREADS) values_kernel(const __grid_constant__
     uint32_t cm[2], cv[2];
     load_codes((const uint8_t*)t.m[k] + at, i, n, vec, cm);
     load_codes((const uint8_t*)t.v[k] + at, i, n, vec, cv);
-    float m[8], v[8];
+    float2 m[4], v[4];
+    values_of(cm, cv, s, q, m, v);
+    float o[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) m[j] = value_m(cm[j / 4], j % 4, s), v[j] = value_v(cv[j / 4], j % 4, q);
-    store8((float*)t.p[k] + at, i, n, vec, m);
-    store8((float*)t.master[k] + at, i, n, vec, v);
+    for (int j = 0; j < 4; ++j) o[2 * j] = m[j].x, o[2 * j + 1] = m[j].y;
+    store8((float*)t.p[k] + at, i, n, vec, o);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) o[2 * j] = v[j].x, o[2 * j + 1] = v[j].y;
+    store8((float*)t.master[k] + at, i, n, vec, o);
   }
 }
 

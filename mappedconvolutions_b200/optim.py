@@ -1,6 +1,8 @@
 """Optimisers on the library's kernels.  Not in the reference, which trains with torch's."""
 import torch
 
+from .host import impl
+
 
 class AdamW(torch.optim.Optimizer):
     """torch.optim.AdamW (decoupled weight decay) with one kernel over all parameters of a group.
@@ -45,10 +47,8 @@ class AdamW(torch.optim.Optimizer):
             state["master"] = p.detach().to(torch.float32, copy=True)
         return state
 
-    @torch.no_grad()
     def step(self, closure=None):
         """One step over all parameters that have a gradient; the others, and their step counts, stay as they are."""
-        from .host import impl
         loss = None
         if closure is not None:
             with torch.enable_grad():
@@ -58,31 +58,29 @@ class AdamW(torch.optim.Optimizer):
         for group in self.param_groups:
             by_device = {}
             for p in group["params"]:
-                if p.grad is None:
+                g = p.grad
+                if g is None:
                     continue
-                if p.grad.layout != torch.strided:
-                    raise RuntimeError("AdamW takes dense gradients")
                 state = self.state[p]
                 if not state:
                     state.update(self._new_state(p, group))
-                by_device.setdefault(p.device, []).append((p, state))
-            for members in by_device.values():
-                params, states = zip(*members)
-                steps = [s["step"] + 1 for s in states]
-                column = lambda k: [s.get(k) for s in states]  # noqa: E731
-                impl.adamw_step(list(params), [p.grad for p in params], column("exp_avg"), column("exp_avg_sq"),
-                                column("exp_avg_scale"), column("exp_avg_sq_scale"), column("master"), steps, float(group["lr"]),
-                                float(group["betas"][0]), float(group["betas"][1]), float(group["eps"]),
+                lists = by_device.get(p.device)
+                if lists is None:
+                    lists = by_device[p.device] = ([], [], [], [], [], [], [], [], [])
+                get = state.get
+                for column, value in zip(lists, (p, g, state["exp_avg"], state["exp_avg_sq"], get("exp_avg_scale"),
+                                                 get("exp_avg_sq_scale"), get("master"), state["step"] + 1, state)):
+                    column.append(value)
+            for *lists, states in by_device.values():
+                impl.adamw_step(*lists, float(group["lr"]), float(group["betas"][0]), float(group["betas"][1]), float(group["eps"]),
                                 float(group["weight_decay"]))
-                for s, n in zip(states, steps):
+                for s, n in zip(states, lists[-1]):
                     s["step"] = n
         return loss
 
-    @torch.no_grad()
     def moments(self):
         """(exp_avg, exp_avg_sq) of every parameter that has taken a step, in the groups' order: the state's own tensors, or the
         float32 values that 8-bit codes stand for."""
-        from .host import impl
         states = [self.state[p] for group in self.param_groups for p in group["params"] if self.state.get(p)]
         out = [(s["exp_avg"], s["exp_avg_sq"]) for s in states]
         by_device = {}
