@@ -218,8 +218,9 @@ __device__ __forceinline__ void encode(const float2 (&m)[4], const float2 (&v)[4
 }
 
 // P: the parameters' type, G: the gradients', M: with float32 copies of bf16 parameters, B8: moments in 8 bits
+// (8 bits: 48 warps an SM.  32: 125 us for 33.6 M bf16 parameters instead of 108, 40: 113.)
 template <int N, typename P, typename G, bool M, bool B8>
-__global__ void __launch_bounds__(THREADS) step_kernel(const __grid_constant__ Table<N> t, const Hyper h) {
+__global__ void __launch_bounds__(THREADS, B8 ? 6 : 1) step_kernel(const __grid_constant__ Table<N> t, const Hyper h) {
   typedef typename Traits<P>::CT CT;
   const CT b1 = (CT)h.b1, c1 = (CT)h.c1, b2 = (CT)h.b2, c2 = (CT)h.c2, eps = (CT)h.eps, keep = (CT)h.keep;
   const int total = t.first[t.n];

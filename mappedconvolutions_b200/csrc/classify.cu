@@ -9,8 +9,9 @@
 // bf16 (tensor cores): the scores of 256 pixels x up to 256 classes stand in TMEM; the forward call keeps their largest and the
 // sum of their exponentials, the backward call computes them again, rounds gz to bf16 - which the next two products' operand is -
 // and multiplies it, a piece of the pixels at a time.
-// float32 and float64 (CUDA cores): scores of a piece of the pixels in the workspace, with the kernels of the channel-mixing
-// layers.  Bound: the products.
+// float32 and float64 (CUDA cores), with the kernels of the channel-mixing layers: up to 128 classes stand in a block's registers, whose
+// threads add up the softmax; scores of more classes go through the workspace, a piece of the pixels at a time.  Bound: the
+// products (FMA issue).
 #include "mix_work.cuh"
 
 namespace mc {
@@ -21,7 +22,8 @@ using mix::View;
 // What a forward call keeps: the number of labelled pixels (a double), from byte 256 on lse of every pixel, and behind it the input as
 // rows of channels where it lies in another way (bf16).
 constexpr size_t KEPT_HEAD = 256;
-constexpr size_t PIECE = 48u << 20;      // bytes of scores at a time, CUDA cores (they stay in L2)
+constexpr size_t PIECE = 256u << 20;     // bytes of scores or gz at a time, CUDA cores
+constexpr int FEW = 128;                 // classes that the CUDA-core kernels keep in registers
 constexpr size_t PIECE_TC = 1024u << 20; // bytes of gz at a time, tensor cores
 constexpr int THREADS = 256;
 constexpr int SUM_BLOCKS = 296;          // blocks that add losses up
@@ -38,26 +40,37 @@ __device__ __forceinline__ CT warp_sum(CT v) {
   return v;
 }
 
-// lse and loss of the rows of a piece, one warp to a row
-template <typename CT>
-__global__ void __launch_bounds__(THREADS) lse_kernel(const CT* __restrict__ z, const int64_t* __restrict__ target, long long n,
-                                                      int V, long long ignore, CT* __restrict__ lse, CT* __restrict__ value) {
+template <typename T> struct alignas(16) Four { T v[4]; };
+// lse and loss of the rows of a piece, one warp to a row of ld (a multiple of 4) scores
+template <typename T>
+__global__ void __launch_bounds__(THREADS) lse_kernel(const T* __restrict__ z, int ld, const int64_t* __restrict__ target, long long n,
+                                                      int V, long long ignore, T* __restrict__ lse, T* __restrict__ value) {
   const long long row = blockIdx.x * (long long)(THREADS / 32) + threadIdx.x / 32;
   if (row >= n) return;
   const int lane = threadIdx.x % 32;
   const long long t = target[row];
-  CT out, loss;
+  T out, loss;
   if (t == ignore) {
-    out = CT(INFINITY), loss = CT(0);
+    out = T(INFINITY), loss = T(0);
   } else if (t < 0 || t >= V) {
-    out = loss = CT(NAN);
+    out = loss = T(NAN);
   } else {
-    const CT* r = z + row * V;
-    CT top = -CT(INFINITY), sum = CT(0);
-    for (int v = lane; v < V; v += 32) top = fmax(top, r[v]);  // (a NaN shows in the sum)
+    const T* r = z + row * ld;
+    T top = -T(INFINITY), sum = T(0);
+#pragma unroll 4
+    for (int v = lane * 4; v < V; v += 128) {
+      const Four<T> q = *reinterpret_cast<const Four<T>*>(r + v);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) top = fmax(top, v + e < V ? q.v[e] : -T(INFINITY));  // (a NaN shows in the sum)
+    }
 #pragma unroll
     for (int o = 16; o; o >>= 1) top = fmax(top, __shfl_xor_sync(~0u, top, o));
-    for (int v = lane; v < V; v += 32) sum += exp_of(r[v] - top);
+#pragma unroll 4
+    for (int v = lane * 4; v < V; v += 128) {
+      const Four<T> q = *reinterpret_cast<const Four<T>*>(r + v);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) sum += v + e < V ? exp_of(q.v[e] - top) : T(0);
+    }
     out = top + log_of(warp_sum(sum));
     loss = out - r[t];
   }
@@ -65,24 +78,30 @@ __global__ void __launch_bounds__(THREADS) lse_kernel(const CT* __restrict__ z, 
 }
 
 // z <- gz
-template <typename CT>
-__global__ void __launch_bounds__(THREADS) score_grad_kernel(CT* __restrict__ z, const int64_t* __restrict__ target,
-                                                             const CT* __restrict__ lse, long long n, int V,
-                                                             const double* count, const CT* grad, bool mean) {
-  const CT scale = mean ? (CT)((double)*grad / *count) : *grad;
+template <typename T>
+__global__ void __launch_bounds__(THREADS) score_grad_kernel(T* __restrict__ z, int ld, const int64_t* __restrict__ target,
+                                                             const T* __restrict__ lse, long long n, int V, const double* count,
+                                                             const T* grad) {
+  const T scale = count ? (T)((double)*grad / *count) : *grad;
   for (long long row = blockIdx.x * (long long)(THREADS / 32) + threadIdx.x / 32; row < n; row += gridDim.x * (long long)(THREADS / 32)) {
-    const CT l = lse[row];
+    const T l = lse[row];
     const long long t = target[row];
-    CT* r = z + row * V;
-    for (int v = threadIdx.x % 32; v < V; v += 32)
-      r[v] = l == CT(INFINITY) ? CT(0) : scale * (exp_of(r[v] - l) - (v == t ? CT(1) : CT(0)));
+    T* r = z + row * ld;
+#pragma unroll 2
+    for (int v = threadIdx.x % 32 * 4; v < V; v += 128) {
+      Four<T> q = *reinterpret_cast<const Four<T>*>(r + v);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) q.v[e] = l == T(INFINITY) ? T(0) : scale * (exp_of(q.v[e] - l) - (v + e == t ? T(1) : T(0)));
+      *reinterpret_cast<Four<T>*>(r + v) = q;
+    }
   }
 }
 
-// (pixels, C) wherever they lie -> rows; those of pixels without a label are zero
+// (images of n pixels, C) wherever they lie -> rows; those of pixels without a label are zero
 template <typename T>
-__global__ void __launch_bounds__(THREADS) rows_kernel(const T* __restrict__ src, long long pix, long long ch, long long n, int C,
-                                                       const T* __restrict__ lse, T* __restrict__ dst) {
+__global__ void __launch_bounds__(THREADS) rows_kernel(const T* __restrict__ src, long long img, long long pix, long long ch, long long n,
+                                                       int C, const T* __restrict__ lse, T* __restrict__ dst) {
+  src += blockIdx.z * img, lse += blockIdx.z * n, dst += blockIdx.z * n * C;
   __shared__ T tile[32][33];
   // 32 pixels x 32 channels, read along whichever direction is contiguous
   const int tx = threadIdx.x % 32, ty = threadIdx.x / 32;
@@ -241,7 +260,7 @@ struct Pieces {
   Pieces(const mc_ce_desc* d) {
     const bool whole = d->layout == MC_NHWC || d->S == 1 || d->B == 1;
     S = whole ? d->B * d->S : d->S, B = whole ? 1 : d->B;
-    const size_t row = (size_t)(d->V > d->C ? d->V : d->C) * csize(d->dtype);
+    const size_t row = (size_t)((d->V > d->C ? d->V : d->C) + 3) / 4 * 4 * csize(d->dtype);
     long long n = (long long)(PIECE / row);
     n = n < 32 ? 32 : n / 32 * 32;
     images = n >= S ? n / S : 1;
@@ -281,12 +300,15 @@ struct General {
   Pieces pieces;
   Memory m;
   cudaStream_t st;
-  T *z, *rows, *value, *part, *csum, *acc;
-  double* sums;
+  const bool few;
+  const int ld;  // of a row of scores
+  T *z = nullptr, *rows = nullptr, *value = nullptr, *part = nullptr, *csum = nullptr, *acc = nullptr;
+  double* sums = nullptr;
 
-  General(const mc_ce_desc* desc, void* ws, bool backward, cudaStream_t s) : d(desc), pieces(desc), m(ws), st(s) {
+  General(const mc_ce_desc* desc, void* ws, bool backward, cudaStream_t s)
+      : d(desc), pieces(desc), m(ws), st(s), few(desc->V <= FEW), ld((desc->V + 3) / 4 * 4) {
     const size_t n = pieces.most(), C = d->C, V = d->V;
-    z = (T*)m.take(n * V * sizeof(T));
+    if (backward || !few) z = (T*)m.take(n * ld * sizeof(T));
     if (!backward) {
       value = (T*)m.take((size_t)d->B * d->S * sizeof(T));
       sums = (double*)m.take(SUM_BLOCKS * 16);
@@ -299,7 +321,7 @@ struct General {
       });
       part = (T*)m.take((size_t)splits * V * C * sizeof(T));
       csum = (T*)m.take((size_t)splits * V * sizeof(T));
-      acc = (T*)m.take((V * C + V) * sizeof(T));
+      acc = (T*)m.take((long long)n < d->B * d->S ? (V * C + V) * sizeof(T) : 0);
     }
   }
   // f(image, first pixel of it, pixels in all)
@@ -320,62 +342,74 @@ struct General {
     v.ptr = p + i * v.img + s * v.pix;
     return v;
   }
-  View flat(const T* p, long long n, int C) const { return View{p, n * C, C, 1}; }
+  View flat(const T* p, long long n, int wide) const { return View{p, n * wide, wide, 1}; }
   // labelled pixels of a piece as rows (several images one after the other)
   void gather(const T* x, long long i, long long s, long long n, const T* lse) {
     const long long per = n < pieces.S ? n : pieces.S;
-    const dim3 tiles((unsigned)((per + 31) / 32), (unsigned)((d->C + 31) / 32 < 64 ? (d->C + 31) / 32 : 64));
-    for (long long k = 0; k * per < n; ++k) {
-      const View v = view(x, i + k, s);
-      rows_kernel<T><<<tiles, THREADS, 0, st>>>((const T*)v.ptr, v.pix, v.ch, per, d->C, lse + k * per, rows + k * per * d->C);
-      MC_COUNT(1);
+    const View v = view(x, i, s);
+    for (long long k = 0; k * per < n; k += 32768) {  // (images are the grid's third dimension)
+      const long long images = n / per - k < 32768 ? n / per - k : 32768;
+      const dim3 tiles((unsigned)((per + 31) / 32), (unsigned)((d->C + 31) / 32 < 64 ? (d->C + 31) / 32 : 64), (unsigned)images);
+      rows_kernel<T><<<tiles, THREADS, 0, st>>>((const T*)v.ptr + k * v.img, v.img, v.pix, v.ch, per, d->C, lse + k * per,
+                                                rows + k * per * d->C), MC_COUNT(1);
     }
   }
-  // z = x W^T + b of a piece
-  int scores(const View& x, long long n, long long S, const T* w, const T* b) {
+  // x W^T + b of n pixels
+  RowsArgs product(const View& x, long long n, long long S, const T* w, const T* b) const {
     RowsArgs r{};
-    r.a = x, r.w = w, r.wn = d->C, r.wk = 1, r.bias = b, r.y = View{z, S * (long long)d->V, d->V, 1}, r.P = n, r.S = (int)S, r.N = d->V, r.K = d->C;
-    return mix::simt_rows_launch(d->dtype, mix::EPI_LAYER, r, st);
+    r.a = x, r.w = w, r.wn = d->C, r.wk = 1, r.bias = b, r.y = View{z, S * (long long)ld, ld, 1}, r.P = n, r.S = (int)S, r.N = d->V, r.K = d->C;
+    return r;
   }
 
   int forward(const T* x, const T* w, const T* b, const int64_t* target, T* loss, void* kept) {
     T* lse = (T*)((char*)kept + KEPT_HEAD);
+    const long long P = d->B * d->S;
     int rc = MC_OK;
-    each([&](long long i, long long s, long long n) {
-      if (rc) return;
-      const long long p = i * pieces.S + s;
-      if ((rc = scores(view(x, i, s), n, n < pieces.S ? n : pieces.S, w, b))) return;
-      lse_kernel<T><<<(unsigned)((n + 7) / 8), THREADS, 0, st>>>(z, target + p, n, d->V, d->ignore_index, lse + p, value + p);
-      MC_COUNT(1);
-    });
+    if (few) {
+      RowsArgs r = product(view(x, 0, 0), P, pieces.S, w, b);
+      r.y.ptr = nullptr;
+      r.labels = mix::Labels{target, d->ignore_index, lse, value};
+      rc = mix::simt_rows_launch(d->dtype, mix::EPI_SCORE_SUM, r, st);
+    } else {
+      each([&](long long i, long long s, long long n) {
+        if (rc) return;
+        const long long p = i * pieces.S + s;
+        if ((rc = mix::simt_rows_launch(d->dtype, mix::EPI_LAYER, product(view(x, i, s), n, n < pieces.S ? n : pieces.S, w, b), st))) return;
+        lse_kernel<T><<<(unsigned)((n + 7) / 8), THREADS, 0, st>>>(z, ld, target + p, n, d->V, d->ignore_index, lse + p, value + p);
+        MC_COUNT(1);
+      });
+    }
     if (rc) return rc;
-    const int blocks = grid_for(d->B * d->S, 4 * THREADS, SUM_BLOCKS);
-    loss_part_kernel<T><<<blocks, THREADS, 0, st>>>(value, target, d->B * d->S, d->ignore_index, sums), MC_COUNT(1);
+    const int blocks = grid_for(P, 4 * THREADS, SUM_BLOCKS);
+    loss_part_kernel<T><<<blocks, THREADS, 0, st>>>(value, target, P, d->ignore_index, sums), MC_COUNT(1);
     loss_kernel<T><<<1, THREADS, 0, st>>>(sums, blocks, d->reduction == MC_REDUCE_MEAN, (double*)kept, loss), MC_COUNT(1);
     MC_CHECK_LAUNCH();
     return MC_OK;
   }
 
   int backward(const T* grad, const T* x, const T* w, const T* b, const int64_t* target, const void* kept, T* gx, T* gw, T* gb) {
-    const T* lse = (const T*)((const char*)kept + KEPT_HEAD);
+    T* lse = (T*)((char*)kept + KEPT_HEAD);
+    const double* count = d->reduction == MC_REDUCE_MEAN ? (const double*)kept : nullptr;
     const long long P = d->B * d->S, VC = (long long)d->V * d->C;
     int rc = MC_OK;
     each([&](long long i, long long s, long long n) {
       if (rc) return;
       const long long p = i * pieces.S + s, S = n < pieces.S ? n : pieces.S;
       gather(x, i, s, n, lse + p);
-      if ((rc = scores(flat(rows, n, d->C), n, n, w, b))) return;
-      score_grad_kernel<T><<<grid_for(n, 8, 148 * 8), THREADS, 0, st>>>(z, target + p, lse + p, n, d->V, (const double*)kept, grad,
-                                                                       d->reduction == MC_REDUCE_MEAN), MC_COUNT(1);
+      RowsArgs r = product(flat(rows, n, d->C), n, n, w, b);
+      r.labels = mix::Labels{target + p, d->ignore_index, lse + p, nullptr, grad, count};
+      if ((rc = mix::simt_rows_launch(d->dtype, few ? mix::EPI_SCORE_GRAD : mix::EPI_LAYER, r, st))) return;
+      if (!few)
+        score_grad_kernel<T><<<grid_for(n, 8, 148 * 8), THREADS, 0, st>>>(z, ld, target + p, lse + p, n, d->V, count, grad), MC_COUNT(1);
       if (gx) {
-        RowsArgs r{};
-        r.a = View{z, S * (long long)d->V, d->V, 1}, r.w = w, r.wn = 1, r.wk = d->C, r.P = n, r.N = d->C, r.K = d->V, r.S = (int)S;
+        r = RowsArgs{};
+        r.a = View{z, S * (long long)ld, ld, 1}, r.w = w, r.wn = 1, r.wk = d->C, r.P = n, r.N = d->C, r.K = d->V, r.S = (int)S;
         r.y = view(gx, i, s);
         if ((rc = mix::simt_rows_launch(d->dtype, mix::EPI_LAYER, r, st))) return;
       }
       if (gw || gb) {
         const Shares sh(n, d->V, d->C);
-        const mix::OuterArgs o{flat(z, n, d->V), flat(rows, n, d->C), part, csum, n, sh.share, d->V, d->C, 1, 1, sh.splits, sh.splits};
+        const mix::OuterArgs o{flat(z, n, ld), flat(rows, n, d->C), part, csum, n, sh.share, d->V, d->C, 1, 1, sh.splits, sh.splits};
         if ((rc = mix::simt_outer_launch(d->dtype, o, st))) return;
         const bool first = p == 0, last = p + n == P;
         if (first && last) {

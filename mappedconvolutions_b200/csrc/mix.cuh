@@ -145,7 +145,18 @@ __device__ __noinline__ ActBoth<CT, W> act_both_call(int act, Values<CT, W> z) {
 enum Epilogue {
   EPI_LAYER = 0,  // z = acc + bias; y = act(z) + res; z kept where z.ptr is set
   EPI_GATE = 1,   // two sums per output, rows n and N + n of w: g, u; y = h = act(g) u; z = [g|u] kept
-  EPI_GATE_BWD = 2  // acc = gh; g, u read from res (= [g|u]); y = [gh u act'(g) | gh act(g)]
+  EPI_GATE_BWD = 2,  // acc = gh; g, u read from res (= [g|u]); y = [gh u act'(g) | gh act(g)]
+  // a classifier of up to 128 classes, z = acc + bias (see Labels):
+  EPI_SCORE_SUM = 3,  // log-sum-exp and loss of every pixel
+  EPI_SCORE_GRAD = 4  // y = scale (exp(z - lse) - [label])
+};
+// Labels of the pixels.  lse: +infinity where there is none, NaN where it is no class.  scale: grad, or grad / count where mean is set.
+struct Labels {
+  const int64_t* target;
+  long long ignore;
+  void *lse, *value;
+  const void* grad;
+  const double* count;
 };
 struct RowsArgs {
   View a;
@@ -155,6 +166,7 @@ struct RowsArgs {
   View res, y, z;  // ptr == nullptr: absent
   long long P;
   int S, N, K, act;
+  Labels labels;
 };
 int simt_rows_launch(int dtype, Epilogue epi, const RowsArgs& a, cudaStream_t st);
 

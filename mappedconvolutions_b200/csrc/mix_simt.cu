@@ -151,6 +151,76 @@ struct RowsFlags {
   bool vec_y, vec_z, vec_r;  // runs of y, z, res are aligned (see aligned_runs)
 };
 
+__device__ __forceinline__ float log_(float v) { return logf(v); }
+__device__ __forceinline__ double log_(double v) { return log(v); }
+// Rows of class scores, all classes of a pixel among sixteen neighbouring threads.
+template <typename T, int EPI, int TN>
+__device__ __forceinline__ void score_rows(const RowsArgs& a, const T (&acc)[8][TN / 16], long long p0, int pixels, int classes,
+                                           int tp, int tc, bool vec) {
+  constexpr int W = TN / 32;
+  const T* bias = (const T*)a.bias;
+  T scale = T(0);
+  if (EPI == EPI_SCORE_GRAD) {
+    scale = *(const T*)a.labels.grad;
+    if (a.labels.count) scale = (T)((double)scale / *a.labels.count);
+  }
+#pragma unroll 1
+  for (int q = 0; q < 2; ++q) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int r = q * 64 + 4 * tp + k;
+      const bool in = r < pixels;
+      const long long p = p0 + (in ? r : 0), t = a.labels.target[p];
+      T z[2 * W];
+#pragma unroll
+      for (int j = 0; j < 2 * W; ++j) {
+        const int n = j / W * (TN / 2) + W * tc + j % W;
+        const T v = q ? acc[4 + k][j] : acc[k][j];
+        z[j] = n < classes ? v + (bias ? bias[n] : T(0)) : -T(INFINITY);
+      }
+      if (EPI == EPI_SCORE_SUM) {
+        T top = z[0], sum = T(0), hit = T(0);
+#pragma unroll
+        for (int j = 1; j < 2 * W; ++j) top = fmax(top, z[j]);  // (a NaN shows in the sum)
+#pragma unroll
+        for (int o = 8; o; o >>= 1) top = fmax(top, __shfl_xor_sync(~0u, top, o));
+#pragma unroll
+        for (int j = 0; j < 2 * W; ++j) {
+          const int n = j / W * (TN / 2) + W * tc + j % W;
+          sum += exp_(z[j] - top);
+          if (n == t) hit = z[j];
+        }
+#pragma unroll
+        for (int o = 8; o; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o), hit += __shfl_xor_sync(~0u, hit, o);
+        if (in && tc == 0) {
+          const bool none = t == a.labels.ignore, bad = !none && (t < 0 || t >= classes);
+          const T lse = none ? T(INFINITY) : bad ? T(NAN) : top + log_(sum);
+          ((T*)a.labels.lse)[p] = lse;
+          ((T*)a.labels.value)[p] = none ? T(0) : lse - hit;
+        }
+      } else {
+        const T lse = ((const T*)a.labels.lse)[p];
+#pragma unroll
+        for (int j = 0; j < 2 * W; ++j) {
+          const int n = j / W * (TN / 2) + W * tc + j % W;
+          z[j] = lse == T(INFINITY) ? T(0) : scale * (exp_(z[j] - lse) - (n == t ? T(1) : T(0)));
+        }
+        if (in) {
+          T* y = (T*)a.y.ptr + p * a.y.pix;
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int n = TN / 2 * h + W * tc;
+            T o[W];
+#pragma unroll
+            for (int e = 0; e < W; ++e) o[e] = z[W * h + e];
+            if (n < classes) store_run(y + n, 1, o, classes - n, vec);
+          }
+        }
+      }
+    }
+  }
+}
+
 // PIX: consecutive threads hold consecutive pixels (outputs in NCHW) instead of channels.
 template <typename T, int EPI, int TN, bool PIX>
 __global__ void __launch_bounds__(256, sizeof(T) == 4 ? 2 : 1) rows_kernel(const RowsArgs a, const PixDiv pd, const RowsFlags f) {
@@ -245,6 +315,10 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 ? 2 : 1) rows_kernel(const
         }
       }
     }
+    return;
+  }
+  if constexpr (EPI == EPI_SCORE_SUM || EPI == EPI_SCORE_GRAD) {
+    score_rows<T, EPI, TN>(a, acc, p0, pixels, channels, tp, tc, f.vec_y);
     return;
   }
 #pragma unroll
@@ -394,7 +468,7 @@ static int rows_go(const RowsArgs& a, cudaStream_t st) {
   const int wide = EPI == EPI_GATE ? TN / 2 : TN, W = TN / 32;
   const dim3 grid((unsigned)((a.P + TM - 1) / TM), (unsigned)((a.N + wide - 1) / wide));
   // runs: four pixels of an image that starts anywhere, or W channels (gate: of both halves of 2 N)
-  const long long other = PIX ? a.S : EPI == EPI_LAYER ? 0 : a.N;
+  const long long other = PIX ? a.S : EPI == EPI_GATE || EPI == EPI_GATE_BWD ? a.N : 0;
   const RowsFlags f{a.a.ch == 1, a.wk == 1, aligned_runs<T>(a.y, PIX ? 4 : W, PIX, other),
                     aligned_runs<T>(a.z, PIX ? 4 : W, PIX, other), aligned_runs<T>(a.res, PIX ? 4 : W, PIX, other)};
   if (!opt_in(rows_kernel<T, EPI, TN, PIX>, smem)) return MC_ERR_LAUNCH;
@@ -417,6 +491,8 @@ static int rows_typed(Epilogue epi, const RowsArgs& a, cudaStream_t st) {
     case EPI_LAYER:
       return a.y.pix == 1 && a.y.ch != 1 ? rows_width<T, EPI_LAYER, true>(a, st) : rows_width<T, EPI_LAYER, false>(a, st);
     case EPI_GATE: return rows_width<T, EPI_GATE, false>(a, st);
+    case EPI_SCORE_SUM: return rows_width<T, EPI_SCORE_SUM, false>(a, st);
+    case EPI_SCORE_GRAD: return rows_width<T, EPI_SCORE_GRAD, false>(a, st);
     default: return rows_width<T, EPI_GATE_BWD, false>(a, st);
   }
 }
