@@ -33,6 +33,27 @@ __device__ __forceinline__ double exp_of(double v) { return exp(v); }
 __device__ __forceinline__ float log_of(float v) { return logf(v); }
 __device__ __forceinline__ double log_of(double v) { return log(v); }
 
+// The kernels that this is called in start while the one before them runs; here they wait until all that it wrote can be read.
+__device__ __forceinline__ void behind_previous_kernel() {
+  asm volatile("griddepcontrol.launch_dependents;");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+template <typename... A>
+static int launch_behind(void (*kern)(A...), int blocks, cudaStream_t st, A... args) {
+  cudaLaunchAttribute attr = {};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(blocks);
+  cfg.blockDim = dim3(THREADS);
+  cfg.stream = st;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  if (cudaLaunchKernelEx(&cfg, kern, args...) != cudaSuccess) return MC_ERR_LAUNCH;
+  MC_COUNT(1);
+  return MC_OK;
+}
+
 template <typename CT>
 __device__ __forceinline__ CT warp_sum(CT v) {
 #pragma unroll
@@ -147,6 +168,7 @@ __global__ void __launch_bounds__(THREADS) loss_part_kernel(const CT* __restrict
 template <typename CT>
 __global__ void __launch_bounds__(THREADS) loss_kernel(const double* part, int blocks, bool mean, double* count, CT* loss) {
   __shared__ double sm[2][THREADS / 32];
+  behind_previous_kernel();
   double s = 0, n = 0;
   for (int i = threadIdx.x; i < blocks; i += THREADS) s += part[2 * i], n += part[2 * i + 1];
   s = warp_sum(s), n = warp_sum(n);
@@ -160,9 +182,9 @@ __global__ void __launch_bounds__(THREADS) loss_kernel(const double* part, int b
 }
 // ---- bf16 -----------------------------------------------------------------------------------------------
 // The tiles' sums of a pixel become its lse; the blocks' losses and labelled pixels go to `part`.
-__global__ void __launch_bounds__(THREADS) finish_kernel(const mix::Scores s, int tiles, long long P, int V, float* __restrict__ lse,
-                                                         double* part) {
+__global__ void __launch_bounds__(THREADS) finish_kernel(mix::Scores s, int tiles, long long P, int V, float* lse, double* part) {
   __shared__ double sm[2][THREADS / 32];
+  behind_previous_kernel();
   double sum = 0, n = 0;
   for (long long p = blockIdx.x * (long long)THREADS + threadIdx.x; p < P; p += gridDim.x * (long long)THREADS) {
     const long long t = s.target[p];
@@ -382,9 +404,8 @@ struct General {
     if (rc) return rc;
     const int blocks = grid_for(P, 4 * THREADS, SUM_BLOCKS);
     loss_part_kernel<T><<<blocks, THREADS, 0, st>>>(value, target, P, d->ignore_index, sums), MC_COUNT(1);
-    loss_kernel<T><<<1, THREADS, 0, st>>>(sums, blocks, d->reduction == MC_REDUCE_MEAN, (double*)kept, loss), MC_COUNT(1);
     MC_CHECK_LAUNCH();
-    return MC_OK;
+    return launch_behind(loss_kernel<T>, 1, st, (const double*)sums, (int)blocks, d->reduction == MC_REDUCE_MEAN, (double*)kept, (T*)loss);
   }
 
   int backward(const T* grad, const T* x, const T* w, const T* b, const int64_t* target, const void* kept, T* gx, T* gw, T* gb) {
@@ -451,8 +472,8 @@ struct TensorCores {
     mix::TcRows xr = rows_of(x, pixels());
     if (!in_place()) {
       xr.p = kept ? kept + KEPT_HEAD + lse_bytes() : nullptr;
-      k.lay_out(&like, x, xr);
-      if (k.run()) labelled(xr.p, xr, target, k.st);
+      k.lay_out(&like, x, xr, target, d->ignore_index);
+      if (k.run() && !mix::Work::as_planes(&like, d->C)) labelled(xr.p, xr, target, k.st);
     }
     const mix::TcRows wr = k.weight(w, d->V, d->C);
     const int tiles = mix::tc_scores_tiles(pixels(), d->C, d->V);
@@ -464,10 +485,11 @@ struct TensorCores {
     k.did(mix::tc_scores_sum(xr, wr, bias, s, k.st));
     if (k.rc) return k.rc;
     const int blocks = grid_for(pixels(), THREADS, SUM_BLOCKS);
-    finish_kernel<<<blocks, THREADS, 0, k.st>>>(s, tiles, pixels(), d->V, (float*)(kept + KEPT_HEAD), part), MC_COUNT(1);
-    loss_kernel<float><<<1, THREADS, 0, k.st>>>(part, blocks, d->reduction == MC_REDUCE_MEAN, (double*)kept, loss), MC_COUNT(1);
-    MC_CHECK_LAUNCH();
-    return MC_OK;
+    k.did(launch_behind(finish_kernel, blocks, k.st, (mix::Scores)s, (int)tiles, (long long)pixels(), (int)d->V,
+                        (float*)(kept + KEPT_HEAD), (double*)part));
+    if (k.rc) return k.rc;
+    return launch_behind(loss_kernel<float>, 1, k.st, (const double*)part, (int)blocks, d->reduction == MC_REDUCE_MEAN, (double*)kept,
+                         (float*)loss);
   }
 
   // Pixels of a piece: whole images, or part of one.

@@ -425,6 +425,16 @@ __device__ __forceinline__ void read_scores(const GemmArgs& g, int set, uint32_t
   float scale = 0.f;
   if (MODE == SCORE_GRAD) scale = g.sc.count ? (float)((double)*g.sc.grad / *g.sc.count) : *g.sc.grad;
   uint32_t it = 0, i = 0;
+  // labels and log-sum-exps of a tile are fetched a tile ahead
+  long long t_next = 0;
+  float l_next = INFINITY;
+  const auto fetch_pixel = [&](const TileWalk& w) {
+    const uint32_t p = (w.m() * 2 + rank) * TILE + row;
+    if (!w.more() || p >= (uint32_t)g.rows) return;
+    t_next = __ldg((const long long*)g.sc.target + p);
+    if (MODE == SCORE_GRAD) l_next = __ldg(g.sc.lse + p);
+  };
+  fetch_pixel(TileWalk(g, set, 2));
   for (TileWalk w(g, set, 2); w.more(); w.next(), ++it) {
     float* bs = bias_s + set * 512 + (g.group == 1 ? 0 : (it & 1) * 256);
     const int n0 = w.nt() * BN;
@@ -444,10 +454,13 @@ __device__ __forceinline__ void read_scores(const GemmArgs& g, int set, uint32_t
     int label = -1;  // of this tile's columns
     float lse2 = INFINITY;
     if (in) {
-      const long long t = __ldg((const long long*)g.sc.target + p);
+      const long long t = t_next;
       if (t >= n0 && t < n0 + BN && t < g.N && t != g.sc.ignore) label = (int)(t - n0);
-      if (MODE == SCORE_GRAD) lse2 = __ldg(g.sc.lse + p) * LOG2E;
+      if (MODE == SCORE_GRAD) lse2 = l_next * LOG2E;
     }
+    TileWalk ahead = w;
+    ahead.next();
+    fetch_pixel(ahead);
     const bool dead = lse2 == INFINITY;
     int live = (g.N - n0 + 15) / 16;  // pieces with classes; a staged tile is filled up with zeros
     if (MODE == SCORE_GRAD) live = (live + PER - 1) / PER * PER;

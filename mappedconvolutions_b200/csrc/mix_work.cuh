@@ -133,9 +133,11 @@ static int copy_rows(const void* src, void* dst, long long R, int from, int to, 
 // memory.  The planes are read value by value, neighbouring threads at neighbouring pixels, because with an
 // odd number of pixels they start anywhere; sixteen values per thread are on their way at once.  64 channels of
 // 8 x 125 x 251 pixels to rows: 35 us with the general transpose.
+// Pixels whose label is `ignore` become rows of zeros (target: null if there are none).
 template <int CT>
 __global__ void __launch_bounds__(256) planes_to_rows_kernel(const bf16* __restrict__ src, bf16* __restrict__ dst,
-                                                             long long S, int C, int ld, int tiles_s, int tiles_c) {
+                                                             long long S, int C, int ld, int tiles_s, int tiles_c,
+                                                             const int64_t* __restrict__ target, long long ignore) {
   constexpr int PX = 4096 / CT, PITCH = CT + 2;
   __shared__ __align__(16) bf16 tile[PX * PITCH];
   const int tc = blockIdx.x % tiles_c, ts = blockIdx.x / tiles_c % tiles_s, c0 = tc * CT;
@@ -146,8 +148,9 @@ __global__ void __launch_bounds__(256) planes_to_rows_kernel(const bf16* __restr
 #pragma unroll
   for (int i = 0; i < 16; ++i)
     v[i] = s0 + s < S && c0 + c + i * (256 / PX) < C ? __ldcs(from + (long long)i * (256 / PX) * S) : bf16(0.f);
+  const bool off = target && s0 + s < S && target[b * S + s0 + s] == ignore;
 #pragma unroll
-  for (int i = 0; i < 16; ++i) tile[s * PITCH + c + i * (256 / PX)] = v[i];
+  for (int i = 0; i < 16; ++i) tile[s * PITCH + c + i * (256 / PX)] = off ? bf16(0.f) : v[i];
   __syncthreads();
 #pragma unroll
   for (int i = threadIdx.x; i < 512; i += 256) {
@@ -182,14 +185,15 @@ struct Work {
     lay_out(d, p, r);
     return r;
   }
-  void lay_out(const mc_mix_desc* d, const void* p, const TcRows& r) {
+  // (a label `ignore` makes zeros of its pixel's row; rows that are planes no more only)
+  void lay_out(const mc_mix_desc* d, const void* p, const TcRows& r, const int64_t* target = nullptr, long long ignore = 0) {
     if (!run()) return;
     const int C = r.cols;
     if (d->layout == MC_NHWC || d->S == 1 || C == 1) {
       did(copy_rows(p, (void*)r.p, r.rows, C, r.ld, st));
     } else {
       planes(d, C, [&](auto ct, unsigned blocks, int ts, int tc) {
-        planes_to_rows_kernel<decltype(ct)::value><<<blocks, 256, 0, st>>>((const bf16*)p, (bf16*)r.p, d->S, C, r.ld, ts, tc);
+        planes_to_rows_kernel<decltype(ct)::value><<<blocks, 256, 0, st>>>((const bf16*)p, (bf16*)r.p, d->S, C, r.ld, ts, tc, target, ignore);
       });
     }
   }
