@@ -476,20 +476,33 @@ struct TensorCores {
       if (k.run() && !mix::Work::as_planes(&like, d->C)) labelled(xr.p, xr, target, k.st);
     }
     const mix::TcRows wr = k.weight(w, d->V, d->C);
-    const int tiles = mix::tc_scores_tiles(pixels(), d->C, d->V);
+    // (the tiles' sums of very many scores: a piece of the pixels at a time)
+    const long long P = pixels(), piece = sum_piece(), last = (P - 1) % piece + 1, pieces = (P + piece - 1) / piece;
+    const auto tiles = [&](long long n) { return mix::tc_scores_tiles(n, d->C, d->V); };
+    const size_t one = (size_t)tiles(piece) * piece, other = (size_t)tiles(last) * last;
     mix::Scores s{target, d->ignore_index};
-    s.part = (float2*)k.take((size_t)tiles * pixels() * 8);
-    s.hit = (float*)k.take((size_t)pixels() * 4);
-    double* part = (double*)k.take(SUM_BLOCKS * 16);
+    s.part = (float2*)k.take((one > other ? one : other) * 8);
+    s.hit = (float*)k.take((size_t)piece * 4);
+    double* part = (double*)k.take((size_t)pieces * SUM_BLOCKS * 16);
     if (!k.run()) return k.rc;
-    k.did(mix::tc_scores_sum(xr, wr, bias, s, k.st));
-    if (k.rc) return k.rc;
-    const int blocks = grid_for(pixels(), THREADS, SUM_BLOCKS);
-    k.did(launch_behind(finish_kernel, blocks, k.st, (mix::Scores)s, (int)tiles, (long long)pixels(), (int)d->V,
-                        (float*)(kept + KEPT_HEAD), (double*)part));
-    if (k.rc) return k.rc;
+    int blocks = 0;
+    for (long long p = 0; p < P; p += piece) {
+      const long long n = P - p < piece ? P - p : piece;
+      s.target = target + p;
+      k.did(mix::tc_scores_sum(rows_of((const bf16*)xr.p + p * xr.ld, n), wr, bias, s, k.st));
+      if (k.rc) return k.rc;
+      const int more = grid_for(n, THREADS, SUM_BLOCKS);
+      k.did(launch_behind(finish_kernel, more, k.st, (mix::Scores)s, (int)tiles(n), (long long)n, (int)d->V,
+                          (float*)(kept + KEPT_HEAD) + p, (double*)(part + 2 * blocks)));
+      if (k.rc) return k.rc;
+      blocks += more;
+    }
     return launch_behind(loss_kernel<float>, 1, k.st, (const double*)part, (int)blocks, d->reduction == MC_REDUCE_MEAN, (double*)kept,
                          (float*)loss);
+  }
+  long long sum_piece() const {
+    const long long most = (long long)(PIECE_TC / 8) / ((d->V + 63) / 64) / 256 * 256;  // (tiles are 64 classes wide at least)
+    return most >= pixels() ? pixels() : most < 256 ? 256 : most;
   }
 
   // Pixels of a piece: whole images, or part of one.

@@ -30,6 +30,12 @@ class AdamW(torch.optim.Optimizer):
         super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay, state_bits=state_bits,
                                       master_weights=bool(master_weights)))
 
+    def __setstate__(self, state):
+        super().__setstate__(state)
+        for group in self.param_groups:  # (of a torch.optim.AdamW, say)
+            group.setdefault("state_bits", 32)
+            group.setdefault("master_weights", False)
+
     @staticmethod
     def _new_state(p, group):
         state = {"step": 0}
@@ -69,7 +75,7 @@ class AdamW(torch.optim.Optimizer):
                     lists = by_device[p.device] = ([], [], [], [], [], [], [], [], [])
                 get = state.get
                 for column, value in zip(lists, (p, g, state["exp_avg"], state["exp_avg_sq"], get("exp_avg_scale"),
-                                                 get("exp_avg_sq_scale"), get("master"), state["step"] + 1, state)):
+                                                 get("exp_avg_sq_scale"), get("master"), int(state["step"]) + 1, state)):
                     column.append(value)
             for *lists, states in by_device.values():
                 impl.adamw_step(*lists, float(group["lr"]), float(group["betas"][0]), float(group["betas"][1]), float(group["eps"]),

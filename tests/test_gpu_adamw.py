@@ -284,6 +284,26 @@ def test_state_dict(bits, master):
         assert x.dtype == F32 and torch.equal(x, y)
 
 
+def test_state_of_torch():
+    """a checkpoint of torch.optim.AdamW goes on as float32 moments"""
+    gen = torch.Generator("cuda").manual_seed(2)
+    mine, theirs = (torch.nn.Parameter(torch.ones(50, 7, device="cuda")) for _ in range(2))
+    a, b = AdamW([mine], lr=0.1), torch.optim.AdamW([theirs], lr=1e-2, weight_decay=0.3)
+    for k in range(6):
+        theirs.grad = torch.randn(50, 7, generator=gen, device="cuda")
+        if k == 3:
+            with torch.no_grad():
+                mine.copy_(theirs)
+            a.load_state_dict(copy.deepcopy(b.state_dict()))
+            assert a.param_groups[0]["lr"] == 1e-2 and a.param_groups[0]["state_bits"] == 32
+        b.step()
+        if k >= 3:
+            mine.grad = theirs.grad
+            a.step()
+    assert a.state[mine]["step"] == 6
+    assert ((mine - theirs).abs() <= 3 * 2.0 ** -20 * (theirs.abs() + 0.02)).all()  # three updates, some roundings each
+
+
 def test_capture_is_refused():
     p = torch.nn.Parameter(torch.ones(10, device="cuda"))
     p.grad = torch.ones(10, device="cuda")

@@ -84,6 +84,39 @@ def test_several_pieces(ops, pixels, classes, dtype):
     R.check(dict(loss=loss, **got), R.cross_entropy(x, weight, bias, target, -100, True, grad), "pieces")
 
 
+@pytest.mark.parametrize("batch,height,width,classes,dtype", [
+    (3, 1, 90_000, 2562, BF),   # bf16: score gradients of more than one piece, whole images and part of one
+    (1, 1, 250_000, 2562, BF),
+    (2, 1, 300_000, 130, F32),  # float32: scores of more than one piece
+    (3, 1, 200_000, 100, F32)])
+@pytest.mark.parametrize("layout", ["nhwc", "nchw"])
+def test_more_than_the_workspace_holds(ops, layout, batch, height, width, classes, dtype):
+    """bf16: a gigabyte of score gradients at a time; float32: a quarter of one.  Checked against the same call in parts."""
+    g = torch.Generator("cuda").manual_seed(31)
+    x = image(g, (batch, 8, height, width), dtype, layout)
+    weight, bias = classifier(g, classes, 8, dtype)
+    target = labels(g, (batch, height, width), classes, 0.1)
+    grad = torch.tensor(1.0, device="cuda")
+    loss, saved = ops.cross_entropy_forward(x, weight, bias, target, -100, False)
+    gx, gw, gb = ops.cross_entropy_backward(grad, saved, x, weight, bias, target, -100, False)
+    total, w_sum, b_sum, u = 0.0, 0.0, 0.0, torch.finfo(dtype).eps / 2
+    for i in range(batch):
+        for k in range(0, width, 30_000):
+            part = x[i:i + 1, :, :, k:k + 30_000]
+            part = part.contiguous(memory_format=torch.channels_last) if layout == "nhwc" else part.contiguous()
+            some = target[i:i + 1, :, k:k + 30_000].contiguous()
+            one, kept = ops.cross_entropy_forward(part, weight, bias, some, -100, False)
+            px, pw, pb = ops.cross_entropy_backward(grad, kept, part, weight, bias, some, -100, False)
+            # (tiles of another width: other orders of the sums)
+            assert (gx[i:i + 1, :, :, k:k + 30_000].double() - px).norm() <= 2 * u * px.double().norm()
+            total, w_sum, b_sum = total + one.double(), w_sum + pw.double(), b_sum + pb.double()
+    n = batch * ((width + 29_999) // 30_000)
+    assert abs(loss.item() - total.item()) <= (n + 1) * 2.0 ** -24 * total.item()
+    # the parts' sums are rounded n times, the whole once; their elements do not cancel more than the parts' sizes say
+    for whole, parts in ((gw, w_sum), (gb, b_sum)):
+        assert (whole.double() - parts).norm() <= (n ** 0.5 + 1) * 2 * u * parts.norm() + 2.0 ** -18 * parts.norm()
+
+
 @pytest.mark.parametrize("layout", ["nhwc", "nchw"])
 @pytest.mark.parametrize("dtype", [BF, F32, F64], ids=["bf16", "f32", "f64"])
 @pytest.mark.parametrize("cin", [40, 64, 300])
