@@ -23,6 +23,7 @@ using mix::View;
 // rows of channels where it lies in another way (bf16).
 constexpr size_t KEPT_HEAD = 256;
 constexpr size_t PIECE = 256u << 20;     // bytes of scores or gz at a time, CUDA cores
+constexpr double FLOATS_FROM = 1e8;      // products from which float32 layers take the tensor cores
 constexpr int FEW = 128;                 // classes that the CUDA-core kernels keep in registers
 constexpr size_t PIECE_TC = 1024u << 20; // bytes of gz at a time, tensor cores
 constexpr int THREADS = 256;
@@ -228,11 +229,50 @@ __global__ void __launch_bounds__(THREADS) labelled_rows_kernel(const uint4* src
     else if (src != dst) dst[i] = __ldg(src + i);
   }
 }
+// n pixels of images of S pixels, wherever they lie -> rows of three bf16 parts of float32 values, 8 bits each, zeros behind the last
+// channel of a part of Cp; pixels without a label are zeros if lse is given.  (An infinity would leave NaN in the lower parts: they
+// are zero there.)
+__global__ void __launch_bounds__(THREADS) parts_kernel(const float* __restrict__ src, long long S, long long img, long long pix,
+                                                        long long ch, long long p1, long long n, int C, int Cp,
+                                                        const float* __restrict__ lse, bf16* __restrict__ dst) {
+  __shared__ float tile[32][33];
+  // 32 pixels x 32 channels, read along whichever direction is contiguous
+  const int tx = threadIdx.x % 32, ty = threadIdx.x / 32;
+  const long long p0 = blockIdx.x * 32ll;
+  for (int c0 = blockIdx.y * 32; c0 < Cp; c0 += gridDim.y * 32) {
+    __syncthreads();
+    for (int k = ty; k < 32; k += THREADS / 32) {
+      const int r = ch == 1 ? k : tx, c = c0 + (ch == 1 ? tx : k);
+      const long long p = p0 + r;
+      float v = 0.f;
+      if (p < n && c < C && !(lse && lse[p] == INFINITY)) {
+        const long long b = (p1 + p) / S;
+        v = __ldg(src + b * img + (p1 + p - b * S) * pix + (long long)c * ch);
+      }
+      tile[r][ch == 1 ? tx : k] = v;
+    }
+    __syncthreads();
+    for (int k = ty; k < 32; k += THREADS / 32) {
+      if (p0 + k >= n || c0 + tx >= Cp) continue;
+      bf16* to = dst + (p0 + k) * 3 * Cp + c0 + tx;
+      float v = tile[k][tx];
+#pragma unroll
+      for (int part = 0; part < 3; ++part) {
+        const bf16 h = __float2bfloat16_rn(v);
+        to[part * Cp] = h;
+        const float f = __bfloat162float(h);
+        v = fabsf(f) < INFINITY ? v - f : 0.f;
+      }
+    }
+  }
+}
+
 // acc (+)= the shares of one piece, in order: sums (V, C) in rows of ldn (a multiple of 4), and V column sums; the last piece's
 // go to gw and gb, rounded.  Four sums to a thread.
+template <typename T>
 __global__ void __launch_bounds__(THREADS) add_piece_kernel(const float* __restrict__ part, const float* __restrict__ csum, int splits,
                                                             int V, int C, int ldn, float* __restrict__ acc, bool first, bool last,
-                                                            bf16* gw, bf16* gb) {
+                                                            T* gw, T* gb) {
   const long long nw = (long long)V * (ldn / 4), i = blockIdx.x * (long long)THREADS + threadIdx.x;
   if (i < nw) {
     float4 s = first ? make_float4(0.f, 0.f, 0.f, 0.f) : reinterpret_cast<const float4*>(acc)[i];
@@ -580,7 +620,123 @@ struct TensorCores {
         if (k.rc) return;
         // (many shares of few sums: several threads for each)
         if (splits >= 64 && p == 0 && n == P) mix::add_shares<bf16, float>(part, d->V, d->C, ldn, gw, csum, gb, splits, k.st);
-        else add_piece_kernel<<<(unsigned)((sums_all + THREADS - 1) / THREADS), THREADS, 0, k.st>>>(
+        else add_piece_kernel<bf16><<<(unsigned)((sums_all + THREADS - 1) / THREADS), THREADS, 0, k.st>>>(
+            part, csum, splits, d->V, d->C, ldn, acc, p == 0, p + n == P, gw, gb), MC_COUNT(1);
+        k.did(cudaGetLastError() == cudaSuccess ? MC_OK : MC_ERR_LAUNCH);
+      }
+    });
+    return k.rc;
+  }
+};
+// The way of float32 layers with many products: the tensor cores, on three bf16 parts of every value (see PRODUCTS in mix_tc.cu).
+struct FloatCores {
+  const mc_ce_desc* d;
+  const long long P;
+  const int Cp, Vp;
+  explicit FloatCores(const mc_ce_desc* desc)
+      : d(desc), P(desc->B * desc->S), Cp((desc->C + 63) / 64 * 64), Vp((desc->V + 63) / 64 * 64) {}
+  // Sums over classes are one MMA accumulator's, which truncates: up to 4096 classes stay within 2^-16 of a sum of one sign.
+  static bool takes(const mc_ce_desc* d) {
+    return d->dtype == MC_F32 && d->V <= 4096 && (double)d->B * d->S * d->V * d->C >= FLOATS_FROM;
+  }
+  bool planes() const { return !(d->layout == MC_NHWC || d->S == 1) && d->C > 1; }
+  mix::TcRows parts_of(const void* p, long long rows, int cols, int wide) const { return mix::TcRows{p, rows, cols, 3 * wide, 0, false, 3}; }
+  static size_t bytes(long long rows, int wide) { return (size_t)rows * 3 * wide * 2; }
+  void split(const float* src, long long S, long long img, long long pix, long long ch, long long p1, long long n, int C, int wide,
+             const float* lse, void* dst, cudaStream_t st) const {
+    const dim3 tiles((unsigned)((n + 31) / 32), (unsigned)((wide + 31) / 32 < 64 ? (wide + 31) / 32 : 64));
+    parts_kernel<<<tiles, THREADS, 0, st>>>(src, S, img, pix, ch, p1, n, C, wide, lse, (bf16*)dst), MC_COUNT(1);
+  }
+  void split_pixels(const float* x, long long p, long long n, const float* lse, void* dst, cudaStream_t st) const {
+    if (planes()) split(x, d->S, d->S * d->C, 1, d->S, p, n, d->C, Cp, lse, dst, st);
+    else split(x, P, P * d->C, d->C, 1, p, n, d->C, Cp, lse, dst, st);
+  }
+
+  int forward(mix::Work& k, const float* x, const float* w, const float* bias, const int64_t* target, float* loss, char* kept) const {
+    long long piece = (long long)(PIECE_TC / ((size_t)((d->V + 63) / 64) * 8 + bytes(1, Cp))) / 256 * 256;
+    if (piece > P) piece = P;
+    const long long last = (P - 1) % piece + 1, pieces = (P + piece - 1) / piece;
+    const auto tiles = [&](long long n) { return mix::tc_scores_tiles(n, d->C, d->V, 3); };
+    const size_t one = (size_t)tiles(piece) * piece, other = (size_t)tiles(last) * last;
+    void* x3 = k.take(bytes(piece, Cp));
+    void* w3 = k.take(bytes(d->V, Cp));
+    mix::Scores s{target, d->ignore_index};
+    s.bias32 = bias;
+    s.part = (float2*)k.take((one > other ? one : other) * 8);
+    s.hit = (float*)k.take((size_t)piece * 4);
+    double* part = (double*)k.take((size_t)pieces * SUM_BLOCKS * 16);
+    if (!k.run()) return k.rc;
+    split(w, d->V, 0, d->C, 1, 0, d->V, d->C, Cp, nullptr, w3, k.st);
+    int blocks = 0;
+    for (long long p = 0; p < P; p += piece) {
+      const long long n = P - p < piece ? P - p : piece;
+      split_pixels(x, p, n, nullptr, x3, k.st);
+      s.target = target + p;
+      k.did(mix::tc_scores_sum(parts_of(x3, n, d->C, Cp), parts_of(w3, d->V, d->C, Cp), nullptr, s, k.st));
+      if (k.rc) return k.rc;
+      const int more = grid_for(n, THREADS, SUM_BLOCKS);
+      k.did(launch_behind(finish_kernel, more, k.st, (mix::Scores)s, (int)tiles(n), (long long)n, (int)d->V,
+                          (float*)(kept + KEPT_HEAD) + p, (double*)(part + 2 * blocks)));
+      if (k.rc) return k.rc;
+      blocks += more;
+    }
+    MC_CHECK_LAUNCH();
+    return launch_behind(loss_kernel<float>, 1, k.st, (const double*)part, (int)blocks, d->reduction == MC_REDUCE_MEAN, (double*)kept, loss);
+  }
+
+  int backward(mix::Work& k, const float* grad, const float* x, const float* w, const float* bias, const int64_t* target,
+               const char* kept, float* gx, float* gw, float* gb) const {
+    // pieces of pixels: whole images, or part of one, where the output lies in planes
+    const long long S = planes() ? d->S : P, B = planes() ? d->B : 1;
+    long long most = (long long)(PIECE_TC / (bytes(1, Vp) + bytes(1, Cp))) / 256 * 256;
+    const long long run = most < S ? most : S, images = most < S ? 1 : most / S < B ? most / S : B;
+    most = images * run;
+    const auto each = [&](auto f) {
+      for (long long i = 0; i < B; i += images)
+        for (long long s = 0; s < S; s += run) f(i, s, (B - i < images ? B - i : images) * (S - s < run ? S - s : run));
+    };
+    void* x3 = k.take(bytes(most, Cp));
+    void* w3 = k.take(bytes(d->V, Cp));
+    void* wt3 = k.take(bytes(d->C, Vp));
+    mix::TcRows gz{nullptr, most, d->V, 64, 0, true, 3};
+    gz.p = k.take(gz.block_bytes());
+    int splits = 0, ldn = 0;
+    size_t floats = 0, sums = 0;
+    long long seen[2] = {0, 0};  // (there are at most a few sizes of pieces)
+    each([&](long long, long long, long long n) {
+      if (n == seen[0] || n == seen[1]) return;
+      seen[1] = seen[0], seen[0] = n;
+      const size_t f = mix::tc_outer_floats(n, d->V, 1, d->C, &splits, &ldn, 3);
+      if (f > floats) floats = f;
+      if ((size_t)splits * d->V > sums) sums = (size_t)splits * d->V;
+    });
+    float* part = (float*)k.take(floats * 4);
+    float* csum = (float*)k.take(sums * 4);
+    float* acc = (float*)k.take(most < P ? ((size_t)d->V * ldn + d->V) * 4 : 0);
+    if (!k.run()) return k.rc;
+    const long long threads = (long long)d->V * (ldn / 4) + d->V;
+    const float* lse = (const float*)(kept + KEPT_HEAD);
+    split(w, d->V, 0, d->C, 1, 0, d->V, d->C, Cp, nullptr, w3, k.st);
+    if (gx) split(w, d->C, 0, 1, d->C, 0, d->C, d->V, Vp, nullptr, wt3, k.st);
+    each([&](long long i, long long s, long long n) {
+      if (k.rc) return;
+      const long long p = i * S + s;
+      split_pixels(x, p, n, lse + p, x3, k.st);
+      mix::Scores sc{target + p, d->ignore_index, nullptr, nullptr, lse + p, grad,
+                     d->reduction == MC_REDUCE_MEAN ? (const double*)kept : nullptr, bias};
+      const mix::TcRows xp = parts_of(x3, n, d->C, Cp), gp{gz.p, n, d->V, 64, 0, true, 3};
+      k.did(mix::tc_scores_grad(xp, parts_of(w3, d->V, d->C, Cp), nullptr, sc, gp, k.st));
+      if (gx && !k.rc) {
+        float* to = planes() ? gx + i * S * d->C + s : gx + p * d->C;
+        k.did(mix::tc_input_grad32(gp, parts_of(wt3, d->C, d->V, Vp), to, planes() ? 0 : d->C, d->S, k.st));
+      }
+      if ((gw || gb) && !k.rc) {
+        mix::tc_outer_floats(n, d->V, 1, d->C, &splits, &ldn, 3);
+        k.did(mix::tc_outer(gp, mix::TcRows{}, xp, part, csum, k.st));
+        if (k.rc) return;
+        // (many shares of few sums: several threads for each)
+        if (splits >= 64 && p == 0 && n == P) mix::add_shares<float, float>(part, d->V, d->C, ldn, gw, csum, gb, splits, k.st);
+        else add_piece_kernel<float><<<(unsigned)((threads + THREADS - 1) / THREADS), THREADS, 0, k.st>>>(
             part, csum, splits, d->V, d->C, ldn, acc, p == 0, p + n == P, gw, gb), MC_COUNT(1);
         k.did(cudaGetLastError() == cudaSuccess ? MC_OK : MC_ERR_LAUNCH);
       }
@@ -622,6 +778,12 @@ size_t mc_cross_entropy_workspace_bytes(const mc_ce_desc* d, int32_t phase) {
       if (phase == MC_PHASE_BACKWARD) t.backward(k, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr);
       else t.forward(k, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr);
     });
+  if (classify::FloatCores::takes(d))
+    return classify::work_size([&](mix::Work& k) {
+      const classify::FloatCores t(d);
+      if (phase == MC_PHASE_BACKWARD) t.backward(k, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr);
+      else t.forward(k, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr);
+    });
   return classify::by_type(d->dtype, [&](auto t) {
     return classify::General<decltype(t)>(d, nullptr, phase == MC_PHASE_BACKWARD, nullptr).m.used;
   });
@@ -638,6 +800,10 @@ int mc_cross_entropy_fwd(const mc_ce_desc* d, const void* x, const void* w, cons
   if (d->dtype == MC_BF16) {
     mix::Work k{(char*)ws, (cudaStream_t)stream};
     return classify::TensorCores(d).forward(k, (const bf16*)x, (const bf16*)w, (const bf16*)bias, target, (float*)loss, (char*)saved);
+  }
+  if (classify::FloatCores::takes(d)) {
+    mix::Work k{(char*)ws, (cudaStream_t)stream};
+    return classify::FloatCores(d).forward(k, (const float*)x, (const float*)w, (const float*)bias, target, (float*)loss, (char*)saved);
   }
   return classify::by_type(d->dtype, [&](auto t) {
     typedef decltype(t) T;
@@ -660,6 +826,11 @@ int mc_cross_entropy_bwd(const mc_ce_desc* d, const void* grad_loss, const void*
     mix::Work k{(char*)ws, (cudaStream_t)stream};
     return classify::TensorCores(d).backward(k, (const float*)grad_loss, (const bf16*)x, (const bf16*)w, (const bf16*)bias, target,
                                              (const char*)saved, (bf16*)gx, (bf16*)gw, (bf16*)gb);
+  }
+  if (classify::FloatCores::takes(d)) {
+    mix::Work k{(char*)ws, (cudaStream_t)stream};
+    return classify::FloatCores(d).backward(k, (const float*)grad_loss, (const float*)x, (const float*)w, (const float*)bias, target,
+                                            (const char*)saved, (float*)gx, (float*)gw, (float*)gb);
   }
   return classify::by_type(d->dtype, [&](auto t) {
     typedef decltype(t) T;

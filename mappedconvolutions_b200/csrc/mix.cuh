@@ -190,7 +190,11 @@ struct TcRows {
   // Blocks of 128 rows x 64 columns one after the other, those of the same rows next to each other; an even number of tiles of 128
   // rows.  (Rows of 20 KB: a tile's 128 rows are 128 places in memory, 1 TB/s.)
   bool blocks = false;
-  int across() const { return (cols + 63) / 64; }
+  // Float32 values in three bf16 parts (8 bits each), the parts of a row behind each other, each filled up with zeros to whole
+  // blocks of 64 columns.
+  int parts = 1;
+  int part_blocks() const { return (cols + 63) / 64; }
+  int across() const { return parts * part_blocks(); }
   size_t block_bytes() const { return (size_t)((rows + 255) / 256) * 2 * across() * (128 * 64 * 2); }
 };
 // y = act(a w^T + bias) + r, or with backward y = r act'(a w^T + bias); w (N, K), r.p may be null (not with backward)
@@ -205,7 +209,7 @@ int tc_gate(const TcRows& x, const TcRows& w_in, const bf16* b_in, int act, cons
 int tc_gate_bwd(const TcRows& x, const TcRows& w_in, const bf16* b_in, int act, const TcRows& gy, const TcRows& w_out_t,
                 const TcRows& gg, const TcRows& gu, cudaStream_t st);
 // part[s] = the s-th share of [g0|g1]^T x (rows of *ldn floats), csum[s] = its column sums of [g0|g1]; g1.p may be null
-size_t tc_outer_floats(long long P, int M, int segs, int N, int* splits, int* ldn);
+size_t tc_outer_floats(long long P, int M, int segs, int N, int* splits, int* ldn, int parts = 1);
 int tc_outer(const TcRows& g0, const TcRows& g1, const TcRows& x, float* part, float* csum, cudaStream_t st);
 // Class scores z = x w^T + bias (w: (V, C)), which are never stored, against labels:
 struct Scores {
@@ -218,11 +222,16 @@ struct Scores {
   const float* lse;
   const float* grad;
   const double* count;
+  const float* bias32;  // of float32 layers
+  bf16* gz;             // of float32 layers: where the three parts of gz go
 };
-int tc_scores_tiles(long long P, int C, int V);  // tiles of classes that tc_scores_sum leaves sums of
+// tensors in parts: the products of float32 values, six products of parts each, small ones first (the accumulators truncate)
+int tc_scores_tiles(long long P, int C, int V, int parts = 1);  // tiles of classes that tc_scores_sum leaves sums of
 int tc_scores_sum(const TcRows& x, const TcRows& w, const bf16* bias, const Scores& s, cudaStream_t st);
 // gz = grad / count (exp(z - lse) - [label]), in blocks
 int tc_scores_grad(const TcRows& x, const TcRows& w, const bf16* bias, const Scores& s, const TcRows& gz, cudaStream_t st);
+// gx = g w^T in float32, g in blocks and parts, w (N, K) in parts; gx rows of ld floats (w.rows of them used), or planes of S pixels
+int tc_input_grad32(const TcRows& g, const TcRows& w, float* gx, long long ld, long long S, cudaStream_t st);
 // mc_mix_plan for a checked bf16 description; false: no such product
 bool tc_plan(const mc_mix_desc* d, int product, int sms, int32_t* out);
 

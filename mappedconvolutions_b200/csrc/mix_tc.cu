@@ -179,8 +179,14 @@ enum Mode {
   GATE_BWD = 2,  // [g|u] as above from the first operands, gh from the second: y0 = gh u act'(g), y1 = gh act(g)
   ACT_BWD = 3,   // y = r act'(A B^T + bias)
   SCORE_SUM = 4, // softmax sums of z = A B^T + bias over the tile's columns, the label's z
-  SCORE_GRAD = 5 // y = scale (exp(z - lse) - [label])
+  SCORE_GRAD = 5,// y = scale (exp(z - lse) - [label])
+  FLOATS = 6     // y = A B^T in float32
 };
+// Products of float32 values in three bf16 parts each, 0 the largest: (2,0) (0,2) (1,1) (1,0) (0,1) (0,0).  The others are below
+// 2^-24 of the product.  Small ones come first: the accumulators truncate, up to 2^-23 of what they hold for every MMA.
+constexpr int PRODUCTS = 6;
+__device__ __forceinline__ int part_a(int product) { return 0x052 >> 2 * product & 3; }
+__device__ __forceinline__ int part_b(int product) { return 0x118 >> 2 * product & 3; }
 // BN: channels of a tile.  It is staged CW channels (128 or 64 swizzled bytes a row) at a time; the two results of
 // GATE_BWD side by side, in smaller tiles because its weights leave little room.
 template <int MODE, int BN> struct Cfg {
@@ -204,6 +210,9 @@ struct alignas(64) GemmArgs {
   const bf16* bias;  // null: none
   int m_pairs, rows; // pairs of tiles; pixels
   int a_across[2], y_across;  // blocks next to each other where a tensor lies in blocks, else 0
+  int per;           // stages of a product of parts where operands are in parts, else 0
+  float* floats;     // FLOATS: y, rows of ld values or (ld == 0) planes
+  long long ld;
   int n_tiles, N, kb[2], act;
   int up;            // distance between a gate's row of b[0] and bias and its factor's
   int res;           // r is read
@@ -445,13 +454,15 @@ __device__ __forceinline__ void read_scores(const GemmArgs& g, int set, uint32_t
       for (int e = row; e < BN; e += 128) {
         float b = n0 + e < g.N ? 0.f : -INFINITY;
         if (g.bias && n0 + e < g.N) b = __bfloat162float(__ushort_as_bfloat16(__ldg((const unsigned short*)g.bias + n0 + e)));
+        if (g.sc.bias32 && n0 + e < g.N) b = __ldg(g.sc.bias32 + n0 + e);
         bs[e] = b;
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(bfull + BAR_BIASED + 8 * set);
       if (!warp_wait(bfull + BAR_BIASED + 8 * set, it & 1, abort_flag, 0x153)) return;  // (bounded, unlike bar.sync)
     }
-    const uint32_t p = (w.m() * 2 + rank) * TILE + row;
+    const int tile0 = (w.m() * 2 + rank) * TILE;
+    const uint32_t p = tile0 + row;
     const bool in = p < (uint32_t)g.rows;
     int label = -1;  // of this tile's columns
     float lse2 = INFINITY;
@@ -482,7 +493,8 @@ __device__ __forceinline__ void read_scores(const GemmArgs& g, int set, uint32_t
         __syncwarp();
         if (lane == 0) arrive_leader(tempty0 + 8 * acc);
       }
-      const bool turn = MODE == SCORE_GRAD && pc % PER == 0, done = MODE == SCORE_GRAD && pc % PER == PER - 1;
+      const bool staged = MODE == SCORE_GRAD && !g.sc.gz;
+      const bool turn = staged && pc % PER == 0, done = staged && pc % PER == PER - 1;
       if (turn && !warp_wait(bar_of(BAR_READY, i), i >> C::SLOT_BITS & 1, abort_flag, 0x152)) return false;
       if (pc < live) {
         float2 z[PW / 2];
@@ -512,13 +524,29 @@ __device__ __forceinline__ void read_scores(const GemmArgs& g, int set, uint32_t
         } else {
           MC_HALF z[j] = exp2_2(fma2(z[j], two(LOG2E), two(-lse2)));
           if (any) MC_HALF z[j] = add2(z[j], make_float2(here == 2 * j ? -1.f : 0.f, here == 2 * j + 1 ? -1.f : 0.f));
-          uint32_t r[PW / 2];
-          MC_HALF z[j] = mul2(z[j], two(scale));
-          MC_HALF r[j] = dead ? 0u : pack_bf16x2(z[j].x, z[j].y);
-          const uint32_t at = at0 + (i & mask) * C::CH_BYTES, j0 = pc % PER * (PW / 8);
+          MC_HALF z[j] = dead ? two(0.f) : mul2(z[j], two(scale));
+          if (staged) {
+            const uint32_t at = at0 + (i & mask) * C::CH_BYTES, j0 = pc % PER * (PW / 8);
+            uint32_t r[PW / 2];
+            MC_HALF r[j] = pack_bf16x2(z[j].x, z[j].y);
 #pragma unroll
-          for (int h = 0; h < PW / 8; ++h)
-            sts16(at + (((j0 + h) << 4) ^ swizzle), make_uint4(r[4 * h], r[4 * h + 1], r[4 * h + 2], r[4 * h + 3]));
+            for (int h = 0; h < PW / 8; ++h)
+              sts16(at + (((j0 + h) << 4) ^ swizzle), make_uint4(r[4 * h], r[4 * h + 1], r[4 * h + 2], r[4 * h + 3]));
+          } else if (tile0 < g.rows) {
+            // 64 bytes of this pixel's row in the block of each part
+            bf16* to = g.sc.gz + (((long long)(tile0 / TILE) * g.y_across + (n0 + PW * pc) / KB) * TILE + row) * KB + PW * pc % KB;
+#pragma unroll
+            for (int part = 0; part < 3; ++part, to += (long long)(g.y_across / 3) * TILE * KB) {
+              uint32_t r[PW / 2];
+              MC_HALF {
+                r[j] = pack_bf16x2(z[j].x, z[j].y);
+                z[j] = add2(z[j], make_float2(-__uint_as_float(r[j] << 16), -__uint_as_float(r[j] & 0xFFFF0000u)));
+              }
+#pragma unroll
+              for (int h = 0; h < PW / 8; ++h)
+                *reinterpret_cast<uint4*>(to + 8 * h) = make_uint4(r[4 * h], r[4 * h + 1], r[4 * h + 2], r[4 * h + 3]);
+            }
+          }
         }
       }
       if (done) {
@@ -540,6 +568,46 @@ __device__ __forceinline__ void read_scores(const GemmArgs& g, int set, uint32_t
   }
 }
 #undef MC_HALF
+
+// Read-out warps of a product in float32: thread = pixel, sixteen columns at a time.
+template <int BN>
+__device__ __forceinline__ void read_floats(const GemmArgs& g, int set, uint32_t rank, uint32_t bfull, volatile int* abort_flag) {
+  typedef Cfg<FLOATS, BN> C;
+  const int lane = threadIdx.x % 32, q = threadIdx.x / 32 & 3, row = q * 32 + lane;
+  const uint32_t tempty0 = of_leader(bfull + BAR_TEMPTY);
+  uint32_t it = 0;
+  for (TileWalk w(g, set, 2); w.more(); w.next(), ++it) {
+    const uint32_t p = (w.m() * 2 + rank) * TILE + row, tile = 2 * it + set, acc = tile % C::NACC;
+    const int n0 = w.nt() * BN, left = g.N - n0, live = left < BN ? (left + 15) / 16 : BN / 16;
+    const bool in = p < (uint32_t)g.rows;
+    long long step = 1;
+    float* to = g.floats;
+    if (in && g.ld) to += p * g.ld + n0;
+    if (in && !g.ld) {
+      uint32_t im, s;
+      g.pd.split(p, im, s);
+      to += ((long long)im * g.N + n0) * g.pd.S + s, step = g.pd.S;
+    }
+    if (!warp_wait(bfull + BAR_TFULL + 8 * acc, tile / C::NACC & 1, abort_flag, 0x161)) return;
+    tc_fence_after_sync();
+    const uint32_t t0 = ((uint32_t)(q * 32) << 16) + acc * C::ACC;
+#pragma unroll 1
+    for (int pc = 0; pc < live; ++pc) {
+      uint32_t v[16];
+      tmem_ld_32x16(t0 + 16 * pc, v);
+      tmem_ld_wait();
+      if (in) {
+#pragma unroll
+        for (int j = 0; j < 16; ++j)
+          if (16 * pc + j < left) to[(16 * pc + j) * step] = __uint_as_float(v[j]);
+      }
+      __syncwarp();
+    }
+    tc_fence_before_sync();
+    __syncwarp();
+    if (lane == 0) arrive_leader(tempty0 + 8 * acc);
+  }
+}
 
 template <int MODE, int BN>
 __global__ void __launch_bounds__(THREADS, 1) rows_tc_kernel(const __grid_constant__ GemmArgs g) {
@@ -605,7 +673,7 @@ __global__ void __launch_bounds__(THREADS, 1) rows_tc_kernel(const __grid_consta
       for (int n = 0; n < g.group; ++n)
         for (int seg = 0; seg < 2; ++seg)
           for (int k = 0; k < g.kb[seg]; ++k) {
-            load_b<MODE, BN>(g, seg, rank, dst, k * KB, (w.base + n) * BN, bar);
+            load_b<MODE, BN>(g, seg, rank, dst, (g.per ? part_b(k / g.per) * g.per + k % g.per : k) * KB, (w.base + n) * BN, bar);
             dst += seg ? C::B1 : C::B0;
           }
     }
@@ -622,8 +690,10 @@ __global__ void __launch_bounds__(THREADS, 1) rows_tc_kernel(const __grid_consta
             const uint32_t bar = of_leader(full(st));
             if (rank == 0) mbar_expect_tx(full(st), 2 * (A_BYTES + (g.group ? 0 : seg ? C::B1 : C::B0)));
             const int across = g.a_across[seg];
-            tma_load_pair(a0 + st * A_BYTES, &g.a[seg], across ? 0 : k * KB, across ? m0 * across + k * TILE : m0, bar);
-            if (!g.group) load_b<MODE, BN>(g, seg, rank, b0 + st * C::BMAX, k * KB, n0, bar);
+            int ka = k, kb = k;
+            if (g.per) ka = part_a(k / g.per) * g.per + k % g.per, kb = part_b(k / g.per) * g.per + k % g.per;
+            tma_load_pair(a0 + st * A_BYTES, &g.a[seg], across ? 0 : ka * KB, across ? m0 * across + ka * TILE : m0, bar);
+            if (!g.group) load_b<MODE, BN>(g, seg, rank, b0 + st * C::BMAX, kb * KB, n0, bar);
           }
           __syncwarp();
           if (++st == (uint32_t)g.stages) st = 0, ph ^= 1;
@@ -687,7 +757,8 @@ __global__ void __launch_bounds__(THREADS, 1) rows_tc_kernel(const __grid_consta
     }
   } else if (warp < 4) {
     // ---- I/O of one set's staged tiles: fill the slots ahead (residual), store what the read-out warps leave in them
-    if (lane == 0 && MODE != SCORE_SUM && !(MODE == LAYER && g.planes && !g.res)) {
+    if (lane == 0 && MODE != SCORE_SUM && MODE != FLOATS && !(MODE == SCORE_GRAD && g.sc.gz) &&
+        !(MODE == LAYER && g.planes && !g.res)) {
       const int set = warp - 2;
       TileWalk lead(g, set, 2);
       int lead_c = 0;
@@ -731,6 +802,8 @@ __global__ void __launch_bounds__(THREADS, 1) rows_tc_kernel(const __grid_consta
     // ---- read-out
     if constexpr (MODE == SCORE_SUM || MODE == SCORE_GRAD) {
       read_scores<MODE, BN>(g, (warp - 4) / 4, rank, bias_s, out0, bfull, abort_flag);
+    } else if constexpr (MODE == FLOATS) {
+      read_floats<BN>(g, (warp - 4) / 4, rank, bfull, abort_flag);
     } else {
       with_act(g.act, [&](auto act) {
         read_out<MODE, BN, decltype(act)>(g, (warp - 4) / 4, rank, bias_s, out0, bfull, abort_flag);
@@ -757,6 +830,8 @@ struct alignas(64) OuterTcArgs {
   int kblocks, per;    // 64-pixel blocks in all, and of a share
   int stages;
   int across;          // blocks next to each other where the first operand lies in blocks, else 0
+  int products;        // of parts: PRODUCTS or 1
+  int g_part, x_part;  // columns from part to part
 };
 constexpr int OUTER_BARS = 3 * MAX_STAGES + 1;
 
@@ -782,7 +857,7 @@ __global__ void __launch_bounds__(THREADS, 1) outer_tc_kernel(const __grid_const
   const int nt = tile % g.n_tiles, mt = tile / g.n_tiles % g.m_tiles, seg = tile / g.n_tiles / g.m_tiles;
   // channel group m of this block starts at m0 + 256 m
   const int m0 = mt * MT * 256 + rank * 128, n0 = nt * BN;
-  const int k0 = split * g.per, k1 = min(g.kblocks, k0 + g.per);
+  const int k0 = split * g.per, k1 = min(g.kblocks, k0 + g.per), len = k1 > k0 ? k1 - k0 : 0, steps = len * g.products;
   const bool sums = nt == 0;
 
   if (threadIdx.x == 0) {
@@ -804,24 +879,27 @@ __global__ void __launch_bounds__(THREADS, 1) outer_tc_kernel(const __grid_const
     const bool elected = elect_one();
     uint32_t st = 0, ph = 0;
     bool ok = true;
-    for (int k = k0; k < k1 && ok; ++k) {
+    int k = k0, product = 0;
+    for (int i = 0; i < steps && ok; ++i) {
       ok = __all_sync(~0u, mbar_wait(empty(st), ph ^ 1, abort_flag, 0x141));
       if (!ok) break;
       if (elected) {
+        const int pa = g.products > 1 ? part_a(product) * g.g_part : 0, pb = g.products > 1 ? part_b(product) * g.x_part : 0;
         const uint32_t bar = of_leader(full(st)), dst = s0 + st * STAGE;
         if (rank == 0) mbar_expect_tx(full(st), 2 * STAGE);
 #pragma unroll
         for (int i = 0; i < 2 * MT; ++i) {
-          const int col = m0 + i / 2 * 256 + i % 2 * 64, row = k * KB;
+          const int col = pa + m0 + i / 2 * 256 + i % 2 * 64, row = k * KB;
           // (columns past the last block are those of the next rows, or zeros: sums that nobody reads)
           if (g.across) tma_load_pair(dst + i * 8192, &g.g[seg], 0, (row / TILE * g.across + col / KB) * TILE + row % TILE, bar);
           else tma_load_pair(dst + i * 8192, &g.g[seg], col, row, bar);
         }
 #pragma unroll
         for (int i = 0; i < BN / 128; ++i)
-          tma_load_pair(dst + GB + i * 8192, &g.x, n0 + rank * (BN / 2) + 64 * i, k * KB, bar);
+          tma_load_pair(dst + GB + i * 8192, &g.x, pb + n0 + rank * (BN / 2) + 64 * i, k * KB, bar);
       }
       __syncwarp();
+      if (++k == k1) k = k0, ++product;
       if (++st == (uint32_t)g.stages) st = 0, ph ^= 1;
     }
     for (int i = 0; i < g.stages && ok; ++i) {  // (no arrival of the leader's commits is left behind)
@@ -834,7 +912,7 @@ __global__ void __launch_bounds__(THREADS, 1) outer_tc_kernel(const __grid_const
       constexpr uint32_t idesc = make_idesc_bf16(256, BN, 1, 1), HI = desc_sw128_hi(1024);
       uint32_t st = 0, ph = 0;
       bool there = false;
-      for (int k = k0; k < k1; ++k) {
+      for (int i = 0; i < steps; ++i) {
         if (!there && !__all_sync(~0u, mbar_wait(full(st), ph, abort_flag, 0x142))) break;
         const uint32_t cur = st;
         if (++st == (uint32_t)g.stages) st = 0, ph ^= 1;
@@ -845,7 +923,7 @@ __global__ void __launch_bounds__(THREADS, 1) outer_tc_kernel(const __grid_const
           for (int m = 0; m < MT; ++m)
 #pragma unroll
             for (int j = 0; j < 4; ++j)  // sixteen pixels each
-              pair_mma(tmem + m * BN, ad + m * (A_BYTES >> 4) + 128 * j, HI, bd + 128 * j, HI, idesc, k != k0 || j != 0);
+              pair_mma(tmem + m * BN, ad + m * (A_BYTES >> 4) + 128 * j, HI, bd + 128 * j, HI, idesc, i != 0 || j != 0);
           pair_commit(empty(cur));
           if (sums) pair_commit(landed(cur));
         }
@@ -863,10 +941,13 @@ __global__ void __launch_bounds__(THREADS, 1) outer_tc_kernel(const __grid_const
       const int piece = ew * PC + lane % PC, box = piece / 8, j = piece % 8;
       float acc[8] = {};
       uint32_t st = 0, ph = 0;
-      for (int k = k0; k < k1; ++k) {
+      int k = 0, product = 0;
+      for (int i = 0; i < steps; ++i) {
         ok = warp_wait(landed(st), ph, abort_flag, 0x143);
         if (!ok) break;
         const uint32_t base = s0 + st * STAGE + box * 8192;
+        // (every part of the first operand once: products 0, 2 and 5)
+        if (g.products == 1 || (0x25 >> product & 1))
 #pragma unroll
         for (int p = lane / PC; p < KB; p += PX) {
           const uint4 r = lds16(base + p * 128 + ((j ^ (p & 7)) << 4));
@@ -879,6 +960,7 @@ __global__ void __launch_bounds__(THREADS, 1) outer_tc_kernel(const __grid_const
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(empty(st));
+        if (++k == len) k = 0, ++product;
         if (++st == (uint32_t)g.stages) st = 0, ph ^= 1;
       }
 #pragma unroll
@@ -890,7 +972,7 @@ __global__ void __launch_bounds__(THREADS, 1) outer_tc_kernel(const __grid_const
       }
     }
     if (ok) ok = warp_wait(done, 0, abort_flag, 0x144);
-    if (ok && k1 > k0) {
+    if (ok && steps) {
       tc_fence_after_sync();
 #pragma unroll 1
       for (int t = ew / 4; t < MT * BN / 32; t += 2) {  // 32 columns each
@@ -936,6 +1018,7 @@ static bool encode(CUtensorMap* tm, const TcRows& t, int box_r, int box_c = KB) 
                               const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
                               CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
   cuuint64_t dims[2] = {(cuuint64_t)t.cols, (cuuint64_t)t.rows}, strides[1] = {(cuuint64_t)t.ld * 2};
+  if (t.parts > 1) dims[0] = (cuuint64_t)t.across() * KB;
   if (t.blocks) dims[0] = KB, dims[1] = t.block_bytes() / (KB * 2), strides[0] = KB * 2;
   const cuuint32_t box[2] = {(cuuint32_t)box_c, (cuuint32_t)box_r}, es[2] = {1, 1};
   for (int attempt = 0; attempt < 2; ++attempt) {
@@ -1133,24 +1216,40 @@ int tc_input_grad(const TcRows& g0, const TcRows& w0, const TcRows& g1, const Tc
   return launch_wide<LAYER>(g, bn, st);
 }
 
-int tc_scores_tiles(long long P, int C, int V) {
-  const int bn = tile_width((P + 2 * TILE - 1) / (2 * TILE), V, kblocks(C), sm_total());
+static int stages_of(const TcRows& a) { return a.parts > 1 ? PRODUCTS * a.part_blocks() : kblocks(a.cols); }
+int tc_scores_tiles(long long P, int C, int V, int parts) {
+  const int bn = tile_width((P + 2 * TILE - 1) / (2 * TILE), V, stages_of(TcRows{nullptr, P, C, 0, 0, false, parts}), sm_total());
   return (V + bn - 1) / bn;
 }
-int tc_scores_sum(const TcRows& x, const TcRows& w, const bf16* bias, const Scores& s, cudaStream_t st) {
-  GemmArgs g = base_args(x, TcRows{nullptr, x.rows, (int)w.rows, 0}, bias, MC_ACT_NONE);
+static GemmArgs score_args(const TcRows& x, int classes, const bf16* bias, const Scores& s) {
+  GemmArgs g = base_args(x, TcRows{nullptr, x.rows, classes, 0}, bias, MC_ACT_NONE);
   g.sc = s;
+  g.kb[0] = stages_of(x);
+  if (x.parts > 1) g.per = x.part_blocks();
+  return g;
+}
+int tc_scores_sum(const TcRows& x, const TcRows& w, const bf16* bias, const Scores& s, cudaStream_t st) {
+  GemmArgs g = score_args(x, (int)w.rows, bias, s);
   const int bn = tile_width(g.m_pairs, g.N, g.kb[0], sm_total());
   if (!encode(&g.a[0], x, TILE) || !encode(&g.b[0], w, bn / 2)) return MC_ERR_LAUNCH;
   return launch_wide<SCORE_SUM>(g, bn, st);
 }
 int tc_scores_grad(const TcRows& x, const TcRows& w, const bf16* bias, const Scores& s, const TcRows& gz, cudaStream_t st) {
-  GemmArgs g = base_args(x, gz, bias, MC_ACT_NONE);
-  g.sc = s;
+  GemmArgs g = score_args(x, gz.cols, bias, s);
   g.y_across = gz.blocks ? gz.across() : 0;
+  if (gz.parts > 1) g.sc.gz = (bf16*)const_cast<void*>(gz.p);
   const int bn = tile_width(g.m_pairs, g.N, g.kb[0], sm_total());
-  if (!encode(&g.a[0], x, TILE) || !encode(&g.b[0], w, bn / 2) || !encode(&g.y[0], gz, TILE)) return MC_ERR_LAUNCH;
+  if (!encode(&g.a[0], x, TILE) || !encode(&g.b[0], w, bn / 2) || (!g.sc.gz && !encode(&g.y[0], gz, TILE))) return MC_ERR_LAUNCH;
   return launch_wide<SCORE_GRAD>(g, bn, st);
+}
+int tc_input_grad32(const TcRows& gz, const TcRows& w, float* gx, long long ld, long long S, cudaStream_t st) {
+  GemmArgs g = base_args(gz, TcRows{nullptr, gz.rows, (int)w.rows, 0}, nullptr, MC_ACT_NONE);
+  g.kb[0] = stages_of(gz), g.per = gz.part_blocks(), g.a_across[0] = gz.across();
+  g.floats = gx, g.ld = ld;
+  if (!ld) g.pd = PixDiv((uint32_t)S);
+  const int bn = long_tile_width(g.m_pairs, g.N, sm_total());
+  if (!encode(&g.a[0], gz, TILE) || !encode(&g.b[0], w, bn / 2)) return MC_ERR_LAUNCH;
+  return launch_wide<FLOATS>(g, bn, st);
 }
 
 // 128 hidden channels a tile of the gate, 64 where that pads less: 38 hidden channels take half the time (wide blocks 4 % more)
@@ -1182,7 +1281,9 @@ constexpr int MOST_PER = (1 << 17) / KB;
 struct OuterPlan {
   int mt, bn, m_tiles, n_tiles, splits, per;
 };
-static OuterPlan outer_plan(long long P, int M, int segs, int N, int sms) {
+// Of float32 values in parts: 2^10 pixels, 2^-18 of a sum of one sign at most.
+constexpr int MOST_PER_PARTS = (1 << 10) / KB;
+static OuterPlan outer_plan(long long P, int M, int segs, int N, int sms, int parts = 1) {
   OuterPlan p;
   p.mt = M > 256 ? 2 : 1;
   p.bn = N <= 128 ? 128 : 256;
@@ -1191,20 +1292,21 @@ static OuterPlan outer_plan(long long P, int M, int segs, int N, int sms) {
   const long long tiles = (long long)segs * p.m_tiles * p.n_tiles, kb = (P + KB - 1) / KB;
   double best = 1e30;
   const int pairs = sms / 2;
-  const long long least = (kb + MOST_PER - 1) / MOST_PER;
+  const int most_per = parts > 1 ? MOST_PER_PARTS : MOST_PER, products = parts > 1 ? PRODUCTS : 1;
+  const long long least = (kb + most_per - 1) / most_per;
   p.splits = 1, p.per = (int)kb;
   for (long long s = least; s < least + pairs && s <= (kb + 3) / 4; ++s) {
     const long long per = (kb + s - 1) / s;
     const double waves = (double)((tiles * s + pairs - 1) / pairs);
     // a pair's stages, and what it costs to write its sums and to add them up again (against eight other numbers of shares,
     // at 642 to 655 488 pixels and ten pairs of channel counts: 1.6 % more time on average, at most 10 %)
-    const double t = waves * (per + 8.0) + 0.05 * tiles * s;
+    const double t = waves * (products * per + 8.0) + 0.05 * tiles * s;
     if (t < best) best = t, p.splits = (int)((kb + per - 1) / per), p.per = (int)per;
   }
   return p;
 }
-size_t tc_outer_floats(long long P, int M, int segs, int N, int* splits, int* ldn) {
-  const OuterPlan p = outer_plan(P, M, segs, N, sm_total());
+size_t tc_outer_floats(long long P, int M, int segs, int N, int* splits, int* ldn, int parts) {
+  const OuterPlan p = outer_plan(P, M, segs, N, sm_total(), parts);
   *splits = p.splits;
   *ldn = (N + 3) / 4 * 4;
   return (size_t)p.splits * segs * M * *ldn;
@@ -1221,7 +1323,9 @@ int tc_outer(const TcRows& g0, const TcRows& g1, const TcRows& x, float* part, f
   OuterTcArgs g{};
   g.segs = g1.p ? 2 : 1;
   g.across = g0.blocks ? g0.across() : 0;
-  const OuterPlan p = outer_plan(x.rows, g0.cols, g.segs, x.cols, sm_total());
+  const OuterPlan p = outer_plan(x.rows, g0.cols, g.segs, x.cols, sm_total(), g0.parts);
+  g.products = g0.parts > 1 ? PRODUCTS : 1;
+  g.g_part = g0.part_blocks() * KB, g.x_part = x.part_blocks() * KB;
   if (!encode(&g.g[0], g0, KB) || (g1.p && !encode(&g.g[1], g1, KB)) || !encode(&g.x, x, KB)) return MC_ERR_LAUNCH;
   g.part = part, g.csum = csum;
   g.M = g0.cols, g.N = x.cols, g.ldn = (x.cols + 3) / 4 * 4;

@@ -84,6 +84,54 @@ def test_several_pieces(ops, pixels, classes, dtype):
     R.check(dict(loss=loss, **got), R.cross_entropy(x, weight, bias, target, -100, True, grad), "pieces")
 
 
+# float32 layers of 10^8 products and more (tensor cores, three bf16 parts of every value): odd counts, one block of channels or
+# classes and one more, one image or several
+MANY = [(3, 67, 101, 77, 99), (1, 1, 40962, 64, 64), (2, 1, 10242, 65, 129), (1, 130, 129, 128, 257), (5, 33, 40, 10, 2562), (1, 1, 600, 200, 1000),
+        (1, 300, 400, 1, 1000), (7, 1, 2562, 130, 63)]
+
+
+@pytest.mark.parametrize("layout", ["nhwc", "nchw"])
+@pytest.mark.parametrize("i", range(len(MANY)))
+def test_float32_of_many_products(ops, i, layout):
+    b, h, w, cin, classes = MANY[i]
+    g = torch.Generator("cuda").manual_seed(50 + i)
+    x = image(g, (b, cin, h, w), F32, layout)
+    weight, bias = classifier(g, classes, cin, F32)
+    target = labels(g, (b, h, w), classes, 0.2)
+    off = (target == -100)[:, None].expand_as(x)
+    grad = torch.tensor(-0.6, device="cuda")
+    mean = i % 2 == 0
+    want = R.cross_entropy(x, weight, bias, target, -100, mean, grad)
+    results = []
+    for value in (0.0, float("nan"), float("inf")):  # whatever the pixels without a label hold
+        x = torch.where(off, torch.full_like(x, value), x)
+        x = x.contiguous(memory_format=torch.channels_last) if layout == "nhwc" else x.contiguous()
+        loss, saved = ops.cross_entropy_forward(x, weight, bias, target, -100, mean)
+        results.append([loss] + ops.cross_entropy_backward(grad, saved, x, weight, bias, target, -100, mean))
+        assert layout_kept(results[-1][1], layout)
+        assert all(torch.equal(p, q) for p, q in zip(results[0], results[-1]))
+    R.check(dict(zip(("loss", "gx", "gw", "gb"), results[0])), want, str(MANY[i]))
+    # as near as float32 sums are: relative errors of whole tensors
+    for got, name in zip(results[0], ("loss", "gx", "gw", "gb")):
+        assert (got.double() - want[name][0]).norm() <= 5e-6 * want[name][0].norm(), name
+    only_x = ops.cross_entropy_backward(grad, saved, x, weight, bias, target, -100, mean, True, False)
+    only_w = ops.cross_entropy_backward(grad, saved, x, weight, bias, target, -100, mean, False, True)
+    assert torch.equal(only_x[0], results[0][1]) and torch.equal(only_w[1], results[0][2])
+    few = bias.clone()
+    few[classes // 2:] = -float("inf")  # classes ruled out, and a label that is none
+    target = target.clamp(max=classes // 2 - 1)
+    x = torch.where(off, torch.zeros_like(x), x)
+    loss, saved = ops.cross_entropy_forward(x, weight, few, target, -100, mean)
+    gx, gw, gb = ops.cross_entropy_backward(grad, saved, x, weight, few, target, -100, mean)
+    half = R.cross_entropy(x, weight[:classes // 2], bias[:classes // 2], target, -100, mean, grad)
+    R.check(dict(loss=loss, gx=gx, gw=gw[:classes // 2], gb=gb[:classes // 2]), half, "ruled out")
+    assert not gw[classes // 2:].any() and not gb[classes // 2:].any()
+    target[0, 0, 0] = classes
+    loss, saved = ops.cross_entropy_forward(x, weight, bias, target, -100, mean)
+    gx, gw, gb = ops.cross_entropy_backward(grad, saved, x, weight, bias, target, -100, mean)
+    assert loss.isnan() and gw.isnan().all() and gb.isnan().all() and gx[0, :, 0, 0].isnan().all() and gx[-1, :, -1, -1].isfinite().all()
+
+
 @pytest.mark.parametrize("batch,height,width,classes,dtype", [
     (3, 1, 90_000, 2562, BF),   # bf16: score gradients of more than one piece, whole images and part of one
     (1, 1, 250_000, 2562, BF),
@@ -100,6 +148,9 @@ def test_more_than_the_workspace_holds(ops, layout, batch, height, width, classe
     loss, saved = ops.cross_entropy_forward(x, weight, bias, target, -100, False)
     gx, gw, gb = ops.cross_entropy_backward(grad, saved, x, weight, bias, target, -100, False)
     total, w_sum, b_sum, u = 0.0, 0.0, 0.0, torch.finfo(dtype).eps / 2
+    # float32: the whole takes the tensor cores, its parts may not; the exponentials and logarithms of either are within 2^-19
+    # (step_reference), and so are a pixel's loss, its probabilities and what is made of them
+    apart = 2 * 2.0 ** -19 if dtype == F32 else 0.0
     for i in range(batch):
         for k in range(0, width, 30_000):
             part = x[i:i + 1, :, :, k:k + 30_000]
@@ -108,10 +159,10 @@ def test_more_than_the_workspace_holds(ops, layout, batch, height, width, classe
             one, kept = ops.cross_entropy_forward(part, weight, bias, some, -100, False)
             px, pw, pb = ops.cross_entropy_backward(grad, kept, part, weight, bias, some, -100, False)
             # (tiles of another width: other orders of the sums)
-            assert (gx[i:i + 1, :, :, k:k + 30_000].double() - px).norm() <= 2 * u * px.double().norm()
+            assert (gx[i:i + 1, :, :, k:k + 30_000].double() - px).norm() <= (2 * u + apart) * px.double().norm()
             total, w_sum, b_sum = total + one.double(), w_sum + pw.double(), b_sum + pb.double()
     n = batch * ((width + 29_999) // 30_000)
-    assert abs(loss.item() - total.item()) <= (n + 1) * 2.0 ** -24 * total.item()
+    assert abs(loss.item() - total.item()) <= ((n + 1) * 2.0 ** -24 + apart) * total.item()
     # the parts' sums are rounded n times, the whole once; their elements do not cancel more than the parts' sizes say
     for whole, parts in ((gw, w_sum), (gb, b_sum)):
         assert (whole.double() - parts).norm() <= (n ** 0.5 + 1) * 2 * u * parts.norm() + 2.0 ** -18 * parts.norm()
