@@ -23,7 +23,6 @@ using mix::View;
 // rows of channels where it lies in another way (bf16).
 constexpr size_t KEPT_HEAD = 256;
 constexpr size_t PIECE = 256u << 20;     // bytes of scores or gz at a time, CUDA cores
-constexpr double FLOATS_FROM = 1e8;      // products from which float32 layers take the tensor cores
 constexpr int FEW = 128;                 // classes that the CUDA-core kernels keep in registers
 constexpr size_t PIECE_TC = 1024u << 20; // bytes of gz at a time, tensor cores
 constexpr int THREADS = 256;
@@ -232,38 +231,48 @@ __global__ void __launch_bounds__(THREADS) labelled_rows_kernel(const uint4* src
 // n pixels of images of S pixels, wherever they lie -> rows of three bf16 parts of float32 values, 8 bits each, zeros behind the last
 // channel of a part of Cp; pixels without a label are zeros if lse is given.  (An infinity would leave NaN in the lower parts: they
 // are zero there.)
+// A block takes 32 pixels x 64 channels, eight values to a thread either way (one at a time: 40 us instead of 15 for 131 072 pixels of
+// 50 channels).
 __global__ void __launch_bounds__(THREADS) parts_kernel(const float* __restrict__ src, long long S, long long img, long long pix,
                                                         long long ch, long long p1, long long n, int C, int Cp,
                                                         const float* __restrict__ lse, bf16* __restrict__ dst) {
-  __shared__ float tile[32][33];
-  // 32 pixels x 32 channels, read along whichever direction is contiguous
-  const int tx = threadIdx.x % 32, ty = threadIdx.x / 32;
+  __shared__ float tile[32][65];
+  const int tx = threadIdx.x % 32, ty = threadIdx.x / 32, c0 = blockIdx.y * 64;
   const long long p0 = blockIdx.x * 32ll;
-  for (int c0 = blockIdx.y * 32; c0 < Cp; c0 += gridDim.y * 32) {
-    __syncthreads();
-    for (int k = ty; k < 32; k += THREADS / 32) {
-      const int r = ch == 1 ? k : tx, c = c0 + (ch == 1 ? tx : k);
-      const long long p = p0 + r;
-      float v = 0.f;
-      if (p < n && c < C && !(lse && lse[p] == INFINITY)) {
-        const long long b = (p1 + p) / S;
-        v = __ldg(src + b * img + (p1 + p - b * S) * pix + (long long)c * ch);
-      }
-      tile[r][ch == 1 ? tx : k] = v;
-    }
-    __syncthreads();
-    for (int k = ty; k < 32; k += THREADS / 32) {
-      if (p0 + k >= n || c0 + tx >= Cp) continue;
-      bf16* to = dst + (p0 + k) * 3 * Cp + c0 + tx;
-      float v = tile[k][tx];
+  const bool along = ch == 1;  // neighbouring threads read neighbouring channels, else pixels
+  float v[8];
+  if (along) {  // (one image)
 #pragma unroll
-      for (int part = 0; part < 3; ++part) {
-        const bf16 h = __float2bfloat16_rn(v);
-        to[part * Cp] = h;
-        const float f = __bfloat162float(h);
-        v = fabsf(f) < INFINITY ? v - f : 0.f;
-      }
+    for (int k = 0; k < 8; ++k) {
+      const int c = c0 + tx + 32 * (k / 4);
+      const long long p = p0 + ty + 8 * (k % 4);
+      v[k] = p < n && c < C && !(lse && lse[p] == INFINITY) ? __ldg(src + (p1 + p) * pix + c) : 0.f;
     }
+  } else {
+    const long long p = p0 + tx, b = (p1 + p) / S;
+    const bool on = p < n && !(lse && lse[p] == INFINITY);
+    const float* from = src + b * img + (p1 + p - b * S) * pix;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = on && c0 + ty + 8 * k < C ? __ldg(from + (c0 + ty + 8 * k) * ch) : 0.f;
+  }
+#pragma unroll
+  for (int k = 0; k < 8; ++k) tile[along ? ty + 8 * (k % 4) : tx][along ? tx + 32 * (k / 4) : ty + 8 * k] = v[k];
+  __syncthreads();
+  const int r = threadIdx.x / 8, c = threadIdx.x % 8 * 8;
+  if (p0 + r >= n) return;
+  bf16* to = dst + (p0 + r) * 3 * Cp + c0 + c;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) v[k] = tile[r][c + k];
+#pragma unroll
+  for (int part = 0; part < 3; ++part) {
+    __align__(16) bf16 h[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      h[k] = __float2bfloat16_rn(v[k]);
+      const float f = __bfloat162float(h[k]);
+      v[k] = fabsf(f) < INFINITY ? v[k] - f : 0.f;
+    }
+    *reinterpret_cast<uint4*>(to + part * Cp) = *reinterpret_cast<const uint4*>(h);
   }
 }
 
@@ -636,15 +645,19 @@ struct FloatCores {
   explicit FloatCores(const mc_ce_desc* desc)
       : d(desc), P(desc->B * desc->S), Cp((desc->C + 63) / 64 * 64), Vp((desc->V + 63) / 64 * 64) {}
   // Sums over classes are one MMA accumulator's, which truncates: up to 4096 classes stay within 2^-16 of a sum of one sign.
+  // Forward and backward together, us, tensor cores / CUDA cores: 131 072 pixels, classes x channels 13 x 64 236 / 195, 40 x 64 242 /
+  // 228, 99 x 50 278 / 314, 128 x 128 390 / 544; 40 962 pixels, 99 x 50 133 / 159, 300 x 96 236 / 468; 10 242 pixels, 99 x 50 90 /
+  // 88, 300 x 64 108 / 125, 700 x 128 155 / 336; 2 562 pixels, 99 x 50 79 / 83, 300 x 64 93 / 94.
   static bool takes(const mc_ce_desc* d) {
-    return d->dtype == MC_F32 && d->V <= 4096 && (double)d->B * d->S * d->V * d->C >= FLOATS_FROM;
+    const double each = (double)d->V * d->C;
+    return d->dtype == MC_F32 && d->V <= 4096 && each >= 4096 && each * d->B * d->S >= 1e8;
   }
   bool planes() const { return !(d->layout == MC_NHWC || d->S == 1) && d->C > 1; }
   mix::TcRows parts_of(const void* p, long long rows, int cols, int wide) const { return mix::TcRows{p, rows, cols, 3 * wide, 0, false, 3}; }
   static size_t bytes(long long rows, int wide) { return (size_t)rows * 3 * wide * 2; }
   void split(const float* src, long long S, long long img, long long pix, long long ch, long long p1, long long n, int C, int wide,
              const float* lse, void* dst, cudaStream_t st) const {
-    const dim3 tiles((unsigned)((n + 31) / 32), (unsigned)((wide + 31) / 32 < 64 ? (wide + 31) / 32 : 64));
+    const dim3 tiles((unsigned)((n + 31) / 32), (unsigned)(wide / 64));
     parts_kernel<<<tiles, THREADS, 0, st>>>(src, S, img, pix, ch, p1, n, C, wide, lse, (bf16*)dst), MC_COUNT(1);
   }
   void split_pixels(const float* x, long long p, long long n, const float* lse, void* dst, cudaStream_t st) const {

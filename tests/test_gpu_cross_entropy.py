@@ -84,7 +84,7 @@ def test_several_pieces(ops, pixels, classes, dtype):
     R.check(dict(loss=loss, **got), R.cross_entropy(x, weight, bias, target, -100, True, grad), "pieces")
 
 
-# float32 layers of 10^8 products and more (tensor cores, three bf16 parts of every value): odd counts, one block of channels or
+# float32 layers of 10^8 products and more (from 4096 weights on: tensor cores, three bf16 parts of every value): odd counts, one block of channels or
 # classes and one more, one image or several
 MANY = [(3, 67, 101, 77, 99), (1, 1, 40962, 64, 64), (2, 1, 10242, 65, 129), (1, 130, 129, 128, 257), (5, 33, 40, 10, 2562), (1, 1, 600, 200, 1000),
         (1, 300, 400, 1, 1000), (7, 1, 2562, 130, 63)]
@@ -136,7 +136,9 @@ def test_float32_of_many_products(ops, i, layout):
     (3, 1, 90_000, 2562, BF),   # bf16: score gradients of more than one piece, whole images and part of one
     (1, 1, 250_000, 2562, BF),
     (2, 1, 300_000, 130, F32),  # float32: scores of more than one piece
-    (3, 1, 200_000, 100, F32)])
+    (3, 1, 200_000, 100, F32),
+    (2, 1, 300_000, 640, F32),  # and on the tensor cores
+    (3, 1, 100_000, 640, F32)])
 @pytest.mark.parametrize("layout", ["nhwc", "nchw"])
 def test_more_than_the_workspace_holds(ops, layout, batch, height, width, classes, dtype):
     """bf16: a gigabyte of score gradients at a time; float32: a quarter of one.  Checked against the same call in parts."""
