@@ -645,12 +645,13 @@ struct FloatCores {
   explicit FloatCores(const mc_ce_desc* desc)
       : d(desc), P(desc->B * desc->S), Cp((desc->C + 63) / 64 * 64), Vp((desc->V + 63) / 64 * 64) {}
   // Sums over classes are one MMA accumulator's, which truncates: up to 4096 classes stay within 2^-16 of a sum of one sign.
-  // Forward and backward together, us, tensor cores / CUDA cores: 131 072 pixels, classes x channels 13 x 64 236 / 195, 40 x 64 242 /
-  // 228, 99 x 50 278 / 314, 128 x 128 390 / 544; 40 962 pixels, 99 x 50 133 / 159, 300 x 96 236 / 468; 10 242 pixels, 99 x 50 90 /
-  // 88, 300 x 64 108 / 125, 700 x 128 155 / 336; 2 562 pixels, 99 x 50 79 / 83, 300 x 64 93 / 94.
+  // Forward and backward together, us, tensor cores / CUDA cores: 131 072 pixels, classes x channels 13 x 64 202 / 195, 40 x 64 204 /
+  // 228, 99 x 50 246 / 314, 128 x 128 324 / 544; 40 962 pixels, 13 x 64 101 / 102, 40 x 64 103 / 116, 99 x 50 120 / 159, 300 x 96 216 /
+  // 468; 10 242 pixels, 40 x 32 72 / 55, 99 x 50 82 / 88, 300 x 64 101 / 125, 700 x 128 143 / 336; 2 562 pixels, 99 x 50 75 / 83,
+  // 300 x 64 85 / 94; 1 000 pixels, 40 x 64 71 / 67; 327 684 pixels, 20 x 32 435 / 308.
   static bool takes(const mc_ce_desc* d) {
     const double each = (double)d->V * d->C;
-    return d->dtype == MC_F32 && d->V <= 4096 && each >= 4096 && each * d->B * d->S >= 1e8;
+    return d->dtype == MC_F32 && d->V <= 4096 && each >= 2048 && each * d->B * d->S >= 1e7;
   }
   bool planes() const { return !(d->layout == MC_NHWC || d->S == 1) && d->C > 1; }
   mix::TcRows parts_of(const void* p, long long rows, int cols, int wide) const { return mix::TcRows{p, rows, cols, 3 * wide, 0, false, 3}; }

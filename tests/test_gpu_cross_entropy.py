@@ -84,10 +84,28 @@ def test_several_pieces(ops, pixels, classes, dtype):
     R.check(dict(loss=loss, **got), R.cross_entropy(x, weight, bias, target, -100, True, grad), "pieces")
 
 
-# float32 layers of 10^8 products and more (from 4096 weights on: tensor cores, three bf16 parts of every value): odd counts, one block of channels or
+# float32 layers of 10^7 products and more (from 2048 weights on: tensor cores, three bf16 parts of every value): odd counts, one block of channels or
 # classes and one more, one image or several
 MANY = [(3, 67, 101, 77, 99), (1, 1, 40962, 64, 64), (2, 1, 10242, 65, 129), (1, 130, 129, 128, 257), (5, 33, 40, 10, 2562), (1, 1, 600, 200, 1000),
         (1, 300, 400, 1, 1000), (7, 1, 2562, 130, 63)]
+
+
+# bf16: tiles of 64, 128 and 256 classes whose weights stay in shared memory, or travel beside several tiles of classes
+WIDE = [(1, 1, 60_001, 40, 13), (3, 100, 203, 64, 99), (1, 1, 45_000, 256, 250), (2, 1, 30_001, 320, 70), (1, 150, 400, 24, 300), (5, 1, 10_242, 96, 129)]
+
+
+@pytest.mark.parametrize("layout", ["nhwc", "nchw"])
+@pytest.mark.parametrize("i", range(len(WIDE)))
+def test_many_pixels(ops, i, layout):
+    b, h, w, cin, classes = WIDE[i]
+    g = torch.Generator("cuda").manual_seed(70 + i)
+    x = image(g, (b, cin, h, w), BF, layout)
+    weight, bias = classifier(g, classes, cin, BF)
+    target = labels(g, (b, h, w), classes, 0.2)
+    grad = torch.tensor(2.5, device="cuda")
+    loss, saved = ops.cross_entropy_forward(x, weight, bias, target)
+    got = dict(zip(("gx", "gw", "gb"), ops.cross_entropy_backward(grad, saved, x, weight, bias, target)))
+    R.check(dict(loss=loss, **got), R.cross_entropy(x, weight, bias, target, -100, True, grad), str(WIDE[i]))
 
 
 @pytest.mark.parametrize("layout", ["nhwc", "nchw"])
