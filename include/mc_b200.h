@@ -503,7 +503,9 @@ int mc_group_norm_bwd(const mc_norm_desc* d, const void* gy, const void* x, cons
  * ignore_index makes the loss and the gradients that its pixel takes part in NaN.
  * saved: mc_cross_entropy_saved_bytes of memory that the forward call fills and the backward call reads; ws: scratch, phases
  * MC_PHASE_FORWARD and MC_PHASE_BACKWARD; both 16-byte aligned.  Any of the gradients may be NULL.  Scores, softmax sums and gradients of
- * parameters are summed in float32 (MC_F64: double), the loss in double, all in a fixed order.
+ * parameters are summed in float32 (MC_F64: double), the loss in double, all in a fixed order.  For MC_BF16 products are the
+ * tensor cores' (sums lose up to 2^-23 per sixteen terms) and gradients of scores are rounded to bf16; MC_F32 may take the tensor
+ * cores in three bf16 parts of every value, within float32's own errors.
  * Limits: B * S <= 2^31 - 256, C and V <= 2^20, C * V <= 2^31. */
 enum { MC_REDUCE_SUM = 0, MC_REDUCE_MEAN = 1 };
 typedef struct mc_ce_desc {

@@ -644,14 +644,16 @@ struct FloatCores {
   const int Cp, Vp;
   explicit FloatCores(const mc_ce_desc* desc)
       : d(desc), P(desc->B * desc->S), Cp((desc->C + 63) / 64 * 64), Vp((desc->V + 63) / 64 * 64) {}
-  // Sums over classes are one MMA accumulator's, which truncates: up to 4096 classes stay within 2^-16 of a sum of one sign.
+  // Sums over channels and over classes are one accumulator's, which truncates up to 2^-23 of what it holds for every sixteen: up to
+  // 1024 channels (scores within 2^-17 of their terms, whose differences the exponential takes) and 4096 classes (2^-15 of a sum of
+  // one sign).  2^20 channels: a loss 7e-4 off.
   // Forward and backward together, us, tensor cores / CUDA cores: 131 072 pixels, classes x channels 13 x 64 202 / 195, 40 x 64 204 /
   // 228, 99 x 50 246 / 314, 128 x 128 324 / 544; 40 962 pixels, 13 x 64 101 / 102, 40 x 64 103 / 116, 99 x 50 120 / 159, 300 x 96 216 /
   // 468; 10 242 pixels, 40 x 32 72 / 55, 99 x 50 82 / 88, 300 x 64 101 / 125, 700 x 128 143 / 336; 2 562 pixels, 99 x 50 75 / 83,
   // 300 x 64 85 / 94; 1 000 pixels, 40 x 64 71 / 67; 327 684 pixels, 20 x 32 435 / 308.
   static bool takes(const mc_ce_desc* d) {
     const double each = (double)d->V * d->C;
-    return d->dtype == MC_F32 && d->V <= 4096 && each >= 2048 && each * d->B * d->S >= 1e7;
+    return d->dtype == MC_F32 && d->C <= 1024 && d->V <= 4096 && each >= 2048 && each * d->B * d->S >= 1e7;
   }
   bool planes() const { return !(d->layout == MC_NHWC || d->S == 1) && d->C > 1; }
   mix::TcRows parts_of(const void* p, long long rows, int cols, int wide) const { return mix::TcRows{p, rows, cols, 3 * wide, 0, false, 3}; }
@@ -668,6 +670,7 @@ struct FloatCores {
 
   int forward(mix::Work& k, const float* x, const float* w, const float* bias, const int64_t* target, float* loss, char* kept) const {
     long long piece = (long long)(PIECE_TC / ((size_t)((d->V + 63) / 64) * 8 + bytes(1, Cp))) / 256 * 256;
+    if (piece < 256) piece = 256;
     if (piece > P) piece = P;
     const long long last = (P - 1) % piece + 1, pieces = (P + piece - 1) / piece;
     const auto tiles = [&](long long n) { return mix::tc_scores_tiles(n, d->C, d->V, 3); };
@@ -703,6 +706,7 @@ struct FloatCores {
     // pieces of pixels: whole images, or part of one, where the output lies in planes
     const long long S = planes() ? d->S : P, B = planes() ? d->B : 1;
     long long most = (long long)(PIECE_TC / (bytes(1, Vp) + bytes(1, Cp))) / 256 * 256;
+    if (most < 256) most = 256;
     const long long run = most < S ? most : S, images = most < S ? 1 : most / S < B ? most / S : B;
     most = images * run;
     const auto each = [&](auto f) {

@@ -86,7 +86,7 @@ def test_several_pieces(ops, pixels, classes, dtype):
 
 # float32 layers of 10^7 products and more (from 2048 weights on: tensor cores, three bf16 parts of every value): odd counts, one block of channels or
 # classes and one more, one image or several
-MANY = [(3, 67, 101, 77, 99), (1, 1, 40962, 64, 64), (2, 1, 10242, 65, 129), (1, 130, 129, 128, 257), (5, 33, 40, 10, 2562), (1, 1, 600, 200, 1000),
+MANY = [(2, 1, 3, 1 << 20, 20), (3, 67, 101, 77, 99), (1, 1, 40962, 64, 64), (2, 1, 10242, 65, 129), (1, 130, 129, 128, 257), (5, 33, 40, 10, 2562), (1, 1, 600, 200, 1000),
         (1, 300, 400, 1, 1000), (7, 1, 2562, 130, 63)]
 
 
@@ -129,9 +129,11 @@ def test_float32_of_many_products(ops, i, layout):
         assert layout_kept(results[-1][1], layout)
         assert all(torch.equal(p, q) for p, q in zip(results[0], results[-1]))
     R.check(dict(zip(("loss", "gx", "gw", "gb"), results[0])), want, str(MANY[i]))
-    # as near as float32 sums are: relative errors of whole tensors
+    # as near as float32 sums are: relative errors of whole tensors.  (A float32 sum of n channels is a random walk of n roundings:
+    # sqrt(n) 2^-24 of the scores, which exponentials pass on as relative errors; below 5e-6 for all but 2^20 channels.)
+    near = max(5e-6, cin ** 0.5 * 2.0 ** -24)
     for got, name in zip(results[0], ("loss", "gx", "gw", "gb")):
-        assert (got.double() - want[name][0]).norm() <= 5e-6 * want[name][0].norm(), name
+        assert (got.double() - want[name][0]).norm() <= near * want[name][0].norm(), name
     only_x = ops.cross_entropy_backward(grad, saved, x, weight, bias, target, -100, mean, True, False)
     only_w = ops.cross_entropy_backward(grad, saved, x, weight, bias, target, -100, mean, False, True)
     assert torch.equal(only_x[0], results[0][1]) and torch.equal(only_w[1], results[0][2])
