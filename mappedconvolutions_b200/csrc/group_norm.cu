@@ -374,7 +374,9 @@ __device__ __forceinline__ void walk_two(const Span& s, const T* x, const T* gy,
     fetch(r, i);
   }
 }
-constexpr int ONE = 4, BOTH = 2;  // vectors on their way, of one tensor and of two
+// Vectors on their way, of one tensor and of two.  (2 and 1: 192 and 352 us for 64 x 10 242 x 256 bf16, 181 and 294 with these; of two
+// tensors 2: 300 us, and 236 instead of 194 for 32 x 100 x 200 x 128 in groups of four channels.)
+constexpr int ONE = 4, BOTH = 4;
 template <typename T, int ACT, typename CT, int N>
 __device__ __forceinline__ void output(const Args& a, const Coefs<T, CT, N>& k, CT (&v)[N]) {
   add_to(v, v, k.neg_mean);
