@@ -9,9 +9,11 @@
 // bf16 (tensor cores): the scores of 256 pixels x up to 256 classes stand in TMEM; the forward call keeps their largest and the
 // sum of their exponentials, the backward call computes them again, rounds gz to bf16 - which the next two products' operand is -
 // and multiplies it, a piece of the pixels at a time.
-// float32 and float64 (CUDA cores), with the kernels of the channel-mixing layers: up to 128 classes stand in a block's registers, whose
-// threads add up the softmax; scores of more classes go through the workspace, a piece of the pixels at a time.  Bound: the
-// products (FMA issue).
+// float32 with many products (tensor cores): the same kernels on three bf16 parts of every value, six products of parts for one
+// (FloatCores below has the rule and both sides measured).  Bound: the products; the parts' copies where channels are few.
+// float64, and float32 otherwise (CUDA cores), with the kernels of the channel-mixing layers: up to 128 classes stand in a block's
+// registers, whose threads add up the softmax; scores of more classes go through the workspace, a piece of the pixels at a time.
+// Bound: the products (FMA issue).
 #include "mix_work.cuh"
 
 namespace mc {
@@ -269,7 +271,8 @@ __global__ void __launch_bounds__(THREADS) parts_kernel(const float* __restrict_
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
       h[k] = __float2bfloat16_rn(v[k]);
-      const float f = __bfloat162float(h[k]);
+      float f = __bfloat162float(h[k]);
+      if (fabsf(f) == INFINITY && fabsf(v[k]) < INFINITY) h[k] = __float2bfloat16_rz(v[k]), f = __bfloat162float(h[k]);  // (largest values)
       v[k] = fabsf(f) < INFINITY ? v[k] - f : 0.f;
     }
     *reinterpret_cast<uint4*>(to + part * Cp) = *reinterpret_cast<const uint4*>(h);

@@ -270,6 +270,24 @@ def test_large_scores_and_classes_ruled_out(ops, dtype):
     assert loss.isnan()
 
 
+def test_largest_weights_in_parts(ops):
+    """float32 values that bf16 would round to infinity"""
+    g = torch.Generator("cuda").manual_seed(27)
+    x = image(g, (2, 40, 50, 60), F32, "nchw")
+    x[:, 5] = 2.0 ** -120
+    weight, bias = classifier(g, 130, 40, F32)
+    weight[:, 5] = 0
+    weight[::7, 5], weight[3::7, 5] = torch.finfo(F32).max, -torch.finfo(F32).max
+    target = labels(g, (2, 50, 60), 130, 0.2)
+    grad = torch.tensor(1.0, device="cuda")
+    loss, saved = ops.cross_entropy_forward(x, weight, bias, target)
+    gx, gw, gb = ops.cross_entropy_backward(grad, saved, x, weight, bias, target)
+    want = R.cross_entropy(x, weight, bias, target, -100, True, grad)
+    rest = torch.arange(40, device="cuda") != 5  # (that channel's weight gradients are below what float32 holds)
+    want["gw"] = tuple(v[:, rest] for v in want["gw"])
+    R.check(dict(loss=loss, gx=gx, gw=gw[:, rest], gb=gb), want, "largest")
+
+
 def test_refusals(ops):
     x = torch.zeros(2, 6, 4, 5, device="cuda")
     w, b, t = torch.zeros(9, 6, 1, device="cuda"), torch.zeros(9, device="cuda"), torch.zeros(2, 4, 5, dtype=torch.int64, device="cuda")
