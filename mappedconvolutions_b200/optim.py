@@ -9,7 +9,7 @@ class AdamW(torch.optim.Optimizer):
 
     state_bits: 32, moments in float32 (float64 for float64 parameters), or 8, moments as 8-bit codes with a float32 scale for
     256 elements each: 2 bytes per element instead of 8.  master_weights: bfloat16 parameters keep a float32 copy that the steps
-    are taken on.  Parameters are float32, bfloat16 or float64 CUDA tensors, each dense in any order of its dimensions.
+    are taken on, so that a value written into such a parameter between steps lasts until the next one.  Parameters are float32, bfloat16 or float64 CUDA tensors, each dense in any order of its dimensions.
 
     state[p]: "step" (a number), "exp_avg" and "exp_avg_sq" - with 8 bits int8 and uint8 codes, "exp_avg_scale" and
     "exp_avg_sq_scale" -, and "master" where there is one.  moments() gives the values.  Step counts are kept on the host: a step
@@ -17,18 +17,25 @@ class AdamW(torch.optim.Optimizer):
     """
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, *, state_bits=32, master_weights=False):
-        if not lr >= 0:
-            raise ValueError("lr must not be negative: %r" % (lr,))
-        if not all(0 <= b < 1 for b in betas) or len(betas) != 2:
-            raise ValueError("betas must be two numbers in [0, 1): %r" % (betas,))
-        if not eps >= 0:
-            raise ValueError("eps must not be negative: %r" % (eps,))
-        if not weight_decay >= 0:
-            raise ValueError("weight_decay must not be negative: %r" % (weight_decay,))
-        if state_bits not in (8, 32):
-            raise ValueError("state_bits must be 8 or 32: %r" % (state_bits,))
         super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay, state_bits=state_bits,
                                       master_weights=bool(master_weights)))
+
+    def add_param_group(self, param_group):
+        self._check_options({**self.defaults, **param_group})
+        super().add_param_group(param_group)
+
+    @staticmethod
+    def _check_options(group):
+        for name in ("lr", "eps", "weight_decay"):
+            if not group[name] >= 0:
+                raise ValueError("%s must not be negative: %r" % (name, group[name]))
+        if len(group["betas"]) != 2 or not all(0 <= b < 1 for b in group["betas"]):
+            raise ValueError("betas must be two numbers in [0, 1): %r" % (group["betas"],))
+        if group.get("state_bits", 32) not in (8, 32):
+            raise ValueError("state_bits must be 8 or 32: %r" % (group["state_bits"],))
+        for name in ("amsgrad", "maximize"):
+            if group.get(name):
+                raise ValueError("%s is not supported" % name)
 
     def __setstate__(self, state):
         super().__setstate__(state)
@@ -102,6 +109,8 @@ class AdamW(torch.optim.Optimizer):
 
     def load_state_dict(self, state_dict):
         """torch's, but every tensor of the state keeps its own type (torch would cast moments to the parameter's)."""
+        for group in state_dict["param_groups"]:
+            self._check_options(group)
         super().load_state_dict(state_dict)
         ids = [i for group in state_dict["param_groups"] for i in group["params"]]
         params = [p for group in self.param_groups for p in group["params"]]

@@ -42,6 +42,26 @@ def test_argument_checks():
             optim.AdamW(p, **bad)
 
 
+def test_options_of_groups_and_loaded_states():
+    p, q = torch.nn.Parameter(torch.zeros(3)), torch.nn.Parameter(torch.zeros(4))
+    opt = optim.AdamW([p])
+    for bad in (dict(state_bits=16), dict(betas=(0.9, 1.0)), dict(lr=-1.0), dict(amsgrad=True), dict(maximize=True)):
+        with pytest.raises(ValueError):
+            opt.add_param_group(dict(params=[q], **bad))
+        with pytest.raises(ValueError):
+            optim.AdamW([dict(params=[q], **bad)])
+    assert len(opt.param_groups) == 1
+    opt.add_param_group(dict(params=[q], state_bits=8, lr=0.5))
+    assert opt.param_groups[1]["state_bits"] == 8 and opt.param_groups[0]["state_bits"] == 32
+    for name in ("amsgrad", "maximize"):  # a state whose next step is another one
+        other = torch.optim.AdamW([p], lr=0.25, **{name: True})
+        with pytest.raises(ValueError, match=name):
+            optim.AdamW([p]).load_state_dict(other.state_dict())
+    opt = optim.AdamW([p])
+    opt.load_state_dict(torch.optim.AdamW([p], lr=0.25).state_dict())
+    assert opt.param_groups[0]["lr"] == 0.25 and opt.param_groups[0]["state_bits"] == 32
+
+
 @pytest.mark.parametrize("ops", [twin] + ([host.impl] if host.COMPILED else []), ids=["ctypes", "compiled"][:1 + host.COMPILED])
 def test_no_cpu_path(ops):
     x, one, t = torch.zeros(1, 6, 4, 5), torch.ones(6), torch.zeros(1, 4, 5, dtype=torch.int64)
