@@ -187,6 +187,13 @@ enum Mode {
 constexpr int PRODUCTS = 6;
 __device__ __forceinline__ int part_a(int product) { return 0x052 >> 2 * product & 3; }
 __device__ __forceinline__ int part_b(int product) { return 0x118 >> 2 * product & 3; }
+// Where the second operand stays in shared memory with all its parts, the first one passes four times, not six: part 2 for (2,0), 1 for
+// (1,1) (1,0), 0 for (0,2) (0,1), and 0 again for (0,0), which comes last as before.  (Input gradient of 131 072 pixels, 99 -> 50: 46 us
+// with six, 34.6 with four; the two kernels that read scores out, 29 -> 28 and 49 -> 48.)
+constexpr int PASSES = 4;
+__device__ __forceinline__ int pass_a(int pass) { return 0x06 >> 2 * pass & 3; }
+__device__ __forceinline__ int pass_b(int pass) { return 0x24 >> 2 * pass & 3; }  // of the first product
+__device__ __forceinline__ bool pass_twice(int pass) { return pass == 1 || pass == 2; }  // the next smaller number is the second's
 // BN: channels of a tile.  It is staged CW channels (128 or 64 swizzled bytes a row) at a time; the two results of
 // GATE_BWD side by side, in smaller tiles because its weights leave little room.
 template <int MODE, int BN> struct Cfg {
@@ -211,6 +218,7 @@ struct alignas(64) GemmArgs {
   int m_pairs, rows; // pairs of tiles; pixels
   int a_across[2], y_across;  // blocks next to each other where a tensor lies in blocks, else 0
   int per;           // stages of a product of parts where operands are in parts, else 0
+  int kw;            // stages of b[0] that stay
   float* floats;     // FLOATS: y, rows of ld values or (ld == 0) planes
   long long ld;
   int n_tiles, N, kb[2], act;
@@ -612,6 +620,7 @@ __device__ __forceinline__ void read_floats(const GemmArgs& g, int set, uint32_t
 template <int MODE, int BN>
 __global__ void __launch_bounds__(THREADS, 1) rows_tc_kernel(const __grid_constant__ GemmArgs g) {
   typedef Cfg<MODE, BN> C;
+  constexpr bool PARTS = MODE == SCORE_SUM || MODE == SCORE_GRAD || MODE == FLOATS;  // can come in parts
   extern __shared__ unsigned char raw[];
   __shared__ volatile int abort_flag_s;
   unsigned char* sm = (unsigned char*)(((uintptr_t)raw + 1023) & ~(uintptr_t)1023);
@@ -620,7 +629,7 @@ __global__ void __launch_bounds__(THREADS, 1) rows_tc_kernel(const __grid_consta
   const uint32_t out0 = smem_u32(sm);
   const uint32_t a0 = out0 + (2 << C::SLOT_BITS) * C::CH_BYTES;
   const uint32_t b0 = a0 + g.stages * A_BYTES;
-  const uint32_t btile = g.kb[0] * C::B0 + g.kb[1] * C::B1;  // a channel tile's weights
+  const uint32_t btile = g.kw * C::B0 + g.kb[1] * C::B1;  // a channel tile's weights
   const int bbytes = g.group ? g.group * btile : g.stages * C::BMAX;
   const uint32_t rank = cluster_rank();
   float* bias_s = (float*)(sm + (b0 - out0) + bbytes);  // two tiles' worth per set
@@ -672,8 +681,8 @@ __global__ void __launch_bounds__(THREADS, 1) rows_tc_kernel(const __grid_consta
       uint32_t dst = b0;
       for (int n = 0; n < g.group; ++n)
         for (int seg = 0; seg < 2; ++seg)
-          for (int k = 0; k < g.kb[seg]; ++k) {
-            load_b<MODE, BN>(g, seg, rank, dst, (g.per ? part_b(k / g.per) * g.per + k % g.per : k) * KB, (w.base + n) * BN, bar);
+          for (int k = 0; k < (seg ? g.kb[1] : g.kw); ++k) {
+            load_b<MODE, BN>(g, seg, rank, dst, k * KB, (w.base + n) * BN, bar);
             dst += seg ? C::B1 : C::B0;
           }
     }
@@ -691,7 +700,8 @@ __global__ void __launch_bounds__(THREADS, 1) rows_tc_kernel(const __grid_consta
             if (rank == 0) mbar_expect_tx(full(st), 2 * (A_BYTES + (g.group ? 0 : seg ? C::B1 : C::B0)));
             const int across = g.a_across[seg];
             int ka = k, kb = k;
-            if (g.per) ka = part_a(k / g.per) * g.per + k % g.per, kb = part_b(k / g.per) * g.per + k % g.per;
+            if (g.per && g.group) ka = pass_a(k / g.per) * g.per + k % g.per;
+            else if (g.per) ka = part_a(k / g.per) * g.per + k % g.per, kb = part_b(k / g.per) * g.per + k % g.per;
             tma_load_pair(a0 + st * A_BYTES, &g.a[seg], across ? 0 : ka * KB, across ? m0 * across + ka * TILE : m0, bar);
             if (!g.group) load_b<MODE, BN>(g, seg, rank, b0 + st * C::BMAX, kb * KB, n0, bar);
           }
@@ -727,21 +737,31 @@ __global__ void __launch_bounds__(THREADS, 1) rows_tc_kernel(const __grid_consta
           constexpr uint32_t HI = desc_sw128_hi(1024);
           const uint32_t idesc = make_idesc_bf16(2 * TILE, seg ? C::N1 : C::N0, 0, 0);
           const uint32_t d = acc * C::ACC + (seg ? C::OFF1 : 0);
+          int pass = 0, kp = 0;  // of the first operand, where it passes several times; stage of the pass
           for (int k = 0; k < g.kb[seg]; ++k) {
             if (!there) {
               ok = __all_sync(~0u, mbar_wait(full(st), ph, abort_flag, 0x113));
               if (!ok) break;
             }
-            const uint32_t cur = st, ad = a_lo + st * (A_BYTES >> 4), bd = g.group ? bres : b_lo + st * (C::BMAX >> 4);
+            const bool passes = PARTS && g.per && g.group;
+            const uint32_t cur = st, ad = a_lo + st * (A_BYTES >> 4);
+            const uint32_t bd = !g.group ? b_lo + st * (C::BMAX >> 4)
+                                         : passes ? bres + (pass_b(pass) * g.per + kp) * (C::B0 >> 4) : bres;
             if (++st == (uint32_t)g.stages) st = 0, ph ^= 1;
             const bool next = mbar_test(full(st), ph);
             if (elected) {
 #pragma unroll
               for (int j = 0; j < 4; ++j)  // sixteen channels, 32 bytes each
                 pair_mma(d, ad + 2 * j, HI, bd + 2 * j, HI, idesc, (k | j) != 0 || (seg && C::OFF1 == 0));
+              if (passes && pass_twice(pass)) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                  pair_mma(d, ad + 2 * j, HI, bd - g.per * (C::B0 >> 4) + 2 * j, HI, idesc, true);
+              }
               pair_commit(empty(cur));
             }
-            bres += (seg ? C::B1 : C::B0) >> 4;
+            if (!passes) bres += (seg ? C::B1 : C::B0) >> 4;
+            else if (++kp == g.per) kp = 0, ++pass;
             there = __all_sync(~0u, next);
           }
           if (!ok) break;
@@ -1113,13 +1133,13 @@ struct RowsPlan {
   size_t smem;
 };
 template <int MODE, int BN>
-static RowsPlan plan_rows(int m_pairs, int N, int kb0, int kb1, int sms) {
+static RowsPlan plan_rows(int m_pairs, int N, int kb0, int kb1, int sms, int kw = 0) {  // kw: stages of the first weights that stay, if not kb0
   typedef Cfg<MODE, BN> C;
   RowsPlan p{};
   p.bn = BN;
   p.n_tiles = (N + BN - 1) / BN;
   const int fixed_bytes = 1024 + 4 * 256 * 4 + ROWS_BARS * 8 + 16 + 64;
-  const int b_tile = kb0 * C::B0 + kb1 * C::B1, pairs = sms / 2;
+  const int b_tile = (kw ? kw : kb0) * C::B0 + kb1 * C::B1, pairs = sms / 2;
   const int left = SMEM_LIMIT - fixed_bytes - (2 << C::SLOT_BITS) * C::CH_BYTES;
   // Weights stay in shared memory where at least three stages of pixels fit beside them.  us at 655 488 pixels, weights that
   // stay / that travel: without activation 96 -> 96 channels 63 / 70, 64 -> 64 49.6 / 50.4, 128 -> 256 114 / 113; ReLU and
@@ -1165,8 +1185,10 @@ static RowsPlan plan_rows(int m_pairs, int N, int kb0, int kb1, int sms) {
 
 template <int MODE, int BN>
 static int launch_rows(GemmArgs& g, cudaStream_t st) {
-  const RowsPlan p = plan_rows<MODE, BN>(g.m_pairs, g.N, g.kb[0], g.kb[1], sm_total());
+  const RowsPlan p = plan_rows<MODE, BN>(g.m_pairs, g.N, g.kb[0], g.kb[1], sm_total(), 3 * g.per);
   g.n_tiles = p.n_tiles, g.group = p.group, g.stages = p.stages;
+  g.kw = g.per ? 3 * g.per : g.kb[0];
+  if (g.per && g.group) g.kb[0] = PASSES * g.per;
   return launch_pairs<rows_tc_kernel<MODE, BN>>(p.pairs, p.smem, g, st);
 }
 
