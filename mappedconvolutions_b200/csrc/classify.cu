@@ -235,12 +235,26 @@ __global__ void __launch_bounds__(THREADS) labelled_rows_kernel(const uint4* src
 // are zero there.)
 // A block takes 32 pixels x 64 channels, eight values to a thread either way (one at a time: 40 us instead of 15 for 131 072 pixels of
 // 50 channels).
-__global__ void __launch_bounds__(THREADS) parts_kernel(const float* __restrict__ src, long long S, long long img, long long pix,
-                                                        long long ch, long long p1, long long n, int C, int Cp,
-                                                        const float* __restrict__ lse, bf16* __restrict__ dst) {
+// Up to three such jobs a launch: weights, their transposes and pixels.
+struct Split {
+  const float* src;
+  long long S, img, pix, ch, p1, n;
+  int C, Cp;
+  const float* lse;
+  bf16* dst;
+  unsigned blocks;
+};
+struct Splits { Split s[3]; };
+__global__ void __launch_bounds__(THREADS) parts_kernel(const __grid_constant__ Splits all) {
   __shared__ float tile[32][65];
-  const int tx = threadIdx.x % 32, ty = threadIdx.x / 32, c0 = blockIdx.y * 64;
-  const long long p0 = blockIdx.x * 32ll;
+  unsigned block = blockIdx.x;
+  int job = 0;
+  while (job < 2 && block >= all.s[job].blocks) block -= all.s[job++].blocks;
+  const Split& a = all.s[job];
+  const float *src = a.src, *lse = a.lse;
+  const long long S = a.S, img = a.img, pix = a.pix, ch = a.ch, p1 = a.p1, n = a.n;
+  const int C = a.C, Cp = a.Cp, tx = threadIdx.x % 32, ty = threadIdx.x / 32, c0 = block % (Cp / 64) * 64;
+  const long long p0 = block / (Cp / 64) * 32ll;
   const bool along = ch == 1;  // neighbouring threads read neighbouring channels, else pixels
   float v[8];
   if (along) {  // (one image)
@@ -262,7 +276,7 @@ __global__ void __launch_bounds__(THREADS) parts_kernel(const float* __restrict_
   __syncthreads();
   const int r = threadIdx.x / 8, c = threadIdx.x % 8 * 8;
   if (p0 + r >= n) return;
-  bf16* to = dst + (p0 + r) * 3 * Cp + c0 + c;
+  bf16* to = a.dst + (p0 + r) * 3 * Cp + c0 + c;
 #pragma unroll
   for (int k = 0; k < 8; ++k) v[k] = tile[r][c + k];
 #pragma unroll
@@ -661,14 +675,19 @@ struct FloatCores {
   bool planes() const { return !(d->layout == MC_NHWC || d->S == 1) && d->C > 1; }
   mix::TcRows parts_of(const void* p, long long rows, int cols, int wide) const { return mix::TcRows{p, rows, cols, 3 * wide, 0, false, 3}; }
   static size_t bytes(long long rows, int wide) { return (size_t)rows * 3 * wide * 2; }
-  void split(const float* src, long long S, long long img, long long pix, long long ch, long long p1, long long n, int C, int wide,
-             const float* lse, void* dst, cudaStream_t st) const {
-    const dim3 tiles((unsigned)((n + 31) / 32), (unsigned)(wide / 64));
-    parts_kernel<<<tiles, THREADS, 0, st>>>(src, S, img, pix, ch, p1, n, C, wide, lse, (bf16*)dst), MC_COUNT(1);
+  static Split job(const float* src, long long S, long long img, long long pix, long long ch, long long p1, long long n, int C, int wide,
+                   const float* lse, void* dst) {
+    return Split{src, S, img, pix, ch, p1, n, C, wide, lse, (bf16*)dst, (unsigned)((n + 31) / 32 * (wide / 64))};
   }
-  void split_pixels(const float* x, long long p, long long n, const float* lse, void* dst, cudaStream_t st) const {
-    if (planes()) split(x, d->S, d->S * d->C, 1, d->S, p, n, d->C, Cp, lse, dst, st);
-    else split(x, P, P * d->C, d->C, 1, p, n, d->C, Cp, lse, dst, st);
+  Split pixels(const float* x, long long p, long long n, const float* lse, void* dst) const {
+    if (planes()) return job(x, d->S, d->S * d->C, 1, d->S, p, n, d->C, Cp, lse, dst);
+    return job(x, P, P * d->C, d->C, 1, p, n, d->C, Cp, lse, dst);
+  }
+  Split weights(const float* w, void* dst) const { return job(w, d->V, 0, d->C, 1, 0, d->V, d->C, Cp, nullptr, dst); }
+  Split transposed(const float* w, void* dst) const { return job(w, d->C, 0, 1, d->C, 0, d->C, d->V, Vp, nullptr, dst); }
+  static int split(const Splits& s, cudaStream_t st) {
+    parts_kernel<<<s.s[0].blocks + s.s[1].blocks + s.s[2].blocks, THREADS, 0, st>>>(s), MC_COUNT(1);
+    return cudaGetLastError() == cudaSuccess ? MC_OK : MC_ERR_LAUNCH;
   }
 
   int forward(mix::Work& k, const float* x, const float* w, const float* bias, const int64_t* target, float* loss, char* kept) const {
@@ -686,11 +705,11 @@ struct FloatCores {
     s.hit = (float*)k.take((size_t)piece * 4);
     double* part = (double*)k.take((size_t)pieces * SUM_BLOCKS * 16);
     if (!k.run()) return k.rc;
-    split(w, d->V, 0, d->C, 1, 0, d->V, d->C, Cp, nullptr, w3, k.st);
     int blocks = 0;
     for (long long p = 0; p < P; p += piece) {
       const long long n = P - p < piece ? P - p : piece;
-      split_pixels(x, p, n, nullptr, x3, k.st);
+      k.did(split(Splits{{pixels(x, p, n, nullptr, x3), p ? Split{} : weights(w, w3)}}, k.st));
+      if (k.rc) return k.rc;
       s.target = target + p;
       k.did(mix::tc_scores_sum(parts_of(x3, n, d->C, Cp), parts_of(w3, d->V, d->C, Cp), nullptr, s, k.st));
       if (k.rc) return k.rc;
@@ -737,12 +756,11 @@ struct FloatCores {
     if (!k.run()) return k.rc;
     const long long threads = (long long)d->V * (ldn / 4) + d->V;
     const float* lse = (const float*)(kept + KEPT_HEAD);
-    split(w, d->V, 0, d->C, 1, 0, d->V, d->C, Cp, nullptr, w3, k.st);
-    if (gx) split(w, d->C, 0, 1, d->C, 0, d->C, d->V, Vp, nullptr, wt3, k.st);
     each([&](long long i, long long s, long long n) {
       if (k.rc) return;
       const long long p = i * S + s;
-      split_pixels(x, p, n, lse + p, x3, k.st);
+      k.did(split(Splits{{pixels(x, p, n, lse + p, x3), p ? Split{} : weights(w, w3), p || !gx ? Split{} : transposed(w, wt3)}}, k.st));
+      if (k.rc) return;
       mix::Scores sc{target + p, d->ignore_index, nullptr, nullptr, lse + p, grad,
                      d->reduction == MC_REDUCE_MEAN ? (const double*)kept : nullptr, bias};
       const mix::TcRows xp = parts_of(x3, n, d->C, Cp), gp{gz.p, n, d->V, 64, 0, true, 3};
