@@ -664,13 +664,14 @@ struct FloatCores {
   // Sums over channels and over classes are one accumulator's, which truncates up to 2^-23 of what it holds for every sixteen: up to
   // 1024 channels (scores within 2^-17 of their terms, whose differences the exponential takes) and 4096 classes (2^-15 of a sum of
   // one sign).  2^20 channels: a loss 7e-4 off.
-  // Forward and backward together, us, tensor cores / CUDA cores: 131 072 pixels, classes x channels 13 x 64 191 / 194, 40 x 64 183 /
-  // 228, 99 x 50 217 / 314, 128 x 128 284 / 544; 40 962 pixels, 13 x 64 95 / 101, 40 x 64 93 / 116, 99 x 50 109 / 159, 300 x 96 210 /
-  // 468; 10 242 pixels, 40 x 32 71 / 55, 99 x 50 82 / 88, 300 x 64 96 / 125, 700 x 128 134 / 336; 2 562 pixels, 99 x 50 73 / 83,
-  // 300 x 64 79 / 94; 1 000 pixels, 40 x 64 68 / 66; 327 684 pixels, 20 x 32 395 / 308.
+  // Forward and backward together, us, tensor cores / CUDA cores: 131 072 pixels, classes x channels 13 x 64 172 / 194, 40 x 64 176 /
+  // 228, 99 x 50 208 / 314, 128 x 128 280 / 544; 40 962 pixels, 13 x 64 80 / 101, 40 x 64 82 / 116, 99 x 50 97 / 159, 300 x 96 201 /
+  // 468; 10 242 pixels, 40 x 32 61 / 55, 99 x 50 70 / 88, 300 x 64 83 / 125, 700 x 128 122 / 336; 2 562 pixels, 99 x 50 56 / 83,
+  // 300 x 64 64 / 94; 1 000 pixels, 40 x 64 52 / 65; 327 684 pixels, 20 x 32 386 / 308, 6 x 16 378 / 255.  (A stage has 64 channels:
+  // fewer are paid for in whole.)
   static bool takes(const mc_ce_desc* d) {
     const double each = (double)d->V * d->C;
-    return d->dtype == MC_F32 && d->C <= 1024 && d->V <= 4096 && each >= 2048 && each * d->B * d->S >= 1e7;
+    return d->dtype == MC_F32 && d->C <= 1024 && d->V <= 4096 && each >= (d->C >= 48 ? 768 : 2048) && each * d->B * d->S >= 2.5e6;
   }
   bool planes() const { return !(d->layout == MC_NHWC || d->S == 1) && d->C > 1; }
   mix::TcRows parts_of(const void* p, long long rows, int cols, int wide) const { return mix::TcRows{p, rows, cols, 3 * wide, 0, false, 3}; }
