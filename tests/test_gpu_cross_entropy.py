@@ -152,6 +152,32 @@ def test_float32_of_many_products(ops, i, layout):
     assert loss.isnan() and gw.isnan().all() and gb.isnan().all() and gx[0, :, 0, 0].isnan().all() and gx[-1, :, -1, -1].isfinite().all()
 
 
+# float32 layers of few classes on both sides of the rule for the tensor cores (768 weights of 48 channels or more, 2.5e6 products), one
+# class among them, odd counts, fewer pixels than a tile in the last image's planes
+FEW = [(1, 1, 3300, 1000, 1), (2, 41, 43, 1024, 1), (1, 1, 1700, 770, 2), (3, 37, 31, 256, 3), (1, 60, 71, 48, 16), (1, 60, 71, 47, 17),
+       (5, 1, 1301, 64, 13), (1, 1, 977, 64, 40), (1, 1, 976, 64, 40), (2, 1, 131, 100, 99)]
+
+
+@pytest.mark.parametrize("layout", ["nhwc", "nchw"])
+@pytest.mark.parametrize("i", range(len(FEW)))
+def test_float32_of_few_classes(ops, i, layout):
+    b, h, w, cin, classes = FEW[i]
+    g = torch.Generator("cuda").manual_seed(90 + i)
+    x = image(g, (b, cin, h, w), F32, layout)
+    weight, bias = classifier(g, classes, cin, F32)
+    target = labels(g, (b, h, w), classes, 0.2)
+    x = torch.where((target == -100)[:, None], torch.full_like(x, float("nan")), x)
+    x = x.contiguous(memory_format=torch.channels_last) if layout == "nhwc" else x.contiguous()
+    grad = torch.tensor(1.3, device="cuda")
+    for mean in (True, False):
+        loss, saved = ops.cross_entropy_forward(x, weight, bias, target, -100, mean)
+        got = ops.cross_entropy_backward(grad, saved, x, weight, bias, target, -100, mean)
+        assert layout_kept(got[0], layout)
+        R.check(dict(zip(("loss", "gx", "gw", "gb"), [loss] + got)), R.cross_entropy(x, weight, bias, target, -100, mean, grad), str(FEW[i]))
+        again = ops.cross_entropy_backward(grad, saved, x, weight, bias, target, -100, mean)
+        assert all(torch.equal(p, q) for p, q in zip(got, again))
+
+
 @pytest.mark.parametrize("batch,height,width,classes,dtype", [
     (3, 1, 90_000, 2562, BF),   # bf16: score gradients of more than one piece, whole images and part of one
     (1, 1, 250_000, 2562, BF),
