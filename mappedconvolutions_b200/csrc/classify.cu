@@ -184,6 +184,8 @@ __global__ void __launch_bounds__(THREADS) loss_kernel(const double* part, int b
 }
 // ---- bf16 -----------------------------------------------------------------------------------------------
 // The tiles' sums of a pixel become its lse; the blocks' losses and labelled pixels go to `part`.
+// (It starts while the kernel that writes those sums still runs, and a later piece's sums take the same place: read behind L1, never
+// through the read-only path.)
 __global__ void __launch_bounds__(THREADS) finish_kernel(mix::Scores s, int tiles, long long P, int V, float* lse, double* part) {
   __shared__ double sm[2][THREADS / 32];
   behind_previous_kernel();
@@ -199,15 +201,15 @@ __global__ void __launch_bounds__(THREADS) finish_kernel(mix::Scores s, int tile
     if (t >= 0 && t < V) {
       float top = -INFINITY;
 #pragma unroll 8
-      for (int k = 0; k < tiles; ++k) top = fmaxf(top, __ldg(&s.part[k * P + p].x));  // (a NaN shows in the sum)
+      for (int k = 0; k < tiles; ++k) top = fmaxf(top, __ldcg(&s.part[k * P + p].x));  // (a NaN shows in the sum)
       float all = 0.f;
 #pragma unroll 8
       for (int k = 0; k < tiles; ++k) {
-        const float2 v = __ldg(s.part + k * P + p);
+        const float2 v = __ldcg(s.part + k * P + p);
         all += v.y * exp2f(v.x - top);
       }
       out = (top + log2f(all)) * 0.69314718056f;
-      sum += (double)(out - s.hit[p]);
+      sum += (double)(out - __ldcg(s.hit + p));
     } else {
       sum = NAN;
     }
