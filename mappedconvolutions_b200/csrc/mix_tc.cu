@@ -698,10 +698,10 @@ __global__ void __launch_bounds__(THREADS, 1) rows_tc_kernel(const __grid_consta
           if (elected) {
             const uint32_t bar = of_leader(full(st));
             if (rank == 0) mbar_expect_tx(full(st), 2 * (A_BYTES + (g.group ? 0 : seg ? C::B1 : C::B0)));
-            const int across = g.a_across[seg];
+            const int across = MODE == LAYER || MODE == FLOATS ? g.a_across[seg] : 0;
             int ka = k, kb = k;
-            if (g.per && g.group) ka = pass_a(k / g.per) * g.per + k % g.per;
-            else if (g.per) ka = part_a(k / g.per) * g.per + k % g.per, kb = part_b(k / g.per) * g.per + k % g.per;
+            if (PARTS && g.per && g.group) ka = pass_a(k / g.per) * g.per + k % g.per;
+            else if (PARTS && g.per) ka = part_a(k / g.per) * g.per + k % g.per, kb = part_b(k / g.per) * g.per + k % g.per;
             tma_load_pair(a0 + st * A_BYTES, &g.a[seg], across ? 0 : ka * KB, across ? m0 * across + ka * TILE : m0, bar);
             if (!g.group) load_b<MODE, BN>(g, seg, rank, b0 + st * C::BMAX, kb * KB, n0, bar);
           }
