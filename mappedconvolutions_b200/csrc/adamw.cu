@@ -260,8 +260,9 @@ __global__ void __launch_bounds__(THREADS, B8 ? 6 : 1) step_kernel(const __grid_
         av = max(av, max(magnitude(v[j].x), magnitude(v[j].y)));
       }
       av = __reduce_max_sync(~0u, av);
-      // A root of less than 2^-63 counts as zero below, and its code is none either, where the block's largest is 2^-45 or more.
-      const bool small = av < __float_as_uint(0x1p-90f) || eps == 0.f;
+      // Approximate roots take those below 2^-63 for zero.  That changes no code where the block's largest is 2^-45 or more, and the
+      // divisor by less than 2^-24 of it where eps is 2^-39 inv_root or more (5.7e-11 at a first step with beta2 = 0.999).
+      const bool small = av < __float_as_uint(0x1p-90f) || eps < 0x1p-39f * inv_root;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         r[j] = small ? make_float2(__fsqrt_rn(v[j].x), __fsqrt_rn(v[j].y)) : make_float2(sqrt_near(v[j].x), sqrt_near(v[j].y));
