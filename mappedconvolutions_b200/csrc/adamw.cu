@@ -165,7 +165,7 @@ __device__ __forceinline__ float mul(float a, float b) { return __fmul_rn(a, b);
 __device__ __forceinline__ double mul(double a, double b) { return __dmul_rn(a, b); }
 __device__ __forceinline__ float root_of(float a) { return __fsqrt_rn(a); }
 __device__ __forceinline__ double root_of(double a) { return sqrt(a); }
-__device__ __forceinline__ float quotient(float a, float b) { return __fdividef(a, b); }  // (2 ulp; b < 2^126, sqrt(v) ends at 2^64)
+__device__ __forceinline__ float quotient(float a, float b) { return __fdiv_rn(a, b); }
 __device__ __forceinline__ double quotient(double a, double b) { return a / b; }
 
 // The codes of a block from its moments, in registers of a warp.
@@ -261,8 +261,9 @@ __global__ void __launch_bounds__(THREADS, B8 ? 6 : 1) step_kernel(const __grid_
       }
       av = __reduce_max_sync(~0u, av);
       // Approximate roots take those below 2^-63 for zero.  That changes no code where the block's largest is 2^-45 or more, and the
-      // divisor by less than 2^-24 of it where eps is 2^-39 inv_root or more (5.7e-11 at a first step with beta2 = 0.999).
-      const bool small = av < __float_as_uint(0x1p-90f) || eps < 0x1p-39f * inv_root;
+      // divisor by less than 2^-24 of it where eps is 2^-39 inv_root or more (5.7e-11 at a first step with beta2 = 0.999).  Approximate
+      // reciprocals are zero from 2^126 on, which only an eps reaches: roots end at 2^64.
+      const bool small = av < __float_as_uint(0x1p-90f) || eps < 0x1p-39f * inv_root || eps > 0x1p125f;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         r[j] = small ? make_float2(__fsqrt_rn(v[j].x), __fsqrt_rn(v[j].y)) : make_float2(sqrt_near(v[j].x), sqrt_near(v[j].y));

@@ -41,3 +41,22 @@ def test_first_steps(ops, eps, beta2, bits):
     ops.adamw_step([q], [g], [m], [v], [scales[0]], [scales[1]], [None], [1], lr, beta1, beta2, eps, 0.0)
     off = (q.double() - want).abs()
     assert (off <= 2.0 ** -21 * parts).all(), (off / parts).max().item()
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+@pytest.mark.parametrize("eps", [4e37, 1e38, 3e38])
+def test_divisors_near_the_largest_number(ops, eps, bits):
+    """m / (sqrt(v) root + eps) with moments as large: no reciprocal may be flushed to zero.  Roundings as above."""
+    n, lr = 600, 1.0
+    p, g = torch.zeros(n, device="cuda"), torch.zeros(n, device="cuda")
+    m32, v32 = torch.full((n,), 2e38, device="cuda"), torch.full((n,), 1.0, device="cuda")
+    if bits == 8:
+        scale = torch.full(((n + 255) // 256,), 2e38 / 127 ** 2, device="cuda")
+        root = torch.full_like(scale, 1.0 / 255 ** 2)
+        m, v = torch.full((n,), 127, dtype=torch.int8, device="cuda"), torch.full((n,), 255, dtype=torch.uint8, device="cuda")
+        m32, v32 = (t[0] for t in ops.adamw_moments([m], [v], [scale], [root]))
+    else:
+        m, v, scale, root = m32.clone(), v32.clone(), None, None
+    want = -(lr / (1 - 0.5 ** 3)) * (m32.double() * 0.5) / ((v32.double() * 0.5).sqrt() / math.sqrt(1 - 0.5 ** 3) + torch.tensor(eps, dtype=F32).double().item())
+    ops.adamw_step([p], [g], [m], [v], [scale], [root], [None], [3], lr, 0.5, 0.5, eps, 0.0)
+    assert ((p.double() - want).abs() <= 2.0 ** -21 * want.abs()).all(), (p[0].item(), want[0].item())
