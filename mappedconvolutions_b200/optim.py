@@ -69,7 +69,7 @@ class AdamW(torch.optim.Optimizer):
         if torch.cuda.is_initialized() and torch.cuda.is_current_stream_capturing():
             raise RuntimeError("a step counts on the host and cannot be captured into a CUDA graph")
         for group in self.param_groups:
-            by_device = {}
+            by_device, masters = {}, group["master_weights"]
             for p in group["params"]:
                 g = p.grad
                 if g is None:
@@ -77,6 +77,8 @@ class AdamW(torch.optim.Optimizer):
                 state = self.state[p]
                 if not state:
                     state.update(self._new_state(p, group))
+                elif masters and p.dtype == torch.bfloat16 and "master" not in state:  # (a state of torch's)
+                    state["master"] = p.detach().to(torch.float32, copy=True)
                 lists = by_device.get(p.device)
                 if lists is None:
                     lists = by_device[p.device] = ([], [], [], [], [], [], [], [], [])
@@ -108,14 +110,75 @@ class AdamW(torch.optim.Optimizer):
         return out
 
     def load_state_dict(self, state_dict):
-        """torch's, but every tensor of the state keeps its own type (torch would cast moments to the parameter's)."""
-        for group in state_dict["param_groups"]:
+        """torch's, but a state is kept as its parameter needs it: moments float32 (float64 for float64 parameters) in the
+        parameter's order of memory, or 8-bit codes as they are.  A state of torch.optim.AdamW leaves this optimiser's state_bits and
+        master_weights in place and takes their form; one that cannot go on the same way is refused before anything changes."""
+        loaded = state_dict["param_groups"]
+        for group in loaded:
             self._check_options(group)
-        super().load_state_dict(state_dict)
-        ids = [i for group in state_dict["param_groups"] for i in group["params"]]
-        params = [p for group in self.param_groups for p in group["params"]]
-        for i, p in zip(ids, params):
-            kept = state_dict["state"].get(i)
-            if kept:
-                self.state[p] = {k: v.detach().to(p.device, copy=True) if isinstance(v, torch.Tensor) else v
-                                 for k, v in kept.items()}
+            if group["weight_decay"] and not group.get("decoupled_weight_decay", True):
+                raise ValueError("a state whose weight decay goes through the moments is not supported")
+        kept = ("state_bits", "master_weights")
+        groups = [{**{k: mine[k] for k in kept}, **group} for mine, group in zip(self.param_groups, loaded)]
+        states = {}
+        if [len(g["params"]) for g in groups] == [len(g["params"]) for g in self.param_groups]:  # (else torch's own refuses it)
+            for mine, group, given in zip(self.param_groups, groups, loaded):
+                bits = 32 if "state_bits" in given else group["state_bits"]
+                for p, i in zip(mine["params"], group["params"]):
+                    if state_dict["state"].get(i):
+                        states[p] = self._state_for(p, state_dict["state"][i], bits)
+        super().load_state_dict({**state_dict, "param_groups": groups + list(loaded[len(groups):])})
+        self.state.update(states)
+
+    @staticmethod
+    def _state_for(p, given, bits):
+        """`given` as the state of p; bits 8: moments that are values become codes"""
+        missing = [k for k in ("step", "exp_avg", "exp_avg_sq") if k not in given]
+        if missing:
+            raise ValueError("a state of AdamW has %s" % ", ".join(missing))
+        state = {k: v.detach().to(p.device, copy=True) if isinstance(v, torch.Tensor) else v for k, v in given.items()}
+        coded = state["exp_avg"].dtype == torch.int8
+        for k in ("exp_avg", "exp_avg_sq", "master"):
+            v = state.get(k)
+            if v is None:
+                continue
+            if v.shape != p.shape:
+                raise ValueError("%s has shape %s, its parameter %s" % (k, tuple(v.shape), tuple(p.shape)))
+            if k == "master" and p.dtype != torch.bfloat16:
+                raise ValueError("only bfloat16 parameters have master weights, not %s" % p.dtype)
+            if coded and k != "master":
+                if p.dtype == torch.float64 or v.dtype != (torch.int8 if k == "exp_avg" else torch.uint8) or \
+                        any(n > 1 and a != b for n, a, b in zip(p.shape, p.stride(), v.stride())) or \
+                        k + "_scale" not in state or tuple(state[k + "_scale"].shape) != ((p.numel() + 255) // 256,):
+                    raise ValueError("moments in 8 bits belong to float32 or bfloat16 parameters that lie as they do, with a scale for 256 elements")
+            else:
+                wide = torch.float64 if p.dtype == torch.float64 else torch.float32
+                state[k] = torch.empty_like(p, dtype=wide, requires_grad=False).copy_(v)
+        if bits == 8 and not coded and p.dtype != torch.float64:
+            state.update(_codes(state["exp_avg"], state["exp_avg_sq"]))
+        return state
+
+
+def _codes(m, v):
+    """The 8-bit form of float32 moments (see mc_adamw_step), the operations of float32 one by one."""
+    def blocks(t):  # as they lie in memory
+        t = t.as_strided((t.numel(),), (1,))
+        return torch.nn.functional.pad(t, (0, -t.numel() % 256)).view(-1, 256)
+
+    def scale(largest, codes):
+        s = largest * torch.tensor(1 / codes, dtype=torch.float32, device=largest.device)
+        s = torch.where(s < 2.0 ** -126, torch.zeros_like(s), s)
+        return s, torch.where(s == 0, torch.zeros_like(s), 1 / s)
+
+    def put(c, like, dtype):
+        out = torch.empty_like(like, dtype=dtype)
+        out.as_strided((like.numel(),), (1,)).copy_(c.reshape(-1)[:like.numel()])
+        return out
+    a, r = blocks(m), torch.sqrt(blocks(v))
+    s, inverse = scale(a.abs().amax(1, keepdim=True), 127.0 ** 2)
+    c = torch.copysign(torch.sqrt(a.abs() * inverse).round().clamp(max=127), a).nan_to_num(0.0)
+    q, inverse = scale(r.amax(1, keepdim=True), 255.0 ** 2)
+    d = torch.sqrt(r * inverse).round().clamp(max=255)
+    d = torch.where((r > 0) & (q > 0), d.clamp(min=1), d).nan_to_num(0.0)  # (a v that is not zero keeps a code that is not zero)
+    return dict(exp_avg=put(c, m, torch.int8), exp_avg_scale=s[:, 0].contiguous(), exp_avg_sq=put(d, v, torch.uint8),
+                exp_avg_sq_scale=q[:, 0].contiguous())
