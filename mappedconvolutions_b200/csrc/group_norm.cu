@@ -43,6 +43,7 @@ struct Args {
   int param_blocks;  // of the third launch
   // channels-last: tiles of `px` pixels, in columns of at most 256 vectors
   int px, cols, V, R, lanes;
+  int column;   // elements of a whole column
   bool joined;  // the channels of a vector are of one group, and w and b start on 16 bytes
   // planes: segments of a plane, and how many a warp takes
   int segs, per;
@@ -729,8 +730,8 @@ template <typename T>
 __device__ __forceinline__ Two<T> peek(const Two<T>* p) {  // (behind L1)
   return Two<T>{__ldcg(&p->a), __ldcg(&p->b)};
 }
-// Statistics of a group by `sub` threads, in double: with d the distance of a part's mean from the first part's,
-// M2 = sum m2 + sum n d^2 - (sum n d)^2 / N  (one pass, its loads independent of each other).
+// Statistics of a group by `sub` threads, in double: with d the distance of a part's mean from that of the part of the group's first
+// value, M2 = sum m2 + sum n d^2 - (sum n d)^2 / N  (one pass, its loads independent of each other).
 template <typename CT>
 __global__ void __launch_bounds__(THREADS) stats_kernel(const __grid_constant__ Args a, bool rows, int sub) {
   let_next_kernel_start();
@@ -741,7 +742,8 @@ __global__ void __launch_bounds__(THREADS) stats_kernel(const __grid_constant__ 
   double n = 0, s = 0, q = 0, base = 0;
   if (b < a.B) {
     const Part<CT>* part = (const Part<CT>*)a.part + (rows ? b * a.tiles * a.G + g : (b * a.C + (long long)g * a.Cg) * a.segs);
-    base = __ldcg(&part->mean);
+    // (channels-last: the first tile's column that holds the group's first channel; parts of other columns may be empty)
+    base = __ldcg(&part[rows ? (long long)g * a.Cg / a.column * step : 0].mean);
 #pragma unroll 4
     for (int i = threadIdx.x % sub; i < count; i += sub) {
       const Part<CT>* p = part + (long long)i * step;
@@ -883,7 +885,7 @@ static int plan(const mc_norm_desc* d, Plan& p) {
     const int n = p.vec ? N : 1;
     a.R = n / gcd(n, d->C), a.V = (int)((long long)a.R * d->C / n);
     a.joined = a.R == 1 && n > 1 && a.Cg % n == 0;
-    a.cols = (a.V + 255) / 256;
+    a.cols = (a.V + 255) / 256, a.column = 256 * n;
     a.lanes = a.cols > 1 ? 1 : 256 / a.V;
     const long long step = (long long)a.lanes * a.R;
     // A thread's rows: as many as a run holds, fewer where that leaves an SM less than eight blocks.  (At most 16, 8: 64 x 10 242 x 256

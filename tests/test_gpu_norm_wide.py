@@ -1,0 +1,41 @@
+"""GPU: group normalisation of more channels than a block holds vectors of."""
+import pytest
+import torch
+
+import step_reference as R
+from mappedconvolutions_b200 import host, ops as twin
+
+pytestmark = pytest.mark.gpu
+BF, F32, F64 = torch.bfloat16, torch.float32, torch.float64
+
+
+@pytest.fixture(params=["ctypes", "compiled"])
+def ops(request):
+    return twin if request.param == "ctypes" else host.impl
+
+
+def image(g, shape, dtype, layout, scale=1.0, offset=0.0):
+    t = (torch.randn(shape, generator=g, device="cuda", dtype=F64) * scale + offset).to(dtype)
+    return t.contiguous(memory_format=torch.channels_last) if layout == "nhwc" else t
+
+
+@pytest.mark.parametrize("layout", ["nhwc"])
+@pytest.mark.parametrize("dtype,channels,groups", [(F64, 1200, 8), (F64, 1536, 48), (F64, 515, 5), (F64, 2049, 3), (F32, 2100, 20), (F32, 3001, 1)])
+@pytest.mark.parametrize("offset", [0.0, 1e4, -1e4])
+def test_values_far_from_zero(ops, dtype, channels, groups, layout, offset):
+    """every group as accurate as the first: groups that lie in later columns of vectors among them"""
+    g = torch.Generator("cuda").manual_seed(1)
+    shape = (2, channels, 3, 5)
+    x, gy = image(g, shape, dtype, layout, 1.0, offset), image(g, shape, dtype, layout)
+    w, b = (torch.randn(channels, generator=g, device="cuda").to(dtype) for _ in range(2))
+    y, stats = ops.group_norm_forward(x, w, b, groups, 1e-5, R.ACTS["silu"])
+    got = dict(zip(("gx", "gw", "gb"), ops.group_norm_backward(gy, stats, x, w, b, groups, 1e-5, R.ACTS["silu"])))
+    R.check(dict(y=y, **got), R.group_norm(x, w, b, groups, 1e-5, "silu", gy), (channels, groups, offset))
+    rstd = stats.view(F64 if dtype == F64 else F32).view(2, groups, 2)[:, :, 1].double()
+    var = x.double().contiguous().reshape(2, groups, -1).var(2, unbiased=False)
+    # Runs of up to 33 differences, merged in double: see the bound of rstd in step_reference.  And the means of a thread's run and of a
+    # tile are each rounded to half a step of |mean|, d in all: the variance of the means changes by 2 sum n_i (mean_i - mean) d_i / n,
+    # at most 2 d deviations, rstd by d / deviation of itself.  (Squares of means instead of differences: 10^8 steps of float64.)
+    t = R.Bounds(dtype)
+    far = 2 * t.step * (abs(offset) + 1) * rstd
+    assert ((rstd * (var + 1e-5).sqrt() - 1).abs() <= t.sum(256) + 4 * t.step + 2.0 ** -50 + far).all()
