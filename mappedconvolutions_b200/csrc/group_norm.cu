@@ -267,6 +267,13 @@ struct Run {  // of differences from the run's first values
     return Part<CT>{n, m - k[e], fmax(q[e] - s[e] * m, CT(0)) + (q[e] - q[e])};  // (NaN and infinities stay)
   }
 };
+// n values whose differences from `near` add up to c, their squares to m2.  (A mean from a sum of means is off by several roundings of a
+// value far from zero; differences from it give the rest.)
+template <typename CT>
+__device__ __forceinline__ Part<CT> centred(CT n, CT near, CT c, CT m2) {
+  const CT m = n > CT(0) ? c / n : CT(0);
+  return Part<CT>{n, near + m, fmax(m2 - c * m, CT(0)) + (m2 - m2)};
+}
 // What a vector adds to S1 and S2 (without rstd), and its gradient.
 template <typename T, int ACT, typename CT, int N>
 __device__ __forceinline__ void slope_terms(const Args& a, const Coefs<T, CT, N>& k, CT (&x)[N], CT (&g)[N]) {  // x <- x - mean, g <- dz
@@ -441,11 +448,14 @@ __device__ __forceinline__ void rows_stats(const Args& a, Shared<CT, N>& sm, lon
     Part<CT> q[N];
     CT mean = CT(0), m2 = CT(0);
 #pragma unroll
-    for (int e = 0; e < N; ++e) q[e] = run.part(e, (CT)rows), mean += q[e].mean;
-    mean /= CT(N);
+    for (int e = 0; e < N; ++e) q[e] = run.part(e, (CT)rows), mean += q[e].mean - q[0].mean;
+    mean /= CT(N);  // (from the first channel's mean)
 #pragma unroll
-    for (int e = 0; e < N; ++e) m2 += q[e].m2 + (CT)rows * (q[e].mean - mean) * (q[e].mean - mean);
-    sm.part[0][threadIdx.x] = Part<CT>{(CT)rows * CT(N), mean, m2};
+    for (int e = 0; e < N; ++e) {
+      const CT d = q[e].mean - q[0].mean - mean;
+      m2 += q[e].m2 + (CT)rows * d * d;
+    }
+    sm.part[0][threadIdx.x] = Part<CT>{(CT)rows * CT(N), q[0].mean + mean, m2};
   } else {
 #pragma unroll
     for (int e = 0; e < N; ++e) sm.part[e][threadIdx.x] = run.part(e, (CT)(rows + (p.tail + e < p.end ? 1 : 0)));
@@ -477,11 +487,15 @@ __device__ __forceinline__ void rows_stats(const Args& a, Shared<CT, N>& sm, lon
         if (entry(i, w)) cnt += w.n, sum += w.n * w.mean;
     for (int o = sub / 2; o; o >>= 1) cnt += __shfl_xor_sync(~0u, cnt, o), sum += __shfl_xor_sync(~0u, sum, o);
     const CT mean = cnt > CT(0) ? sum / cnt : CT(0);
+    CT c = CT(0);  // what the roundings of that sum left of the differences
     if (g < a.G)
       for (int i = threadIdx.x % sub; i < entries; i += sub)
-        if (entry(i, w)) m2 += w.m2 + w.n * (w.mean - mean) * (w.mean - mean);
-    for (int o = sub / 2; o; o >>= 1) m2 += __shfl_xor_sync(~0u, m2, o);
-    if (g < a.G && threadIdx.x % sub == 0) out[g] = Part<CT>{cnt, mean, m2};
+        if (entry(i, w)) {
+          const CT d = w.mean - mean;
+          m2 += w.m2 + w.n * d * d, c += w.n * d;
+        }
+    for (int o = sub / 2; o; o >>= 1) m2 += __shfl_xor_sync(~0u, m2, o), c += __shfl_xor_sync(~0u, c, o);
+    if (g < a.G && threadIdx.x % sub == 0) out[g] = centred(cnt, mean, c, m2);
   }
 }
 
@@ -636,8 +650,9 @@ __device__ __forceinline__ void planes_stats(const Args& a, long long b, int til
     const CT m = n > CT(0) ? s / n : CT(0);
     CT m2 = fmax(q - s * m, CT(0)) + (q - q);
     const CT mean = k[0] + m, cnt = warp_sum(n), all = warp_sum(n > CT(0) ? n * mean : CT(0)) / cnt;
-    m2 = warp_sum(n > CT(0) ? m2 + n * (mean - all) * (mean - all) : CT(0));
-    if (threadIdx.x % 32 == 0) ((Part<CT>*)a.part)[b * a.C * a.segs + item] = Part<CT>{cnt, all, m2};
+    const CT d = mean - all, c = warp_sum(n > CT(0) ? n * d : CT(0));
+    m2 = warp_sum(n > CT(0) ? m2 + n * d * d : CT(0));
+    if (threadIdx.x % 32 == 0) ((Part<CT>*)a.part)[b * a.C * a.segs + item] = centred(cnt, all, c, m2);
   });
 }
 template <typename T, int ACT, typename CT, int N>

@@ -19,7 +19,7 @@ def image(g, shape, dtype, layout, scale=1.0, offset=0.0):
     return t.contiguous(memory_format=torch.channels_last) if layout == "nhwc" else t
 
 
-@pytest.mark.parametrize("layout", ["nhwc"])
+@pytest.mark.parametrize("layout", ["nhwc", "nchw"])
 @pytest.mark.parametrize("dtype,channels,groups", [(F64, 1200, 8), (F64, 1536, 48), (F64, 515, 5), (F64, 2049, 3), (F32, 2100, 20), (F32, 3001, 1)])
 @pytest.mark.parametrize("offset", [0.0, 1e4, -1e4])
 def test_values_far_from_zero(ops, dtype, channels, groups, layout, offset):
@@ -30,7 +30,10 @@ def test_values_far_from_zero(ops, dtype, channels, groups, layout, offset):
     w, b = (torch.randn(channels, generator=g, device="cuda").to(dtype) for _ in range(2))
     y, stats = ops.group_norm_forward(x, w, b, groups, 1e-5, R.ACTS["silu"])
     got = dict(zip(("gx", "gw", "gb"), ops.group_norm_backward(gy, stats, x, w, b, groups, 1e-5, R.ACTS["silu"])))
-    R.check(dict(y=y, **got), R.group_norm(x, w, b, groups, 1e-5, "silu", gy), (channels, groups, offset))
+    # (x - offset is exact, and its normalised values are the same: the formulas' own sums in 64 bits are off by steps of the mean)
+    want, near = (R.group_norm(t, w, b, groups, 1e-5, "silu", gy) for t in (x, x - offset))
+    assert torch.equal((x - offset).double(), x.double() - offset) and torch.equal(x.double() - offset + offset, x.double())
+    R.check(dict(y=y, **got), {k: (near[k][0], want[k][1]) for k in want}, (channels, groups, offset))
     rstd = stats.view(F64 if dtype == F64 else F32).view(2, groups, 2)[:, :, 1].double()
     var = x.double().contiguous().reshape(2, groups, -1).var(2, unbiased=False)
     # Runs of up to 33 differences, merged in double: see the bound of rstd in step_reference.  And the means of a thread's run and of a
@@ -39,3 +42,20 @@ def test_values_far_from_zero(ops, dtype, channels, groups, layout, offset):
     t = R.Bounds(dtype)
     far = 2 * t.step * (abs(offset) + 1) * rstd
     assert ((rstd * (var + 1e-5).sqrt() - 1).abs() <= t.sum(256) + 4 * t.step + 2.0 ** -50 + far).all()
+
+
+@pytest.mark.parametrize("layout", ["nhwc", "nchw"])
+@pytest.mark.parametrize("dtype", [F32, F64], ids=["f32", "f64"])
+@pytest.mark.parametrize("shape,groups", [((3, 64, 40, 50), 4), ((2, 48, 1, 15), 48), ((1, 30, 9, 33), 5), ((1, 8, 1, 40962), 1), ((40, 32, 2, 7), 2)])
+def test_means_far_from_zero(ops, shape, groups, dtype, layout):
+    """A mean is off by roundings of itself where runs, tiles and the group leave theirs, half a step each, and by those of the
+    differences."""
+    g = torch.Generator("cuda").manual_seed(2)
+    t = R.Bounds(dtype)
+    for offset in (1e4, -3.7e5, 1.7):
+        x = image(g, shape, dtype, layout, 1.0, offset)
+        stats = ops.group_norm_forward(x, None, None, groups)[1].view(dtype).view(shape[0], groups, 2)
+        rows = x.double().contiguous().reshape(shape[0], groups, -1)
+        mean = rows[:, :, :1] + (rows - rows[:, :, :1]).mean(2, keepdim=True)
+        dev = (rows - mean).abs().mean(2)
+        assert ((stats[:, :, 0].double() - mean[:, :, 0]).abs() <= 3 * t.step * mean[:, :, 0].abs() + t.sum(256) * dev).all(), offset
