@@ -43,7 +43,10 @@ struct Args {
   int param_blocks;  // of the third launch
   // channels-last: tiles of `px` pixels, in columns of at most 256 vectors
   int px, cols, V, R, lanes;
-  int column;   // elements of a whole column
+  // Elements of a whole column; channels and groups that the part of a column has room for: all there are, or those that a column can
+  // hold any of, from its first one on and around the end.  (Room for all in each column: scratch of C^2, 8.6 GB for 4 MB of 2^20 channels.)
+  int column, chans, grps;
+  bool wide;    // more than a column to a row
   bool joined;  // the channels of a vector are of one group, and w and b start on 16 bytes
   // planes: segments of a plane, and how many a warp takes
   int segs, per;
@@ -422,6 +425,13 @@ struct Place {
     }
   }
 };
+// Whose sums come first in the part of a column, and where those of group g stand.
+__device__ __forceinline__ int first_channel(const Args& a, int col) { return a.chans < a.C ? (int)((long long)col * a.column % a.C) : 0; }
+__device__ __forceinline__ int first_group(const Args& a, int col) { return a.grps < a.G ? (int)((long long)col * a.column % a.C) / a.Cg : 0; }
+__device__ __forceinline__ int group_slot(const Args& a, int col, int g) {
+  const int s = g - first_group(a, col);
+  return s < 0 ? s + a.G : s;
+}
 template <typename CT, int N> union Shared {
   Part<CT> part[N][THREADS];
   Two<CT> two[N][THREADS];
@@ -462,40 +472,52 @@ __device__ __forceinline__ void rows_stats(const Args& a, Shared<CT, N>& sm, lon
   }
   __syncthreads();
   // what the threads of a group's channels left, a few threads to a group
-  const int each = J ? a.Cg / N : a.Cg * a.R, entries = each * a.lanes;
-  const int sub = entries > 16 ? 32 : entries > 8 ? 16 : entries > 4 ? 8 : 4;
-  Part<CT>* out = (Part<CT>*)a.part + (b * a.tiles + tile) * a.G;
-  for (int g0 = 0; g0 < a.G; g0 += THREADS / sub) {
-    const int g = g0 + threadIdx.x / sub;
-    const auto entry = [&](int i, Part<CT>& v) {
-      const int l = i / each, k = i - l * each;
-      int e = 0, j;
-      if constexpr (J) {
-        j = g * each + k - p.col * 256;
-      } else {
-        const int rr = k / a.Cg, f = rr * a.C + g * a.Cg + k - rr * a.Cg;
-        j = f / N - p.col * 256, e = f % N;
+  const int each = J ? a.Cg / N : a.Cg * a.R, entries = a.wide ? min(each, J ? 256 : a.column) : each * a.lanes;
+  const int sub = entries > 16 ? 32 : entries > 8 ? 16 : entries > 4 ? 8 : 4, me = threadIdx.x % sub;
+  Part<CT>* out = (Part<CT>*)a.part + (b * a.tiles + tile) * a.grps;
+  for (int s0 = 0; s0 < a.grps; s0 += THREADS / sub) {
+    const int slot = s0 + threadIdx.x / sub;
+    const bool on = slot < a.grps;
+    int g = slot + first_group(a, p.col);
+    if (g >= a.G) g -= a.G;
+    // f(part) of every one of this group's in the column, this thread's share of them
+    const auto each_entry = [&](auto f) {
+      if (!on) return;
+      if (!a.wide) {
+        for (int i = me; i < entries; i += sub) {
+          const int l = i / each, k = i - l * each;
+          int e = 0, j;
+          if constexpr (J) {
+            j = g * each + k;
+          } else {
+            const int rr = k / a.Cg, at = rr * a.C + g * a.Cg + k - rr * a.Cg;
+            j = at / N, e = at % N;
+          }
+          const Part<CT> v = sm.part[e][l * p.vc + j];
+          if (v.n > CT(0)) f(v);
+        }
+      } else {  // (one lane: the group's elements in each pixel of the row, as far as the column reaches)
+        const int from = p.col * a.column, to = from + p.vc * N;
+        for (int r = 0; r < a.R; ++r) {
+          const int lo = max(r * a.C + g * a.Cg, from) - from, hi = min(r * a.C + (g + 1) * a.Cg, to) - from;
+          for (int i = (J ? lo / N : lo) + me; i < (J ? hi / N : hi); i += sub) {
+            const Part<CT> v = J ? sm.part[0][i] : sm.part[i % N][i / N];
+            if (v.n > CT(0)) f(v);
+          }
+        }
       }
-      if (j < 0 || j >= p.vc) return false;
-      v = sm.part[e][l * p.vc + j];
-      return v.n > CT(0);
     };
     CT cnt = CT(0), sum = CT(0), m2 = CT(0);
-    Part<CT> w;
-    if (g < a.G)
-      for (int i = threadIdx.x % sub; i < entries; i += sub)
-        if (entry(i, w)) cnt += w.n, sum += w.n * w.mean;
+    each_entry([&](const Part<CT>& w) { cnt += w.n, sum += w.n * w.mean; });
     for (int o = sub / 2; o; o >>= 1) cnt += __shfl_xor_sync(~0u, cnt, o), sum += __shfl_xor_sync(~0u, sum, o);
     const CT mean = cnt > CT(0) ? sum / cnt : CT(0);
     CT c = CT(0);  // what the roundings of that sum left of the differences
-    if (g < a.G)
-      for (int i = threadIdx.x % sub; i < entries; i += sub)
-        if (entry(i, w)) {
-          const CT d = w.mean - mean;
-          m2 += w.m2 + w.n * d * d, c += w.n * d;
-        }
+    each_entry([&](const Part<CT>& w) {
+      const CT d = w.mean - mean;
+      m2 += w.m2 + w.n * d * d, c += w.n * d;
+    });
     for (int o = sub / 2; o; o >>= 1) m2 += __shfl_xor_sync(~0u, m2, o), c += __shfl_xor_sync(~0u, c, o);
-    if (g < a.G && threadIdx.x % sub == 0) out[g] = centred(cnt, mean, c, m2);
+    if (on && me == 0) out[slot] = centred(cnt, mean, c, m2);
   }
 }
 
@@ -544,23 +566,27 @@ __device__ __forceinline__ void rows_sums(const Args& a, Shared<CT, N>& sm, long
 #pragma unroll
   for (int e = 0; e < N; ++e) sm.two[e][threadIdx.x] = Two<CT>{sums.s1[e], sums.s2[e]};
   __syncthreads();
-  const int entries = a.R * a.lanes;
+  const bool once = a.C > a.column;  // each channel of a column is in one place of it
+  const int entries = once ? 1 : a.R * a.lanes;
   // threads that share a channel, as many as the channels leave
   const int sub = a.C >= 128 ? 1 : a.C >= 32 ? 8 : 32;
-  Two<CT>* out = (Two<CT>*)a.part + (b * a.tiles + tile) * a.C;
-  for (int c0 = 0; c0 < a.C; c0 += THREADS / sub) {
-    const int c = c0 + threadIdx.x / sub;
+  Two<CT>* out = (Two<CT>*)a.part + (b * a.tiles + tile) * a.chans;
+  for (int s0 = 0; s0 < a.chans; s0 += THREADS / sub) {
+    const int slot = s0 + threadIdx.x / sub;
+    int c = slot + first_channel(a, p.col);
+    if (c >= a.C) c -= a.C;
     CT u = CT(0), v = CT(0);
-    if (c < a.C)
+    if (slot < a.chans)
       for (int i = threadIdx.x % sub; i < entries; i += sub) {
-        const int l = a.R == 1 ? i : i / a.R, r = i - l * a.R, f = r * a.C + c, j = f / N - p.col * 256;
+        const int l = a.R == 1 ? i : i / a.R, r = i - l * a.R, f = once ? slot : r * a.C + c, j = once ? f / N : f / N - p.col * 256;
         if (j >= 0 && j < p.vc) {
           const Two<CT> t = sm.two[f % N][l * p.vc + j];
           u += t.a, v += t.b;
         }
       }
     for (int o = sub / 2; o; o >>= 1) u += __shfl_xor_sync(~0u, u, o), v += __shfl_xor_sync(~0u, v, o);
-    if (c < a.C && threadIdx.x % sub == 0) out[c] = Two<CT>{u, v * __ldcg((const CT*)a.stats + 2 * (b * a.G + c / a.Cg) + 1)};
+    if (slot < a.chans && threadIdx.x % sub == 0)
+      out[slot] = Two<CT>{u, v * __ldcg((const CT*)a.stats + 2 * (b * a.G + c / a.Cg) + 1)};
   }
 }
 
@@ -753,17 +779,38 @@ __global__ void __launch_bounds__(THREADS) stats_kernel(const __grid_constant__ 
   behind_previous_kernel();
   const long long group = (blockIdx.x * (long long)THREADS + threadIdx.x) / sub;
   const long long b = group / a.G;
-  const int g = (int)(group % a.G), count = rows ? a.tiles : a.Cg * a.segs, step = rows ? a.G : 1;
+  const int g = (int)(group % a.G), me = threadIdx.x % sub;
   double n = 0, s = 0, q = 0, base = 0;
-  if (b < a.B) {
-    const Part<CT>* part = (const Part<CT>*)a.part + (rows ? b * a.tiles * a.G + g : (b * a.C + (long long)g * a.Cg) * a.segs);
-    // (channels-last: the first tile's column that holds the group's first channel; parts of other columns may be empty)
-    base = __ldcg(&part[rows ? (long long)g * a.Cg / a.column * step : 0].mean);
+  const auto merge = [&](const Part<CT>* p) {
+    const double k = __ldcg(&p->n), m = __ldcg(&p->mean), m2 = __ldcg(&p->m2), d = k > 0 ? m - base : 0.0;
+    n += k, s += k * d, q += m2 + k * d * d;
+  };
+  if (b < a.B && !rows) {
+    const Part<CT>* part = (const Part<CT>*)a.part + (b * a.C + (long long)g * a.Cg) * a.segs;
+    base = __ldcg(&part->mean);
 #pragma unroll 4
-    for (int i = threadIdx.x % sub; i < count; i += sub) {
-      const Part<CT>* p = part + (long long)i * step;
-      const double k = __ldcg(&p->n), m = __ldcg(&p->mean), m2 = __ldcg(&p->m2), d = k > 0 ? m - base : 0.0;
-      n += k, s += k * d, q += m2 + k * d * d;
+    for (int i = me; i < a.Cg * a.segs; i += sub) merge(part + i);
+  } else if (b < a.B) {
+    const Part<CT>* part = (const Part<CT>*)a.part + b * a.tiles * a.grps;
+    const auto at = [&](int col) { return part + (long long)col * a.grps + group_slot(a, col, g); };
+    const long long step = (long long)a.cols * a.grps;  // from pixels to pixels
+    const int count = a.tiles / a.cols;
+    // (the first tile's column that holds the group's first channel; parts of other columns may be empty)
+    base = __ldcg(&at(g * a.Cg / a.column)->mean);
+    if (!a.wide) {
+      const Part<CT>* p = at(0);
+#pragma unroll 4
+      for (int i = me; i < count; i += sub) merge(p + i * step);
+    } else {  // the columns that hold any of the group, pixel by pixel of a row
+      int done = 0;
+      const bool all = a.C <= a.column;
+      for (int r = 0; r < (all ? 1 : a.R); ++r) {
+        const int f = r * a.C + g * a.Cg, lo = max(all ? 0 : f / a.column, done);
+        const int hi = all ? a.cols : min((f + a.Cg - 1) / a.column + 1, a.cols), wide = hi - lo;
+        if (wide <= 0) continue;
+        for (long long i = me; i < (long long)wide * count; i += sub) merge(at(lo + (int)(i % wide)) + i / wide * step);
+        done = hi;
+      }
     }
   }
   for (int o = sub / 2; o; o >>= 1) n += __shfl_xor_sync(~0u, n, o), s += __shfl_xor_sync(~0u, s, o), q += __shfl_xor_sync(~0u, q, o);
@@ -781,19 +828,26 @@ __global__ void __launch_bounds__(THREADS) coef_kernel(const __grid_constant__ A
   let_next_kernel_start();
   behind_previous_kernel();
   const long long b = blockIdx.x / a.G;
-  const int g = (int)(blockIdx.x % a.G), count = rows ? a.tiles : a.segs;
-  const long long step = rows ? a.C : 1;
+  const int g = (int)(blockIdx.x % a.G), count = rows ? a.tiles / a.cols : a.segs;
+  const long long step = rows ? (long long)a.cols * a.chans : 1;
+  const bool once = rows && a.C > a.column;
+  const int places = !rows || !a.wide ? 1 : once ? a.R : a.cols;  // of a channel in a row of pixels
   Two<double>* sums = (Two<double>*)a.sums + b * a.C;
   double gu = 0, gv = 0;
   for (int i0 = 0; i0 < a.Cg; i0 += THREADS / sub) {
     const int i = i0 + threadIdx.x / sub, c = g * a.Cg + i;
     double u = 0, v = 0;
     if (i < a.Cg) {
-      const Two<CT>* part = (const Two<CT>*)a.part + (rows ? b * count * a.C + c : (b * a.C + c) * count);
+      for (int r = 0; r < places; ++r) {
+        const int f = r * a.C + c, col = once ? f / a.column : r;
+        if (rows && col >= a.cols) break;
+        const Two<CT>* part = (const Two<CT>*)a.part +
+                              (rows ? (b * a.tiles + col) * a.chans + (once ? f - col * a.column : c) : (b * a.C + c) * count);
 #pragma unroll 8
-      for (int k = threadIdx.x % sub; k < count; k += sub) {
-        const Two<CT> t = peek(part + k * step);
-        u += t.a, v += t.b;
+        for (int k = threadIdx.x % sub; k < count; k += sub) {
+          const Two<CT> t = peek(part + k * step);
+          u += t.a, v += t.b;
+        }
       }
     }
     for (int o = sub / 2; o; o >>= 1) u += __shfl_xor_sync(~0u, u, o), v += __shfl_xor_sync(~0u, v, o);
@@ -900,8 +954,11 @@ static int plan(const mc_norm_desc* d, Plan& p) {
     const int n = p.vec ? N : 1;
     a.R = n / gcd(n, d->C), a.V = (int)((long long)a.R * d->C / n);
     a.joined = a.R == 1 && n > 1 && a.Cg % n == 0;
-    a.cols = (a.V + 255) / 256, a.column = 256 * n;
-    a.lanes = a.cols > 1 ? 1 : 256 / a.V;
+    a.cols = (a.V + 255) / 256, a.column = 256 * n, a.wide = a.V > 256;
+    if (a.wide && d->S < a.R) a.cols = (int)((d->S * d->C + a.column - 1) / a.column);  // (of a row that the only image does not fill)
+    a.chans = d->C > a.column ? a.column : d->C;
+    a.grps = d->C > a.column && a.column / a.Cg + 2 < a.G ? a.column / a.Cg + 2 : a.G;
+    a.lanes = a.wide ? 1 : 256 / a.V;
     const long long step = (long long)a.lanes * a.R;
     // A thread's rows: as many as a run holds, fewer where that leaves an SM less than eight blocks.  (At most 16, 8: 64 x 10 242 x 256
     // bf16 forward 196, 230 us instead of 181; backward, with two vectors of either tensor on their way, 309, 350 instead of 300.)
@@ -909,7 +966,7 @@ static int plan(const mc_norm_desc* d, Plan& p) {
     k = k < 1 ? 1 : k > RUN ? RUN : k;
     a.px = (int)(step * k);
     tiles = (d->S + a.px - 1) / a.px * a.cols;
-    p.part_f = (size_t)(d->B * tiles) * a.G * 3 * ct, p.part_b = (size_t)(d->B * tiles) * a.C * 2 * ct;
+    p.part_f = (size_t)(d->B * tiles) * a.grps * 3 * ct, p.part_b = (size_t)(d->B * tiles) * a.chans * 2 * ct;
   } else {
     p.vec = true;
     a.segs = (int)((d->S + SEGMENT - 1) / SEGMENT);
@@ -957,7 +1014,7 @@ static int three(const Plan& p, cudaStream_t st) {
   if (rc) return rc;
   const long long groups = a.B * a.G;
   if (BWD) {
-    int sub = sharers(a.B * a.C, ROWS ? a.tiles : a.segs);
+    int sub = sharers(a.B * a.C, ROWS ? a.tiles / a.cols : a.segs);
     while (sub < 32 && sub * a.Cg < THREADS) sub *= 2;  // (a block has one group's channels only)
     rc = launch(coef_kernel<T>, (unsigned)groups, true, st, (Args)a, (bool)ROWS, (int)sub);
     a.param_blocks = a.gw || a.gb ? (a.C + THREADS / 8 - 1) / (THREADS / 8) : 0;

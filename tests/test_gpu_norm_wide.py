@@ -59,3 +59,27 @@ def test_means_far_from_zero(ops, shape, groups, dtype, layout):
         mean = rows[:, :, :1] + (rows - rows[:, :, :1]).mean(2, keepdim=True)
         dev = (rows - mean).abs().mean(2)
         assert ((stats[:, :, 0].double() - mean[:, :, 0]).abs() <= 3 * t.step * mean[:, :, 0].abs() + t.sum(256) * dev).all(), offset
+
+
+# rows of several columns of vectors: one pixel or some to a row, fewer pixels than a row has, groups of one channel, within columns and over
+# them, one group, ends around the last channel; one column and one vector more
+SHAPES = [((1, 1 << 20, 1, 1), 1 << 10), ((2, 70_000, 1, 1), 7), ((3, 5000, 2, 3), 8), ((1, 30_011, 1, 5), 1), ((1, 30_011, 1, 5), 30_011),
+          ((2, 4100, 1, 2), 2050), ((2, 4100, 1, 2), 1), ((2, 4100, 4, 5), 41), ((1, 2049, 1, 3), 3), ((1, 2049, 3, 11), 683), ((2, 2056, 2, 4), 257),
+          ((1, 16_385, 1, 1), 5), ((1, 16_385, 1, 9), 3277), ((4, 8192, 5, 7), 16), ((2, 6150, 1, 4), 2), ((2, 257, 5, 8), 257), ((1, 1025, 7, 7), 41)]
+
+
+@pytest.mark.parametrize("layout", ["nhwc", "nchw"])
+@pytest.mark.parametrize("dtype", [BF, F32, F64], ids=["bf16", "f32", "f64"])
+@pytest.mark.parametrize("i", range(len(SHAPES)))
+def test_many_channels(ops, i, dtype, layout):
+    shape, groups = SHAPES[i]
+    g = torch.Generator("cuda").manual_seed(i)
+    x, gy = image(g, shape, dtype, layout, 2.0, 0.5), image(g, shape, dtype, layout)
+    w, b = (torch.randn(shape[1], generator=g, device="cuda").to(dtype) for _ in range(2))
+    name = [None, "relu", "silu"][i % 3]
+    y, stats = ops.group_norm_forward(x, w, b, groups, 1e-5, R.ACTS[name])
+    got = dict(zip(("gx", "gw", "gb"), ops.group_norm_backward(gy, stats, x, w, b, groups, 1e-5, R.ACTS[name])))
+    R.check(dict(y=y, **got), R.group_norm(x, w, b, groups, 1e-5, name, gy), SHAPES[i])
+    again = ops.group_norm_forward(x, w, b, groups, 1e-5, R.ACTS[name])
+    assert torch.equal(y, again[0]) and torch.equal(stats, again[1])
+    assert torch.equal(got["gx"], ops.group_norm_backward(gy, stats, x, w, b, groups, 1e-5, R.ACTS[name])[0])
