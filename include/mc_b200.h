@@ -477,7 +477,8 @@ int mc_grad_clip(int32_t n, const void* const* src, const int32_t* src_dtype, vo
  * stats: mc_group_norm_stats_bytes of memory that the forward call fills (mean and 1 / sqrt(var + eps) of every group of
  * every image, float32 or double) and the backward call reads.  ws: scratch, phases MC_PHASE_FORWARD and MC_PHASE_BACKWARD.  Both
  * 16-byte aligned.  Any of the gradients may be NULL.  Arithmetic is float32 (double for MC_F64), sums over tiles are double
- * and in a fixed order: results repeat bit for bit.  Limits: B * S <= 2^31 - 256, C <= 2^20. */
+ * and in a fixed order: results repeat bit for bit.  Limits: B * S <= 2^31 - 256, C <= 2^20, B * groups < 2^31; MC_NCHW with S > 1: C times the
+ * pieces of 4096 pixels of a plane < 2^30. */
 typedef struct mc_norm_desc {
   int64_t B, S;
   int32_t C, groups;

@@ -980,7 +980,8 @@ static int plan(const mc_norm_desc* d, Plan& p) {
     p.part_f = (size_t)(d->B * items) * 3 * ct, p.part_b = (size_t)(d->B * items) * 2 * ct;
   }
   p.sums = (size_t)d->B * d->C * 16, p.coef = (size_t)d->B * d->groups * 2 * ct;
-  if (d->B * tiles >= (1ll << 31) - (1 << 20) || d->B * d->groups >= (1ll << 31) / 32) return MC_ERR_TOO_LARGE;
+  // (a grid's blocks: tiles and blocks of parameter gradients, groups)
+  if (d->B * tiles >= (1ll << 31) - (1 << 20) || d->B * d->groups >= (1ll << 31)) return MC_ERR_TOO_LARGE;
   a.tiles = (int)tiles, p.blocks = (unsigned)(d->B * tiles);
   return MC_OK;
 }

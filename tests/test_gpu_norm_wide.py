@@ -83,3 +83,20 @@ def test_many_channels(ops, i, dtype, layout):
     again = ops.group_norm_forward(x, w, b, groups, 1e-5, R.ACTS[name])
     assert torch.equal(y, again[0]) and torch.equal(stats, again[1])
     assert torch.equal(got["gx"], ops.group_norm_backward(gy, stats, x, w, b, groups, 1e-5, R.ACTS[name])[0])
+
+
+@pytest.mark.parametrize("layout", ["nhwc", "nchw"])
+@pytest.mark.parametrize("shape,groups", [((1 << 21, 64, 1, 1), 32), ((1 << 20, 64, 1, 3), 64), ((70, 1 << 20, 1, 1), 1 << 20)])
+def test_many_groups(shape, groups, layout):
+    """2^26 groups and more: the first, the last and images between them against the formulas"""
+    g = torch.Generator("cuda").manual_seed(7)
+    assert shape[0] * groups >= 1 << 26
+    x, gy = (torch.empty(shape, dtype=BF, device="cuda", memory_format=torch.channels_last if layout == "nhwc" else torch.contiguous_format).normal_(generator=g)
+             for _ in range(2))
+    w, b = (torch.randn(shape[1], generator=g, device="cuda").to(BF) for _ in range(2))
+    y, stats = host.impl.group_norm_forward(x, w, b, groups, 1e-5, 1)
+    gx, gw, gb = host.impl.group_norm_backward(gy, stats, x, w, b, groups, 1e-5, 1)
+    for at in (slice(0, 3), slice(shape[0] // 2, shape[0] // 2 + 3), slice(shape[0] - 3, shape[0])):
+        want = R.group_norm(x[at], w, b, groups, 1e-5, "relu", gy[at])
+        R.check(dict(y=y[at], gx=gx[at]), {k: want[k] for k in ("y", "gx")}, at)
+    assert gw.isfinite().all() and gb.isfinite().all()

@@ -20,3 +20,20 @@ def test_scratch_grows_with_the_input(dtype, size):
                 for phase in (0, 1):
                     got = L.mc_group_norm_workspace_bytes(d, phase)
                     assert 0 < got <= n * (3 * wide + 16 + 2 * wide) + 256 * 16 * 3 * wide + 4096, (b, s, c, groups, layout, phase, got / n)
+
+
+def test_limits():
+    L = _lib.lib()
+
+    def answer(b, s, c, groups, layout):
+        d = _lib.McNormDesc(b, s, c, groups, 0, _lib.MC_BF16, layout, 1e-5)
+        fits = L.mc_group_norm_workspace_bytes(d, 0) > 0
+        assert fits == (L.mc_group_norm_workspace_bytes(d, 1) > 0)
+        rc = L.mc_group_norm_fwd(d, *[256] * 6, 16, None)
+        assert rc == (-3 if fits else -6)  # the scratch is too small, or the limit is told
+        return fits
+    for layout in (_lib.MC_NHWC, _lib.MC_NCHW):
+        assert answer(1 << 20, 2, 64, 64, layout) and answer(1 << 21, 4, 64, 32, layout) and answer((1 << 25) - 1, 2, 64, 64, layout)
+        assert not answer(1 << 25, 2, 64, 64, layout) and not answer(1 << 11, 1, 1 << 20, 1 << 20, layout)
+        assert answer((1 << 11) - 1, 1, 1 << 20, 1 << 20, layout)
+    assert answer(1, 4096 * 1023, 1 << 20, 1, _lib.MC_NCHW) and not answer(1, 4096 * 1023 + 1, 1 << 20, 1, _lib.MC_NCHW)
