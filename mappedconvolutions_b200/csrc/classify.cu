@@ -1,10 +1,11 @@
 // Softmax cross entropy of a pointwise classifier.
 //
 // With P = B * S pixels, row vectors x_p, class scores z_p = x_p W^T + b (V of them) and labels t_p:
-//   lse_p = log sum_v exp(z_pv),   loss = scale sum_p (lse_p - z_p,t_p),   scale = 1 / labelled pixels, or 1
-//   gz_pv = g scale (exp(z_pv - lse_p) - [v = t_p]),   gx = gz W,   gW = gz^T x,   gb = sum_p gz
-// A pixel whose label is `ignore` counts nothing: its lse is kept as +infinity, its gz is zero and its features are read as
-// zeros, whatever they are.  A label outside [0, V) makes the loss NaN, and the gradients that the pixel takes part in: its lse is kept as NaN.
+//   top_p = max_v z_pv,   rest_p = log sum_v exp(z_pv - top_p),   loss_p = (top_p - z_p,t_p) + rest_p,   loss = scale sum_p loss_p
+//   gz_pv = g scale exp((z_pv - top_p) - rest_p),  of the label g scale (e^-loss_p - 1),   gx = gz W,   gW = gz^T x,   gb = sum_p gz
+// with scale = 1 / labelled pixels, or 1.  (top + rest is never formed: see Softmax.)
+// A pixel whose label is `ignore` counts nothing: its top is kept as +infinity, its gz is zero and its features are read as
+// zeros, whatever they are.  A label outside [0, V) makes the loss NaN, and the gradients that the pixel takes part in: its top is kept as NaN.
 //
 // bf16 (tensor cores): the scores of 256 pixels x up to 256 classes stand in TMEM; the forward call keeps their largest and the
 // sum of their exponentials, the backward call computes them again, rounds gz to bf16 - which the next two products' operand is -
@@ -14,6 +15,7 @@
 // float64, and float32 otherwise (CUDA cores), with the kernels of the channel-mixing layers: up to 128 classes stand in a block's
 // registers, whose threads add up the softmax; scores of more classes go through the workspace, a piece of the pixels at a time.
 // Bound: the products (FMA issue).
+#include "act_pairs.cuh"
 #include "mix_work.cuh"
 
 namespace mc {
@@ -21,9 +23,18 @@ namespace classify {
 using mix::RowsArgs;
 using mix::View;
 
-// What a forward call keeps: the number of labelled pixels (a double), from byte 256 on lse of every pixel, and behind it the input as
-// rows of channels where it lies in another way (bf16).
+// What a forward call keeps: the number of labelled pixels (a double), from byte 256 on top, rest (in base 2 where the tensor cores read it)
+// and miss of every pixel, and behind them the input as rows of channels where it lies in another way (bf16).
 constexpr size_t KEPT_HEAD = 256;
+using mix::Softmax;
+template <typename T>
+static size_t kept_bytes(long long pixels) { return KEPT_HEAD + 3 * mix::up256((size_t)pixels * sizeof(T)); }
+template <typename T>
+static Softmax<T> softmax_of(void* kept, long long pixels) {
+  char* p = (char*)kept + KEPT_HEAD;
+  const size_t n = mix::up256((size_t)pixels * sizeof(T));
+  return Softmax<T>{(T*)p, (T*)(p + n), (T*)(p + 2 * n)};
+}
 constexpr size_t PIECE = 256u << 20;     // bytes of scores or gz at a time, CUDA cores
 constexpr int FEW = 128;                 // classes that the CUDA-core kernels keep in registers
 constexpr size_t PIECE_TC = 1024u << 20; // bytes of gz at a time, tensor cores
@@ -34,6 +45,8 @@ __device__ __forceinline__ float exp_of(float v) { return expf(v); }
 __device__ __forceinline__ double exp_of(double v) { return exp(v); }
 __device__ __forceinline__ float log_of(float v) { return logf(v); }
 __device__ __forceinline__ double log_of(double v) { return log(v); }
+__device__ __forceinline__ float expm1_of(float v) { return expm1f(v); }
+__device__ __forceinline__ double expm1_of(double v) { return expm1(v); }
 
 // The kernels that this is called in start while the one before them runs; here they wait until all that it wrote can be read.
 __device__ __forceinline__ void behind_previous_kernel() {
@@ -64,22 +77,22 @@ __device__ __forceinline__ CT warp_sum(CT v) {
 }
 
 template <typename T> struct alignas(16) Four { T v[4]; };
-// lse and loss of the rows of a piece, one warp to a row of ld (a multiple of 4) scores
+// what is kept of the rows of a piece, and their losses, one warp to a row of ld (a multiple of 4) scores
 template <typename T>
-__global__ void __launch_bounds__(THREADS) lse_kernel(const T* __restrict__ z, int ld, const int64_t* __restrict__ target, long long n,
-                                                      int V, long long ignore, T* __restrict__ lse, T* __restrict__ value) {
+__global__ void __launch_bounds__(THREADS) softmax_kernel(const T* __restrict__ z, int ld, const int64_t* __restrict__ target,
+                                                          long long n, int V, long long ignore, Softmax<T> kept, T* __restrict__ value) {
   const long long row = blockIdx.x * (long long)(THREADS / 32) + threadIdx.x / 32;
   if (row >= n) return;
   const int lane = threadIdx.x % 32;
   const long long t = target[row];
-  T out, loss;
+  T top = -T(INFINITY), rest = T(0), loss = T(0);
   if (t == ignore) {
-    out = T(INFINITY), loss = T(0);
+    top = T(INFINITY);
   } else if (t < 0 || t >= V) {
-    out = loss = T(NAN);
+    top = loss = T(NAN);
   } else {
     const T* r = z + row * ld;
-    T top = -T(INFINITY), sum = T(0);
+    T sum = T(0);
 #pragma unroll 4
     for (int v = lane * 4; v < V; v += 128) {
       const Four<T> q = *reinterpret_cast<const Four<T>*>(r + v);
@@ -94,27 +107,26 @@ __global__ void __launch_bounds__(THREADS) lse_kernel(const T* __restrict__ z, i
 #pragma unroll
       for (int e = 0; e < 4; ++e) sum += v + e < V ? exp_of(q.v[e] - top) : T(0);
     }
-    out = top + log_of(warp_sum(sum));
-    loss = out - r[t];
+    rest = log_of(warp_sum(sum));
+    loss = top - r[t] + rest;
   }
-  if (lane == 0) lse[row] = out, value[row] = loss;
+  if (lane == 0) kept.top[row] = top, kept.rest[row] = rest, kept.miss[row] = expm1_of(-loss), value[row] = loss;
 }
 
 // z <- gz
 template <typename T>
 __global__ void __launch_bounds__(THREADS) score_grad_kernel(T* __restrict__ z, int ld, const int64_t* __restrict__ target,
-                                                             const T* __restrict__ lse, long long n, int V, const double* count,
-                                                             const T* grad) {
+                                                             Softmax<T> kept, long long n, int V, const double* count, const T* grad) {
   const T scale = count ? (T)((double)*grad / *count) : *grad;
   for (long long row = blockIdx.x * (long long)(THREADS / 32) + threadIdx.x / 32; row < n; row += gridDim.x * (long long)(THREADS / 32)) {
-    const T l = lse[row];
+    const T top = kept.top[row], rest = kept.rest[row], miss = kept.miss[row];
     const long long t = target[row];
     T* r = z + row * ld;
 #pragma unroll 2
     for (int v = threadIdx.x % 32 * 4; v < V; v += 128) {
       Four<T> q = *reinterpret_cast<const Four<T>*>(r + v);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) q.v[e] = l == T(INFINITY) ? T(0) : scale * (exp_of(q.v[e] - l) - (v + e == t ? T(1) : T(0)));
+      for (int e = 0; e < 4; ++e) q.v[e] = top == T(INFINITY) ? T(0) : scale * (v + e == t ? miss : exp_of(q.v[e] - top - rest));
       *reinterpret_cast<Four<T>*>(r + v) = q;
     }
   }
@@ -123,8 +135,8 @@ __global__ void __launch_bounds__(THREADS) score_grad_kernel(T* __restrict__ z, 
 // (images of n pixels, C) wherever they lie -> rows; those of pixels without a label are zero
 template <typename T>
 __global__ void __launch_bounds__(THREADS) rows_kernel(const T* __restrict__ src, long long img, long long pix, long long ch, long long n,
-                                                       int C, const T* __restrict__ lse, T* __restrict__ dst) {
-  src += blockIdx.z * img, lse += blockIdx.z * n, dst += blockIdx.z * n * C;
+                                                       int C, const T* __restrict__ top, T* __restrict__ dst) {
+  src += blockIdx.z * img, top += blockIdx.z * n, dst += blockIdx.z * n * C;
   __shared__ T tile[32][33];
   // 32 pixels x 32 channels, read along whichever direction is contiguous
   const int tx = threadIdx.x % 32, ty = threadIdx.x / 32;
@@ -134,7 +146,7 @@ __global__ void __launch_bounds__(THREADS) rows_kernel(const T* __restrict__ src
     for (int k = ty; k < 32; k += THREADS / 32) {
       const long long p = p0 + (ch == 1 ? k : tx);
       const int c = c0 + (ch == 1 ? tx : k);
-      tile[ch == 1 ? k : tx][ch == 1 ? tx : k] = p < n && c < C && lse[p] != T(INFINITY) ? src[p * pix + (long long)c * ch] : T(0);
+      tile[ch == 1 ? k : tx][ch == 1 ? tx : k] = p < n && c < C && top[p] != T(INFINITY) ? src[p * pix + (long long)c * ch] : T(0);
     }
     __syncthreads();
     for (int k = ty; k < 32; k += THREADS / 32)
@@ -183,37 +195,36 @@ __global__ void __launch_bounds__(THREADS) loss_kernel(const double* part, int b
   }
 }
 // ---- bf16 -----------------------------------------------------------------------------------------------
-// The tiles' sums of a pixel become its lse; the blocks' losses and labelled pixels go to `part`.
+// The tiles' sums of a pixel become what is kept of it; the blocks' losses and labelled pixels go to `part`.
 // (It starts while the kernel that writes those sums still runs, and a later piece's sums take the same place: read behind L1, never
 // through the read-only path.)
-__global__ void __launch_bounds__(THREADS) finish_kernel(mix::Scores s, int tiles, long long P, int V, float* lse, double* part) {
+__global__ void __launch_bounds__(THREADS) finish_kernel(mix::Scores s, int tiles, long long P, int V, Softmax<float> kept, double* part) {
   __shared__ double sm[2][THREADS / 32];
   behind_previous_kernel();
   double sum = 0, n = 0;
   for (long long p = blockIdx.x * (long long)THREADS + threadIdx.x; p < P; p += gridDim.x * (long long)THREADS) {
     const long long t = s.target[p];
     if (t == s.ignore) {
-      lse[p] = INFINITY;
+      kept.top[p] = INFINITY, kept.rest[p] = kept.miss[p] = 0.f;
       continue;
     }
     n += 1;
-    float out = NAN;
+    float top = NAN, rest = 0.f, loss = NAN;
     if (t >= 0 && t < V) {
-      float top = -INFINITY;
+      top = -INFINITY;
 #pragma unroll 8
       for (int k = 0; k < tiles; ++k) top = fmaxf(top, __ldcg(&s.part[k * P + p].x));  // (a NaN shows in the sum)
       float all = 0.f;
 #pragma unroll 8
       for (int k = 0; k < tiles; ++k) {
         const float2 v = __ldcg(s.part + k * P + p);
-        all += v.y * exp2f(v.x - top);
+        all += v.y * exp2f((v.x - top) * mix::LOG2E);
       }
-      out = (top + log2f(all)) * 0.69314718056f;
-      sum += (double)(out - __ldcg(s.hit + p));
-    } else {
-      sum = NAN;
+      rest = log2f(all);
+      loss = top - __ldcg(s.hit + p) + rest * 0.69314718056f;
     }
-    lse[p] = out;
+    sum += (double)loss;
+    kept.top[p] = top, kept.rest[p] = rest, kept.miss[p] = expm1f(-loss);
   }
   sum = warp_sum(sum), n = warp_sum(n);
   if (threadIdx.x % 32 == 0) sm[0][threadIdx.x / 32] = sum, sm[1][threadIdx.x / 32] = n;
@@ -233,7 +244,7 @@ __global__ void __launch_bounds__(THREADS) labelled_rows_kernel(const uint4* src
   }
 }
 // n pixels of images of S pixels, wherever they lie -> rows of three bf16 parts of float32 values, 8 bits each, zeros behind the last
-// channel of a part of Cp; pixels without a label are zeros if lse is given.  (An infinity would leave NaN in the lower parts: they
+// channel of a part of Cp; pixels without a label are zeros if top is given.  (An infinity would leave NaN in the lower parts: they
 // are zero there.)
 // A block takes 32 pixels x 64 channels, eight values to a thread either way (one at a time: 40 us instead of 15 for 131 072 pixels of
 // 50 channels).
@@ -242,7 +253,7 @@ struct Split {
   const float* src;
   long long S, img, pix, ch, p1, n;
   int C, Cp;
-  const float* lse;
+  const float* top;
   bf16* dst;
   unsigned blocks;
 };
@@ -253,7 +264,7 @@ __global__ void __launch_bounds__(THREADS) parts_kernel(const __grid_constant__ 
   int job = 0;
   while (job < 2 && block >= all.s[job].blocks) block -= all.s[job++].blocks;
   const Split& a = all.s[job];
-  const float *src = a.src, *lse = a.lse;
+  const float *src = a.src, *top = a.top;
   const long long S = a.S, img = a.img, pix = a.pix, ch = a.ch, p1 = a.p1, n = a.n;
   const int C = a.C, Cp = a.Cp, tx = threadIdx.x % 32, ty = threadIdx.x / 32, c0 = block % (Cp / 64) * 64;
   const long long p0 = block / (Cp / 64) * 32ll;
@@ -264,11 +275,11 @@ __global__ void __launch_bounds__(THREADS) parts_kernel(const __grid_constant__ 
     for (int k = 0; k < 8; ++k) {
       const int c = c0 + tx + 32 * (k / 4);
       const long long p = p0 + ty + 8 * (k % 4);
-      v[k] = p < n && c < C && !(lse && lse[p] == INFINITY) ? __ldg(src + (p1 + p) * pix + c) : 0.f;
+      v[k] = p < n && c < C && !(top && top[p] == INFINITY) ? __ldg(src + (p1 + p) * pix + c) : 0.f;
     }
   } else {
     const long long p = p0 + tx, b = (p1 + p) / S;
-    const bool on = p < n && !(lse && lse[p] == INFINITY);
+    const bool on = p < n && !(top && top[p] == INFINITY);
     const float* from = src + b * img + (p1 + p - b * S) * pix;
 #pragma unroll
     for (int k = 0; k < 8; ++k) v[k] = on && c0 + ty + 8 * k < C ? __ldg(from + (c0 + ty + 8 * k) * ch) : 0.f;
@@ -434,13 +445,13 @@ struct General {
   }
   View flat(const T* p, long long n, int wide) const { return View{p, n * wide, wide, 1}; }
   // labelled pixels of a piece as rows (several images one after the other)
-  void gather(const T* x, long long i, long long s, long long n, const T* lse) {
+  void gather(const T* x, long long i, long long s, long long n, const T* top) {
     const long long per = n < pieces.S ? n : pieces.S;
     const View v = view(x, i, s);
     for (long long k = 0; k * per < n; k += 32768) {  // (images are the grid's third dimension)
       const long long images = n / per - k < 32768 ? n / per - k : 32768;
       const dim3 tiles((unsigned)((per + 31) / 32), (unsigned)((d->C + 31) / 32 < 64 ? (d->C + 31) / 32 : 64), (unsigned)images);
-      rows_kernel<T><<<tiles, THREADS, 0, st>>>((const T*)v.ptr + k * v.img, v.img, v.pix, v.ch, per, d->C, lse + k * per,
+      rows_kernel<T><<<tiles, THREADS, 0, st>>>((const T*)v.ptr + k * v.img, v.img, v.pix, v.ch, per, d->C, top + k * per,
                                                 rows + k * per * d->C), MC_COUNT(1);
     }
   }
@@ -452,20 +463,20 @@ struct General {
   }
 
   int forward(const T* x, const T* w, const T* b, const int64_t* target, T* loss, void* kept) {
-    T* lse = (T*)((char*)kept + KEPT_HEAD);
     const long long P = d->B * d->S;
+    const Softmax<T> soft = softmax_of<T>(kept, P);
     int rc = MC_OK;
     if (few) {
       RowsArgs r = product(view(x, 0, 0), P, pieces.S, w, b);
       r.y.ptr = nullptr;
-      r.labels = mix::Labels{target, d->ignore_index, lse, value};
+      r.labels = mix::Labels{target, d->ignore_index, soft.top, soft.rest, soft.miss, value};
       rc = mix::simt_rows_launch(d->dtype, mix::EPI_SCORE_SUM, r, st);
     } else {
       each([&](long long i, long long s, long long n) {
         if (rc) return;
         const long long p = i * pieces.S + s;
         if ((rc = mix::simt_rows_launch(d->dtype, mix::EPI_LAYER, product(view(x, i, s), n, n < pieces.S ? n : pieces.S, w, b), st))) return;
-        lse_kernel<T><<<(unsigned)((n + 7) / 8), THREADS, 0, st>>>(z, ld, target + p, n, d->V, d->ignore_index, lse + p, value + p);
+        softmax_kernel<T><<<(unsigned)((n + 7) / 8), THREADS, 0, st>>>(z, ld, target + p, n, d->V, d->ignore_index, soft.at(p), value + p);
         MC_COUNT(1);
       });
     }
@@ -477,19 +488,20 @@ struct General {
   }
 
   int backward(const T* grad, const T* x, const T* w, const T* b, const int64_t* target, const void* kept, T* gx, T* gw, T* gb) {
-    T* lse = (T*)((char*)kept + KEPT_HEAD);
+    const long long P = d->B * d->S;
+    const Softmax<T> soft = softmax_of<T>((void*)kept, P);
     const double* count = d->reduction == MC_REDUCE_MEAN ? (const double*)kept : nullptr;
-    const long long P = d->B * d->S, VC = (long long)d->V * d->C;
+    const long long VC = (long long)d->V * d->C;
     int rc = MC_OK;
     each([&](long long i, long long s, long long n) {
       if (rc) return;
       const long long p = i * pieces.S + s, S = n < pieces.S ? n : pieces.S;
-      gather(x, i, s, n, lse + p);
+      gather(x, i, s, n, soft.top + p);
       RowsArgs r = product(flat(rows, n, d->C), n, n, w, b);
-      r.labels = mix::Labels{target + p, d->ignore_index, lse + p, nullptr, grad, count};
+      r.labels = mix::Labels{target + p, d->ignore_index, soft.top + p, soft.rest + p, soft.miss + p, nullptr, grad, count};
       if ((rc = mix::simt_rows_launch(d->dtype, few ? mix::EPI_SCORE_GRAD : mix::EPI_LAYER, r, st))) return;
       if (!few)
-        score_grad_kernel<T><<<grid_for(n, 8, 148 * 8), THREADS, 0, st>>>(z, ld, target + p, lse + p, n, d->V, count, grad), MC_COUNT(1);
+        score_grad_kernel<T><<<grid_for(n, 8, 148 * 8), THREADS, 0, st>>>(z, ld, target + p, soft.at(p), n, d->V, count, grad), MC_COUNT(1);
       if (gx) {
         r = RowsArgs{};
         r.a = View{z, S * (long long)ld, ld, 1}, r.w = w, r.wn = 1, r.wk = d->C, r.P = n, r.N = d->C, r.K = d->V, r.S = (int)S;
@@ -523,10 +535,9 @@ struct TensorCores {
     like = mc_mix_desc{d->B, d->S, d->C, d->V, 0, MC_ACT_NONE, MC_BF16, d->layout};
   }
   long long pixels() const { return d->B * d->S; }
-  size_t lse_bytes() const { return up256((size_t)pixels() * 4); }
   bool in_place() const { return mix::Work::in_place(&like, d->C); }
   size_t saved_bytes() const {
-    return KEPT_HEAD + lse_bytes() + (in_place() ? 0 : up256((size_t)pixels() * mix::pad8(d->C) * 2));
+    return kept_bytes<float>(pixels()) + (in_place() ? 0 : up256((size_t)pixels() * mix::pad8(d->C) * 2));
   }
   mix::TcRows rows_of(const void* p, long long n) const { return mix::TcRows{p, n, d->C, mix::pad8(d->C)}; }
   void labelled(const void* src, const mix::TcRows& r, const int64_t* target, cudaStream_t st) const {
@@ -539,7 +550,7 @@ struct TensorCores {
   int forward(mix::Work& k, const bf16* x, const bf16* w, const bf16* bias, const int64_t* target, float* loss, char* kept) const {
     mix::TcRows xr = rows_of(x, pixels());
     if (!in_place()) {
-      xr.p = kept ? kept + KEPT_HEAD + lse_bytes() : nullptr;
+      xr.p = kept ? kept + kept_bytes<float>(pixels()) : nullptr;
       k.lay_out(&like, x, xr, target, d->ignore_index);
       if (k.run() && !mix::Work::as_planes(&like, d->C)) labelled(xr.p, xr, target, k.st);
     }
@@ -561,7 +572,7 @@ struct TensorCores {
       if (k.rc) return k.rc;
       const int more = grid_for(n, THREADS, SUM_BLOCKS);
       k.did(launch_behind(finish_kernel, more, k.st, (mix::Scores)s, (int)tiles(n), (long long)n, (int)d->V,
-                          (float*)(kept + KEPT_HEAD) + p, (double*)(part + 2 * blocks)));
+                          softmax_of<float>(kept, P).at(p), (double*)(part + 2 * blocks)));
       if (k.rc) return k.rc;
       blocks += more;
     }
@@ -593,7 +604,7 @@ struct TensorCores {
     const Cut cut(*this);
     const bool planes = mix::Work::as_planes(&like, d->C);
     const long long S = planes ? d->S : P, B = planes ? d->B : 1, most = cut.images * cut.run;
-    mix::TcRows xr = rows_of(kept ? kept + KEPT_HEAD + lse_bytes() : nullptr, P);
+    mix::TcRows xr = rows_of(kept ? kept + kept_bytes<float>(P) : nullptr, P);
     if (in_place()) {
       xr = k.fresh(P, d->C);
       if (k.run()) labelled(x, xr, target, k.st);
@@ -627,11 +638,11 @@ struct TensorCores {
     const long long sums_all = (long long)d->V * (ldn / 4) + d->V;  // threads of add_piece_kernel
     float* acc = (float*)k.take(most < P ? ((size_t)d->V * ldn + d->V) * 4 : 0);
     if (!k.run()) return k.rc;
-    const float* lse = (const float*)(kept + KEPT_HEAD);
+    const Softmax<float> soft = softmax_of<float>((void*)kept, P);
     each([&](long long i, long long s, long long n) {
       if (k.rc) return;
       const long long p = i * S + s;
-      mix::Scores sc{target + p, d->ignore_index, nullptr, nullptr, lse + p, grad,
+      mix::Scores sc{target + p, d->ignore_index, nullptr, nullptr, {soft.top + p, soft.rest + p, soft.miss + p}, grad,
                      d->reduction == MC_REDUCE_MEAN ? (const double*)kept : nullptr};
       const mix::TcRows xp = rows_of((const bf16*)xr.p + p * xr.ld, n), gp{gz.p, n, d->V, gz.ld, 0, gz.blocks};
       k.did(mix::tc_scores_grad(xp, wr, bias, sc, gp, k.st));
@@ -679,12 +690,12 @@ struct FloatCores {
   mix::TcRows parts_of(const void* p, long long rows, int cols, int wide) const { return mix::TcRows{p, rows, cols, 3 * wide, 0, false, 3}; }
   static size_t bytes(long long rows, int wide) { return (size_t)rows * 3 * wide * 2; }
   static Split job(const float* src, long long S, long long img, long long pix, long long ch, long long p1, long long n, int C, int wide,
-                   const float* lse, void* dst) {
-    return Split{src, S, img, pix, ch, p1, n, C, wide, lse, (bf16*)dst, (unsigned)((n + 31) / 32 * (wide / 64))};
+                   const float* top, void* dst) {
+    return Split{src, S, img, pix, ch, p1, n, C, wide, top, (bf16*)dst, (unsigned)((n + 31) / 32 * (wide / 64))};
   }
-  Split pixels(const float* x, long long p, long long n, const float* lse, void* dst) const {
-    if (planes()) return job(x, d->S, d->S * d->C, 1, d->S, p, n, d->C, Cp, lse, dst);
-    return job(x, P, P * d->C, d->C, 1, p, n, d->C, Cp, lse, dst);
+  Split pixels(const float* x, long long p, long long n, const float* top, void* dst) const {
+    if (planes()) return job(x, d->S, d->S * d->C, 1, d->S, p, n, d->C, Cp, top, dst);
+    return job(x, P, P * d->C, d->C, 1, p, n, d->C, Cp, top, dst);
   }
   Split weights(const float* w, void* dst) const { return job(w, d->V, 0, d->C, 1, 0, d->V, d->C, Cp, nullptr, dst); }
   Split transposed(const float* w, void* dst) const { return job(w, d->C, 0, 1, d->C, 0, d->C, d->V, Vp, nullptr, dst); }
@@ -718,7 +729,7 @@ struct FloatCores {
       if (k.rc) return k.rc;
       const int more = grid_for(n, THREADS, SUM_BLOCKS);
       k.did(launch_behind(finish_kernel, more, k.st, (mix::Scores)s, (int)tiles(n), (long long)n, (int)d->V,
-                          (float*)(kept + KEPT_HEAD) + p, (double*)(part + 2 * blocks)));
+                          softmax_of<float>(kept, P).at(p), (double*)(part + 2 * blocks)));
       if (k.rc) return k.rc;
       blocks += more;
     }
@@ -758,13 +769,13 @@ struct FloatCores {
     float* acc = (float*)k.take(most < P ? ((size_t)d->V * ldn + d->V) * 4 : 0);
     if (!k.run()) return k.rc;
     const long long threads = (long long)d->V * (ldn / 4) + d->V;
-    const float* lse = (const float*)(kept + KEPT_HEAD);
+    const Softmax<float> soft = softmax_of<float>((void*)kept, P);
     each([&](long long i, long long s, long long n) {
       if (k.rc) return;
       const long long p = i * S + s;
-      k.did(split(Splits{{pixels(x, p, n, lse + p, x3), p ? Split{} : weights(w, w3), p || !gx ? Split{} : transposed(w, wt3)}}, k.st));
+      k.did(split(Splits{{pixels(x, p, n, soft.top + p, x3), p ? Split{} : weights(w, w3), p || !gx ? Split{} : transposed(w, wt3)}}, k.st));
       if (k.rc) return;
-      mix::Scores sc{target + p, d->ignore_index, nullptr, nullptr, lse + p, grad,
+      mix::Scores sc{target + p, d->ignore_index, nullptr, nullptr, {soft.top + p, soft.rest + p, soft.miss + p}, grad,
                      d->reduction == MC_REDUCE_MEAN ? (const double*)kept : nullptr, bias};
       const mix::TcRows xp = parts_of(x3, n, d->C, Cp), gp{gz.p, n, d->V, 64, 0, true, 3};
       k.did(mix::tc_scores_grad(xp, parts_of(w3, d->V, d->C, Cp), nullptr, sc, gp, k.st));
@@ -810,7 +821,8 @@ extern "C" {
 size_t mc_cross_entropy_saved_bytes(const mc_ce_desc* d) {
   if (classify::check_desc(d)) return 0;
   if (d->dtype == MC_BF16) return classify::TensorCores(d).saved_bytes();
-  return classify::KEPT_HEAD + classify::up256((size_t)d->B * d->S * classify::csize(d->dtype));
+  const long long pixels = d->B * d->S;
+  return d->dtype == MC_F64 ? classify::kept_bytes<double>(pixels) : classify::kept_bytes<float>(pixels);
 }
 size_t mc_cross_entropy_workspace_bytes(const mc_ce_desc* d, int32_t phase) {
   if (classify::check_desc(d)) return 0;

@@ -147,14 +147,22 @@ enum Epilogue {
   EPI_GATE = 1,   // two sums per output, rows n and N + n of w: g, u; y = h = act(g) u; z = [g|u] kept
   EPI_GATE_BWD = 2,  // acc = gh; g, u read from res (= [g|u]); y = [gh u act'(g) | gh act(g)]
   // a classifier of up to 128 classes, z = acc + bias (see Labels):
-  EPI_SCORE_SUM = 3,  // log-sum-exp and loss of every pixel
-  EPI_SCORE_GRAD = 4  // y = scale (exp(z - lse) - [label])
+  EPI_SCORE_SUM = 3,  // what is kept of every pixel's scores, and its loss
+  EPI_SCORE_GRAD = 4  // y = scale exp(z - top - rest), the label's scale miss
 };
-// Labels of the pixels.  lse: +infinity where there is none, NaN where it is no class.  scale: grad, or grad / count where mean is set.
+// What is kept of a pixel's scores: the largest one and the logarithm of the sum of exponentials of their differences from it, apart (their
+// sum, log-sum-exp, would be rounded by its own size: scores of 100 by 4e-6, of 10^7 by one), and the label's probability less one, e^-loss
+// - 1 (1 - p would be a rounding of one).  top: +infinity where there is no label, NaN where it is no class.
+template <typename T>
+struct Softmax {
+  T *top, *rest, *miss;
+  __host__ __device__ Softmax at(long long p) const { return Softmax{top + p, rest + p, miss + p}; }
+};
+// Labels of the pixels.  scale: grad, or grad / count where mean is set.
 struct Labels {
   const int64_t* target;
   long long ignore;
-  void *lse, *value;
+  void *top, *rest, *miss, *value;
   const void* grad;
   const double* count;
 };
@@ -218,8 +226,8 @@ struct Scores {
   // tc_scores_sum: the largest score of every tile of classes and the sum of exp(score - it), [tile][pixel]; the label's score
   float2* part;
   float* hit;
-  // tc_scores_grad: log-sum-exp (+infinity: no label, NaN: a bad one), gradient of the loss, pixels that it is divided by (or null)
-  const float* lse;
+  // tc_scores_grad: what is kept, `rest` in base 2; gradient of the loss, pixels that it is divided by (or null)
+  Softmax<const float> kept;
   const float* grad;
   const double* count;
   const float* bias32;  // of float32 layers
@@ -228,7 +236,7 @@ struct Scores {
 // tensors in parts: the products of float32 values, six products of parts each, small ones first (the accumulators truncate)
 int tc_scores_tiles(long long P, int C, int V, int parts = 1);  // tiles of classes that tc_scores_sum leaves sums of
 int tc_scores_sum(const TcRows& x, const TcRows& w, const bf16* bias, const Scores& s, cudaStream_t st);
-// gz = grad / count (exp(z - lse) - [label]), in blocks
+// gz = grad / count exp(z - top - rest), the label's grad / count miss, in blocks
 int tc_scores_grad(const TcRows& x, const TcRows& w, const bf16* bias, const Scores& s, const TcRows& gz, cudaStream_t st);
 // gx = g w^T in float32, g in blocks and parts, w (N, K) in parts; gx rows of ld floats (w.rows of them used), or planes of S pixels
 int tc_input_grad32(const TcRows& g, const TcRows& w, float* gx, long long ld, long long S, cudaStream_t st);

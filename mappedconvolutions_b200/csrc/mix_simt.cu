@@ -153,6 +153,8 @@ struct RowsFlags {
 
 __device__ __forceinline__ float log_(float v) { return logf(v); }
 __device__ __forceinline__ double log_(double v) { return log(v); }
+__device__ __forceinline__ float expm1_(float v) { return expm1f(v); }
+__device__ __forceinline__ double expm1_(double v) { return expm1(v); }
 // Rows of class scores, all classes of a pixel among sixteen neighbouring threads.
 template <typename T, int EPI, int TN>
 __device__ __forceinline__ void score_rows(const RowsArgs& a, const T (&acc)[8][TN / 16], long long p0, int pixels, int classes,
@@ -194,16 +196,18 @@ __device__ __forceinline__ void score_rows(const RowsArgs& a, const T (&acc)[8][
         for (int o = 8; o; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o), hit += __shfl_xor_sync(~0u, hit, o);
         if (in && tc == 0) {
           const bool none = t == a.labels.ignore, bad = !none && (t < 0 || t >= classes);
-          const T lse = none ? T(INFINITY) : bad ? T(NAN) : top + log_(sum);
-          ((T*)a.labels.lse)[p] = lse;
-          ((T*)a.labels.value)[p] = none ? T(0) : lse - hit;
+          const T rest = log_(sum), loss = none ? T(0) : bad ? T(NAN) : top - hit + rest;
+          ((T*)a.labels.top)[p] = none ? T(INFINITY) : bad ? T(NAN) : top;
+          ((T*)a.labels.rest)[p] = rest;
+          ((T*)a.labels.value)[p] = loss;
+          ((T*)a.labels.miss)[p] = expm1_(-loss);
         }
       } else {
-        const T lse = ((const T*)a.labels.lse)[p];
+        const T top = ((const T*)a.labels.top)[p], rest = ((const T*)a.labels.rest)[p], miss = ((const T*)a.labels.miss)[p];
 #pragma unroll
         for (int j = 0; j < 2 * W; ++j) {
           const int n = j / W * (TN / 2) + W * tc + j % W;
-          z[j] = lse == T(INFINITY) ? T(0) : scale * (exp_(z[j] - lse) - (n == t ? T(1) : T(0)));
+          z[j] = top == T(INFINITY) ? T(0) : scale * (n == t ? miss : exp_(z[j] - top - rest));
         }
         if (in) {
           T* y = (T*)a.y.ptr + p * a.y.pix;

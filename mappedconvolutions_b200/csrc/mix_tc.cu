@@ -179,7 +179,7 @@ enum Mode {
   GATE_BWD = 2,  // [g|u] as above from the first operands, gh from the second: y0 = gh u act'(g), y1 = gh act(g)
   ACT_BWD = 3,   // y = r act'(A B^T + bias)
   SCORE_SUM = 4, // softmax sums of z = A B^T + bias over the tile's columns, the label's z
-  SCORE_GRAD = 5,// y = scale (exp(z - lse) - [label])
+  SCORE_GRAD = 5,// y = scale exp(z - top - rest), the label's scale (e^-loss - 1)
   FLOATS = 6     // y = A B^T in float32
 };
 // Products of float32 values in three bf16 parts each, 0 the largest: (2,0) (0,2) (1,1) (1,0) (0,1) (0,0).  The others are below
@@ -428,7 +428,7 @@ __device__ __forceinline__ void read_out(const GemmArgs& g, int set, uint32_t ra
 
 // Read-out warps of a classifier: thread = pixel, 32 classes at a time (sixteen: 304 and 328 us instead of 297 and 294
 // for 40 968 pixels x 10 242 classes x 256 channels).
-// SCORE_SUM keeps the running maximum and sum of the tile's classes, in base 2; SCORE_GRAD leaves bf16 gradients of the scores in the
+// SCORE_SUM keeps the running maximum and sum of the tile's classes; SCORE_GRAD leaves bf16 gradients of the scores in the
 // staged tiles.  Classes behind the last one have a bias of -infinity: exp makes zeros of them.
 template <int MODE, int BN>
 __device__ __forceinline__ void read_scores(const GemmArgs& g, int set, uint32_t rank, float* bias_s, uint32_t out0,
@@ -444,14 +444,14 @@ __device__ __forceinline__ void read_scores(const GemmArgs& g, int set, uint32_t
   float scale = 0.f;
   if (MODE == SCORE_GRAD) scale = g.sc.count ? (float)((double)*g.sc.grad / *g.sc.count) : *g.sc.grad;
   uint32_t it = 0, i = 0;
-  // labels and log-sum-exps of a tile are fetched a tile ahead
+  // labels and what is kept of a tile are fetched a tile ahead
   long long t_next = 0;
-  float l_next = INFINITY;
+  float top_next = INFINITY, rest_next = 0.f, miss_next = 0.f;
   const auto fetch_pixel = [&](const TileWalk& w) {
     const uint32_t p = (w.m() * 2 + rank) * TILE + row;
     if (!w.more() || p >= (uint32_t)g.rows) return;
     t_next = __ldg((const long long*)g.sc.target + p);
-    if (MODE == SCORE_GRAD) l_next = __ldg(g.sc.lse + p);
+    if (MODE == SCORE_GRAD) top_next = __ldg(g.sc.kept.top + p), rest_next = __ldg(g.sc.kept.rest + p), miss_next = __ldg(g.sc.kept.miss + p);
   };
   fetch_pixel(TileWalk(g, set, 2));
   for (TileWalk w(g, set, 2); w.more(); w.next(), ++it) {
@@ -473,16 +473,16 @@ __device__ __forceinline__ void read_scores(const GemmArgs& g, int set, uint32_t
     const uint32_t p = tile0 + row;
     const bool in = p < (uint32_t)g.rows;
     int label = -1;  // of this tile's columns
-    float lse2 = INFINITY;
+    float kept = INFINITY, rest = 0.f, miss = 0.f;  // (kept: the largest score of all)
     if (in) {
       const long long t = t_next;
       if (t >= n0 && t < n0 + BN && t < g.N && t != g.sc.ignore) label = (int)(t - n0);
-      if (MODE == SCORE_GRAD) lse2 = l_next * LOG2E;
+      if (MODE == SCORE_GRAD) kept = top_next, rest = rest_next, miss = miss_next;
     }
     TileWalk ahead = w;
     ahead.next();
     fetch_pixel(ahead);
-    const bool dead = lse2 == INFINITY;
+    const bool dead = kept == INFINITY;
     int live = (g.N - n0 + PW - 1) / PW;  // pieces with classes; a staged tile is filled up with zeros
     if (MODE == SCORE_GRAD) live = (live + PER - 1) / PER * PER;
     if (live > NP) live = NP;
@@ -512,7 +512,6 @@ __device__ __forceinline__ void read_scores(const GemmArgs& g, int set, uint32_t
         const bool any = __any_sync(~0u, here >= 0);
         if (MODE == SCORE_SUM) {
           if (any) MC_HALF hit = here == 2 * j ? z[j].x : here == 2 * j + 1 ? z[j].y : hit;
-          MC_HALF z[j] = mul2(z[j], two(LOG2E));
           float t[PW / 2];
           MC_HALF t[j] = fmaxf(z[j].x, z[j].y);
 #pragma unroll
@@ -521,8 +520,9 @@ __device__ __forceinline__ void read_scores(const GemmArgs& g, int set, uint32_t
             for (int j = 0; j < o; ++j) t[j] = fmaxf(t[j], t[j + o]);
           const float m = fmaxf(top, t[0]);
           const float base = m == -INFINITY ? 0.f : m;  // (nothing but ruled-out classes so far: sums of zeros)
-          sum *= exp2_(top - base);
-          MC_HALF z[j] = exp2_2(add2(z[j], two(-base)));
+          // (differences first: they lose nothing, and the largest score's exponential is one, its products with log2(e) rounded or not)
+          sum *= exp2_((top - base) * LOG2E);
+          MC_HALF z[j] = exp2_2(mul2(add2(z[j], two(-base)), two(LOG2E)));
 #pragma unroll
           for (int o = PW / 4; o; o /= 2)
 #pragma unroll
@@ -530,8 +530,8 @@ __device__ __forceinline__ void read_scores(const GemmArgs& g, int set, uint32_t
           sum += z[0].x + z[0].y;
           top = m;
         } else {
-          MC_HALF z[j] = exp2_2(fma2(z[j], two(LOG2E), two(-lse2)));
-          if (any) MC_HALF z[j] = add2(z[j], make_float2(here == 2 * j ? -1.f : 0.f, here == 2 * j + 1 ? -1.f : 0.f));
+          MC_HALF z[j] = exp2_2(fma2(add2(z[j], two(-kept)), two(LOG2E), two(-rest)));
+          if (any) MC_HALF z[j] = make_float2(here == 2 * j ? miss : z[j].x, here == 2 * j + 1 ? miss : z[j].y);
           MC_HALF z[j] = dead ? two(0.f) : mul2(z[j], two(scale));
           if (staged) {
             const uint32_t at = at0 + (i & mask) * C::CH_BYTES, j0 = pc % PER * (PW / 8);
