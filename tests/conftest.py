@@ -52,7 +52,7 @@ def op_binding(request, monkeypatch):
 
 # Modules after each of whose tests no bounded device-side wait may have run out: one that gives up after the results are
 # stored shows in the device status only.
-_WAITS_CHECKED = {"test_gpu_cross_entropy", "test_gpu_confident_loss", "test_gpu_loss_pieces", "test_gpu_long_offsets", "test_gpu_mix", "test_gpu_mix_paths", "test_gpu_mix_strict", "test_gpu_mix_autograd"}
+_WAITS_CHECKED = {"test_gpu_cross_entropy", "test_gpu_loss_sums", "test_gpu_confident_loss", "test_gpu_loss_pieces", "test_gpu_long_offsets", "test_gpu_mix", "test_gpu_mix_paths", "test_gpu_mix_strict", "test_gpu_mix_autograd"}
 
 
 @pytest.fixture(autouse=True)
