@@ -793,20 +793,18 @@ __global__ void __launch_bounds__(THREADS) stats_kernel(const __grid_constant__ 
   } else if (b < a.B) {
     const Part<CT>* part = (const Part<CT>*)a.part + b * a.tiles * a.grps;
     const auto at = [&](int col) { return part + (long long)col * a.grps + group_slot(a, col, g); };
-    const long long step = (long long)a.cols * a.grps;  // from pixels to pixels
-    const int count = a.tiles / a.cols;
     // (the first tile's column that holds the group's first channel; parts of other columns may be empty)
     base = __ldcg(&at(g * a.Cg / a.column)->mean);
-    if (!a.wide) {
+    if (a.C <= a.column) {  // every part has room for every group
       const Part<CT>* p = at(0);
 #pragma unroll 4
-      for (int i = me; i < count; i += sub) merge(p + i * step);
+      for (int i = me; i < a.tiles; i += sub) merge(p + (long long)i * a.grps);
     } else {  // the columns that hold any of the group, pixel by pixel of a row
+      const long long step = (long long)a.cols * a.grps;
+      const int count = a.tiles / a.cols;
       int done = 0;
-      const bool all = a.C <= a.column;
-      for (int r = 0; r < (all ? 1 : a.R); ++r) {
-        const int f = r * a.C + g * a.Cg, lo = max(all ? 0 : f / a.column, done);
-        const int hi = all ? a.cols : min((f + a.Cg - 1) / a.column + 1, a.cols), wide = hi - lo;
+      for (int r = 0; r < a.R; ++r) {
+        const int f = r * a.C + g * a.Cg, lo = max(f / a.column, done), hi = min((f + a.Cg - 1) / a.column + 1, a.cols), wide = hi - lo;
         if (wide <= 0) continue;
         for (long long i = me; i < (long long)wide * count; i += sub) merge(at(lo + (int)(i % wide)) + i / wide * step);
         done = hi;
@@ -828,19 +826,18 @@ __global__ void __launch_bounds__(THREADS) coef_kernel(const __grid_constant__ A
   let_next_kernel_start();
   behind_previous_kernel();
   const long long b = blockIdx.x / a.G;
-  const int g = (int)(blockIdx.x % a.G), count = rows ? a.tiles / a.cols : a.segs;
-  const long long step = rows ? (long long)a.cols * a.chans : 1;
-  const bool once = rows && a.C > a.column;
-  const int places = !rows || !a.wide ? 1 : once ? a.R : a.cols;  // of a channel in a row of pixels
+  const bool once = rows && a.C > a.column;  // a column has room for some channels only; else each part has a place for every one
+  const int g = (int)(blockIdx.x % a.G), count = once ? a.tiles / a.cols : rows ? a.tiles : a.segs;
+  const long long step = once ? (long long)a.cols * a.chans : rows ? a.chans : 1;
   Two<double>* sums = (Two<double>*)a.sums + b * a.C;
   double gu = 0, gv = 0;
   for (int i0 = 0; i0 < a.Cg; i0 += THREADS / sub) {
     const int i = i0 + threadIdx.x / sub, c = g * a.Cg + i;
     double u = 0, v = 0;
     if (i < a.Cg) {
-      for (int r = 0; r < places; ++r) {
-        const int f = r * a.C + c, col = once ? f / a.column : r;
-        if (rows && col >= a.cols) break;
+      for (int r = 0; r < (once ? a.R : 1); ++r) {
+        const int f = r * a.C + c, col = once ? f / a.column : 0;
+        if (once && col >= a.cols) break;
         const Two<CT>* part = (const Two<CT>*)a.part +
                               (rows ? (b * a.tiles + col) * a.chans + (once ? f - col * a.column : c) : (b * a.C + c) * count);
 #pragma unroll 8
@@ -1015,7 +1012,7 @@ static int three(const Plan& p, cudaStream_t st) {
   if (rc) return rc;
   const long long groups = a.B * a.G;
   if (BWD) {
-    int sub = sharers(a.B * a.C, ROWS ? a.tiles / a.cols : a.segs);
+    int sub = sharers(a.B * a.C, !ROWS ? a.segs : a.C > a.column ? a.tiles / a.cols : a.tiles);
     while (sub < 32 && sub * a.Cg < THREADS) sub *= 2;  // (a block has one group's channels only)
     rc = launch(coef_kernel<T>, (unsigned)groups, true, st, (Args)a, (bool)ROWS, (int)sub);
     a.param_blocks = a.gw || a.gb ? (a.C + THREADS / 8 - 1) / (THREADS / 8) : 0;
