@@ -472,53 +472,58 @@ __device__ __forceinline__ void rows_stats(const Args& a, Shared<CT, N>& sm, lon
   }
   __syncthreads();
   // what the threads of a group's channels left, a few threads to a group
-  const int each = J ? a.Cg / N : a.Cg * a.R, entries = a.wide ? min(each, J ? 256 : a.column) : each * a.lanes;
-  const int sub = entries > 16 ? 32 : entries > 8 ? 16 : entries > 4 ? 8 : 4, me = threadIdx.x % sub;
   Part<CT>* out = (Part<CT>*)a.part + (b * a.tiles + tile) * a.grps;
-  for (int s0 = 0; s0 < a.grps; s0 += THREADS / sub) {
-    const int slot = s0 + threadIdx.x / sub;
-    const bool on = slot < a.grps;
-    int g = slot + first_group(a, p.col);
-    if (g >= a.G) g -= a.G;
-    // f(part) of every one of this group's in the column, this thread's share of them
-    const auto each_entry = [&](auto f) {
-      if (!on) return;
-      if (!a.wide) {
-        for (int i = me; i < entries; i += sub) {
-          const int l = i / each, k = i - l * each;
-          int e = 0, j;
-          if constexpr (J) {
-            j = g * each + k;
-          } else {
-            const int rr = k / a.Cg, at = rr * a.C + g * a.Cg + k - rr * a.Cg;
-            j = at / N, e = at % N;
-          }
-          const Part<CT> v = sm.part[e][l * p.vc + j];
-          if (v.n > CT(0)) f(v);
-        }
-      } else {  // (one lane: the group's elements in each pixel of the row, as far as the column reaches)
-        const int from = p.col * a.column, to = from + p.vc * N;
-        for (int r = 0; r < a.R; ++r) {
-          const int lo = max(r * a.C + g * a.Cg, from) - from, hi = min(r * a.C + (g + 1) * a.Cg, to) - from;
-          for (int i = (J ? lo / N : lo) + me; i < (J ? hi / N : hi); i += sub) {
-            const Part<CT> v = J ? sm.part[0][i] : sm.part[i % N][i / N];
+  const auto groups = [&](auto wide) {
+    constexpr bool WIDE = decltype(wide)::value;
+    const int each = J ? a.Cg / N : a.Cg * a.R, entries = WIDE ? min(each, J ? 256 : a.column) : each * a.lanes;
+    const int sub = entries > 16 ? 32 : entries > 8 ? 16 : entries > 4 ? 8 : 4, me = threadIdx.x % sub;
+    const int g0 = WIDE ? first_group(a, p.col) : 0;
+    for (int s0 = 0; s0 < a.grps; s0 += THREADS / sub) {
+      const int slot = s0 + threadIdx.x / sub;
+      const bool on = slot < a.grps;
+      int g = slot + g0;
+      if (WIDE && g >= a.G) g -= a.G;
+      // f(part) of every one of this group's in the column, this thread's share of them
+      const auto each_entry = [&](auto f) {
+        if (!on) return;
+        if constexpr (!WIDE) {
+          for (int i = me; i < entries; i += sub) {
+            const int l = i / each, k = i - l * each;
+            int e = 0, j;
+            if constexpr (J) {
+              j = g * each + k;
+            } else {
+              const int rr = k / a.Cg, at = rr * a.C + g * a.Cg + k - rr * a.Cg;
+              j = at / N, e = at % N;
+            }
+            const Part<CT> v = sm.part[e][l * p.vc + j];
             if (v.n > CT(0)) f(v);
           }
+        } else {  // (one lane: the group's elements in each pixel of the row, as far as the column reaches)
+          const int from = p.col * a.column, to = from + p.vc * N;
+          for (int r = 0; r < a.R; ++r) {
+            const int lo = max(r * a.C + g * a.Cg, from) - from, hi = min(r * a.C + (g + 1) * a.Cg, to) - from;
+            for (int i = (J ? lo / N : lo) + me; i < (J ? hi / N : hi); i += sub) {
+              const Part<CT> v = J ? sm.part[0][i] : sm.part[i % N][i / N];
+              if (v.n > CT(0)) f(v);
+            }
+          }
         }
-      }
-    };
-    CT cnt = CT(0), sum = CT(0), m2 = CT(0);
-    each_entry([&](const Part<CT>& w) { cnt += w.n, sum += w.n * w.mean; });
-    for (int o = sub / 2; o; o >>= 1) cnt += __shfl_xor_sync(~0u, cnt, o), sum += __shfl_xor_sync(~0u, sum, o);
-    const CT mean = cnt > CT(0) ? sum / cnt : CT(0);
-    CT c = CT(0);  // what the roundings of that sum left of the differences
-    each_entry([&](const Part<CT>& w) {
-      const CT d = w.mean - mean;
-      m2 += w.m2 + w.n * d * d, c += w.n * d;
-    });
-    for (int o = sub / 2; o; o >>= 1) m2 += __shfl_xor_sync(~0u, m2, o), c += __shfl_xor_sync(~0u, c, o);
-    if (on && me == 0) out[slot] = centred(cnt, mean, c, m2);
-  }
+      };
+      CT cnt = CT(0), sum = CT(0), m2 = CT(0);
+      each_entry([&](const Part<CT>& w) { cnt += w.n, sum += w.n * w.mean; });
+      for (int o = sub / 2; o; o >>= 1) cnt += __shfl_xor_sync(~0u, cnt, o), sum += __shfl_xor_sync(~0u, sum, o);
+      const CT mean = cnt > CT(0) ? sum / cnt : CT(0);
+      CT c = CT(0);  // what the roundings of that sum left of the differences
+      each_entry([&](const Part<CT>& w) {
+        const CT d = w.mean - mean;
+        m2 += w.m2 + w.n * d * d, c += w.n * d;
+      });
+      for (int o = sub / 2; o; o >>= 1) m2 += __shfl_xor_sync(~0u, m2, o), c += __shfl_xor_sync(~0u, c, o);
+      if (on && me == 0) out[slot] = centred(cnt, mean, c, m2);
+    }
+  };
+  a.wide ? groups(std::true_type()) : groups(std::false_type());
 }
 
 template <typename T, int ACT, bool J, typename CT, int N>
@@ -794,7 +799,7 @@ __global__ void __launch_bounds__(THREADS) stats_kernel(const __grid_constant__ 
     const Part<CT>* part = (const Part<CT>*)a.part + b * a.tiles * a.grps;
     const auto at = [&](int col) { return part + (long long)col * a.grps + group_slot(a, col, g); };
     // (the first tile's column that holds the group's first channel; parts of other columns may be empty)
-    base = __ldcg(&at(g * a.Cg / a.column)->mean);
+    base = __ldcg(&at(a.wide ? g * a.Cg / a.column : 0)->mean);
     if (a.C <= a.column) {  // every part has room for every group
       const Part<CT>* p = at(0);
 #pragma unroll 4
@@ -827,24 +832,27 @@ __global__ void __launch_bounds__(THREADS) coef_kernel(const __grid_constant__ A
   behind_previous_kernel();
   const long long b = blockIdx.x / a.G;
   const bool once = rows && a.C > a.column;  // a column has room for some channels only; else each part has a place for every one
-  const int g = (int)(blockIdx.x % a.G), count = once ? a.tiles / a.cols : rows ? a.tiles : a.segs;
-  const long long step = once ? (long long)a.cols * a.chans : rows ? a.chans : 1;
+  const int g = (int)(blockIdx.x % a.G);
   Two<double>* sums = (Two<double>*)a.sums + b * a.C;
   double gu = 0, gv = 0;
   for (int i0 = 0; i0 < a.Cg; i0 += THREADS / sub) {
     const int i = i0 + threadIdx.x / sub, c = g * a.Cg + i;
     double u = 0, v = 0;
-    if (i < a.Cg) {
-      for (int r = 0; r < (once ? a.R : 1); ++r) {
-        const int f = r * a.C + c, col = once ? f / a.column : 0;
-        if (once && col >= a.cols) break;
-        const Two<CT>* part = (const Two<CT>*)a.part +
-                              (rows ? (b * a.tiles + col) * a.chans + (once ? f - col * a.column : c) : (b * a.C + c) * count);
+    const auto add = [&](const Two<CT>* part, int count, long long step) {
 #pragma unroll 8
-        for (int k = threadIdx.x % sub; k < count; k += sub) {
-          const Two<CT> t = peek(part + k * step);
-          u += t.a, v += t.b;
-        }
+      for (int k = threadIdx.x % sub; k < count; k += sub) {
+        const Two<CT> t = peek(part + k * step);
+        u += t.a, v += t.b;
+      }
+    };
+    if (i < a.Cg && !once) {
+      const int count = rows ? a.tiles : a.segs;
+      add((const Two<CT>*)a.part + (rows ? b * count * a.C + c : (b * a.C + c) * count), count, rows ? a.C : 1);
+    } else if (i < a.Cg) {
+      for (int r = 0; r < a.R; ++r) {
+        const int f = r * a.C + c, col = f / a.column;
+        if (col >= a.cols) break;
+        add((const Two<CT>*)a.part + (b * a.tiles + col) * a.chans + f - col * a.column, a.tiles / a.cols, (long long)a.cols * a.chans);
       }
     }
     for (int o = sub / 2; o; o >>= 1) u += __shfl_xor_sync(~0u, u, o), v += __shfl_xor_sync(~0u, v, o);
