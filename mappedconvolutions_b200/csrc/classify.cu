@@ -306,18 +306,31 @@ __global__ void __launch_bounds__(THREADS) parts_kernel(const __grid_constant__ 
   }
 }
 
-// acc (+)= the shares of one piece, in order: sums (V, C) in rows of ldn (a multiple of 4), and V column sums; the last piece's
-// go to gw and gb, rounded.  Four sums to a thread.
+// (V, C) -> (C, 2 pad): every channel's weights twice, zeros behind the last class of each (pad: a multiple of 8)
+__global__ void __launch_bounds__(THREADS) twice_transposed_kernel(const bf16* __restrict__ w, bf16* __restrict__ dst, int V, int C, int pad) {
+  const int c = blockIdx.x * THREADS + threadIdx.x;
+  if (c >= C) return;
+  for (int v0 = 0; v0 < pad; v0 += 8) {
+    __align__(16) bf16 q[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) q[e] = v0 + e < V ? w[(long long)(v0 + e) * C + c] : bf16(0.f);
+#pragma unroll
+    for (int part = 0; part < 2; ++part)
+      *reinterpret_cast<uint4*>(dst + (long long)c * 2 * pad + part * pad + v0) = *reinterpret_cast<const uint4*>(q);
+  }
+}
+// acc (+)= the shares of one piece, in order: sums (V, C) in rows of ldn (a multiple of 4), and V column sums, of shares of R rows; the
+// last piece's go to gw and gb, rounded.  Four sums to a thread.
 template <typename T>
 __global__ void __launch_bounds__(THREADS) add_piece_kernel(const float* __restrict__ part, const float* __restrict__ csum, int splits,
-                                                            int V, int C, int ldn, float* __restrict__ acc, bool first, bool last,
-                                                            T* gw, T* gb) {
-  const long long nw = (long long)V * (ldn / 4), i = blockIdx.x * (long long)THREADS + threadIdx.x;
+                                                            int V, int R, int C, int ldn, float* __restrict__ acc, bool first,
+                                                            bool last, T* gw, T* gb) {
+  const long long nw = (long long)V * (ldn / 4), step = (long long)R * (ldn / 4), i = blockIdx.x * (long long)THREADS + threadIdx.x;
   if (i < nw) {
     float4 s = first ? make_float4(0.f, 0.f, 0.f, 0.f) : reinterpret_cast<const float4*>(acc)[i];
 #pragma unroll 8
     for (int j = 0; j < splits; ++j) {
-      const float4 v = __ldcs(reinterpret_cast<const float4*>(part) + j * nw + i);
+      const float4 v = __ldcs(reinterpret_cast<const float4*>(part) + j * step + i);
       s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
     }
     if (!last) {
@@ -332,7 +345,7 @@ __global__ void __launch_bounds__(THREADS) add_piece_kernel(const float* __restr
   } else if (i < nw + V) {
     const long long v = i - nw;
     float s = first ? 0.f : acc[4 * nw + v];
-    for (int j = 0; j < splits; ++j) s += csum[j * (long long)V + v];
+    for (int j = 0; j < splits; ++j) s += csum[j * (long long)R + v];
     if (!last) acc[4 * nw + v] = s;
     else if (gb) stv(gb + v, s);
   }
@@ -536,6 +549,7 @@ struct TensorCores {
   }
   long long pixels() const { return d->B * d->S; }
   bool in_place() const { return mix::Work::in_place(&like, d->C); }
+  int parts() const { return d->V <= 32 ? 2 : 1; }  // of gz, see backward
   size_t saved_bytes() const {
     return kept_bytes<float>(pixels()) + (in_place() ? 0 : up256((size_t)pixels() * mix::pad8(d->C) * 2));
   }
@@ -591,7 +605,7 @@ struct TensorCores {
       const mc_ce_desc* d = t.d;
       const bool whole = !mix::Work::as_planes(&t.like, d->C);  // (the output need not be cut at images)
       const long long S = whole ? d->B * d->S : d->S, B = whole ? 1 : d->B;
-      long long n = (long long)(PIECE_TC / ((size_t)mix::pad8(d->V) * 2)) / 256 * 256;
+      long long n = (long long)(PIECE_TC / ((size_t)mix::pad8(d->V) * 2 * t.parts())) / 256 * 256;
       if (n < 256) n = 256;
       images = n >= S ? n / S : 1;
       if (images > B) images = B;
@@ -609,9 +623,19 @@ struct TensorCores {
       xr = k.fresh(P, d->C);
       if (k.run()) labelled(x, xr, target, k.st);
     }
-    const mix::TcRows wr = k.weight(w, d->V, d->C), wt = k.weight_t(w, d->V, d->C);
+    const mix::TcRows wr = k.weight(w, d->V, d->C);
+    // Up to 32 classes: gz in two bf16 parts side by side, against every weight twice.  Both products' stages hold 64 columns in any case:
+    // gx and gW are rounded once, not twice, at no cost.  (More classes: see read_scores.)
+    const int pad = mix::pad8(d->V), parts = this->parts(), across = parts * (parts > 1 ? pad : d->V);
+    mix::TcRows wt{nullptr, d->C, across, parts * pad};
+    if (parts > 1) {
+      wt.p = k.take((size_t)d->C * wt.ld * 2);
+      if (k.run() && gx) twice_transposed_kernel<<<(d->C + THREADS - 1) / THREADS, THREADS, 0, k.st>>>(w, (bf16*)wt.p, d->V, d->C, pad), MC_COUNT(1);
+    } else {
+      wt = k.weight_t(w, d->V, d->C);
+    }
     // (up to 64 classes are one block across: rows of their own length are shorter)
-    mix::TcRows gz{nullptr, most, d->V, d->V > 64 ? 64 : mix::pad8(d->V), 0, d->V > 64};
+    mix::TcRows gz{nullptr, most, across, d->V > 64 ? 64 : parts * pad, 0, d->V > 64};
     gz.p = k.take(gz.blocks ? gz.block_bytes() : (size_t)most * gz.ld * 2);
     mix::TcRows out = rows_of(nullptr, most);
     if (!planes && !in_place()) out = k.fresh(most, d->C);
@@ -629,9 +653,9 @@ struct TensorCores {
     each([&](long long, long long, long long n) {
       if (n == seen[0] || n == seen[1]) return;
       seen[1] = seen[0], seen[0] = n;
-      const size_t f = mix::tc_outer_floats(n, d->V, 1, d->C, &splits, &ldn);
+      const size_t f = mix::tc_outer_floats(n, across, 1, d->C, &splits, &ldn);
       if (f > floats) floats = f;
-      if ((size_t)splits * d->V > sums) sums = (size_t)splits * d->V;
+      if ((size_t)splits * across > sums) sums = (size_t)splits * across;
     });
     float* part = (float*)k.take(floats * 4);
     float* csum = (float*)k.take(sums * 4);
@@ -643,8 +667,8 @@ struct TensorCores {
       if (k.rc) return;
       const long long p = i * S + s;
       mix::Scores sc{target + p, d->ignore_index, nullptr, nullptr, {soft.top + p, soft.rest + p, soft.miss + p}, grad,
-                     d->reduction == MC_REDUCE_MEAN ? (const double*)kept : nullptr};
-      const mix::TcRows xp = rows_of((const bf16*)xr.p + p * xr.ld, n), gp{gz.p, n, d->V, gz.ld, 0, gz.blocks};
+                     d->reduction == MC_REDUCE_MEAN ? (const double*)kept : nullptr, parts > 1 ? pad / 8 : 0};
+      const mix::TcRows xp = rows_of((const bf16*)xr.p + p * xr.ld, n), gp{gz.p, n, across, gz.ld, 0, gz.blocks};
       k.did(mix::tc_scores_grad(xp, wr, bias, sc, gp, k.st));
       if (gx && !k.rc) {
         mix::TcRows to = rows_of(out.p, n);
@@ -654,13 +678,15 @@ struct TensorCores {
         if (!planes && !in_place() && !k.rc) k.did(mix::copy_rows(to.p, gx + p * d->C, n, to.ld, d->C, k.st));
       }
       if ((gw || gb) && !k.rc) {
-        mix::tc_outer_floats(n, d->V, 1, d->C, &splits, &ldn);
+        mix::tc_outer_floats(n, across, 1, d->C, &splits, &ldn);
         k.did(mix::tc_outer(gp, mix::TcRows{}, xp, part, csum, k.st));
         if (k.rc) return;
+        // (a part's sums are a share of their own)
+        const int shares = splits * parts, rows = across / parts;
         // (many shares of few sums: several threads for each)
-        if (splits >= 64 && p == 0 && n == P) mix::add_shares<bf16, float>(part, d->V, d->C, ldn, gw, csum, gb, splits, k.st);
+        if (shares >= 64 && p == 0 && n == P) mix::add_shares<bf16, float>(part, d->V, d->C, ldn, gw, csum, gb, shares, k.st, rows);
         else add_piece_kernel<bf16><<<(unsigned)((sums_all + THREADS - 1) / THREADS), THREADS, 0, k.st>>>(
-            part, csum, splits, d->V, d->C, ldn, acc, p == 0, p + n == P, gw, gb), MC_COUNT(1);
+            part, csum, shares, d->V, rows, d->C, ldn, acc, p == 0, p + n == P, gw, gb), MC_COUNT(1);
         k.did(cudaGetLastError() == cudaSuccess ? MC_OK : MC_ERR_LAUNCH);
       }
     });
@@ -776,7 +802,7 @@ struct FloatCores {
       k.did(split(Splits{{pixels(x, p, n, soft.top + p, x3), p ? Split{} : weights(w, w3), p || !gx ? Split{} : transposed(w, wt3)}}, k.st));
       if (k.rc) return;
       mix::Scores sc{target + p, d->ignore_index, nullptr, nullptr, {soft.top + p, soft.rest + p, soft.miss + p}, grad,
-                     d->reduction == MC_REDUCE_MEAN ? (const double*)kept : nullptr, bias};
+                     d->reduction == MC_REDUCE_MEAN ? (const double*)kept : nullptr, 0, bias};
       const mix::TcRows xp = parts_of(x3, n, d->C, Cp), gp{gz.p, n, d->V, 64, 0, true, 3};
       k.did(mix::tc_scores_grad(xp, parts_of(w3, d->V, d->C, Cp), nullptr, sc, gp, k.st));
       if (gx && !k.rc) {
@@ -790,7 +816,7 @@ struct FloatCores {
         // (many shares of few sums: several threads for each)
         if (splits >= 64 && p == 0 && n == P) mix::add_shares<float, float>(part, d->V, d->C, ldn, gw, csum, gb, splits, k.st);
         else add_piece_kernel<float><<<(unsigned)((threads + THREADS - 1) / THREADS), THREADS, 0, k.st>>>(
-            part, csum, splits, d->V, d->C, ldn, acc, p == 0, p + n == P, gw, gb), MC_COUNT(1);
+            part, csum, splits, d->V, d->V, d->C, ldn, acc, p == 0, p + n == P, gw, gb), MC_COUNT(1);
         k.did(cudaGetLastError() == cudaSuccess ? MC_OK : MC_ERR_LAUNCH);
       }
     });

@@ -230,6 +230,8 @@ struct Scores {
   Softmax<const float> kept;
   const float* grad;
   const double* count;
+  // of bf16 layers: gz in two parts, the second one this many pieces of 8 columns behind the first (at most 4, 64 columns in all); 0: one
+  int second;
   const float* bias32;  // of float32 layers
   bf16* gz;             // of float32 layers: where the three parts of gz go
 };

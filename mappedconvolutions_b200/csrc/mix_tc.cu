@@ -441,6 +441,8 @@ __device__ __forceinline__ void read_scores(const GemmArgs& g, int set, uint32_t
   const uint32_t at0 = out0 + (set << C::SLOT_BITS) * C::CH_BYTES + row * C::CW * 2, swizzle = (row & 7) << 4;
   const auto bar_of = [&](uint32_t base, uint32_t i) { return bfull + base + 32 * set + 8 * (i & mask); };
   const uint32_t tempty0 = of_leader(bfull + BAR_TEMPTY);
+  // (few classes take narrow tiles; a test for them in the widest took 388 us instead of 315 for 40 968 pixels x 10 242 classes)
+  const int second = BN == 64 ? g.sc.second : 0;
   float scale = 0.f;
   if (MODE == SCORE_GRAD) scale = g.sc.count ? (float)((double)*g.sc.grad / *g.sc.count) : *g.sc.grad;
   uint32_t it = 0, i = 0;
@@ -484,7 +486,7 @@ __device__ __forceinline__ void read_scores(const GemmArgs& g, int set, uint32_t
     fetch_pixel(ahead);
     const bool dead = kept == INFINITY;
     int live = (g.N - n0 + PW - 1) / PW;  // pieces with classes; a staged tile is filled up with zeros
-    if (MODE == SCORE_GRAD) live = (live + PER - 1) / PER * PER;
+    if (MODE == SCORE_GRAD) live = second ? 1 : (live + PER - 1) / PER * PER;
     if (live > NP) live = NP;
     uint32_t v[2][PW];
     const uint32_t tile = 2 * it + set, acc = tile % C::NACC;
@@ -539,7 +541,17 @@ __device__ __forceinline__ void read_scores(const GemmArgs& g, int set, uint32_t
             MC_HALF r[j] = pack_bf16x2(z[j].x, z[j].y);
 #pragma unroll
             for (int h = 0; h < PW / 8; ++h)
-              sts16(at + (((j0 + h) << 4) ^ swizzle), make_uint4(r[4 * h], r[4 * h + 1], r[4 * h + 2], r[4 * h + 3]));
+              if (!second || h < second) sts16(at + (((j0 + h) << 4) ^ swizzle), make_uint4(r[4 * h], r[4 * h + 1], r[4 * h + 2], r[4 * h + 3]));
+            if (second) {  // (the first 32 columns are all there are)
+              MC_HALF {
+                z[j] = add2(z[j], make_float2(-__uint_as_float(r[j] << 16), -__uint_as_float(r[j] & 0xFFFF0000u)));
+                r[j] = pack_bf16x2(z[j].x, z[j].y);
+              }
+#pragma unroll
+              for (int h = 0; h < PW / 8; ++h)
+                if (h < second)
+                  sts16(at + (((second + h) << 4) ^ swizzle), make_uint4(r[4 * h], r[4 * h + 1], r[4 * h + 2], r[4 * h + 3]));
+            }
           } else if (tile0 < g.rows) {
             // 64 bytes of this pixel's row in the block of each part
             bf16* to = g.sc.gz + (((long long)(tile0 / TILE) * g.y_across + (n0 + PW * pc) / KB) * TILE + row) * KB + PW * pc % KB;
@@ -1286,10 +1298,10 @@ int tc_scores_sum(const TcRows& x, const TcRows& w, const bf16* bias, const Scor
   return launch_wide<SCORE_SUM>(g, bn, st);
 }
 int tc_scores_grad(const TcRows& x, const TcRows& w, const bf16* bias, const Scores& s, const TcRows& gz, cudaStream_t st) {
-  GemmArgs g = score_args(x, gz.cols, bias, s);
+  GemmArgs g = score_args(x, (int)w.rows, bias, s);
   g.y_across = gz.blocks ? gz.across() : 0;
   if (gz.parts > 1) g.sc.gz = (bf16*)const_cast<void*>(gz.p);
-  const int bn = tile_width(g.m_pairs, g.N, g.kb[0], sm_total());
+  const int bn = s.second ? 64 : tile_width(g.m_pairs, g.N, g.kb[0], sm_total());
   if (!encode(&g.a[0], x, TILE) || !encode(&g.b[0], w, bn / 2) || (!g.sc.gz && !encode(&g.y[0], gz, TILE))) return MC_ERR_LAUNCH;
   return launch_wide<SCORE_GRAD>(g, bn, st);
 }

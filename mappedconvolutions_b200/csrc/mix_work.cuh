@@ -20,10 +20,10 @@ static size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
 
 static long long pixels(const mc_mix_desc* d) { return d->B * d->S; }
 
-// gw (M, N) and gb (M), either of which may be null: the shares' sums, rounded once.  Rows of part have ldn elements.
+// gw (M, N) and gb (M), either of which may be null: the shares' sums, rounded once.  Shares have R rows (M or more) of ldn elements.
 // A block takes 32 sums; G threads for each add every G-th share, and their results are added in order.
 template <typename T, typename CT, int G>
-__global__ void __launch_bounds__(32 * G) add_shares_kernel(const CT* __restrict__ part, int M, int N, int ldn,
+__global__ void __launch_bounds__(32 * G) add_shares_kernel(const CT* __restrict__ part, int M, int R, int N, int ldn,
                                                             T* __restrict__ gw, const CT* __restrict__ csum,
                                                             T* __restrict__ gb, int splits) {
   __shared__ CT sums[G][32];
@@ -33,7 +33,7 @@ __global__ void __launch_bounds__(32 * G) add_shares_kernel(const CT* __restrict
   CT s = CT(0);
   if (in) {
     const CT* src = w ? part + i / N * ldn + i % N : csum + (i - nw);
-    const long long step = w ? (long long)M * ldn : M;
+    const long long step = w ? (long long)R * ldn : R;
 #pragma unroll 8
     for (int j = j0; j < splits; j += G) s += src[j * step];
   }
@@ -47,10 +47,11 @@ __global__ void __launch_bounds__(32 * G) add_shares_kernel(const CT* __restrict
 // Many shares of few sums: 32 threads for each (296 shares of 99 x 50 sums: 6 us instead of 10), as long as the blocks run
 // at one time (74 shares of 256 x 128 sums: 10 us instead of 6).
 template <typename T, typename CT>
-static void add_shares(const CT* part, int M, int N, int ldn, T* gw, const CT* csum, T* gb, int splits, cudaStream_t st) {
+static void add_shares(const CT* part, int M, int N, int ldn, T* gw, const CT* csum, T* gb, int splits, cudaStream_t st, int R = 0) {
+  if (!R) R = M;
   const unsigned blocks = (unsigned)(((long long)M * N + M + 31) / 32);
-  if (splits >= 64 && blocks <= 2 * 148) add_shares_kernel<T, CT, 32><<<blocks, 1024, 0, st>>>(part, M, N, ldn, gw, csum, gb, splits);
-  else add_shares_kernel<T, CT, 8><<<blocks, 256, 0, st>>>(part, M, N, ldn, gw, csum, gb, splits);
+  if (splits >= 64 && blocks <= 2 * 148) add_shares_kernel<T, CT, 32><<<blocks, 1024, 0, st>>>(part, M, R, N, ldn, gw, csum, gb, splits);
+  else add_shares_kernel<T, CT, 8><<<blocks, 256, 0, st>>>(part, M, R, N, ldn, gw, csum, gb, splits);
   MC_COUNT(1);
 }
 

@@ -41,3 +41,33 @@ def test_sums_of_one_sign(ops, pixels, channels, classes):
     assert ((gw[:, :, 0].double() - gz.T @ rows).abs() <= e_gz.T @ rows + own * (gz.abs().T @ rows)).all()
     # (column sums: float32 sums of 64 of a share's pixels to a thread, then the threads' and the shares')
     assert ((gb.double() - gz.sum(0)).abs() <= e_gz.sum(0) + (own + 64 * 2.0 ** -24) * gz.abs().sum(0)).all()
+
+
+@pytest.mark.parametrize("layout", ["nhwc", "nchw"])
+@pytest.mark.parametrize("shape,channels,classes,mean", [((4, 60, 80), 64, 13, True), ((2, 1, 2562), 32, 32, False), ((1, 50, 41), 40, 9, True),
+                                                         ((3, 1, 777), 16, 2, True), ((1, 1, 5000), 300, 24, False), ((1, 7, 9), 5, 1, True),
+                                                         ((2, 1, 129), 8, 31, True), ((70, 30, 31), 17, 8, False)])
+def test_few_classes_are_rounded_once(ops, shape, channels, classes, mean, layout):
+    """bf16, up to 32 classes: gradients of scores are kept in two parts, 16 bits.  What the results are off beside their own rounding is the
+    scores' and the exponentials' errors (2^-19 of a probability, step_reference): less than a hundredth of it."""
+    bf16 = torch.bfloat16
+    g = torch.Generator("cuda").manual_seed(classes)
+    x = torch.randn(shape[0], channels, *shape[1:], generator=g, device="cuda").to(bf16)
+    x = x.contiguous(memory_format=torch.channels_last) if layout == "nhwc" else x
+    weight = ((torch.rand(classes, channels, 1, generator=g, device="cuda") * 2 - 1) * 4 / channels ** 0.5).to(bf16)
+    bias = torch.randn(classes, generator=g, device="cuda").to(bf16)
+    target = torch.randint(0, classes, shape, generator=g, device="cuda")
+    target[torch.rand(shape, generator=g, device="cuda") < 0.2] = -100
+    loss, saved = ops.cross_entropy_forward(x, weight, bias, target, -100, mean)
+    got = ops.cross_entropy_backward(torch.ones_like(loss), saved, x, weight, bias, target, -100, mean)
+    valid = (target != -100).reshape(-1)
+    rows = x.double().permute(0, 2, 3, 1).reshape(-1, channels)
+    gz = (rows @ weight.double()[:, :, 0].T + bias.double()).softmax(1)
+    gz[torch.arange(len(gz), device="cuda"), target.reshape(-1).clamp(min=0)] -= 1
+    gz = gz * valid[:, None] / (valid.sum() if mean else 1)
+    want = (gz @ weight.double()[:, :, 0]).view(shape[0], *shape[1:], channels).permute(0, 3, 1, 2), (gz.T @ rows)[:, :, None], gz.sum(0)
+    for a, b in zip(got, want):
+        assert (a.double() - b).norm() <= 1.05 * (b.to(bf16).double() - b).norm()
+    for need in ((False, True), (True, False)):
+        part = ops.cross_entropy_backward(torch.ones_like(loss), saved, x, weight, bias, target, -100, mean, *need)
+        assert all(a is None or torch.equal(a, b) for a, b in zip(part, got))
