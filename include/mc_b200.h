@@ -506,10 +506,10 @@ int mc_group_norm_bwd(const mc_norm_desc* d, const void* gy, const void* x, cons
  * MC_PHASE_FORWARD and MC_PHASE_BACKWARD; both 16-byte aligned.  Any of the gradients may be NULL.  Scores, softmax sums and gradients of
  * parameters are summed in float32 (MC_F64: double), the loss in double, all in a fixed order.  For MC_BF16 products are the
  * tensor cores' (sums lose up to 2^-23 per sixteen terms) and gradients of scores are rounded to bf16 before all three gradients
- * are made of them.  MC_F32 with many products takes the tensor cores in three bf16 parts of every value: products keep 24 bits, but
- * a sum of terms of one sign can lose up to 2^-17 of itself over 1024 channels (scores), 2^-15 over 4096 classes (gx) and 2^-17 (gw,
- * gb), where float32 operations one after the other would be off by the square root of as many half steps; sums are no longer than
- * that there.
+ * are made of them (up to 32 classes: to two bf16 parts, 16 bits).  MC_F32 with many products takes the tensor cores in three bf16
+ * parts of every value: products keep 24 bits, but a sum of terms of one sign can lose up to 2^-17 of itself over 1024 channels
+ * (scores), 2^-15 over 4096 classes (gx) and 2^-17 (gw, gb), where float32 operations one after the other would be off by the square
+ * root of as many half steps; sums are no longer than that there.
  * Limits: B * S <= 2^31 - 256, C and V <= 2^20, C * V <= 2^31. */
 enum { MC_REDUCE_SUM = 0, MC_REDUCE_MEAN = 1 };
 typedef struct mc_ce_desc {
